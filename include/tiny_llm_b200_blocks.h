@@ -354,6 +354,22 @@ int tlb_moe_combine_tanh(float *x, const float *pair_out, const float *gate, con
 /* Row-wise arg-max of fp32 logits [rows, vocab] (lowest index wins a tie). */
 int tlb_argmax_rows(const float *logits, int32_t *out, int rows, int vocab, void *stream);
 
+/* Products over matrices of 8-bit numbers (e4m3) with one fp32 scale for each block of 128 x 128: w [n, ldw] bytes (ldw a multiple of 16, the
+ * base 16-byte aligned, zero behind column k), sw [ceil(n / 128), ceil(k / 128)].  The rows x [rows, k] (`dtype`, ldx apart) are rounded to e4m3 with
+ * one scale for each run of 128 of a row:  m = max(|x| of the run, 2^-100), q = e4m3(x * (448 / m)), scale = m / 448, every operation rounded
+ * to fp32 once; a run with an infinity or a NaN has the scale NaN.  out[t, :] = sum over runs of scale * block scale * (q . w) in fp32, plus bias
+ * (`dtype` [n], or NULL), rounded to `dtype`.  A row's result does not depend on the other rows, nor do its bits as long as the number of rows is in the same
+ * range of the kernel's tiles.  The workspace need not be initialised; calls that may run at once need one each. */
+size_t tlb_fp8_linear_workspace(int rows, int k);
+int tlb_fp8_linear(const void *x, long long ldx, const void *w, int ldw, const float *sw, const void *bias, void *out, int rows, int n, int k, void *workspace,
+                   size_t workspace_bytes, int dtype, void *stream);
+/* out [rows, dim] = down(act(gate x) * (up x)): w_gate_up holds runs of 128 rows of the gate and of the up projection in turn, 2 * 128 * ceil(ff / 128)
+ * rows in all, zero where a run passes ff, with scales [2 * ceil(ff / 128), ceil(dim / 128)]; w_down [dim, ld_down].  The gated rows stay fp32 until
+ * they are rounded to e4m3 as x is.  act: 0 silu, 1 gelu (tanh), 3 clamped swish with limit and slope (tlb_gated_act). */
+size_t tlb_fp8_gated_mlp_workspace(int rows, int dim, int ff);
+int tlb_fp8_gated_mlp(const void *x, long long ldx, const void *w_gate_up, int ld_gate_up, const float *s_gate_up, const void *w_down, int ld_down, const float *s_down,
+                      void *out, int rows, int dim, int ff, int act, float limit, float slope, void *workspace, size_t workspace_bytes, int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,80 @@
+"""Products over 8-bit weights against float64: sizes at the edges of blocks, tiles and reductions, strides, empty inputs, numbers that are none,
+streams and captured graphs; the gated feed-forward; the refusals of both.
+
+Tolerance of a product: the products of two e4m3 numbers are exact, a block's 128 of them are added in the tensor cores (an addition is off by at most
+2^-23 of what is added, if it cuts), the blocks in fp32 with two roundings each, and the result is rounded to its type once."""
+
+import pytest
+import torch
+
+from tiny_llm_b200.fp8 import BLOCK, Fp8Weights, fp8_linear
+from tiny_llm_b200.mlp import Fp8GatedMLP
+
+DEV = "cuda"
+gpu = pytest.mark.gpu
+
+
+def nearest_e4m3(v):
+    _, e = torch.frexp(v)
+    step = torch.exp2(torch.clamp(e.double() - 4, min=-9.0))
+    return torch.clamp(torch.round(v / step) * step, -448.0, 448.0)
+
+
+def rounded_rows(x):
+    """float64: what the rows stand for once they are e4m3 numbers (scales and products rounded to fp32 as the operator says)."""
+    x = x.detach().cpu().float().double()
+    out = torch.empty_like(x)
+    for k in range(0, x.shape[1], BLOCK):
+        part = x[:, k : k + BLOCK]
+        most = part.abs().amax(dim=1, keepdim=True)
+        most = torch.where(most < 2.0**-100, torch.full_like(most, 2.0**-100), most)
+        top = torch.full_like(most, 448.0)
+        q = nearest_e4m3((part * (top / most).float().double()).float().double()) * (most / top).float().double()
+        out[:, k : k + BLOCK] = torch.where(torch.isfinite(most), q, torch.full_like(q, torch.nan))
+    return out
+
+
+def make(rows, n, k, dtype, seed=0, bias=False):
+    gen = torch.Generator().manual_seed(seed + rows * 7 + n * 3 + k)
+    x = (torch.randn(rows, k, generator=gen) * torch.exp(torch.randn(k, generator=gen))).to(dtype)
+    w = Fp8Weights.from_tensor(torch.randn(n, k, generator=gen) * torch.exp(torch.randn(n, 1, generator=gen)) * k**-0.5)
+    return x.to(DEV), Fp8Weights(w.values[:, :k].to(DEV), w.scales.to(DEV)), torch.randn(n, generator=gen).to(dtype).to(DEV) if bias else None
+
+
+def product_tolerance(rows64, w64, want, dtype):
+    """Per entry: see the head of the file; ``rows64`` and ``w64`` are what is multiplied."""
+    most = rows64.abs() @ w64.abs().t()
+    blocks = -(-rows64.shape[1] // BLOCK)
+    return (2 * BLOCK + 3 * blocks + 4) * 2.0**-24 * most + torch.finfo(dtype).eps / 2 * want.abs() * 1.001 + 1e-38
+
+
+def check_linear(x, w, bias, got):
+    xq, w64 = rounded_rows(x), w.dequantize(torch.float64).cpu()
+    # dequantize() rounds value * scale to fp32: multiply in 64 bits instead
+    n, k = w.shape
+    w64 = w.values[:, :k].float().double().cpu() * w.scales.double().cpu().repeat_interleave(BLOCK, 0)[:n].repeat_interleave(BLOCK, 1)[:, :k]
+    want = xq @ w64.t()
+    if bias is not None:
+        want = want + bias.double().cpu()
+    tol = product_tolerance(xq, w64, want, x.dtype)
+    if bias is not None:
+        tol = tol + 2.0**-23 * (want.abs() + bias.double().cpu().abs())
+    assert got.dtype == x.dtype and got.shape == want.shape
+    off = (got.double().cpu() - want).abs()
+    assert bool((off <= tol).all()), f"worst {(off / tol).max().item():.2f} times the tolerance"
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 2, 8, 9, 16, 17, 33, 64, 65, 128, 129, 257, 300])
+@pytest.mark.parametrize("n,k", [(1, 1), (128, 128), (129, 127), (200, 300), (640, 1000), (333, 2048)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_linear(rows, n, k, dtype):
+    x, w, bias = make(rows, n, k, dtype, bias=n % 2 == 1)
+    check_linear(x, w, bias, fp8_linear(x, w, bias))
+
+
+@gpu
+@pytest.mark.parametrize("rows,n,k", [(1, 2560, 9728), (24, 2560, 4096), (48, 5000, 3000), (100, 2048, 6144), (700, 1200, 2600), (2100, 900, 1111)])
+def test_linear_of_real_sizes(rows, n, k):
+    x, w, bias = make(rows, n, k, torch.bfloat16)
+    check_linear(x, w, bias, fp8_linear(x, w, bias))

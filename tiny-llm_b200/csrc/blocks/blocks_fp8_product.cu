@@ -1,0 +1,285 @@
+// Rows of e4m3 numbers times a matrix of them on the 5th-generation tensor cores: tcgen05.mma (kind::f8f6f4) fed by TMA.
+//
+//   out[t, n] = sum over blocks b of 128 of  sx[b, t] * sw[n / 128, b] * (sum over k in b of q[t, k] w[n, k])
+//
+// The inner sum is exact products added in the tensor cores, over one block at a time: four instructions of 32, into an accumulator that
+// starts from zero.  The outer sum is kept in registers, in fp32: the epilogue's warps take every block's accumulator out of tensor memory
+// and add it times the two scales.  128 rows of the matrix are a tile's M side (a lane each, and one scale for all of them), BN tokens its
+// N side, so the second scale is a column's: a warp has its columns' products of scales in shared memory, a broadcast read for four.
+//
+// 12 warps: 0 TMA of both operands (boxes of 128 bytes, 128-byte swizzle: one block of the reduction a stage), 1 the products, 4-11 the sums.
+//
+// Few tokens make few tiles: then the CTAs of a cluster share a tile's blocks and add their sums through each other's shared memory, every
+// sum in rank order, so no memory and no atomics stand between two launches, and the result does not depend on their timing.
+#include <algorithm>
+
+#include "blocks_fp8.cuh"
+#include "blocks_tc.cuh"
+
+namespace tlb {
+
+constexpr int kF8Threads = 12 * 32;
+constexpr int kF8SumWarps = 8;
+constexpr int kF8WeightBytes = 128 * 128;
+
+template <int BN>
+struct F8Tile {
+    static constexpr int kStage = kF8WeightBytes + BN * 128;
+    static constexpr int kPerSm = BN <= 64 ? 2 : 1;
+    static constexpr int kBuffers = BN >= 128 ? 2 : 4;  // accumulators
+    static constexpr int kTmem = BN * kBuffers;         // columns: 64, 128, 256, 256, 512
+    static constexpr int kFactors = kF8SumWarps * (BN / 2) * 4;
+    static constexpr int kStages = std::min(8, (227 * 1024 / kPerSm - 1024 - kFactors - 512) / kStage);
+    static constexpr int kSmem = kStages * kStage + kFactors + 256;
+};
+
+struct F8Args {
+    const float *sx, *sw;
+    const void *bias;
+    void *out;
+    int ld_sx, rows, n, k_blocks, m_blocks, tiles, splits;
+};
+
+// C consecutive columns (8 or 16) of the warp's lanes, without the wait.
+__device__ __forceinline__ void f8_ld(uint32_t at, uint32_t (&v)[8]) { tc_ld8(at, v); }
+__device__ __forceinline__ void f8_ld(uint32_t at, uint32_t (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+                   "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(at)
+                 : "memory");
+}
+__device__ __forceinline__ void f8_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+                 "r"(accumulate)
+                 : "memory");
+}
+// e4m3 x e4m3 -> f32, 128 rows, n columns, both K-major
+__host__ __device__ constexpr uint32_t f8_idesc(int n) { return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24); }
+
+template <typename T, int BN>
+__global__ void __launch_bounds__(kF8Threads, F8Tile<BN>::kPerSm)
+fp8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_q, const F8Args a) {
+    using Tile = F8Tile<BN>;
+    constexpr int COLS = BN / 2, STEP = COLS < 16 ? 8 : 16;  // columns of a warp, of one read of tensor memory
+    extern __shared__ __align__(1024) unsigned char f8_smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t base = g_smem_u32(f8_smem);
+    float *factors = reinterpret_cast<float *>(f8_smem + Tile::kStages * Tile::kStage);
+    const uint32_t bars = base + Tile::kStages * Tile::kStage + Tile::kFactors;
+    const uint32_t full = bars, empty = full + 64, acc_full = empty + 64, acc_empty = acc_full + 32;
+    volatile int *dead = reinterpret_cast<volatile int *>(f8_smem + Tile::kStages * Tile::kStage + Tile::kFactors + 192);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(const_cast<int *>(dead)) + 1;
+
+    if (warp == 0 && lane == 0) {
+        for (int i = 0; i < Tile::kStages; ++i) g_mbar_init(full + 8 * i, 1), g_mbar_init(empty + 8 * i, 1);
+        for (int i = 0; i < Tile::kBuffers; ++i) g_mbar_init(acc_full + 8 * i, 1), g_mbar_init(acc_empty + 8 * i, kF8SumWarps);
+        *dead = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(g_smem_u32(tmem_slot)), "n"(Tile::kTmem) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    g_tc_fence_before();
+    __syncthreads();
+    g_tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    const int rank = blockIdx.x % a.splits, first = blockIdx.x / a.splits, step = gridDim.x / a.splits;
+    const int kb0 = (int)((long long)a.k_blocks * rank / a.splits), kb1 = (int)((long long)a.k_blocks * (rank + 1) / a.splits);
+
+    if (warp == 0) {
+        int s = 0;
+        uint32_t ph = 1;
+        auto load_w = [&](int stage, int tile, int kb) {
+            if (g_elect_one()) {
+                g_mbar_expect_tx(full + 8 * stage, Tile::kStage);
+                g_tma_load_2d(base + stage * Tile::kStage, &map_w, kb * 128, tile % a.m_blocks * 128, full + 8 * stage);
+            }
+            __syncwarp();
+        };
+        auto load_q = [&](int stage, int tile, int kb) {
+            if (g_elect_one()) g_tma_load_2d(base + stage * Tile::kStage + kF8WeightBytes, &map_q, kb * 128, tile / a.m_blocks * BN, full + 8 * stage);
+            __syncwarp();
+        };
+        // the first stages' weights are asked for while the rows' launch is still running: they are older than it
+        const int ahead = min(Tile::kStages, kb1 - kb0);
+        if (first < a.tiles)
+            for (int i = 0; i < ahead; ++i) load_w(i, first, kb0 + i);
+        tl::griddep_wait();
+        int early = ahead;
+        for (int tile = first; tile < a.tiles; tile += step)
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (early > 0) {
+                    --early;
+                } else {
+                    if (!tc_wait(empty + 8 * s, ph, dead)) goto out;
+                    load_w(s, tile, kb);
+                }
+                load_q(s, tile, kb);
+                if (++s == Tile::kStages) s = 0, ph ^= 1u;
+            }
+    } else if (warp == 1) {
+        int s = 0, buf = 0;
+        uint32_t ph = 0, acc_ph = 1;
+        for (int tile = first; tile < a.tiles; tile += step)
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!tc_wait(acc_empty + 8 * buf, acc_ph, dead)) goto out;
+                if (!tc_wait(full + 8 * s, ph, dead)) goto out;
+                g_tc_fence_after();
+                if (g_elect_one()) {
+                    const uint64_t w = g_smem_desc_sw128(base + s * Tile::kStage, 0, 1024), q = g_smem_desc_sw128(base + s * Tile::kStage + kF8WeightBytes, 0, 1024);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) f8_mma(tmem + buf * BN, w + 2 * k, q + 2 * k, f8_idesc(BN), k > 0);
+                    g_tc_commit(empty + 8 * s);
+                    g_tc_commit(acc_full + 8 * buf);
+                }
+                __syncwarp();
+                if (++s == Tile::kStages) s = 0, ph ^= 1u;
+                if (++buf == Tile::kBuffers) buf = 0, acc_ph ^= 1u;
+            }
+    } else if (warp >= 4) {
+        const int quarter = warp & 3, half = (warp - 4) >> 2;
+        float *mine = factors + (warp - 4) * COLS;
+        int buf = 0;
+        uint32_t acc_ph = 0;
+        tl::griddep_wait();
+        for (int tile = first; tile < a.tiles; tile += step) {
+            const int m = tile % a.m_blocks, col0 = tile / a.m_blocks * BN + half * COLS, f = m * 128 + quarter * 32 + lane;
+            constexpr int PER = (COLS + 31) / 32;
+            float acc[COLS], next[PER], next_w = 0.f;
+#pragma unroll
+            for (int i = 0; i < COLS; ++i) acc[i] = 0.f;
+            auto fetch = [&](int kb) {
+                next_w = a.sw[(size_t)m * a.k_blocks + kb];
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    const int c = lane + 32 * i;
+                    next[i] = c < COLS && col0 + c < a.rows ? tl::ld_cg(a.sx + (size_t)kb * a.ld_sx + col0 + c) : 0.f;
+                }
+            };
+            if (kb0 < kb1) fetch(kb0);
+            bool ok = true;
+            for (int kb = kb0; kb < kb1; ++kb) {
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+                    if (lane + 32 * i < COLS) mine[lane + 32 * i] = next[i] * next_w;
+                if (kb + 1 < kb1) fetch(kb + 1);
+                __syncwarp();
+                ok &= tc_wait(acc_full + 8 * buf, acc_ph, dead);
+                g_tc_fence_after();
+                const uint32_t at = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN + half * COLS;
+#pragma unroll
+                for (int c = 0; c < COLS; c += STEP) {
+                    uint32_t v[STEP];
+                    f8_ld(at + c, v);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                    for (int i = 0; i < STEP; i += 4) {
+                        const float4 s4 = *reinterpret_cast<const float4 *>(mine + c + i);
+                        acc[c + i] = fmaf(__uint_as_float(v[i]), s4.x, acc[c + i]);
+                        acc[c + i + 1] = fmaf(__uint_as_float(v[i + 1]), s4.y, acc[c + i + 1]);
+                        acc[c + i + 2] = fmaf(__uint_as_float(v[i + 2]), s4.z, acc[c + i + 2]);
+                        acc[c + i + 3] = fmaf(__uint_as_float(v[i + 3]), s4.w, acc[c + i + 3]);
+                    }
+                }
+                g_tc_fence_before();
+                __syncwarp();
+                if (lane == 0) g_mbar_arrive(acc_empty + 8 * buf);
+                if (++buf == Tile::kBuffers) buf = 0, acc_ph ^= 1u;
+            }
+            const float bad = tc_verdict(ok, dead);
+            if (a.splits == 1) {
+                const float b = a.bias && f < a.n ? to_f(static_cast<const T *>(a.bias)[f]) : 0.f;
+                T *out = static_cast<T *>(a.out) + (size_t)col0 * a.n + f;
+#pragma unroll
+                for (int c = 0; c < COLS; ++c)
+                    if (f < a.n && col0 + c < a.rows) out[(size_t)c * a.n] = from_f<T>((acc[c] + b) * bad);
+            } else {  // the stages are done with: the last accumulator came behind all products
+                float *part = reinterpret_cast<float *>(f8_smem) + half * COLS * 128 + quarter * 32 + lane;
+#pragma unroll
+                for (int c = 0; c < COLS; ++c) part[c * 128] = acc[c] * bad;
+            }
+        }
+    }
+out:  // also from a role whose wait gave up
+    if (a.splits > 1) {  // one tile a cluster; a CTA adds its share of the tokens
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        const int share = BN / a.splits, m = first % a.m_blocks, col0 = first / a.m_blocks * BN + rank * share;
+        for (int i = threadIdx.x; i < share * 32; i += kF8Threads) {
+            const int c = i >> 5, f = m * 128 + (i & 31) * 4, at = ((rank * share + c) * 128 + (i & 31) * 4) * 4;
+            if (col0 + c >= a.rows) break;
+            float sum[4] = {};
+            for (int p = 0; p < a.splits; ++p) {
+                float v[4];
+                asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [ra];\n\t}"
+                             : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+                             : "r"(base + at), "r"(p)
+                             : "memory");
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[j] += v[j];
+            }
+            const float bad = tc_verdict(true, dead);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (f + j < a.n) static_cast<T *>(a.out)[(size_t)(col0 + c) * a.n + f + j] = from_f<T>((sum[j] + (a.bias ? to_f(static_cast<const T *>(a.bias)[f + j]) : 0.f)) * bad);
+        }
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    g_tc_fence_before();
+    __syncthreads();
+    if (warp == 2) {
+        tc_settle(dead);
+        g_tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(Tile::kTmem) : "memory");
+    }
+}
+
+template <typename T, int BN>
+static int f8_launch(const F8Product &p, cudaStream_t st) {
+    using Tile = F8Tile<BN>;
+    static_assert(Tile::kStages >= 3 && Tile::kStages <= 8 && Tile::kStages * Tile::kStage >= BN * 128 * 4, "the sums of a split tile lie over the stages");
+    CUtensorMap mw, mq;
+    if (int e = tc_map_bytes(&mw, p.w, p.ldw, p.n, p.ldw, 128)) return e;
+    if (int e = tc_map_bytes(&mq, p.q, p.ldq, p.rows, p.ldq, BN)) return e;
+    F8Args a{p.sx, p.sw, p.bias, p.out, p.ld_sx, p.rows, p.n, ceil_div(p.k, kF8Block), ceil_div(p.n, 128), 0, 1};
+    const long long tiles = (long long)a.m_blocks * ceil_div(p.rows, BN);
+    if (tiles > 0x3fffffff) return tl::fail(TL_EINVAL, "fp8_product: too large");
+    a.tiles = (int)tiles;
+    const int room = sm_count() * Tile::kPerSm;
+    if (BN <= 128)
+        while (a.splits < 8 && tiles * a.splits * 2 <= room && a.k_blocks >= 4 * a.splits) a.splits *= 2;
+    if (cudaFuncSetAttribute(fp8_product_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmem) != cudaSuccess) {
+        cudaGetLastError();
+        return tl::fail(TL_ECUDA, "fp8_product: no shared memory");
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(a.splits > 1 ? tiles * a.splits : std::min<long long>(tiles, room)));
+    cfg.blockDim = dim3(kF8Threads);
+    cfg.dynamicSmemBytes = Tile::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = a.splits, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = tl::use_pdl() ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, fp8_product_kernel<T, BN>, mw, mq, a);
+    TL_LAUNCH_CHECK("fp8_product");
+    return TL_OK;
+}
+
+int f8_product(const F8Product &p, cudaStream_t st) {
+    TLB_DISPATCH(p.dtype, "fp8_product", if (p.rows <= 16) return f8_launch<T, 16>(p, st); if (p.rows <= 32) return f8_launch<T, 32>(p, st);
+                 if (p.rows <= 64) return f8_launch<T, 64>(p, st); if (p.rows <= 128) return f8_launch<T, 128>(p, st); return f8_launch<T, 256>(p, st));
+    return TL_OK;
+}
+
+long long f8_gave_up() { return tl::read_gave_up(); }
+
+}  // namespace tlb

@@ -1,0 +1,143 @@
+// Rows of numbers rounded to e4m3, one scale for each run of 128, and the entry points of the products over 8-bit weights.
+//
+// A half warp takes a run: eight numbers a lane (one or two 16-byte loads), their largest by four exchanges, eight bytes out.  Bound by
+// HBM: a number is read once and a byte written.
+#include "blocks_fp8.cuh"
+
+namespace tlb {
+
+constexpr int kRowsThreads = 256;
+
+template <typename T, bool WIDE>
+__device__ __forceinline__ void rows_load(const T *p, int left, float (&v)[8]) {
+    if constexpr (WIDE && sizeof(T) == 2) {
+        const uint4 u = tl::ld_cg(reinterpret_cast<const uint4 *>(p));
+        const uint32_t c[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = tl::unpack2<T>(c[i]);
+            v[2 * i] = f.x, v[2 * i + 1] = f.y;
+        }
+    } else if constexpr (WIDE) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint4 u = tl::ld_cg(reinterpret_cast<const uint4 *>(p) + i);
+            v[4 * i] = __uint_as_float(u.x), v[4 * i + 1] = __uint_as_float(u.y), v[4 * i + 2] = __uint_as_float(u.z), v[4 * i + 3] = __uint_as_float(u.w);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < left ? to_f(tl::ld_cg(p + i)) : 0.f;
+    }
+}
+
+// WIDE: every group of eight is whole and aligned to 16 bytes.
+template <typename T, bool GATED, bool WIDE>
+__global__ void __launch_bounds__(kRowsThreads)
+fp8_rows_kernel(const T *x, long long ldx, int rows, int cols, int act, float limit, float slope, uint8_t *q, int ldq, float *scales, int ld_scales) {
+    const int runs = (cols + kF8Block - 1) / kF8Block, lane = threadIdx.x & 15;
+    const long long at = ((long long)blockIdx.x * kRowsThreads + threadIdx.x) >> 4;
+    tl::griddep_wait();
+    tl::griddep_launch();  // behind the wait: what a dependent reads ahead of its own is older than this launch
+    const bool live = at < (long long)rows * runs;  // a half warp as one
+    const int row = live ? (int)(at / runs) : 0, run = live ? (int)(at % runs) : 0, k = run * kF8Block + lane * 8, left = live ? cols - k : 0;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    if (left > 0) {
+        if constexpr (GATED) {  // the columns of a whole run are there, those past the last feature are zero
+            const T *from = x + row * ldx + run * 2 * kF8Block + lane * 8;
+            float g[8], u[8];
+            rows_load<T, WIDE>(from, 8, g);
+            rows_load<T, WIDE>(from + kF8Block, 8, u);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = i < left ? gated_pair(g[i], u[i], act, limit, slope) : 0.f;
+        } else {
+            rows_load<T, WIDE>(x + row * ldx + k, left, v);
+        }
+    }
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = f8_most(most, fabsf(v[i]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) most = f8_most(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const F8Scale s = f8_scale(most);
+    if (!live) return;
+    if (lane == 0) scales[(size_t)run * ld_scales + row] = s.scale;
+    if (k >= ldq) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], s.times);
+    *reinterpret_cast<uint2 *>(q + (size_t)row * ldq + k) = make_uint2(f8_pack4(v[0], v[1], v[2], v[3]), f8_pack4(v[4], v[5], v[6], v[7]));
+}
+
+int f8_rows(const F8Rows &a, cudaStream_t st) {
+    const long long halves = (long long)a.rows * ceil_div(a.cols, kF8Block);
+    const long long grid = (halves * 16 + kRowsThreads - 1) / kRowsThreads;
+    if (grid > 0x7fffffffLL) return tl::fail(TL_EINVAL, "fp8_rows: too many rows");
+#define TLB_ROWS(T, G, W)                                                                                                                               \
+    tl::launch_chained(fp8_rows_kernel<T, G, W>, dim3((unsigned)grid), dim3(kRowsThreads), 0, st, (const T *)a.x, a.ldx, a.rows, a.cols, a.act, a.limit, a.slope, a.q, \
+                       a.ldq, a.scales, a.ld_scales)
+    if (a.gated) {
+        TLB_ROWS(float, true, true);
+    } else {
+        const size_t es = a.dtype == TL_BF16 ? 2 : 4;
+        const bool wide = a.cols % 8 == 0 && (a.ldx * es) % 16 == 0 && tl::aligned16(a.x);
+        TLB_DISPATCH(a.dtype, "fp8_rows", if (wide) TLB_ROWS(T, false, true); else TLB_ROWS(T, false, false));
+    }
+#undef TLB_ROWS
+    TL_LAUNCH_CHECK("fp8_rows");
+    return TL_OK;
+}
+
+// The rounded rows of one product in a caller's scratch: bytes, then scales.
+static size_t f8_rows_bytes(int rows, int cols) {
+    return (size_t)rows * f8_up(cols, 16) + (size_t)ceil_div(cols, kF8Block) * f8_up(rows, 4) * sizeof(float);
+}
+
+}  // namespace tlb
+
+using namespace tlb;
+
+extern "C" {
+
+size_t tlb_fp8_linear_workspace(int rows, int k) { return rows <= 0 || k <= 0 ? 0 : f8_rows_bytes(rows, k); }
+
+int tlb_fp8_linear(const void *x, long long ldx, const void *w, int ldw, const float *sw, const void *bias, void *out, int rows, int n, int k, void *workspace,
+                   size_t workspace_bytes, int dtype, void *stream) {
+    if (rows <= 0) return TL_OK;
+    if (!x || !w || !sw || !out || !workspace || n <= 0 || k <= 0 || ldx < k || ldw < k || ldw % 16 || !tl::aligned16(w) || !tl::aligned16(workspace))
+        return tl::fail(TL_EINVAL, "fp8_linear: bad argument");
+    if (dtype != TL_F32 && dtype != TL_BF16) return tl::fail(TL_EDTYPE, "fp8_linear: dtype must be float32 or bfloat16");
+    if (workspace_bytes < f8_rows_bytes(rows, k)) return tl::fail(TL_EINVAL, "fp8_linear: workspace too small");
+    const int ldq = f8_up(k, 16), ld_sx = f8_up(rows, 4);
+    uint8_t *q = (uint8_t *)workspace;
+    float *sx = (float *)(q + (size_t)rows * ldq);
+    if (int e = f8_rows({x, ldx, rows, k, dtype, false, 0, 0.f, 1.f, q, ldq, sx, ld_sx}, as_stream(stream))) return e;
+    return f8_product({q, sx, ldq, ld_sx, rows, (const uint8_t *)w, sw, ldw, n, k, bias, out, dtype}, as_stream(stream));
+}
+
+size_t tlb_fp8_gated_mlp_workspace(int rows, int dim, int ff) {
+    if (rows <= 0 || dim <= 0 || ff <= 0) return 0;
+    return ((f8_rows_bytes(rows, dim) + 15) & ~(size_t)15) + ((f8_rows_bytes(rows, ff) + 15) & ~(size_t)15) + (size_t)rows * 2 * f8_up(ff, kF8Block) * sizeof(float);
+}
+
+int tlb_fp8_gated_mlp(const void *x, long long ldx, const void *w_gate_up, int ld_gate_up, const float *s_gate_up, const void *w_down, int ld_down, const float *s_down,
+                      void *out, int rows, int dim, int ff, int act, float limit, float slope, void *workspace, size_t workspace_bytes, int dtype, void *stream) {
+    if (rows <= 0) return TL_OK;
+    if (!x || !w_gate_up || !s_gate_up || !w_down || !s_down || !out || !workspace || dim <= 0 || ff <= 0 || ldx < dim || ld_gate_up < dim || ld_gate_up % 16 ||
+        ld_down < ff || ld_down % 16 || !tl::aligned16(w_gate_up) || !tl::aligned16(w_down) || !tl::aligned16(workspace) || (act != 0 && act != 1 && act != 3) ||
+        (act == 3 && !(limit > 0.f)))
+        return tl::fail(TL_EINVAL, "fp8_gated_mlp: bad argument");
+    if (dtype != TL_F32 && dtype != TL_BF16) return tl::fail(TL_EDTYPE, "fp8_gated_mlp: dtype must be float32 or bfloat16");
+    if (workspace_bytes < tlb_fp8_gated_mlp_workspace(rows, dim, ff)) return tl::fail(TL_EINVAL, "fp8_gated_mlp: workspace too small");
+    const cudaStream_t st = as_stream(stream);
+    const int ld_sx = f8_up(rows, 4), wide = 2 * f8_up(ff, kF8Block);
+    uint8_t *q = (uint8_t *)workspace, *q2 = q + ((f8_rows_bytes(rows, dim) + 15) & ~(size_t)15);
+    float *sx = (float *)(q + (size_t)rows * f8_up(dim, 16)), *sx2 = (float *)(q2 + (size_t)rows * f8_up(ff, 16));
+    float *inner = (float *)(q2 + ((f8_rows_bytes(rows, ff) + 15) & ~(size_t)15));
+    if (int e = f8_rows({x, ldx, rows, dim, dtype, false, 0, 0.f, 1.f, q, f8_up(dim, 16), sx, ld_sx}, st)) return e;
+    if (int e = f8_product({q, sx, f8_up(dim, 16), ld_sx, rows, (const uint8_t *)w_gate_up, s_gate_up, ld_gate_up, wide, dim, nullptr, inner, TL_F32}, st)) return e;
+    if (int e = f8_rows({inner, wide, rows, ff, TL_F32, true, act, limit, slope, q2, f8_up(ff, 16), sx2, ld_sx}, st)) return e;
+    return f8_product({q2, sx2, f8_up(ff, 16), ld_sx, rows, (const uint8_t *)w_down, s_down, ld_down, dim, ff, nullptr, out, dtype}, st);
+}
+
+}  // extern "C"

@@ -458,7 +458,7 @@ using namespace tlb;
 
 extern "C" {
 
-int tlb_abi_version(void) { return 10; }
+int tlb_abi_version(void) { return 11; }
 int tlb_set_pdl(int enabled) {
     tl::g_use_pdl.store(enabled != 0, std::memory_order_relaxed);
     return TL_OK;

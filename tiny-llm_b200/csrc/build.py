@@ -58,6 +58,8 @@ BLOCKS_SOURCES = [
     "blocks/blocks_streams.cu",
     "blocks/blocks_tanh_norm.cu",
     "blocks/blocks_matrix_memory.cu",
+    "blocks/blocks_fp8_rows.cu",
+    "blocks/blocks_fp8_product.cu",
 ]
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")

@@ -7,6 +7,7 @@ The library is built on first use when it is missing (a handful of translation u
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import importlib.util
 import os
@@ -92,10 +93,14 @@ _SIGNATURES = {
     "tlb_tc_gave_up": (_LL, []),
     "tlb_moe_combine": (_I, [_VP, _VP, _VP, _VP, _VP, _I, _VP, _VP, _I, _I, _I, _I, _VP]),
     "tlb_argmax_rows": (_I, [_VP, _VP, _I, _I, _VP]),
+    "tlb_fp8_linear_workspace": (ctypes.c_size_t, [_I, _I]),
+    "tlb_fp8_linear": (_I, [_VP, _LL, _VP, _I, _VP, _VP, _VP, _I, _I, _I, _VP, ctypes.c_size_t, _I, _VP]),
+    "tlb_fp8_gated_mlp_workspace": (ctypes.c_size_t, [_I, _I, _I]),
+    "tlb_fp8_gated_mlp": (_I, [_VP, _LL, _VP, _I, _VP, _VP, _I, _VP, _VP, _I, _I, _I, _I, _F, _F, _VP, ctypes.c_size_t, _I, _VP]),
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 
-ABI_VERSION = 10
+ABI_VERSION = 11
 ATTENTION_TILE_TOKENS = 4
 ACT_SILU, ACT_GELU_TANH, ACT_RELU_SQUARED, ACT_CLAMPED_SWISH, ACT_TANH = 0, 1, 2, 3, 4
 WEIGHTS_SOFTMAX, WEIGHTS_SIGMOID = 0, 1
@@ -1073,4 +1078,59 @@ def shift_mix(h, mu, *, seq_info, state, max_tokens: int):
     out = torch.empty((n, T, dim), dtype=h.dtype, device=h.device)
     _check(library().tlb_shift_mix(_ptr(h), h.stride(0), _ptr(mu), n, dim, _ptr(seq_info), seq_info.shape[0], max(1, int(max_tokens)), _ptr(state),
                                    state.stride(0), state.shape[0], _ptr(out), T * dim, _code(h.dtype), _stream(h)))
+    return out
+
+
+def _rows_of(op: str, x: torch.Tensor, width: int, device) -> torch.Tensor:
+    """``x`` as a matrix of rows with unit inner stride on the weights' device."""
+    if x.shape[-1] != width:
+        raise RuntimeError(f"{op}: rows of {x.shape[-1]} for weights of {width} columns")
+    if not x.is_cuda or x.device != device:
+        raise RuntimeError(f"{op}: the blocks extension is GPU-only, and rows and weights must be on one device")
+    rows = x if x.dim() == 2 else x.reshape(-1, width)
+    return rows if rows.stride(1) == 1 and rows.stride(0) >= width or rows.shape[0] <= 1 and rows.stride(1) == 1 else rows.contiguous()
+
+
+class _on:
+    """Launches go to the tensors' device, whichever is current."""
+
+    def __new__(cls, device):
+        return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def fp8_linear(x: torch.Tensor, values: torch.Tensor, scales: torch.Tensor, width: int, bias=None) -> torch.Tensor:
+    """``x [.., width]`` (bf16 or fp32; rows may be apart) times ``values [N, >= width]`` (e4m3, rows of a multiple of 16 bytes,
+    zero behind ``width``) with ``scales [ceil(N / 128), ceil(width / 128)]`` fp32, plus ``bias [N]`` -> ``[.., N]`` in ``x``'s dtype.  The rows are
+    rounded to e4m3 with a scale for each run of 128, see ``tlb_fp8_linear``."""
+    n = values.shape[0]
+    rows = _rows_of("fp8_linear", x, width, values.device)
+    if bias is not None and (bias.shape != (n,) or bias.dtype != x.dtype or bias.device != values.device or not bias.is_contiguous()):
+        raise RuntimeError("fp8_linear: bias must be [outputs] of the rows' dtype")
+    code, T = _code(x.dtype), rows.shape[0]
+    lib = library()
+    with _on(values.device):
+        out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=values.device)
+        if T:
+            size = lib.tlb_fp8_linear_workspace(T, width)
+            scratch = torch.empty(size, dtype=torch.uint8, device=values.device)
+            _check(lib.tlb_fp8_linear(rows.data_ptr(), max(rows.stride(0), width), values.data_ptr(), values.stride(0), scales.data_ptr(), _ptr(bias), out.data_ptr(), T, n,
+                                      width, scratch.data_ptr(), size, code, _stream(values)))
+    return out
+
+
+def fp8_gated_mlp(x: torch.Tensor, gate_up, down, width: int, inner: int, act: int, limit: float = 0.0, slope: float = 1.0) -> torch.Tensor:
+    """``down(act(gate x) * (up x))`` over e4m3 matrices, the inner rows rounded as ``x``'s are (from fp32) -> ``x``'s shape and dtype.  ``gate_up`` =
+    (values ``[2 * 128 * ceil(inner / 128), ..]``, scales): runs of 128 rows of the gate and of the up projection in turn, zero behind
+    ``inner``; ``down`` = (values ``[width, ..]``, scales).  ``limit`` and ``slope`` go with ``ACT_CLAMPED_SWISH``."""
+    (wg, sg), (wd, sd) = gate_up, down
+    rows = _rows_of("fp8_gated_mlp", x, width, wg.device)
+    code, T = _code(x.dtype), rows.shape[0]
+    lib = library()
+    with _on(wg.device):
+        out = torch.empty((*x.shape[:-1], wd.shape[0]), dtype=x.dtype, device=wg.device)
+        if T:
+            size = lib.tlb_fp8_gated_mlp_workspace(T, width, inner)
+            scratch = torch.empty(size, dtype=torch.uint8, device=wg.device)
+            _check(lib.tlb_fp8_gated_mlp(rows.data_ptr(), max(rows.stride(0), width), wg.data_ptr(), wg.stride(0), sg.data_ptr(), wd.data_ptr(), wd.stride(0), sd.data_ptr(),
+                                         out.data_ptr(), T, width, inner, act, float(limit), float(slope), scratch.data_ptr(), size, code, _stream(wg)))
     return out

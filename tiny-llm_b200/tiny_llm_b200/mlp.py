@@ -61,6 +61,32 @@ class GatedMLP:
         return (linear_wide if wide else linear)(self.inner(h), self.w_down)
 
 
+class Fp8GatedMLP:
+    """``down(act(gate x) * (up x))`` over matrices of 8-bit numbers (``Fp8Weights``): both products in 8 bits, the inner rows fp32 until
+    they are rounded as the input's are.  ``act``, ``limit``, ``slope``: see ``GatedMLP``."""
+
+    def __init__(self, w_gate, w_up, w_down, act: str, limit: float = 0.0, slope: float = 1.0):
+        from .fp8 import Fp8Weights, interleaved
+
+        if not all(isinstance(w, Fp8Weights) and len(w.shape) == 2 for w in (w_gate, w_up, w_down)):
+            raise ValueError("Fp8GatedMLP: three matrices as Fp8Weights")
+        if w_gate.shape != w_up.shape or w_down.shape != w_up.shape[::-1] or len({w.device for w in (w_gate, w_up, w_down)}) != 1:
+            raise ValueError(f"Fp8GatedMLP: gate {w_gate.shape}, up {w_up.shape} and down {w_down.shape} do not go together")
+        if act not in ("silu", "gelu_tanh", "clamped_swish"):
+            raise ValueError(f"Fp8GatedMLP: no gated activation {act!r}")
+        self.inner_width, self.width = w_up.shape
+        self.w_gate_up, self.s_gate_up = interleaved(w_gate, w_up)
+        self.w_down, self.s_down = w_down.values, w_down.scales
+        self.act, self.limit, self.slope = ACTIVATIONS[act], float(limit), float(slope)
+        if act == "clamped_swish" and not self.limit > 0:
+            raise ValueError("Fp8GatedMLP: the clamped activation needs a positive limit")
+
+    def __call__(self, h: torch.Tensor) -> torch.Tensor:
+        from extensions_b200.tiny_llm_ext_b200 import blocks
+
+        return blocks.fp8_gated_mlp(h, (self.w_gate_up, self.s_gate_up), (self.w_down, self.s_down), self.width, self.inner_width, self.act, self.limit, self.slope)
+
+
 class TopKRouter:
     def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None, top: int, scoring: str = "softmax", choice_bias: torch.Tensor | None = None,
                  weight_scale: float = 1.0, groups: tuple | None = None):
