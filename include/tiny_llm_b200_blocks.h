@@ -354,6 +354,21 @@ int tlb_moe_combine_tanh(float *x, const float *pair_out, const float *gate, con
 /* Row-wise arg-max of fp32 logits [rows, vocab] (lowest index wins a tie). */
 int tlb_argmax_rows(const float *logits, int32_t *out, int rows, int vocab, void *stream);
 
+/* A whole mixture-of-experts layer for a few bf16 tokens x [tokens, dim], in two launches: the router and its choice as tlb_moe_route makes it (router
+ * [outputs, dim], bias, choice_bias, scoring, groups; side_w: the gate of the shared expert), then
+ *   y[t] = sum over choices  weight * down_e(act(gate_e x) * (up_e x))   (+ sigmoid(side_w . x) * shared[t], shared bf16 [tokens, dim] or NULL)
+ * rounded to bf16, or fp32 (out_f32).  Experts w_gate, w_up [experts, ff, ld_in bytes], w_down [experts, dim, ld_out bytes], bf16 (fp8 = 0) or e4m3 with scales
+ * [experts, ceil(rows / 128), ceil(columns / 128)]; rows are whole 16-byte pieces, zero behind the last number; w_gate NULL: act(up_e x), act 2 allowed.
+ * Ids from `experts` up to `outputs` are identity experts.  The inner rows are kept to 2^-11 of their value or better.  dim must be a multiple of 8.
+ * tlb_moe_few_tokens: the most tokens a call takes at these sizes (0: none).  A token's result does not depend on the others, but for the ranges
+ * 1-8, 9-16, 17-32 of tokens in a call. */
+int tlb_moe_few_tokens(int dim, int outputs, int experts, int top, int group_count, int fp8);
+size_t tlb_moe_few_workspace(int tokens, int top, int experts, int ff);
+int tlb_moe_few(const void *x, const void *router, const void *router_bias, const void *choice_bias, const void *side_w, int tokens, int dim, int outputs, int experts,
+                int top, int scoring, float weight_scale, int group_count, int group_keep, const void *w_gate, const void *w_up, const void *w_down, const float *s_gate,
+                const float *s_up, const float *s_down, int fp8, int ff, int ld_in, int ld_out, int act, float limit, float slope, const void *shared, void *out, int out_f32,
+                void *workspace, size_t workspace_bytes, void *stream);
+
 /* Products over matrices of 8-bit numbers (e4m3) with one fp32 scale for each block of 128 x 128: w [n, ldw] bytes (ldw a multiple of 16, the
  * base 16-byte aligned, zero behind column k), sw [ceil(n / 128), ceil(k / 128)].  The rows x [rows, k] (`dtype`, ldx apart) are rounded to e4m3 with
  * one scale for each run of 128 of a row:  m = max(|x| of the run, 2^-100), q = e4m3(x * (448 / m)), scale = m / 448, every operation rounded

@@ -150,64 +150,7 @@ moe_route_kernel(const T *__restrict__ h, const T *__restrict__ w, const T *__re
     float *z = logits + warp * per_token;  // [experts]: what the choice is made by
     float *p_all = z + experts;            // [experts]: scoring 2, the softmax over all outputs
     float *best = p_all + experts;         // [group_count]: the largest choice score of every group
-    if (scoring == 2) {  // scores = softmax over ALL outputs; the choice adds a bias to them, the weights do not
-        float m = -INFINITY, sum = 0.f;
-        for (int e = lane; e < experts; e += 32) m = fmaxf(m, z[e]);
-        m = warp_max(m);
-        for (int e = lane; e < experts; e += 32) sum += expf(z[e] - m);
-        sum = warp_sum(sum);
-        for (int e = lane; e < experts; e += 32) {
-            float p = expf(z[e] - m) / sum;
-            p_all[e] = p;
-            z[e] = p + (choice_bias ? to_f(choice_bias[e]) : 0.f);
-        }
-        __syncwarp();
-    }
-    if (group_keep > 0 && group_keep < group_count) {  // only the outputs of the best groups of neighbours can be chosen
-        const int size = experts / group_count;
-        for (int j = lane; j < group_count; j += 32) {
-            float m = -INFINITY;
-            for (int e = j * size; e < (j + 1) * size; ++e) m = fmaxf(m, z[e]);
-            best[j] = m;
-        }
-        __syncwarp();
-        for (int e = lane; e < experts; e += 32) {
-            const int j = e / size;
-            int ahead = 0;  // groups in front of this one (lower index wins a tie)
-            for (int i = 0; i < group_count; ++i) ahead += best[i] > best[j] || (best[i] == best[j] && i < j);
-            if (ahead >= group_keep) z[e] = -INFINITY;
-        }
-        __syncwarp();
-    }
-    // top-k by repeated arg-max over the warp (lower index wins a tie); weights = softmax over the chosen logits
-    float first_v = 0.f, denom = 0.f;
-    for (int k = 0; k < top; ++k) {
-        float bv = -INFINITY;
-        int bi = 0x7fffffff;
-        for (int e = lane; e < experts; e += 32) {
-            float v = z[e];
-            if (v > bv || (v == bv && e < bi)) bv = v, bi = e;
-        }
-        for (int o = 16; o > 0; o >>= 1) {
-            float ov = __shfl_xor_sync(0xffffffffu, bv, o);
-            int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-            if (ov > bv || (ov == bv && oi < bi)) bv = ov, bi = oi;
-        }
-        if (k == 0) first_v = bv;
-        // scoring 0: softmax over the chosen logits (the first choice is the largest); 1: each choice's own sigmoid, as it is
-        float p = scoring == 1 ? 1.0f / (1.0f + expf(-bv)) : scoring == 2 ? p_all[min(bi, experts - 1)] : expf(bv - first_v);
-        denom += p;
-        if (lane == 0) {
-            idx[(size_t)t * top + k] = bi;
-            gate[(size_t)t * top + k] = p;
-            if (bi != 0x7fffffff) z[bi] = -INFINITY;
-        }
-        __syncwarp();
-    }
-    if (scoring == 1) return;
-    // scoring 2: the chosen scores renormalised (a guard against an all-zero choice) and scaled
-    for (int k = lane; k < top; k += 32)
-        gate[(size_t)t * top + k] = scoring == 2 ? gate[(size_t)t * top + k] / (denom + 1e-20f) * weight_scale : gate[(size_t)t * top + k] / denom;
+    moe_choose(z, p_all, best, lane, experts, top, scoring, choice_bias, weight_scale, group_count, group_keep, idx + (size_t)t * top, gate + (size_t)t * top);
 }
 
 // C tile [32 rows x 64 columns] of  A[rows, K] . W[e][cols, K]^T, fp32 accumulation in k order.

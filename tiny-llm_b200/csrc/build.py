@@ -58,6 +58,7 @@ BLOCKS_SOURCES = [
     "blocks/blocks_streams.cu",
     "blocks/blocks_tanh_norm.cu",
     "blocks/blocks_matrix_memory.cu",
+    "blocks/blocks_moe_few.cu",
     "blocks/blocks_fp8_rows.cu",
     "blocks/blocks_fp8_product.cu",
 ]

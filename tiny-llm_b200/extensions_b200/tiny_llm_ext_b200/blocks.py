@@ -93,6 +93,10 @@ _SIGNATURES = {
     "tlb_tc_gave_up": (_LL, []),
     "tlb_moe_combine": (_I, [_VP, _VP, _VP, _VP, _VP, _I, _VP, _VP, _I, _I, _I, _I, _VP]),
     "tlb_argmax_rows": (_I, [_VP, _VP, _I, _I, _VP]),
+    "tlb_moe_few_tokens": (_I, [_I, _I, _I, _I, _I, _I]),
+    "tlb_moe_few_workspace": (ctypes.c_size_t, [_I, _I, _I, _I]),
+    "tlb_moe_few": (_I, [_VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _F, _I, _I, _VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _F, _F, _VP, _VP, _I, _VP,
+                         ctypes.c_size_t, _VP]),
     "tlb_fp8_linear_workspace": (ctypes.c_size_t, [_I, _I]),
     "tlb_fp8_linear": (_I, [_VP, _LL, _VP, _I, _VP, _VP, _VP, _I, _I, _I, _VP, ctypes.c_size_t, _I, _VP]),
     "tlb_fp8_gated_mlp_workspace": (ctypes.c_size_t, [_I, _I, _I]),
@@ -1133,4 +1137,52 @@ def fp8_gated_mlp(x: torch.Tensor, gate_up, down, width: int, inner: int, act: i
             scratch = torch.empty(size, dtype=torch.uint8, device=wg.device)
             _check(lib.tlb_fp8_gated_mlp(rows.data_ptr(), max(rows.stride(0), width), wg.data_ptr(), wg.stride(0), sg.data_ptr(), wd.data_ptr(), wd.stride(0), sd.data_ptr(),
                                          out.data_ptr(), T, width, inner, act, float(limit), float(slope), scratch.data_ptr(), size, code, _stream(wg)))
+    return out
+
+
+def moe_few_tokens(dim: int, outputs: int, experts: int, top: int, group_count: int = 0, fp8: bool = False) -> int:
+    """The most tokens that ``moe_few`` takes at these sizes."""
+    return int(library().tlb_moe_few_tokens(dim, outputs, experts, top, group_count, int(fp8)))
+
+
+def moe_few(h, router_w, router_b, top: int, w_gate, w_up, w_down, act: int, *, scales=None, inner: int, scoring: int = SCORE_SOFTMAX, choice_bias=None,
+            weight_scale: float = 1.0, groups=(0, 0), side_w=None, limit: float = 0.0, slope: float = 1.0, shared=None, wide: bool = False) -> torch.Tensor:
+    """A mixture-of-experts layer for a few bf16 tokens ``h [T, D]`` in two launches -> ``[T, D]`` bf16, or (``wide``) fp32.  The router's arguments are those
+    of ``moe_route``; ``w_gate`` (or None), ``w_up [E, inner, ..]``, ``w_down [E, D, ..]`` bf16, or e4m3 with ``scales`` = (gate's, up's, down's): rows of whole
+    16-byte pieces, zero behind the last number.  Outputs of the router from ``E`` up are identity experts.  ``shared [T, D]`` is added, times
+    ``sigmoid(side_w . h)`` with ``side_w``."""
+    _gpu("moe_few", h, router_w, router_b, choice_bias, side_w, w_gate, w_up, w_down, shared)
+    _contig("moe_few", h, router_w, router_b, choice_bias, side_w, w_gate, w_up, w_down, shared)
+    T, D = h.shape
+    fp8 = scales is not None
+    E, size = w_up.shape[0], w_up.element_size()
+    for t in (h, router_w, router_b, choice_bias, side_w, shared):
+        if t is not None and t.dtype != torch.bfloat16:
+            raise RuntimeError("moe_few: activations, router and shared rows must be bfloat16")
+    if any(w is not None and w.dtype != (torch.float8_e4m3fn if fp8 else torch.bfloat16) for w in (w_gate, w_up, w_down)):
+        raise RuntimeError("moe_few: experts must be bfloat16, or float8_e4m3fn with scales")
+    if router_w.shape[1] != D or (router_b is not None and router_b.numel() != router_w.shape[0]) or (choice_bias is not None and choice_bias.numel() != router_w.shape[0]):
+        raise RuntimeError("moe_few: router must be [outputs, D], its biases [outputs]")
+    if (side_w is not None and (side_w.numel() != D or shared is None)) or (shared is not None and shared.shape != h.shape):
+        raise RuntimeError("moe_few: shared must be [T, D], side_w [1, D] with it")
+    if w_up.dim() != 3 or w_up.shape[1] != inner or w_up.shape[2] < D or w_down.dim() != 3 or w_down.shape[:2] != (E, D) or w_down.shape[2] < inner or (
+            w_gate is not None and w_gate.shape != w_up.shape):
+        raise RuntimeError("moe_few: experts must be [E, inner, >= D] and [E, D, >= inner]")
+    sg, su, sd = scales if fp8 else (None, None, None)
+    blocks_of = lambda n, k: (E, -(-n // 128), -(-k // 128))  # noqa: E731
+    for s, shape in ((sg, blocks_of(inner, D)), (su, blocks_of(inner, D)), (sd, blocks_of(D, inner))) if fp8 else ():
+        if s is not None and (s.dtype != torch.float32 or tuple(s.shape) != shape or not s.is_contiguous() or not s.is_cuda):
+            raise RuntimeError("moe_few: scales must be float32, one for each block of 128 x 128")
+    if len({t.device for t in (h, router_w, router_b, choice_bias, side_w, w_gate, w_up, w_down, shared, sg, su, sd) if t is not None}) != 1:
+        raise RuntimeError("moe_few: tensors on two devices")
+    lib = library()
+    with _on(h.device):
+        out = torch.empty((T, D), dtype=torch.float32 if wide else torch.bfloat16, device=h.device)
+        if T:
+            size_ws = lib.tlb_moe_few_workspace(T, top, E, inner)
+            scratch = torch.empty(size_ws, dtype=torch.uint8, device=h.device)
+            _check(lib.tlb_moe_few(h.data_ptr(), router_w.data_ptr(), _ptr(router_b), _ptr(choice_bias), _ptr(side_w), T, D, router_w.shape[0], E, top, int(scoring),
+                                   float(weight_scale), int(groups[0]), int(groups[1]), _ptr(w_gate), w_up.data_ptr(), w_down.data_ptr(), _ptr(sg), _ptr(su), _ptr(sd),
+                                   int(fp8), inner, w_up.shape[2] * size, w_down.shape[2] * size, act, float(limit), float(slope), _ptr(shared), out.data_ptr(), int(wide),
+                                   scratch.data_ptr(), size_ws, _stream(h)))
     return out

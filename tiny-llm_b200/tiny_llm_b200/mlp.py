@@ -156,3 +156,76 @@ class MixtureOfExperts:
         join = beside._join if beside is not None and self.shared is not None else None
         return blocks.moe_experts(h, idx, gate, self.w_gate, self.w_up, self.w_down, self.act, shared, scale_input=self.scale_input, identity=self.identity > 0,
                                   limit=self.limit, slope=self.slope, shared_gate=side, into=into, before_sum=join)
+
+
+def _whole_rows(w: torch.Tensor, rows: int) -> torch.Tensor:
+    """A stack of matrices with ``rows`` rows of whole 16-byte pieces, zero behind what it holds; itself where it is laid out so."""
+    per = 16 // w.element_size()
+    n, k = w.shape[1:]
+    if n == rows and k % per == 0 and w.is_contiguous() and w.data_ptr() % 16 == 0:
+        return w
+    wide = torch.zeros((w.shape[0], rows, -(-k // per) * per * w.element_size()), dtype=torch.uint8, device=w.device).view(w.dtype)
+    wide.view(torch.uint8)[:, :n, : k * w.element_size()] = w.contiguous().view(torch.uint8)
+    return wide
+
+
+class FewTokenExperts:
+    """A whole mixture-of-experts layer for the few tokens of a decoding step in two launches: router and first products, second products
+    and their sum.  Arguments as ``MixtureOfExperts`` takes them, the experts bf16 ``[E, ff, D]`` / ``[E, D, ff]`` or ``Fp8Weights`` of those shapes; the
+    router's weight is on the experts' output.  A step of more tokens than one call takes (32, fewer for very wide ones) is several calls, each of which reads its
+    experts anew: prompts are better served by ``MixtureOfExperts``."""
+
+    def __init__(self, router: TopKRouter, w_gate, w_up, w_down, act: str, shared: GatedMLP | None = None, identity: int = 0, limit: float = 0.0, slope: float = 1.0,
+                 shared_gate: torch.Tensor | None = None):
+        from extensions_b200.tiny_llm_ext_b200 import blocks
+
+        from .fp8 import Fp8Weights
+
+        weights = [w for w in (w_gate, w_up, w_down) if w is not None]
+        fp8 = isinstance(w_up, Fp8Weights)
+        if any(isinstance(w, Fp8Weights) != fp8 for w in weights) or any(len(w.shape) != 3 for w in weights):
+            raise ValueError("FewTokenExperts: stacks of matrices, all of 8 bits or none")
+        E, ff, D = w_up.shape
+        if tuple(w_down.shape) != (E, D, ff) or (w_gate is not None and tuple(w_gate.shape) != (E, ff, D)):
+            raise ValueError(f"FewTokenExperts: up {tuple(w_up.shape)} and down {tuple(w_down.shape)} do not go together")
+        if not fp8 and any(w.dtype != torch.bfloat16 for w in weights):
+            raise ValueError("FewTokenExperts: unquantised experts must be bfloat16")
+        if identity < 0 or router.weight.shape != (E + identity, D) or router.weight.dtype != torch.bfloat16:
+            raise ValueError(f"FewTokenExperts: the router must be bfloat16 [{E} experts + {identity} identity experts, {D}]")
+        if (act == "relu_squared" and w_gate is not None) or (act == "clamped_swish" and (w_gate is None or not limit > 0)):
+            raise ValueError(f"FewTokenExperts: activation {act!r} does not go with {'gated' if w_gate is not None else 'ungated'} experts")
+        if shared_gate is not None and (shared is None or shared_gate.numel() != D):
+            raise ValueError("FewTokenExperts: a shared gate of [1, width] goes with a shared expert")
+        if len({w.device for w in (*weights, router.weight)}) != 1:
+            raise ValueError("FewTokenExperts: router and experts on two devices")
+        self.router, self.shared, self.width, self.inner_width = router, shared, D, ff
+        self.act, self.limit, self.slope = ACTIVATIONS[act], float(limit), float(slope)
+        self._pad = -D % 8
+        rows = D + self._pad
+        raw = lambda w, n: None if w is None else _whole_rows(w.values if fp8 else w.contiguous(), n)  # noqa: E731
+        self.w_gate, self.w_up, self.w_down = raw(w_gate, ff), raw(w_up, ff), raw(w_down, rows)
+        self.scales = None if not fp8 else tuple(None if w is None else w.scales for w in (w_gate, w_up, w_down))
+        wider = lambda t: t if t is None or not self._pad else torch.nn.functional.pad(t.reshape(-1, D), (0, self._pad)).contiguous()  # noqa: E731
+        self.router_w = wider(router.weight)
+        self.shared_gate = None if shared_gate is None else wider(shared_gate.contiguous())
+        self.run = blocks.moe_few_tokens(rows, E + identity, E, router.top, router.groups[0], fp8) if w_up.device.type == "cuda" else 0
+        if w_up.device.type == "cuda" and self.run == 0:
+            raise ValueError(f"FewTokenExperts: width {D}, {E + identity} router outputs and {router.top} choices do not fit")
+
+    def __call__(self, h: torch.Tensor, wide: bool = False) -> torch.Tensor:
+        """``h [T, D]`` bf16 -> ``[T, D]`` bf16, or with ``wide`` the fp32 sums."""
+        from extensions_b200.tiny_llm_ext_b200 import blocks
+
+        if h.dim() != 2 or h.shape[1] != self.width or h.dtype != torch.bfloat16:
+            raise RuntimeError(f"FewTokenExperts: expected bfloat16 [tokens, {self.width}]")
+        shared = None if self.shared is None else self.shared(h)
+        if self._pad:
+            h, shared = (None if t is None else torch.nn.functional.pad(t, (0, self._pad)) for t in (h, shared))
+        h = h.contiguous() if h.data_ptr() % 16 == 0 else h.clone(memory_format=torch.contiguous_format)
+        r = self.router
+        parts = [blocks.moe_few(h[t : t + self.run], self.router_w, r.bias, r.top, self.w_gate, self.w_up, self.w_down, self.act, scales=self.scales, inner=self.inner_width,
+                                scoring=r.scoring, choice_bias=r.choice_bias, weight_scale=r.weight_scale, groups=r.groups, side_w=self.shared_gate, limit=self.limit,
+                                slope=self.slope, shared=None if shared is None else shared[t : t + self.run], wide=wide)
+                 for t in range(0, max(1, h.shape[0]), max(1, self.run))]
+        y = parts[0] if len(parts) == 1 else torch.cat(parts)
+        return y[:, : self.width] if self._pad else y
