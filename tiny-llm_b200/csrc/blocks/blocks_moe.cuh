@@ -59,18 +59,21 @@ __device__ __forceinline__ void moe_choose(float *z, float *p_all, float *best, 
     }
     // top-k by repeated arg-max over the warp (lower index wins a tie); weights = softmax over the chosen logits
     float first_v = 0.f, denom = 0.f;
+    // A number's bits in an order that whole numbers have too; 0 for NaN, which is never chosen.  Minus zero counts as zero.
+    auto ordered = [](float v) {
+        const uint32_t u = __float_as_uint(v + 0.f);
+        return v != v ? 0u : u & 0x80000000u ? ~u : u | 0x80000000u;
+    };
     for (int k = 0; k < top; ++k) {
-        float bv = -INFINITY;
+        uint32_t best_v = 0;
         int bi = 0x7fffffff;
         for (int e = lane; e < experts; e += 32) {
-            float v = z[e];
-            if (v > bv || (v == bv && e < bi)) bv = v, bi = e;
+            const uint32_t v = ordered(z[e]);
+            if (v > best_v) best_v = v, bi = e;
         }
-        for (int o = 16; o > 0; o >>= 1) {
-            float ov = __shfl_xor_sync(0xffffffffu, bv, o);
-            int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-            if (ov > bv || (ov == bv && oi < bi)) bv = ov, bi = oi;
-        }
+        const uint32_t most = __reduce_max_sync(0xffffffffu, best_v);
+        bi = __reduce_min_sync(0xffffffffu, best_v == most && most ? bi : 0x7fffffff);
+        const float bv = most ? __uint_as_float(most & 0x80000000u ? most & 0x7fffffffu : ~most) : -INFINITY;
         if (k == 0) first_v = bv;
         // scoring 0: softmax over the chosen logits (the first choice is the largest); 1: each choice's own sigmoid, as it is
         float p = scoring == 1 ? 1.0f / (1.0f + expf(-bv)) : scoring == 2 ? p_all[min(bi, experts - 1)] : expf(bv - first_v);

@@ -49,6 +49,8 @@ struct FewArgs {
     float *inner;      // [tokens * top, ld_inner], zero behind ff
     float *most;       // e4m3: [(run of features) + (position of the expert)][32], the largest magnitude of a token's inner row in that run
     int ld_inner, runs;  // runs of features: teams of the first launch
+    int room;            // bytes of shared memory that a launch may use
+    int prefetch;        // bytes that a CTA of the first launch asks into L2 for the second
 };
 
 // ---- small things ----------------------------------------------------------------------------------------------------
@@ -84,21 +86,69 @@ __device__ __forceinline__ int few_exponent(float most) {
 }
 __device__ __forceinline__ float few_exp2(int e) { return __int_as_float((e + 127) << 23); }
 
-// A warp's piece of 16 rows: 128 bytes of each.  A lane has rows g = lane / 4 and g + 8, 16 bytes at t * 16 (t = lane % 4) of either half.
+// A warp's piece of 16 rows: 128 bytes of each.  A lane has rows g = lane / 4 and g + 8, 16 bytes at t * 16 (t = lane % 4) of either half: it asks for exactly
+// what it will use (cp.async), into places of its own, so a piece is waited for by counting one's own copies, without a barrier.
 struct FewPiece {
     uint4 a[2], b[2];  // rows g, g + 8
     float sa, sb;      // their scales
 };
+constexpr int kFewPiece = 4 * kFewThreads * 16;  // bytes of one piece of all warps, its scales behind it
+static inline __host__ __device__ int few_place(bool fp8) { return kFewPiece + (fp8 ? 2 * kFewThreads * 4 : 0); }
+__device__ __forceinline__ void few_copy16(uint32_t to, const uint8_t *from, bool there) {
+    const int bytes = there ? 16 : 0;  // 0: zeros
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void few_copy4(uint32_t to, const float *from, bool there) {
+    const int bytes = there ? 4 : 0;
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void few_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// place: of the queue, in shared memory; base: any address that may be read, for what is not there.
 template <bool FP8>
-__device__ __forceinline__ void few_load(FewPiece &p, const uint8_t *row_a, const uint8_t *row_b, int at, int bytes) {
-    const uint4 none = make_uint4(0, 0, 0, 0);
+__device__ __forceinline__ void few_ask(uint32_t place, const uint8_t *row_a, bool va, const uint8_t *row_b, bool vb, int at, int bytes, const float *sa, const float *sb,
+                                        const uint8_t *base) {
+    const uint32_t to = place + threadIdx.x * 16;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
         const int o = at + c * 64;
-        p.a[c] = row_a && o < bytes ? few_ldg(row_a + o) : none;
-        p.b[c] = row_b && o < bytes ? few_ldg(row_b + o) : none;
+        const bool ta = va && o < bytes, tb = vb && o < bytes;
+        few_copy16(to + c * kFewThreads * 16, ta ? row_a + o : base, ta);
+        few_copy16(to + (2 + c) * kFewThreads * 16, tb ? row_b + o : base, tb);
+    }
+    if constexpr (FP8) {
+        const uint32_t scales = place + kFewPiece + threadIdx.x * 4;
+        few_copy4(scales, va ? sa : reinterpret_cast<const float *>(base), va);
+        few_copy4(scales + kFewThreads * 4, vb ? sb : reinterpret_cast<const float *>(base), vb);
     }
 }
+template <bool FP8>
+__device__ __forceinline__ FewPiece few_take(const unsigned char *place) {
+    FewPiece p;
+    const unsigned char *from = place + threadIdx.x * 16;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        p.a[c] = *reinterpret_cast<const uint4 *>(from + c * kFewThreads * 16);
+        p.b[c] = *reinterpret_cast<const uint4 *>(from + (2 + c) * kFewThreads * 16);
+    }
+    if constexpr (FP8) {
+        p.sa = *reinterpret_cast<const float *>(place + kFewPiece + threadIdx.x * 4);
+        p.sb = *reinterpret_cast<const float *>(place + kFewPiece + kFewThreads * 4 + threadIdx.x * 4);
+    }
+    return p;
+}
+// The oldest of `depth` groups of this thread's copies is there (the others may still be on their way).
+__device__ __forceinline__ void few_wait(int depth) {
+    switch (depth) {
+        case 1: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
+        case 2: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+        case 3: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+        case 4: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+        case 5: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
+        default: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
+    }
+}
+constexpr int kFewDepth = 6;  // the most places of a queue
+
 // The products of half a piece (64 bytes of each row) with one tile of eight columns: x, the lane's 16 bytes' worth of column g.
 template <bool FP8>
 __device__ __forceinline__ void few_half(const uint4 &a, const uint4 &b, const uint32_t (&x)[FP8 ? 8 : 4], float (&d)[4]) {
@@ -116,45 +166,56 @@ __device__ __forceinline__ void few_half(const uint4 &a, const uint4 &b, const u
     }
 }
 
-// The chosen experts in ascending order and which choice of theirs a token has: both launches make these for themselves.
+// The chosen experts in ascending order and the tokens that chose each, in ascending order: a token's place is its column.  Both launches make these for
+// themselves.
 struct FewLists {
-    int *active;      // [kFewPairs]
-    uint8_t *choice;  // [kFewPairs][32]: choice + 1 of a token, 0: not chosen
+    uint32_t *words;   // [32]: a bit for every expert, zero at the start
+    uint32_t *tokens;  // [most]: the tokens of an active expert, zero at the start
+    int *active;       // [most]
+    uint16_t *column;  // [most][32]: token * 256 + choice
     int *count;
 };
-// All threads of the CTA; place [experts] is scratch.  idx: the choices, in shared memory.
-__device__ __forceinline__ void few_lists(const FewArgs &a, const int *idx, short *place, const FewLists &l) {
-    const int tid = threadIdx.x, lane = tid & 31;
-    for (int e = tid; e < a.experts; e += kFewThreads) place[e] = -1;
-    for (int i = tid; i < min(a.experts, a.tokens * a.top) * 8; i += kFewThreads) reinterpret_cast<uint32_t *>(l.choice)[i] = 0;
-    __syncthreads();
-    for (int p = tid; p < a.tokens * a.top; p += kFewThreads)
-        if (idx[p] < a.experts) place[idx[p]] = 0;
-    __syncthreads();
-    if (tid < 32) {
-        int n = 0;
-        for (int e0 = 0; e0 < a.experts; e0 += 32) {
-            const int e = e0 + lane;
-            const bool here = e < a.experts && place[e] == 0;
-            const uint32_t all = __ballot_sync(0xffffffffu, here);
-            if (here) {
-                const int at = n + __popc(all & ((1u << lane) - 1));
-                l.active[at] = e, place[e] = (short)at;
-            }
-            n += __popc(all);
-        }
-        if (lane == 0) *l.count = n;
+struct FewListsSmem {  // from `at` on, a multiple of 4
+    int words, tokens, active, count, column, end;
+    __host__ __device__ FewListsSmem(int at, int tokens_, int top, int experts) {
+        const int most = tokens_ * top < experts ? tokens_ * top : experts;
+        words = at, tokens = words + 128, active = tokens + most * 4, count = active + most * 4, column = count + 4, end = (column + most * 64 + 15) / 16 * 16;
     }
+    __device__ FewLists lists(unsigned char *smem) const {
+        return {reinterpret_cast<uint32_t *>(smem + words), reinterpret_cast<uint32_t *>(smem + tokens), reinterpret_cast<int *>(smem + active),
+                reinterpret_cast<uint16_t *>(smem + column), reinterpret_cast<int *>(smem + count)};
+    }
+    __device__ void clear(unsigned char *smem) const {  // words and tokens lie side by side
+        for (int i = threadIdx.x; i < (active - words) / 4; i += kFewThreads) reinterpret_cast<uint32_t *>(smem + words)[i] = 0;
+    }
+};
+// All threads of the CTA, a pair each; behind a barrier after clear() and the last write of idx, which is in shared memory.
+// -> the position of this thread's pair's expert, or -1.
+__device__ __forceinline__ int few_lists(const FewArgs &a, const int *idx, const FewLists &l) {
+    static_assert(kFewPairs <= kFewThreads, "a pair a thread");
+    const int p = threadIdx.x, lane = p & 31, t = p / a.top, k = p % a.top;
+    int e = p < a.tokens * a.top ? idx[p] : a.experts;
+    for (int j = 1; j <= k && e < a.experts; ++j)  // a token that names an expert twice (equal logits of minus infinity) has it once, by its first choice
+        if (idx[p - j] == e) e = a.experts;
+    const bool live = e < a.experts;
+    if (live) atomicOr(&l.words[e >> 5], 1u << (e & 31));
     __syncthreads();
-    if (tid < a.tokens)  // a token that names an expert twice (equal logits of minus infinity) has it once, by its first choice
-        for (int k = 0; k < a.top; ++k) {
-            const int e = idx[tid * a.top + k];
-            if (e < a.experts) {
-                uint8_t &c = l.choice[place[e] * 32 + tid];
-                if (c == 0) c = (uint8_t)(k + 1);
-            }
-        }
+    const uint32_t word = l.words[lane];
+    int before = __popc(word);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += v;
+    }
+    if (p == 31) *l.count = before;
+    before -= __popc(word);
+    const int at = live ? e >> 5 : 0, first = __shfl_sync(0xffffffffu, before, at);
+    const int pos = first + __popc(__shfl_sync(0xffffffffu, word, at) & ((1u << (e & 31)) - 1));
+    if (live) l.active[pos] = e, atomicOr(&l.tokens[pos], 1u << t);
     __syncthreads();
+    if (live) l.column[pos * 32 + __popc(l.tokens[pos] & ((1u << t) - 1))] = (uint16_t)(t * 256 + k);
+    __syncthreads();
+    return live ? pos : -1;
 }
 
 // Features 0 .. total - 1 in `runs` runs that differ by one at most.
@@ -166,26 +227,30 @@ __device__ __forceinline__ int few_run_of(int total, int runs, int f) {
 
 // ---- first launch ----------------------------------------------------------------------------------------------------
 
+constexpr int kFewCluster = 2;
+
 static inline __host__ __device__ int few_x_stride(int dim, bool fp8) {  // bytes of a token's row in shared memory: its 16-byte reads meet no bank conflict
     return (dim + 127) / 128 * 256 + (fp8 ? 16 : 64);
 }
 struct FewFirstSmem {
-    int x, red, logits, times, idx, gate, active, choice, place, flags, total;
-    __host__ __device__ FewFirstSmem(int tokens, int nt, int dim, int outputs, int experts, int top, int groups, bool fp8) {
+    int x, red, most, idx, gate, queue, logits, depth, total;
+    FewListsSmem lists;
+    __host__ __device__ FewFirstSmem(int tokens, int nt, int dim, int outputs, int experts, int top, int groups, bool fp8, int room) : lists(0, tokens, top, experts) {
         x = 0;
-        red = x + nt * 8 * few_x_stride(dim, fp8);
-        const int sums = kFewWarps * 16 * nt * 8 * 4;  // the teams' sums, or the router's
-        logits = red + sums;
-        const int per_token = 2 * outputs + groups;
-        times = logits + (tokens * per_token * 4 + tokens * 4 + 15) / 16 * 16;
-        idx = times + nt * 8 * 4;
+        red = x + tokens * few_x_stride(dim, fp8);
+        const int teams = 2 * kFewWarps * 16 * 8 * 4, router = kFewWarps * 16 * nt * 8 * 4;  // sums of a tile's eight columns, in turn in two places; the router's sums
+        most = red + teams;
+        idx = most + kFewTokens * 4;
         gate = idx + tokens * top * 4;
-        active = gate + tokens * top * 4;
-        const int most = tokens * top < experts ? tokens * top : experts;
-        choice = active + (most * 4 + 15) / 16 * 16;
-        place = choice + most * 32;
-        flags = (place + experts * 2 + 15) / 16 * 16;
-        total = flags + 16;
+        lists = FewListsSmem(gate + tokens * top * 4, tokens, top, experts);
+        // the router's sums and logits are done with when the queue's first copies are asked for
+        queue = lists.end;
+        logits = queue + router;
+        const int early = router + (tokens * (2 * outputs + groups) + tokens) * 4;
+        depth = (room - queue) / few_place(fp8);
+        if (depth > kFewDepth) depth = kFewDepth;
+        const int late = depth * few_place(fp8);
+        total = queue + (early > late ? early : late);
     }
 };
 
@@ -193,68 +258,96 @@ template <bool FP8, bool GATED, int NT>
 __global__ void __launch_bounds__(kFewThreads, 1)
 moe_few_first_kernel(const FewArgs a) {
     extern __shared__ __align__(128) unsigned char few_smem[];
-    const FewFirstSmem at(a.tokens, NT, a.dim, a.outputs, a.experts, a.top, a.group_count, FP8);
+    const FewFirstSmem at(a.tokens, NT, a.dim, a.outputs, a.experts, a.top, a.group_count, FP8, a.room);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     const int stride = few_x_stride(a.dim, FP8);
     uint32_t rank, ranks;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
-    float *red = reinterpret_cast<float *>(few_smem + at.red), *logits = reinterpret_cast<float *>(few_smem + at.logits);
+    // Another CTA's shared memory may be written once that CTA runs: arrived at here, waited for ahead of the first such store.
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    float *logits = reinterpret_cast<float *>(few_smem + at.logits), *router_red = reinterpret_cast<float *>(few_smem + at.queue);
     const int per_token = 2 * a.outputs + a.group_count;
-    float *side = logits + a.tokens * per_token;
+    float *side = logits + a.tokens * per_token, *gate = reinterpret_cast<float *>(few_smem + at.gate);
+    uint32_t *most = reinterpret_cast<uint32_t *>(few_smem + at.most);
     int *idx = reinterpret_cast<int *>(few_smem + at.idx);
-    float *gate = reinterpret_cast<float *>(few_smem + at.gate);
+    const FewLists lists = at.lists.lists(few_smem);
+    at.lists.clear(few_smem);
+    if (tid < kFewTokens) most[tid] = 0;
+    __syncthreads();
 
     tl::griddep_wait();
-    // the tokens' rows, zero behind the last entry and the last token
-    for (int i = tid; i < NT * 8 * (stride / 16); i += kFewThreads) {
-        const int t = i / (stride / 16), d = i % (stride / 16) * 8;
+    tl::griddep_launch();  // the second launch reads nothing ahead of its own wait
+    // ---- the router's rows, 16 for eight warps each, which share the reduction; a CTA of the cluster every ranks-th 32 of them
+    const int rows = a.outputs + (a.side_w ? 1 : 0), pieces = (a.dim * 2 + 127) / 128, part = warp & 7;
+    constexpr int AT_ONCE = 4;
+    uint4 wa[AT_ONCE][2], wb[AT_ONCE][2];
+    auto row_of = [&](int r) { return reinterpret_cast<const uint8_t *>(r < a.outputs ? a.router + (size_t)r * a.dim : r < rows ? a.side_w : nullptr); };
+    auto ask = [&](int m, int s0) {
+        const uint8_t *ra = row_of(m * 16 + g), *rb = row_of(m * 16 + g + 8);
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int o = (s0 + u * 8) * 128 + c * 64 + t4 * 16;
+                wa[u][c] = ra && o < a.dim * 2 ? few_ldg(ra + o) : make_uint4(0, 0, 0, 0);
+                wb[u][c] = rb && o < a.dim * 2 ? few_ldg(rb + o) : make_uint4(0, 0, 0, 0);
+            }
+    };
+    const int m_first = rank * 2 + (warp >> 3);
+    ask(m_first, part);
+    // ---- the tokens' rows, 256 entries a warp, zero behind the last one, and (8 bits) their largest magnitudes
+    const int entries = (a.dim + 127) / 128 * 128, segs = (entries + 255) / 256;
+    for (int i = warp; i < a.tokens * segs; i += kFewWarps) {
+        const int t = i / segs, d = i % segs * 256 + lane * 8;
         uint4 v = make_uint4(0, 0, 0, 0);
-        if (t < a.tokens && d < a.dim) v = tl::ld_cg(reinterpret_cast<const uint4 *>(a.x + (size_t)t * a.dim + d));
-        *reinterpret_cast<uint4 *>(few_smem + t * stride + d * 2) = v;
+        if (d < a.dim) v = tl::ld_cg(reinterpret_cast<const uint4 *>(a.x + (size_t)t * a.dim + d));
+        if (d < entries) *reinterpret_cast<uint4 *>(few_smem + t * stride + d * 2) = v;
+        if constexpr (FP8) {
+            const uint32_t c[4] = {v.x, v.y, v.z, v.w};
+            uint32_t top = 0;  // of the 15 bits of a magnitude, which are in order; an infinity is above all numbers, a NaN above that
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top = max(top, max(c[j] & 0x7fffu, c[j] >> 16 & 0x7fffu));
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0) atomicMax(&most[t], top);
+        }
     }
-    // The cluster's CTAs are known to run: their shared memory may be written.
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-
-    // ---- the router: 16 rows at a time, a CTA of the cluster every ranks-th of them, the reduction dealt to the 16 warps
-    const int rows = a.outputs + (a.side_w ? 1 : 0), pieces = (a.dim * 2 + 127) / 128;
-    for (int m = rank; m * 16 < rows; m += ranks) {
+    __syncthreads();
+    bool waited = false;
+    for (int m = m_first; (m - (warp >> 3)) * 16 < rows; m += ranks * 2) {
         float acc[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-        auto row_of = [&](int r) -> const uint8_t * {
-            return reinterpret_cast<const uint8_t *>(r < a.outputs ? a.router + (size_t)r * a.dim : r < rows ? a.side_w : nullptr);
-        };
-        const uint8_t *ra = row_of(m * 16 + g), *rb = row_of(m * 16 + g + 8);
-        for (int s = warp; s < pieces; s += 2 * kFewWarps) {
-            FewPiece p[2];
+        for (int s = part; s < pieces; s += AT_ONCE * 8) {
+            if (m != m_first || s != part) ask(m, s);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) few_load<false>(p[u], ra, rb, (s + u * kFewWarps) * 128 + t4 * 16, a.dim * 2);
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-                if (s + u * kFewWarps < pieces)
+            for (int u = 0; u < AT_ONCE; ++u)
+                if (s + u * 8 < pieces)
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            const uint4 v = *reinterpret_cast<const uint4 *>(few_smem + (n * 8 + g) * stride + (s + u * kFewWarps) * 128 + c * 64 + t4 * 16);
+                        for (int n = 0; n < NT; ++n) {  // columns past the last token: the last one, not used
+                            const uint4 v = *reinterpret_cast<const uint4 *>(few_smem + min(n * 8 + g, a.tokens - 1) * stride + (s + u * 8) * 128 + c * 64 + t4 * 16);
                             const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-                            few_half<false>(p[u].a[c], p[u].b[c], x, acc[n]);
+                            few_half<false>(wa[u][c], wb[u][c], x, acc[n]);
                         }
         }
-        float *mine = red + warp * 16 * NT * 8;
+        float *mine = router_red + warp * 16 * NT * 8;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             *reinterpret_cast<float2 *>(mine + g * NT * 8 + n * 8 + 2 * t4) = make_float2(acc[n][0], acc[n][1]);
             *reinterpret_cast<float2 *>(mine + (g + 8) * NT * 8 + n * 8 + 2 * t4) = make_float2(acc[n][2], acc[n][3]);
         }
         __syncthreads();
-        for (int i = tid; i < 16 * NT * 8; i += kFewThreads) {
-            const int r = m * 16 + i / (NT * 8), t = i % (NT * 8);
+        if (!waited) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all CTAs of the cluster run
+        waited = true;
+        const int m0 = m - (warp >> 3);
+        for (int i = tid; i < 2 * 16 * NT * 8; i += kFewThreads) {
+            const int in = i % (16 * NT * 8), r = (m0 + i / (16 * NT * 8)) * 16 + in / (NT * 8), t = in % (NT * 8);
             if (r >= rows || t >= a.tokens) continue;
             float z = 0.f;
 #pragma unroll
-            for (int w = 0; w < kFewWarps; ++w) z += red[w * 16 * NT * 8 + i];
+            for (int w = 0; w < 8; ++w) z += router_red[(i / (16 * NT * 8) * 8 + w) * 16 * NT * 8 + in];
             if (r < a.outputs && a.router_bias) z += to_f(a.router_bias[r]);
             const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(r < a.outputs ? logits + t * per_token + r : side + t));
             for (uint32_t c = 0; c < ranks; ++c)
@@ -262,7 +355,27 @@ moe_few_first_kernel(const FewArgs a) {
         }
         __syncthreads();
     }
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (!waited) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    if constexpr (FP8) {  // the rows as fp16 times a power of two; the router is done with them
+        for (int i = warp; i < a.tokens * segs; i += kFewWarps) {
+            const int t = i / segs, d = i % segs * 256 + lane * 8;
+            const float down = few_exp2(-few_exponent(__uint_as_float(most[t] << 16)));
+            if (d < entries) {
+                uint4 *p = reinterpret_cast<uint4 *>(few_smem + t * stride + d * 2);
+                const uint4 u = *p;
+                const uint32_t c[4] = {u.x, u.y, u.z, u.w};
+                uint32_t o[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 f = tl::unpack2<bf16>(c[j]);
+                    o[j] = few_half2(f.x * down, f.y * down);
+                }
+                *p = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+        }
+    }
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 
     // ---- the choice, by every CTA for itself
     for (int t = warp; t < a.tokens; t += kFewWarps) {
@@ -275,47 +388,11 @@ moe_few_first_kernel(const FewArgs a) {
         for (int p = tid; p < a.tokens * a.top; p += kFewThreads) a.idx[p] = idx[p], a.gate[p] = gate[p];
         if (a.side_w && tid < a.tokens) a.side[tid] = sigmoid(side[tid]);
     }
-    int *count = reinterpret_cast<int *>(few_smem + at.flags);
-    const FewLists lists{reinterpret_cast<int *>(few_smem + at.active), few_smem + at.choice, count};
-    few_lists(a, idx, reinterpret_cast<short *>(few_smem + at.place), lists);
-
-    // ---- with 8 bits: the rows as fp16 times a power of two
-    float *times = reinterpret_cast<float *>(few_smem + at.times);
-    if constexpr (FP8) {
-        for (int t = warp; t < NT * 8; t += kFewWarps) {
-            float most = 0.f;
-            const int entries = (a.dim + 127) / 128 * 128;
-            for (int d = lane * 8; d < entries; d += 256) {
-                const uint4 u = *reinterpret_cast<const uint4 *>(few_smem + t * stride + d * 2);
-                const uint32_t c[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 f = tl::unpack2<bf16>(c[i]);
-                    most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
-                }
-            }
-            const int e = few_exponent(warp_max(most));
-            const float down = few_exp2(-e);
-            for (int d = lane * 8; d < entries; d += 256) {
-                uint4 *p = reinterpret_cast<uint4 *>(few_smem + t * stride + d * 2);
-                const uint4 u = *p;
-                const uint32_t c[4] = {u.x, u.y, u.z, u.w};
-                uint32_t o[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 f = tl::unpack2<bf16>(c[i]);
-                    o[i] = few_half2(f.x * down, f.y * down);
-                }
-                *p = make_uint4(o[0], o[1], o[2], o[3]);
-            }
-            if (lane == 0) times[t] = few_exp2(e);
-        }
-        __syncthreads();
-    }
+    few_lists(a, idx, lists);
 
     // ---- the first products: a team takes its run of the chosen experts' features, up to 8 (with a gate; else 16) of one expert at a time
     constexpr int TILE = GATED ? 8 : 16;
-    const int team = warp / kFewTeam, sub = warp % kFewTeam, run = blockIdx.x * kFewTeams + team, total = *count * a.ff;
+    const int team = warp / kFewTeam, sub = warp % kFewTeam, run = blockIdx.x * kFewTeams + team, total = *lists.count * a.ff;
     const int blocks_in = (a.bytes_in + 127) / 128, iters = (blocks_in + kFewTeam - 1) / kFewTeam;
     const int scale_cols = (a.dim + 127) / 128, scale_rows = (a.ff + 127) / 128;
     struct Tile {
@@ -333,193 +410,193 @@ moe_few_first_kernel(const FewArgs a) {
         tile.left = f1 - f0, tile.pos = f0 / a.ff, tile.row = f0 % a.ff;
         cut(tile);
     }
+    const uint32_t queue = static_cast<uint32_t>(__cvta_generic_to_shared(few_smem + at.queue));
+    const int place = few_place(FP8);
     Tile ahead = tile;
-    int ahead_it = 0;
-    auto issue = [&](FewPiece &p) {
-        if (ahead.left <= 0) return;
-        const int e = lists.active[ahead.pos], b = sub + ahead_it * kFewTeam;
-        const size_t r0 = (size_t)e * a.ff + ahead.row;
-        const int second = GATED ? g : g + 8;
-        const bool va = g < ahead.here && b < blocks_in, vb = second < ahead.here && b < blocks_in;
-        few_load<FP8>(p, va ? a.w0 + (r0 + g) * a.ld_in : nullptr, vb ? (GATED ? a.w1 : a.w0) + (r0 + second) * a.ld_in : nullptr, b * 128 + t4 * 16, a.bytes_in);
-        if constexpr (FP8) {
+    int ahead_it = 0, ask_at = 0, take_at = 0;
+    auto issue = [&] {
+        if (ahead.left > 0) {
+            const int e = lists.active[ahead.pos], b = sub + ahead_it * kFewTeam;
+            const size_t r0 = (size_t)e * a.ff + ahead.row;
+            const int second = GATED ? g : g + 8;
+            const bool va = g < ahead.here && b < blocks_in, vb = second < ahead.here && b < blocks_in;
             const size_t s0 = (size_t)e * scale_rows;
-            p.sa = va ? __ldg(a.s0 + (s0 + (ahead.row + g) / 128) * scale_cols + b) : 0.f;
-            p.sb = vb ? __ldg((GATED ? a.s1 : a.s0) + (s0 + (ahead.row + second) / 128) * scale_cols + b) : 0.f;
+            few_ask<FP8>(queue + ask_at * place, a.w0 + (r0 + g) * a.ld_in, va, (GATED ? a.w1 : a.w0) + (r0 + second) * a.ld_in, vb, b * 128 + t4 * 16, a.bytes_in,
+                         a.s0 + (s0 + (ahead.row + g) / 128) * scale_cols + b, (GATED ? a.s1 : a.s0) + (s0 + (ahead.row + second) / 128) * scale_cols + b, a.w0);
+            if (++ahead_it == iters) {
+                ahead_it = 0, advance(ahead);
+                if (ahead.left <= 0) {
+                    // the last weights of this launch are on their way: the first of the next one's are asked into L2 behind them
+                    const int d0 = (int)((long long)a.dim * blockIdx.x / gridDim.x), d1 = (int)((long long)a.dim * (blockIdx.x + 1) / gridDim.x);
+                    const int bytes = (d1 - d0) * a.ld_out, experts = bytes > 0 ? min(*lists.count, a.prefetch / bytes) : 0;
+                    for (int q = team * kFewTeam + sub + lane * kFewWarps; q < experts; q += 32 * kFewWarps)
+                        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a.w2 + ((size_t)lists.active[q] * a.dim + d0) * a.ld_out), "r"(bytes) : "memory");
+                }
+            }
         }
-        if (++ahead_it == iters) ahead_it = 0, advance(ahead);
+        few_commit();  // an empty group where nothing is left: the count of groups stays that of the places
+        if (++ask_at == at.depth) ask_at = 0;
     };
     float acc[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-    int it = 0;
-    float largest[NT > 2 ? 2 : 1] = {};
-    float *team_red = red + team * kFewTeam * 16 * NT * 8;
-    auto report = [&](int pos) {  // the run's share of this expert ends
-        const int i = sub * 32 + lane;
-        if constexpr (FP8) {
+    int it = 0, turn = 0;
+    float largest[NT];  // e4m3: of this thread's column in every tile of eight
 #pragma unroll
-            for (int h = 0; h < (NT > 2 ? 2 : 1); ++h) {
-                const int col = (i >> 3) + 16 * h;
-                if ((i & 7) == 0 && col < NT * 8) a.most[(size_t)(run + pos) * 32 + col] = largest[h];
-                largest[h] = 0.f;
-            }
-        }
-    };
-    auto finish = [&] {  // the tile's sums over the team's warps, the activation, the inner rows
-        float *mine = team_red + sub * 16 * NT * 8;
+    for (int n = 0; n < NT; ++n) largest[n] = 0.f;
+    const int i128 = sub * 32 + lane, f8 = i128 & 7, col8 = i128 >> 3 & 7;  // the first 64 threads of a team finish a feature (two without a gate) of a column each
+    auto finish = [&](int columns) {  // the tile's sums over the team's warps, the activation, the inner rows
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            *reinterpret_cast<float2 *>(mine + g * NT * 8 + n * 8 + 2 * t4) = make_float2(acc[n][0], acc[n][1]);
-            *reinterpret_cast<float2 *>(mine + (g + 8) * NT * 8 + n * 8 + 2 * t4) = make_float2(acc[n][2], acc[n][3]);
+            if (n * 8 >= columns) break;
+            float *sums = reinterpret_cast<float *>(few_smem + at.red) + ((turn ^= 1) * kFewTeams + team) * kFewTeam * 128, *mine = sums + sub * 128;
+            *reinterpret_cast<float2 *>(mine + g * 8 + 2 * t4) = make_float2(acc[n][0], acc[n][1]);
+            *reinterpret_cast<float2 *>(mine + (g + 8) * 8 + 2 * t4) = make_float2(acc[n][2], acc[n][3]);
             acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-        }
-        asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(kFewTeam * 32) : "memory");
-        const int i = sub * 32 + lane;
+            // one barrier for each use of either place: a place is written again only behind the other's
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(kFewTeam * 32) : "memory");
+            if (i128 < 64) {
+                const int col = n * 8 + col8;
+                float y_most = 0.f;
+                if (col < columns) {
+                    const int c = lists.column[tile.pos * 32 + col], t = c >> 8;
+                    float v[2] = {};
 #pragma unroll
-        for (int h = 0; h < (NT > 2 ? 2 : 1); ++h) {
-            const int f = i & 7, col = (i >> 3) + 16 * h;
-            if (col < NT * 8) {
-                const int c = lists.choice[tile.pos * 32 + col];
-                float v[2] = {};
-                for (int w = 0; w < kFewTeam; ++w) v[0] += team_red[w * 16 * NT * 8 + f * NT * 8 + col], v[1] += team_red[w * 16 * NT * 8 + (f + 8) * NT * 8 + col];
-                if constexpr (FP8) v[0] *= times[col], v[1] *= times[col];
-                float most = 0.f;
-                if (c) {
-                    float *to = a.inner + ((size_t)col * a.top + c - 1) * a.ld_inner + tile.row;
+                    for (int w = 0; w < kFewTeam; ++w) v[0] += sums[w * 128 + f8 * 8 + col8], v[1] += sums[w * 128 + (f8 + 8) * 8 + col8];
+                    if constexpr (FP8) {
+                        const float up = few_exp2(few_exponent(__uint_as_float(most[t] << 16)));
+                        v[0] *= up, v[1] *= up;
+                    }
+                    float *to = a.inner + ((size_t)t * a.top + (c & 255)) * a.ld_inner + tile.row;
                     if constexpr (GATED) {
-                        if (f < tile.here) {
+                        if (f8 < tile.here) {
                             const float y = gated_pair(v[0], v[1], a.act, a.limit, a.slope);
-                            to[f] = y, most = fabsf(y);
+                            to[f8] = y, y_most = fabsf(y);
                         }
                     } else {
 #pragma unroll
                         for (int u = 0; u < 2; ++u)
-                            if (f + 8 * u < tile.here) {
+                            if (f8 + 8 * u < tile.here) {
                                 const float y = a.act == 2 ? (v[u] > 0.f ? v[u] * v[u] : v[u] == v[u] ? 0.f : v[u]) : act_apply(v[u], a.act);
-                                to[f + 8 * u] = y, most = most < fabsf(y) || y != y ? fabsf(y) : most;
+                                to[f8 + 8 * u] = y, y_most = fmaxf(y_most, fabsf(y));
                             }
                     }
                     if (tile.row + tile.here == a.ff)
-                        for (int z = a.ff + f; z < a.ld_inner; z += 8) to[z - tile.row] = 0.f;
+                        for (int z = a.ff + f8; z < a.ld_inner; z += 8) to[z - tile.row] = 0.f;
                 }
                 if constexpr (FP8) {
 #pragma unroll
-                    for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                    largest[h] = fmaxf(largest[h], most);
+                    for (int o = 1; o < 8; o <<= 1) y_most = fmaxf(y_most, __shfl_xor_sync(0xffffffffu, y_most, o));
+                    largest[n] = fmaxf(largest[n], y_most);
                 }
             }
         }
         const int pos = tile.pos;
         advance(tile);
-        if (tile.left <= 0 || tile.pos != pos) report(pos);
-        asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(kFewTeam * 32) : "memory");
-    };
-    auto consume = [&](FewPiece &p) -> bool {
-        if (tile.left <= 0) return false;
-        const int b = sub + it * kFewTeam;
-        if (b < blocks_in) {
-            float d[NT][4];
-            if constexpr (FP8) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.f;
-            }
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
+        if constexpr (FP8) {
+            if (tile.left <= 0 || tile.pos != pos) {  // the run's share of this expert ends
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const unsigned char *row = few_smem + (n * 8 + g) * stride;
-                    if constexpr (FP8) {
-                        const uint4 u = *reinterpret_cast<const uint4 *>(row + b * 256 + c * 128 + t4 * 32), v = *reinterpret_cast<const uint4 *>(row + b * 256 + c * 128 + t4 * 32 + 16);
-                        const uint32_t x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-                        few_half<true>(p.a[c], p.b[c], x, d[n]);
-                    } else {
-                        const uint4 u = *reinterpret_cast<const uint4 *>(row + b * 128 + c * 64 + t4 * 16);
-                        const uint32_t x[4] = {u.x, u.y, u.z, u.w};
-                        few_half<false>(p.a[c], p.b[c], x, acc[n]);
-                    }
-                }
-            if constexpr (FP8) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    acc[n][0] = fmaf(d[n][0], p.sa, acc[n][0]), acc[n][1] = fmaf(d[n][1], p.sa, acc[n][1]);
-                    acc[n][2] = fmaf(d[n][2], p.sb, acc[n][2]), acc[n][3] = fmaf(d[n][3], p.sb, acc[n][3]);
+                    if (i128 < 64 && f8 == 0) a.most[(size_t)(run + pos) * 32 + n * 8 + col8] = largest[n];
+                    largest[n] = 0.f;
                 }
             }
         }
-        issue(p);
-        if (++it == iters) it = 0, finish();
-        return true;
     };
-    FewPiece p0, p1, p2;
-    issue(p0), issue(p1), issue(p2);
-    while (consume(p0) && consume(p1) && consume(p2)) {}
-    tl::griddep_launch();
+    for (int i = 0; i < at.depth; ++i) issue();
+    while (tile.left > 0) {
+        const int columns = __popc(lists.tokens[tile.pos]);
+        int row[NT];  // this lane's columns' rows; past the last column the first token's, not used
+#pragma unroll
+        for (int n = 0; n < NT; ++n) row[n] = n * 8 + g < columns ? (lists.column[tile.pos * 32 + n * 8 + g] >> 8) * stride : 0;
+        for (it = 0; it < iters; ++it) {
+            few_wait(at.depth);
+            const FewPiece p = few_take<FP8>(few_smem + at.queue + take_at * place);
+            if (++take_at == at.depth) take_at = 0;
+            const int b = sub + it * kFewTeam;
+            if (b < blocks_in) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    if (n * 8 >= columns) break;
+                    float d[4] = {};
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        if constexpr (FP8) {
+                            const unsigned char *from = few_smem + row[n] + b * 256 + c * 128 + t4 * 32;
+                            const uint4 u = *reinterpret_cast<const uint4 *>(from), v = *reinterpret_cast<const uint4 *>(from + 16);
+                            const uint32_t x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+                            few_half<true>(p.a[c], p.b[c], x, d);
+                        } else {
+                            const uint4 u = *reinterpret_cast<const uint4 *>(few_smem + row[n] + b * 128 + c * 64 + t4 * 16);
+                            const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+                            few_half<false>(p.a[c], p.b[c], x, acc[n]);
+                        }
+                    }
+                    if constexpr (FP8) {
+                        acc[n][0] = fmaf(d[0], p.sa, acc[n][0]), acc[n][1] = fmaf(d[1], p.sa, acc[n][1]);
+                        acc[n][2] = fmaf(d[2], p.sb, acc[n][2]), acc[n][3] = fmaf(d[3], p.sb, acc[n][3]);
+                    }
+                }
+            }
+            issue();
+        }
+        finish(columns);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // ---- second launch ---------------------------------------------------------------------------------------------------
 
 struct FewSecondSmem {
-    int red, idx, factor, times, active, choice, place, flags, total;
-    __host__ __device__ FewSecondSmem(int tokens, int nt, int experts, int top) {
-        red = 0;
-        idx = red + kFewWarps * 16 * nt * 8 * 4;
+    int sums, idx, factor, times, queue, depth, total;
+    FewListsSmem lists;
+    __host__ __device__ FewSecondSmem(int tokens, int experts, int top, bool fp8, int room) : lists(0, tokens, top, experts) {
+        sums = 0;
+        idx = sums + kFewWarps * few_sum_stride(tokens) * 4;
         factor = idx + tokens * top * 4;
         times = factor + tokens * top * 4;
-        active = times + tokens * top * 4;
-        const int most = tokens * top < experts ? tokens * top : experts;
-        choice = active + (most * 4 + 15) / 16 * 16;
-        place = choice + most * 32;
-        flags = (place + experts * 2 + 15) / 16 * 16;
-        total = flags + 16;
+        lists = FewListsSmem(times + tokens * top * 4, tokens, top, experts);
+        queue = lists.end;
+        depth = (room - queue) / few_place(fp8);
+        if (depth > kFewDepth) depth = kFewDepth;
+        total = queue + depth * few_place(fp8);
     }
+    // a warp's sums, [token][17] (16 rows, and one place that keeps the tokens' from falling into the same banks)
+    static __host__ __device__ int few_sum_stride(int tokens) { return (tokens * 17 + 3) / 4 * 4; }
 };
 
 template <bool FP8, int NT, typename OUT>
 __global__ void __launch_bounds__(kFewThreads, 1)
 moe_few_second_kernel(const FewArgs a) {
     extern __shared__ __align__(128) unsigned char few_smem[];
-    const FewSecondSmem at(a.tokens, NT, a.experts, a.top);
+    const FewSecondSmem at(a.tokens, a.experts, a.top, FP8, a.room);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
-    float *red = reinterpret_cast<float *>(few_smem + at.red), *factor = reinterpret_cast<float *>(few_smem + at.factor), *times = reinterpret_cast<float *>(few_smem + at.times);
-    int *idx = reinterpret_cast<int *>(few_smem + at.idx), *count = reinterpret_cast<int *>(few_smem + at.flags);
-    const FewLists lists{reinterpret_cast<int *>(few_smem + at.active), few_smem + at.choice, count};
+    const int sum_stride = FewSecondSmem::few_sum_stride(a.tokens);
+    float *sums = reinterpret_cast<float *>(few_smem + at.sums) + warp * sum_stride, *factor = reinterpret_cast<float *>(few_smem + at.factor);
+    float *times = reinterpret_cast<float *>(few_smem + at.times);
+    int *idx = reinterpret_cast<int *>(few_smem + at.idx);
+    const FewLists lists = at.lists.lists(few_smem);
+    at.lists.clear(few_smem);
+    for (int i = lane; i < sum_stride; i += 32) sums[i] = 0.f;
     tl::griddep_wait();
     tl::griddep_launch();
-    for (int p = tid; p < a.tokens * a.top; p += kFewThreads) idx[p] = tl::ld_cg(a.idx + p), factor[p] = tl::ld_cg(a.gate + p);
+    const int pairs = a.tokens * a.top;
+    if (tid < pairs) idx[tid] = tl::ld_cg(a.idx + tid), factor[tid] = tl::ld_cg(a.gate + tid);
     __syncthreads();
-    short *place = reinterpret_cast<short *>(few_smem + at.place);
-    few_lists(a, idx, place, lists);
-    const int total = *count * a.ff;
-    if constexpr (FP8) {  // an inner row's power of two, from what every run of its features left
-        for (int p = warp; p < a.tokens * a.top; p += kFewWarps) {
-            const int t = p / a.top, e = idx[p];
-            if (e >= a.experts) continue;
-            const int pos = place[e], f0 = pos * a.ff, v0 = few_run_of(total, a.runs, f0), v1 = few_run_of(total, a.runs, f0 + a.ff - 1);
-            float most = 0.f;
-            for (int v = v0 + lane; v <= v1; v += 32) {
-                const float m = tl::ld_cg(a.most + (size_t)(v + pos) * 32 + t);
-                most = most < m ? m : most;
-            }
-            const int x = few_exponent(warp_max(most));
-            if (lane == 0) times[p] = few_exp2(-x), factor[p] *= few_exp2(x);
-        }
-        __syncthreads();
-    }
+    const int my_pos = few_lists(a, idx, lists), count = *lists.count, total = count * a.ff;
 
     const int col0 = (int)((long long)a.dim * blockIdx.x / gridDim.x), col1 = (int)((long long)a.dim * (blockIdx.x + 1) / gridDim.x);
     const int blocks_out = (a.bytes_out + 127) / 128, scale_cols = (a.ff + 127) / 128, scale_rows = (a.dim + 127) / 128;
+    const uint32_t queue = static_cast<uint32_t>(__cvta_generic_to_shared(few_smem + at.queue));
+    const int place = few_place(FP8);
     for (int c0 = col0; c0 < col1; c0 += 16) {
         const int here = min(16, col1 - c0);
-        float acc[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
         // an expert's block b goes to warp (expert * blocks + b) % 16, whichever experts are chosen beside it
         struct Step {
             int pos, b;
         };
         auto enter = [&](Step &s) {
-            while (s.pos < *count) {
+            while (s.pos < count) {
                 s.b = (warp - lists.active[s.pos] * blocks_out) & (kFewWarps - 1);
                 if (s.b < blocks_out) return;
                 ++s.pos;
@@ -531,102 +608,134 @@ moe_few_second_kernel(const FewArgs a) {
         };
         Step now{0, 0}, ahead{0, 0};
         enter(now), enter(ahead);
-        auto issue = [&](FewPiece &p) {
-            if (ahead.pos >= *count) return;
-            const int e = lists.active[ahead.pos];
-            const uint8_t *row = a.w2 + ((size_t)e * a.dim + c0 + g) * a.ld_out;
-            const bool va = g < here, vb = g + 8 < here;
-            few_load<FP8>(p, va ? row : nullptr, vb ? row + (size_t)8 * a.ld_out : nullptr, ahead.b * 128 + t4 * 16, a.bytes_out);
-            if constexpr (FP8) {
+        int ask_at = 0, take_at = 0;
+        auto issue = [&] {
+            if (ahead.pos < count) {
+                const int e = lists.active[ahead.pos];
+                const uint8_t *row = a.w2 + ((size_t)e * a.dim + c0 + g) * a.ld_out;
                 const size_t s0 = (size_t)e * scale_rows;
-                p.sa = va ? __ldg(a.s2 + (s0 + (c0 + g) / 128) * scale_cols + ahead.b) : 0.f;
-                p.sb = vb ? __ldg(a.s2 + (s0 + (c0 + g + 8) / 128) * scale_cols + ahead.b) : 0.f;
+                few_ask<FP8>(queue + ask_at * place, row, g < here, row + (size_t)8 * a.ld_out, g + 8 < here, ahead.b * 128 + t4 * 16, a.bytes_out,
+                             a.s2 + (s0 + (c0 + g) / 128) * scale_cols + ahead.b, a.s2 + (s0 + (c0 + g + 8) / 128) * scale_cols + ahead.b, a.w2);
+                next(ahead);
             }
-            next(ahead);
+            few_commit();
+            if (++ask_at == at.depth) ask_at = 0;
         };
-        auto consume = [&](FewPiece &p) -> bool {
-            if (now.pos >= *count) return false;
-            const uint8_t *choice = lists.choice + now.pos * 32;
+        for (int i = 0; i < at.depth; ++i) issue();
+        if constexpr (FP8) {
+            if (c0 == col0) {  // an inner row's power of two, from what every run of its features left; the first weights are on their way
+                int *held = reinterpret_cast<int *>(times);  // for the warps that look: the position of every pair's expert
+                if (tid < pairs) held[tid] = my_pos;
+                __syncthreads();
+                for (int p = warp; p < pairs; p += kFewWarps) {
+                    const int pos = held[p], t = p / a.top;
+                    if (pos < 0) continue;
+                    const int f0 = pos * a.ff, v0 = few_run_of(total, a.runs, f0), v1 = few_run_of(total, a.runs, f0 + a.ff - 1);
+                    const int col = __popc(lists.tokens[pos] & ((1u << t) - 1));
+                    float most = 0.f;
+                    for (int v = v0 + lane; v <= v1; v += 32) most = fmaxf(most, tl::ld_cg(a.most + (size_t)(v + pos) * 32 + col));
+                    const int x = few_exponent(warp_max(most));
+                    if (lane == 0) times[p] = few_exp2(-x), factor[p] *= few_exp2(x);
+                }
+                __syncthreads();
+            }
+        }
+        constexpr int ENTRIES = FP8 ? 16 : 8;  // of either half of a block, a lane's
+        float h[2][ENTRIES];
+        auto fetch = [&](const Step &s, int n) {  // a column's inner numbers; of a column that is not there: zeros
+            const bool mine = n * 8 + g < __popc(lists.tokens[s.pos]);
+            const int c = mine ? lists.column[s.pos * 32 + n * 8 + g] : 0;
+            const float *row = a.inner + ((size_t)(c >> 8) * a.top + (c & 255)) * a.ld_inner;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int k = s.b * 8 * ENTRIES + u * 4 * ENTRIES + t4 * ENTRIES;
+#pragma unroll
+                for (int i = 0; i < ENTRIES; i += 4) {
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (mine && k < a.ld_inner) v = tl::ld_cg(reinterpret_cast<const uint4 *>(row + k + i));
+                    h[u][i] = __uint_as_float(v.x), h[u][i + 1] = __uint_as_float(v.y), h[u][i + 2] = __uint_as_float(v.z), h[u][i + 3] = __uint_as_float(v.w);
+                }
+            }
+        };
+        if (now.pos < count) fetch(now, 0);
+        while (now.pos < count) {
+            few_wait(at.depth);
+            const FewPiece p = few_take<FP8>(few_smem + at.queue + take_at * place);
+            if (++take_at == at.depth) take_at = 0;
+            const int columns = __popc(lists.tokens[now.pos]);
+            const uint16_t *column = lists.column + now.pos * 32;
+            Step later = now;
+            next(later);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const int mine = n * 8 + g < a.tokens ? choice[n * 8 + g] : 0;
-                if (NT > 1 && !__any_sync(0xffffffffu, mine)) continue;
-                const int pair = (n * 8 + g) * a.top + mine - 1;
-                const float *row = a.inner + (size_t)(mine ? pair : 0) * a.ld_inner;
-                const float down = FP8 && mine ? times[pair] : 1.f;
+                if (n * 8 >= columns) break;
+                if (n > 0) fetch(now, n);
+                constexpr int TERMS = FP8 ? 1 : 2, WORDS = FP8 ? 8 : 4;
+                uint32_t x[2][TERMS][WORDS];
+                float down = 1.f;
+                if constexpr (FP8) {
+                    const int c = n * 8 + g < columns ? column[n * 8 + g] : column[0];
+                    down = times[(c >> 8) * a.top + (c & 255)];
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < WORDS; ++i) {
+                        const float lo = h[u][2 * i], hi = h[u][2 * i + 1];
+                        if constexpr (FP8) {
+                            x[u][0][i] = few_half2(lo * down, hi * down);
+                        } else {
+                            x[u][0][i] = tl::pack2<bf16>(lo, hi);
+                            const float2 f = tl::unpack2<bf16>(x[u][0][i]);
+                            // an infinity has no second term
+                            x[u][1][i] = tl::pack2<bf16>(fabsf(f.x) < INFINITY ? lo - f.x : 0.f, fabsf(f.y) < INFINITY ? hi - f.y : 0.f);
+                        }
+                    }
+                if (n == 0 && columns <= 8 && later.pos < count) fetch(later, 0);  // on its way under the products
                 float d[4] = {};
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    constexpr int ENTRIES = FP8 ? 16 : 8;
-                    const int k = now.b * (FP8 ? 128 : 64) + c * (FP8 ? 64 : 32) + t4 * ENTRIES;
-                    float h[ENTRIES] = {};
-                    if (mine && k < a.ld_inner) {
+                for (int u = 0; u < 2; ++u)
 #pragma unroll
-                        for (int i = 0; i < ENTRIES; i += 4) {
-                            const uint4 u = tl::ld_cg(reinterpret_cast<const uint4 *>(row + k + i));
-                            h[i] = __uint_as_float(u.x), h[i + 1] = __uint_as_float(u.y), h[i + 2] = __uint_as_float(u.z), h[i + 3] = __uint_as_float(u.w);
-                        }
-                    }
-                    if constexpr (FP8) {
-                        uint32_t x[8];
+                    for (int term = 0; term < TERMS; ++term) few_half<FP8>(p.a[u], p.b[u], x[u][term], d);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) x[i] = few_half2(h[2 * i] * down, h[2 * i + 1] * down);
-                        few_half<true>(p.a[c], p.b[c], x, d);
-                    } else {
-                        uint32_t x[4], low[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            x[i] = tl::pack2<bf16>(h[2 * i], h[2 * i + 1]);
-                            const float2 f = tl::unpack2<bf16>(x[i]);
-                            // an infinity has no second term
-                            low[i] = tl::pack2<bf16>(fabsf(f.x) < INFINITY ? h[2 * i] - f.x : 0.f, fabsf(f.y) < INFINITY ? h[2 * i + 1] - f.y : 0.f);
-                        }
-                        few_half<false>(p.a[c], p.b[c], x, d);
-                        few_half<false>(p.a[c], p.b[c], low, d);
-                    }
-                }
-                // a token that did not choose this expert gets nothing of it, not even a product with zero
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int t = n * 8 + 2 * t4 + u, k = t < a.tokens ? choice[t] : 0;
-                    if (k) {
-                        const float f = factor[t * a.top + k - 1];
-                        acc[n][u] = fmaf(d[u], FP8 ? f * p.sa : f, acc[n][u]);
-                        acc[n][2 + u] = fmaf(d[2 + u], FP8 ? f * p.sb : f, acc[n][2 + u]);
+                for (int v = 0; v < 2; ++v) {
+                    const int col = n * 8 + 2 * t4 + v;
+                    if (col < columns) {
+                        const int t = column[col] >> 8;
+                        const float f = factor[t * a.top + (column[col] & 255)];
+                        float *to = sums + t * 17 + g;
+                        to[0] = fmaf(d[v], FP8 ? f * p.sa : f, to[0]), to[8] = fmaf(d[2 + v], FP8 ? f * p.sb : f, to[8]);
                     }
                 }
             }
-            next(now);
-            issue(p);
-            return true;
-        };
-        FewPiece p0, p1, p2;
-        issue(p0), issue(p1), issue(p2);
-        while (consume(p0) && consume(p1) && consume(p2)) {}
-
-        __syncthreads();  // the sums of the columns before
-        float *mine = red + warp * 16 * NT * 8;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            *reinterpret_cast<float2 *>(mine + g * NT * 8 + n * 8 + 2 * t4) = make_float2(acc[n][0], acc[n][1]);
-            *reinterpret_cast<float2 *>(mine + (g + 8) * NT * 8 + n * 8 + 2 * t4) = make_float2(acc[n][2], acc[n][3]);
+            __syncwarp();  // the next expert's column of a token may be another lane's
+            if (columns > 8 && later.pos < count) fetch(later, 0);
+            now = later;
+            issue();
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         __syncthreads();
-        for (int i = tid; i < 16 * NT * 8; i += kFewThreads) {
+        const float *all = reinterpret_cast<const float *>(few_smem + at.sums);
+        for (int i = tid; i < 16 * a.tokens; i += kFewThreads) {
             const int r = i % 16, t = i / 16;
-            if (r >= here || t >= a.tokens) continue;
+            if (r >= here) continue;
             float y = 0.f;
 #pragma unroll
-            for (int w = 0; w < kFewWarps; ++w) y += red[w * 16 * NT * 8 + r * NT * 8 + t];
+            for (int w = 0; w < kFewWarps; ++w) y += all[w * sum_stride + t * 17 + r];
             const int d = c0 + r;
             for (int k = 0; k < a.top; ++k) {
                 const int e = idx[t * a.top + k];
                 if (e < a.experts) continue;
                 // an identity expert; no output at all: the token's logits are no numbers
-                y = e < a.outputs ? fmaf(factor[t * a.top + k], to_f(a.x[(size_t)t * a.dim + d]), y) : __int_as_float(0x7fffffff);
+                y = e < a.outputs ? fmaf(factor[t * a.top + k], to_f(tl::ld_cg(a.x + (size_t)t * a.dim + d)), y) : __int_as_float(0x7fffffff);
             }
             if (a.shared) y = fmaf(a.side_w ? tl::ld_cg(a.side + t) : 1.f, to_f(tl::ld_cg(a.shared + (size_t)t * a.dim + d)), y);
             static_cast<OUT *>(a.out)[(size_t)t * a.dim + d] = from_f<OUT>(y);
+        }
+        if (c0 + 16 < col1) {
+            __syncthreads();
+            for (int i = lane; i < sum_stride; i += 32) sums[i] = 0.f;
+            __syncwarp();
         }
     }
 }
@@ -635,12 +744,15 @@ moe_few_second_kernel(const FewArgs a) {
 
 constexpr int kFewSmem = 227 * 1024;
 
-// CTAs of a cluster, and how many clusters of the first launch are resident at once.
-constexpr int kFewCluster = 4;
+// CTAs of the first launch: whole clusters (with clusters of four 132 CTAs are resident at once, with two all 148).
 static int few_grid() {
     const int sms = sm_count();
     return sms / kFewCluster * kFewCluster;
 }
+
+// Two places of the queue at least: a piece on its way while one is used.
+static bool few_fits(const FewFirstSmem &s) { return s.depth >= 2 && s.total <= kFewSmem; }
+constexpr int kFewPrefetch = 40 << 20;  // a third of L2
 
 static int few_inner_ld(int ff) { return (ff + 15) / 16 * 16; }
 static int few_nt(int tokens) { return tokens <= 8 ? 1 : tokens <= 16 ? 2 : 4; }
@@ -679,7 +791,7 @@ static int few_run(const FewArgs &a, int first_smem, bool wide, cudaStream_t st)
     int e = a.w1 ? few_launch(moe_few_first_kernel<FP8, true, NT>, gated, dim3(grid), kFewCluster, first_smem, st, a)
                  : few_launch(moe_few_first_kernel<FP8, false, NT>, plain, dim3(grid), kFewCluster, first_smem, st, a);
     if (e) return e;
-    const int smem = FewSecondSmem(a.tokens, NT, a.experts, a.top).total;
+    const int smem = FewSecondSmem(a.tokens, a.experts, a.top, FP8, kFewSmem).total;
     const dim3 cols(std::min(sm_count(), a.dim));
     return wide ? few_launch(moe_few_second_kernel<FP8, NT, float>, second32, cols, 1, smem, st, a)
                 : few_launch(moe_few_second_kernel<FP8, NT, bf16>, second16, cols, 1, smem, st, a);
@@ -694,7 +806,7 @@ extern "C" {
 int tlb_moe_few_tokens(int dim, int outputs, int experts, int top, int group_count, int fp8) {
     if (dim <= 0 || outputs <= 0 || outputs > kFewOutputs || experts <= 0 || experts > outputs || top <= 0 || top > outputs || top > 255 || group_count < 0) return 0;
     int tokens = std::min(kFewTokens, kFewPairs / top);
-    while (tokens > 0 && FewFirstSmem(tokens, few_nt(tokens), dim, outputs, experts, top, group_count, fp8 != 0).total > kFewSmem) --tokens;
+    while (tokens > 0 && !few_fits(FewFirstSmem(tokens, few_nt(tokens), dim, outputs, experts, top, group_count, fp8 != 0, kFewSmem))) --tokens;
     return tokens;
 }
 
@@ -732,8 +844,9 @@ int tlb_moe_few(const void *x, const void *router, const void *router_bias, cons
     a.gate = (float *)at, at += few_align(pairs * 4);
     a.side = (float *)at, at += few_align((size_t)tokens * 4);
     a.inner = (float *)at, a.ld_inner = few_inner_ld(ff), at += pairs * a.ld_inner * 4;
-    a.most = (float *)at, a.runs = few_grid() * kFewTeams;
-    const int nt = few_nt(tokens), smem = FewFirstSmem(tokens, nt, dim, outputs, experts, top, group_count, fp8 != 0).total;
+    a.most = (float *)at, a.runs = few_grid() * kFewTeams, a.room = kFewSmem;
+    a.prefetch = kFewPrefetch / few_grid();
+    const int nt = few_nt(tokens), smem = FewFirstSmem(tokens, nt, dim, outputs, experts, top, group_count, fp8 != 0, kFewSmem).total;
     const cudaStream_t st = as_stream(stream);
     if (fp8) return nt == 1 ? few_run<true, 1>(a, smem, out_f32, st) : nt == 2 ? few_run<true, 2>(a, smem, out_f32, st) : few_run<true, 4>(a, smem, out_f32, st);
     return nt == 1 ? few_run<false, 1>(a, smem, out_f32, st) : nt == 2 ? few_run<false, 2>(a, smem, out_f32, st) : few_run<false, 4>(a, smem, out_f32, st);
