@@ -78,3 +78,50 @@ def test_linear(rows, n, k, dtype):
 def test_linear_of_real_sizes(rows, n, k):
     x, w, bias = make(rows, n, k, torch.bfloat16)
     check_linear(x, w, bias, fp8_linear(x, w, bias))
+
+
+def check_mlp(x, gate, up, down, act, got, limit=0.0, slope=1.0):
+    """The inner rows are rounded by the operator from its own fp32 sums: an entry next to a border may be rounded the other way, which is one step of its
+    run's scale.  So the second product's tolerance counts one step for each inner number that lies within the first product's tolerance of a border."""
+    plain = lambda w: w.values[:, : w.shape[1]].float().double().cpu() * w.scales.double().cpu().repeat_interleave(BLOCK, 0)[: w.shape[0]].repeat_interleave(BLOCK, 1)[:, : w.shape[1]]  # noqa: E731
+    xq, wg, wu, wd = rounded_rows(x), plain(gate), plain(up), plain(down)
+    g, u = xq @ wg.t(), xq @ wu.t()
+    blocks = -(-xq.shape[1] // BLOCK)
+    sums = (2 * BLOCK + 3 * blocks + 4) * 2.0**-24
+    dg, du = sums * (xq.abs() @ wg.abs().t()), sums * (xq.abs() @ wu.abs().t())
+    if act == "clamped_swish":
+        gc, uc = g.clamp(max=limit), u.clamp(-limit, limit) + 1
+        inner, di = gc * torch.sigmoid(slope * gc) * uc, 1.1 * max(1.0, slope) * dg * uc.abs() + (gc * torch.sigmoid(slope * gc)).abs() * du
+    else:
+        f = torch.nn.functional.silu if act == "silu" else lambda v: torch.nn.functional.gelu(v, approximate="tanh")
+        inner, di = f(g) * u, 1.2 * dg * u.abs() + f(g).abs() * du + (8 * 2.0**-24 * g.abs() * u.abs() if act == "gelu_tanh" else 0)
+    di = di + 40 * 2.0**-24 * inner.abs()
+    low, high, near = torch.empty_like(inner), torch.empty_like(inner), torch.empty_like(inner)
+    for k in range(0, inner.shape[1], BLOCK):
+        part, d = inner[:, k : k + BLOCK], di[:, k : k + BLOCK]
+        most = part.abs().amax(dim=1, keepdim=True).clamp_min(2.0**-100)
+        off = (d.amax(dim=1, keepdim=True) / most).clamp_max(1.0) + 4 * 2.0**-24  # the scale's own
+        v, dv = part * (448.0 / most), d * (448.0 / most) + 2 * off * part.abs() * (448.0 / most)
+        s = most / 448.0
+        near[:, k : k + BLOCK] = nearest_e4m3(v) * s
+        low[:, k : k + BLOCK], high[:, k : k + BLOCK] = nearest_e4m3(v - dv) * s, nearest_e4m3(v + dv) * s
+        spread = off * nearest_e4m3(v).abs() * s
+        low[:, k : k + BLOCK] -= spread
+        high[:, k : k + BLOCK] += spread
+    want = near @ wd.t()
+    tol = torch.maximum(high - near, near - low) @ wd.abs().t() + product_tolerance(near, wd, want, x.dtype)
+    tol = tol + torch.finfo(x.dtype).eps / 2 * tol
+    off = (got.double().cpu() - want).abs()
+    assert got.dtype == x.dtype and got.shape == want.shape
+    assert bool((off <= tol).all()), f"worst {(off / tol).max().item():.2f} times the tolerance"
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 5, 16, 17, 70, 128, 129, 300])
+@pytest.mark.parametrize("dim,ff,act", [(16, 1, "silu"), (128, 128, "silu"), (200, 129, "clamped_swish"), (333, 700, "gelu_tanh"), (640, 1400, "silu")])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gated_mlp(rows, dim, ff, act, dtype):
+    x, gate, _ = make(rows, ff, dim, dtype, seed=1)
+    up, down = make(1, ff, dim, dtype, seed=2)[1], make(1, dim, ff, dtype, seed=3)[1]
+    layer = Fp8GatedMLP(gate, up, down, act, limit=1.5 if act == "clamped_swish" else 0.0, slope=1.7 if act == "clamped_swish" else 1.0)
+    check_mlp(x, gate, up, down, act, layer(x), 1.5, 1.7 if act == "clamped_swish" else 1.0)

@@ -63,7 +63,11 @@ struct F8Product {
     int dtype;  // of bias and out
 };
 int f8_product(const F8Product &a, cudaStream_t st);
+// blocks_fp8_pairs.cu: the same for many rows, and, of 128 rows of a gate and 128 of an up projection in turn, the gated rows rounded to e4m3 (to.q, to.scales)
+int f8_pairs(const F8Product &a, cudaStream_t st);
+int f8_pairs_gated(const F8Product &a, const F8Rows &to, cudaStream_t st);
 long long f8_gave_up();
+long long f8_pairs_gave_up();
 
 static inline int f8_up(int n, int to) { return (n + to - 1) / to * to; }
 

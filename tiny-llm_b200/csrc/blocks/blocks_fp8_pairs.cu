@@ -1,0 +1,335 @@
+// Many rows of e4m3 numbers times a matrix of them, on pairs of CTAs (tcgen05.mma, cta_group::2, kind::f8f6f4).
+//
+// What is computed is blocks_fp8_product.cu's sum over blocks of 128.  A tile is 256 tokens by 256 rows of the matrix; either CTA of a pair loads its 128
+// tokens and half of the matrix rows, 32 KB for a block's 512 cycles of tensor work (one CTA by itself would load 48 KB: more than L2 hands an SM in that
+// time).  The tokens are the M side: a token's scale is a lane's and a block scale holds for 128 columns, so taking a block's accumulator over into
+// the sums is one multiply-add an entry, all with one factor.  Eight
+// warps do it, 128 columns each (16 warps with 64 took 30 % longer: the SM's issue slots went into what a warp does a block beside the multiply-adds; two multiply-adds an
+// instruction, fma.rn.f32x2, took longer than two).  Sums live in registers.  A block's accumulator is two halves of 128 columns, in two places each: what keeps the
+// tensor cores waiting is the way round from a finished accumulator to an empty one, and a half's is shorter and overlaps the other half's products.
+//
+// 12 warps: 0 and 3 TMA, 1 the products (leader) or the news that the own stage is there (peer), 4-11 the sums.  The first four give registers to the others.
+//
+// kGated: the matrix rows are 128 of a gate and the 128 of an up projection that belong to them; a thread then has both of 64 features of its token, and what
+// is stored are the gated rows, rounded to e4m3 with one scale for the 128, which two warps find together.
+#include <algorithm>
+
+#include "blocks_fp8.cuh"
+#include "blocks_tc.cuh"
+
+namespace tlb {
+
+constexpr int kPrSumWarps = 8;
+constexpr int kPrThreads = (4 + kPrSumWarps) * 32;
+constexpr int kPrStages = 6;
+constexpr int kPrStage = 2 * 128 * 128;
+constexpr int kPrOutStride = 68, kPrOut = 32 * kPrOutStride;  // a warp's staging rows: 64 bytes, and 4 that keep the lanes' words in different banks
+constexpr int kPrMost = 2 * 128 * 4;                          // kGated: the two warps' maxima of every token
+constexpr int kPrSmem = kPrStages * kPrStage + kPrSumWarps * kPrOut + kPrMost + 256;
+
+struct F8PairArgs {
+    const float *sx, *sw;
+    const void *bias;
+    void *out;
+    int ld_sx, rows, n, k_blocks, m_tiles, tiles;
+    bool aligned;  // rows of `out` are whole 32-byte pieces
+    // kGated
+    uint8_t *q;
+    float *scales;
+    int ldq, ld_scales, ff, act;
+    float limit, slope;
+};
+
+__device__ __forceinline__ uint32_t pr_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void pr_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
+    constexpr uint32_t idesc = (1u << 4) | ((256u >> 3) << 17) | ((256u >> 4) << 24);  // e4m3 x e4m3 -> f32, 256 x 256, both K-major
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+                 "r"(accumulate)
+                 : "memory");
+}
+// completion of all products so far: an arrival on the barrier at this offset in both CTAs
+__device__ __forceinline__ void pr_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(static_cast<unsigned short>(3)) : "memory");
+}
+__device__ __forceinline__ void pr_store32(void *p, const uint32_t (&v)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+
+template <typename T, bool GATED>
+__global__ void __launch_bounds__(kPrThreads, 1)
+fp8_pairs_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_w, const F8PairArgs a) {
+    extern __shared__ __align__(1024) unsigned char pr_smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)pr_rank();
+    const int unit = blockIdx.x >> 1, units = gridDim.x >> 1;
+    const uint32_t base = g_smem_u32(pr_smem);
+    constexpr int kBars = kPrStages * kPrStage + kPrSumWarps * kPrOut + kPrMost;
+    const uint32_t full = base + kBars, empty = full + 8 * kPrStages, acc_full = empty + 8 * kPrStages, acc_empty = acc_full + 16;
+    volatile int *dead = reinterpret_cast<volatile int *>(pr_smem + kBars + 16 * kPrStages + 32);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(const_cast<int *>(dead)) + 1;
+    if (warp == 1 && lane == 0) {
+        for (int i = 0; i < kPrStages; ++i) g_mbar_init(full + 8 * i, rank == 0 ? 3 : 2), g_mbar_init(empty + 8 * i, 1);  // both kinds of copies, and on the leader's the peer's word
+        for (int i = 0; i < 2; ++i) g_mbar_init(acc_full + 8 * i, 1), g_mbar_init(acc_empty + 8 * i, 2 * kPrSumWarps);  // both CTAs' warps, on the leader's
+        *dead = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(g_smem_u32(tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    g_tc_fence_before();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");  // both CTAs' barriers are ready
+    g_tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    auto arrive_leader = [&](uint32_t bar) {  // what it reports is in the arriving CTA's own memory, ordered there
+        asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, 0;\n\tmbarrier.arrive.shared::cluster.b64 _, [ra];\n\t}" ::"r"(bar) : "memory");
+    };
+    // Tiles of one band of matrix rows follow one another: the band stays in L2 while the tokens pass.
+    auto token0 = [&](int tile) { return tile % a.m_tiles * 256 + rank * 128; };
+    auto row0 = [&](int tile) { return tile / a.m_tiles * 256; };
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        // A thread by itself for each role: with the whole warp in the loop a block cost twice the cycles.
+        if (warp == 0 || warp == 3) {  // the matrix's copies and the rows': one thread gets a box of 16 KB under way in 380 cycles, two get two
+            if (g_elect_one()) {
+                int s = 0;
+                uint32_t ph = 1;
+                bool ok = true;
+                if (warp == 3) tl::griddep_wait();  // the matrix is older than the rows' launch, which may still be running
+                for (int tile = unit; ok && tile < a.tiles; tile += units)
+                    for (int kb = 0; kb < a.k_blocks; ++kb) {
+                        if (!(ok = tc_wait_one(empty + 8 * s, ph, dead))) break;
+                        g_mbar_expect_tx(full + 8 * s, kPrStage / 2);
+                        if (warp == 0) g_tma_load_2d(base + s * kPrStage + 128 * 128, &map_w, kb * 128, row0(tile) + rank * 128, full + 8 * s);
+                        else g_tma_load_2d(base + s * kPrStage, &map_q, kb * 128, token0(tile), full + 8 * s);
+                        if (++s == kPrStages) s = 0, ph ^= 1u;
+                    }
+            }
+        } else if (warp == 1 && rank == 0) {
+            if (g_elect_one()) {
+                int s = 0, buf = 0;
+                uint32_t ph = 0, acc_ph = 1;
+                bool ok = true;
+                for (int tile = unit; ok && tile < a.tiles; tile += units)
+                    for (int kb = 0; kb < a.k_blocks; ++kb) {
+                        if (!(ok = tc_wait_one(acc_empty + 8 * buf, acc_ph, dead) && tc_wait_one(full + 8 * s, ph, dead))) break;
+                        g_tc_fence_after();
+                        const uint64_t q = g_smem_desc_sw128(base + s * kPrStage, 0, 1024), w = g_smem_desc_sw128(base + s * kPrStage + 128 * 128, 0, 1024);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) pr_mma(tmem + buf * 256, q + 2 * k, w + 2 * k, k > 0);
+                        pr_commit(acc_full + 8 * buf);
+                        pr_commit(empty + 8 * s);
+                        if (++s == kPrStages) s = 0, ph ^= 1u;
+                        if (++buf == 2) buf = 0, acc_ph ^= 1u;
+                    }
+            }
+        } else if (warp == 1) {
+            if (g_elect_one()) {
+                int s = 0;
+                uint32_t ph = 0;
+                bool ok = true;
+                for (int tile = unit; ok && tile < a.tiles; tile += units)
+                    for (int kb = 0; kb < a.k_blocks; ++kb) {
+                        if (!(ok = tc_wait_one(full + 8 * s, ph, dead))) break;
+                        arrive_leader(full + 8 * s);
+                        if (++s == kPrStages) s = 0, ph ^= 1u;
+                    }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");  // 4 x 40 + 8 x 232 <= 12 x 168 a lane
+        // this warp's two runs of 64 matrix rows: the same of either block of 128 (a gate's and the up projection's of the same features)
+        const int quarter = warp & 3, half = (warp - 4) >> 2, row_a = half * 64, row_b = row_a + 128;
+        int buf = 0;
+        uint32_t acc_ph = 0;
+        tl::griddep_wait();
+        for (int tile = unit; tile < a.tiles; tile += units) {
+            const int t0 = token0(tile), r0 = row0(tile), t = t0 + quarter * 32 + lane;
+            float acc_a[64], acc_b[64];
+#pragma unroll
+            for (int i = 0; i < 64; ++i) acc_a[i] = acc_b[i] = 0.f;
+            // of tokens and matrix rows past the end: the last ones', for sums that are not stored
+            const float *sx = a.sx + min(t, a.rows - 1);
+            const int last = (a.n + 127) / 128 - 1;
+            const float *sw_a = a.sw + (size_t)min((r0 + row_a) >> 7, last) * a.k_blocks, *sw_b = a.sw + (size_t)min((r0 + row_b) >> 7, last) * a.k_blocks;
+            float next_x = tl::ld_cg(sx), next_a = __ldg(sw_a), next_b = __ldg(sw_b);
+            bool ok = true;
+            for (int kb = 0; kb < a.k_blocks; ++kb) {
+                const float fa = next_x * next_a, fb = next_x * next_b;
+                if (kb + 1 < a.k_blocks) {
+                    next_x = tl::ld_cg(sx + (size_t)(kb + 1) * a.ld_sx), next_a = __ldg(sw_a + kb + 1), next_b = __ldg(sw_b + kb + 1);
+                }
+                ok &= tc_wait(acc_full + 8 * buf, acc_ph, dead);
+                g_tc_fence_after();
+                const uint32_t at = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buf * 256 + row_a;
+                uint32_t v[2][32];  // two runs on their way, and again two as soon as their places are free: the accumulator is empty after half of the additions
+                tl::g_tmem_ld32_nowait(at, v[0]);
+                tl::g_tmem_ld32_nowait(at + 32, v[1]);
+                tl::g_tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) acc_a[i] = fmaf(__uint_as_float(v[0][i]), fa, acc_a[i]);
+                tl::g_tmem_ld32_nowait(at + 128, v[0]);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) acc_a[32 + i] = fmaf(__uint_as_float(v[1][i]), fa, acc_a[32 + i]);
+                tl::g_tmem_ld32_nowait(at + 160, v[1]);
+                tl::g_tmem_ld_wait();
+                g_tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (rank == 0) g_mbar_arrive(acc_empty + 8 * buf);
+                    else arrive_leader(acc_empty + 8 * buf);
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) acc_b[i] = fmaf(__uint_as_float(v[0][i]), fb, acc_b[i]), acc_b[32 + i] = fmaf(__uint_as_float(v[1][i]), fb, acc_b[32 + i]);
+                if (++buf == 2) buf = 0, acc_ph ^= 1u;
+            }
+            const float bad = tc_verdict(ok, dead);
+            if constexpr (GATED) {
+                float *most = reinterpret_cast<float *>(pr_smem + kPrStages * kPrStage + kPrSumWarps * kPrOut);  // [part][token]
+                const int f0 = (r0 >> 1) + row_a;
+                float largest = 0.f;
+#pragma unroll
+                for (int i = 0; i < 64; ++i) {
+                    acc_a[i] = f0 + i < a.ff ? gated_pair(acc_a[i] * bad, acc_b[i], a.act, a.limit, a.slope) : 0.f;
+                    largest = f8_most(largest, fabsf(acc_a[i]));
+                }
+                most[half * 128 + quarter * 32 + lane] = largest;
+                asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");  // the two warps of these tokens
+                largest = f8_most(largest, most[(half ^ 1) * 128 + quarter * 32 + lane]);
+                asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");  // read by both before the next tile's are written
+                const F8Scale s = f8_scale(largest);
+                if (t < a.rows) {
+                    if (half == 0) a.scales[(size_t)(r0 >> 8) * a.ld_scales + t] = s.scale;
+                    uint8_t *to = a.q + (size_t)t * a.ldq + f0;
+#pragma unroll
+                    for (int i = 0; i < 64; i += 16)
+                        if (f0 + i < a.ldq) {  // a multiple of 16
+                            uint32_t w[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                w[j] = f8_pack4(__fmul_rn(acc_a[i + 4 * j], s.times), __fmul_rn(acc_a[i + 4 * j + 1], s.times), __fmul_rn(acc_a[i + 4 * j + 2], s.times),
+                                                __fmul_rn(acc_a[i + 4 * j + 3], s.times));
+                            *reinterpret_cast<uint4 *>(to + i) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                }
+            } else {
+                constexpr int PER = 32 / (int)sizeof(T);  // of 32 bytes
+                const int c_a = r0 + row_a, c_b = r0 + row_b;
+                if (a.bias) {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) {
+                        if (c_a + i < a.n) acc_a[i] += to_f(static_cast<const T *>(a.bias)[c_a + i]);
+                        if (c_b + i < a.n) acc_b[i] += to_f(static_cast<const T *>(a.bias)[c_b + i]);
+                    }
+                }
+                auto piece = [&](const float *v, uint32_t (&w)[8]) {  // PER numbers
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        if constexpr (sizeof(T) == 2) w[j] = tl::pack2<T>(v[2 * j] * bad, v[2 * j + 1] * bad);
+                        else w[j] = __float_as_uint(v[j] * bad);
+                    }
+                };
+                T *out = static_cast<T *>(a.out);
+                if (a.aligned) {
+                    if (t < a.rows) {
+#pragma unroll
+                        for (int i = 0; i < 64; i += PER) {  // a piece is whole or not at all
+                            uint32_t w[8];
+                            piece(acc_a + i, w);
+                            if (c_a + i < a.n) pr_store32(out + (size_t)t * a.n + c_a + i, w);
+                            piece(acc_b + i, w);
+                            if (c_b + i < a.n) pr_store32(out + (size_t)t * a.n + c_b + i, w);
+                        }
+                    }
+                } else {  // through staging rows of 64 bytes, so that lanes lie along the columns
+                    unsigned char *stage = pr_smem + kPrStages * kPrStage + (warp - 4) * kPrOut;
+                    constexpr int COLS = 64 / (int)sizeof(T);
+#pragma unroll
+                    for (int i = 0; i < 128; i += COLS) {
+                        __syncwarp();
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            uint32_t w[8];
+                            const int k = i + h * PER;
+                            piece(k < 64 ? acc_a + k : acc_b + k - 64, w);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) *reinterpret_cast<uint32_t *>(stage + lane * kPrOutStride + h * 32 + j * 4) = w[j];
+                        }
+                        __syncwarp();
+                        const int c = (i < 64 ? c_a + i : c_b + i - 64) + lane % COLS;
+#pragma unroll 4
+                        for (int r = lane / COLS; r < 32; r += 32 / COLS) {
+                            const int tr = t0 + quarter * 32 + r;
+                            if (tr < a.rows && c < a.n) out[(size_t)tr * a.n + c] = *reinterpret_cast<const T *>(stage + r * kPrOutStride + lane % COLS * sizeof(T));
+                        }
+                    }
+                }
+            }
+        }
+    }
+    __syncwarp();  // also behind a role whose wait gave up
+    g_tc_fence_before();
+    __syncthreads();
+    if (warp == 2) tc_settle(dead);
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");  // the other CTA is done with this one's memory
+    if (warp == 2) {
+        g_tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+template <typename T, bool GATED>
+static int pr_launch(const F8Product &p, F8PairArgs &a, cudaStream_t st) {
+    CUtensorMap mq, mw;
+    if (int e = tc_map_bytes(&mq, p.q, p.ldq, p.rows, p.ldq, 128)) return e;
+    if (int e = tc_map_bytes(&mw, p.w, p.ldw, p.n, p.ldw, 128)) return e;
+    a.sx = p.sx, a.sw = p.sw, a.ld_sx = p.ld_sx, a.rows = p.rows, a.n = p.n, a.k_blocks = ceil_div(p.k, kF8Block), a.m_tiles = ceil_div(p.rows, 256);
+    const long long tiles = (long long)a.m_tiles * ceil_div(p.n, 256);
+    if (tiles > 0x3fffffff) return tl::fail(TL_EINVAL, "fp8_product: too large");
+    a.tiles = (int)tiles;
+    if (cudaFuncSetAttribute(fp8_pairs_kernel<T, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPrSmem) != cudaSuccess) {
+        cudaGetLastError();
+        return tl::fail(TL_ECUDA, "fp8_product: no shared memory");
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(2 * (unsigned)std::min<long long>(tiles, sm_count() / 2));
+    cfg.blockDim = dim3(kPrThreads);
+    cfg.dynamicSmemBytes = kPrSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = tl::use_pdl() ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, fp8_pairs_kernel<T, GATED>, mq, mw, a);
+    TL_LAUNCH_CHECK("fp8_product");
+    return TL_OK;
+}
+
+int f8_pairs(const F8Product &p, cudaStream_t st) {
+    F8PairArgs a{};
+    a.bias = p.bias, a.out = p.out;
+    const size_t size = p.dtype == TL_BF16 ? 2 : 4;
+    a.aligned = (p.n * size) % 32 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 31) == 0;
+    TLB_DISPATCH(p.dtype, "fp8_product", return (pr_launch<T, false>(p, a, st)));
+    return TL_OK;
+}
+
+int f8_pairs_gated(const F8Product &p, const F8Rows &to, cudaStream_t st) {
+    F8PairArgs a{};
+    a.q = to.q, a.scales = to.scales, a.ldq = to.ldq, a.ld_scales = to.ld_scales, a.ff = to.cols, a.act = to.act, a.limit = to.limit, a.slope = to.slope;
+    return pr_launch<float, true>(p, a, st);
+}
+
+long long f8_pairs_gave_up() { return tl::read_gave_up(); }
+
+}  // namespace tlb

@@ -7,7 +7,8 @@
 // and add it times the two scales.  128 rows of the matrix are a tile's M side (a lane each, and one scale for all of them), BN tokens its
 // N side, so the second scale is a column's: a warp has its columns' products of scales in shared memory, a broadcast read for four.
 //
-// 12 warps: 0 TMA of both operands (boxes of 128 bytes, 128-byte swizzle: one block of the reduction a stage), 1 the products, 4-11 the sums.
+// Warps: 0 and 3 TMA of the matrix and of the rows (boxes of 128 bytes, 128-byte swizzle: one block of the reduction a stage), 1 the products, the sums from 4 on: 8, or 16
+// above 64 tokens, where a block's accumulator would otherwise wait for its turn in two long chains of reads of tensor memory.
 //
 // Few tokens make few tiles: then the CTAs of a cluster share a tile's blocks and add their sums through each other's shared memory, every
 // sum in rank order, so no memory and no atomics stand between two launches, and the result does not depend on their timing.
@@ -18,17 +19,17 @@
 
 namespace tlb {
 
-constexpr int kF8Threads = 12 * 32;
-constexpr int kF8SumWarps = 8;
 constexpr int kF8WeightBytes = 128 * 128;
 
 template <int BN>
 struct F8Tile {
     static constexpr int kStage = kF8WeightBytes + BN * 128;
     static constexpr int kPerSm = BN <= 64 ? 2 : 1;
-    static constexpr int kBuffers = BN >= 128 ? 2 : 4;  // accumulators
-    static constexpr int kTmem = BN * kBuffers;         // columns: 64, 128, 256, 256, 512
-    static constexpr int kFactors = kF8SumWarps * (BN / 2) * 4;
+    static constexpr int kSumWarps = BN <= 64 ? 8 : 16, kThreads = (4 + kSumWarps) * 32;
+    static constexpr int kCols = BN / (kSumWarps / 4);  // of a warp
+    static constexpr int kBuffers = 4;           // accumulators
+    static constexpr int kTmem = BN * kBuffers;  // columns: 64, 128, 256, 512
+    static constexpr int kFactors = kSumWarps * kCols * 4;
     static constexpr int kStages = std::min(8, (227 * 1024 / kPerSm - 1024 - kFactors - 512) / kStage);
     static constexpr int kSmem = kStages * kStage + kFactors + 256;
 };
@@ -58,10 +59,10 @@ __device__ __forceinline__ void f8_mma(uint32_t d, uint64_t a, uint64_t b, uint3
 __host__ __device__ constexpr uint32_t f8_idesc(int n) { return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24); }
 
 template <typename T, int BN>
-__global__ void __launch_bounds__(kF8Threads, F8Tile<BN>::kPerSm)
+__global__ void __launch_bounds__(F8Tile<BN>::kThreads, F8Tile<BN>::kPerSm)
 fp8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_q, const F8Args a) {
     using Tile = F8Tile<BN>;
-    constexpr int COLS = BN / 2, STEP = COLS < 16 ? 8 : 16;  // columns of a warp, of one read of tensor memory
+    constexpr int COLS = Tile::kCols, STEP = COLS < 16 ? 8 : 16;  // columns of a warp, of one read of tensor memory
     extern __shared__ __align__(1024) unsigned char f8_smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = g_smem_u32(f8_smem);
@@ -72,8 +73,8 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(const_cast<int *>(dead)) + 1;
 
     if (warp == 0 && lane == 0) {
-        for (int i = 0; i < Tile::kStages; ++i) g_mbar_init(full + 8 * i, 1), g_mbar_init(empty + 8 * i, 1);
-        for (int i = 0; i < Tile::kBuffers; ++i) g_mbar_init(acc_full + 8 * i, 1), g_mbar_init(acc_empty + 8 * i, kF8SumWarps);
+        for (int i = 0; i < Tile::kStages; ++i) g_mbar_init(full + 8 * i, 2), g_mbar_init(empty + 8 * i, 1);  // full: either kind of copies
+        for (int i = 0; i < Tile::kBuffers; ++i) g_mbar_init(acc_full + 8 * i, 1), g_mbar_init(acc_empty + 8 * i, Tile::kSumWarps);
         *dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
@@ -91,64 +92,48 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const int rank = blockIdx.x % a.splits, first = blockIdx.x / a.splits, step = gridDim.x / a.splits;
     const int kb0 = (int)((long long)a.k_blocks * rank / a.splits), kb1 = (int)((long long)a.k_blocks * (rank + 1) / a.splits);
 
-    if (warp == 0) {
-        int s = 0;
-        uint32_t ph = 1;
-        auto load_w = [&](int stage, int tile, int kb) {
-            if (g_elect_one()) {
-                g_mbar_expect_tx(full + 8 * stage, Tile::kStage);
-                g_tma_load_2d(base + stage * Tile::kStage, &map_w, kb * 128, tile % a.m_blocks * 128, full + 8 * stage);
-            }
-            __syncwarp();
-        };
-        auto load_q = [&](int stage, int tile, int kb) {
-            if (g_elect_one()) g_tma_load_2d(base + stage * Tile::kStage + kF8WeightBytes, &map_q, kb * 128, tile / a.m_blocks * BN, full + 8 * stage);
-            __syncwarp();
-        };
-        // the first stages' weights are asked for while the rows' launch is still running: they are older than it
-        const int ahead = min(Tile::kStages, kb1 - kb0);
-        if (first < a.tiles)
-            for (int i = 0; i < ahead; ++i) load_w(i, first, kb0 + i);
-        tl::griddep_wait();
-        int early = ahead;
-        for (int tile = first; tile < a.tiles; tile += step)
-            for (int kb = kb0; kb < kb1; ++kb) {
-                if (early > 0) {
-                    --early;
-                } else {
-                    if (!tc_wait(empty + 8 * s, ph, dead)) goto out;
-                    load_w(s, tile, kb);
+    // A thread by itself for each role: with the whole warp in the loop a block cost twice the cycles.
+    if (warp == 0 || warp == 3) {  // the matrix's copies and the rows'
+        if (g_elect_one()) {
+            int s = 0;
+            uint32_t ph = 1;
+            bool ok = true;
+            if (warp == 3) tl::griddep_wait();  // the matrix is older than the rows' launch, which may still be running
+            for (int tile = first; ok && tile < a.tiles; tile += step)
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (!(ok = tc_wait_one(empty + 8 * s, ph, dead))) break;
+                    g_mbar_expect_tx(full + 8 * s, warp == 0 ? kF8WeightBytes : BN * 128);
+                    if (warp == 0) g_tma_load_2d(base + s * Tile::kStage, &map_w, kb * 128, tile % a.m_blocks * 128, full + 8 * s);
+                    else g_tma_load_2d(base + s * Tile::kStage + kF8WeightBytes, &map_q, kb * 128, tile / a.m_blocks * BN, full + 8 * s);
+                    if (++s == Tile::kStages) s = 0, ph ^= 1u;
                 }
-                load_q(s, tile, kb);
-                if (++s == Tile::kStages) s = 0, ph ^= 1u;
-            }
+        }
     } else if (warp == 1) {
-        int s = 0, buf = 0;
-        uint32_t ph = 0, acc_ph = 1;
-        for (int tile = first; tile < a.tiles; tile += step)
-            for (int kb = kb0; kb < kb1; ++kb) {
-                if (!tc_wait(acc_empty + 8 * buf, acc_ph, dead)) goto out;
-                if (!tc_wait(full + 8 * s, ph, dead)) goto out;
-                g_tc_fence_after();
-                if (g_elect_one()) {
+        if (g_elect_one()) {
+            int s = 0, buf = 0;
+            uint32_t ph = 0, acc_ph = 1;
+            bool ok = true;
+            for (int tile = first; ok && tile < a.tiles; tile += step)
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (!(ok = tc_wait_one(acc_empty + 8 * buf, acc_ph, dead) && tc_wait_one(full + 8 * s, ph, dead))) break;
+                    g_tc_fence_after();
                     const uint64_t w = g_smem_desc_sw128(base + s * Tile::kStage, 0, 1024), q = g_smem_desc_sw128(base + s * Tile::kStage + kF8WeightBytes, 0, 1024);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) f8_mma(tmem + buf * BN, w + 2 * k, q + 2 * k, f8_idesc(BN), k > 0);
-                    g_tc_commit(empty + 8 * s);
                     g_tc_commit(acc_full + 8 * buf);
+                    g_tc_commit(empty + 8 * s);
+                    if (++s == Tile::kStages) s = 0, ph ^= 1u;
+                    if (++buf == Tile::kBuffers) buf = 0, acc_ph ^= 1u;
                 }
-                __syncwarp();
-                if (++s == Tile::kStages) s = 0, ph ^= 1u;
-                if (++buf == Tile::kBuffers) buf = 0, acc_ph ^= 1u;
-            }
+        }
     } else if (warp >= 4) {
-        const int quarter = warp & 3, half = (warp - 4) >> 2;
+        const int quarter = warp & 3, part = (warp - 4) >> 2;
         float *mine = factors + (warp - 4) * COLS;
         int buf = 0;
         uint32_t acc_ph = 0;
         tl::griddep_wait();
         for (int tile = first; tile < a.tiles; tile += step) {
-            const int m = tile % a.m_blocks, col0 = tile / a.m_blocks * BN + half * COLS, f = m * 128 + quarter * 32 + lane;
+            const int m = tile % a.m_blocks, col0 = tile / a.m_blocks * BN + part * COLS, f = m * 128 + quarter * 32 + lane;
             constexpr int PER = (COLS + 31) / 32;
             float acc[COLS], next[PER], next_w = 0.f;
 #pragma unroll
@@ -171,7 +156,7 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 __syncwarp();
                 ok &= tc_wait(acc_full + 8 * buf, acc_ph, dead);
                 g_tc_fence_after();
-                const uint32_t at = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN + half * COLS;
+                const uint32_t at = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN + part * COLS;
 #pragma unroll
                 for (int c = 0; c < COLS; c += STEP) {
                     uint32_t v[STEP];
@@ -199,17 +184,17 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 for (int c = 0; c < COLS; ++c)
                     if (f < a.n && col0 + c < a.rows) out[(size_t)c * a.n] = from_f<T>((acc[c] + b) * bad);
             } else {  // the stages are done with: the last accumulator came behind all products
-                float *part = reinterpret_cast<float *>(f8_smem) + half * COLS * 128 + quarter * 32 + lane;
+                float *sums = reinterpret_cast<float *>(f8_smem) + part * COLS * 128 + quarter * 32 + lane;
 #pragma unroll
-                for (int c = 0; c < COLS; ++c) part[c * 128] = acc[c] * bad;
+                for (int c = 0; c < COLS; ++c) sums[c * 128] = acc[c] * bad;
             }
         }
     }
-out:  // also from a role whose wait gave up
+    __syncwarp();  // also behind a role whose wait gave up
     if (a.splits > 1) {  // one tile a cluster; a CTA adds its share of the tokens
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
         const int share = BN / a.splits, m = first % a.m_blocks, col0 = first / a.m_blocks * BN + rank * share;
-        for (int i = threadIdx.x; i < share * 32; i += kF8Threads) {
+        for (int i = threadIdx.x; i < share * 32; i += Tile::kThreads) {
             const int c = i >> 5, f = m * 128 + (i & 31) * 4, at = ((rank * share + c) * 128 + (i & 31) * 4) * 4;
             if (col0 + c >= a.rows) break;
             float sum[4] = {};
@@ -239,6 +224,13 @@ out:  // also from a role whose wait gave up
     }
 }
 
+// The CTAs that share a tile's blocks, so that few tiles fill the SMs; two blocks each at least.
+static int f8_splits(long long tiles, int k_blocks, int room) {
+    int splits = 1;
+    while (splits < 8 && tiles * splits * 2 <= room && k_blocks >= 4 * splits) splits *= 2;
+    return splits;
+}
+
 template <typename T, int BN>
 static int f8_launch(const F8Product &p, cudaStream_t st) {
     using Tile = F8Tile<BN>;
@@ -251,15 +243,14 @@ static int f8_launch(const F8Product &p, cudaStream_t st) {
     if (tiles > 0x3fffffff) return tl::fail(TL_EINVAL, "fp8_product: too large");
     a.tiles = (int)tiles;
     const int room = sm_count() * Tile::kPerSm;
-    if (BN <= 128)
-        while (a.splits < 8 && tiles * a.splits * 2 <= room && a.k_blocks >= 4 * a.splits) a.splits *= 2;
+    a.splits = f8_splits(tiles, a.k_blocks, room);
     if (cudaFuncSetAttribute(fp8_product_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmem) != cudaSuccess) {
         cudaGetLastError();
         return tl::fail(TL_ECUDA, "fp8_product: no shared memory");
     }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(a.splits > 1 ? tiles * a.splits : std::min<long long>(tiles, room)));
-    cfg.blockDim = dim3(kF8Threads);
+    cfg.blockDim = dim3(Tile::kThreads);
     cfg.dynamicSmemBytes = Tile::kSmem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -274,12 +265,39 @@ static int f8_launch(const F8Product &p, cudaStream_t st) {
     return TL_OK;
 }
 
+// Which kernel, by the time that its rounds of tiles take: blocks of a CTA one after another, times what one takes, by measurement over 200 to 700 rows of 2560 to
+// 9728 numbers and 2560 to 19456 outputs (us a block: 32 tokens 0.48, 64 0.66, 128 0.56, a pair's 256 x 256 0.58).  Up to 128 rows the smallest tile that holds them
+// all, which reads the matrix once, was the fastest throughout.
+static int f8_tile(const F8Product &p) {
+    for (int bn : {16, 32, 64, 128})
+        if (p.rows <= bn) return bn;
+    const int k_blocks = ceil_div(p.k, kF8Block), sms = sm_count();
+    const struct {
+        int tokens, outputs, room;
+        float block;
+    } kinds[] = {{32, 128, 2 * sms, 0.48f}, {64, 128, 2 * sms, 0.66f}, {128, 128, sms, 0.56f}, {256, 256, sms / 2, 0.58f}};
+    int best = 0;
+    float least = INFINITY;
+    for (const auto &t : kinds) {
+        const long long tiles = (long long)ceil_div(p.n, t.outputs) * ceil_div(p.rows, t.tokens);
+        const int splits = t.tokens == 256 ? 1 : f8_splits(tiles, k_blocks, t.room);
+        const float time = (float)((tiles * splits + t.room - 1) / t.room) * ceil_div(k_blocks, splits) * t.block;
+        if (time < least) least = time, best = t.tokens;
+    }
+    return best;
+}
+
 int f8_product(const F8Product &p, cudaStream_t st) {
-    TLB_DISPATCH(p.dtype, "fp8_product", if (p.rows <= 16) return f8_launch<T, 16>(p, st); if (p.rows <= 32) return f8_launch<T, 32>(p, st);
-                 if (p.rows <= 64) return f8_launch<T, 64>(p, st); if (p.rows <= 128) return f8_launch<T, 128>(p, st); return f8_launch<T, 256>(p, st));
+    const int tile = f8_tile(p);
+    if (tile == 256) return f8_pairs(p, st);
+    TLB_DISPATCH(p.dtype, "fp8_product", return tile == 16 ? f8_launch<T, 16>(p, st) : tile == 32 ? f8_launch<T, 32>(p, st) : tile == 64 ? f8_launch<T, 64>(p, st)
+                                                                                                               : f8_launch<T, 128>(p, st));
     return TL_OK;
 }
 
-long long f8_gave_up() { return tl::read_gave_up(); }
+long long f8_gave_up() {
+    const long long one = tl::read_gave_up(), pairs = f8_pairs_gave_up();
+    return one < 0 || pairs < 0 ? -1 : one + pairs;
+}
 
 }  // namespace tlb

@@ -30,63 +30,75 @@ __device__ __forceinline__ void rows_load(const T *p, int left, float (&v)[8]) {
     }
 }
 
-// WIDE: every group of eight is whole and aligned to 16 bytes.
-template <typename T, bool GATED, bool WIDE>
+// WIDE: every group of eight is whole and aligned to 16 bytes.  A half warp takes U runs, neighbours in its row-by-row order, all on their way at once.
+template <typename T, bool GATED, bool WIDE, int U>
 __global__ void __launch_bounds__(kRowsThreads)
 fp8_rows_kernel(const T *x, long long ldx, int rows, int cols, int act, float limit, float slope, uint8_t *q, int ldq, float *scales, int ld_scales) {
-    const int runs = (cols + kF8Block - 1) / kF8Block, lane = threadIdx.x & 15;
-    const long long at = ((long long)blockIdx.x * kRowsThreads + threadIdx.x) >> 4;
+    const unsigned runs = (cols + kF8Block - 1) / kF8Block, total = rows * runs, lane = threadIdx.x & 15;
+    const unsigned first = ((blockIdx.x * kRowsThreads + threadIdx.x) >> 4) * U;
     tl::griddep_wait();
     tl::griddep_launch();  // behind the wait: what a dependent reads ahead of its own is older than this launch
-    const bool live = at < (long long)rows * runs;  // a half warp as one
-    const int row = live ? (int)(at / runs) : 0, run = live ? (int)(at % runs) : 0, k = run * kF8Block + lane * 8, left = live ? cols - k : 0;
-    float v[8];
+    float v[U][8];
+    unsigned row[U], run[U];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    if (left > 0) {
-        if constexpr (GATED) {  // the columns of a whole run are there, those past the last feature are zero
-            const T *from = x + row * ldx + run * 2 * kF8Block + lane * 8;
-            float g[8], u[8];
-            rows_load<T, WIDE>(from, 8, g);
-            rows_load<T, WIDE>(from + kF8Block, 8, u);
+    for (int u = 0; u < U; ++u) {
+        const bool live = first + u < total;  // a half warp as one
+        row[u] = live ? (first + u) / runs : 0, run[u] = live ? first + u - row[u] * runs : 0;
+        const int k = run[u] * kF8Block + lane * 8, left = live ? cols - k : 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = i < left ? gated_pair(g[i], u[i], act, limit, slope) : 0.f;
-        } else {
-            rows_load<T, WIDE>(x + row * ldx + k, left, v);
+        for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
+        if (left > 0) {
+            if constexpr (GATED) {  // the columns of a whole run are there, those past the last feature are zero
+                const T *from = x + row[u] * ldx + run[u] * 2 * kF8Block + lane * 8;
+                float g[8], up[8];
+                rows_load<T, WIDE>(from, 8, g);
+                rows_load<T, WIDE>(from + kF8Block, 8, up);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[u][i] = i < left ? gated_pair(g[i], up[i], act, limit, slope) : 0.f;
+            } else {
+                rows_load<T, WIDE>(x + row[u] * ldx + k, left, v[u]);
+            }
         }
     }
-    float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) most = f8_most(most, fabsf(v[i]));
+    for (int u = 0; u < U; ++u) {
+        float most = 0.f;
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) most = f8_most(most, __shfl_xor_sync(0xffffffffu, most, o));
-    const F8Scale s = f8_scale(most);
-    if (!live) return;
-    if (lane == 0) scales[(size_t)run * ld_scales + row] = s.scale;
-    if (k >= ldq) return;
+        for (int i = 0; i < 8; ++i) most = f8_most(most, fabsf(v[u][i]));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], s.times);
-    *reinterpret_cast<uint2 *>(q + (size_t)row * ldq + k) = make_uint2(f8_pack4(v[0], v[1], v[2], v[3]), f8_pack4(v[4], v[5], v[6], v[7]));
+        for (int o = 8; o > 0; o >>= 1) most = f8_most(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const F8Scale s = f8_scale(most);
+        if (first + u >= total) continue;
+        if (lane == 0) scales[(size_t)run[u] * ld_scales + row[u]] = s.scale;
+        const int k = run[u] * kF8Block + lane * 8;
+        if (k >= ldq) continue;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[u][i] = __fmul_rn(v[u][i], s.times);
+        *reinterpret_cast<uint2 *>(q + (size_t)row[u] * ldq + k) = make_uint2(f8_pack4(v[u][0], v[u][1], v[u][2], v[u][3]), f8_pack4(v[u][4], v[u][5], v[u][6], v[u][7]));
+    }
 }
 
 int f8_rows(const F8Rows &a, cudaStream_t st) {
-    const long long halves = (long long)a.rows * ceil_div(a.cols, kF8Block);
-    const long long grid = (halves * 16 + kRowsThreads - 1) / kRowsThreads;
-    if (grid > 0x7fffffffLL) return tl::fail(TL_EINVAL, "fp8_rows: too many rows");
-#define TLB_ROWS(T, G, W)                                                                                                                               \
-    tl::launch_chained(fp8_rows_kernel<T, G, W>, dim3((unsigned)grid), dim3(kRowsThreads), 0, st, (const T *)a.x, a.ldx, a.rows, a.cols, a.act, a.limit, a.slope, a.q, \
-                       a.ldq, a.scales, a.ld_scales)
+    const long long runs = (long long)a.rows * ceil_div(a.cols, kF8Block);
+    if (runs > 0x7fffff00LL) return tl::fail(TL_EINVAL, "fp8_rows: too many rows");
+    const bool many = runs >= 32 * 1024;  // below, one run a half warp puts more warps to work
+#define TLB_ROWS(T, G, W, U)                                                                                                                            \
+    tl::launch_chained(fp8_rows_kernel<T, G, W, U>, dim3((unsigned)((runs + 16 * U - 1) / (16 * U))), dim3(kRowsThreads), 0, st, (const T *)a.x, a.ldx, a.rows, a.cols, \
+                       a.act, a.limit, a.slope, a.q, a.ldq, a.scales, a.ld_scales)
     if (a.gated) {
-        TLB_ROWS(float, true, true);
+        TLB_ROWS(float, true, true, 1);
     } else {
         const size_t es = a.dtype == TL_BF16 ? 2 : 4;
         const bool wide = a.cols % 8 == 0 && (a.ldx * es) % 16 == 0 && tl::aligned16(a.x);
-        TLB_DISPATCH(a.dtype, "fp8_rows", if (wide) TLB_ROWS(T, false, true); else TLB_ROWS(T, false, false));
+        TLB_DISPATCH(a.dtype, "fp8_rows", if (wide && many) TLB_ROWS(T, false, true, 4); else if (wide) TLB_ROWS(T, false, true, 1); else TLB_ROWS(T, false, false, 1));
     }
 #undef TLB_ROWS
     TL_LAUNCH_CHECK("fp8_rows");
     return TL_OK;
 }
+
+// Above this many rows the first product of a feed-forward leaves its gated rows rounded, below it fp32 sums and a launch that gates and rounds them.
+constexpr int kF8Fused = 128;
 
 // The rounded rows of one product in a caller's scratch: bytes, then scales.
 static size_t f8_rows_bytes(int rows, int cols) {
@@ -117,7 +129,8 @@ int tlb_fp8_linear(const void *x, long long ldx, const void *w, int ldw, const f
 
 size_t tlb_fp8_gated_mlp_workspace(int rows, int dim, int ff) {
     if (rows <= 0 || dim <= 0 || ff <= 0) return 0;
-    return ((f8_rows_bytes(rows, dim) + 15) & ~(size_t)15) + ((f8_rows_bytes(rows, ff) + 15) & ~(size_t)15) + (size_t)rows * 2 * f8_up(ff, kF8Block) * sizeof(float);
+    return ((f8_rows_bytes(rows, dim) + 15) & ~(size_t)15) + ((f8_rows_bytes(rows, ff) + 15) & ~(size_t)15) +
+           (rows > kF8Fused ? 0 : (size_t)rows * 2 * f8_up(ff, kF8Block) * sizeof(float));
 }
 
 int tlb_fp8_gated_mlp(const void *x, long long ldx, const void *w_gate_up, int ld_gate_up, const float *s_gate_up, const void *w_down, int ld_down, const float *s_down,
@@ -135,8 +148,14 @@ int tlb_fp8_gated_mlp(const void *x, long long ldx, const void *w_gate_up, int l
     float *sx = (float *)(q + (size_t)rows * f8_up(dim, 16)), *sx2 = (float *)(q2 + (size_t)rows * f8_up(ff, 16));
     float *inner = (float *)(q2 + ((f8_rows_bytes(rows, ff) + 15) & ~(size_t)15));
     if (int e = f8_rows({x, ldx, rows, dim, dtype, false, 0, 0.f, 1.f, q, f8_up(dim, 16), sx, ld_sx}, st)) return e;
-    if (int e = f8_product({q, sx, f8_up(dim, 16), ld_sx, rows, (const uint8_t *)w_gate_up, s_gate_up, ld_gate_up, wide, dim, nullptr, inner, TL_F32}, st)) return e;
-    if (int e = f8_rows({inner, wide, rows, ff, TL_F32, true, act, limit, slope, q2, f8_up(ff, 16), sx2, ld_sx}, st)) return e;
+    const F8Product first{q, sx, f8_up(dim, 16), ld_sx, rows, (const uint8_t *)w_gate_up, s_gate_up, ld_gate_up, wide, dim, nullptr, inner, TL_F32};
+    const F8Rows gated{inner, wide, rows, ff, TL_F32, true, act, limit, slope, q2, f8_up(ff, 16), sx2, ld_sx};
+    if (rows > kF8Fused) {
+        if (int e = f8_pairs_gated(first, gated, st)) return e;
+    } else {
+        if (int e = f8_product(first, st)) return e;
+        if (int e = f8_rows(gated, st)) return e;
+    }
     return f8_product({q2, sx2, f8_up(ff, 16), ld_sx, rows, (const uint8_t *)w_down, s_down, ld_down, dim, ff, nullptr, out, dtype}, st);
 }
 

@@ -22,6 +22,7 @@ using tl::g_tma_load_2d;
 using tl::tc_settle;
 using tl::tc_verdict;
 using tl::tc_wait;
+using tl::tc_wait_one;
 
 long long flash_tc_gave_up();  // of the attention kernels
 long long f8_gave_up();        // of the 8-bit products

@@ -61,6 +61,7 @@ BLOCKS_SOURCES = [
     "blocks/blocks_moe_few.cu",
     "blocks/blocks_fp8_rows.cu",
     "blocks/blocks_fp8_product.cu",
+    "blocks/blocks_fp8_pairs.cu",
 ]
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
