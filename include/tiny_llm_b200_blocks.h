@@ -364,10 +364,15 @@ int tlb_argmax_rows(const float *logits, int32_t *out, int rows, int vocab, void
  * 1-8, 9-16, 17-32 of tokens in a call. */
 int tlb_moe_few_tokens(int dim, int outputs, int experts, int top, int group_count, int fp8);
 size_t tlb_moe_few_workspace(int tokens, int top, int experts, int ff);
-int tlb_moe_few(const void *x, const void *router, const void *router_bias, const void *choice_bias, const void *side_w, int tokens, int dim, int outputs, int experts,
-                int top, int scoring, float weight_scale, int group_count, int group_keep, const void *w_gate, const void *w_up, const void *w_down, const float *s_gate,
-                const float *s_up, const float *s_down, int fp8, int ff, int ld_in, int ld_out, int act, float limit, float slope, const void *shared, void *out, int out_f32,
-                void *workspace, size_t workspace_bytes, void *stream);
+typedef struct {
+    const void *router, *router_bias, *choice_bias, *side_w; /* biases and side_w may be NULL */
+    const void *w_gate, *w_up, *w_down;
+    const float *s_gate, *s_up, *s_down; /* fp8 */
+    int dim, outputs, experts, top, scoring, group_count, group_keep;
+    int fp8, ff, ld_in, ld_out, act;
+    float weight_scale, limit, slope;
+} tlb_moe_few_layer;
+int tlb_moe_few(const tlb_moe_few_layer *layer, const void *x, int tokens, const void *shared, void *out, int out_f32, void *workspace, size_t workspace_bytes, void *stream);
 
 /* Products over matrices of 8-bit numbers (e4m3) with one fp32 scale for each block of 128 x 128: w [n, ldw] bytes (ldw a multiple of 16, the
  * base 16-byte aligned, zero behind column k), sw [ceil(n / 128), ceil(k / 128)].  The rows x [rows, k] (`dtype`, ldx apart) are rounded to e4m3 with

@@ -63,6 +63,9 @@ struct F8Product {
     int dtype;  // of bias and out
 };
 int f8_product(const F8Product &a, cudaStream_t st);
+// the same from rows that are not rounded yet, where f8_own says so (p.q, p.sx and p.ldq are not read)
+bool f8_own(const F8Product &p);
+int f8_product_own(const F8Product &a, const F8Rows &x, cudaStream_t st);
 // blocks_fp8_pairs.cu: the same for many rows, and, of 128 rows of a gate and 128 of an up projection in turn, the gated rows rounded to e4m3 (to.q, to.scales)
 int f8_pairs(const F8Product &a, cudaStream_t st);
 int f8_pairs_gated(const F8Product &a, const F8Rows &to, cudaStream_t st);

@@ -16,6 +16,7 @@
 
 #include "blocks_fp8.cuh"
 #include "blocks_tc.cuh"
+#include "../per_device.h"
 
 namespace tlb {
 
@@ -294,7 +295,10 @@ static int pr_launch(const F8Product &p, F8PairArgs &a, cudaStream_t st) {
     const long long tiles = (long long)a.m_tiles * ceil_div(p.n, 256);
     if (tiles > 0x3fffffff) return tl::fail(TL_EINVAL, "fp8_product: too large");
     a.tiles = (int)tiles;
-    if (cudaFuncSetAttribute(fp8_pairs_kernel<T, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPrSmem) != cudaSuccess) {
+    static tl::PerDevice ready;
+    int device = 0;
+    cudaGetDevice(&device);
+    if (!ready(device, [&] { return cudaFuncSetAttribute(fp8_pairs_kernel<T, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPrSmem) == cudaSuccess; })) {
         cudaGetLastError();
         return tl::fail(TL_ECUDA, "fp8_product: no shared memory");
     }

@@ -16,29 +16,37 @@
 
 #include "blocks_fp8.cuh"
 #include "blocks_tc.cuh"
+#include "../per_device.h"
 
 namespace tlb {
 
 constexpr int kF8WeightBytes = 128 * 128;
 
-template <int BN>
+// Where the rows come from: rounded by a launch before, or (few rows) rounded here, by every CTA its own blocks of them, once for all its tiles.
+constexpr int kF8Tma = 0, kF8Plain = 1, kF8Gated = 2;
+constexpr int kF8OwnRows = 8, kF8OwnBlocks = 32;  // the most rows, and blocks of the reduction of a CTA
+
+template <int BN, bool OWN>
 struct F8Tile {
-    static constexpr int kStage = kF8WeightBytes + BN * 128;
+    static constexpr int kStage = kF8WeightBytes + (OWN ? 0 : BN * 128);
     static constexpr int kPerSm = BN <= 64 ? 2 : 1;
     static constexpr int kSumWarps = BN <= 64 ? 8 : 16, kThreads = (4 + kSumWarps) * 32;
     static constexpr int kCols = BN / (kSumWarps / 4);  // of a warp
     static constexpr int kBuffers = 4;           // accumulators
     static constexpr int kTmem = BN * kBuffers;  // columns: 64, 128, 256, 512
     static constexpr int kFactors = kSumWarps * kCols * 4;
-    static constexpr int kStages = std::min(8, (227 * 1024 / kPerSm - 1024 - kFactors - 512) / kStage);
-    static constexpr int kSmem = kStages * kStage + kFactors + 256;
+    static constexpr int kOwn = OWN ? kF8OwnBlocks * kF8OwnRows * (kF8Block + 4) : 0;  // rows that the kernel rounds itself, and their scales
+    static constexpr int kStages = std::min(8, (227 * 1024 / kPerSm - 1024 - kFactors - kOwn - 512) / kStage);
+    static constexpr int kSmem = kStages * kStage + kFactors + kOwn + 256;
 };
 
 struct F8Args {
+    F8Rows x;  // kF8Own: the rows as they come; of it x, ldx, gated, act, limit, slope
     const float *sx, *sw;
     const void *bias;
     void *out;
     int ld_sx, rows, n, k_blocks, m_blocks, tiles, splits;
+    int second;  // the launch before is one of these products or the rows' rounding, which waited for what was before it: the matrix is older than both
 };
 
 // C consecutive columns (8 or 16) of the warp's lanes, without the wait.
@@ -58,22 +66,53 @@ __device__ __forceinline__ void f8_mma(uint32_t d, uint64_t a, uint64_t b, uint3
 // e4m3 x e4m3 -> f32, 128 rows, n columns, both K-major
 __host__ __device__ constexpr uint32_t f8_idesc(int n) { return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24); }
 
-template <typename T, int BN>
-__global__ void __launch_bounds__(F8Tile<BN>::kThreads, F8Tile<BN>::kPerSm)
+// Four numbers of a row from column k on, zero behind the last one; of gated rows (fp32, 128 of the gate and 128 of the up projection in turn) the gated ones.
+template <typename X, int ROWS>
+__device__ __forceinline__ float4 f8_four(const F8Rows &r, int row, int k, bool whole) {
+    const X *from = static_cast<const X *>(r.x) + (size_t)row * r.ldx;
+    if constexpr (ROWS == kF8Gated) {
+        const int at = k / kF8Block * 2 * kF8Block + k % kF8Block;
+        const uint4 g = tl::ld_cg(reinterpret_cast<const uint4 *>(from + at)), u = tl::ld_cg(reinterpret_cast<const uint4 *>(from + at + kF8Block));
+        auto pair = [&](uint32_t a, uint32_t b, int i) { return k + i < r.cols ? gated_pair(__uint_as_float(a), __uint_as_float(b), r.act, r.limit, r.slope) : 0.f; };
+        return make_float4(pair(g.x, u.x, 0), pair(g.y, u.y, 1), pair(g.z, u.z, 2), pair(g.w, u.w, 3));
+    } else if (whole && k + 4 <= r.cols) {
+        if constexpr (sizeof(X) == 4) {
+            const uint4 v = tl::ld_cg(reinterpret_cast<const uint4 *>(from + k));
+            return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+        } else {
+            uint2 v;
+            asm volatile("ld.global.cg.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(from + k) : "memory");
+            const float2 a = tl::unpack2<X>(v.x), b = tl::unpack2<X>(v.y);
+            return make_float4(a.x, a.y, b.x, b.y);
+        }
+    } else {
+        float v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = k + i < r.cols ? to_f(tl::ld_cg(from + k + i)) : 0.f;
+        return make_float4(v[0], v[1], v[2], v[3]);
+    }
+}
+
+template <typename T, int BN, int ROWS = kF8Tma, typename X = T>
+__global__ void __launch_bounds__(F8Tile<BN, ROWS != kF8Tma>::kThreads, F8Tile<BN, ROWS != kF8Tma>::kPerSm)
 fp8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_q, const F8Args a) {
-    using Tile = F8Tile<BN>;
+    constexpr bool OWN = ROWS != kF8Tma;
+    using Tile = F8Tile<BN, OWN>;
     constexpr int COLS = Tile::kCols, STEP = COLS < 16 ? 8 : 16;  // columns of a warp, of one read of tensor memory
     extern __shared__ __align__(1024) unsigned char f8_smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = g_smem_u32(f8_smem);
-    float *factors = reinterpret_cast<float *>(f8_smem + Tile::kStages * Tile::kStage);
-    const uint32_t bars = base + Tile::kStages * Tile::kStage + Tile::kFactors;
-    const uint32_t full = bars, empty = full + 64, acc_full = empty + 64, acc_empty = acc_full + 32;
-    volatile int *dead = reinterpret_cast<volatile int *>(f8_smem + Tile::kStages * Tile::kStage + Tile::kFactors + 192);
+    const uint32_t own = base + Tile::kStages * Tile::kStage;  // [block][8 rows of 128 bytes, in the swizzled order]
+    float *own_scales = reinterpret_cast<float *>(f8_smem + Tile::kStages * Tile::kStage + (OWN ? kF8OwnBlocks * kF8OwnRows * kF8Block : 0));  // [block][8]
+    float *factors = reinterpret_cast<float *>(f8_smem + Tile::kStages * Tile::kStage + Tile::kOwn);
+    const uint32_t bars = base + Tile::kStages * Tile::kStage + Tile::kFactors + Tile::kOwn;
+    const uint32_t full = bars, empty = full + 64, acc_full = empty + 64, acc_empty = acc_full + 32, rows_there = acc_empty + 32;
+    volatile int *dead = reinterpret_cast<volatile int *>(f8_smem + Tile::kStages * Tile::kStage + Tile::kFactors + Tile::kOwn + 200);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(const_cast<int *>(dead)) + 1;
 
     if (warp == 0 && lane == 0) {
-        for (int i = 0; i < Tile::kStages; ++i) g_mbar_init(full + 8 * i, 2), g_mbar_init(empty + 8 * i, 1);  // full: either kind of copies
+        for (int i = 0; i < Tile::kStages; ++i) g_mbar_init(full + 8 * i, OWN ? 1 : 2), g_mbar_init(empty + 8 * i, 1);  // full: either kind of copies
+        g_mbar_init(rows_there, 10);
         for (int i = 0; i < Tile::kBuffers; ++i) g_mbar_init(acc_full + 8 * i, 1), g_mbar_init(acc_empty + 8 * i, Tile::kSumWarps);
         *dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -89,16 +128,49 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     g_tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
+    if constexpr (OWN) {  // a second product of a feed-forward may ask for its matrix meanwhile
+        if (!a.second) tl::griddep_wait();
+        tl::griddep_launch();
+    }
     const int rank = blockIdx.x % a.splits, first = blockIdx.x / a.splits, step = gridDim.x / a.splits;
     const int kb0 = (int)((long long)a.k_blocks * rank / a.splits), kb1 = (int)((long long)a.k_blocks * (rank + 1) / a.splits);
 
     // A thread by itself for each role: with the whole warp in the loop a block cost twice the cycles.
-    if (warp == 0 || warp == 3) {  // the matrix's copies and the rows'
+    if constexpr (OWN) {
+        if (warp >= 2) {  // the rows of this CTA's blocks, one of either a warp at a time, two on their way
+            const bool whole = ROWS == kF8Gated || (a.x.ldx % 4 == 0 && (reinterpret_cast<uintptr_t>(a.x.x) & (4 * sizeof(X) - 1)) == 0);
+            if (a.second) tl::griddep_wait();
+            const int blocks = kb1 - kb0, pieces = a.rows * blocks;
+            for (int i0 = warp - 2; i0 < pieces; i0 += 20) {
+                float4 v[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    if (i0 + 10 * u < pieces) v[u] = f8_four<X, ROWS>(a.x, (i0 + 10 * u) / blocks, (kb0 + (i0 + 10 * u) % blocks) * kF8Block + lane * 4, whole);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    if (i0 + 10 * u >= pieces) break;
+                    const int t = (i0 + 10 * u) / blocks, b = (i0 + 10 * u) % blocks;
+                    // magnitudes are in the order of their bits, an infinity above all numbers and a NaN above that
+                    const uint32_t most = __reduce_max_sync(0xffffffffu, max(max(__float_as_uint(v[u].x) & 0x7fffffffu, __float_as_uint(v[u].y) & 0x7fffffffu),
+                                                                             max(__float_as_uint(v[u].z) & 0x7fffffffu, __float_as_uint(v[u].w) & 0x7fffffffu)));
+                    const F8Scale f = f8_scale(__uint_as_float(most));
+                    if (lane == 0) own_scales[b * kF8OwnRows + t] = f.scale;
+                    const uint32_t q = f8_pack4(__fmul_rn(v[u].x, f.times), __fmul_rn(v[u].y, f.times), __fmul_rn(v[u].z, f.times), __fmul_rn(v[u].w, f.times));
+                    *reinterpret_cast<uint32_t *>(f8_smem + Tile::kStages * Tile::kStage + (b * kF8OwnRows + t) * kF8Block + (((lane >> 2) ^ t) << 4) + (lane & 3) * 4) = q;
+                }
+            }
+            tl::g_fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) g_mbar_arrive(rows_there);
+            asm volatile("bar.sync 1, 320;" ::: "memory");  // the scales, for the warps that add
+        }
+    }
+    if (warp == 0 || (!OWN && warp == 3)) {  // the matrix's copies and the rows'
         if (g_elect_one()) {
             int s = 0;
             uint32_t ph = 1;
             bool ok = true;
-            if (warp == 3) tl::griddep_wait();  // the matrix is older than the rows' launch, which may still be running
+            if (warp == 3 || !a.second) tl::griddep_wait();
             for (int tile = first; ok && tile < a.tiles; tile += step)
                 for (int kb = kb0; kb < kb1; ++kb) {
                     if (!(ok = tc_wait_one(empty + 8 * s, ph, dead))) break;
@@ -112,12 +184,13 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         if (g_elect_one()) {
             int s = 0, buf = 0;
             uint32_t ph = 0, acc_ph = 1;
-            bool ok = true;
+            bool ok = !OWN || tc_wait_one(rows_there, 0, dead);
             for (int tile = first; ok && tile < a.tiles; tile += step)
                 for (int kb = kb0; kb < kb1; ++kb) {
                     if (!(ok = tc_wait_one(acc_empty + 8 * buf, acc_ph, dead) && tc_wait_one(full + 8 * s, ph, dead))) break;
                     g_tc_fence_after();
-                    const uint64_t w = g_smem_desc_sw128(base + s * Tile::kStage, 0, 1024), q = g_smem_desc_sw128(base + s * Tile::kStage + kF8WeightBytes, 0, 1024);
+                    const uint64_t w = g_smem_desc_sw128(base + s * Tile::kStage, 0, 1024), // own rows: columns 8-15 are what lies behind the block, and not used
+                                   q = OWN ? g_smem_desc_sw128(own + (kb - kb0) * kF8OwnRows * kF8Block, 0, 1024) : g_smem_desc_sw128(base + s * Tile::kStage + kF8WeightBytes, 0, 1024);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) f8_mma(tmem + buf * BN, w + 2 * k, q + 2 * k, f8_idesc(BN), k > 0);
                     g_tc_commit(acc_full + 8 * buf);
@@ -143,18 +216,26 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 #pragma unroll
                 for (int i = 0; i < PER; ++i) {
                     const int c = lane + 32 * i;
-                    next[i] = c < COLS && col0 + c < a.rows ? tl::ld_cg(a.sx + (size_t)kb * a.ld_sx + col0 + c) : 0.f;
+                    if constexpr (!OWN) next[i] = c < COLS && col0 + c < a.rows ? tl::ld_cg(a.sx + (size_t)kb * a.ld_sx + col0 + c) : 0.f;
                 }
             };
             if (kb0 < kb1) fetch(kb0);
             bool ok = true;
             for (int kb = kb0; kb < kb1; ++kb) {
+                if constexpr (!OWN) {
 #pragma unroll
-                for (int i = 0; i < PER; ++i)
-                    if (lane + 32 * i < COLS) mine[lane + 32 * i] = next[i] * next_w;
-                if (kb + 1 < kb1) fetch(kb + 1);
-                __syncwarp();
-                ok &= tc_wait(acc_full + 8 * buf, acc_ph, dead);
+                    for (int i = 0; i < PER; ++i)
+                        if (lane + 32 * i < COLS) mine[lane + 32 * i] = next[i] * next_w;
+                    if (kb + 1 < kb1) fetch(kb + 1);
+                    __syncwarp();
+                    ok &= tc_wait(acc_full + 8 * buf, acc_ph, dead);
+                } else {  // the block's scales were written before its products
+                    const float this_w = next_w;
+                    if (kb + 1 < kb1) fetch(kb + 1);
+                    ok &= tc_wait(acc_full + 8 * buf, acc_ph, dead);
+                    if (lane < COLS) mine[lane] = col0 + lane < a.rows ? own_scales[(kb - kb0) * kF8OwnRows + col0 + lane] * this_w : 0.f;
+                    __syncwarp();
+                }
                 g_tc_fence_after();
                 const uint32_t at = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN + part * COLS;
 #pragma unroll
@@ -231,20 +312,24 @@ static int f8_splits(long long tiles, int k_blocks, int room) {
     return splits;
 }
 
-template <typename T, int BN>
-static int f8_launch(const F8Product &p, cudaStream_t st) {
-    using Tile = F8Tile<BN>;
+template <typename T, int BN, int ROWS = kF8Tma, typename X = T>
+static int f8_launch(const F8Product &p, cudaStream_t st, const F8Rows *x = nullptr) {
+    using Tile = F8Tile<BN, ROWS != kF8Tma>;
     static_assert(Tile::kStages >= 3 && Tile::kStages <= 8 && Tile::kStages * Tile::kStage >= BN * 128 * 4, "the sums of a split tile lie over the stages");
     CUtensorMap mw, mq;
     if (int e = tc_map_bytes(&mw, p.w, p.ldw, p.n, p.ldw, 128)) return e;
-    if (int e = tc_map_bytes(&mq, p.q, p.ldq, p.rows, p.ldq, BN)) return e;
-    F8Args a{p.sx, p.sw, p.bias, p.out, p.ld_sx, p.rows, p.n, ceil_div(p.k, kF8Block), ceil_div(p.n, 128), 0, 1};
+    if (ROWS != kF8Tma) mq = mw;  // not read
+    else if (int e = tc_map_bytes(&mq, p.q, p.ldq, p.rows, p.ldq, BN)) return e;
+    F8Args a{x ? *x : F8Rows{}, p.sx, p.sw, p.bias, p.out, p.ld_sx, p.rows, p.n, ceil_div(p.k, kF8Block), ceil_div(p.n, 128), 0, 1, ROWS != kF8Plain};
     const long long tiles = (long long)a.m_blocks * ceil_div(p.rows, BN);
     if (tiles > 0x3fffffff) return tl::fail(TL_EINVAL, "fp8_product: too large");
     a.tiles = (int)tiles;
     const int room = sm_count() * Tile::kPerSm;
     a.splits = f8_splits(tiles, a.k_blocks, room);
-    if (cudaFuncSetAttribute(fp8_product_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmem) != cudaSuccess) {
+    static tl::PerDevice ready;
+    int device = 0;
+    cudaGetDevice(&device);
+    if (!ready(device, [&] { return cudaFuncSetAttribute(fp8_product_kernel<T, BN, ROWS, X>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::kSmem) == cudaSuccess; })) {
         cudaGetLastError();
         return tl::fail(TL_ECUDA, "fp8_product: no shared memory");
     }
@@ -260,7 +345,7 @@ static int f8_launch(const F8Product &p, cudaStream_t st) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = tl::use_pdl() ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, fp8_product_kernel<T, BN>, mw, mq, a);
+    cudaLaunchKernelEx(&cfg, fp8_product_kernel<T, BN, ROWS, X>, mw, mq, a);
     TL_LAUNCH_CHECK("fp8_product");
     return TL_OK;
 }
@@ -292,6 +377,19 @@ int f8_product(const F8Product &p, cudaStream_t st) {
     if (tile == 256) return f8_pairs(p, st);
     TLB_DISPATCH(p.dtype, "fp8_product", return tile == 16 ? f8_launch<T, 16>(p, st) : tile == 32 ? f8_launch<T, 32>(p, st) : tile == 64 ? f8_launch<T, 64>(p, st)
                                                                                                                : f8_launch<T, 128>(p, st));
+    return TL_OK;
+}
+
+// The rows as they come, rounded by the product's own warps, whose blocks of a CTA have to fit beside its stages: one launch in place of two.  2560 -> 6144, us with
+// one launch and two: 1 row 7.8 and 9.0, 4 rows 8.6 and 9.3, 8 rows 10.1 and 9.5.
+bool f8_own(const F8Product &p) {
+    const int k_blocks = ceil_div(p.k, kF8Block);
+    return p.rows <= 4 && ceil_div(k_blocks, f8_splits(ceil_div(p.n, 128), k_blocks, 2 * sm_count())) <= kF8OwnBlocks;
+}
+int f8_product_own(const F8Product &p, const F8Rows &x, cudaStream_t st) {
+    if (x.gated) TLB_DISPATCH(p.dtype, "fp8_product", return (f8_launch<T, 16, kF8Gated, float>(p, st, &x)));
+    else if (x.dtype == p.dtype) TLB_DISPATCH(p.dtype, "fp8_product", return (f8_launch<T, 16, kF8Plain, T>(p, st, &x)));
+    else return (f8_launch<float, 16, kF8Plain, bf16>(p, st, &x));  // the first product of a feed-forward
     return TL_OK;
 }
 

@@ -119,12 +119,15 @@ int tlb_fp8_linear(const void *x, long long ldx, const void *w, int ldw, const f
     if (!x || !w || !sw || !out || !workspace || n <= 0 || k <= 0 || ldx < k || ldw < k || ldw % 16 || !tl::aligned16(w) || !tl::aligned16(workspace))
         return tl::fail(TL_EINVAL, "fp8_linear: bad argument");
     if (dtype != TL_F32 && dtype != TL_BF16) return tl::fail(TL_EDTYPE, "fp8_linear: dtype must be float32 or bfloat16");
-    if (workspace_bytes < f8_rows_bytes(rows, k)) return tl::fail(TL_EINVAL, "fp8_linear: workspace too small");
+    if (workspace_bytes < tlb_fp8_linear_workspace(rows, k)) return tl::fail(TL_EINVAL, "fp8_linear: workspace too small");
     const int ldq = f8_up(k, 16), ld_sx = f8_up(rows, 4);
     uint8_t *q = (uint8_t *)workspace;
     float *sx = (float *)(q + (size_t)rows * ldq);
-    if (int e = f8_rows({x, ldx, rows, k, dtype, false, 0, 0.f, 1.f, q, ldq, sx, ld_sx}, as_stream(stream))) return e;
-    return f8_product({q, sx, ldq, ld_sx, rows, (const uint8_t *)w, sw, ldw, n, k, bias, out, dtype}, as_stream(stream));
+    const F8Rows from{x, ldx, rows, k, dtype, false, 0, 0.f, 1.f, q, ldq, sx, ld_sx};
+    const F8Product product{q, sx, ldq, ld_sx, rows, (const uint8_t *)w, sw, ldw, n, k, bias, out, dtype};
+    if (f8_own(product)) return f8_product_own(product, from, as_stream(stream));
+    if (int e = f8_rows(from, as_stream(stream))) return e;
+    return f8_product(product, as_stream(stream));
 }
 
 size_t tlb_fp8_gated_mlp_workspace(int rows, int dim, int ff) {
@@ -147,16 +150,22 @@ int tlb_fp8_gated_mlp(const void *x, long long ldx, const void *w_gate_up, int l
     uint8_t *q = (uint8_t *)workspace, *q2 = q + ((f8_rows_bytes(rows, dim) + 15) & ~(size_t)15);
     float *sx = (float *)(q + (size_t)rows * f8_up(dim, 16)), *sx2 = (float *)(q2 + (size_t)rows * f8_up(ff, 16));
     float *inner = (float *)(q2 + ((f8_rows_bytes(rows, ff) + 15) & ~(size_t)15));
-    if (int e = f8_rows({x, ldx, rows, dim, dtype, false, 0, 0.f, 1.f, q, f8_up(dim, 16), sx, ld_sx}, st)) return e;
+    const F8Rows from{x, ldx, rows, dim, dtype, false, 0, 0.f, 1.f, q, f8_up(dim, 16), sx, ld_sx};
     const F8Product first{q, sx, f8_up(dim, 16), ld_sx, rows, (const uint8_t *)w_gate_up, s_gate_up, ld_gate_up, wide, dim, nullptr, inner, TL_F32};
     const F8Rows gated{inner, wide, rows, ff, TL_F32, true, act, limit, slope, q2, f8_up(ff, 16), sx2, ld_sx};
+    const F8Product second{q2, sx2, f8_up(ff, 16), ld_sx, rows, (const uint8_t *)w_down, s_down, ld_down, dim, ff, nullptr, out, dtype};
+    if (f8_own(first) && f8_own(second)) {
+        if (int e = f8_product_own(first, from, st)) return e;
+        return f8_product_own(second, gated, st);
+    }
+    if (int e = f8_rows(from, st)) return e;
     if (rows > kF8Fused) {
         if (int e = f8_pairs_gated(first, gated, st)) return e;
     } else {
         if (int e = f8_product(first, st)) return e;
         if (int e = f8_rows(gated, st)) return e;
     }
-    return f8_product({q2, sx2, f8_up(ff, 16), ld_sx, rows, (const uint8_t *)w_down, s_down, ld_down, dim, ff, nullptr, out, dtype}, st);
+    return f8_product(second, st);
 }
 
 }  // extern "C"

@@ -814,31 +814,30 @@ size_t tlb_moe_few_workspace(int tokens, int top, int experts, int ff) {
     return tokens <= 0 || top <= 0 || experts <= 0 || ff <= 0 ? 0 : few_bytes(tokens, top, experts, ff);
 }
 
-int tlb_moe_few(const void *x, const void *router, const void *router_bias, const void *choice_bias, const void *side_w, int tokens, int dim, int outputs, int experts,
-                int top, int scoring, float weight_scale, int group_count, int group_keep, const void *w_gate, const void *w_up, const void *w_down, const float *s_gate,
-                const float *s_up, const float *s_down, int fp8, int ff, int ld_in, int ld_out, int act, float limit, float slope, const void *shared, void *out, int out_f32,
-                void *workspace, size_t workspace_bytes, void *stream) {
+int tlb_moe_few(const tlb_moe_few_layer *l, const void *x, int tokens, const void *shared, void *out, int out_f32, void *workspace, size_t workspace_bytes, void *stream) {
     if (tokens <= 0) return TL_OK;
-    if (!x || !router || !w_up || !w_down || !out || !workspace || ff <= 0 || ff > (1 << 20) || scoring < 0 || scoring > 2 || (side_w && !shared))
+    if (!l || !x || !l->router || !l->w_up || !l->w_down || !out || !workspace || l->ff <= 0 || l->ff > (1 << 20) || l->scoring < 0 || l->scoring > 2 || (l->side_w && !shared))
         return tl::fail(TL_EINVAL, "moe_few: bad argument");
-    if (tokens > tlb_moe_few_tokens(dim, outputs, experts, top, group_count, fp8)) return tl::fail(TL_EINVAL, "moe_few: %d tokens are too many for these sizes", tokens);
-    if (group_keep < 0 || group_keep > group_count || (group_count > 0 && (outputs % group_count || group_keep * (outputs / group_count) < top)))
+    const int dim = l->dim, ff = l->ff, top = l->top, experts = l->experts, outputs = l->outputs, groups = l->group_count, fp8 = l->fp8, size = fp8 ? 1 : 2;
+    if (tokens > tlb_moe_few_tokens(dim, outputs, experts, top, groups, fp8)) return tl::fail(TL_EINVAL, "moe_few: %d tokens are too many for these sizes", tokens);
+    if (l->group_keep < 0 || l->group_keep > groups || (groups > 0 && (outputs % groups || l->group_keep * (outputs / groups) < top)))
         return tl::fail(TL_EINVAL, "moe_few: bad groups");
-    if (w_gate ? (act != 0 && act != 1 && act != 3) || (act == 3 && !(limit > 0.f)) : act < 0 || act > 2) return tl::fail(TL_EINVAL, "moe_few: bad activation");
-    if (fp8 && (!s_up || !s_down || (w_gate && !s_gate))) return tl::fail(TL_EINVAL, "moe_few: 8-bit weights without scales");
-    const int size = fp8 ? 1 : 2;
-    if (dim % 8 || ld_in < dim * size || ld_out < ff * size || ld_in % 16 || ld_out % 16 || !tl::aligned16(x) || !tl::aligned16(router) || (side_w && !tl::aligned16(side_w)) ||
-        (w_gate && !tl::aligned16(w_gate)) || !tl::aligned16(w_up) || !tl::aligned16(w_down) || !tl::aligned16(workspace))
+    if (l->w_gate ? (l->act != 0 && l->act != 1 && l->act != 3) || (l->act == 3 && !(l->limit > 0.f)) : l->act < 0 || l->act > 2)
+        return tl::fail(TL_EINVAL, "moe_few: bad activation");
+    if (fp8 && (!l->s_up || !l->s_down || (l->w_gate && !l->s_gate))) return tl::fail(TL_EINVAL, "moe_few: 8-bit weights without scales");
+    if (dim % 8 || l->ld_in < dim * size || l->ld_out < ff * size || l->ld_in % 16 || l->ld_out % 16 || !tl::aligned16(x) || !tl::aligned16(l->router) ||
+        !tl::aligned16(l->side_w) || !tl::aligned16(l->w_gate) || !tl::aligned16(l->w_up) || !tl::aligned16(l->w_down) || !tl::aligned16(workspace))
         return tl::fail(TL_EINVAL, "moe_few: rows must be whole 16-byte pieces");
     if (workspace_bytes < few_bytes(tokens, top, experts, ff)) return tl::fail(TL_EINVAL, "moe_few: workspace too small");
     const size_t pairs = (size_t)tokens * top;
     FewArgs a{};
-    a.x = (const bf16 *)x, a.router = (const bf16 *)router, a.router_bias = (const bf16 *)router_bias, a.choice_bias = (const bf16 *)choice_bias, a.side_w = (const bf16 *)side_w;
-    a.tokens = tokens, a.dim = dim, a.outputs = outputs, a.experts = experts, a.top = top, a.scoring = scoring, a.group_count = group_count, a.group_keep = group_keep;
-    a.weight_scale = weight_scale;
-    a.w0 = (const uint8_t *)(w_gate ? w_gate : w_up), a.w1 = (const uint8_t *)(w_gate ? w_up : nullptr), a.w2 = (const uint8_t *)w_down;
-    a.s0 = w_gate ? s_gate : s_up, a.s1 = w_gate ? s_up : nullptr, a.s2 = s_down;
-    a.ff = ff, a.ld_in = ld_in, a.ld_out = ld_out, a.bytes_in = (int)few_align((size_t)dim * size), a.bytes_out = (int)few_align((size_t)ff * size), a.act = act, a.limit = limit, a.slope = slope, a.shared = (const bf16 *)shared, a.out = out;
+    a.x = (const bf16 *)x, a.router = (const bf16 *)l->router, a.router_bias = (const bf16 *)l->router_bias, a.choice_bias = (const bf16 *)l->choice_bias;
+    a.side_w = (const bf16 *)l->side_w, a.tokens = tokens, a.dim = dim, a.outputs = outputs, a.experts = experts, a.top = top, a.scoring = l->scoring, a.group_count = groups;
+    a.group_keep = l->group_keep, a.weight_scale = l->weight_scale;
+    a.w0 = (const uint8_t *)(l->w_gate ? l->w_gate : l->w_up), a.w1 = (const uint8_t *)(l->w_gate ? l->w_up : nullptr), a.w2 = (const uint8_t *)l->w_down;
+    a.s0 = l->w_gate ? l->s_gate : l->s_up, a.s1 = l->w_gate ? l->s_up : nullptr, a.s2 = l->s_down;
+    a.ff = ff, a.ld_in = l->ld_in, a.ld_out = l->ld_out, a.bytes_in = (int)few_align((size_t)dim * size), a.bytes_out = (int)few_align((size_t)ff * size);
+    a.act = l->act, a.limit = l->limit, a.slope = l->slope, a.shared = (const bf16 *)shared, a.out = out;
     uint8_t *at = (uint8_t *)workspace;
     a.idx = (int32_t *)at, at += few_align(pairs * 4);
     a.gate = (float *)at, at += few_align(pairs * 4);
@@ -846,7 +845,7 @@ int tlb_moe_few(const void *x, const void *router, const void *router_bias, cons
     a.inner = (float *)at, a.ld_inner = few_inner_ld(ff), at += pairs * a.ld_inner * 4;
     a.most = (float *)at, a.runs = few_grid() * kFewTeams, a.room = kFewSmem;
     a.prefetch = kFewPrefetch / few_grid();
-    const int nt = few_nt(tokens), smem = FewFirstSmem(tokens, nt, dim, outputs, experts, top, group_count, fp8 != 0, kFewSmem).total;
+    const int nt = few_nt(tokens), smem = FewFirstSmem(tokens, nt, dim, outputs, experts, top, groups, fp8 != 0, kFewSmem).total;
     const cudaStream_t st = as_stream(stream);
     if (fp8) return nt == 1 ? few_run<true, 1>(a, smem, out_f32, st) : nt == 2 ? few_run<true, 2>(a, smem, out_f32, st) : few_run<true, 4>(a, smem, out_f32, st);
     return nt == 1 ? few_run<false, 1>(a, smem, out_f32, st) : nt == 2 ? few_run<false, 2>(a, smem, out_f32, st) : few_run<false, 4>(a, smem, out_f32, st);

@@ -7,7 +7,6 @@ The library is built on first use when it is missing (a handful of translation u
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import importlib.util
 import os
@@ -95,8 +94,7 @@ _SIGNATURES = {
     "tlb_argmax_rows": (_I, [_VP, _VP, _I, _I, _VP]),
     "tlb_moe_few_tokens": (_I, [_I, _I, _I, _I, _I, _I]),
     "tlb_moe_few_workspace": (ctypes.c_size_t, [_I, _I, _I, _I]),
-    "tlb_moe_few": (_I, [_VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _F, _I, _I, _VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _F, _F, _VP, _VP, _I, _VP,
-                         ctypes.c_size_t, _VP]),
+    "tlb_moe_few": (_I, [_VP, _VP, _I, _VP, _VP, _I, _VP, ctypes.c_size_t, _VP]),
     "tlb_fp8_linear_workspace": (ctypes.c_size_t, [_I, _I]),
     "tlb_fp8_linear": (_I, [_VP, _LL, _VP, _I, _VP, _VP, _VP, _I, _I, _I, _VP, ctypes.c_size_t, _I, _VP]),
     "tlb_fp8_gated_mlp_workspace": (ctypes.c_size_t, [_I, _I, _I]),
@@ -1085,41 +1083,51 @@ def shift_mix(h, mu, *, seq_info, state, max_tokens: int):
     return out
 
 
-def _rows_of(op: str, x: torch.Tensor, width: int, device) -> torch.Tensor:
+def _rows_of(op: str, x: torch.Tensor, width: int, device: int) -> torch.Tensor:
     """``x`` as a matrix of rows with unit inner stride on the weights' device."""
     if x.shape[-1] != width:
         raise RuntimeError(f"{op}: rows of {x.shape[-1]} for weights of {width} columns")
-    if not x.is_cuda or x.device != device:
+    if x.get_device() != device or device < 0:
         raise RuntimeError(f"{op}: the blocks extension is GPU-only, and rows and weights must be on one device")
-    rows = x if x.dim() == 2 else x.reshape(-1, width)
-    return rows if rows.stride(1) == 1 and rows.stride(0) >= width or rows.shape[0] <= 1 and rows.stride(1) == 1 else rows.contiguous()
+    if x.dim() != 2:
+        x = x.reshape(-1, width)
+    return x if x.is_contiguous() or (x.stride(1) == 1 and x.stride(0) >= width) else x.contiguous()
 
 
-class _on:
-    """Launches go to the tensors' device, whichever is current."""
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
-    def __new__(cls, device):
-        return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+def _on_device(device: int, call):
+    """``call()`` with ``device`` as the current one: launches go to the tensors' device."""
+    if _current_device() == device:
+        return call()
+    with torch.cuda.device(device):
+        return call()
 
 
 def fp8_linear(x: torch.Tensor, values: torch.Tensor, scales: torch.Tensor, width: int, bias=None) -> torch.Tensor:
     """``x [.., width]`` (bf16 or fp32; rows may be apart) times ``values [N, >= width]`` (e4m3, rows of a multiple of 16 bytes,
     zero behind ``width``) with ``scales [ceil(N / 128), ceil(width / 128)]`` fp32, plus ``bias [N]`` -> ``[.., N]`` in ``x``'s dtype.  The rows are
     rounded to e4m3 with a scale for each run of 128, see ``tlb_fp8_linear``."""
-    n = values.shape[0]
-    rows = _rows_of("fp8_linear", x, width, values.device)
-    if bias is not None and (bias.shape != (n,) or bias.dtype != x.dtype or bias.device != values.device or not bias.is_contiguous()):
+    device = values.get_device()
+    rows = _rows_of("fp8_linear", x, width, device)
+    n, ld = values.shape[0], values.stride(0)
+    if bias is not None and (bias.shape != (n,) or bias.dtype != x.dtype or bias.get_device() != device or not bias.is_contiguous()):
         raise RuntimeError("fp8_linear: bias must be [outputs] of the rows' dtype")
     code, T = _code(x.dtype), rows.shape[0]
-    lib = library()
-    with _on(values.device):
-        out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=values.device)
+
+    def call():
+        out = rows.new_empty((T, n))
         if T:
+            lib = library()
             size = lib.tlb_fp8_linear_workspace(T, width)
-            scratch = torch.empty(size, dtype=torch.uint8, device=values.device)
-            _check(lib.tlb_fp8_linear(rows.data_ptr(), max(rows.stride(0), width), values.data_ptr(), values.stride(0), scales.data_ptr(), _ptr(bias), out.data_ptr(), T, n,
-                                      width, scratch.data_ptr(), size, code, _stream(values)))
-    return out
+            scratch = rows.new_empty(size, dtype=torch.uint8)
+            _check(lib.tlb_fp8_linear(rows.data_ptr(), max(rows.stride(0), width), values.data_ptr(), ld, scales.data_ptr(), _ptr(bias), out.data_ptr(), T, n, width,
+                                      scratch.data_ptr(), size, code, _raw_stream(device)))
+        return out
+
+    out = _on_device(device, call)
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], n)
 
 
 def fp8_gated_mlp(x: torch.Tensor, gate_up, down, width: int, inner: int, act: int, limit: float = 0.0, slope: float = 1.0) -> torch.Tensor:
@@ -1127,17 +1135,22 @@ def fp8_gated_mlp(x: torch.Tensor, gate_up, down, width: int, inner: int, act: i
     (values ``[2 * 128 * ceil(inner / 128), ..]``, scales): runs of 128 rows of the gate and of the up projection in turn, zero behind
     ``inner``; ``down`` = (values ``[width, ..]``, scales).  ``limit`` and ``slope`` go with ``ACT_CLAMPED_SWISH``."""
     (wg, sg), (wd, sd) = gate_up, down
-    rows = _rows_of("fp8_gated_mlp", x, width, wg.device)
+    device = wg.get_device()
+    rows = _rows_of("fp8_gated_mlp", x, width, device)
     code, T = _code(x.dtype), rows.shape[0]
-    lib = library()
-    with _on(wg.device):
-        out = torch.empty((*x.shape[:-1], wd.shape[0]), dtype=x.dtype, device=wg.device)
+
+    def call():
+        out = rows.new_empty((T, width))
         if T:
+            lib = library()
             size = lib.tlb_fp8_gated_mlp_workspace(T, width, inner)
-            scratch = torch.empty(size, dtype=torch.uint8, device=wg.device)
+            scratch = rows.new_empty(size, dtype=torch.uint8)
             _check(lib.tlb_fp8_gated_mlp(rows.data_ptr(), max(rows.stride(0), width), wg.data_ptr(), wg.stride(0), sg.data_ptr(), wd.data_ptr(), wd.stride(0), sd.data_ptr(),
-                                         out.data_ptr(), T, width, inner, act, float(limit), float(slope), scratch.data_ptr(), size, code, _stream(wg)))
-    return out
+                                         out.data_ptr(), T, width, inner, act, limit, slope, scratch.data_ptr(), size, code, _raw_stream(device)))
+        return out
+
+    out = _on_device(device, call)
+    return out if x.dim() == 2 else out.view(x.shape)
 
 
 def moe_few_tokens(dim: int, outputs: int, experts: int, top: int, group_count: int = 0, fp8: bool = False) -> int:
@@ -1145,44 +1158,68 @@ def moe_few_tokens(dim: int, outputs: int, experts: int, top: int, group_count: 
     return int(library().tlb_moe_few_tokens(dim, outputs, experts, top, group_count, int(fp8)))
 
 
-def moe_few(h, router_w, router_b, top: int, w_gate, w_up, w_down, act: int, *, scales=None, inner: int, scoring: int = SCORE_SOFTMAX, choice_bias=None,
-            weight_scale: float = 1.0, groups=(0, 0), side_w=None, limit: float = 0.0, slope: float = 1.0, shared=None, wide: bool = False) -> torch.Tensor:
-    """A mixture-of-experts layer for a few bf16 tokens ``h [T, D]`` in two launches -> ``[T, D]`` bf16, or (``wide``) fp32.  The router's arguments are those
-    of ``moe_route``; ``w_gate`` (or None), ``w_up [E, inner, ..]``, ``w_down [E, D, ..]`` bf16, or e4m3 with ``scales`` = (gate's, up's, down's): rows of whole
-    16-byte pieces, zero behind the last number.  Outputs of the router from ``E`` up are identity experts.  ``shared [T, D]`` is added, times
-    ``sigmoid(side_w . h)`` with ``side_w``."""
-    _gpu("moe_few", h, router_w, router_b, choice_bias, side_w, w_gate, w_up, w_down, shared)
-    _contig("moe_few", h, router_w, router_b, choice_bias, side_w, w_gate, w_up, w_down, shared)
-    T, D = h.shape
-    fp8 = scales is not None
-    E, size = w_up.shape[0], w_up.element_size()
-    for t in (h, router_w, router_b, choice_bias, side_w, shared):
-        if t is not None and t.dtype != torch.bfloat16:
-            raise RuntimeError("moe_few: activations, router and shared rows must be bfloat16")
-    if any(w is not None and w.dtype != (torch.float8_e4m3fn if fp8 else torch.bfloat16) for w in (w_gate, w_up, w_down)):
-        raise RuntimeError("moe_few: experts must be bfloat16, or float8_e4m3fn with scales")
-    if router_w.shape[1] != D or (router_b is not None and router_b.numel() != router_w.shape[0]) or (choice_bias is not None and choice_bias.numel() != router_w.shape[0]):
-        raise RuntimeError("moe_few: router must be [outputs, D], its biases [outputs]")
-    if (side_w is not None and (side_w.numel() != D or shared is None)) or (shared is not None and shared.shape != h.shape):
-        raise RuntimeError("moe_few: shared must be [T, D], side_w [1, D] with it")
-    if w_up.dim() != 3 or w_up.shape[1] != inner or w_up.shape[2] < D or w_down.dim() != 3 or w_down.shape[:2] != (E, D) or w_down.shape[2] < inner or (
-            w_gate is not None and w_gate.shape != w_up.shape):
-        raise RuntimeError("moe_few: experts must be [E, inner, >= D] and [E, D, >= inner]")
-    sg, su, sd = scales if fp8 else (None, None, None)
-    blocks_of = lambda n, k: (E, -(-n // 128), -(-k // 128))  # noqa: E731
-    for s, shape in ((sg, blocks_of(inner, D)), (su, blocks_of(inner, D)), (sd, blocks_of(D, inner))) if fp8 else ():
-        if s is not None and (s.dtype != torch.float32 or tuple(s.shape) != shape or not s.is_contiguous() or not s.is_cuda):
-            raise RuntimeError("moe_few: scales must be float32, one for each block of 128 x 128")
-    if len({t.device for t in (h, router_w, router_b, choice_bias, side_w, w_gate, w_up, w_down, shared, sg, su, sd) if t is not None}) != 1:
-        raise RuntimeError("moe_few: tensors on two devices")
-    lib = library()
-    with _on(h.device):
-        out = torch.empty((T, D), dtype=torch.float32 if wide else torch.bfloat16, device=h.device)
-        if T:
-            size_ws = lib.tlb_moe_few_workspace(T, top, E, inner)
-            scratch = torch.empty(size_ws, dtype=torch.uint8, device=h.device)
-            _check(lib.tlb_moe_few(h.data_ptr(), router_w.data_ptr(), _ptr(router_b), _ptr(choice_bias), _ptr(side_w), T, D, router_w.shape[0], E, top, int(scoring),
-                                   float(weight_scale), int(groups[0]), int(groups[1]), _ptr(w_gate), w_up.data_ptr(), w_down.data_ptr(), _ptr(sg), _ptr(su), _ptr(sd),
-                                   int(fp8), inner, w_up.shape[2] * size, w_down.shape[2] * size, act, float(limit), float(slope), _ptr(shared), out.data_ptr(), int(wide),
-                                   scratch.data_ptr(), size_ws, _stream(h)))
-    return out
+class FewLayer(ctypes.Structure):
+    """``tlb_moe_few_layer``"""
+
+    _fields_ = [("router", _VP), ("router_bias", _VP), ("choice_bias", _VP), ("side_w", _VP), ("w_gate", _VP), ("w_up", _VP), ("w_down", _VP), ("s_gate", _VP), ("s_up", _VP),
+                ("s_down", _VP), ("dim", _I), ("outputs", _I), ("experts", _I), ("top", _I), ("scoring", _I), ("group_count", _I), ("group_keep", _I), ("fp8", _I), ("ff", _I),
+                ("ld_in", _I), ("ld_out", _I), ("act", _I), ("weight_scale", _F), ("limit", _F), ("slope", _F)]
+
+
+class MoeFew:
+    """A mixture-of-experts layer for a few bf16 tokens in two launches.  The router's arguments are those of ``moe_route``; ``w_gate`` (or None),
+    ``w_up [E, inner, ..]``, ``w_down [E, D, ..]`` bf16, or e4m3 with ``scales`` = (gate's, up's, down's): rows of whole 16-byte pieces, zero behind the last
+    number.  Outputs of the router from ``E`` up are identity experts.  The tensors are kept and must stay where they are."""
+
+    def __init__(self, router_w, router_b, top: int, w_gate, w_up, w_down, act: int, *, scales=None, inner: int, scoring: int = SCORE_SOFTMAX, choice_bias=None,
+                 weight_scale: float = 1.0, groups=(0, 0), side_w=None, limit: float = 0.0, slope: float = 1.0):
+        _gpu("moe_few", router_w, router_b, choice_bias, side_w, w_gate, w_up, w_down)
+        _contig("moe_few", router_w, router_b, choice_bias, side_w, w_gate, w_up, w_down)
+        fp8, size = scales is not None, w_up.element_size()
+        (outputs, D), E = router_w.shape, w_up.shape[0]
+        if any(t is not None and t.dtype != torch.bfloat16 for t in (router_w, router_b, choice_bias, side_w)):
+            raise RuntimeError("moe_few: the router must be bfloat16")
+        if any(w is not None and w.dtype != (torch.float8_e4m3fn if fp8 else torch.bfloat16) for w in (w_gate, w_up, w_down)):
+            raise RuntimeError("moe_few: experts must be bfloat16, or float8_e4m3fn with scales")
+        if any(b is not None and b.numel() != outputs for b in (router_b, choice_bias)) or (side_w is not None and side_w.numel() != D):
+            raise RuntimeError("moe_few: router must be [outputs, D], its biases [outputs], side_w [1, D]")
+        if w_up.dim() != 3 or w_up.shape[1] != inner or w_up.shape[2] < D or w_down.dim() != 3 or w_down.shape[:2] != (E, D) or w_down.shape[2] < inner or (
+                w_gate is not None and w_gate.shape != w_up.shape):
+            raise RuntimeError("moe_few: experts must be [E, inner, >= D] and [E, D, >= inner]")
+        sg, su, sd = scales if fp8 else (None, None, None)
+        blocks_of = lambda n, k: (E, -(-n // 128), -(-k // 128))  # noqa: E731
+        if fp8 and (su is None or sd is None or (sg is None) != (w_gate is None)):
+            raise RuntimeError("moe_few: scales of every matrix")
+        for s, shape in ((sg, blocks_of(inner, D)), (su, blocks_of(inner, D)), (sd, blocks_of(D, inner))):
+            if s is not None and (s.dtype != torch.float32 or tuple(s.shape) != shape or not s.is_contiguous()):
+                raise RuntimeError("moe_few: scales must be float32, one for each block of 128 x 128")
+        self._keep = (router_w, router_b, choice_bias, side_w, w_gate, w_up, w_down, sg, su, sd)
+        if len({t.device for t in self._keep if t is not None}) != 1:
+            raise RuntimeError("moe_few: tensors on two devices")
+        self.device, self.width = router_w.get_device(), D
+        self.tokens = moe_few_tokens(D, outputs, E, top, int(groups[0]), fp8)
+        self.workspace = lambda T: library().tlb_moe_few_workspace(T, top, E, inner)
+        self.layer = FewLayer(*(_ptr(t) for t in self._keep), D, outputs, E, top, int(scoring), int(groups[0]), int(groups[1]), int(fp8), inner, w_up.shape[2] * size,
+                              w_down.shape[2] * size, act, float(weight_scale), float(limit), float(slope))
+        self._layer = ctypes.addressof(self.layer)
+
+    def __call__(self, h: torch.Tensor, shared=None, wide: bool = False) -> torch.Tensor:
+        """``h [T, D]`` of at most ``tokens`` rows -> ``[T, D]`` bf16, or (``wide``) the fp32 sums.  ``shared [T, D]`` is added, times ``sigmoid(side_w . h)``
+        with ``side_w``."""
+        T = h.shape[0]
+        if h.dtype != torch.bfloat16 or h.dim() != 2 or h.shape[1] != self.width or not h.is_contiguous() or h.get_device() != self.device:
+            raise RuntimeError(f"moe_few: tokens must be contiguous bfloat16 [T, {self.width}] on the experts' device")
+        if shared is not None and (shared.dtype != torch.bfloat16 or shared.shape != h.shape or not shared.is_contiguous() or shared.get_device() != self.device):
+            raise RuntimeError("moe_few: shared must be contiguous bfloat16 [T, D] on the experts' device")
+        if T > self.tokens:
+            raise RuntimeError(f"moe_few: {T} tokens, at most {self.tokens} at these sizes")
+
+        def call():
+            out = h.new_empty((T, self.width), dtype=torch.float32) if wide else torch.empty_like(h)
+            if T:
+                size = self.workspace(T)
+                scratch = h.new_empty(size, dtype=torch.uint8)
+                _check(library().tlb_moe_few(self._layer, h.data_ptr(), T, _ptr(shared), out.data_ptr(), wide, scratch.data_ptr(), size, _raw_stream(self.device)))
+            return out
+
+        return _on_device(self.device, call)

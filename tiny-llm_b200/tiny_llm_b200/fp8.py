@@ -8,6 +8,8 @@ from __future__ import annotations
 
 import torch
 
+from extensions_b200.tiny_llm_ext_b200 import blocks
+
 BLOCK = 128
 LARGEST = 448.0  # of the e4m3 numbers
 
@@ -72,8 +74,6 @@ class Fp8Weights:
 
 def fp8_linear(x: torch.Tensor, w: Fp8Weights, bias: torch.Tensor | None = None) -> torch.Tensor:
     """``x [.., K]`` (bf16 or fp32) times the transposed matrix -> ``[.., N]`` in ``x``'s dtype, any number of rows from none up."""
-    from extensions_b200.tiny_llm_ext_b200 import blocks
-
     if len(w.shape) != 2:
         raise ValueError("fp8_linear: one matrix, not a stack")
     return blocks.fp8_linear(x, w.values, w.scales, w.shape[1], bias)

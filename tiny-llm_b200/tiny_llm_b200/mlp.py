@@ -66,6 +66,8 @@ class Fp8GatedMLP:
     they are rounded as the input's are.  ``act``, ``limit``, ``slope``: see ``GatedMLP``."""
 
     def __init__(self, w_gate, w_up, w_down, act: str, limit: float = 0.0, slope: float = 1.0):
+        from extensions_b200.tiny_llm_ext_b200 import blocks
+
         from .fp8 import Fp8Weights, interleaved
 
         if not all(isinstance(w, Fp8Weights) and len(w.shape) == 2 for w in (w_gate, w_up, w_down)):
@@ -75,16 +77,13 @@ class Fp8GatedMLP:
         if act not in ("silu", "gelu_tanh", "clamped_swish"):
             raise ValueError(f"Fp8GatedMLP: no gated activation {act!r}")
         self.inner_width, self.width = w_up.shape
-        self.w_gate_up, self.s_gate_up = interleaved(w_gate, w_up)
-        self.w_down, self.s_down = w_down.values, w_down.scales
+        self.gate_up, self.down, self._blocks = interleaved(w_gate, w_up), (w_down.values, w_down.scales), blocks
         self.act, self.limit, self.slope = ACTIVATIONS[act], float(limit), float(slope)
         if act == "clamped_swish" and not self.limit > 0:
             raise ValueError("Fp8GatedMLP: the clamped activation needs a positive limit")
 
     def __call__(self, h: torch.Tensor) -> torch.Tensor:
-        from extensions_b200.tiny_llm_ext_b200 import blocks
-
-        return blocks.fp8_gated_mlp(h, (self.w_gate_up, self.s_gate_up), (self.w_down, self.s_down), self.width, self.inner_width, self.act, self.limit, self.slope)
+        return self._blocks.fp8_gated_mlp(h, self.gate_up, self.down, self.width, self.inner_width, self.act, self.limit, self.slope)
 
 
 class TopKRouter:
@@ -198,34 +197,31 @@ class FewTokenExperts:
             raise ValueError("FewTokenExperts: a shared gate of [1, width] goes with a shared expert")
         if len({w.device for w in (*weights, router.weight)}) != 1:
             raise ValueError("FewTokenExperts: router and experts on two devices")
-        self.router, self.shared, self.width, self.inner_width = router, shared, D, ff
-        self.act, self.limit, self.slope = ACTIVATIONS[act], float(limit), float(slope)
+        self.router, self.shared, self.width = router, shared, D
         self._pad = -D % 8
         rows = D + self._pad
         raw = lambda w, n: None if w is None else _whole_rows(w.values if fp8 else w.contiguous(), n)  # noqa: E731
-        self.w_gate, self.w_up, self.w_down = raw(w_gate, ff), raw(w_up, ff), raw(w_down, rows)
-        self.scales = None if not fp8 else tuple(None if w is None else w.scales for w in (w_gate, w_up, w_down))
         wider = lambda t: t if t is None or not self._pad else torch.nn.functional.pad(t.reshape(-1, D), (0, self._pad)).contiguous()  # noqa: E731
-        self.router_w = wider(router.weight)
-        self.shared_gate = None if shared_gate is None else wider(shared_gate.contiguous())
-        self.run = blocks.moe_few_tokens(rows, E + identity, E, router.top, router.groups[0], fp8) if w_up.device.type == "cuda" else 0
-        if w_up.device.type == "cuda" and self.run == 0:
+        self._few = blocks.MoeFew(wider(router.weight), router.bias, router.top, raw(w_gate, ff), raw(w_up, ff), raw(w_down, rows), ACTIVATIONS[act],
+                                  scales=None if not fp8 else tuple(None if w is None else w.scales for w in (w_gate, w_up, w_down)), inner=ff, scoring=router.scoring,
+                                  choice_bias=router.choice_bias, weight_scale=router.weight_scale, groups=router.groups,
+                                  side_w=None if shared_gate is None else wider(shared_gate.contiguous()), limit=limit, slope=slope)
+        self.run = self._few.tokens
+        if self.run == 0:
             raise ValueError(f"FewTokenExperts: width {D}, {E + identity} router outputs and {router.top} choices do not fit")
 
     def __call__(self, h: torch.Tensor, wide: bool = False) -> torch.Tensor:
         """``h [T, D]`` bf16 -> ``[T, D]`` bf16, or with ``wide`` the fp32 sums."""
-        from extensions_b200.tiny_llm_ext_b200 import blocks
-
-        if h.dim() != 2 or h.shape[1] != self.width or h.dtype != torch.bfloat16:
-            raise RuntimeError(f"FewTokenExperts: expected bfloat16 [tokens, {self.width}]")
         shared = None if self.shared is None else self.shared(h)
         if self._pad:
+            if h.dim() != 2 or h.shape[1] != self.width:
+                raise RuntimeError(f"FewTokenExperts: expected bfloat16 [tokens, {self.width}]")
             h, shared = (None if t is None else torch.nn.functional.pad(t, (0, self._pad)) for t in (h, shared))
-        h = h.contiguous() if h.data_ptr() % 16 == 0 else h.clone(memory_format=torch.contiguous_format)
-        r = self.router
-        parts = [blocks.moe_few(h[t : t + self.run], self.router_w, r.bias, r.top, self.w_gate, self.w_up, self.w_down, self.act, scales=self.scales, inner=self.inner_width,
-                                scoring=r.scoring, choice_bias=r.choice_bias, weight_scale=r.weight_scale, groups=r.groups, side_w=self.shared_gate, limit=self.limit,
-                                slope=self.slope, shared=None if shared is None else shared[t : t + self.run], wide=wide)
-                 for t in range(0, max(1, h.shape[0]), max(1, self.run))]
-        y = parts[0] if len(parts) == 1 else torch.cat(parts)
+        if not h.is_contiguous() or h.data_ptr() % 16:
+            h = h.clone(memory_format=torch.contiguous_format)
+        T = h.shape[0]
+        if T <= self.run:
+            y = self._few(h, shared, wide)
+        else:
+            y = torch.cat([self._few(h[t : t + self.run], None if shared is None else shared[t : t + self.run], wide) for t in range(0, T, self.run)])
         return y[:, : self.width] if self._pad else y
