@@ -64,16 +64,30 @@ __device__ __forceinline__ void moe_choose(float *z, float *p_all, float *best, 
         const uint32_t u = __float_as_uint(v + 0.f);
         return v != v ? 0u : u & 0x80000000u ? ~u : u | 0x80000000u;
     };
+    constexpr int KEPT = 4;  // outputs of a lane that stay in registers: up to 128 of them
+    uint32_t kept[KEPT];
+    const bool keep = experts <= 32 * KEPT;
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i) kept[i] = keep && lane + 32 * i < experts ? ordered(z[lane + 32 * i]) : 0;
     for (int k = 0; k < top; ++k) {
         uint32_t best_v = 0;
         int bi = 0x7fffffff;
-        for (int e = lane; e < experts; e += 32) {
-            const uint32_t v = ordered(z[e]);
-            if (v > best_v) best_v = v, bi = e;
+        if (keep) {
+#pragma unroll
+            for (int i = 0; i < KEPT; ++i)
+                if (kept[i] > best_v) best_v = kept[i], bi = lane + 32 * i;
+        } else {
+            for (int e = lane; e < experts; e += 32) {
+                const uint32_t v = ordered(z[e]);
+                if (v > best_v) best_v = v, bi = e;
+            }
         }
         const uint32_t most = __reduce_max_sync(0xffffffffu, best_v);
         bi = __reduce_min_sync(0xffffffffu, best_v == most && most ? bi : 0x7fffffff);
         const float bv = most ? __uint_as_float(most & 0x80000000u ? most & 0x7fffffffu : ~most) : -INFINITY;
+#pragma unroll
+        for (int i = 0; i < KEPT; ++i)
+            if (bi == lane + 32 * i) kept[i] = ordered(-INFINITY);
         if (k == 0) first_v = bv;
         // scoring 0: softmax over the chosen logits (the first choice is the largest); 1: each choice's own sigmoid, as it is
         float p = scoring == 1 ? 1.0f / (1.0f + expf(-bv)) : scoring == 2 ? p_all[min(bi, experts - 1)] : expf(bv - first_v);

@@ -12,8 +12,8 @@
 // Order of the reduction index: a lane holds 16 consecutive bytes of a row (one load), which is what it contributes to the products' k index,
 // of both operands alike; no operand is ever shuffled.
 //
-// e4m3 numbers become fp16 exactly; then x (a power of two for each token) and the inner rows (a power of two for each pair, from the largest
-// magnitude that the first launch leaves) are fp16 as well, off by 2^-11 of the value or 2^-24 of the row's largest (x's own numbers of 8 bits only by the latter).  bf16
+// e4m3 numbers become fp16 exactly; then x (a power of two for each token) and the inner rows (a power of two for each block of 128)
+// are fp16 as well, off by 2^-11 of the value or 2^-24 of the row's or block's largest (x's own numbers of 8 bits only by the latter).  bf16
 // numbers meet bf16 ones: x is as it came, and an inner row is two bf16 terms, off by 2^-16.  Sums are fp32 throughout; with 8 bits the 128 of a block are added before their scale multiplies them.
 //
 // No CTA waits for another outside its cluster: the cluster's CTAs share the router's rows, exchange the logits through shared memory, and every
@@ -47,7 +47,6 @@ struct FewArgs {
     float *gate;       // [tokens, top]
     float *side;       // [tokens]
     float *inner;      // [tokens * top, ld_inner], zero behind ff
-    float *most;       // e4m3: [(run of features) + (position of the expert)][32], the largest magnitude of a token's inner row in that run
     int ld_inner, runs;  // runs of features: teams of the first launch
     int room;            // bytes of shared memory that a launch may use
     int prefetch;        // bytes that a CTA of the first launch asks into L2 for the second
@@ -86,68 +85,66 @@ __device__ __forceinline__ int few_exponent(float most) {
 }
 __device__ __forceinline__ float few_exp2(int e) { return __int_as_float((e + 127) << 23); }
 
-// A warp's piece of 16 rows: 128 bytes of each.  A lane has rows g = lane / 4 and g + 8, 16 bytes at t * 16 (t = lane % 4) of either half: it asks for exactly
-// what it will use (cp.async), into places of its own, so a piece is waited for by counting one's own copies, without a barrier.
+// A warp's piece of 16 rows, 128 bytes of each: four copies of four whole lines (cp.async) into a place of the warp's own, so that a piece is waited for by
+// counting one's copies, without a barrier of the CTA.  Behind it the scales of rows 0-7 and 8-15.  A lane then has rows g = lane / 4 and g + 8, 16 bytes at
+// t * 16 (t = lane % 4) of either half; odd rows keep their halves exchanged, which spares those reads bank conflicts.
 struct FewPiece {
     uint4 a[2], b[2];  // rows g, g + 8
-    float sa, sb;      // their scales
+    float2 scale;
 };
-constexpr int kFewPiece = 4 * kFewThreads * 16;  // bytes of one piece of all warps, its scales behind it
-static inline __host__ __device__ int few_place(bool fp8) { return kFewPiece + (fp8 ? 2 * kFewThreads * 4 : 0); }
-__device__ __forceinline__ void few_copy16(uint32_t to, const uint8_t *from, bool there) {
-    const int bytes = there ? 16 : 0;  // 0: zeros
+constexpr int kFewPiece = 2048, kFewPlace = kFewWarps * (kFewPiece + 8);  // bytes of a piece, of one place of all warps
+__device__ __forceinline__ void few_copy16(uint32_t to, const uint8_t *from, bool there) {  // not there: zeros, nothing is read
+    const int bytes = there ? 16 : 0;
     asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void few_copy4(uint32_t to, const float *from, bool there) {
-    const int bytes = there ? 4 : 0;
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void few_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// place: of the queue, in shared memory; base: any address that may be read, for what is not there.
-template <bool FP8>
-__device__ __forceinline__ void few_ask(uint32_t place, const uint8_t *row_a, bool va, const uint8_t *row_b, bool vb, int at, int bytes, const float *sa, const float *sb,
-                                        const uint8_t *base) {
-    const uint32_t to = place + threadIdx.x * 16;
+// The queue: `depth` places in turn.  place: this warp's share of the first one.
+struct FewQueue {
+    uint32_t place;
+    const unsigned char *at;
+    uint32_t scales;  // bytes from this warp's piece to its scales
+    int depth, ask, take;
+    __device__ FewQueue(unsigned char *smem, int from, int depth_, int warp)
+        : place(static_cast<uint32_t>(__cvta_generic_to_shared(smem + from + warp * kFewPiece))), at(smem + from + warp * kFewPiece),
+          scales((kFewWarps - warp) * kFewPiece + warp * 8), depth(depth_), ask(0), take(0) {}
+    // low, high: this lane's 16 bytes of rows lane / 8 of the first and of the second eight; l0, l1, h0, h1: whether they and those four rows further on are there
+    __device__ __forceinline__ void copy(const uint8_t *low, const uint8_t *high, size_t four, bool l0, bool l1, bool h0, bool h1) const {
+        __syncwarp();  // the place's last piece has been used by all lanes
+        const int lane = threadIdx.x & 31;
+        const uint32_t to = place + ask * kFewPlace + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 1 & 4)) << 4);
+        few_copy16(to, low, l0), few_copy16(to + 512, low + four, l1), few_copy16(to + 1024, high, h0), few_copy16(to + 1536, high + four, h1);
+    }
+    __device__ __forceinline__ void copy_scale(const float *from) const {  // lanes 0 and 1
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(place + ask * kFewPlace + scales + (threadIdx.x & 31) * 4), "l"(from) : "memory");
+    }
+    __device__ __forceinline__ void asked() {
+        few_commit();
+        if (++ask == depth) ask = 0;
+    }
+    template <bool FP8>
+    __device__ __forceinline__ FewPiece next() {
+        switch (depth) {  // all but the newest depth - 1 of this thread's groups are there
+            case 2: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+            case 3: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+            case 4: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+            case 5: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
+            default: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
+        }
+        __syncwarp();
+        const int lane = threadIdx.x & 31, g = lane >> 2;
+        const unsigned char *from = at + take * kFewPlace + g * 128 + ((lane & 3) << 4);
+        FewPiece p;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        const int o = at + c * 64;
-        const bool ta = va && o < bytes, tb = vb && o < bytes;
-        few_copy16(to + c * kFewThreads * 16, ta ? row_a + o : base, ta);
-        few_copy16(to + (2 + c) * kFewThreads * 16, tb ? row_b + o : base, tb);
+        for (int c = 0; c < 2; ++c) {
+            const unsigned char *half = from + ((c ^ (g & 1)) << 6);
+            p.a[c] = *reinterpret_cast<const uint4 *>(half), p.b[c] = *reinterpret_cast<const uint4 *>(half + 1024);
+        }
+        if constexpr (FP8) p.scale = *reinterpret_cast<const float2 *>(at + take * kFewPlace + scales);
+        if (++take == depth) take = 0;
+        return p;
     }
-    if constexpr (FP8) {
-        const uint32_t scales = place + kFewPiece + threadIdx.x * 4;
-        few_copy4(scales, va ? sa : reinterpret_cast<const float *>(base), va);
-        few_copy4(scales + kFewThreads * 4, vb ? sb : reinterpret_cast<const float *>(base), vb);
-    }
-}
-template <bool FP8>
-__device__ __forceinline__ FewPiece few_take(const unsigned char *place) {
-    FewPiece p;
-    const unsigned char *from = place + threadIdx.x * 16;
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        p.a[c] = *reinterpret_cast<const uint4 *>(from + c * kFewThreads * 16);
-        p.b[c] = *reinterpret_cast<const uint4 *>(from + (2 + c) * kFewThreads * 16);
-    }
-    if constexpr (FP8) {
-        p.sa = *reinterpret_cast<const float *>(place + kFewPiece + threadIdx.x * 4);
-        p.sb = *reinterpret_cast<const float *>(place + kFewPiece + kFewThreads * 4 + threadIdx.x * 4);
-    }
-    return p;
-}
-// The oldest of `depth` groups of this thread's copies is there (the others may still be on their way).
-__device__ __forceinline__ void few_wait(int depth) {
-    switch (depth) {
-        case 1: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
-        case 2: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-        case 3: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-        case 4: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-        case 5: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
-        default: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
-    }
-}
-constexpr int kFewDepth = 6;  // the most places of a queue
+};
+constexpr int kFewDepth = 6;  // the most places
 
 // The products of half a piece (64 bytes of each row) with one tile of eight columns: x, the lane's 16 bytes' worth of column g.
 template <bool FP8>
@@ -190,8 +187,7 @@ struct FewListsSmem {  // from `at` on, a multiple of 4
     }
 };
 // All threads of the CTA, a pair each; behind a barrier after clear() and the last write of idx, which is in shared memory.
-// -> the position of this thread's pair's expert, or -1.
-__device__ __forceinline__ int few_lists(const FewArgs &a, const int *idx, const FewLists &l) {
+__device__ __forceinline__ void few_lists(const FewArgs &a, const int *idx, const FewLists &l) {
     static_assert(kFewPairs <= kFewThreads, "a pair a thread");
     const int p = threadIdx.x, lane = p & 31, t = p / a.top, k = p % a.top;
     int e = p < a.tokens * a.top ? idx[p] : a.experts;
@@ -215,16 +211,10 @@ __device__ __forceinline__ int few_lists(const FewArgs &a, const int *idx, const
     __syncthreads();
     if (live) l.column[pos * 32 + __popc(l.tokens[pos] & ((1u << t) - 1))] = (uint16_t)(t * 256 + k);
     __syncthreads();
-    return live ? pos : -1;
 }
 
 // Features 0 .. total - 1 in `runs` runs that differ by one at most.
 __device__ __forceinline__ int few_run_start(int total, int runs, int v) { return v * (total / runs) + min(v, total % runs); }
-__device__ __forceinline__ int few_run_of(int total, int runs, int f) {
-    const int q = total / runs, r = total % runs;
-    return f < r * (q + 1) ? f / (q + 1) : r + (f - r * (q + 1)) / q;
-}
-
 // ---- first launch ----------------------------------------------------------------------------------------------------
 
 constexpr int kFewCluster = 2;
@@ -247,9 +237,9 @@ struct FewFirstSmem {
         queue = lists.end;
         logits = queue + router;
         const int early = router + (tokens * (2 * outputs + groups) + tokens) * 4;
-        depth = (room - queue) / few_place(fp8);
+        depth = (room - queue) / kFewPlace;
         if (depth > kFewDepth) depth = kFewDepth;
-        const int late = depth * few_place(fp8);
+        const int late = depth * kFewPlace;
         total = queue + (early > late ? early : late);
     }
 };
@@ -298,18 +288,28 @@ moe_few_first_kernel(const FewArgs a) {
     ask(m_first, part);
     // ---- the tokens' rows, 256 entries a warp, zero behind the last one, and (8 bits) their largest magnitudes
     const int entries = (a.dim + 127) / 128 * 128, segs = (entries + 255) / 256;
-    for (int i = warp; i < a.tokens * segs; i += kFewWarps) {
-        const int t = i / segs, d = i % segs * 256 + lane * 8;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (d < a.dim) v = tl::ld_cg(reinterpret_cast<const uint4 *>(a.x + (size_t)t * a.dim + d));
-        if (d < entries) *reinterpret_cast<uint4 *>(few_smem + t * stride + d * 2) = v;
-        if constexpr (FP8) {
-            const uint32_t c[4] = {v.x, v.y, v.z, v.w};
-            uint32_t top = 0;  // of the 15 bits of a magnitude, which are in order; an infinity is above all numbers, a NaN above that
+    constexpr int X_AT_ONCE = 4;
+    for (int i0 = warp; i0 < a.tokens * segs; i0 += X_AT_ONCE * kFewWarps) {
+        uint4 v[X_AT_ONCE];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) top = max(top, max(c[j] & 0x7fffu, c[j] >> 16 & 0x7fffu));
-            top = __reduce_max_sync(0xffffffffu, top);
-            if (lane == 0) atomicMax(&most[t], top);
+        for (int u = 0; u < X_AT_ONCE; ++u) {
+            const int i = i0 + u * kFewWarps, t = i / segs, d = (i - t * segs) * 256 + lane * 8;
+            v[u] = make_uint4(0, 0, 0, 0);
+            if (t < a.tokens && d < a.dim) v[u] = tl::ld_cg(reinterpret_cast<const uint4 *>(a.x + (size_t)t * a.dim + d));
+        }
+#pragma unroll
+        for (int u = 0; u < X_AT_ONCE; ++u) {
+            const int i = i0 + u * kFewWarps, t = i / segs, d = (i - t * segs) * 256 + lane * 8;
+            if (t >= a.tokens) break;
+            if (d < entries) *reinterpret_cast<uint4 *>(few_smem + t * stride + d * 2) = v[u];
+            if constexpr (FP8) {
+                const uint32_t c[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+                uint32_t top = 0;  // of the 15 bits of a magnitude, which are in order; an infinity is above all numbers, a NaN above that
+#pragma unroll
+                for (int j = 0; j < 4; ++j) top = max(top, max(c[j] & 0x7fffu, c[j] >> 16 & 0x7fffu));
+                top = __reduce_max_sync(0xffffffffu, top);
+                if (lane == 0) atomicMax(&most[t], top);
+            }
         }
     }
     __syncthreads();
@@ -398,7 +398,7 @@ moe_few_first_kernel(const FewArgs a) {
     struct Tile {
         int pos, row, here, left;
     };
-    auto cut = [&](Tile &s) { s.here = min(min(TILE, a.ff - s.row), s.left); };
+    auto cut = [&](Tile &s) { s.here = min(min(TILE, a.ff - s.row), min(s.left, 128 - (s.row & 127))); };  // within one block of scales
     auto advance = [&](Tile &s) {
         s.left -= s.here, s.row += s.here;
         if (s.row == a.ff) s.row = 0, ++s.pos;
@@ -410,40 +410,46 @@ moe_few_first_kernel(const FewArgs a) {
         tile.left = f1 - f0, tile.pos = f0 / a.ff, tile.row = f0 % a.ff;
         cut(tile);
     }
-    const uint32_t queue = static_cast<uint32_t>(__cvta_generic_to_shared(few_smem + at.queue));
-    const int place = few_place(FP8);
+    FewQueue queue(few_smem, at.queue, at.depth, warp);
     Tile ahead = tile;
-    int ahead_it = 0, ask_at = 0, take_at = 0;
+    const uint8_t *low = nullptr, *high = nullptr;  // this lane's 16 bytes of the next piece
+    const float *scale = nullptr;
+    int byte = 0, piece = 0;
+    const size_t four = (size_t)4 * a.ld_in;
+    auto enter = [&] {
+        if (ahead.left <= 0) return;
+        const int e = lists.active[ahead.pos];
+        const size_t row = (size_t)e * a.ff + ahead.row + (lane >> 3);
+        byte = sub * 128 + (lane & 7) * 16, piece = sub;
+        low = a.w0 + row * a.ld_in + byte, high = GATED ? a.w1 + row * a.ld_in + byte : low + 2 * four;
+        if constexpr (FP8) scale = (GATED && lane == 1 ? a.s1 : a.s0) + ((size_t)e * scale_rows + (ahead.row >> 7)) * scale_cols + sub;
+    };
+    enter();
     auto issue = [&] {
         if (ahead.left > 0) {
-            const int e = lists.active[ahead.pos], b = sub + ahead_it * kFewTeam;
-            const size_t r0 = (size_t)e * a.ff + ahead.row;
-            const int second = GATED ? g : g + 8;
-            const bool va = g < ahead.here && b < blocks_in, vb = second < ahead.here && b < blocks_in;
-            const size_t s0 = (size_t)e * scale_rows;
-            few_ask<FP8>(queue + ask_at * place, a.w0 + (r0 + g) * a.ld_in, va, (GATED ? a.w1 : a.w0) + (r0 + second) * a.ld_in, vb, b * 128 + t4 * 16, a.bytes_in,
-                         a.s0 + (s0 + (ahead.row + g) / 128) * scale_cols + b, (GATED ? a.s1 : a.s0) + (s0 + (ahead.row + second) / 128) * scale_cols + b, a.w0);
-            if (++ahead_it == iters) {
-                ahead_it = 0, advance(ahead);
+            const bool in = byte < a.bytes_in;
+            const int left = in ? ahead.here - (lane >> 3) : 0;
+            queue.copy(low, high, four, left > 0, left > 4, left > (GATED ? 0 : 8), left > (GATED ? 4 : 12));
+            if (FP8 && lane < 2 && piece < blocks_in) queue.copy_scale(scale);
+            if constexpr (FP8) scale += kFewTeam;
+            low += kFewTeam * 128, high += kFewTeam * 128, byte += kFewTeam * 128, piece += kFewTeam;
+            if (piece - sub >= iters * kFewTeam) {
+                advance(ahead), enter();
                 if (ahead.left <= 0) {
                     // the last weights of this launch are on their way: the first of the next one's are asked into L2 behind them
                     const int d0 = (int)((long long)a.dim * blockIdx.x / gridDim.x), d1 = (int)((long long)a.dim * (blockIdx.x + 1) / gridDim.x);
                     const int bytes = (d1 - d0) * a.ld_out, experts = bytes > 0 ? min(*lists.count, a.prefetch / bytes) : 0;
-                    for (int q = team * kFewTeam + sub + lane * kFewWarps; q < experts; q += 32 * kFewWarps)
+                    for (int q = warp + lane * kFewWarps; q < experts; q += 32 * kFewWarps)
                         asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a.w2 + ((size_t)lists.active[q] * a.dim + d0) * a.ld_out), "r"(bytes) : "memory");
                 }
             }
         }
-        few_commit();  // an empty group where nothing is left: the count of groups stays that of the places
-        if (++ask_at == at.depth) ask_at = 0;
+        queue.asked();  // an empty group where nothing is left: the count of groups stays that of the places
     };
     float acc[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
     int it = 0, turn = 0;
-    float largest[NT];  // e4m3: of this thread's column in every tile of eight
-#pragma unroll
-    for (int n = 0; n < NT; ++n) largest[n] = 0.f;
     const int i128 = sub * 32 + lane, f8 = i128 & 7, col8 = i128 >> 3 & 7;  // the first 64 threads of a team finish a feature (two without a gate) of a column each
     auto finish = [&](int columns) {  // the tile's sums over the team's warps, the activation, the inner rows
 #pragma unroll
@@ -457,7 +463,6 @@ moe_few_first_kernel(const FewArgs a) {
             asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(kFewTeam * 32) : "memory");
             if (i128 < 64) {
                 const int col = n * 8 + col8;
-                float y_most = 0.f;
                 if (col < columns) {
                     const int c = lists.column[tile.pos * 32 + col], t = c >> 8;
                     float v[2] = {};
@@ -470,71 +475,54 @@ moe_few_first_kernel(const FewArgs a) {
                     float *to = a.inner + ((size_t)t * a.top + (c & 255)) * a.ld_inner + tile.row;
                     if constexpr (GATED) {
                         if (f8 < tile.here) {
-                            const float y = gated_pair(v[0], v[1], a.act, a.limit, a.slope);
-                            to[f8] = y, y_most = fabsf(y);
+                            to[f8] = gated_pair(v[0], v[1], a.act, a.limit, a.slope);
                         }
                     } else {
 #pragma unroll
                         for (int u = 0; u < 2; ++u)
                             if (f8 + 8 * u < tile.here) {
-                                const float y = a.act == 2 ? (v[u] > 0.f ? v[u] * v[u] : v[u] == v[u] ? 0.f : v[u]) : act_apply(v[u], a.act);
-                                to[f8 + 8 * u] = y, y_most = fmaxf(y_most, fabsf(y));
+                                to[f8 + 8 * u] = a.act == 2 ? (v[u] > 0.f ? v[u] * v[u] : v[u] == v[u] ? 0.f : v[u]) : act_apply(v[u], a.act);
                             }
                     }
                     if (tile.row + tile.here == a.ff)
                         for (int z = a.ff + f8; z < a.ld_inner; z += 8) to[z - tile.row] = 0.f;
                 }
-                if constexpr (FP8) {
-#pragma unroll
-                    for (int o = 1; o < 8; o <<= 1) y_most = fmaxf(y_most, __shfl_xor_sync(0xffffffffu, y_most, o));
-                    largest[n] = fmaxf(largest[n], y_most);
-                }
             }
         }
-        const int pos = tile.pos;
         advance(tile);
-        if constexpr (FP8) {
-            if (tile.left <= 0 || tile.pos != pos) {  // the run's share of this expert ends
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    if (i128 < 64 && f8 == 0) a.most[(size_t)(run + pos) * 32 + n * 8 + col8] = largest[n];
-                    largest[n] = 0.f;
-                }
-            }
-        }
     };
     for (int i = 0; i < at.depth; ++i) issue();
     while (tile.left > 0) {
         const int columns = __popc(lists.tokens[tile.pos]);
         int row[NT];  // this lane's columns' rows; past the last column the first token's, not used
 #pragma unroll
-        for (int n = 0; n < NT; ++n) row[n] = n * 8 + g < columns ? (lists.column[tile.pos * 32 + n * 8 + g] >> 8) * stride : 0;
+        for (int n = 0; n < NT; ++n) row[n] = (n * 8 + g < columns ? lists.column[tile.pos * 32 + n * 8 + g] >> 8 : 0) * stride + t4 * (FP8 ? 32 : 16);
         for (it = 0; it < iters; ++it) {
-            few_wait(at.depth);
-            const FewPiece p = few_take<FP8>(few_smem + at.queue + take_at * place);
-            if (++take_at == at.depth) take_at = 0;
+            const FewPiece p = queue.next<FP8>();
             const int b = sub + it * kFewTeam;
             if (b < blocks_in) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     if (n * 8 >= columns) break;
-                    float d[4] = {};
+                    if constexpr (FP8) {
+                        float d[2][4] = {};
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        if constexpr (FP8) {
-                            const unsigned char *from = few_smem + row[n] + b * 256 + c * 128 + t4 * 32;
+                        for (int c = 0; c < 2; ++c) {
+                            const unsigned char *from = few_smem + row[n] + b * 256 + c * 128;
                             const uint4 u = *reinterpret_cast<const uint4 *>(from), v = *reinterpret_cast<const uint4 *>(from + 16);
                             const uint32_t x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-                            few_half<true>(p.a[c], p.b[c], x, d);
-                        } else {
-                            const uint4 u = *reinterpret_cast<const uint4 *>(few_smem + row[n] + b * 128 + c * 64 + t4 * 16);
+                            few_half<true>(p.a[c], p.b[c], x, d[c]);
+                        }
+                        const float sb = GATED ? p.scale.y : p.scale.x;
+                        acc[n][0] = fmaf(d[0][0] + d[1][0], p.scale.x, acc[n][0]), acc[n][1] = fmaf(d[0][1] + d[1][1], p.scale.x, acc[n][1]);
+                        acc[n][2] = fmaf(d[0][2] + d[1][2], sb, acc[n][2]), acc[n][3] = fmaf(d[0][3] + d[1][3], sb, acc[n][3]);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const uint4 u = *reinterpret_cast<const uint4 *>(few_smem + row[n] + b * 128 + c * 64);
                             const uint32_t x[4] = {u.x, u.y, u.z, u.w};
                             few_half<false>(p.a[c], p.b[c], x, acc[n]);
                         }
-                    }
-                    if constexpr (FP8) {
-                        acc[n][0] = fmaf(d[0], p.sa, acc[n][0]), acc[n][1] = fmaf(d[1], p.sa, acc[n][1]);
-                        acc[n][2] = fmaf(d[2], p.sb, acc[n][2]), acc[n][3] = fmaf(d[3], p.sb, acc[n][3]);
                     }
                 }
             }
@@ -548,18 +536,17 @@ moe_few_first_kernel(const FewArgs a) {
 // ---- second launch ---------------------------------------------------------------------------------------------------
 
 struct FewSecondSmem {
-    int sums, idx, factor, times, queue, depth, total;
+    int sums, idx, factor, queue, depth, total;
     FewListsSmem lists;
     __host__ __device__ FewSecondSmem(int tokens, int experts, int top, bool fp8, int room) : lists(0, tokens, top, experts) {
         sums = 0;
         idx = sums + kFewWarps * few_sum_stride(tokens) * 4;
         factor = idx + tokens * top * 4;
-        times = factor + tokens * top * 4;
-        lists = FewListsSmem(times + tokens * top * 4, tokens, top, experts);
+        lists = FewListsSmem(factor + tokens * top * 4, tokens, top, experts);
         queue = lists.end;
-        depth = (room - queue) / few_place(fp8);
+        depth = (room - queue) / kFewPlace;
         if (depth > kFewDepth) depth = kFewDepth;
-        total = queue + depth * few_place(fp8);
+        total = queue + depth * kFewPlace;
     }
     // a warp's sums, [token][17] (16 rows, and one place that keeps the tokens' from falling into the same banks)
     static __host__ __device__ int few_sum_stride(int tokens) { return (tokens * 17 + 3) / 4 * 4; }
@@ -573,7 +560,6 @@ moe_few_second_kernel(const FewArgs a) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     const int sum_stride = FewSecondSmem::few_sum_stride(a.tokens);
     float *sums = reinterpret_cast<float *>(few_smem + at.sums) + warp * sum_stride, *factor = reinterpret_cast<float *>(few_smem + at.factor);
-    float *times = reinterpret_cast<float *>(few_smem + at.times);
     int *idx = reinterpret_cast<int *>(few_smem + at.idx);
     const FewLists lists = at.lists.lists(few_smem);
     at.lists.clear(few_smem);
@@ -583,14 +569,14 @@ moe_few_second_kernel(const FewArgs a) {
     const int pairs = a.tokens * a.top;
     if (tid < pairs) idx[tid] = tl::ld_cg(a.idx + tid), factor[tid] = tl::ld_cg(a.gate + tid);
     __syncthreads();
-    const int my_pos = few_lists(a, idx, lists), count = *lists.count, total = count * a.ff;
+    few_lists(a, idx, lists);
+    const int count = *lists.count;
 
     const int col0 = (int)((long long)a.dim * blockIdx.x / gridDim.x), col1 = (int)((long long)a.dim * (blockIdx.x + 1) / gridDim.x);
     const int blocks_out = (a.bytes_out + 127) / 128, scale_cols = (a.ff + 127) / 128, scale_rows = (a.dim + 127) / 128;
-    const uint32_t queue = static_cast<uint32_t>(__cvta_generic_to_shared(few_smem + at.queue));
-    const int place = few_place(FP8);
     for (int c0 = col0; c0 < col1; c0 += 16) {
         const int here = min(16, col1 - c0);
+        const int turn_row = 128 - (c0 & 127);  // rows from here on have the next block's scales
         // an expert's block b goes to warp (expert * blocks + b) % 16, whichever experts are chosen beside it
         struct Step {
             int pos, b;
@@ -608,38 +594,22 @@ moe_few_second_kernel(const FewArgs a) {
         };
         Step now{0, 0}, ahead{0, 0};
         enter(now), enter(ahead);
-        int ask_at = 0, take_at = 0;
+        FewQueue queue(few_smem, at.queue, at.depth, warp);
+        const size_t four = (size_t)4 * a.ld_out;
+        const uint8_t *lane_w = a.w2 + ((size_t)c0 + (lane >> 3)) * a.ld_out + (lane & 7) * 16;
+        const float *lane_s = FP8 ? a.s2 + (size_t)min((c0 >> 7) + lane, scale_rows - 1) * scale_cols : nullptr;  // lanes 0 and 1: of this block and the next
         auto issue = [&] {
             if (ahead.pos < count) {
                 const int e = lists.active[ahead.pos];
-                const uint8_t *row = a.w2 + ((size_t)e * a.dim + c0 + g) * a.ld_out;
-                const size_t s0 = (size_t)e * scale_rows;
-                few_ask<FP8>(queue + ask_at * place, row, g < here, row + (size_t)8 * a.ld_out, g + 8 < here, ahead.b * 128 + t4 * 16, a.bytes_out,
-                             a.s2 + (s0 + (c0 + g) / 128) * scale_cols + ahead.b, a.s2 + (s0 + (c0 + g + 8) / 128) * scale_cols + ahead.b, a.w2);
+                const uint8_t *low = lane_w + (size_t)e * a.dim * a.ld_out + ahead.b * 128;
+                const int left = ahead.b * 128 + (lane & 7) * 16 < a.bytes_out ? here - (lane >> 3) : 0;
+                queue.copy(low, low + 2 * four, four, left > 0, left > 4, left > 8, left > 12);
+                if (FP8 && lane < 2) queue.copy_scale(lane_s + (size_t)e * scale_rows * scale_cols + ahead.b);
                 next(ahead);
             }
-            few_commit();
-            if (++ask_at == at.depth) ask_at = 0;
+            queue.asked();
         };
         for (int i = 0; i < at.depth; ++i) issue();
-        if constexpr (FP8) {
-            if (c0 == col0) {  // an inner row's power of two, from what every run of its features left; the first weights are on their way
-                int *held = reinterpret_cast<int *>(times);  // for the warps that look: the position of every pair's expert
-                if (tid < pairs) held[tid] = my_pos;
-                __syncthreads();
-                for (int p = warp; p < pairs; p += kFewWarps) {
-                    const int pos = held[p], t = p / a.top;
-                    if (pos < 0) continue;
-                    const int f0 = pos * a.ff, v0 = few_run_of(total, a.runs, f0), v1 = few_run_of(total, a.runs, f0 + a.ff - 1);
-                    const int col = __popc(lists.tokens[pos] & ((1u << t) - 1));
-                    float most = 0.f;
-                    for (int v = v0 + lane; v <= v1; v += 32) most = fmaxf(most, tl::ld_cg(a.most + (size_t)(v + pos) * 32 + col));
-                    const int x = few_exponent(warp_max(most));
-                    if (lane == 0) times[p] = few_exp2(-x), factor[p] *= few_exp2(x);
-                }
-                __syncthreads();
-            }
-        }
         constexpr int ENTRIES = FP8 ? 16 : 8;  // of either half of a block, a lane's
         float h[2][ENTRIES];
         auto fetch = [&](const Step &s, int n) {  // a column's inner numbers; of a column that is not there: zeros
@@ -659,9 +629,8 @@ moe_few_second_kernel(const FewArgs a) {
         };
         if (now.pos < count) fetch(now, 0);
         while (now.pos < count) {
-            few_wait(at.depth);
-            const FewPiece p = few_take<FP8>(few_smem + at.queue + take_at * place);
-            if (++take_at == at.depth) take_at = 0;
+            const FewPiece p = queue.next<FP8>();
+            const float scale_a = FP8 && g < turn_row ? p.scale.x : p.scale.y, scale_b = FP8 && g + 8 < turn_row ? p.scale.x : p.scale.y;
             const int columns = __popc(lists.tokens[now.pos]);
             const uint16_t *column = lists.column + now.pos * 32;
             Step later = now;
@@ -673,9 +642,16 @@ moe_few_second_kernel(const FewArgs a) {
                 constexpr int TERMS = FP8 ? 1 : 2, WORDS = FP8 ? 8 : 4;
                 uint32_t x[2][TERMS][WORDS];
                 float down = 1.f;
-                if constexpr (FP8) {
-                    const int c = n * 8 + g < columns ? column[n * 8 + g] : column[0];
-                    down = times[(c >> 8) * a.top + (c & 255)];
+                int e = 0;
+                if constexpr (FP8) {  // a power of two for a column's 128 numbers of this block, which the block's promotion takes back
+                    uint32_t most = 0;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int i = 0; i < ENTRIES; ++i) most = max(most, __float_as_uint(h[u][i]) & 0x7fffffffu);
+                    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                    e = few_exponent(__uint_as_float(most)), down = few_exp2(-e);
                 }
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
@@ -692,19 +668,20 @@ moe_few_second_kernel(const FewArgs a) {
                         }
                     }
                 if (n == 0 && columns <= 8 && later.pos < count) fetch(later, 0);  // on its way under the products
-                float d[4] = {};
+                float d[2][4] = {};
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int term = 0; term < TERMS; ++term) few_half<FP8>(p.a[u], p.b[u], x[u][term], d);
+                    for (int term = 0; term < TERMS; ++term) few_half<FP8>(p.a[u], p.b[u], x[u][term], d[u]);
 #pragma unroll
                 for (int v = 0; v < 2; ++v) {
                     const int col = n * 8 + 2 * t4 + v;
+                    const int up = FP8 ? __shfl_sync(0xffffffffu, e, (2 * t4 + v) * 4) : 0;
                     if (col < columns) {
                         const int t = column[col] >> 8;
-                        const float f = factor[t * a.top + (column[col] & 255)];
+                        const float f = factor[t * a.top + (column[col] & 255)] * few_exp2(up);
                         float *to = sums + t * 17 + g;
-                        to[0] = fmaf(d[v], FP8 ? f * p.sa : f, to[0]), to[8] = fmaf(d[2 + v], FP8 ? f * p.sb : f, to[8]);
+                        to[0] = fmaf(d[0][v] + d[1][v], FP8 ? f * scale_a : f, to[0]), to[8] = fmaf(d[0][2 + v] + d[1][2 + v], FP8 ? f * scale_b : f, to[8]);
                     }
                 }
             }
@@ -758,9 +735,9 @@ static int few_inner_ld(int ff) { return (ff + 15) / 16 * 16; }
 static int few_nt(int tokens) { return tokens <= 8 ? 1 : tokens <= 16 ? 2 : 4; }
 
 static size_t few_align(size_t n) { return (n + 15) & ~(size_t)15; }
-static size_t few_bytes(int tokens, int top, int experts, int ff) {
-    const size_t pairs = (size_t)tokens * top, runs = (size_t)few_grid() * kFewTeams + std::min<size_t>(pairs, experts);
-    return few_align(pairs * 4) * 2 + few_align((size_t)tokens * 4) + pairs * few_inner_ld(ff) * 4 + runs * 32 * 4;
+static size_t few_bytes(int tokens, int top, int ff) {
+    const size_t pairs = (size_t)tokens * top;
+    return few_align(pairs * 4) * 2 + few_align((size_t)tokens * 4) + pairs * few_inner_ld(ff) * 4;
 }
 
 template <typename K>
@@ -811,7 +788,7 @@ int tlb_moe_few_tokens(int dim, int outputs, int experts, int top, int group_cou
 }
 
 size_t tlb_moe_few_workspace(int tokens, int top, int experts, int ff) {
-    return tokens <= 0 || top <= 0 || experts <= 0 || ff <= 0 ? 0 : few_bytes(tokens, top, experts, ff);
+    return tokens <= 0 || top <= 0 || experts <= 0 || ff <= 0 ? 0 : few_bytes(tokens, top, ff);
 }
 
 int tlb_moe_few(const tlb_moe_few_layer *l, const void *x, int tokens, const void *shared, void *out, int out_f32, void *workspace, size_t workspace_bytes, void *stream) {
@@ -828,7 +805,7 @@ int tlb_moe_few(const tlb_moe_few_layer *l, const void *x, int tokens, const voi
     if (dim % 8 || l->ld_in < dim * size || l->ld_out < ff * size || l->ld_in % 16 || l->ld_out % 16 || !tl::aligned16(x) || !tl::aligned16(l->router) ||
         !tl::aligned16(l->side_w) || !tl::aligned16(l->w_gate) || !tl::aligned16(l->w_up) || !tl::aligned16(l->w_down) || !tl::aligned16(workspace))
         return tl::fail(TL_EINVAL, "moe_few: rows must be whole 16-byte pieces");
-    if (workspace_bytes < few_bytes(tokens, top, experts, ff)) return tl::fail(TL_EINVAL, "moe_few: workspace too small");
+    if (workspace_bytes < few_bytes(tokens, top, ff)) return tl::fail(TL_EINVAL, "moe_few: workspace too small");
     const size_t pairs = (size_t)tokens * top;
     FewArgs a{};
     a.x = (const bf16 *)x, a.router = (const bf16 *)l->router, a.router_bias = (const bf16 *)l->router_bias, a.choice_bias = (const bf16 *)l->choice_bias;
@@ -842,8 +819,7 @@ int tlb_moe_few(const tlb_moe_few_layer *l, const void *x, int tokens, const voi
     a.idx = (int32_t *)at, at += few_align(pairs * 4);
     a.gate = (float *)at, at += few_align(pairs * 4);
     a.side = (float *)at, at += few_align((size_t)tokens * 4);
-    a.inner = (float *)at, a.ld_inner = few_inner_ld(ff), at += pairs * a.ld_inner * 4;
-    a.most = (float *)at, a.runs = few_grid() * kFewTeams, a.room = kFewSmem;
+    a.inner = (float *)at, a.ld_inner = few_inner_ld(ff), a.runs = few_grid() * kFewTeams, a.room = kFewSmem;
     a.prefetch = kFewPrefetch / few_grid();
     const int nt = few_nt(tokens), smem = FewFirstSmem(tokens, nt, dim, outputs, experts, top, groups, fp8 != 0, kFewSmem).total;
     const cudaStream_t st = as_stream(stream);
