@@ -46,15 +46,28 @@ __device__ __forceinline__ uint32_t pr_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
-__device__ __forceinline__ void pr_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
+// A block's four products of 32 into `d`, from zero, their completion reported to both CTAs' `done` (the accumulator is full) and `used` (the stage may be
+// written), and whether two barriers' phases are over.  Asking a barrier takes 180 cycles, whatever the answer: the questions for the next block are on their way
+// while this one's products are issued, and their answers are looked at last.
+__device__ __forceinline__ void pr_block(uint32_t d, uint64_t a, uint64_t b, uint32_t done, uint32_t used, uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1,
+                                         uint32_t &over0, uint32_t &over1) {
     constexpr uint32_t idesc = (1u << 4) | ((256u >> 3) << 17) | ((256u >> 4) << 24);  // e4m3 x e4m3 -> f32, 256 x 256, both K-major
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-                 "r"(accumulate)
-                 : "memory");
-}
-// completion of all products so far: an arrival on the barrier at this offset in both CTAs
-__device__ __forceinline__ void pr_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(static_cast<unsigned short>(3)) : "memory");
+    asm volatile(
+        "{\n\t.reg .pred p, q, on, off;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t.reg .b16 both;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%8], %9;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 q, [%10], %11;\n\t"
+        "setp.eq.u32 on, %2, %2;\n\tsetp.ne.u32 off, %2, %2;\n\t"
+        "add.u64 a1, %3, 2;\n\tadd.u64 a2, %3, 4;\n\tadd.u64 a3, %3, 6;\n\tadd.u64 b1, %4, 2;\n\tadd.u64 b2, %4, 4;\n\tadd.u64 b3, %4, 6;\n\tmov.b16 both, 3;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%2], %3, %4, %5, off;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%2], a1, b1, %5, on;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%2], a2, b2, %5, on;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%2], a3, b3, %5, on;\n\t"
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%6], both;\n\t"
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%7], both;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\tselp.u32 %1, 1, 0, q;\n\t}"
+        : "=r"(over0), "=r"(over1)
+        : "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(done), "r"(used), "r"(bar0), "r"(parity0), "r"(bar1), "r"(parity1)
+        : "memory");
 }
 __device__ __forceinline__ void pr_store32(void *p, const uint32_t (&v)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
@@ -117,17 +130,16 @@ fp8_pairs_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 int s = 0, buf = 0;
                 uint32_t ph = 0, acc_ph = 1;
                 bool ok = true;
+                uint32_t acc_free = 0, there = 0;  // of the next block's, as far as is known
                 for (int tile = unit; ok && tile < a.tiles; tile += units)
                     for (int kb = 0; kb < a.k_blocks; ++kb) {
-                        if (!(ok = tc_wait_one(acc_empty + 8 * buf, acc_ph, dead) && tc_wait_one(full + 8 * s, ph, dead))) break;
+                        if (!(ok = (acc_free || tc_wait_one(acc_empty + 8 * buf, acc_ph, dead)) && (there || tc_wait_one(full + 8 * s, ph, dead)))) break;
                         g_tc_fence_after();
                         const uint64_t q = g_smem_desc_sw128(base + s * kPrStage, 0, 1024), w = g_smem_desc_sw128(base + s * kPrStage + 128 * 128, 0, 1024);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) pr_mma(tmem + buf * 256, q + 2 * k, w + 2 * k, k > 0);
-                        pr_commit(acc_full + 8 * buf);
-                        pr_commit(empty + 8 * s);
+                        const uint32_t d = tmem + buf * 256, done = acc_full + 8 * buf, used = empty + 8 * s;
                         if (++s == kPrStages) s = 0, ph ^= 1u;
                         if (++buf == 2) buf = 0, acc_ph ^= 1u;
+                        pr_block(d, q, w, done, used, acc_empty + 8 * buf, acc_ph, full + 8 * s, ph, acc_free, there);
                     }
             }
         } else if (warp == 1) {

@@ -58,10 +58,27 @@ __device__ __forceinline__ void f8_ld(uint32_t at, uint32_t (&v)[16]) {
                  : "r"(at)
                  : "memory");
 }
-__device__ __forceinline__ void f8_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-                 "r"(accumulate)
-                 : "memory");
+// A block's four products of 32 into `d`, from zero, their completion reported to `done` (the accumulator is full) and `used` (the stage may be written), and whether
+// two barriers' phases are over.  Asking a barrier takes 180 cycles, whatever the answer: the questions for the next block are on their way while this one's
+// products are issued, and their answers are looked at last.
+__device__ __forceinline__ void f8_block(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t done, uint32_t used, uint32_t bar0, uint32_t parity0, uint32_t bar1,
+                                         uint32_t parity1, uint32_t &over0, uint32_t &over1) {
+    asm volatile(
+        "{\n\t.reg .pred p, q, on, off;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%8], %9;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 q, [%10], %11;\n\t"
+        "setp.eq.u32 on, %2, %2;\n\tsetp.ne.u32 off, %2, %2;\n\t"
+        "add.u64 a1, %3, 2;\n\tadd.u64 a2, %3, 4;\n\tadd.u64 a3, %3, 6;\n\tadd.u64 b1, %4, 2;\n\tadd.u64 b2, %4, 4;\n\tadd.u64 b3, %4, 6;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%2], %3, %4, %5, off;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%2], a1, b1, %5, on;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%2], a2, b2, %5, on;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%2], a3, b3, %5, on;\n\t"
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%6];\n\t"
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%7];\n\t"
+        "selp.u32 %0, 1, 0, p;\n\tselp.u32 %1, 1, 0, q;\n\t}"
+        : "=r"(over0), "=r"(over1)
+        : "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(done), "r"(used), "r"(bar0), "r"(parity0), "r"(bar1), "r"(parity1)
+        : "memory");
 }
 // e4m3 x e4m3 -> f32, 128 rows, n columns, both K-major
 __host__ __device__ constexpr uint32_t f8_idesc(int n) { return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24); }
@@ -185,18 +202,18 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             int s = 0, buf = 0;
             uint32_t ph = 0, acc_ph = 1;
             bool ok = !OWN || tc_wait_one(rows_there, 0, dead);
+            uint32_t acc_free = 0, there = 0;  // of the next block's, as far as is known
             for (int tile = first; ok && tile < a.tiles; tile += step)
                 for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!(ok = tc_wait_one(acc_empty + 8 * buf, acc_ph, dead) && tc_wait_one(full + 8 * s, ph, dead))) break;
+                    if (!(ok = (acc_free || tc_wait_one(acc_empty + 8 * buf, acc_ph, dead)) && (there || tc_wait_one(full + 8 * s, ph, dead)))) break;
                     g_tc_fence_after();
-                    const uint64_t w = g_smem_desc_sw128(base + s * Tile::kStage, 0, 1024), // own rows: columns 8-15 are what lies behind the block, and not used
+                    const uint64_t w = g_smem_desc_sw128(base + s * Tile::kStage, 0, 1024),
+                                   // own rows: columns 8-15 are what lies behind the block, and not used
                                    q = OWN ? g_smem_desc_sw128(own + (kb - kb0) * kF8OwnRows * kF8Block, 0, 1024) : g_smem_desc_sw128(base + s * Tile::kStage + kF8WeightBytes, 0, 1024);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) f8_mma(tmem + buf * BN, w + 2 * k, q + 2 * k, f8_idesc(BN), k > 0);
-                    g_tc_commit(acc_full + 8 * buf);
-                    g_tc_commit(empty + 8 * s);
+                    const uint32_t d = tmem + buf * BN, done = acc_full + 8 * buf, used = empty + 8 * s;
                     if (++s == Tile::kStages) s = 0, ph ^= 1u;
                     if (++buf == Tile::kBuffers) buf = 0, acc_ph ^= 1u;
+                    f8_block(d, w, q, f8_idesc(BN), done, used, acc_empty + 8 * buf, acc_ph, full + 8 * s, ph, acc_free, there);
                 }
         }
     } else if (warp >= 4) {
