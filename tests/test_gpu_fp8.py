@@ -125,3 +125,98 @@ def test_gated_mlp(rows, dim, ff, act, dtype):
     up, down = make(1, ff, dim, dtype, seed=2)[1], make(1, dim, ff, dtype, seed=3)[1]
     layer = Fp8GatedMLP(gate, up, down, act, limit=1.5 if act == "clamped_swish" else 0.0, slope=1.7 if act == "clamped_swish" else 1.0)
     check_mlp(x, gate, up, down, act, layer(x), 1.5, 1.7 if act == "clamped_swish" else 1.0)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [0, 1, 3, 8, 40, 200])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_that_are_apart_or_unaligned(rows, dtype):
+    _, w, bias = make(1, 200, 300, dtype, bias=True)
+    gen = torch.Generator().manual_seed(rows)
+    wide = torch.randn(rows + 1, 2, 411, generator=gen).to(dtype).to(DEV)
+    x = wide[:rows, 1, 7:307]  # rows 822 entries apart, an odd start
+    assert rows <= 1 or not x.is_contiguous()
+    got = fp8_linear(x, w, bias)
+    check_linear(x, w, bias, got)
+    assert torch.equal(got, fp8_linear(x.contiguous(), w, bias))
+    lead = fp8_linear(x.contiguous().reshape(1, rows, 1, 300), w, bias)
+    assert lead.shape == (1, rows, 1, 200) and torch.equal(lead.reshape(rows, 200), got)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 4, 30, 150])
+def test_numbers_that_are_none(rows):
+    """A run with an infinity or a NaN makes its row NaN, and no other; zeros stay zeros, runs of tiny numbers lose only what is below their scale."""
+    x, w, _ = make(rows + 3, 300, 400, torch.bfloat16)
+    x[0, 5] = float("inf")
+    x[1, 399] = float("nan")
+    x[2] = 0
+    x[2, 130:140] = 2.0**-126
+    got = fp8_linear(x, w)
+    assert torch.isnan(got[:2]).all() and torch.isfinite(got[2:]).all() and got[2].abs().max() < 2.0**-90
+    check_linear(x[2:], w, None, got[2:])
+    layer = Fp8GatedMLP(w, Fp8Weights(w.values[:, :400], w.scales), make(1, 400, 300, torch.bfloat16)[1], "silu")
+    out = layer(x)
+    assert torch.isnan(out[:2]).all() and torch.isfinite(out[2:]).all()
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 20, 130, 300])
+def test_a_row_does_not_depend_on_the_others(rows):
+    x, w, _ = make(rows, 520, 700, torch.bfloat16)
+    got = fp8_linear(x, w)
+    y = x.flip(0).contiguous()
+    y[0] = float("nan")
+    other = fp8_linear(y, w).flip(0)
+    assert torch.equal(other[:-1], got[:-1]) and torch.isnan(other[-1]).all()
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 24, 200])
+def test_captured_and_on_two_streams(rows):
+    """Two captured graphs and eager calls on two streams at once give what one call after another gives."""
+    xs, w, _ = make(rows, 640, 1000, torch.bfloat16)
+    layer = Fp8GatedMLP(w, w, make(1, 1000, 640, torch.bfloat16, seed=5)[1], "silu")
+    inputs = [torch.roll(xs, i, 1).contiguous() for i in range(6)]
+    want = [(fp8_linear(x, w), layer(x)) for x in inputs]
+    torch.cuda.synchronize()
+    graphs = []
+    for i in range(2):
+        x = inputs[i].clone()
+        layer(x)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = fp8_linear(x, w), layer(x)
+        graphs.append((g, x, out))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for turn in range(10):
+        for (g, x, out), s, k in zip(graphs, streams, (turn % 6, (turn + 3) % 6)):
+            with torch.cuda.stream(s):
+                x.copy_(inputs[k])
+                g.replay()
+        torch.cuda.synchronize()
+        for (g, x, out), k in zip(graphs, (turn % 6, (turn + 3) % 6)):
+            assert torch.equal(out[0], want[k][0]) and torch.equal(out[1], want[k][1])
+    got = {}
+    for turn in range(6):
+        for j, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[turn, j] = fp8_linear(inputs[turn], w), layer(inputs[turn])
+    torch.cuda.synchronize()
+    for (turn, _), (a, b) in got.items():
+        assert torch.equal(a, want[turn][0]) and torch.equal(b, want[turn][1])
+
+
+@gpu
+def test_weights_written_right_before_the_call():
+    """The kernels ask for weights early: never for ones that the launch before may still be writing."""
+    x, w, _ = make(2, 4096, 2048, torch.bfloat16)
+    other = make(2, 4096, 2048, torch.bfloat16, seed=9)[1]
+    want = [fp8_linear(x, v) for v in (w, other)]
+    store = Fp8Weights(w.values.clone(), w.scales.clone())
+    for turn in range(40):
+        v = (w, other)[turn % 2]
+        store.values.view(torch.uint8).copy_(v.values.view(torch.uint8))
+        store.scales.copy_(v.scales)
+        assert torch.equal(fp8_linear(x, store), want[turn % 2])

@@ -21,6 +21,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <atomic>
+
 #include "../per_device.h"
 #include "blocks_moe.cuh"
 
@@ -217,7 +219,7 @@ __device__ __forceinline__ void few_lists(const FewArgs &a, const int *idx, cons
 __device__ __forceinline__ int few_run_start(int total, int runs, int v) { return v * (total / runs) + min(v, total % runs); }
 // ---- first launch ----------------------------------------------------------------------------------------------------
 
-constexpr int kFewCluster = 2;
+constexpr int kFewCluster = 4;
 
 static inline __host__ __device__ int few_x_stride(int dim, bool fp8) {  // bytes of a token's row in shared memory: its 16-byte reads meet no bank conflict
     return (dim + 127) / 128 * 256 + (fp8 ? 16 : 64);
@@ -719,12 +721,30 @@ moe_few_second_kernel(const FewArgs a) {
 
 // ---- host ------------------------------------------------------------------------------------------------------------
 
-constexpr int kFewSmem = 227 * 1024;
+constexpr int kFewSmem = 227 * 1024, kFewMostGrid = 1024;
 
-// CTAs of the first launch: whole clusters (with clusters of four 132 CTAs are resident at once, with two all 148).
-static int few_grid() {
-    const int sms = sm_count();
-    return sms / kFewCluster * kFewCluster;
+// CTAs of the first launch: as many clusters as are resident at once, which a device's SMs in groups decide (132 CTAs of a B200; in pairs all 148 are, but then
+// every CTA reads half of the router's rows: 1 token of the benchmark's experts 30.2 us in 8 bits against 28.6, 32 tokens 183 and 184).
+template <typename K>
+static int few_grid(K kernel, int smem) {
+    static std::atomic<int> known[64];
+    int device = 0;
+    cudaGetDevice(&device);
+    if (device >= 0 && device < 64 && known[device].load(std::memory_order_acquire) > 0) return known[device].load(std::memory_order_relaxed);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(kFewCluster), cfg.blockDim = dim3(kFewThreads), cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kFewCluster, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess || clusters <= 0) {
+        cudaGetLastError();
+        clusters = std::max(1, sm_count() / (2 * kFewCluster));  // fewer are slower, not wrong
+    }
+    const int grid = std::min(clusters * kFewCluster, kFewMostGrid);
+    if (device >= 0 && device < 64) known[device].store(grid, std::memory_order_release);
+    return grid;
 }
 
 // Two places of the queue at least: a piece on its way while one is used.
@@ -741,13 +761,15 @@ static size_t few_bytes(int tokens, int top, int ff) {
 }
 
 template <typename K>
-static int few_launch(K kernel, tl::PerDevice &ready, dim3 grid, int cluster, int smem, cudaStream_t st, const FewArgs &a) {
+static int few_ready(K kernel, tl::PerDevice &ready) {
     int device = 0;
     cudaGetDevice(&device);
-    if (!ready(device, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem) == cudaSuccess; })) {
-        cudaGetLastError();
-        return tl::fail(TL_ECUDA, "moe_few: no shared memory");
-    }
+    if (ready(device, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem) == cudaSuccess; })) return TL_OK;
+    cudaGetLastError();
+    return tl::fail(TL_ECUDA, "moe_few: no shared memory");
+}
+template <typename K>
+static int few_launch(K kernel, dim3 grid, int cluster, int smem, cudaStream_t st, const FewArgs &a) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid, cfg.blockDim = dim3(kFewThreads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -761,17 +783,24 @@ static int few_launch(K kernel, tl::PerDevice &ready, dim3 grid, int cluster, in
     return TL_OK;
 }
 
+template <typename K>
+static int few_first(K kernel, tl::PerDevice &ready, int smem, cudaStream_t st, FewArgs &a) {
+    if (int e = few_ready(kernel, ready)) return e;
+    const int grid = few_grid(kernel, kFewSmem);
+    a.runs = grid * kFewTeams, a.prefetch = kFewPrefetch / grid;
+    return few_launch(kernel, dim3(grid), kFewCluster, smem, st, a);
+}
+template <typename K>
+static int few_second(K kernel, tl::PerDevice &ready, int smem, cudaStream_t st, const FewArgs &a) {
+    if (int e = few_ready(kernel, ready)) return e;
+    return few_launch(kernel, dim3(std::min(sm_count(), a.dim)), 1, smem, st, a);
+}
 template <bool FP8, int NT>
-static int few_run(const FewArgs &a, int first_smem, bool wide, cudaStream_t st) {
+static int few_run(FewArgs &a, int first_smem, bool wide, cudaStream_t st) {
     static tl::PerDevice gated, plain, second16, second32;
-    const int grid = few_grid();
-    int e = a.w1 ? few_launch(moe_few_first_kernel<FP8, true, NT>, gated, dim3(grid), kFewCluster, first_smem, st, a)
-                 : few_launch(moe_few_first_kernel<FP8, false, NT>, plain, dim3(grid), kFewCluster, first_smem, st, a);
-    if (e) return e;
+    if (int e = a.w1 ? few_first(moe_few_first_kernel<FP8, true, NT>, gated, first_smem, st, a) : few_first(moe_few_first_kernel<FP8, false, NT>, plain, first_smem, st, a)) return e;
     const int smem = FewSecondSmem(a.tokens, a.experts, a.top, FP8, kFewSmem).total;
-    const dim3 cols(std::min(sm_count(), a.dim));
-    return wide ? few_launch(moe_few_second_kernel<FP8, NT, float>, second32, cols, 1, smem, st, a)
-                : few_launch(moe_few_second_kernel<FP8, NT, bf16>, second16, cols, 1, smem, st, a);
+    return wide ? few_second(moe_few_second_kernel<FP8, NT, float>, second32, smem, st, a) : few_second(moe_few_second_kernel<FP8, NT, bf16>, second16, smem, st, a);
 }
 
 }  // namespace tlb
@@ -819,8 +848,7 @@ int tlb_moe_few(const tlb_moe_few_layer *l, const void *x, int tokens, const voi
     a.idx = (int32_t *)at, at += few_align(pairs * 4);
     a.gate = (float *)at, at += few_align(pairs * 4);
     a.side = (float *)at, at += few_align((size_t)tokens * 4);
-    a.inner = (float *)at, a.ld_inner = few_inner_ld(ff), a.runs = few_grid() * kFewTeams, a.room = kFewSmem;
-    a.prefetch = kFewPrefetch / few_grid();
+    a.inner = (float *)at, a.ld_inner = few_inner_ld(ff), a.room = kFewSmem;
     const int nt = few_nt(tokens), smem = FewFirstSmem(tokens, nt, dim, outputs, experts, top, groups, fp8 != 0, kFewSmem).total;
     const cudaStream_t st = as_stream(stream);
     if (fp8) return nt == 1 ? few_run<true, 1>(a, smem, out_f32, st) : nt == 2 ? few_run<true, 2>(a, smem, out_f32, st) : few_run<true, 4>(a, smem, out_f32, st);

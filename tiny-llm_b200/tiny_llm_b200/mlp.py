@@ -135,12 +135,24 @@ class MixtureOfExperts:
         if shared_gate is not None and (shared is None or shared_gate.numel() != w_up.shape[2]):
             raise ValueError("mixture of experts: a shared gate of [1, width] goes with a shared expert")
         self.shared_gate = None if shared_gate is None else shared_gate.contiguous()
+        self.few = None
+
+    def use_few_tokens(self) -> "MixtureOfExperts":
+        """Steps of at most as many tokens as one call of ``FewTokenExperts`` takes go to it from now on (bf16 experts whose weight is on their output; the
+        same definition, sums in another order and inner rows of more bits than bf16)."""
+        if self.scale_input:
+            raise ValueError("mixture of experts: the few-token layer takes the router's weight on the experts' output")
+        act = next(name for name, code in ACTIVATIONS.items() if code == self.act)
+        self.few = FewTokenExperts(self.router, self.w_gate, self.w_up, self.w_down, act, self.shared, self.identity, self.limit, self.slope, self.shared_gate)
+        return self
 
     def __call__(self, h: torch.Tensor, into: tuple | None = None, beside=None) -> torch.Tensor:
         """-> fp32 [T, D], or (``into`` = (stream, post norm, next norm)) the fused end of the sublayer, see ``blocks.moe_experts``.
         ``beside``: a model whose second stream runs the shared expert while this one routes (``RaggedDecoderModel._beside``)."""
         from extensions_b200.tiny_llm_ext_b200 import blocks
 
+        if self.few is not None and into is None and h.shape[0] <= self.few.run:
+            return self.few(h, wide=True)
         shared = side = None
         if beside is not None and self.shared is not None:
             shared = torch.empty_like(h)

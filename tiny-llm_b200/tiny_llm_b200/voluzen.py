@@ -49,7 +49,11 @@ class VoluzenModel(RaggedDecoderModel):
     architecture = "Voluzen"
 
     def __init__(self, config: dict, tensors: dict, dtype=torch.bfloat16, device="cuda", page_size: int = 64, max_tokens: int | None = None,
-                 max_requests: int | None = None):  # max_requests: accepted for all designs; no per-request state here
+                 max_requests: int | None = None, few_token_experts: bool = False):
+        """``max_requests``: accepted for all designs; no per-request state here.  ``few_token_experts`` (bf16): steps of up to 32 tokens run their experts'
+        layers in two launches (``mlp.FewTokenExperts``)."""
+        if few_token_experts and dtype != torch.bfloat16:
+            raise ValueError("few_token_experts: bfloat16 only")
         if dtype not in (torch.bfloat16, torch.float32):
             raise ValueError("Voluzen runs in bfloat16 or float32")
         self.config, self.precision, self.device = config, dtype, torch.device(device)
@@ -93,6 +97,8 @@ class VoluzenModel(RaggedDecoderModel):
                 widths.append(mixer.cache_width)
             norm1 = ResidualRMSNorm(take(f"l{i}.norm1"), self.eps, weight_offset=1.0, scale=take(f"l{i}.ls1"))
             mlp, norm2 = self._feed_forward(spec.get("mlp"), f"l{i}.mlp.", take), None
+            if few_token_experts and isinstance(mlp, MixtureOfExperts):
+                mlp.use_few_tokens()
             if mlp is not None:
                 norm2 = ResidualRMSNorm(take(f"l{i}.norm2"), self.eps, weight_offset=1.0, scale=take(f"l{i}.ls2"))
             self.layers.append(VoluzenLayer(mixer, norm1, mlp, norm2, slab_of[i if own else source]))
