@@ -363,7 +363,7 @@ int tlb_argmax_rows(const float *logits, int32_t *out, int rows, int vocab, void
  * tlb_moe_few_tokens: the most tokens a call takes at these sizes (0: none).  A token's result does not depend on the others, but for the ranges
  * 1-8, 9-16, 17-32 of tokens in a call. */
 int tlb_moe_few_tokens(int dim, int outputs, int experts, int top, int group_count, int fp8);
-size_t tlb_moe_few_workspace(int tokens, int top, int experts, int ff);
+size_t tlb_moe_few_workspace(int tokens, int dim, int experts, int top, int ff, int fp8);
 typedef struct {
     const void *router, *router_bias, *choice_bias, *side_w; /* biases and side_w may be NULL */
     const void *w_gate, *w_up, *w_down;

@@ -106,7 +106,7 @@ def test_interleaved_halves():
 def test_how_many_tokens_a_call_takes():
     few = blocks.moe_few_tokens
     assert few(2048, 64, 64, 6, 0, True) == 32 and few(2048, 64, 64, 6, 0, False) == 32
-    assert 0 < few(16384, 64, 64, 6) < 32 and few(1 << 20, 64, 64, 6) == 0
+    assert 0 < few(8192, 64, 64, 6) < 32 and few(1 << 20, 64, 64, 6) == 0
     assert few(2048, 1025, 1025, 6) == 0 and few(2048, 64, 65, 6) == 0 and few(2048, 64, 64, 65) == 0 and few(0, 64, 64, 6) == 0
     assert few(256, 512, 512, 64) == 8  # at most 512 pairs
 

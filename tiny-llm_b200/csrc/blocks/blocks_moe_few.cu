@@ -4,165 +4,113 @@
 //   first launch:  logits = router . x, the choice, inner[pair] = act(gate_e x) * (up_e x)        pair = (token, choice)
 //   second launch: y[t] = sum over choices  weight * (down_e inner[pair])  (+ identity experts, + shared expert)
 //
-// Bound by HBM: every matrix of a chosen expert is read once.  So the features of all chosen experts are one list that is cut into equal runs,
-// whatever the number of tokens and experts, and a warp keeps several 2 KB pieces of weights on their way in registers.  The arithmetic
-// is m16n8k16 products of the tensor cores' warp form with the weights as the 16 rows, the tokens as the columns: at 1 to 32 columns they
-// need a small part of the SM's issue slots, and a column is a token for all experts, so a piece's B operand is an indexed read.
+// Bound by HBM: every matrix of a chosen expert is read once.  The products are tcgen05.mma with 128 matrix rows as the M side, fed by TMA in boxes of 128 bytes
+// a row, and the tokens as 16 to 64 columns; a matrix costs no thread more than its copies and the sums' additions.  What the columns hold:
 //
-// Order of the reduction index: a lane holds 16 consecutive bytes of a row (one load), which is what it contributes to the products' k index,
-// of both operands alike; no operand is ever shuffled.
+//   bf16 experts:  x as it is; an inner row as two bf16 terms (off by 2^-16 of a number)
+//   e4m3 experts:  both operands of a product have 8 bits, so a number is several e4m3 terms, a column each, added when the sums are taken out: x, whose 8 bits
+//                  two terms of 4 hold exactly (times a power of two for each token; numbers below 2^-22 of the row's largest lose bits), an inner row three
+//                  (off by 2^-12, times a power of two for each block of 128).  A block of 128 is added in the tensor cores, then times its scales in fp32.
 //
-// e4m3 numbers become fp16 exactly; then x (a power of two for each token) and the inner rows (a power of two for each block of 128)
-// are fp16 as well, off by 2^-11 of the value or 2^-24 of the row's or block's largest (x's own numbers of 8 bits only by the latter).  bf16
-// numbers meet bf16 ones: x is as it came, and an inner row is two bf16 terms, off by 2^-16.  Sums are fp32 throughout; with 8 bits the 128 of a block are added before their scale multiplies them.
-//
-// No CTA waits for another outside its cluster: the cluster's CTAs share the router's rows, exchange the logits through shared memory, and every
-// CTA makes the same choices for itself.  The second launch reads the choices and the inner rows behind the wait for the first.
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
-
+// First launch: the CTAs of a cluster share the router's rows and exchange the logits through shared memory, and every CTA makes the same choices and the columns
+// for itself.  A tile is 64 features of an expert, gate rows and up rows in one accumulator.  Second launch: an item is 128 output columns of an expert for up to
+// 10 (16) of its tokens, over a part of the reduction; its partial sums go to memory, and the CTA that finishes an output block's last item adds them all, in
+// order (a counter tells; no CTA waits for another outside its cluster).
 #include <atomic>
 
 #include "../per_device.h"
+#include "blocks_fp8.cuh"
 #include "blocks_moe.cuh"
+#include "blocks_tc.cuh"
 
 namespace tlb {
 
 constexpr int kFewThreads = 512, kFewWarps = 16;
 constexpr int kFewTokens = 32, kFewPairs = 512, kFewOutputs = 1024;
-constexpr int kFewTeams = 4, kFewTeam = 4;  // first launch: teams of a CTA, each with its own run of features; warps of a team, which share the reduction
+constexpr int kFewStage = 128 * 128;  // a stage of the ring: 128 matrix rows of 128 bytes
+constexpr int kFewMostStages = 8;
+constexpr int kFewItemBlocks = 12;    // second launch: the most blocks of the reduction of an item
 
 struct FewArgs {
     const bf16 *x, *router, *router_bias, *choice_bias, *side_w;
     int tokens, dim, outputs /* of the router */, experts, top, scoring, group_count, group_keep;
     float weight_scale;
-    const uint8_t *w0, *w1, *w2;  // gate, up (w1 NULL: w0 is the up projection), down
-    const float *s0, *s1, *s2;    // block scales
-    int ff, ld_in, ld_out;        // bytes from row to row of w0 / w1 and of w2
-    int bytes_in, bytes_out;      // of a row that are read: whole pieces of 16, zero behind the last number
-    int act;
+    const float *s0, *s1, *s2;  // block scales: gate (up where there is no gate), up, down
+    int ff, act;
     float limit, slope;
     const bf16 *shared;
     void *out;
+    const uint8_t *w2;
+    int ld_out, row_out /* whole 16 bytes of a row */, prefetch;  // the first launch asks the second's first matrices into L2: bytes of a CTA
     // between the launches
-    int32_t *idx;      // [tokens, top]
-    float *gate;       // [tokens, top]
-    float *side;       // [tokens]
-    float *inner;      // [tokens * top, ld_inner], zero behind ff
-    int ld_inner, runs;  // runs of features: teams of the first launch
-    int room;            // bytes of shared memory that a launch may use
-    int prefetch;        // bytes that a CTA of the first launch asks into L2 for the second
+    int32_t *idx;        // [tokens, top]
+    float *gate;         // [tokens, top]
+    float *side;         // [tokens]
+    uint32_t *finished;  // [blocks of 128 output columns]: items
+    float *inner;        // [tokens * top, ld_inner], zero behind ff
+    float *part;         // [splits][tokens * top, dim]
+    int ld_inner, splits, room /* bytes of shared memory that a launch may use */;
 };
 
 // ---- small things ----------------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ uint4 few_ldg(const uint8_t *p) {  // weights: read once
+__device__ __forceinline__ uint4 few_ldg(const uint8_t *p) {
     uint4 r;
-    asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
     return r;
 }
-template <bool FP8>
-__device__ __forceinline__ void few_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    if constexpr (FP8)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// four e4m3 numbers -> two pairs of fp16 ones
-__device__ __forceinline__ void few_wide(uint32_t v, uint32_t &lo, uint32_t &hi) {
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(v));
-}
-__device__ __forceinline__ uint32_t few_half2(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
+// 16 rows of 32 entries, a lane 8 of row lane / 4 (a) and of the row 8 further on (b), times 8 columns: x, the lane's 8 entries of column lane / 4.  All operands
+// in the order in which the lanes hold them, which is that of the reduction index for both.
+__device__ __forceinline__ void few_mma(float (&d)[4], const uint4 &a, const uint4 &b, const uint4 &x) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a.x), "r"(b.x), "r"(a.y), "r"(b.y), "r"(x.x), "r"(x.y));
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a.z), "r"(b.z), "r"(a.w), "r"(b.w), "r"(x.z), "r"(x.w));
 }
 // 2^e with |v| 2^-e in [0.5, 1) for a normal v, within what fp32 holds both ways
-__device__ __forceinline__ int few_exponent(float most) {
-    const int e = static_cast<int>(__float_as_uint(most) >> 23) - 126;
-    return most < INFINITY ? min(126, max(-100, e)) : 0;  // an infinity or NaN stays what it is
-}
+__device__ __forceinline__ int few_exponent(float most) { return max(-100, static_cast<int>(__float_as_uint(most) >> 23) - 126); }
 __device__ __forceinline__ float few_exp2(int e) { return __int_as_float((e + 127) << 23); }
-
-// A warp's piece of 16 rows, 128 bytes of each: four copies of four whole lines (cp.async) into a place of the warp's own, so that a piece is waited for by
-// counting one's copies, without a barrier of the CTA.  Behind it the scales of rows 0-7 and 8-15.  A lane then has rows g = lane / 4 and g + 8, 16 bytes at
-// t * 16 (t = lane % 4) of either half; odd rows keep their halves exchanged, which spares those reads bank conflicts.
-struct FewPiece {
-    uint4 a[2], b[2];  // rows g, g + 8
-    float2 scale;
-};
-constexpr int kFewPiece = 2048, kFewPlace = kFewWarps * (kFewPiece + 8);  // bytes of a piece, of one place of all warps
-__device__ __forceinline__ void few_copy16(uint32_t to, const uint8_t *from, bool there) {  // not there: zeros, nothing is read
-    const int bytes = there ? 16 : 0;
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+// Four numbers v (at most 256) as e4m3, and what is left of them, times 16.
+__device__ __forceinline__ uint32_t few_term(float (&v)[4]) {
+    const uint32_t q = f8_pack4(v[0], v[1], v[2], v[3]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(q >> 16 * i), __NV_E4M3);
+        const float2 f = __half22float2(__half2(h));
+        v[2 * i] = (v[2 * i] - f.x) * 16.f, v[2 * i + 1] = (v[2 * i + 1] - f.y) * 16.f;
+    }
+    return q;
 }
-__device__ __forceinline__ void few_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// The queue: `depth` places in turn.  place: this warp's share of the first one.
-struct FewQueue {
-    uint32_t place;
-    const unsigned char *at;
-    uint32_t scales;  // bytes from this warp's piece to its scales
-    int depth, ask, take;
-    __device__ FewQueue(unsigned char *smem, int from, int depth_, int warp)
-        : place(static_cast<uint32_t>(__cvta_generic_to_shared(smem + from + warp * kFewPiece))), at(smem + from + warp * kFewPiece),
-          scales((kFewWarps - warp) * kFewPiece + warp * 8), depth(depth_), ask(0), take(0) {}
-    // low, high: this lane's 16 bytes of rows lane / 8 of the first and of the second eight; l0, l1, h0, h1: whether they and those four rows further on are there
-    __device__ __forceinline__ void copy(const uint8_t *low, const uint8_t *high, size_t four, bool l0, bool l1, bool h0, bool h1) const {
-        __syncwarp();  // the place's last piece has been used by all lanes
-        const int lane = threadIdx.x & 31;
-        const uint32_t to = place + ask * kFewPlace + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 1 & 4)) << 4);
-        few_copy16(to, low, l0), few_copy16(to + 512, low + four, l1), few_copy16(to + 1024, high, h0), few_copy16(to + 1536, high + four, h1);
-    }
-    __device__ __forceinline__ void copy_scale(const float *from) const {  // lanes 0 and 1
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(place + ask * kFewPlace + scales + (threadIdx.x & 31) * 4), "l"(from) : "memory");
-    }
-    __device__ __forceinline__ void asked() {
-        few_commit();
-        if (++ask == depth) ask = 0;
-    }
-    template <bool FP8>
-    __device__ __forceinline__ FewPiece next() {
-        switch (depth) {  // all but the newest depth - 1 of this thread's groups are there
-            case 2: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-            case 3: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-            case 4: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-            case 5: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
-            default: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
-        }
-        __syncwarp();
-        const int lane = threadIdx.x & 31, g = lane >> 2;
-        const unsigned char *from = at + take * kFewPlace + g * 128 + ((lane & 3) << 4);
-        FewPiece p;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const unsigned char *half = from + ((c ^ (g & 1)) << 6);
-            p.a[c] = *reinterpret_cast<const uint4 *>(half), p.b[c] = *reinterpret_cast<const uint4 *>(half + 1024);
-        }
-        if constexpr (FP8) p.scale = *reinterpret_cast<const float2 *>(at + take * kFewPlace + scales);
-        if (++take == depth) take = 0;
-        return p;
-    }
-};
-constexpr int kFewDepth = 6;  // the most places
-
-// The products of half a piece (64 bytes of each row) with one tile of eight columns: x, the lane's 16 bytes' worth of column g.
+__device__ __forceinline__ uint32_t few_most4(const float (&v)[4]) {  // magnitudes are in the order of their bits, an infinity above all numbers, a NaN above that
+    return max(max(__float_as_uint(v[0]) & 0x7fffffffu, __float_as_uint(v[1]) & 0x7fffffffu), max(__float_as_uint(v[2]) & 0x7fffffffu, __float_as_uint(v[3]) & 0x7fffffffu));
+}
+// Where byte `at` of row r of an operand lies: rows of 128 bytes in groups of 8, 16-byte pieces exchanged by row (128-byte swizzle).
+__device__ __forceinline__ uint32_t few_swizzled(int r, int at) { return r * 128 + (((at >> 4) ^ (r & 7)) << 4) + (at & 15); }
 template <bool FP8>
-__device__ __forceinline__ void few_half(const uint4 &a, const uint4 &b, const uint32_t (&x)[FP8 ? 8 : 4], float (&d)[4]) {
-    const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
-    if constexpr (FP8) {
+__device__ __forceinline__ void few_product(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (FP8)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+                     "r"(accumulate)
+                     : "memory");
+    else g_tc_mma(d, a, b, idesc, accumulate);
+}
+template <bool FP8>
+__device__ __forceinline__ uint32_t few_idesc(int n) {
+    return FP8 ? (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24) : tc_idesc(n);
+}
+__device__ __forceinline__ void few_tma(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, uint32_t bar) { tl::g_tma_load_3d(dst, map, c0, c1, c2, bar); }
+template <int COLS>
+__device__ __forceinline__ void few_ld(uint32_t at, uint32_t (&v)[COLS]) {  // columns of tensor memory, with the wait
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint32_t a0, a2, b0, b2;
-            few_wide(wa[j], a0, a2), few_wide(wb[j], b0, b2);
-            few_mma<true>(d, a0, b0, a2, b2, x[2 * j], x[2 * j + 1]);
-        }
-    } else {
+    for (int c = 0; c < COLS; c += 8) {
+        uint32_t w[8];
+        tc_ld8(at + c, w);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) few_mma<false>(d, wa[2 * j], wb[2 * j], wa[2 * j + 1], wb[2 * j + 1], x[2 * j], x[2 * j + 1]);
+        for (int i = 0; i < 8; ++i) v[c + i] = w[i];
     }
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
 // The chosen experts in ascending order and the tokens that chose each, in ascending order: a token's place is its column.  Both launches make these for
@@ -188,8 +136,8 @@ struct FewListsSmem {  // from `at` on, a multiple of 4
         for (int i = threadIdx.x; i < (active - words) / 4; i += kFewThreads) reinterpret_cast<uint32_t *>(smem + words)[i] = 0;
     }
 };
-// All threads of the CTA, a pair each; behind a barrier after clear() and the last write of idx, which is in shared memory.
-__device__ __forceinline__ void few_lists(const FewArgs &a, const int *idx, const FewLists &l) {
+// All threads of the CTA, a pair each; behind a barrier after clear() and the last write of idx, which is in shared memory.  Whether the pair has an expert's product.
+__device__ __forceinline__ bool few_lists(const FewArgs &a, const int *idx, const FewLists &l) {
     static_assert(kFewPairs <= kFewThreads, "a pair a thread");
     const int p = threadIdx.x, lane = p & 31, t = p / a.top, k = p % a.top;
     int e = p < a.tokens * a.top ? idx[p] : a.experts;
@@ -213,63 +161,99 @@ __device__ __forceinline__ void few_lists(const FewArgs &a, const int *idx, cons
     __syncthreads();
     if (live) l.column[pos * 32 + __popc(l.tokens[pos] & ((1u << t) - 1))] = (uint16_t)(t * 256 + k);
     __syncthreads();
+    return live;
 }
 
-// Features 0 .. total - 1 in `runs` runs that differ by one at most.
-__device__ __forceinline__ int few_run_start(int total, int runs, int v) { return v * (total / runs) + min(v, total % runs); }
+// Barriers of either launch: the ring's, the accumulators', the second launch's columns'.
+struct FewBars {
+    uint32_t full, empty, acc_full, acc_empty, cols_full, cols_empty;
+    volatile int *dead;
+    uint32_t *tmem, *last;
+    static constexpr int kBytes = 16 * kFewMostStages + 64 + 32 + 16;
+    __device__ FewBars(unsigned char *smem, int at) {
+        full = g_smem_u32(smem + at), empty = full + 8 * kFewMostStages, acc_full = empty + 8 * kFewMostStages, acc_empty = acc_full + 32, cols_full = acc_empty + 32;
+        cols_empty = cols_full + 16;
+        dead = reinterpret_cast<volatile int *>(smem + at + 16 * kFewMostStages + 96);
+        tmem = reinterpret_cast<uint32_t *>(smem + at + 16 * kFewMostStages + 100), last = tmem + 1;
+    }
+};
+constexpr int kFewBuffers = 4;  // accumulators, of bf16 experts 2 are used
+
 // ---- first launch ----------------------------------------------------------------------------------------------------
 
 constexpr int kFewCluster = 4;
+// Columns of the products, for eight tokens each.  e4m3: the first half is of the first half of the tokens, their first terms and then their second; so the second.
+__host__ __device__ constexpr int few_columns(int nt, bool fp8) { return fp8 ? 16 * nt : nt <= 2 ? 16 : 32; }
+constexpr int few_tmem(int columns) { return columns <= 32 ? 32 : columns <= 64 ? 64 : columns <= 128 ? 128 : 256; }
 
-static inline __host__ __device__ int few_x_stride(int dim, bool fp8) {  // bytes of a token's row in shared memory: its 16-byte reads meet no bank conflict
-    return (dim + 127) / 128 * 256 + (fp8 ? 16 : 64);
-}
 struct FewFirstSmem {
-    int x, red, most, idx, gate, queue, logits, depth, total;
+    int cols, cols_block, ring, stages, sums, router, logits, most, idx, gate, bars, total;
     FewListsSmem lists;
     __host__ __device__ FewFirstSmem(int tokens, int nt, int dim, int outputs, int experts, int top, int groups, bool fp8, int room) : lists(0, tokens, top, experts) {
-        x = 0;
-        red = x + tokens * few_x_stride(dim, fp8);
-        const int teams = 2 * kFewWarps * 16 * 8 * 4, router = kFewWarps * 16 * nt * 8 * 4;  // sums of a tile's eight columns, in turn in two places; the router's sums
-        most = red + teams;
+        const int n = few_columns(nt, fp8);
+        cols = 0;
+        cols_block = fp8 && tokens > 4 ? n * 128 : (tokens + 7) / 8 * 1024;  // of 128 bytes of the reduction; what the columns past the last token hold does not matter
+        sums = (fp8 ? (dim + 127) / 128 : (dim + 63) / 64) * cols_block + n * 128;
+        most = sums + (fp8 ? n / 2 : n) * 512;
         idx = most + kFewTokens * 4;
         gate = idx + tokens * top * 4;
         lists = FewListsSmem(gate + tokens * top * 4, tokens, top, experts);
-        // the router's sums and logits are done with when the queue's first copies are asked for
-        queue = lists.end;
-        logits = queue + router;
-        const int early = router + (tokens * (2 * outputs + groups) + tokens) * 4;
-        depth = (room - queue) / kFewPlace;
-        if (depth > kFewDepth) depth = kFewDepth;
-        const int late = depth * kFewPlace;
-        total = queue + (early > late ? early : late);
+        bars = lists.end;
+        ring = (bars + FewBars::kBytes + 1023) / 1024 * 1024;
+        // the router's sums and logits are done with when the ring's first copies are asked for
+        router = ring;
+        logits = router + kFewWarps * 16 * nt * 8 * 4;
+        const int early = logits + (tokens * (2 * outputs + groups) + tokens) * 4;
+        stages = (room - ring) / kFewStage;
+        if (stages > kFewMostStages) stages = kFewMostStages;
+        total = ring + stages * kFewStage;
+        if (total < early) total = early;
     }
 };
 
 template <bool FP8, bool GATED, int NT>
 __global__ void __launch_bounds__(kFewThreads, 1)
-moe_few_first_kernel(const FewArgs a) {
-    extern __shared__ __align__(128) unsigned char few_smem[];
+moe_few_first_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUtensorMap map1, const FewArgs a) {
+    extern __shared__ __align__(1024) unsigned char few_smem[];
+    constexpr int BUFFERS = FP8 ? kFewBuffers : 2, ENTRIES = FP8 ? 128 : 64;  // of the reduction, in a stage
+    constexpr int N = few_columns(NT, FP8), COLS = N / 2, SUMS = FP8 ? COLS / 2 : COLS /* of a thread */, TMEM = few_tmem(N * BUFFERS);
     const FewFirstSmem at(a.tokens, NT, a.dim, a.outputs, a.experts, a.top, a.group_count, FP8, a.room);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
-    const int stride = few_x_stride(a.dim, FP8);
     uint32_t rank, ranks;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
     // Another CTA's shared memory may be written once that CTA runs: arrived at here, waited for ahead of the first such store.
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-    float *logits = reinterpret_cast<float *>(few_smem + at.logits), *router_red = reinterpret_cast<float *>(few_smem + at.queue);
+    float *logits = reinterpret_cast<float *>(few_smem + at.logits), *router_red = reinterpret_cast<float *>(few_smem + at.router);
     const int per_token = 2 * a.outputs + a.group_count;
     float *side = logits + a.tokens * per_token, *gate = reinterpret_cast<float *>(few_smem + at.gate);
     uint32_t *most = reinterpret_cast<uint32_t *>(few_smem + at.most);
     int *idx = reinterpret_cast<int *>(few_smem + at.idx);
     const FewLists lists = at.lists.lists(few_smem);
+    const FewBars bars(few_smem, at.bars);
     at.lists.clear(few_smem);
     if (tid < kFewTokens) most[tid] = 0;
+    if (warp == 1 && lane == 0) {
+        for (int i = 0; i < at.stages; ++i) g_mbar_init(bars.full + 8 * i, GATED ? 2 : 1), g_mbar_init(bars.empty + 8 * i, 1);
+        for (int i = 0; i < BUFFERS; ++i) g_mbar_init(bars.acc_full + 8 * i, 1), g_mbar_init(bars.acc_empty + 8 * i, 8);
+        *bars.dead = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map0) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map1) : "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(g_smem_u32(bars.tmem)), "n"(TMEM) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    g_tc_fence_before();
     __syncthreads();
+    g_tc_fence_after();
+    const uint32_t tmem = *bars.tmem;
 
     tl::griddep_wait();
     tl::griddep_launch();  // the second launch reads nothing ahead of its own wait
+    if (blockIdx.x == 0)
+        for (int i = tid; i < (a.dim + 127) / 128; i += kFewThreads) a.finished[i] = 0;
     // ---- the router's rows, 16 for eight warps each, which share the reduction; a CTA of the cluster every ranks-th 32 of them
     const int rows = a.outputs + (a.side_w ? 1 : 0), pieces = (a.dim * 2 + 127) / 128, part = warp & 7;
     constexpr int AT_ONCE = 4;
@@ -288,25 +272,23 @@ moe_few_first_kernel(const FewArgs a) {
     };
     const int m_first = rank * 2 + (warp >> 3);
     ask(m_first, part);
-    // ---- the tokens' rows, 256 entries a warp, zero behind the last one, and (8 bits) their largest magnitudes
-    const int entries = (a.dim + 127) / 128 * 128, segs = (entries + 255) / 256;
-    constexpr int X_AT_ONCE = 4;
-    for (int i0 = warp; i0 < a.tokens * segs; i0 += X_AT_ONCE * kFewWarps) {
-        uint4 v[X_AT_ONCE];
+    if constexpr (FP8) {  // the tokens' largest magnitudes, 256 entries a warp
+        const int segs = (a.dim + 255) / 256;
+        constexpr int X_AT_ONCE = 4;
+        for (int i0 = warp; i0 < a.tokens * segs; i0 += X_AT_ONCE * kFewWarps) {
+            uint4 v[X_AT_ONCE];
 #pragma unroll
-        for (int u = 0; u < X_AT_ONCE; ++u) {
-            const int i = i0 + u * kFewWarps, t = i / segs, d = (i - t * segs) * 256 + lane * 8;
-            v[u] = make_uint4(0, 0, 0, 0);
-            if (t < a.tokens && d < a.dim) v[u] = tl::ld_cg(reinterpret_cast<const uint4 *>(a.x + (size_t)t * a.dim + d));
-        }
+            for (int u = 0; u < X_AT_ONCE; ++u) {
+                const int i = i0 + u * kFewWarps, t = i / segs, d = (i - t * segs) * 256 + lane * 8;
+                v[u] = make_uint4(0, 0, 0, 0);
+                if (t < a.tokens && d < a.dim) v[u] = tl::ld_cg(reinterpret_cast<const uint4 *>(a.x + (size_t)t * a.dim + d));
+            }
 #pragma unroll
-        for (int u = 0; u < X_AT_ONCE; ++u) {
-            const int i = i0 + u * kFewWarps, t = i / segs, d = (i - t * segs) * 256 + lane * 8;
-            if (t >= a.tokens) break;
-            if (d < entries) *reinterpret_cast<uint4 *>(few_smem + t * stride + d * 2) = v[u];
-            if constexpr (FP8) {
+            for (int u = 0; u < X_AT_ONCE; ++u) {
+                const int t = (i0 + u * kFewWarps) / segs;
+                if (t >= a.tokens) break;
                 const uint32_t c[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-                uint32_t top = 0;  // of the 15 bits of a magnitude, which are in order; an infinity is above all numbers, a NaN above that
+                uint32_t top = 0;  // of the 15 bits of a magnitude
 #pragma unroll
                 for (int j = 0; j < 4; ++j) top = max(top, max(c[j] & 0x7fffu, c[j] >> 16 & 0x7fffu));
                 top = __reduce_max_sync(0xffffffffu, top);
@@ -314,7 +296,6 @@ moe_few_first_kernel(const FewArgs a) {
             }
         }
     }
-    __syncthreads();
     bool waited = false;
     for (int m = m_first; (m - (warp >> 3)) * 16 < rows; m += ranks * 2) {
         float acc[NT][4];
@@ -323,16 +304,21 @@ moe_few_first_kernel(const FewArgs a) {
         for (int s = part; s < pieces; s += AT_ONCE * 8) {
             if (m != m_first || s != part) ask(m, s);
 #pragma unroll
-            for (int u = 0; u < AT_ONCE; ++u)
-                if (s + u * 8 < pieces)
+            for (int u = 0; u < AT_ONCE; ++u) {
+                uint4 x[2][NT];
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
+                for (int c = 0; c < 2; ++c)
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {  // columns past the last token: the last one, not used
-                            const uint4 v = *reinterpret_cast<const uint4 *>(few_smem + min(n * 8 + g, a.tokens - 1) * stride + (s + u * 8) * 128 + c * 64 + t4 * 16);
-                            const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-                            few_half<false>(wa[u][c], wb[u][c], x, acc[n]);
-                        }
+                    for (int n = 0; n < NT; ++n) {  // columns past the last token: the last one, not used
+                        const int o = (s + u * 8) * 64 + c * 32 + t4 * 8;
+                        x[c][n] = make_uint4(0, 0, 0, 0);
+                        if (o < a.dim) x[c][n] = tl::ld_cg(reinterpret_cast<const uint4 *>(a.x + (size_t)min(n * 8 + g, a.tokens - 1) * a.dim + o));
+                    }
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) few_mma(acc[n], wa[u][c], wb[u][c], x[c][n]);
+            }
         }
         float *mine = router_red + warp * 16 * NT * 8;
 #pragma unroll
@@ -359,23 +345,37 @@ moe_few_first_kernel(const FewArgs a) {
     }
     if (!waited) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    if constexpr (FP8) {  // the rows as fp16 times a power of two; the router is done with them
-        for (int i = warp; i < a.tokens * segs; i += kFewWarps) {
-            const int t = i / segs, d = i % segs * 256 + lane * 8;
-            const float down = few_exp2(-few_exponent(__uint_as_float(most[t] << 16)));
-            if (d < entries) {
-                uint4 *p = reinterpret_cast<uint4 *>(few_smem + t * stride + d * 2);
-                const uint4 u = *p;
-                const uint32_t c[4] = {u.x, u.y, u.z, u.w};
-                uint32_t o[4];
+    __syncthreads();  // the largest magnitudes
+    // ---- the columns: what of all tokens stands beside an expert's rows
+    {
+        constexpr int C_AT_ONCE = 4;
+        const int blocks = (a.dim + 127) / 128;  // of 128 entries
+        for (int i0 = warp; i0 < a.tokens * blocks; i0 += C_AT_ONCE * kFewWarps) {
+            uint2 v[C_AT_ONCE];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 f = tl::unpack2<bf16>(c[j]);
-                    o[j] = few_half2(f.x * down, f.y * down);
+            for (int u = 0; u < C_AT_ONCE; ++u) {
+                const int i = i0 + u * kFewWarps, t = i / blocks, d = (i - t * blocks) * 128 + lane * 4;
+                v[u] = make_uint2(0, 0);
+                if (t < a.tokens && d < a.dim) asm volatile("ld.global.cg.v2.u32 {%0,%1}, [%2];" : "=r"(v[u].x), "=r"(v[u].y) : "l"(a.x + (size_t)t * a.dim + d) : "memory");
+            }
+#pragma unroll
+            for (int u = 0; u < C_AT_ONCE; ++u) {
+                const int i = i0 + u * kFewWarps, t = i / blocks, b = i - t * blocks;
+                if (t >= a.tokens) break;
+                if constexpr (FP8) {
+                    const float up = few_exp2(8 - few_exponent(__uint_as_float(most[t] << 16)));
+                    const float2 lo = tl::unpack2<bf16>(v[u].x), hi = tl::unpack2<bf16>(v[u].y);
+                    float w[4] = {lo.x * up, lo.y * up, hi.x * up, hi.y * up};
+                    unsigned char *to = few_smem + at.cols + b * at.cols_block;
+                    const int column = t + t / SUMS * SUMS;
+                    *reinterpret_cast<uint32_t *>(to + few_swizzled(column, lane * 4)) = few_term(w);
+                    *reinterpret_cast<uint32_t *>(to + few_swizzled(column + SUMS, lane * 4)) = few_term(w);
+                } else if (b * 2 + (lane >> 4) < (a.dim + 63) / 64) {
+                    *reinterpret_cast<uint2 *>(few_smem + at.cols + (b * 2 + (lane >> 4)) * at.cols_block + few_swizzled(t, (lane & 15) * 8)) = v[u];
                 }
-                *p = make_uint4(o[0], o[1], o[2], o[3]);
             }
         }
+        tl::g_fence_proxy_async();
     }
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 
@@ -390,349 +390,466 @@ moe_few_first_kernel(const FewArgs a) {
         for (int p = tid; p < a.tokens * a.top; p += kFewThreads) a.idx[p] = idx[p], a.gate[p] = gate[p];
         if (a.side_w && tid < a.tokens) a.side[tid] = sigmoid(side[tid]);
     }
+    tl::g_fence_proxy_async();  // the logits have been read, copies may come over them
     few_lists(a, idx, lists);
 
-    // ---- the first products: a team takes its run of the chosen experts' features, up to 8 (with a gate; else 16) of one expert at a time
-    constexpr int TILE = GATED ? 8 : 16;
-    const int team = warp / kFewTeam, sub = warp % kFewTeam, run = blockIdx.x * kFewTeams + team, total = *lists.count * a.ff;
-    const int blocks_in = (a.bytes_in + 127) / 128, iters = (blocks_in + kFewTeam - 1) / kFewTeam;
+    // ---- the first products: tiles of 64 features with their gates, or 128 without
+    constexpr int FEATURES = GATED ? 64 : 128;
+    const int count = *lists.count, tiles_of = (a.ff + FEATURES - 1) / FEATURES, tiles = count * tiles_of, blocks = (a.dim + ENTRIES - 1) / ENTRIES;
     const int scale_cols = (a.dim + 127) / 128, scale_rows = (a.ff + 127) / 128;
-    struct Tile {
-        int pos, row, here, left;
-    };
-    auto cut = [&](Tile &s) { s.here = min(min(TILE, a.ff - s.row), min(s.left, 128 - (s.row & 127))); };  // within one block of scales
-    auto advance = [&](Tile &s) {
-        s.left -= s.here, s.row += s.here;
-        if (s.row == a.ff) s.row = 0, ++s.pos;
-        cut(s);
-    };
-    Tile tile;
-    {
-        const int f0 = few_run_start(total, a.runs, run), f1 = few_run_start(total, a.runs, run + 1);
-        tile.left = f1 - f0, tile.pos = f0 / a.ff, tile.row = f0 % a.ff;
-        cut(tile);
+    if (warp == 0 || (GATED && warp == 3)) {
+        if (g_elect_one()) {
+            int s = 0;
+            uint32_t ph = 1;
+            bool ok = true;
+            for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+                const int e = lists.active[tile / tiles_of], f0 = tile % tiles_of * FEATURES;
+                for (int b = 0; b < blocks; ++b) {
+                    if (!(ok = tc_wait_one(bars.empty + 8 * s, ph, bars.dead))) break;
+                    g_mbar_expect_tx(bars.full + 8 * s, GATED ? kFewStage / 2 : kFewStage);
+                    few_tma(g_smem_u32(few_smem + at.ring) + s * kFewStage + (warp == 3 ? kFewStage / 2 : 0), warp == 3 ? &map1 : &map0, b * 128, f0, e,
+                            bars.full + 8 * s);
+                    if (++s == at.stages) s = 0, ph ^= 1u;
+                }
+            }
+            if (warp == 0) {  // the last weights of this launch are on their way: the first of the next one's are asked into L2 behind them
+                const int outs = (a.dim + 127) / 128, all = count * outs;
+                for (int i = blockIdx.x, left = a.prefetch; i < all && left > 0; i += gridDim.x) {
+                    const int d0 = i % outs * 128, bytes = (min(128, a.dim - d0) - 1) * a.ld_out + a.row_out;  // not past the last row's last number
+                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a.w2 + ((size_t)lists.active[i / outs] * a.dim + d0) * a.ld_out), "r"(bytes) : "memory");
+                    left -= bytes;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (g_elect_one()) {
+            int s = 0, buf = 0;
+            uint32_t ph = 0, acc_ph = 1;
+            bool ok = true;
+            const uint32_t ring = g_smem_u32(few_smem + at.ring), cols = g_smem_u32(few_smem + at.cols);
+            for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x)
+                for (int b = 0; b < blocks; ++b) {
+                    if (FP8 || b == 0) ok = tc_wait_one(bars.acc_empty + 8 * buf, acc_ph, bars.dead);
+                    if (!ok || !(ok = tc_wait_one(bars.full + 8 * s, ph, bars.dead))) break;
+                    g_tc_fence_after();
+                    const uint64_t w = g_smem_desc_sw128(ring + s * kFewStage, 0, 1024), x = g_smem_desc_sw128(cols + b * at.cols_block, 0, 1024);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) few_product<FP8>(tmem + buf * N, w + 2 * k, x + 2 * k, few_idesc<FP8>(N), FP8 ? k > 0 : b > 0 || k > 0);
+                    const bool last = FP8 || b == blocks - 1;
+                    if (last) g_tc_commit(bars.acc_full + 8 * buf);
+                    g_tc_commit(bars.empty + 8 * s);
+                    if (++s == at.stages) s = 0, ph ^= 1u;
+                    if (last && ++buf == BUFFERS) buf = 0, acc_ph ^= 1u;
+                }
+        }
+    } else if (warp >= 8) {
+        const int quarter = warp & 3, half = (warp - 8) >> 2, row = quarter * 32 + lane, me = tid - 256;
+        float *sums = reinterpret_cast<float *>(few_smem + at.sums);  // [token][128]
+        int buf = 0;
+        uint32_t acc_ph = 0;
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+            const int pos = tile / tiles_of, e = lists.active[pos], f0 = tile % tiles_of * FEATURES;
+            float acc[SUMS];
+#pragma unroll
+            for (int c = 0; c < SUMS; ++c) acc[c] = 0.f;
+            bool ok = true;
+            const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * COLS;
+            if constexpr (FP8) {
+                // the rows' block of scales: a gate's (or, without gates, all), the up projection's
+                const float *scales = (GATED && quarter >= 2 ? a.s1 : a.s0) + ((size_t)e * scale_rows + (f0 >> 7)) * scale_cols;
+                float next = __ldg(scales);
+                for (int b = 0; b < blocks; ++b) {
+                    const float scale = next;
+                    if (b + 1 < blocks) next = __ldg(scales + b + 1);
+                    ok &= tc_wait(bars.acc_full + 8 * buf, acc_ph, bars.dead);
+                    g_tc_fence_after();
+                    uint32_t v[COLS];
+                    few_ld(from + buf * N, v);
+                    g_tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) g_mbar_arrive(bars.acc_empty + 8 * buf);
+#pragma unroll
+                    for (int c = 0; c < SUMS; ++c) acc[c] = fmaf(fmaf(__uint_as_float(v[c + SUMS]), 0.0625f, __uint_as_float(v[c])), scale, acc[c]);
+                    if (++buf == BUFFERS) buf = 0, acc_ph ^= 1u;
+                }
+            } else {
+                ok &= tc_wait(bars.acc_full + 8 * buf, acc_ph, bars.dead);
+                g_tc_fence_after();
+                uint32_t v[COLS];
+                few_ld(from + buf * N, v);
+                g_tc_fence_before();
+                __syncwarp();
+                if (lane == 0) g_mbar_arrive(bars.acc_empty + 8 * buf);
+#pragma unroll
+                for (int c = 0; c < SUMS; ++c) acc[c] = __uint_as_float(v[c]);
+                if (++buf == BUFFERS) buf = 0, acc_ph ^= 1u;
+            }
+#pragma unroll
+            for (int c = 0; c < SUMS; ++c) sums[(half * SUMS + c) * 128 + row] = acc[c];
+            const float bad = tc_verdict(ok, bars.dead);
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const int columns = __popc(lists.tokens[pos]), here = min(FEATURES, a.ff - f0);
+            for (int i = me; i < columns * FEATURES; i += 256) {
+                const int f = i % FEATURES, c = lists.column[pos * 32 + i / FEATURES], t = c >> 8;
+                if (f >= here) continue;
+                auto of = [&](int r) {
+                    if constexpr (!FP8) return sums[t * 128 + r];
+                    // a token with an infinity or a NaN has none of its numbers
+                    const uint32_t m = most[t] << 16;
+                    const float scale = m < 0x7f800000u ? few_exp2(few_exponent(__uint_as_float(m)) - 8) : __int_as_float(0x7fffffff);
+                    return sums[t * 128 + r] * scale;
+                };
+                const float v = of(f) * bad;
+                float y;
+                if constexpr (GATED) y = gated_pair(v, of(f + 64), a.act, a.limit, a.slope);
+                else y = a.act == 2 ? (v > 0.f ? v * v : v == v ? 0.f : v) : act_apply(v, a.act);
+                float *to = a.inner + ((size_t)t * a.top + (c & 255)) * a.ld_inner + f0;
+                to[f] = y;
+                if (f0 + here == a.ff)
+                    for (int z = a.ff + f; z < a.ld_inner; z += here) to[z - f0] = 0.f;
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");  // read before the next tile's are written
+        }
     }
-    FewQueue queue(few_smem, at.queue, at.depth, warp);
-    Tile ahead = tile;
-    const uint8_t *low = nullptr, *high = nullptr;  // this lane's 16 bytes of the next piece
-    const float *scale = nullptr;
-    int byte = 0, piece = 0;
-    const size_t four = (size_t)4 * a.ld_in;
-    auto enter = [&] {
-        if (ahead.left <= 0) return;
-        const int e = lists.active[ahead.pos];
-        const size_t row = (size_t)e * a.ff + ahead.row + (lane >> 3);
-        byte = sub * 128 + (lane & 7) * 16, piece = sub;
-        low = a.w0 + row * a.ld_in + byte, high = GATED ? a.w1 + row * a.ld_in + byte : low + 2 * four;
-        if constexpr (FP8) scale = (GATED && lane == 1 ? a.s1 : a.s0) + ((size_t)e * scale_rows + (ahead.row >> 7)) * scale_cols + sub;
-    };
-    enter();
-    auto issue = [&] {
-        if (ahead.left > 0) {
-            const bool in = byte < a.bytes_in;
-            const int left = in ? ahead.here - (lane >> 3) : 0;
-            queue.copy(low, high, four, left > 0, left > 4, left > (GATED ? 0 : 8), left > (GATED ? 4 : 12));
-            if (FP8 && lane < 2 && piece < blocks_in) queue.copy_scale(scale);
-            if constexpr (FP8) scale += kFewTeam;
-            low += kFewTeam * 128, high += kFewTeam * 128, byte += kFewTeam * 128, piece += kFewTeam;
-            if (piece - sub >= iters * kFewTeam) {
-                advance(ahead), enter();
-                if (ahead.left <= 0) {
-                    // the last weights of this launch are on their way: the first of the next one's are asked into L2 behind them
-                    const int d0 = (int)((long long)a.dim * blockIdx.x / gridDim.x), d1 = (int)((long long)a.dim * (blockIdx.x + 1) / gridDim.x);
-                    const int bytes = (d1 - d0) * a.ld_out, experts = bytes > 0 ? min(*lists.count, a.prefetch / bytes) : 0;
-                    for (int q = warp + lane * kFewWarps; q < experts; q += 32 * kFewWarps)
-                        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a.w2 + ((size_t)lists.active[q] * a.dim + d0) * a.ld_out), "r"(bytes) : "memory");
-                }
-            }
-        }
-        queue.asked();  // an empty group where nothing is left: the count of groups stays that of the places
-    };
-    float acc[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-    int it = 0, turn = 0;
-    const int i128 = sub * 32 + lane, f8 = i128 & 7, col8 = i128 >> 3 & 7;  // the first 64 threads of a team finish a feature (two without a gate) of a column each
-    auto finish = [&](int columns) {  // the tile's sums over the team's warps, the activation, the inner rows
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            if (n * 8 >= columns) break;
-            float *sums = reinterpret_cast<float *>(few_smem + at.red) + ((turn ^= 1) * kFewTeams + team) * kFewTeam * 128, *mine = sums + sub * 128;
-            *reinterpret_cast<float2 *>(mine + g * 8 + 2 * t4) = make_float2(acc[n][0], acc[n][1]);
-            *reinterpret_cast<float2 *>(mine + (g + 8) * 8 + 2 * t4) = make_float2(acc[n][2], acc[n][3]);
-            acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-            // one barrier for each use of either place: a place is written again only behind the other's
-            asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(kFewTeam * 32) : "memory");
-            if (i128 < 64) {
-                const int col = n * 8 + col8;
-                if (col < columns) {
-                    const int c = lists.column[tile.pos * 32 + col], t = c >> 8;
-                    float v[2] = {};
-#pragma unroll
-                    for (int w = 0; w < kFewTeam; ++w) v[0] += sums[w * 128 + f8 * 8 + col8], v[1] += sums[w * 128 + (f8 + 8) * 8 + col8];
-                    if constexpr (FP8) {
-                        const float up = few_exp2(few_exponent(__uint_as_float(most[t] << 16)));
-                        v[0] *= up, v[1] *= up;
-                    }
-                    float *to = a.inner + ((size_t)t * a.top + (c & 255)) * a.ld_inner + tile.row;
-                    if constexpr (GATED) {
-                        if (f8 < tile.here) {
-                            to[f8] = gated_pair(v[0], v[1], a.act, a.limit, a.slope);
-                        }
-                    } else {
-#pragma unroll
-                        for (int u = 0; u < 2; ++u)
-                            if (f8 + 8 * u < tile.here) {
-                                to[f8 + 8 * u] = a.act == 2 ? (v[u] > 0.f ? v[u] * v[u] : v[u] == v[u] ? 0.f : v[u]) : act_apply(v[u], a.act);
-                            }
-                    }
-                    if (tile.row + tile.here == a.ff)
-                        for (int z = a.ff + f8; z < a.ld_inner; z += 8) to[z - tile.row] = 0.f;
-                }
-            }
-        }
-        advance(tile);
-    };
-    for (int i = 0; i < at.depth; ++i) issue();
-    while (tile.left > 0) {
-        const int columns = __popc(lists.tokens[tile.pos]);
-        int row[NT];  // this lane's columns' rows; past the last column the first token's, not used
-#pragma unroll
-        for (int n = 0; n < NT; ++n) row[n] = (n * 8 + g < columns ? lists.column[tile.pos * 32 + n * 8 + g] >> 8 : 0) * stride + t4 * (FP8 ? 32 : 16);
-        for (it = 0; it < iters; ++it) {
-            const FewPiece p = queue.next<FP8>();
-            const int b = sub + it * kFewTeam;
-            if (b < blocks_in) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    if (n * 8 >= columns) break;
-                    if constexpr (FP8) {
-                        float d[2][4] = {};
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            const unsigned char *from = few_smem + row[n] + b * 256 + c * 128;
-                            const uint4 u = *reinterpret_cast<const uint4 *>(from), v = *reinterpret_cast<const uint4 *>(from + 16);
-                            const uint32_t x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-                            few_half<true>(p.a[c], p.b[c], x, d[c]);
-                        }
-                        const float sb = GATED ? p.scale.y : p.scale.x;
-                        acc[n][0] = fmaf(d[0][0] + d[1][0], p.scale.x, acc[n][0]), acc[n][1] = fmaf(d[0][1] + d[1][1], p.scale.x, acc[n][1]);
-                        acc[n][2] = fmaf(d[0][2] + d[1][2], sb, acc[n][2]), acc[n][3] = fmaf(d[0][3] + d[1][3], sb, acc[n][3]);
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            const uint4 u = *reinterpret_cast<const uint4 *>(few_smem + row[n] + b * 128 + c * 64);
-                            const uint32_t x[4] = {u.x, u.y, u.z, u.w};
-                            few_half<false>(p.a[c], p.b[c], x, acc[n]);
-                        }
-                    }
-                }
-            }
-            issue();
-        }
-        finish(columns);
+    __syncwarp();
+    g_tc_fence_before();
+    __syncthreads();
+    if (warp == 2) {
+        tc_settle(bars.dead);
+        g_tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(TMEM) : "memory");
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // ---- second launch ---------------------------------------------------------------------------------------------------
 
+constexpr int kFewSecondN = 32;  // the most columns of an item: terms times tokens
+
 struct FewSecondSmem {
-    int sums, idx, factor, queue, depth, total;
+    int cols, factors, sums, idx, gate, group, bars, ring, stages, total;
+    static constexpr int kCols = kFewItemBlocks * 4096 + 4096, kFactors = kFewItemBlocks * kFewSecondN * 4;  // of either place of an item's columns
     FewListsSmem lists;
-    __host__ __device__ FewSecondSmem(int tokens, int experts, int top, bool fp8, int room) : lists(0, tokens, top, experts) {
-        sums = 0;
-        idx = sums + kFewWarps * few_sum_stride(tokens) * 4;
-        factor = idx + tokens * top * 4;
-        lists = FewListsSmem(factor + tokens * top * 4, tokens, top, experts);
-        queue = lists.end;
-        depth = (room - queue) / kFewPlace;
-        if (depth > kFewDepth) depth = kFewDepth;
-        total = queue + depth * kFewPlace;
+    __host__ __device__ FewSecondSmem(int tokens, int experts, int top, int room) : lists(0, tokens, top, experts) {
+        cols = 0;
+        factors = cols + 2 * kCols;
+        sums = factors + 2 * kFactors;
+        idx = sums + kFewSecondN * 128 * 4;
+        gate = idx + tokens * top * 4;
+        group = gate + tokens * top * 4;
+        lists = FewListsSmem((group + tokens * top * 4 + 4 + 3) / 4 * 4, tokens, top, experts);
+        bars = lists.end;
+        ring = (bars + FewBars::kBytes + 1023) / 1024 * 1024;
+        stages = (room - ring) / kFewStage;
+        if (stages > kFewMostStages) stages = kFewMostStages;
+        total = ring + stages * kFewStage;
     }
-    // a warp's sums, [token][17] (16 rows, and one place that keeps the tokens' from falling into the same banks)
-    static __host__ __device__ int few_sum_stride(int tokens) { return (tokens * 17 + 3) / 4 * 4; }
 };
 
-template <bool FP8, int NT, typename OUT>
+// An identity expert's part of an output; a choice that is no output at all: the token's logits are no numbers.
+__device__ __forceinline__ float few_identity(const FewArgs &a, int e, float weight, int t, int d, float y) {
+    return e < a.outputs ? fmaf(weight, to_f(tl::ld_cg(a.x + (size_t)t * a.dim + d)), y) : __int_as_float(0x7fffffff);
+}
+template <typename OUT>
+__device__ __forceinline__ void few_store(const FewArgs &a, int t, int d, float y) {
+    if (a.shared) y = fmaf(a.side_w ? tl::ld_cg(a.side + t) : 1.f, to_f(tl::ld_cg(a.shared + (size_t)t * a.dim + d)), y);
+    static_cast<OUT *>(a.out)[(size_t)t * a.dim + d] = from_f<OUT>(y);
+}
+
+template <bool FP8, typename OUT>
 __global__ void __launch_bounds__(kFewThreads, 1)
-moe_few_second_kernel(const FewArgs a) {
-    extern __shared__ __align__(128) unsigned char few_smem[];
-    const FewSecondSmem at(a.tokens, a.experts, a.top, FP8, a.room);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
-    const int sum_stride = FewSecondSmem::few_sum_stride(a.tokens);
-    float *sums = reinterpret_cast<float *>(few_smem + at.sums) + warp * sum_stride, *factor = reinterpret_cast<float *>(few_smem + at.factor);
-    int *idx = reinterpret_cast<int *>(few_smem + at.idx);
+moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) {
+    extern __shared__ __align__(1024) unsigned char few_smem[];
+    constexpr int TERMS = FP8 ? 3 : 2, GROUP = kFewSecondN / TERMS, BUFFERS = FP8 ? kFewBuffers : 2, TMEM = kFewSecondN * BUFFERS, ENTRIES = FP8 ? 128 : 64;
+    const FewSecondSmem at(a.tokens, a.experts, a.top, a.room);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, pairs = a.tokens * a.top;
+    float *sums = reinterpret_cast<float *>(few_smem + at.sums), *gate = reinterpret_cast<float *>(few_smem + at.gate), *factors = reinterpret_cast<float *>(few_smem + at.factors);
+    int *idx = reinterpret_cast<int *>(few_smem + at.idx), *group = reinterpret_cast<int *>(few_smem + at.group);  // group: [groups] position * 4 + number
     const FewLists lists = at.lists.lists(few_smem);
+    const FewBars bars(few_smem, at.bars);
     at.lists.clear(few_smem);
-    for (int i = lane; i < sum_stride; i += 32) sums[i] = 0.f;
+    if (warp == 1 && lane == 0) {
+        for (int i = 0; i < at.stages; ++i) g_mbar_init(bars.full + 8 * i, 1), g_mbar_init(bars.empty + 8 * i, 1);
+        for (int i = 0; i < BUFFERS; ++i) g_mbar_init(bars.acc_full + 8 * i, 1), g_mbar_init(bars.acc_empty + 8 * i, 8);
+        for (int i = 0; i < 2; ++i) g_mbar_init(bars.cols_full + 8 * i, 4), g_mbar_init(bars.cols_empty + 8 * i, 1 + 8);  // by the warps that write; by the products, and the sums
+        *bars.dead = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(g_smem_u32(bars.tmem)), "n"(TMEM) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
     tl::griddep_wait();
     tl::griddep_launch();
-    const int pairs = a.tokens * a.top;
-    if (tid < pairs) idx[tid] = tl::ld_cg(a.idx + tid), factor[tid] = tl::ld_cg(a.gate + tid);
+    if (tid < pairs) idx[tid] = tl::ld_cg(a.idx + tid), gate[tid] = tl::ld_cg(a.gate + tid);
+    g_tc_fence_before();
     __syncthreads();
-    few_lists(a, idx, lists);
+    g_tc_fence_after();
+    const uint32_t tmem = *bars.tmem;
+    const bool live = few_lists(a, idx, lists);
+    if (tid < pairs && !live && idx[tid] < a.experts) idx[tid] = -1;  // named twice
     const int count = *lists.count;
-
-    const int col0 = (int)((long long)a.dim * blockIdx.x / gridDim.x), col1 = (int)((long long)a.dim * (blockIdx.x + 1) / gridDim.x);
-    const int blocks_out = (a.bytes_out + 127) / 128, scale_cols = (a.ff + 127) / 128, scale_rows = (a.dim + 127) / 128;
-    for (int c0 = col0; c0 < col1; c0 += 16) {
-        const int here = min(16, col1 - c0);
-        const int turn_row = 128 - (c0 & 127);  // rows from here on have the next block's scales
-        // an expert's block b goes to warp (expert * blocks + b) % 16, whichever experts are chosen beside it
-        struct Step {
-            int pos, b;
-        };
-        auto enter = [&](Step &s) {
-            while (s.pos < count) {
-                s.b = (warp - lists.active[s.pos] * blocks_out) & (kFewWarps - 1);
-                if (s.b < blocks_out) return;
-                ++s.pos;
-            }
-        };
-        auto next = [&](Step &s) {
-            s.b += kFewWarps;
-            if (s.b >= blocks_out) ++s.pos, enter(s);
-        };
-        Step now{0, 0}, ahead{0, 0};
-        enter(now), enter(ahead);
-        FewQueue queue(few_smem, at.queue, at.depth, warp);
-        const size_t four = (size_t)4 * a.ld_out;
-        const uint8_t *lane_w = a.w2 + ((size_t)c0 + (lane >> 3)) * a.ld_out + (lane & 7) * 16;
-        const float *lane_s = FP8 ? a.s2 + (size_t)min((c0 >> 7) + lane, scale_rows - 1) * scale_cols : nullptr;  // lanes 0 and 1: of this block and the next
-        auto issue = [&] {
-            if (ahead.pos < count) {
-                const int e = lists.active[ahead.pos];
-                const uint8_t *low = lane_w + (size_t)e * a.dim * a.ld_out + ahead.b * 128;
-                const int left = ahead.b * 128 + (lane & 7) * 16 < a.bytes_out ? here - (lane >> 3) : 0;
-                queue.copy(low, low + 2 * four, four, left > 0, left > 4, left > 8, left > 12);
-                if (FP8 && lane < 2) queue.copy_scale(lane_s + (size_t)e * scale_rows * scale_cols + ahead.b);
-                next(ahead);
-            }
-            queue.asked();
-        };
-        for (int i = 0; i < at.depth; ++i) issue();
-        constexpr int ENTRIES = FP8 ? 16 : 8;  // of either half of a block, a lane's
-        float h[2][ENTRIES];
-        auto fetch = [&](const Step &s, int n) {  // a column's inner numbers; of a column that is not there: zeros
-            const bool mine = n * 8 + g < __popc(lists.tokens[s.pos]);
-            const int c = mine ? lists.column[s.pos * 32 + n * 8 + g] : 0;
-            const float *row = a.inner + ((size_t)(c >> 8) * a.top + (c & 255)) * a.ld_inner;
+    if (warp == 0) {  // the experts' groups of up to GROUP tokens, in order
+        int n = 0;
+        for (int p0 = 0; p0 < count; p0 += 32) {
+            const int mine = p0 + lane < count ? (__popc(lists.tokens[p0 + lane]) + GROUP - 1) / GROUP : 0;
+            int before = mine;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int k = s.b * 8 * ENTRIES + u * 4 * ENTRIES + t4 * ENTRIES;
-#pragma unroll
-                for (int i = 0; i < ENTRIES; i += 4) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (mine && k < a.ld_inner) v = tl::ld_cg(reinterpret_cast<const uint4 *>(row + k + i));
-                    h[u][i] = __uint_as_float(v.x), h[u][i + 1] = __uint_as_float(v.y), h[u][i + 2] = __uint_as_float(v.z), h[u][i + 3] = __uint_as_float(v.w);
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, before, o);
+                if (lane >= o) before += v;
+            }
+            for (int j = 0; j < mine; ++j) group[n + before - mine + j] = (p0 + lane) * 4 + j;
+            n += __shfl_sync(0xffffffffu, before, 31);
+        }
+        if (lane == 0) group[pairs] = n;
+    }
+    __syncthreads();
+    const int groups = group[pairs], outs = (a.dim + 127) / 128, of_group = outs * a.splits, items = groups * of_group, blocks = (a.ff + ENTRIES - 1) / ENTRIES;
+    const int scale_cols = (a.ff + 127) / 128, scale_rows = (a.dim + 127) / 128;
+    struct Item {
+        int pos, first, tokens, n, m, split, b0, b1;  // n: columns of the products; b0, b1: blocks of the reduction
+    };
+    auto item_of = [&](int i) {
+        Item it;
+        const int entry = group[i / of_group], r = i % of_group;
+        it.pos = entry >> 2, it.first = (entry & 3) * GROUP, it.tokens = min(GROUP, __popc(lists.tokens[it.pos]) - it.first), it.n = (it.tokens * TERMS + 15) & ~15;
+        it.m = r / a.splits, it.split = r % a.splits;
+        it.b0 = blocks * it.split / a.splits, it.b1 = blocks * (it.split + 1) / a.splits;
+        return it;
+    };
+    if (warp == 0) {
+        if (g_elect_one()) {
+            int s = 0;
+            uint32_t ph = 1;
+            bool ok = true;
+            for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
+                const Item it = item_of(i);
+                for (int b = it.b0; b < it.b1; ++b) {
+                    if (!(ok = tc_wait_one(bars.empty + 8 * s, ph, bars.dead))) break;
+                    g_mbar_expect_tx(bars.full + 8 * s, kFewStage);
+                    few_tma(g_smem_u32(few_smem + at.ring) + s * kFewStage, &map, b * 128, it.m * 128, lists.active[it.pos], bars.full + 8 * s);
+                    if (++s == at.stages) s = 0, ph ^= 1u;
                 }
             }
-        };
-        if (now.pos < count) fetch(now, 0);
-        while (now.pos < count) {
-            const FewPiece p = queue.next<FP8>();
-            const float scale_a = FP8 && g < turn_row ? p.scale.x : p.scale.y, scale_b = FP8 && g + 8 < turn_row ? p.scale.x : p.scale.y;
-            const int columns = __popc(lists.tokens[now.pos]);
-            const uint16_t *column = lists.column + now.pos * 32;
-            Step later = now;
-            next(later);
+        }
+    } else if (warp == 1) {
+        if (g_elect_one()) {
+            int s = 0, buf = 0, place = 0;
+            uint32_t ph = 0, acc_ph = 1, cols_ph = 0;
+            bool ok = true;
+            const uint32_t ring = g_smem_u32(few_smem + at.ring);
+            for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
+                const Item it = item_of(i);
+                const int cols_block = (it.tokens * TERMS + 7) / 8 * 1024;
+                const uint32_t cols = g_smem_u32(few_smem + at.cols) + place * FewSecondSmem::kCols;
+                if (!(ok = tc_wait_one(bars.cols_full + 8 * place, cols_ph, bars.dead))) break;
+                for (int b = it.b0; b < it.b1; ++b) {
+                    if (FP8 || b == it.b0) ok = tc_wait_one(bars.acc_empty + 8 * buf, acc_ph, bars.dead);
+                    if (!ok || !(ok = tc_wait_one(bars.full + 8 * s, ph, bars.dead))) break;
+                    g_tc_fence_after();
+                    const uint64_t w = g_smem_desc_sw128(ring + s * kFewStage, 0, 1024), h = g_smem_desc_sw128(cols + (b - it.b0) * cols_block, 0, 1024);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                if (n * 8 >= columns) break;
-                if (n > 0) fetch(now, n);
-                constexpr int TERMS = FP8 ? 1 : 2, WORDS = FP8 ? 8 : 4;
-                uint32_t x[2][TERMS][WORDS];
-                float down = 1.f;
-                int e = 0;
-                if constexpr (FP8) {  // a power of two for a column's 128 numbers of this block, which the block's promotion takes back
-                    uint32_t most = 0;
+                    for (int k = 0; k < 4; ++k)
+                        few_product<FP8>(tmem + buf * kFewSecondN, w + 2 * k, h + 2 * k, few_idesc<FP8>(it.n), FP8 ? k > 0 : b > it.b0 || k > 0);
+                    const bool last = FP8 || b == it.b1 - 1;
+                    if (last) g_tc_commit(bars.acc_full + 8 * buf);
+                    g_tc_commit(bars.empty + 8 * s);
+                    if (++s == at.stages) s = 0, ph ^= 1u;
+                    if (last && ++buf == BUFFERS) buf = 0, acc_ph ^= 1u;
+                }
+                g_tc_commit(bars.cols_empty + 8 * place);
+                if (++place == 2) place = 0, cols_ph ^= 1u;
+            }
+        }
+    } else if (warp >= 4 && warp < 8) {  // the columns of an item, two items ahead at most
+        int place = 0;
+        uint32_t cols_ph = 1;
+        for (int i = blockIdx.x; i < items; i += gridDim.x) {
+            const Item it = item_of(i);
+            const int cols_block = (it.tokens * TERMS + 7) / 8 * 1024, here = it.b1 - it.b0;
+            unsigned char *cols = few_smem + at.cols + place * FewSecondSmem::kCols;
+            float *factor = factors + place * (FewSecondSmem::kFactors / 4);
+            const float *scales = FP8 ? a.s2 + ((size_t)lists.active[it.pos] * scale_rows + it.m) * scale_cols : nullptr;
+            if (!tc_wait(bars.cols_empty + 8 * place, cols_ph, bars.dead)) break;
+            const int runs = FP8 ? here : (here + 1) / 2, all = it.tokens * runs;  // of 128 entries
+            constexpr int H_AT_ONCE = 4;
+            for (int j0 = warp - 4; j0 < all; j0 += 4 * H_AT_ONCE) {
+                float v[H_AT_ONCE][4], scale[H_AT_ONCE];
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
-#pragma unroll
-                        for (int i = 0; i < ENTRIES; ++i) most = max(most, __float_as_uint(h[u][i]) & 0x7fffffffu);
-                    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                    e = few_exponent(__uint_as_float(most)), down = few_exp2(-e);
+                for (int u = 0; u < H_AT_ONCE; ++u) {
+                    const int j = j0 + 4 * u, c = j / runs, r = j - c * runs, k = it.b0 * ENTRIES + r * 128 + lane * 4;
+                    v[u][0] = v[u][1] = v[u][2] = v[u][3] = scale[u] = 0.f;
+                    if (c < it.tokens) {
+                        const int column = lists.column[it.pos * 32 + it.first + c];
+                        if (k < a.ld_inner) {
+                            const uint4 w = tl::ld_cg(reinterpret_cast<const uint4 *>(a.inner + ((size_t)(column >> 8) * a.top + (column & 255)) * a.ld_inner + k));
+                            v[u][0] = __uint_as_float(w.x), v[u][1] = __uint_as_float(w.y), v[u][2] = __uint_as_float(w.z), v[u][3] = __uint_as_float(w.w);
+                        }
+                        if constexpr (FP8) scale[u] = __ldg(scales + it.b0 + r);
+                    }
                 }
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < H_AT_ONCE; ++u) {
+                    const int j = j0 + 4 * u, c = j / runs, r = j - c * runs;
+                    if (c >= it.tokens) break;
+                    if constexpr (FP8) {
+                        const uint32_t most = __reduce_max_sync(0xffffffffu, few_most4(v[u]));
+                        const int e = few_exponent(__uint_as_float(most));
+                        const float up = few_exp2(8 - e);
 #pragma unroll
-                    for (int i = 0; i < WORDS; ++i) {
-                        const float lo = h[u][2 * i], hi = h[u][2 * i + 1];
-                        if constexpr (FP8) {
-                            x[u][0][i] = few_half2(lo * down, hi * down);
-                        } else {
-                            x[u][0][i] = tl::pack2<bf16>(lo, hi);
-                            const float2 f = tl::unpack2<bf16>(x[u][0][i]);
-                            // an infinity has no second term
-                            x[u][1][i] = tl::pack2<bf16>(fabsf(f.x) < INFINITY ? lo - f.x : 0.f, fabsf(f.y) < INFINITY ? hi - f.y : 0.f);
+                        for (int q = 0; q < 4; ++q) v[u][q] *= up;
+                        float f = most < 0x7f800000u ? few_exp2(e - 8) * scale[u] : __int_as_float(0x7fffffff);  // of a term
+#pragma unroll
+                        for (int term = 0; term < TERMS; ++term, f *= 0.0625f) {
+                            *reinterpret_cast<uint32_t *>(cols + r * cols_block + few_swizzled(term * it.tokens + c, lane * 4)) = few_term(v[u]);
+                            if (lane == 0) factor[r * kFewSecondN + term * it.tokens + c] = f;
+                        }
+                    } else {
+                        const int b = r * 2 + (lane >> 4);
+                        if (b < here) {
+                            uint32_t hi[2], lo[2];
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                hi[q] = tl::pack2<bf16>(v[u][2 * q], v[u][2 * q + 1]);
+                                const float2 f = tl::unpack2<bf16>(hi[q]);
+                                // an infinity has no second term
+                                lo[q] = tl::pack2<bf16>(fabsf(f.x) < INFINITY ? v[u][2 * q] - f.x : 0.f, fabsf(f.y) < INFINITY ? v[u][2 * q + 1] - f.y : 0.f);
+                            }
+                            *reinterpret_cast<uint2 *>(cols + b * cols_block + few_swizzled(c, (lane & 15) * 8)) = make_uint2(hi[0], hi[1]);
+                            *reinterpret_cast<uint2 *>(cols + b * cols_block + few_swizzled(it.tokens + c, (lane & 15) * 8)) = make_uint2(lo[0], lo[1]);
                         }
                     }
-                if (n == 0 && columns <= 8 && later.pos < count) fetch(later, 0);  // on its way under the products
-                float d[2][4] = {};
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int term = 0; term < TERMS; ++term) few_half<FP8>(p.a[u], p.b[u], x[u][term], d[u]);
-#pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    const int col = n * 8 + 2 * t4 + v;
-                    const int up = FP8 ? __shfl_sync(0xffffffffu, e, (2 * t4 + v) * 4) : 0;
-                    if (col < columns) {
-                        const int t = column[col] >> 8;
-                        const float f = factor[t * a.top + (column[col] & 255)] * few_exp2(up);
-                        float *to = sums + t * 17 + g;
-                        to[0] = fmaf(d[0][v] + d[1][v], FP8 ? f * scale_a : f, to[0]), to[8] = fmaf(d[0][2 + v] + d[1][2 + v], FP8 ? f * scale_b : f, to[8]);
-                    }
                 }
             }
-            __syncwarp();  // the next expert's column of a token may be another lane's
-            if (columns > 8 && later.pos < count) fetch(later, 0);
-            now = later;
-            issue();
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        __syncthreads();
-        const float *all = reinterpret_cast<const float *>(few_smem + at.sums);
-        for (int i = tid; i < 16 * a.tokens; i += kFewThreads) {
-            const int r = i % 16, t = i / 16;
-            if (r >= here) continue;
-            float y = 0.f;
-#pragma unroll
-            for (int w = 0; w < kFewWarps; ++w) y += all[w * sum_stride + t * 17 + r];
-            const int d = c0 + r;
-            for (int k = 0; k < a.top; ++k) {
-                const int e = idx[t * a.top + k];
-                if (e < a.experts) continue;
-                // an identity expert; no output at all: the token's logits are no numbers
-                y = e < a.outputs ? fmaf(factor[t * a.top + k], to_f(tl::ld_cg(a.x + (size_t)t * a.dim + d)), y) : __int_as_float(0x7fffffff);
-            }
-            if (a.shared) y = fmaf(a.side_w ? tl::ld_cg(a.side + t) : 1.f, to_f(tl::ld_cg(a.shared + (size_t)t * a.dim + d)), y);
-            static_cast<OUT *>(a.out)[(size_t)t * a.dim + d] = from_f<OUT>(y);
-        }
-        if (c0 + 16 < col1) {
-            __syncthreads();
-            for (int i = lane; i < sum_stride; i += 32) sums[i] = 0.f;
+            tl::g_fence_proxy_async();
             __syncwarp();
+            if (lane == 0) g_mbar_arrive(bars.cols_full + 8 * place);
+            if (++place == 2) place = 0, cols_ph ^= 1u;
         }
+    } else if (warp >= 8) {
+        const int quarter = warp & 3, half = (warp - 8) >> 2, row = quarter * 32 + lane, me = tid - 256;
+        int buf = 0, place = 0;
+        uint32_t acc_ph = 0, cols_ph = 0;
+        for (int i = blockIdx.x; i < items; i += gridDim.x) {
+            const Item it = item_of(i);
+            bool ok = tc_wait(bars.cols_full + 8 * place, cols_ph, bars.dead);  // their factors
+            const float *factor = factors + place * (FewSecondSmem::kFactors / 4);
+            auto add = [&](auto wide) {  // the columns of this half: 8, or 16
+                constexpr int COLS = decltype(wide)::value;
+                float acc[COLS];
+#pragma unroll
+                for (int c = 0; c < COLS; ++c) acc[c] = 0.f;
+                const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * COLS;
+                for (int b = it.b0; b < (FP8 ? it.b1 : it.b0 + 1); ++b) {
+                    float4 f[COLS / 4];
+                    if constexpr (FP8) {
+#pragma unroll
+                        for (int c = 0; c < COLS / 4; ++c) f[c] = *reinterpret_cast<const float4 *>(factor + (b - it.b0) * kFewSecondN + half * COLS + c * 4);
+                    }
+                    ok &= tc_wait(bars.acc_full + 8 * buf, acc_ph, bars.dead);
+                    g_tc_fence_after();
+                    uint32_t v[COLS];
+                    few_ld(from + buf * kFewSecondN, v);
+                    g_tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) g_mbar_arrive(bars.acc_empty + 8 * buf);
+#pragma unroll
+                    for (int c = 0; c < COLS; ++c) {
+                        if constexpr (FP8) acc[c] = fmaf(__uint_as_float(v[c]), c % 4 == 0 ? f[c / 4].x : c % 4 == 1 ? f[c / 4].y : c % 4 == 2 ? f[c / 4].z : f[c / 4].w, acc[c]);
+                        else acc[c] = __uint_as_float(v[c]);
+                    }
+                    if (++buf == BUFFERS) buf = 0, acc_ph ^= 1u;
+                }
+#pragma unroll
+                for (int c = 0; c < COLS; ++c) sums[(half * COLS + c) * 128 + row] = acc[c];
+            };
+            if (it.n == 16) add(std::integral_constant<int, 8>());
+            else add(std::integral_constant<int, 16>());
+            __syncwarp();  // every lane has used its factors: the sums that are in memory hold them
+            if (lane == 0) g_mbar_arrive(bars.cols_empty + 8 * place);
+            if (++place == 2) place = 0, cols_ph ^= 1u;
+            const float bad = tc_verdict(ok, bars.dead);
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            for (int j = me; j < it.tokens * 128; j += 256) {
+                const int r = j & 127, c = j >> 7, column = lists.column[it.pos * 32 + it.first + c], d = it.m * 128 + r;
+                float y = sums[c * 128 + r];
+#pragma unroll
+                for (int term = 1; term < TERMS; ++term) y += sums[(term * it.tokens + c) * 128 + r];
+                if (d < a.dim) a.part[((size_t)it.split * pairs + (column >> 8) * a.top + (column & 255)) * a.dim + d] = y * bad;
+            }
+            // ---- the last item of these output columns: all partial sums, in order
+            __threadfence();
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (me == 0) *bars.last = atomicAdd(a.finished + it.m, 1u);
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (*bars.last != static_cast<uint32_t>(groups * a.splits - 1)) continue;
+            __threadfence();
+            for (int j = me; j < a.tokens * 32; j += 256) {
+                const int t = j >> 5, d = it.m * 128 + (j & 31) * 4;  // four columns; a row has a multiple of eight
+                if (d >= a.dim) continue;
+                float y[4] = {0.f, 0.f, 0.f, 0.f};
+                constexpr int AT_ONCE = 8;
+                for (int k0 = 0; k0 < a.top; k0 += AT_ONCE) {
+                    float4 z[AT_ONCE];
+                    int e[AT_ONCE];
+#pragma unroll
+                    for (int u = 0; u < AT_ONCE; ++u) z[u] = make_float4(0.f, 0.f, 0.f, 0.f), e[u] = k0 + u < a.top ? idx[t * a.top + k0 + u] : -1;
+                    for (int s = 0; s < a.splits; ++s)
+#pragma unroll
+                        for (int u = 0; u < AT_ONCE; ++u)
+                            if (e[u] >= 0 && e[u] < a.experts) {
+                                const uint4 w = tl::ld_cg(reinterpret_cast<const uint4 *>(a.part + ((size_t)s * pairs + t * a.top + k0 + u) * a.dim + d));
+                                z[u].x += __uint_as_float(w.x), z[u].y += __uint_as_float(w.y), z[u].z += __uint_as_float(w.z), z[u].w += __uint_as_float(w.w);
+                            }
+#pragma unroll
+                    for (int u = 0; u < AT_ONCE; ++u) {
+                        if (e[u] < 0) continue;
+                        const float w = gate[t * a.top + k0 + u];
+                        if (e[u] >= a.experts) {
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) y[c] = few_identity(a, e[u], w, t, d + c, y[c]);
+                        } else {
+                            y[0] = fmaf(w, z[u].x, y[0]), y[1] = fmaf(w, z[u].y, y[1]), y[2] = fmaf(w, z[u].z, y[2]), y[3] = fmaf(w, z[u].w, y[3]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) few_store<OUT>(a, t, d + c, y[c]);
+            }
+        }
+        if (items == 0)  // every choice an identity expert, or none
+            for (int j = blockIdx.x * 256 + me; j < a.tokens * a.dim; j += gridDim.x * 256) {
+                const int t = j / a.dim, d = j % a.dim;
+                float y = 0.f;
+                for (int k = 0; k < a.top; ++k) y = few_identity(a, idx[t * a.top + k], gate[t * a.top + k], t, d, y);
+                few_store<OUT>(a, t, d, y);
+            }
+    }
+    __syncwarp();
+    g_tc_fence_before();
+    __syncthreads();
+    if (warp == 2) {
+        tc_settle(bars.dead);
+        g_tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(TMEM) : "memory");
     }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
 
 constexpr int kFewSmem = 227 * 1024, kFewMostGrid = 1024;
+constexpr int kFewPrefetch = 40 << 20;  // a third of L2
 
-// CTAs of the first launch: as many clusters as are resident at once, which a device's SMs in groups decide (132 CTAs of a B200; in pairs all 148 are, but then
-// every CTA reads half of the router's rows: 1 token of the benchmark's experts 30.2 us in 8 bits against 28.6, 32 tokens 183 and 184).
+// CTAs of the first launch: as many clusters as are resident at once, which a device's SMs in groups decide (132 CTAs of a B200).
 template <typename K>
-static int few_grid(K kernel, int smem) {
+static int few_grid(K kernel) {
     static std::atomic<int> known[64];
     int device = 0;
     cudaGetDevice(&device);
     if (device >= 0 && device < 64 && known[device].load(std::memory_order_acquire) > 0) return known[device].load(std::memory_order_relaxed);
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(kFewCluster), cfg.blockDim = dim3(kFewThreads), cfg.dynamicSmemBytes = smem;
+    cfg.gridDim = dim3(kFewCluster), cfg.blockDim = dim3(kFewThreads), cfg.dynamicSmemBytes = kFewSmem;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = kFewCluster, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
@@ -747,61 +864,73 @@ static int few_grid(K kernel, int smem) {
     return grid;
 }
 
-// Two places of the queue at least: a piece on its way while one is used.
-static bool few_fits(const FewFirstSmem &s) { return s.depth >= 2 && s.total <= kFewSmem; }
-constexpr int kFewPrefetch = 40 << 20;  // a third of L2
+// Two stages of the ring at least: one on its way while one is used.
+static bool few_fits(int tokens, int nt, int dim, int outputs, int experts, int top, int groups, bool fp8) {
+    const FewFirstSmem a(tokens, nt, dim, outputs, experts, top, groups, fp8, kFewSmem);
+    const FewSecondSmem b(tokens, experts, top, kFewSmem);
+    return a.stages >= 2 && a.total <= kFewSmem && b.stages >= 2 && b.total <= kFewSmem;
+}
 
 static int few_inner_ld(int ff) { return (ff + 15) / 16 * 16; }
-static int few_nt(int tokens) { return tokens <= 8 ? 1 : tokens <= 16 ? 2 : 4; }
+static int few_nt(int tokens) { return ceil_div(tokens, 8); }
+static int few_blocks(int ff, bool fp8) { return ceil_div(ff, fp8 ? 128 : 64); }
+
+// Parts of the second product's reduction: as many as an item's columns need, or more where they let the SMs end closer together, by the blocks that the busiest
+// takes (and two more an item for what it costs besides), if no two tokens choose the same expert.  The number of experts does not matter: it changes no bits.
+static int few_splits(int tokens, int dim, int top, int ff, bool fp8) {
+    const int blocks = few_blocks(ff, fp8), outs = ceil_div(dim, 128);
+    const int fewest = ceil_div(blocks, kFewItemBlocks);
+    int best = fewest;
+    long long least = 0;
+    for (int s = fewest; s <= std::max(fewest, std::min(blocks, 8)); ++s) {
+        const long long time = (long long)ceil_div(tokens * top * outs * s, 148) * (ceil_div(blocks, s) + 2);
+        if (s == fewest || time < least) best = s, least = time;
+    }
+    return best;
+}
 
 static size_t few_align(size_t n) { return (n + 15) & ~(size_t)15; }
-static size_t few_bytes(int tokens, int top, int ff) {
+static size_t few_bytes(int tokens, int dim, int top, int ff, bool fp8) {
     const size_t pairs = (size_t)tokens * top;
-    return few_align(pairs * 4) * 2 + few_align((size_t)tokens * 4) + pairs * few_inner_ld(ff) * 4;
+    return few_align(pairs * 4) * 2 + few_align((size_t)tokens * 4) + few_align((size_t)ceil_div(dim, 128) * 4) + pairs * few_inner_ld(ff) * 4 +
+           (size_t)few_splits(tokens, dim, top, ff, fp8) * pairs * dim * 4;
 }
 
-template <typename K>
-static int few_ready(K kernel, tl::PerDevice &ready) {
+template <typename K, typename... A>
+static int few_launch(K kernel, tl::PerDevice &ready, int grid, int cluster, int smem, cudaStream_t st, const A &...args) {
     int device = 0;
     cudaGetDevice(&device);
-    if (ready(device, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem) == cudaSuccess; })) return TL_OK;
-    cudaGetLastError();
-    return tl::fail(TL_ECUDA, "moe_few: no shared memory");
-}
-template <typename K>
-static int few_launch(K kernel, dim3 grid, int cluster, int smem, cudaStream_t st, const FewArgs &a) {
+    if (!ready(device, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem) == cudaSuccess; })) {
+        cudaGetLastError();
+        return tl::fail(TL_ECUDA, "moe_few: no shared memory");
+    }
+    if (grid == 0) grid = few_grid(kernel);
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid, cfg.blockDim = dim3(kFewThreads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+    cfg.gridDim = dim3(grid), cfg.blockDim = dim3(kFewThreads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cluster, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr, cfg.numAttrs = tl::use_pdl() ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, kernel, a);
+    cudaLaunchKernelEx(&cfg, kernel, args...);
     TL_LAUNCH_CHECK("moe_few");
     return TL_OK;
 }
 
-template <typename K>
-static int few_first(K kernel, tl::PerDevice &ready, int smem, cudaStream_t st, FewArgs &a) {
-    if (int e = few_ready(kernel, ready)) return e;
-    const int grid = few_grid(kernel, kFewSmem);
-    a.runs = grid * kFewTeams, a.prefetch = kFewPrefetch / grid;
-    return few_launch(kernel, dim3(grid), kFewCluster, smem, st, a);
-}
-template <typename K>
-static int few_second(K kernel, tl::PerDevice &ready, int smem, cudaStream_t st, const FewArgs &a) {
-    if (int e = few_ready(kernel, ready)) return e;
-    return few_launch(kernel, dim3(std::min(sm_count(), a.dim)), 1, smem, st, a);
-}
 template <bool FP8, int NT>
-static int few_run(FewArgs &a, int first_smem, bool wide, cudaStream_t st) {
-    static tl::PerDevice gated, plain, second16, second32;
-    if (int e = a.w1 ? few_first(moe_few_first_kernel<FP8, true, NT>, gated, first_smem, st, a) : few_first(moe_few_first_kernel<FP8, false, NT>, plain, first_smem, st, a)) return e;
-    const int smem = FewSecondSmem(a.tokens, a.experts, a.top, FP8, kFewSmem).total;
-    return wide ? few_second(moe_few_second_kernel<FP8, NT, float>, second32, smem, st, a) : few_second(moe_few_second_kernel<FP8, NT, bf16>, second16, smem, st, a);
+static int few_run(const CUtensorMap &m0, const CUtensorMap &m1, const CUtensorMap &m2, const FewArgs &a, bool gated, bool wide, cudaStream_t st) {
+    static tl::PerDevice with, without, second16, second32;
+    const int smem = FewFirstSmem(a.tokens, NT, a.dim, a.outputs, a.experts, a.top, a.group_count, FP8, kFewSmem).total;
+    if (int e = gated ? few_launch(moe_few_first_kernel<FP8, true, NT>, with, 0, kFewCluster, smem, st, m0, m1, a)
+                      : few_launch(moe_few_first_kernel<FP8, false, NT>, without, 0, kFewCluster, smem, st, m0, m1, a))
+        return e;
+    const int smem2 = FewSecondSmem(a.tokens, a.experts, a.top, kFewSmem).total;
+    return wide ? few_launch(moe_few_second_kernel<FP8, float>, second32, sm_count(), 1, smem2, st, m2, a)
+                : few_launch(moe_few_second_kernel<FP8, bf16>, second16, sm_count(), 1, smem2, st, m2, a);
 }
+
+long long few_gave_up() { return tl::read_gave_up(); }
 
 }  // namespace tlb
 
@@ -812,12 +941,12 @@ extern "C" {
 int tlb_moe_few_tokens(int dim, int outputs, int experts, int top, int group_count, int fp8) {
     if (dim <= 0 || outputs <= 0 || outputs > kFewOutputs || experts <= 0 || experts > outputs || top <= 0 || top > outputs || top > 255 || group_count < 0) return 0;
     int tokens = std::min(kFewTokens, kFewPairs / top);
-    while (tokens > 0 && !few_fits(FewFirstSmem(tokens, few_nt(tokens), dim, outputs, experts, top, group_count, fp8 != 0, kFewSmem))) --tokens;
+    while (tokens > 0 && !few_fits(tokens, few_nt(tokens), dim, outputs, experts, top, group_count, fp8 != 0)) --tokens;
     return tokens;
 }
 
-size_t tlb_moe_few_workspace(int tokens, int top, int experts, int ff) {
-    return tokens <= 0 || top <= 0 || experts <= 0 || ff <= 0 ? 0 : few_bytes(tokens, top, ff);
+size_t tlb_moe_few_workspace(int tokens, int dim, int experts, int top, int ff, int fp8) {
+    return tokens <= 0 || dim <= 0 || top <= 0 || experts <= 0 || ff <= 0 ? 0 : few_bytes(tokens, dim, top, ff, fp8 != 0);
 }
 
 int tlb_moe_few(const tlb_moe_few_layer *l, const void *x, int tokens, const void *shared, void *out, int out_f32, void *workspace, size_t workspace_bytes, void *stream) {
@@ -834,25 +963,41 @@ int tlb_moe_few(const tlb_moe_few_layer *l, const void *x, int tokens, const voi
     if (dim % 8 || l->ld_in < dim * size || l->ld_out < ff * size || l->ld_in % 16 || l->ld_out % 16 || !tl::aligned16(x) || !tl::aligned16(l->router) ||
         !tl::aligned16(l->side_w) || !tl::aligned16(l->w_gate) || !tl::aligned16(l->w_up) || !tl::aligned16(l->w_down) || !tl::aligned16(workspace))
         return tl::fail(TL_EINVAL, "moe_few: rows must be whole 16-byte pieces");
-    if (workspace_bytes < few_bytes(tokens, top, ff)) return tl::fail(TL_EINVAL, "moe_few: workspace too small");
+    if (workspace_bytes < few_bytes(tokens, dim, top, ff, fp8 != 0)) return tl::fail(TL_EINVAL, "moe_few: workspace too small");
     const size_t pairs = (size_t)tokens * top;
     FewArgs a{};
     a.x = (const bf16 *)x, a.router = (const bf16 *)l->router, a.router_bias = (const bf16 *)l->router_bias, a.choice_bias = (const bf16 *)l->choice_bias;
     a.side_w = (const bf16 *)l->side_w, a.tokens = tokens, a.dim = dim, a.outputs = outputs, a.experts = experts, a.top = top, a.scoring = l->scoring, a.group_count = groups;
     a.group_keep = l->group_keep, a.weight_scale = l->weight_scale;
-    a.w0 = (const uint8_t *)(l->w_gate ? l->w_gate : l->w_up), a.w1 = (const uint8_t *)(l->w_gate ? l->w_up : nullptr), a.w2 = (const uint8_t *)l->w_down;
     a.s0 = l->w_gate ? l->s_gate : l->s_up, a.s1 = l->w_gate ? l->s_up : nullptr, a.s2 = l->s_down;
-    a.ff = ff, a.ld_in = l->ld_in, a.ld_out = l->ld_out, a.bytes_in = (int)few_align((size_t)dim * size), a.bytes_out = (int)few_align((size_t)ff * size);
+    a.ff = ff, a.w2 = (const uint8_t *)l->w_down, a.ld_out = l->ld_out, a.row_out = ff * size / 16 * 16, a.prefetch = kFewPrefetch / sm_count();
     a.act = l->act, a.limit = l->limit, a.slope = l->slope, a.shared = (const bf16 *)shared, a.out = out;
     uint8_t *at = (uint8_t *)workspace;
     a.idx = (int32_t *)at, at += few_align(pairs * 4);
     a.gate = (float *)at, at += few_align(pairs * 4);
     a.side = (float *)at, at += few_align((size_t)tokens * 4);
-    a.inner = (float *)at, a.ld_inner = few_inner_ld(ff), a.room = kFewSmem;
-    const int nt = few_nt(tokens), smem = FewFirstSmem(tokens, nt, dim, outputs, experts, top, groups, fp8 != 0, kFewSmem).total;
+    a.finished = (uint32_t *)at, at += few_align((size_t)ceil_div(dim, 128) * 4);
+    a.inner = (float *)at, a.ld_inner = few_inner_ld(ff), at += pairs * a.ld_inner * 4;
+    a.part = (float *)at, a.splits = few_splits(tokens, dim, top, ff, fp8 != 0), a.room = kFewSmem;
+    // what lies between a row's last number and the next row is read as zeros
+    const uint64_t in = (uint64_t)dim * size, inner = (uint64_t)ff * size;
+    CUtensorMap m0, m1, m2;
+    if (int e = tc_map_bytes3(&m0, l->w_gate ? l->w_gate : l->w_up, in, ff, experts, l->ld_in, l->w_gate ? 64 : 128)) return e;
+    if (int e = tc_map_bytes3(&m1, l->w_up, in, ff, experts, l->ld_in, 64)) return e;
+    if (int e = tc_map_bytes3(&m2, l->w_down, inner, dim, experts, l->ld_out, 128)) return e;
+    const int nt = few_nt(tokens);
     const cudaStream_t st = as_stream(stream);
-    if (fp8) return nt == 1 ? few_run<true, 1>(a, smem, out_f32, st) : nt == 2 ? few_run<true, 2>(a, smem, out_f32, st) : few_run<true, 4>(a, smem, out_f32, st);
-    return nt == 1 ? few_run<false, 1>(a, smem, out_f32, st) : nt == 2 ? few_run<false, 2>(a, smem, out_f32, st) : few_run<false, 4>(a, smem, out_f32, st);
+    const bool gated = l->w_gate != nullptr, wide = out_f32 != 0;
+    switch (nt + (fp8 ? 4 : 0)) {
+        case 1: return few_run<false, 1>(m0, m1, m2, a, gated, wide, st);
+        case 2: return few_run<false, 2>(m0, m1, m2, a, gated, wide, st);
+        case 3: return few_run<false, 3>(m0, m1, m2, a, gated, wide, st);
+        case 4: return few_run<false, 4>(m0, m1, m2, a, gated, wide, st);
+        case 5: return few_run<true, 1>(m0, m1, m2, a, gated, wide, st);
+        case 6: return few_run<true, 2>(m0, m1, m2, a, gated, wide, st);
+        case 7: return few_run<true, 3>(m0, m1, m2, a, gated, wide, st);
+        default: return few_run<true, 4>(m0, m1, m2, a, gated, wide, st);
+    }
 }
 
 }  // extern "C"

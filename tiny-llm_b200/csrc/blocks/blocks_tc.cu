@@ -36,4 +36,10 @@ int tc_map_bytes(CUtensorMap *map, const void *ptr, uint64_t cols, uint64_t rows
     return tc_encode(map, ptr, 2, dims, strides, box, CU_TENSOR_MAP_DATA_TYPE_UINT8);
 }
 
+int tc_map_bytes3(CUtensorMap *map, const void *ptr, uint64_t cols, uint64_t rows, uint64_t matrices, uint64_t stride, uint32_t box_rows) {
+    const cuuint64_t dims[3] = {cols, rows, matrices}, strides[2] = {stride, stride * rows};
+    const cuuint32_t box[3] = {128, box_rows, 1};
+    return tc_encode(map, ptr, 3, dims, strides, box, CU_TENSOR_MAP_DATA_TYPE_UINT8);
+}
+
 }  // namespace tlb

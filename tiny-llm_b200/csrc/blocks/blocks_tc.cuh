@@ -26,6 +26,7 @@ using tl::tc_wait_one;
 
 long long flash_tc_gave_up();  // of the attention kernels
 long long f8_gave_up();        // of the 8-bit products
+long long few_gave_up();       // of the experts for few tokens
 
 // kind::f16 instruction descriptor: bf16 x bf16 -> f32, 128 rows, n columns; A K-major, B K-major or (b_mn) MN-major.
 __host__ __device__ __forceinline__ constexpr uint32_t tc_idesc(int n, bool b_mn = false) {
@@ -46,5 +47,7 @@ int tc_map_2d(CUtensorMap *map, const void *ptr, uint64_t cols, uint64_t rows, u
 int tc_map_3d(CUtensorMap *map, const void *ptr, uint64_t cols, uint64_t heads, uint64_t rows, uint64_t head, uint64_t row, uint32_t box_heads, uint32_t box_rows);
 // A matrix of bytes [rows, cols], rows `stride` (a multiple of 16) apart, in boxes of box_rows x 128.
 int tc_map_bytes(CUtensorMap *map, const void *ptr, uint64_t cols, uint64_t rows, uint64_t stride, uint32_t box_rows);
+// A stack of such matrices, one behind the other, a box in one of them.
+int tc_map_bytes3(CUtensorMap *map, const void *ptr, uint64_t cols, uint64_t rows, uint64_t matrices, uint64_t stride, uint32_t box_rows);
 
 }  // namespace tlb

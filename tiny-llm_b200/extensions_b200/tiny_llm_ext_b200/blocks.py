@@ -93,7 +93,7 @@ _SIGNATURES = {
     "tlb_moe_combine": (_I, [_VP, _VP, _VP, _VP, _VP, _I, _VP, _VP, _I, _I, _I, _I, _VP]),
     "tlb_argmax_rows": (_I, [_VP, _VP, _I, _I, _VP]),
     "tlb_moe_few_tokens": (_I, [_I, _I, _I, _I, _I, _I]),
-    "tlb_moe_few_workspace": (ctypes.c_size_t, [_I, _I, _I, _I]),
+    "tlb_moe_few_workspace": (ctypes.c_size_t, [_I, _I, _I, _I, _I, _I]),
     "tlb_moe_few": (_I, [_VP, _VP, _I, _VP, _VP, _I, _VP, ctypes.c_size_t, _VP]),
     "tlb_fp8_linear_workspace": (ctypes.c_size_t, [_I, _I]),
     "tlb_fp8_linear": (_I, [_VP, _LL, _VP, _I, _VP, _VP, _VP, _I, _I, _I, _VP, ctypes.c_size_t, _I, _VP]),
@@ -1198,7 +1198,7 @@ class MoeFew:
             raise RuntimeError("moe_few: tensors on two devices")
         self.device, self.width = router_w.get_device(), D
         self.tokens = moe_few_tokens(D, outputs, E, top, int(groups[0]), fp8)
-        self.workspace = lambda T: library().tlb_moe_few_workspace(T, top, E, inner)
+        self.workspace = lambda T: library().tlb_moe_few_workspace(T, D, E, top, inner, int(fp8))
         self.layer = FewLayer(*(_ptr(t) for t in self._keep), D, outputs, E, top, int(scoring), int(groups[0]), int(groups[1]), int(fp8), inner, w_up.shape[2] * size,
                               w_down.shape[2] * size, act, float(weight_scale), float(limit), float(slope))
         self._layer = ctypes.addressof(self.layer)
