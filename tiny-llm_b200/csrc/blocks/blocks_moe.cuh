@@ -69,6 +69,31 @@ __device__ __forceinline__ void moe_choose(float *z, float *p_all, float *best, 
     const bool keep = experts <= 32 * KEPT;
 #pragma unroll
     for (int i = 0; i < KEPT; ++i) kept[i] = keep && lane + 32 * i < experts ? ordered(z[lane + 32 * i]) : 0;
+    auto number = [](uint32_t v) { return v ? __uint_as_float(v & 0x80000000u ? v & 0x7fffffffu : ~v) : -INFINITY; };
+    if (keep && top <= 32) {  // lane k keeps choice k; the weights are made side by side, added in the choices' order
+        uint32_t my_v = 0, first = 0;
+        int my_i = 0x7fffffff;
+        for (int k = 0; k < top; ++k) {
+            uint32_t best_v = 0;
+            int bi = 0x7fffffff;
+#pragma unroll
+            for (int i = 0; i < KEPT; ++i)
+                if (kept[i] > best_v) best_v = kept[i], bi = lane + 32 * i;
+            const uint32_t most = __reduce_max_sync(0xffffffffu, best_v);
+            bi = __reduce_min_sync(0xffffffffu, best_v == most && most ? bi : 0x7fffffff);
+#pragma unroll
+            for (int i = 0; i < KEPT; ++i)
+                if (bi == lane + 32 * i) kept[i] = ordered(-INFINITY);
+            if (k == 0) first = most;
+            if (lane == k) my_v = most, my_i = bi;
+        }
+        const float bv = number(my_v);
+        const float p = scoring == 1 ? 1.0f / (1.0f + expf(-bv)) : scoring == 2 ? p_all[min(my_i, experts - 1)] : expf(bv - number(first));
+        if (scoring != 1)
+            for (int k = 0; k < top; ++k) denom += __shfl_sync(0xffffffffu, p, k);
+        if (lane < top) idx[lane] = my_i, gate[lane] = scoring == 1 ? p : scoring == 2 ? p / (denom + 1e-20f) * weight_scale : p / denom;
+        return;
+    }
     for (int k = 0; k < top; ++k) {
         uint32_t best_v = 0;
         int bi = 0x7fffffff;
@@ -84,7 +109,7 @@ __device__ __forceinline__ void moe_choose(float *z, float *p_all, float *best, 
         }
         const uint32_t most = __reduce_max_sync(0xffffffffu, best_v);
         bi = __reduce_min_sync(0xffffffffu, best_v == most && most ? bi : 0x7fffffff);
-        const float bv = most ? __uint_as_float(most & 0x80000000u ? most & 0x7fffffffu : ~most) : -INFINITY;
+        const float bv = number(most);
 #pragma unroll
         for (int i = 0; i < KEPT; ++i)
             if (bi == lane + 32 * i) kept[i] = ordered(-INFINITY);

@@ -29,7 +29,7 @@ constexpr int kFewThreads = 512, kFewWarps = 16;
 constexpr int kFewTokens = 32, kFewPairs = 512, kFewOutputs = 1024;
 constexpr int kFewStage = 128 * 128;  // a stage of the ring: 128 matrix rows of 128 bytes
 constexpr int kFewMostStages = 8;
-constexpr int kFewItemBlocks = 12;    // second launch: the most blocks of the reduction of an item
+constexpr int kFewItemCols = 48 * 1024, kFewItemBlocks = kFewItemCols / 1024;  // second launch: bytes of an item's columns, the most blocks of its reduction
 
 struct FewArgs {
     const bf16 *x, *router, *router_bias, *choice_bias, *side_w;
@@ -46,7 +46,7 @@ struct FewArgs {
     int32_t *idx;        // [tokens, top]
     float *gate;         // [tokens, top]
     float *side;         // [tokens]
-    uint32_t *finished;  // [blocks of 128 output columns]: items
+    uint32_t *finished;  // [blocks of 128 output columns][32 tokens]: partial sums that are written
     float *inner;        // [tokens * top, ld_inner], zero behind ff
     float *part;         // [splits][tokens * top, dim]
     int ld_inner, splits, room /* bytes of shared memory that a launch may use */;
@@ -88,30 +88,43 @@ __device__ __forceinline__ uint32_t few_most4(const float (&v)[4]) {  // magnitu
 }
 // Where byte `at` of row r of an operand lies: rows of 128 bytes in groups of 8, 16-byte pieces exchanged by row (128-byte swizzle).
 __device__ __forceinline__ uint32_t few_swizzled(int r, int at) { return r * 128 + (((at >> 4) ^ (r & 7)) << 4) + (at & 15); }
+// Products of a stage, its accumulator kept or begun.  Ahead of them two barriers are asked whether their phase is over: a question costs the thread that asks
+// some 200 cycles, which the products' own time hides.  `done` is arrived at if it is the accumulator's last stage, `used` in any case.
+#define FEW_BLOCK(KIND)                                                                                                                                       \
+    asm volatile(                                                                                                                                             \
+        "{\n\t.reg .pred p, q, on, begun, last;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"                                                                     \
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%8], %9;\n\t"                                                                                          \
+        "mbarrier.test_wait.parity.shared::cta.b64 q, [%10], %11;\n\t"                                                                                        \
+        "setp.eq.u32 on, %2, %2;\n\tsetp.ne.u32 begun, %12, 0;\n\tsetp.ne.u32 last, %13, 0;\n\t"                                                             \
+        "add.u64 a1, %3, 2;\n\tadd.u64 a2, %3, 4;\n\tadd.u64 a3, %3, 6;\n\tadd.u64 b1, %4, 2;\n\tadd.u64 b2, %4, 4;\n\tadd.u64 b3, %4, 6;\n\t"                  \
+        "tcgen05.mma.cta_group::1.kind::" KIND " [%2], %3, %4, %5, begun;\n\t"                                                                                \
+        "tcgen05.mma.cta_group::1.kind::" KIND " [%2], a1, b1, %5, on;\n\t"                                                                                   \
+        "tcgen05.mma.cta_group::1.kind::" KIND " [%2], a2, b2, %5, on;\n\t"                                                                                   \
+        "tcgen05.mma.cta_group::1.kind::" KIND " [%2], a3, b3, %5, on;\n\t"                                                                                   \
+        "@last tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%6];\n\t"                                                               \
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%7];\n\t"                                                                     \
+        "selp.u32 %0, 1, 0, p;\n\tselp.u32 %1, 1, 0, q;\n\t}"                                                                                                \
+        : "=r"(over0), "=r"(over1)                                                                                                                            \
+        : "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(done), "r"(used), "r"(bar0), "r"(parity0), "r"(bar1), "r"(parity1), "r"(begun), "r"(last)                   \
+        : "memory")
 template <bool FP8>
-__device__ __forceinline__ void few_product(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    if constexpr (FP8)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-                     "r"(accumulate)
-                     : "memory");
-    else g_tc_mma(d, a, b, idesc, accumulate);
+__device__ __forceinline__ void few_block(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t begun, uint32_t last, uint32_t done, uint32_t used, uint32_t bar0,
+                                          uint32_t parity0, uint32_t bar1, uint32_t parity1, uint32_t &over0, uint32_t &over1) {
+    if constexpr (FP8) FEW_BLOCK("f8f6f4");
+    else FEW_BLOCK("f16");
 }
+#undef FEW_BLOCK
 template <bool FP8>
 __device__ __forceinline__ uint32_t few_idesc(int n) {
     return FP8 ? (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24) : tc_idesc(n);
 }
-__device__ __forceinline__ void few_tma(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, uint32_t bar) { tl::g_tma_load_3d(dst, map, c0, c1, c2, bar); }
 template <int COLS>
-__device__ __forceinline__ void few_ld(uint32_t at, uint32_t (&v)[COLS]) {  // columns of tensor memory, with the wait
+__device__ __forceinline__ void few_ld(uint32_t at, uint32_t *v) {  // columns of tensor memory, behind them tcgen05.wait::ld
 #pragma unroll
-    for (int c = 0; c < COLS; c += 8) {
-        uint32_t w[8];
-        tc_ld8(at + c, w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[c + i] = w[i];
-    }
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    for (int c = 0; c < COLS; c += 4)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[c]), "=r"(v[c + 1]), "=r"(v[c + 2]), "=r"(v[c + 3]) : "r"(at + c) : "memory");
 }
+__device__ __forceinline__ void few_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // The chosen experts in ascending order and the tokens that chose each, in ascending order: a token's place is its column.  Both launches make these for
 // themselves.
@@ -166,15 +179,15 @@ __device__ __forceinline__ bool few_lists(const FewArgs &a, const int *idx, cons
 
 // Barriers of either launch: the ring's, the accumulators', the second launch's columns'.
 struct FewBars {
-    uint32_t full, empty, acc_full, acc_empty, cols_full, cols_empty;
+    uint32_t full, empty, acc_full, acc_empty, cols_full, cols_empty, part_full, part_empty;
     volatile int *dead;
-    uint32_t *tmem, *last;
-    static constexpr int kBytes = 16 * kFewMostStages + 64 + 32 + 16;
+    uint32_t *tmem;
+    static constexpr int kBytes = 16 * kFewMostStages + 64 + 64 + 16;
     __device__ FewBars(unsigned char *smem, int at) {
         full = g_smem_u32(smem + at), empty = full + 8 * kFewMostStages, acc_full = empty + 8 * kFewMostStages, acc_empty = acc_full + 32, cols_full = acc_empty + 32;
-        cols_empty = cols_full + 16;
-        dead = reinterpret_cast<volatile int *>(smem + at + 16 * kFewMostStages + 96);
-        tmem = reinterpret_cast<uint32_t *>(smem + at + 16 * kFewMostStages + 100), last = tmem + 1;
+        cols_empty = cols_full + 16, part_full = cols_empty + 16, part_empty = part_full + 16;
+        dead = reinterpret_cast<volatile int *>(smem + at + 16 * kFewMostStages + 128);
+        tmem = reinterpret_cast<uint32_t *>(smem + at + 16 * kFewMostStages + 132);
     }
 };
 constexpr int kFewBuffers = 4;  // accumulators, of bf16 experts 2 are used
@@ -182,8 +195,9 @@ constexpr int kFewBuffers = 4;  // accumulators, of bf16 experts 2 are used
 // ---- first launch ----------------------------------------------------------------------------------------------------
 
 constexpr int kFewCluster = 4;
-// Columns of the products, for eight tokens each.  e4m3: the first half is of the first half of the tokens, their first terms and then their second; so the second.
+// Columns of the products, for eight tokens each; e4m3: the first terms of all tokens, then the second.
 __host__ __device__ constexpr int few_columns(int nt, bool fp8) { return fp8 ? 16 * nt : nt <= 2 ? 16 : 32; }
+__host__ __device__ constexpr int few_router_sums(int nt) { return 16 * (nt * 8 + 2); }  // of a warp: 16 rows
 constexpr int few_tmem(int columns) { return columns <= 32 ? 32 : columns <= 64 ? 64 : columns <= 128 ? 128 : 256; }
 
 struct FewFirstSmem {
@@ -192,9 +206,9 @@ struct FewFirstSmem {
     __host__ __device__ FewFirstSmem(int tokens, int nt, int dim, int outputs, int experts, int top, int groups, bool fp8, int room) : lists(0, tokens, top, experts) {
         const int n = few_columns(nt, fp8);
         cols = 0;
-        cols_block = fp8 && tokens > 4 ? n * 128 : (tokens + 7) / 8 * 1024;  // of 128 bytes of the reduction; what the columns past the last token hold does not matter
-        sums = (fp8 ? (dim + 127) / 128 : (dim + 63) / 64) * cols_block + n * 128;
-        most = sums + (fp8 ? n / 2 : n) * 512;
+        cols_block = nt * (fp8 ? 2048 : 1024);  // of 128 bytes of the reduction; bf16: what the columns past the last token hold does not matter
+        sums = (fp8 ? (dim + 127) / 128 * cols_block : (dim + 63) / 64 * cols_block + n * 128);
+        most = sums + (fp8 ? n / 2 : n) * 256;
         idx = most + kFewTokens * 4;
         gate = idx + tokens * top * 4;
         lists = FewListsSmem(gate + tokens * top * 4, tokens, top, experts);
@@ -202,7 +216,7 @@ struct FewFirstSmem {
         ring = (bars + FewBars::kBytes + 1023) / 1024 * 1024;
         // the router's sums and logits are done with when the ring's first copies are asked for
         router = ring;
-        logits = router + kFewWarps * 16 * nt * 8 * 4;
+        logits = router + kFewWarps * few_router_sums(nt) * 4;
         const int early = logits + (tokens * (2 * outputs + groups) + tokens) * 4;
         stages = (room - ring) / kFewStage;
         if (stages > kFewMostStages) stages = kFewMostStages;
@@ -213,7 +227,7 @@ struct FewFirstSmem {
 
 template <bool FP8, bool GATED, int NT>
 __global__ void __launch_bounds__(kFewThreads, 1)
-moe_few_first_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUtensorMap map1, const FewArgs a) {
+moe_few_first_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUtensorMap map1, const FewArgs a) {
     extern __shared__ __align__(1024) unsigned char few_smem[];
     constexpr int BUFFERS = FP8 ? kFewBuffers : 2, ENTRIES = FP8 ? 128 : 64;  // of the reduction, in a stage
     constexpr int N = few_columns(NT, FP8), COLS = N / 2, SUMS = FP8 ? COLS / 2 : COLS /* of a thread */, TMEM = few_tmem(N * BUFFERS);
@@ -232,12 +246,13 @@ moe_few_first_kernel(const __grid_constant__ CUtensorMap map0, const __grid_cons
     const FewLists lists = at.lists.lists(few_smem);
     const FewBars bars(few_smem, at.bars);
     at.lists.clear(few_smem);
-    if (tid < kFewTokens) most[tid] = 0;
     if (warp == 1 && lane == 0) {
         for (int i = 0; i < at.stages; ++i) g_mbar_init(bars.full + 8 * i, GATED ? 2 : 1), g_mbar_init(bars.empty + 8 * i, 1);
         for (int i = 0; i < BUFFERS; ++i) g_mbar_init(bars.acc_full + 8 * i, 1), g_mbar_init(bars.acc_empty + 8 * i, 8);
+        g_mbar_init(bars.cols_full, 1);
         *bars.dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map0) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map1) : "memory");
     }
@@ -252,10 +267,18 @@ moe_few_first_kernel(const __grid_constant__ CUtensorMap map0, const __grid_cons
 
     tl::griddep_wait();
     tl::griddep_launch();  // the second launch reads nothing ahead of its own wait
+    // ---- the tokens, 64 entries of all of them a copy: bf16 columns as they are
+    const int rows = a.outputs + (a.side_w ? 1 : 0), pieces = (a.dim + 63) / 64;
+    // 16 of the router's rows are shared by all warps, or by eight where there are more than the cluster has at once
+    const int parts = rows > 16 * static_cast<int>(ranks) ? 8 : 16, part = warp & (parts - 1), group = parts == 8 ? warp >> 3 : 0, groups = kFewWarps / parts;
+    if (warp == 1 && g_elect_one()) {
+        g_mbar_expect_tx(bars.cols_full, pieces * NT * 1024);
+        for (int i = 0; i < pieces; ++i) tl::g_tma_load_2d(g_smem_u32(few_smem + at.cols) + i * NT * 1024, &map_x, i * 128, 0, bars.cols_full);
+    }
+    __syncwarp();
     if (blockIdx.x == 0)
-        for (int i = tid; i < (a.dim + 127) / 128; i += kFewThreads) a.finished[i] = 0;
-    // ---- the router's rows, 16 for eight warps each, which share the reduction; a CTA of the cluster every ranks-th 32 of them
-    const int rows = a.outputs + (a.side_w ? 1 : 0), pieces = (a.dim * 2 + 127) / 128, part = warp & 7;
+        for (int i = tid; i < (a.dim + 127) / 128 * kFewTokens; i += kFewThreads) a.finished[i] = 0;
+    // ---- the router's rows, 16 for eight or all warps, which share the reduction
     constexpr int AT_ONCE = 4;
     uint4 wa[AT_ONCE][2], wb[AT_ONCE][2];
     auto row_of = [&](int r) { return reinterpret_cast<const uint8_t *>(r < a.outputs ? a.router + (size_t)r * a.dim : r < rows ? a.side_w : nullptr); };
@@ -265,77 +288,66 @@ moe_few_first_kernel(const __grid_constant__ CUtensorMap map0, const __grid_cons
         for (int u = 0; u < AT_ONCE; ++u)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const int o = (s0 + u * 8) * 128 + c * 64 + t4 * 16;
+                const int o = (s0 + u * parts) * 128 + c * 64 + t4 * 16;
                 wa[u][c] = ra && o < a.dim * 2 ? few_ldg(ra + o) : make_uint4(0, 0, 0, 0);
                 wb[u][c] = rb && o < a.dim * 2 ? few_ldg(rb + o) : make_uint4(0, 0, 0, 0);
             }
     };
-    const int m_first = rank * 2 + (warp >> 3);
+    const int m_first = rank * groups + group;
     ask(m_first, part);
-    if constexpr (FP8) {  // the tokens' largest magnitudes, 256 entries a warp
-        const int segs = (a.dim + 255) / 256;
-        constexpr int X_AT_ONCE = 4;
-        for (int i0 = warp; i0 < a.tokens * segs; i0 += X_AT_ONCE * kFewWarps) {
-            uint4 v[X_AT_ONCE];
-#pragma unroll
-            for (int u = 0; u < X_AT_ONCE; ++u) {
-                const int i = i0 + u * kFewWarps, t = i / segs, d = (i - t * segs) * 256 + lane * 8;
-                v[u] = make_uint4(0, 0, 0, 0);
-                if (t < a.tokens && d < a.dim) v[u] = tl::ld_cg(reinterpret_cast<const uint4 *>(a.x + (size_t)t * a.dim + d));
+    tc_wait(bars.cols_full, 0, bars.dead);
+    const unsigned char *raw = few_smem + at.cols;
+    auto entries = [&](int b, int t) {  // four of a token, of 128 that a warp has
+        return *reinterpret_cast<const uint2 *>(raw + (b * 2 + (lane >> 4)) * NT * 1024 + few_swizzled(t, (lane & 15) * 8));
+    };
+    if constexpr (FP8)  // the tokens' largest magnitudes
+        for (int t = warp; t < 8 * NT; t += kFewWarps) {  // zeros behind the last
+            uint32_t top = 0;
+            for (int i = lane >> 3; i < pieces; i += 4) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(raw + i * NT * 1024 + t * 128 + (lane & 7) * 16);
+                top = __vmaxu2(top, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
             }
-#pragma unroll
-            for (int u = 0; u < X_AT_ONCE; ++u) {
-                const int t = (i0 + u * kFewWarps) / segs;
-                if (t >= a.tokens) break;
-                const uint32_t c[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-                uint32_t top = 0;  // of the 15 bits of a magnitude
-#pragma unroll
-                for (int j = 0; j < 4; ++j) top = max(top, max(c[j] & 0x7fffu, c[j] >> 16 & 0x7fffu));
-                top = __reduce_max_sync(0xffffffffu, top);
-                if (lane == 0) atomicMax(&most[t], top);
-            }
+            top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+            if (lane == 0) most[t] = top;
         }
-    }
     bool waited = false;
-    for (int m = m_first; (m - (warp >> 3)) * 16 < rows; m += ranks * 2) {
+    for (int m = m_first; (m - group) * 16 < rows; m += ranks * groups) {
         float acc[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-        for (int s = part; s < pieces; s += AT_ONCE * 8) {
+        for (int s = part; s < pieces; s += AT_ONCE * parts) {
             if (m != m_first || s != part) ask(m, s);
 #pragma unroll
             for (int u = 0; u < AT_ONCE; ++u) {
+                if (s + u * parts >= pieces) break;
                 uint4 x[2][NT];
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {  // columns past the last token: the last one, not used
-                        const int o = (s + u * 8) * 64 + c * 32 + t4 * 8;
-                        x[c][n] = make_uint4(0, 0, 0, 0);
-                        if (o < a.dim) x[c][n] = tl::ld_cg(reinterpret_cast<const uint4 *>(a.x + (size_t)min(n * 8 + g, a.tokens - 1) * a.dim + o));
-                    }
+                    for (int n = 0; n < NT; ++n) x[c][n] = *reinterpret_cast<const uint4 *>(raw + (s + u * parts) * NT * 1024 + few_swizzled(n * 8 + g, c * 64 + t4 * 16));
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
                     for (int n = 0; n < NT; ++n) few_mma(acc[n], wa[u][c], wb[u][c], x[c][n]);
             }
         }
-        float *mine = router_red + warp * 16 * NT * 8;
+        constexpr int RED = few_router_sums(NT) / 16;
+        float *mine = router_red + warp * 16 * RED;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            *reinterpret_cast<float2 *>(mine + g * NT * 8 + n * 8 + 2 * t4) = make_float2(acc[n][0], acc[n][1]);
-            *reinterpret_cast<float2 *>(mine + (g + 8) * NT * 8 + n * 8 + 2 * t4) = make_float2(acc[n][2], acc[n][3]);
+            *reinterpret_cast<float2 *>(mine + g * RED + n * 8 + 2 * t4) = make_float2(acc[n][0], acc[n][1]);
+            *reinterpret_cast<float2 *>(mine + (g + 8) * RED + n * 8 + 2 * t4) = make_float2(acc[n][2], acc[n][3]);
         }
         __syncthreads();
         if (!waited) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all CTAs of the cluster run
         waited = true;
-        const int m0 = m - (warp >> 3);
-        for (int i = tid; i < 2 * 16 * NT * 8; i += kFewThreads) {
+        const int m0 = m - group;
+        for (int i = tid; i < groups * 16 * NT * 8; i += kFewThreads) {
             const int in = i % (16 * NT * 8), r = (m0 + i / (16 * NT * 8)) * 16 + in / (NT * 8), t = in % (NT * 8);
             if (r >= rows || t >= a.tokens) continue;
             float z = 0.f;
-#pragma unroll
-            for (int w = 0; w < 8; ++w) z += router_red[(i / (16 * NT * 8) * 8 + w) * 16 * NT * 8 + in];
+#pragma unroll 8
+            for (int w = 0; w < parts; ++w) z += router_red[((i / (16 * NT * 8) * parts + w) * 16 + in / (NT * 8)) * RED + t];
             if (r < a.outputs && a.router_bias) z += to_f(a.router_bias[r]);
             const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(r < a.outputs ? logits + t * per_token + r : side + t));
             for (uint32_t c = 0; c < ranks; ++c)
@@ -345,33 +357,33 @@ moe_few_first_kernel(const __grid_constant__ CUtensorMap map0, const __grid_cons
     }
     if (!waited) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    __syncthreads();  // the largest magnitudes
-    // ---- the columns: what of all tokens stands beside an expert's rows
-    {
-        constexpr int C_AT_ONCE = 4;
-        const int blocks = (a.dim + 127) / 128;  // of 128 entries
-        for (int i0 = warp; i0 < a.tokens * blocks; i0 += C_AT_ONCE * kFewWarps) {
-            uint2 v[C_AT_ONCE];
+    // ---- the columns of e4m3 experts, in the place of the tokens: a warp takes 128 entries of all of them
+    if constexpr (FP8) {
+        __syncthreads();  // the largest magnitudes; the router has read the tokens
+        for (int b = warp; b * 2 < pieces; b += kFewWarps) {
+            const bool there = b * 2 + (lane >> 4) < pieces;
+            unsigned char *to = few_smem + at.cols + b * at.cols_block;
+            for (int t0 = 0; t0 < a.tokens; t0 += 4) {  // a token's two terms stand where its 128 entries stood
+                uint2 v[4];
 #pragma unroll
-            for (int u = 0; u < C_AT_ONCE; ++u) {
-                const int i = i0 + u * kFewWarps, t = i / blocks, d = (i - t * blocks) * 128 + lane * 4;
-                v[u] = make_uint2(0, 0);
-                if (t < a.tokens && d < a.dim) asm volatile("ld.global.cg.v2.u32 {%0,%1}, [%2];" : "=r"(v[u].x), "=r"(v[u].y) : "l"(a.x + (size_t)t * a.dim + d) : "memory");
-            }
+                for (int u = 0; u < 4; ++u) {
+                    v[u] = make_uint2(0, 0);
+                    if (there) v[u] = entries(b, t0 + u);
+                }
+                __syncwarp();
 #pragma unroll
-            for (int u = 0; u < C_AT_ONCE; ++u) {
-                const int i = i0 + u * kFewWarps, t = i / blocks, b = i - t * blocks;
-                if (t >= a.tokens) break;
-                if constexpr (FP8) {
-                    const float up = few_exp2(8 - few_exponent(__uint_as_float(most[t] << 16)));
+                for (int u = 0; u < 4; ++u) {
+                    // at most 256 in magnitude; a half holds eight bits of what counts
+                    const float up = few_exp2(8 - few_exponent(__uint_as_float(most[t0 + u] << 16)));
                     const float2 lo = tl::unpack2<bf16>(v[u].x), hi = tl::unpack2<bf16>(v[u].y);
-                    float w[4] = {lo.x * up, lo.y * up, hi.x * up, hi.y * up};
-                    unsigned char *to = few_smem + at.cols + b * at.cols_block;
-                    const int column = t + t / SUMS * SUMS;
-                    *reinterpret_cast<uint32_t *>(to + few_swizzled(column, lane * 4)) = few_term(w);
-                    *reinterpret_cast<uint32_t *>(to + few_swizzled(column + SUMS, lane * 4)) = few_term(w);
-                } else if (b * 2 + (lane >> 4) < (a.dim + 63) / 64) {
-                    *reinterpret_cast<uint2 *>(few_smem + at.cols + (b * 2 + (lane >> 4)) * at.cols_block + few_swizzled(t, (lane & 15) * 8)) = v[u];
+                    const __half2 h0 = __floats2half2_rn(lo.x * up, lo.y * up), h1 = __floats2half2_rn(hi.x * up, hi.y * up);
+                    const uint32_t q0 = __nv_cvt_halfraw2_to_fp8x2(h0, __NV_SATFINITE, __NV_E4M3), q1 = __nv_cvt_halfraw2_to_fp8x2(h1, __NV_SATFINITE, __NV_E4M3);
+                    const __half2 sixteen = __float2half2_rn(16.f);
+                    const __half2 r0 = __hmul2(__hsub2(h0, __half2(__nv_cvt_fp8x2_to_halfraw2(q0, __NV_E4M3))), sixteen);
+                    const __half2 r1 = __hmul2(__hsub2(h1, __half2(__nv_cvt_fp8x2_to_halfraw2(q1, __NV_E4M3))), sixteen);
+                    *reinterpret_cast<uint32_t *>(to + few_swizzled(t0 + u, lane * 4)) = q0 | q1 << 16;
+                    *reinterpret_cast<uint32_t *>(to + few_swizzled(8 * NT + t0 + u, lane * 4)) =
+                        __nv_cvt_halfraw2_to_fp8x2(r0, __NV_SATFINITE, __NV_E4M3) | static_cast<uint32_t>(__nv_cvt_halfraw2_to_fp8x2(r1, __NV_SATFINITE, __NV_E4M3)) << 16;
                 }
             }
         }
@@ -407,7 +419,7 @@ moe_few_first_kernel(const __grid_constant__ CUtensorMap map0, const __grid_cons
                 for (int b = 0; b < blocks; ++b) {
                     if (!(ok = tc_wait_one(bars.empty + 8 * s, ph, bars.dead))) break;
                     g_mbar_expect_tx(bars.full + 8 * s, GATED ? kFewStage / 2 : kFewStage);
-                    few_tma(g_smem_u32(few_smem + at.ring) + s * kFewStage + (warp == 3 ? kFewStage / 2 : 0), warp == 3 ? &map1 : &map0, b * 128, f0, e,
+                    tl::g_tma_load_3d(g_smem_u32(few_smem + at.ring) + s * kFewStage + (warp == 3 ? kFewStage / 2 : 0), warp == 3 ? &map1 : &map0, b * 128, f0, e,
                             bars.full + 8 * s);
                     if (++s == at.stages) s = 0, ph ^= 1u;
                 }
@@ -427,24 +439,24 @@ moe_few_first_kernel(const __grid_constant__ CUtensorMap map0, const __grid_cons
             uint32_t ph = 0, acc_ph = 1;
             bool ok = true;
             const uint32_t ring = g_smem_u32(few_smem + at.ring), cols = g_smem_u32(few_smem + at.cols);
+            uint32_t acc_free = 0, there = 0;  // asked ahead
             for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x)
                 for (int b = 0; b < blocks; ++b) {
-                    if (FP8 || b == 0) ok = tc_wait_one(bars.acc_empty + 8 * buf, acc_ph, bars.dead);
-                    if (!ok || !(ok = tc_wait_one(bars.full + 8 * s, ph, bars.dead))) break;
+                    if ((FP8 || b == 0) && !acc_free) ok = tc_wait_one(bars.acc_empty + 8 * buf, acc_ph, bars.dead);
+                    if (ok && !there) ok = tc_wait_one(bars.full + 8 * s, ph, bars.dead);
+                    if (!ok) break;
                     g_tc_fence_after();
                     const uint64_t w = g_smem_desc_sw128(ring + s * kFewStage, 0, 1024), x = g_smem_desc_sw128(cols + b * at.cols_block, 0, 1024);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) few_product<FP8>(tmem + buf * N, w + 2 * k, x + 2 * k, few_idesc<FP8>(N), FP8 ? k > 0 : b > 0 || k > 0);
+                    const uint32_t d = tmem + buf * N, done = bars.acc_full + 8 * buf, used = bars.empty + 8 * s;
                     const bool last = FP8 || b == blocks - 1;
-                    if (last) g_tc_commit(bars.acc_full + 8 * buf);
-                    g_tc_commit(bars.empty + 8 * s);
                     if (++s == at.stages) s = 0, ph ^= 1u;
                     if (last && ++buf == BUFFERS) buf = 0, acc_ph ^= 1u;
+                    few_block<FP8>(d, w, x, few_idesc<FP8>(N), !FP8 && b > 0, last, done, used, bars.acc_empty + 8 * buf, acc_ph, bars.full + 8 * s, ph, acc_free, there);
                 }
         }
     } else if (warp >= 8) {
-        const int quarter = warp & 3, half = (warp - 8) >> 2, row = quarter * 32 + lane, me = tid - 256;
-        float *sums = reinterpret_cast<float *>(few_smem + at.sums);  // [token][128]
+        const int quarter = warp & 3, half = (warp - 8) >> 2, me = tid - 256;
+        float *sums = reinterpret_cast<float *>(few_smem + at.sums);  // [token][64]
         int buf = 0;
         uint32_t acc_ph = 0;
         for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
@@ -453,7 +465,7 @@ moe_few_first_kernel(const __grid_constant__ CUtensorMap map0, const __grid_cons
 #pragma unroll
             for (int c = 0; c < SUMS; ++c) acc[c] = 0.f;
             bool ok = true;
-            const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * COLS;
+            const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * SUMS;
             if constexpr (FP8) {
                 // the rows' block of scales: a gate's (or, without gates, all), the up projection's
                 const float *scales = (GATED && quarter >= 2 ? a.s1 : a.s0) + ((size_t)e * scale_rows + (f0 >> 7)) * scale_cols;
@@ -464,7 +476,8 @@ moe_few_first_kernel(const __grid_constant__ CUtensorMap map0, const __grid_cons
                     ok &= tc_wait(bars.acc_full + 8 * buf, acc_ph, bars.dead);
                     g_tc_fence_after();
                     uint32_t v[COLS];
-                    few_ld(from + buf * N, v);
+                    few_ld<SUMS>(from + buf * N, v), few_ld<SUMS>(from + buf * N + N / 2, v + SUMS);
+                    few_ld_wait();
                     g_tc_fence_before();
                     __syncwarp();
                     if (lane == 0) g_mbar_arrive(bars.acc_empty + 8 * buf);
@@ -476,7 +489,8 @@ moe_few_first_kernel(const __grid_constant__ CUtensorMap map0, const __grid_cons
                 ok &= tc_wait(bars.acc_full + 8 * buf, acc_ph, bars.dead);
                 g_tc_fence_after();
                 uint32_t v[COLS];
-                few_ld(from + buf * N, v);
+                few_ld<COLS>(from + buf * N, v);
+                few_ld_wait();
                 g_tc_fence_before();
                 __syncwarp();
                 if (lane == 0) g_mbar_arrive(bars.acc_empty + 8 * buf);
@@ -484,31 +498,38 @@ moe_few_first_kernel(const __grid_constant__ CUtensorMap map0, const __grid_cons
                 for (int c = 0; c < SUMS; ++c) acc[c] = __uint_as_float(v[c]);
                 if (++buf == BUFFERS) buf = 0, acc_ph ^= 1u;
             }
-#pragma unroll
-            for (int c = 0; c < SUMS; ++c) sums[(half * SUMS + c) * 128 + row] = acc[c];
             const float bad = tc_verdict(ok, bars.dead);
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            // two passes of half of the features each: what they hand over takes half of the memory
             const int columns = __popc(lists.tokens[pos]), here = min(FEATURES, a.ff - f0);
-            for (int i = me; i < columns * FEATURES; i += 256) {
-                const int f = i % FEATURES, c = lists.column[pos * 32 + i / FEATURES], t = c >> 8;
-                if (f >= here) continue;
-                auto of = [&](int r) {
-                    if constexpr (!FP8) return sums[t * 128 + r];
-                    // a token with an infinity or a NaN has none of its numbers
-                    const uint32_t m = most[t] << 16;
-                    const float scale = m < 0x7f800000u ? few_exp2(few_exponent(__uint_as_float(m)) - 8) : __int_as_float(0x7fffffff);
-                    return sums[t * 128 + r] * scale;
-                };
-                const float v = of(f) * bad;
-                float y;
-                if constexpr (GATED) y = gated_pair(v, of(f + 64), a.act, a.limit, a.slope);
-                else y = a.act == 2 ? (v > 0.f ? v * v : v == v ? 0.f : v) : act_apply(v, a.act);
-                float *to = a.inner + ((size_t)t * a.top + (c & 255)) * a.ld_inner + f0;
-                to[f] = y;
-                if (f0 + here == a.ff)
-                    for (int z = a.ff + f; z < a.ld_inner; z += here) to[z - f0] = 0.f;
+            for (int pass = 0; pass < 2; ++pass) {
+                const bool mine = GATED ? (quarter & 1) == pass : (quarter >> 1) == pass;
+                if (mine) {
+                    const int at_row = GATED ? (quarter >> 1) * 32 + lane : (quarter & 1) * 32 + lane;
+#pragma unroll
+                    for (int c = 0; c < SUMS; ++c) sums[(half * SUMS + c) * 64 + at_row] = acc[c];
+                }
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                for (int i = me; i < columns * (FEATURES / 2); i += 256) {
+                    const int in = i % (FEATURES / 2), f = pass * (FEATURES / 2) + in, c = lists.column[pos * 32 + i / (FEATURES / 2)], t = c >> 8;
+                    if (f >= here) continue;
+                    auto of = [&](int r) {
+                        if constexpr (!FP8) return sums[t * 64 + r];
+                        // a token with an infinity or a NaN has none of its numbers
+                        const uint32_t m = most[t] << 16;
+                        const float scale = m < 0x7f800000u ? few_exp2(few_exponent(__uint_as_float(m)) - 8) : __int_as_float(0x7fffffff);
+                        return sums[t * 64 + r] * scale;
+                    };
+                    const float v = of(in) * bad;
+                    float y;
+                    if constexpr (GATED) y = gated_pair(v, of(in + 32), a.act, a.limit, a.slope);
+                    else y = a.act == 2 ? (v > 0.f ? v * v : v == v ? 0.f : v) : act_apply(v, a.act);
+                    float *to = a.inner + ((size_t)t * a.top + (c & 255)) * a.ld_inner + f0;
+                    to[f] = y;
+                    if (f0 + here == a.ff && f >= here - 16)  // zeros behind the last features
+                        for (int z = a.ff + here - 1 - f; z < a.ld_inner; z += min(here, 16)) to[z - f0] = 0.f;
+                }
+                asm volatile("bar.sync 1, 256;" ::: "memory");  // read before the next are written
             }
-            asm volatile("bar.sync 1, 256;" ::: "memory");  // read before the next tile's are written
         }
     }
     __syncwarp();
@@ -526,8 +547,8 @@ moe_few_first_kernel(const __grid_constant__ CUtensorMap map0, const __grid_cons
 constexpr int kFewSecondN = 32;  // the most columns of an item: terms times tokens
 
 struct FewSecondSmem {
-    int cols, factors, sums, idx, gate, group, bars, ring, stages, total;
-    static constexpr int kCols = kFewItemBlocks * 4096 + 4096, kFactors = kFewItemBlocks * kFewSecondN * 4;  // of either place of an item's columns
+    int cols, factors, sums, idx, gate, need, group, bars, ring, stages, total;
+    static constexpr int kCols = kFewItemCols + 4096, kFactors = kFewItemBlocks * kFewSecondN * 4;  // of either place of an item's columns
     FewListsSmem lists;
     __host__ __device__ FewSecondSmem(int tokens, int experts, int top, int room) : lists(0, tokens, top, experts) {
         cols = 0;
@@ -535,7 +556,8 @@ struct FewSecondSmem {
         sums = factors + 2 * kFactors;
         idx = sums + kFewSecondN * 128 * 4;
         gate = idx + tokens * top * 4;
-        group = gate + tokens * top * 4;
+        need = gate + tokens * top * 4;
+        group = need + kFewTokens * 4;
         lists = FewListsSmem((group + tokens * top * 4 + 4 + 3) / 4 * 4, tokens, top, experts);
         bars = lists.end;
         ring = (bars + FewBars::kBytes + 1023) / 1024 * 1024;
@@ -545,14 +567,45 @@ struct FewSecondSmem {
     }
 };
 
-// An identity expert's part of an output; a choice that is no output at all: the token's logits are no numbers.
-__device__ __forceinline__ float few_identity(const FewArgs &a, int e, float weight, int t, int d, float y) {
-    return e < a.outputs ? fmaf(weight, to_f(tl::ld_cg(a.x + (size_t)t * a.dim + d)), y) : __int_as_float(0x7fffffff);
-}
+// Four columns of a token's output (a row has a multiple of eight).  A few choices' numbers are asked for together: one at a time, each waits for memory while
+// the weights stream.
 template <typename OUT>
-__device__ __forceinline__ void few_store(const FewArgs &a, int t, int d, float y) {
-    if (a.shared) y = fmaf(a.side_w ? tl::ld_cg(a.side + t) : 1.f, to_f(tl::ld_cg(a.shared + (size_t)t * a.dim + d)), y);
-    static_cast<OUT *>(a.out)[(size_t)t * a.dim + d] = from_f<OUT>(y);
+__device__ __forceinline__ void few_output(const FewArgs &a, int t, int d, int pairs, const int *idx, const float *gate) {
+    if (d >= a.dim) return;
+    float y[4] = {0.f, 0.f, 0.f, 0.f};
+    constexpr int AT_ONCE = 4;
+    for (int k0 = t * a.top; k0 < (t + 1) * a.top; k0 += AT_ONCE) {
+        float4 z[AT_ONCE];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) z[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s = 0; s < a.splits; ++s) {
+            uint4 w[AT_ONCE];
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                w[u] = make_uint4(0, 0, 0, 0);
+                if (k0 + u < (t + 1) * a.top && static_cast<uint32_t>(idx[k0 + u]) < static_cast<uint32_t>(a.experts))
+                    w[u] = tl::ld_cg(reinterpret_cast<const uint4 *>(a.part + ((size_t)s * pairs + k0 + u) * a.dim + d));
+            }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) z[u].x += __uint_as_float(w[u].x), z[u].y += __uint_as_float(w[u].y), z[u].z += __uint_as_float(w[u].z), z[u].w += __uint_as_float(w[u].w);
+        }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const float g = k0 + u < (t + 1) * a.top && static_cast<uint32_t>(idx[k0 + u]) < static_cast<uint32_t>(a.experts) ? gate[k0 + u] : 0.f;
+            y[0] = fmaf(g, z[u].x, y[0]), y[1] = fmaf(g, z[u].y, y[1]), y[2] = fmaf(g, z[u].z, y[2]), y[3] = fmaf(g, z[u].w, y[3]);
+        }
+    }
+    if (a.experts < a.outputs || a.shared)
+        for (int c = 0; c < 4; ++c) {
+            const float x = to_f(tl::ld_cg(a.x + (size_t)t * a.dim + d + c));
+            for (int k = t * a.top; k < (t + 1) * a.top; ++k)  // identity experts
+                if (idx[k] >= a.experts && idx[k] < a.outputs) y[c] = fmaf(gate[k], x, y[c]);
+            if (a.shared) y[c] = fmaf(a.side_w ? tl::ld_cg(a.side + t) : 1.f, to_f(tl::ld_cg(a.shared + (size_t)t * a.dim + d + c)), y[c]);
+        }
+    for (int k = t * a.top; k < (t + 1) * a.top; ++k)  // a choice that is no output at all: the token's logits are no numbers
+        if (idx[k] >= a.outputs) y[0] = y[1] = y[2] = y[3] = __int_as_float(0x7fffffff);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) static_cast<OUT *>(a.out)[(size_t)t * a.dim + d + c] = from_f<OUT>(y[c]);
 }
 
 template <bool FP8, typename OUT>
@@ -563,6 +616,7 @@ moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) 
     const FewSecondSmem at(a.tokens, a.experts, a.top, a.room);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, pairs = a.tokens * a.top;
     float *sums = reinterpret_cast<float *>(few_smem + at.sums), *gate = reinterpret_cast<float *>(few_smem + at.gate), *factors = reinterpret_cast<float *>(few_smem + at.factors);
+    int *need = reinterpret_cast<int *>(few_smem + at.need);  // [tokens]: the partial sums of an output
     int *idx = reinterpret_cast<int *>(few_smem + at.idx), *group = reinterpret_cast<int *>(few_smem + at.group);  // group: [groups] position * 4 + number
     const FewLists lists = at.lists.lists(few_smem);
     const FewBars bars(few_smem, at.bars);
@@ -571,6 +625,7 @@ moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) 
         for (int i = 0; i < at.stages; ++i) g_mbar_init(bars.full + 8 * i, 1), g_mbar_init(bars.empty + 8 * i, 1);
         for (int i = 0; i < BUFFERS; ++i) g_mbar_init(bars.acc_full + 8 * i, 1), g_mbar_init(bars.acc_empty + 8 * i, 8);
         for (int i = 0; i < 2; ++i) g_mbar_init(bars.cols_full + 8 * i, 4), g_mbar_init(bars.cols_empty + 8 * i, 1 + 8);  // by the warps that write; by the products, and the sums
+        for (int i = 0; i < 2; ++i) g_mbar_init(bars.part_full + 8 * i, 1), g_mbar_init(bars.part_empty + 8 * i, 2);
         *bars.dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
@@ -582,12 +637,14 @@ moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) 
     tl::griddep_wait();
     tl::griddep_launch();
     if (tid < pairs) idx[tid] = tl::ld_cg(a.idx + tid), gate[tid] = tl::ld_cg(a.gate + tid);
+    if (tid < kFewTokens) need[tid] = 0;
     g_tc_fence_before();
     __syncthreads();
     g_tc_fence_after();
     const uint32_t tmem = *bars.tmem;
     const bool live = few_lists(a, idx, lists);
-    if (tid < pairs && !live && idx[tid] < a.experts) idx[tid] = -1;  // named twice
+    if (live) atomicAdd(&need[tid / a.top], a.splits);
+    else if (tid < pairs && idx[tid] < a.experts) idx[tid] = -1;  // named twice
     const int count = *lists.count;
     if (warp == 0) {  // the experts' groups of up to GROUP tokens, in order
         int n = 0;
@@ -628,7 +685,7 @@ moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) 
                 for (int b = it.b0; b < it.b1; ++b) {
                     if (!(ok = tc_wait_one(bars.empty + 8 * s, ph, bars.dead))) break;
                     g_mbar_expect_tx(bars.full + 8 * s, kFewStage);
-                    few_tma(g_smem_u32(few_smem + at.ring) + s * kFewStage, &map, b * 128, it.m * 128, lists.active[it.pos], bars.full + 8 * s);
+                    tl::g_tma_load_3d(g_smem_u32(few_smem + at.ring) + s * kFewStage, &map, b * 128, it.m * 128, lists.active[it.pos], bars.full + 8 * s);
                     if (++s == at.stages) s = 0, ph ^= 1u;
                 }
             }
@@ -638,6 +695,7 @@ moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) 
             int s = 0, buf = 0, place = 0;
             uint32_t ph = 0, acc_ph = 1, cols_ph = 0;
             bool ok = true;
+            uint32_t acc_free = 0, there = 0;  // asked ahead
             const uint32_t ring = g_smem_u32(few_smem + at.ring);
             for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
                 const Item it = item_of(i);
@@ -645,18 +703,16 @@ moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) 
                 const uint32_t cols = g_smem_u32(few_smem + at.cols) + place * FewSecondSmem::kCols;
                 if (!(ok = tc_wait_one(bars.cols_full + 8 * place, cols_ph, bars.dead))) break;
                 for (int b = it.b0; b < it.b1; ++b) {
-                    if (FP8 || b == it.b0) ok = tc_wait_one(bars.acc_empty + 8 * buf, acc_ph, bars.dead);
-                    if (!ok || !(ok = tc_wait_one(bars.full + 8 * s, ph, bars.dead))) break;
+                    if ((FP8 || b == it.b0) && !acc_free) ok = tc_wait_one(bars.acc_empty + 8 * buf, acc_ph, bars.dead);
+                    if (ok && !there) ok = tc_wait_one(bars.full + 8 * s, ph, bars.dead);
+                    if (!ok) break;
                     g_tc_fence_after();
                     const uint64_t w = g_smem_desc_sw128(ring + s * kFewStage, 0, 1024), h = g_smem_desc_sw128(cols + (b - it.b0) * cols_block, 0, 1024);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        few_product<FP8>(tmem + buf * kFewSecondN, w + 2 * k, h + 2 * k, few_idesc<FP8>(it.n), FP8 ? k > 0 : b > it.b0 || k > 0);
+                    const uint32_t d = tmem + buf * kFewSecondN, done = bars.acc_full + 8 * buf, used = bars.empty + 8 * s;
                     const bool last = FP8 || b == it.b1 - 1;
-                    if (last) g_tc_commit(bars.acc_full + 8 * buf);
-                    g_tc_commit(bars.empty + 8 * s);
                     if (++s == at.stages) s = 0, ph ^= 1u;
                     if (last && ++buf == BUFFERS) buf = 0, acc_ph ^= 1u;
+                    few_block<FP8>(d, w, h, few_idesc<FP8>(it.n), !FP8 && b > it.b0, last, done, used, bars.acc_empty + 8 * buf, acc_ph, bars.full + 8 * s, ph, acc_free, there);
                 }
                 g_tc_commit(bars.cols_empty + 8 * place);
                 if (++place == 2) place = 0, cols_ph ^= 1u;
@@ -727,10 +783,31 @@ moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) 
             if (lane == 0) g_mbar_arrive(bars.cols_full + 8 * place);
             if (++place == 2) place = 0, cols_ph ^= 1u;
         }
+    } else if (warp == 2 || warp == 3) {  // the tokens whose last partial sums an item's were: all of them, in order; a token a warp
+        int slot = 0;
+        uint32_t ph = 0;
+        for (int i = blockIdx.x; i < items; i += gridDim.x) {
+            const Item it = item_of(i);
+            if (!tc_wait(bars.part_full + 8 * slot, ph, bars.dead)) break;
+            const int c = lane * 2 + warp - 2;
+            bool last = false;
+            if (c < it.tokens) {
+                const int t = lists.column[it.pos * 32 + it.first + c] >> 8;
+                uint32_t before;  // the release is for what the sums' warps wrote ahead of the barrier
+                asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(a.finished + it.m * kFewTokens + t) : "memory");
+                last = before == static_cast<uint32_t>(need[t] - 1);
+            }
+            uint32_t whole = __ballot_sync(0xffffffffu, last);
+            __threadfence();  // the other lanes read behind the acquiring lane
+            for (; whole; whole &= whole - 1)
+                few_output<OUT>(a, lists.column[it.pos * 32 + it.first + (__ffs(whole) - 1) * 2 + warp - 2] >> 8, it.m * 128 + lane * 4, pairs, idx, gate);
+            if (lane == 0) g_mbar_arrive(bars.part_empty + 8 * slot);
+            if (++slot == 2) slot = 0, ph ^= 1u;
+        }
     } else if (warp >= 8) {
         const int quarter = warp & 3, half = (warp - 8) >> 2, row = quarter * 32 + lane, me = tid - 256;
-        int buf = 0, place = 0;
-        uint32_t acc_ph = 0, cols_ph = 0;
+        int buf = 0, place = 0, slot = 0;
+        uint32_t acc_ph = 0, cols_ph = 0, part_ph = 1;
         for (int i = blockIdx.x; i < items; i += gridDim.x) {
             const Item it = item_of(i);
             bool ok = tc_wait(bars.cols_full + 8 * place, cols_ph, bars.dead);  // their factors
@@ -742,7 +819,7 @@ moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) 
                 for (int c = 0; c < COLS; ++c) acc[c] = 0.f;
                 const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * COLS;
                 for (int b = it.b0; b < (FP8 ? it.b1 : it.b0 + 1); ++b) {
-                    float4 f[COLS / 4];
+                    [[maybe_unused]] float4 f[COLS / 4];
                     if constexpr (FP8) {
 #pragma unroll
                         for (int c = 0; c < COLS / 4; ++c) f[c] = *reinterpret_cast<const float4 *>(factor + (b - it.b0) * kFewSecondN + half * COLS + c * 4);
@@ -750,7 +827,8 @@ moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) 
                     ok &= tc_wait(bars.acc_full + 8 * buf, acc_ph, bars.dead);
                     g_tc_fence_after();
                     uint32_t v[COLS];
-                    few_ld(from + buf * kFewSecondN, v);
+                    few_ld<COLS>(from + buf * kFewSecondN, v);
+                    few_ld_wait();
                     g_tc_fence_before();
                     __syncwarp();
                     if (lane == 0) g_mbar_arrive(bars.acc_empty + 8 * buf);
@@ -778,53 +856,16 @@ moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) 
                 for (int term = 1; term < TERMS; ++term) y += sums[(term * it.tokens + c) * 128 + r];
                 if (d < a.dim) a.part[((size_t)it.split * pairs + (column >> 8) * a.top + (column & 255)) * a.dim + d] = y * bad;
             }
-            // ---- the last item of these output columns: all partial sums, in order
-            __threadfence();
+            // written by all of these warps: two other warps see to what follows from it, two items behind at most
             asm volatile("bar.sync 1, 256;" ::: "memory");
-            if (me == 0) *bars.last = atomicAdd(a.finished + it.m, 1u);
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            if (*bars.last != static_cast<uint32_t>(groups * a.splits - 1)) continue;
-            __threadfence();
-            for (int j = me; j < a.tokens * 32; j += 256) {
-                const int t = j >> 5, d = it.m * 128 + (j & 31) * 4;  // four columns; a row has a multiple of eight
-                if (d >= a.dim) continue;
-                float y[4] = {0.f, 0.f, 0.f, 0.f};
-                constexpr int AT_ONCE = 8;
-                for (int k0 = 0; k0 < a.top; k0 += AT_ONCE) {
-                    float4 z[AT_ONCE];
-                    int e[AT_ONCE];
-#pragma unroll
-                    for (int u = 0; u < AT_ONCE; ++u) z[u] = make_float4(0.f, 0.f, 0.f, 0.f), e[u] = k0 + u < a.top ? idx[t * a.top + k0 + u] : -1;
-                    for (int s = 0; s < a.splits; ++s)
-#pragma unroll
-                        for (int u = 0; u < AT_ONCE; ++u)
-                            if (e[u] >= 0 && e[u] < a.experts) {
-                                const uint4 w = tl::ld_cg(reinterpret_cast<const uint4 *>(a.part + ((size_t)s * pairs + t * a.top + k0 + u) * a.dim + d));
-                                z[u].x += __uint_as_float(w.x), z[u].y += __uint_as_float(w.y), z[u].z += __uint_as_float(w.z), z[u].w += __uint_as_float(w.w);
-                            }
-#pragma unroll
-                    for (int u = 0; u < AT_ONCE; ++u) {
-                        if (e[u] < 0) continue;
-                        const float w = gate[t * a.top + k0 + u];
-                        if (e[u] >= a.experts) {
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) y[c] = few_identity(a, e[u], w, t, d + c, y[c]);
-                        } else {
-                            y[0] = fmaf(w, z[u].x, y[0]), y[1] = fmaf(w, z[u].y, y[1]), y[2] = fmaf(w, z[u].z, y[2]), y[3] = fmaf(w, z[u].w, y[3]);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int c = 0; c < 4; ++c) few_store<OUT>(a, t, d + c, y[c]);
+            if (warp == 8) {
+                tc_wait(bars.part_empty + 8 * slot, part_ph, bars.dead);
+                if (lane == 0) g_mbar_arrive(bars.part_full + 8 * slot);
             }
+            if (++slot == 2) slot = 0, part_ph ^= 1u;
         }
-        if (items == 0)  // every choice an identity expert, or none
-            for (int j = blockIdx.x * 256 + me; j < a.tokens * a.dim; j += gridDim.x * 256) {
-                const int t = j / a.dim, d = j % a.dim;
-                float y = 0.f;
-                for (int k = 0; k < a.top; ++k) y = few_identity(a, idx[t * a.top + k], gate[t * a.top + k], t, d, y);
-                few_store<OUT>(a, t, d, y);
-            }
+        for (int j = blockIdx.x * 8 + warp - 8; j < a.tokens * outs; j += gridDim.x * 8)  // tokens without an expert's product
+            if (need[j / outs] == 0) few_output<OUT>(a, j / outs, j % outs * 128 + lane * 4, pairs, idx, gate);
     }
     __syncwarp();
     g_tc_fence_before();
@@ -876,14 +917,14 @@ static int few_nt(int tokens) { return ceil_div(tokens, 8); }
 static int few_blocks(int ff, bool fp8) { return ceil_div(ff, fp8 ? 128 : 64); }
 
 // Parts of the second product's reduction: as many as an item's columns need, or more where they let the SMs end closer together, by the blocks that the busiest
-// takes (and two more an item for what it costs besides), if no two tokens choose the same expert.  The number of experts does not matter: it changes no bits.
+// takes (and six more an item for what it costs besides), if no two tokens choose the same expert.  The number of experts does not matter: it changes no bits.
 static int few_splits(int tokens, int dim, int top, int ff, bool fp8) {
     const int blocks = few_blocks(ff, fp8), outs = ceil_div(dim, 128);
-    const int fewest = ceil_div(blocks, kFewItemBlocks);
+    const int terms = fp8 ? 3 : 2, cols_block = ceil_div(std::min(tokens, kFewSecondN / terms) * terms, 8) * 1024, fewest = ceil_div(blocks, kFewItemCols / cols_block);
     int best = fewest;
     long long least = 0;
     for (int s = fewest; s <= std::max(fewest, std::min(blocks, 8)); ++s) {
-        const long long time = (long long)ceil_div(tokens * top * outs * s, 148) * (ceil_div(blocks, s) + 2);
+        const long long time = (long long)ceil_div(tokens * top * outs * s, 148) * (ceil_div(blocks, s) + 6);
         if (s == fewest || time < least) best = s, least = time;
     }
     return best;
@@ -892,7 +933,7 @@ static int few_splits(int tokens, int dim, int top, int ff, bool fp8) {
 static size_t few_align(size_t n) { return (n + 15) & ~(size_t)15; }
 static size_t few_bytes(int tokens, int dim, int top, int ff, bool fp8) {
     const size_t pairs = (size_t)tokens * top;
-    return few_align(pairs * 4) * 2 + few_align((size_t)tokens * 4) + few_align((size_t)ceil_div(dim, 128) * 4) + pairs * few_inner_ld(ff) * 4 +
+    return few_align(pairs * 4) * 2 + few_align((size_t)tokens * 4) + few_align((size_t)ceil_div(dim, 128) * kFewTokens * 4) + pairs * few_inner_ld(ff) * 4 +
            (size_t)few_splits(tokens, dim, top, ff, fp8) * pairs * dim * 4;
 }
 
@@ -919,11 +960,11 @@ static int few_launch(K kernel, tl::PerDevice &ready, int grid, int cluster, int
 }
 
 template <bool FP8, int NT>
-static int few_run(const CUtensorMap &m0, const CUtensorMap &m1, const CUtensorMap &m2, const FewArgs &a, bool gated, bool wide, cudaStream_t st) {
+static int few_run(const CUtensorMap &mx, const CUtensorMap &m0, const CUtensorMap &m1, const CUtensorMap &m2, const FewArgs &a, bool gated, bool wide, cudaStream_t st) {
     static tl::PerDevice with, without, second16, second32;
     const int smem = FewFirstSmem(a.tokens, NT, a.dim, a.outputs, a.experts, a.top, a.group_count, FP8, kFewSmem).total;
-    if (int e = gated ? few_launch(moe_few_first_kernel<FP8, true, NT>, with, 0, kFewCluster, smem, st, m0, m1, a)
-                      : few_launch(moe_few_first_kernel<FP8, false, NT>, without, 0, kFewCluster, smem, st, m0, m1, a))
+    if (int e = gated ? few_launch(moe_few_first_kernel<FP8, true, NT>, with, 0, kFewCluster, smem, st, mx, m0, m1, a)
+                      : few_launch(moe_few_first_kernel<FP8, false, NT>, without, 0, kFewCluster, smem, st, mx, m0, m1, a))
         return e;
     const int smem2 = FewSecondSmem(a.tokens, a.experts, a.top, kFewSmem).total;
     return wide ? few_launch(moe_few_second_kernel<FP8, float>, second32, sm_count(), 1, smem2, st, m2, a)
@@ -976,27 +1017,28 @@ int tlb_moe_few(const tlb_moe_few_layer *l, const void *x, int tokens, const voi
     a.idx = (int32_t *)at, at += few_align(pairs * 4);
     a.gate = (float *)at, at += few_align(pairs * 4);
     a.side = (float *)at, at += few_align((size_t)tokens * 4);
-    a.finished = (uint32_t *)at, at += few_align((size_t)ceil_div(dim, 128) * 4);
+    a.finished = (uint32_t *)at, at += few_align((size_t)ceil_div(dim, 128) * kFewTokens * 4);
     a.inner = (float *)at, a.ld_inner = few_inner_ld(ff), at += pairs * a.ld_inner * 4;
     a.part = (float *)at, a.splits = few_splits(tokens, dim, top, ff, fp8 != 0), a.room = kFewSmem;
     // what lies between a row's last number and the next row is read as zeros
     const uint64_t in = (uint64_t)dim * size, inner = (uint64_t)ff * size;
-    CUtensorMap m0, m1, m2;
+    CUtensorMap mx, m0, m1, m2;
+    const int nt = few_nt(tokens);
+    if (int e = tc_map_bytes(&mx, x, (uint64_t)dim * 2, tokens, (uint64_t)dim * 2, 8 * nt)) return e;
     if (int e = tc_map_bytes3(&m0, l->w_gate ? l->w_gate : l->w_up, in, ff, experts, l->ld_in, l->w_gate ? 64 : 128)) return e;
     if (int e = tc_map_bytes3(&m1, l->w_up, in, ff, experts, l->ld_in, 64)) return e;
     if (int e = tc_map_bytes3(&m2, l->w_down, inner, dim, experts, l->ld_out, 128)) return e;
-    const int nt = few_nt(tokens);
     const cudaStream_t st = as_stream(stream);
     const bool gated = l->w_gate != nullptr, wide = out_f32 != 0;
     switch (nt + (fp8 ? 4 : 0)) {
-        case 1: return few_run<false, 1>(m0, m1, m2, a, gated, wide, st);
-        case 2: return few_run<false, 2>(m0, m1, m2, a, gated, wide, st);
-        case 3: return few_run<false, 3>(m0, m1, m2, a, gated, wide, st);
-        case 4: return few_run<false, 4>(m0, m1, m2, a, gated, wide, st);
-        case 5: return few_run<true, 1>(m0, m1, m2, a, gated, wide, st);
-        case 6: return few_run<true, 2>(m0, m1, m2, a, gated, wide, st);
-        case 7: return few_run<true, 3>(m0, m1, m2, a, gated, wide, st);
-        default: return few_run<true, 4>(m0, m1, m2, a, gated, wide, st);
+        case 1: return few_run<false, 1>(mx, m0, m1, m2, a, gated, wide, st);
+        case 2: return few_run<false, 2>(mx, m0, m1, m2, a, gated, wide, st);
+        case 3: return few_run<false, 3>(mx, m0, m1, m2, a, gated, wide, st);
+        case 4: return few_run<false, 4>(mx, m0, m1, m2, a, gated, wide, st);
+        case 5: return few_run<true, 1>(mx, m0, m1, m2, a, gated, wide, st);
+        case 6: return few_run<true, 2>(mx, m0, m1, m2, a, gated, wide, st);
+        case 7: return few_run<true, 3>(mx, m0, m1, m2, a, gated, wide, st);
+        default: return few_run<true, 4>(mx, m0, m1, m2, a, gated, wide, st);
     }
 }
 
