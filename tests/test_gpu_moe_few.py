@@ -149,6 +149,17 @@ def bf(gen, *shape, std=1.0):
 
 @gpu
 @pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("T,D,ff,E,top", [
+    # inner rows in several parts; all tokens on one expert, in several groups; more router outputs than a cluster takes at once; the widest rows
+    (1, 64, 6500, 2, 1), (12, 136, 3300, 3, 2), (32, 72, 1700, 1, 1), (32, 72, 100, 2, 2), (3, 64, 40, 300, 2), (20, 264, 40, 140, 7), (2, 11264, 40, 2, 1),
+])
+def test_long_crowded_and_wide(T, D, ff, E, top, fp8):
+    h, router, wg, wu, wd = make(T, D, ff, E, fp8)
+    check(FewTokenExperts(TopKRouter(router, None, top), wg, wu, wd, "silu"), h, reference(h, router, wg, wu, wd, "silu", top=top))
+
+
+@gpu
+@pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("T,scoring,groups,identity,act,gated", [
     (3, "sigmoid", None, 0, "gelu_tanh", True), (12, "softmax_all", None, 2, "silu", True), (6, "softmax_all", (4, 2), 0, "clamped_swish", True),
     (20, "softmax", (3, 1), 1, "silu", False), (8, "sigmoid", None, 0, "relu_squared", False), (27, "softmax", None, 0, "relu_squared", False),
