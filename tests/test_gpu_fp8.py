@@ -74,6 +74,18 @@ def test_linear(rows, n, k, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("n", [4108, 4112, 6001, 6112, 7105, 7120, 8331, 8336])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_linear_of_every_width_of_tile(n, dtype):
+    """Tiles of 160, 192, 224 and 256 outputs, whole pieces of a row and not; the tile's width changes no bits."""
+    x, w, bias = make(257, n, 300, dtype, bias=n % 2 == 1)
+    got = fp8_linear(x, w, bias)
+    check_linear(x, w, bias, got)
+    part = fp8_linear(x, Fp8Weights(w.values[:4096, :300], w.scales[:32].contiguous()), None if bias is None else bias[:4096].contiguous())
+    assert torch.equal(part, got[:, :4096])
+
+
+@gpu
 @pytest.mark.parametrize("rows,n,k", [(1, 2560, 9728), (24, 2560, 4096), (48, 5000, 3000), (100, 2048, 6144), (700, 1200, 2600), (2100, 900, 1111)])
 def test_linear_of_real_sizes(rows, n, k):
     x, w, bias = make(rows, n, k, torch.bfloat16)

@@ -67,6 +67,11 @@ int f8_product(const F8Product &a, cudaStream_t st);
 bool f8_own(const F8Product &p);
 int f8_product_own(const F8Product &a, const F8Rows &x, cudaStream_t st);
 // blocks_fp8_pairs.cu: the same for many rows, and, of 128 rows of a gate and 128 of an up projection in turn, the gated rows rounded to e4m3 (to.q, to.scales)
+struct F8PairsWidth {
+    int outputs;  // of a tile
+    float block;  // us of a block of a tile; of the widths' best: of a block of all tiles of a pair
+};
+F8PairsWidth f8_pairs_width(int rows, int n);
 int f8_pairs(const F8Product &a, cudaStream_t st);
 int f8_pairs_gated(const F8Product &a, const F8Rows &to, cudaStream_t st);
 long long f8_gave_up();

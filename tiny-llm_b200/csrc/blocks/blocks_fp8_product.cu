@@ -377,12 +377,12 @@ static int f8_tile(const F8Product &p) {
     const struct {
         int tokens, outputs, room;
         float block;
-    } kinds[] = {{32, 128, 2 * sms, 0.48f}, {64, 128, 2 * sms, 0.66f}, {128, 128, sms, 0.56f}, {256, 256, sms / 2, 0.58f}};
-    int best = 0;
-    float least = INFINITY;
+    } kinds[] = {{32, 128, 2 * sms, 0.48f}, {64, 128, 2 * sms, 0.66f}, {128, 128, sms, 0.56f}};
+    int best = 256;
+    float least = f8_pairs_width(p.rows, p.n).block * k_blocks;
     for (const auto &t : kinds) {
         const long long tiles = (long long)ceil_div(p.n, t.outputs) * ceil_div(p.rows, t.tokens);
-        const int splits = t.tokens == 256 ? 1 : f8_splits(tiles, k_blocks, t.room);
+        const int splits = f8_splits(tiles, k_blocks, t.room);
         const float time = (float)((tiles * splits + t.room - 1) / t.room) * ceil_div(k_blocks, splits) * t.block;
         if (time < least) least = time, best = t.tokens;
     }
