@@ -74,6 +74,24 @@ def test_linear(rows, n, k, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("rows,k,apart", [(33000, 112, 0), (16400, 144, 16), (11001, 384, 0), (4100, 1040, 8), (4100, 1048, 0), (3700, 1200, 3)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_linear_of_many_rows(rows, k, apart, dtype):
+    """Enough rows for the rounding of several runs a warp: runs that end early, rows apart, rows that are no whole pieces."""
+    x, w, _ = make(rows, 24, k, dtype)
+    if apart:
+        wide = torch.zeros(rows, k + apart, dtype=dtype, device=DEV)
+        wide[:, :k] = x
+        x = wide[:, :k]
+    x[7, :] = 0
+    x[8, k // 2] = float("inf")
+    got = fp8_linear(x, w)
+    assert torch.isnan(got[8]).all() and (got[7] == 0).all()
+    keep = torch.arange(rows, device=DEV) != 8
+    check_linear(x[keep], w, None, got[keep])
+
+
+@gpu
 @pytest.mark.parametrize("n", [4108, 4112, 6001, 6112, 7105, 7120, 8331, 8336])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_linear_of_every_width_of_tile(n, dtype):

@@ -2,6 +2,7 @@
 //
 // A half warp takes a run: eight numbers a lane (one or two 16-byte loads), their largest by four exchanges, eight bytes out.  Bound by
 // HBM: a number is read once and a byte written.
+// Few rows are bound by the launch.
 #include "blocks_fp8.cuh"
 
 namespace tlb {
@@ -30,67 +31,122 @@ __device__ __forceinline__ void rows_load(const T *p, int left, float (&v)[8]) {
     }
 }
 
-// WIDE: every group of eight is whole and aligned to 16 bytes.  A half warp takes U runs, neighbours in its row-by-row order, all on their way at once.
-template <typename T, bool GATED, bool WIDE, int U>
+// WIDE: every group of eight is whole and aligned to 16 bytes.
+template <typename T, bool GATED, bool WIDE>
 __global__ void __launch_bounds__(kRowsThreads)
 fp8_rows_kernel(const T *x, long long ldx, int rows, int cols, int act, float limit, float slope, uint8_t *q, int ldq, float *scales, int ld_scales) {
-    const unsigned runs = (cols + kF8Block - 1) / kF8Block, total = rows * runs, lane = threadIdx.x & 15;
-    const unsigned first = ((blockIdx.x * kRowsThreads + threadIdx.x) >> 4) * U;
+    const unsigned runs = (cols + kF8Block - 1) / kF8Block, total = rows * runs, lane = threadIdx.x & 15, mine = (blockIdx.x * kRowsThreads + threadIdx.x) >> 4;
     tl::griddep_wait();
     tl::griddep_launch();  // behind the wait: what a dependent reads ahead of its own is older than this launch
-    float v[U][8];
-    unsigned row[U], run[U];
+    const bool live = mine < total;  // a half warp as one
+    const unsigned row = live ? mine / runs : 0, run = live ? mine - row * runs : 0;
+    const int k = run * kF8Block + lane * 8, left = live ? cols - k : 0;
+    float v[8];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const bool live = first + u < total;  // a half warp as one
-        row[u] = live ? (first + u) / runs : 0, run[u] = live ? first + u - row[u] * runs : 0;
-        const int k = run[u] * kF8Block + lane * 8, left = live ? cols - k : 0;
+    for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    if (left > 0) {
+        if constexpr (GATED) {  // the columns of a whole run are there, those past the last feature are zero
+            const T *from = x + row * ldx + run * 2 * kF8Block + lane * 8;
+            float g[8], up[8];
+            rows_load<T, WIDE>(from, 8, g);
+            rows_load<T, WIDE>(from + kF8Block, 8, up);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
-        if (left > 0) {
-            if constexpr (GATED) {  // the columns of a whole run are there, those past the last feature are zero
-                const T *from = x + row[u] * ldx + run[u] * 2 * kF8Block + lane * 8;
-                float g[8], up[8];
-                rows_load<T, WIDE>(from, 8, g);
-                rows_load<T, WIDE>(from + kF8Block, 8, up);
+            for (int i = 0; i < 8; ++i) v[i] = i < left ? gated_pair(g[i], up[i], act, limit, slope) : 0.f;
+        } else {
+            rows_load<T, WIDE>(x + row * ldx + k, left, v);
+        }
+    }
+    float most = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[u][i] = i < left ? gated_pair(g[i], up[i], act, limit, slope) : 0.f;
-            } else {
-                rows_load<T, WIDE>(x + row[u] * ldx + k, left, v[u]);
-            }
+    for (int i = 0; i < 8; ++i) most = f8_most(most, fabsf(v[i]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) most = f8_most(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const F8Scale s = f8_scale(most);
+    if (!live) return;
+    if (lane == 0) scales[(size_t)run * ld_scales + row] = s.scale;
+    if (k >= ldq) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], s.times);
+    *reinterpret_cast<uint2 *>(q + (size_t)row * ldq + k) = make_uint2(f8_pack4(v[0], v[1], v[2], v[3]), f8_pack4(v[4], v[5], v[6], v[7]));
+}
+
+// The same for many rows of whole groups of 16, which the instructions of a run's two quotients and of finding it bound in the form above (4096 rows of 9728:
+// 64 % of the issue slots at half of HBM's rate).  Here eight lanes take a run, 16 numbers each, a warp eight runs, neighbours in their row-by-row order; eight lanes
+// make the quotients of all eight, and one division finds the first.
+template <typename T>
+__global__ void __launch_bounds__(kRowsThreads)
+fp8_many_rows_kernel(const T *x, long long ldx, int rows, int cols, uint8_t *q, int ldq, float *scales, int ld_scales) {
+    const unsigned runs = (cols + kF8Block - 1) / kF8Block, total = rows * runs, lane = threadIdx.x & 31;
+    const unsigned first = ((blockIdx.x * kRowsThreads + threadIdx.x) >> 5) * 8;
+    tl::griddep_wait();
+    tl::griddep_launch();
+    if (first >= total) return;
+    const unsigned row0 = first / runs, run0 = first - row0 * runs;
+    auto place = [&](unsigned i, unsigned &row, unsigned &run) {  // of the warp's run i
+        row = row0, run = run0 + i;
+        while (run >= runs) run -= runs, ++row;
+    };
+    float v[2][16], most[2];
+    unsigned row[2], run[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const unsigned i = u * 4 + (lane >> 3);
+        place(i, row[u], run[u]);
+        const int k = run[u] * kF8Block + (lane & 7) * 16;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float half[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (first + i < total && k < cols) rows_load<T, true>(x + row[u] * ldx + k + h * 8, 8, half);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[u][h * 8 + j] = half[j];
         }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        float most = 0.f;
+    for (int u = 0; u < 2; ++u) {
+        most[u] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) most = f8_most(most, fabsf(v[u][i]));
+        for (int j = 0; j < 16; ++j) most[u] = f8_most(most[u], fabsf(v[u][j]));
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) most = f8_most(most, __shfl_xor_sync(0xffffffffu, most, o));
-        const F8Scale s = f8_scale(most);
-        if (first + u >= total) continue;
-        if (lane == 0) scales[(size_t)run[u] * ld_scales + row[u]] = s.scale;
-        const int k = run[u] * kF8Block + lane * 8;
-        if (k >= ldq) continue;
+        for (int o = 4; o > 0; o >>= 1) most[u] = f8_most(most[u], __shfl_xor_sync(0xffffffffu, most[u], o));
+    }
+    const float a = __shfl_sync(0xffffffffu, most[0], (lane & 3) * 8), b = __shfl_sync(0xffffffffu, most[1], (lane & 3) * 8);
+    const F8Scale s = f8_scale(lane & 4 ? b : a);  // of the warp's run lane & 7
+    if (lane < 8 && first + lane < total) {
+        unsigned at_row, at_run;
+        place(lane, at_row, at_run);
+        scales[(size_t)at_run * ld_scales + at_row] = s.scale;
+    }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[u][i] = __fmul_rn(v[u][i], s.times);
-        *reinterpret_cast<uint2 *>(q + (size_t)row[u] * ldq + k) = make_uint2(f8_pack4(v[u][0], v[u][1], v[u][2], v[u][3]), f8_pack4(v[u][4], v[u][5], v[u][6], v[u][7]));
+    for (int u = 0; u < 2; ++u) {
+        const unsigned i = u * 4 + (lane >> 3);
+        const float times = __shfl_sync(0xffffffffu, s.times, i);
+        const int k = run[u] * kF8Block + (lane & 7) * 16;
+        if (first + i >= total || k >= ldq) continue;
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            w[j] = f8_pack4(__fmul_rn(v[u][4 * j], times), __fmul_rn(v[u][4 * j + 1], times), __fmul_rn(v[u][4 * j + 2], times), __fmul_rn(v[u][4 * j + 3], times));
+        *reinterpret_cast<uint4 *>(q + (size_t)row[u] * ldq + k) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
 int f8_rows(const F8Rows &a, cudaStream_t st) {
     const long long runs = (long long)a.rows * ceil_div(a.cols, kF8Block);
     if (runs > 0x7fffff00LL) return tl::fail(TL_EINVAL, "fp8_rows: too many rows");
-    const bool many = runs >= 32 * 1024;  // below, one run a half warp puts more warps to work
-#define TLB_ROWS(T, G, W, U)                                                                                                                            \
-    tl::launch_chained(fp8_rows_kernel<T, G, W, U>, dim3((unsigned)((runs + 16 * U - 1) / (16 * U))), dim3(kRowsThreads), 0, st, (const T *)a.x, a.ldx, a.rows, a.cols, \
-                       a.act, a.limit, a.slope, a.q, a.ldq, a.scales, a.ld_scales)
+#define TLB_ROWS(T, G, W)                                                                                                                                          \
+    tl::launch_chained(fp8_rows_kernel<T, G, W>, dim3((unsigned)((runs + 15) / 16)), dim3(kRowsThreads), 0, st, (const T *)a.x, a.ldx, a.rows, a.cols, a.act, a.limit, \
+                       a.slope, a.q, a.ldq, a.scales, a.ld_scales)
     if (a.gated) {
-        TLB_ROWS(float, true, true, 1);
+        TLB_ROWS(float, true, true);
     } else {
         const size_t es = a.dtype == TL_BF16 ? 2 : 4;
         const bool wide = a.cols % 8 == 0 && (a.ldx * es) % 16 == 0 && tl::aligned16(a.x);
-        TLB_DISPATCH(a.dtype, "fp8_rows", if (wide && many) TLB_ROWS(T, false, true, 4); else if (wide) TLB_ROWS(T, false, true, 1); else TLB_ROWS(T, false, false, 1));
+        if (wide && a.cols % 16 == 0 && runs >= 32 * 1024) {  // below, fewer numbers a warp put more warps to work
+            const dim3 grid((unsigned)((runs + kRowsThreads / 4 - 1) / (kRowsThreads / 4)));
+            TLB_DISPATCH(a.dtype, "fp8_rows", tl::launch_chained(fp8_many_rows_kernel<T>, grid, dim3(kRowsThreads), 0, st, (const T *)a.x, a.ldx, a.rows, a.cols, a.q, a.ldq, a.scales, a.ld_scales));
+        } else {
+            TLB_DISPATCH(a.dtype, "fp8_rows", if (wide) TLB_ROWS(T, false, true); else TLB_ROWS(T, false, false));
+        }
     }
 #undef TLB_ROWS
     TL_LAUNCH_CHECK("fp8_rows");
