@@ -4,18 +4,25 @@
 //   first launch:  logits = router . x, the choice, inner[pair] = act(gate_e x) * (up_e x)        pair = (token, choice)
 //   second launch: y[t] = sum over choices  weight * (down_e inner[pair])  (+ identity experts, + shared expert)
 //
-// Bound by HBM: every matrix of a chosen expert is read once.  The products are tcgen05.mma with 128 matrix rows as the M side, fed by TMA in boxes of 128 bytes
-// a row, and the tokens as 16 to 64 columns; a matrix costs no thread more than its copies and the sums' additions.  What the columns hold:
+// Bound by HBM where many experts are chosen: every matrix of a chosen expert is read once.  The products are tcgen05.mma with 128 matrix rows as the M side, fed by
+// TMA in boxes of 128 bytes a row, and the tokens as 16 to 64 columns: a matrix costs no thread more than its copies and the sums' additions (mma.sync on
+// fragments that threads unpack took 380 instructions for 2 KB).  What the columns hold:
 //
 //   bf16 experts:  x as it is; an inner row as two bf16 terms (off by 2^-16 of a number)
 //   e4m3 experts:  both operands of a product have 8 bits, so a number is several e4m3 terms, a column each, added when the sums are taken out: x, whose 8 bits
-//                  two terms of 4 hold exactly (times a power of two for each token; numbers below 2^-22 of the row's largest lose bits), an inner row three
-//                  (off by 2^-12, times a power of two for each block of 128).  A block of 128 is added in the tensor cores, then times its scales in fp32.
+//                  two terms of 4 hold exactly (times a power of two for each token; bits below 2^-21 of the token's largest magnitude are lost), an inner row
+//                  three (off by 2^-12, or by 2^-25 of the largest of its block of 128: a power of two for each block).  A block of 128 is added in the
+//                  tensor cores, then times its scales in fp32.
 //
 // First launch: the CTAs of a cluster share the router's rows and exchange the logits through shared memory, and every CTA makes the same choices and the columns
-// for itself.  A tile is 64 features of an expert, gate rows and up rows in one accumulator.  Second launch: an item is 128 output columns of an expert for up to
-// 10 (16) of its tokens, over a part of the reduction; its partial sums go to memory, and the CTA that finishes an output block's last item adds them all, in
-// order (a counter tells; no CTA waits for another outside its cluster).
+// for itself, in the place the tokens were copied to.  A tile is 64 features of an expert, gate rows and up rows in one accumulator.  Second launch: an item is 128 output
+// columns of an expert for up to 10 (bf16: 16) of its tokens, over a part of the reduction; its partial sums go to memory, and whoever writes a token's last one adds
+// them all, in order (a counter tells; no CTA waits for another outside its cluster).
+//
+// 64 experts of 1408 x 2048, 6 a token: 1 token 30 us in e4m3 and 38 in bf16, of which some 17 are the weights' and the rest one latency behind another (tokens and
+// router rows, choice, first tile, sums, inner rows, sums, outputs); 32 tokens 136 us in e4m3, 528 MB of weights: 3.9 TB/s over the whole call, about 6 within the
+// two launches' tiles, some 17 us of prologue (all CTAs: 128 KB of tokens, their columns, 32 choices).  With tokens in fp16 on mma.sync and weights through a queue of
+// cp.async it took 184.
 #include <atomic>
 
 #include "../per_device.h"
@@ -788,7 +795,13 @@ moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) 
         uint32_t ph = 0;
         for (int i = blockIdx.x; i < items; i += gridDim.x) {
             const Item it = item_of(i);
-            if (!tc_wait(bars.part_full + 8 * slot, ph, bars.dead)) break;
+            if (!tc_wait(bars.part_full + 8 * slot, ph, bars.dead)) {  // nobody else makes these outputs: what is not counted here never becomes whole
+                for (int c = warp - 2; c < it.tokens; c += 2)
+                    for (int d = it.m * 128 + lane; d < min(a.dim, it.m * 128 + 128); d += 32)
+                        static_cast<OUT *>(a.out)[(size_t)(lists.column[it.pos * 32 + it.first + c] >> 8) * a.dim + d] = from_f<OUT>(__int_as_float(0x7fffffff));
+                if (++slot == 2) slot = 0, ph ^= 1u;
+                continue;
+            }
             const int c = lane * 2 + warp - 2;
             bool last = false;
             if (c < it.tokens) {
