@@ -183,8 +183,9 @@ def _whole_rows(w: torch.Tensor, rows: int) -> torch.Tensor:
 class FewTokenExperts:
     """A whole mixture-of-experts layer for the few tokens of a decoding step in two launches: router and first products, second products
     and their sum.  Arguments as ``MixtureOfExperts`` takes them, the experts bf16 ``[E, ff, D]`` / ``[E, D, ff]`` or ``Fp8Weights`` of those shapes; the
-    router's weight is on the experts' output.  A step of more tokens than one call takes (32, fewer for very wide ones) is several calls, each of which reads its
-    experts anew: prompts are better served by ``MixtureOfExperts``."""
+    router's weight is on the experts' output.  A step of more tokens than one call takes (``run``: 32, at width 4096 16, 8 up to 11264, wider ones are refused) is
+    several calls, each of which reads its experts anew: prompts are better served by ``MixtureOfExperts``.  Inner rows keep 2^-16 of a number over bf16 experts and 2^-12 over
+    8-bit ones, which use of a token what lies above 2^-21 of its largest magnitude."""
 
     def __init__(self, router: TopKRouter, w_gate, w_up, w_down, act: str, shared: GatedMLP | None = None, identity: int = 0, limit: float = 0.0, slope: float = 1.0,
                  shared_gate: torch.Tensor | None = None):
