@@ -5,9 +5,9 @@
 // hands an SM in that time).  The tokens are the M side: a token's scale is a lane's and a block scale holds for a run of columns, so taking a block's accumulator
 // over into the sums, which live in registers, is one multiply-add an entry.  Eight warps do it, 128 columns each (16 warps with 64 took 30 % longer: the SM's issue
 // slots went into what a warp does a block beside the multiply-adds; two multiply-adds an instruction, fma.rn.f32x2, took longer than two).  Two accumulators of
-// all columns take turns: one is multiplied into while the other is taken over.
+// all columns (three of 160) take turns: one is multiplied into while another is taken over; asking the sums' barrier ahead as the products' thread does changed nothing.
 //
-// 8192 x 4096 -> 9472: 322 us, 1970 TF/s; 4096 x 9728 -> 2560: 149 us (1370 TF/s: 160 tiles for 74 pairs are three rounds, the last of 12 tiles).  Bound by
+// 8192 x 4096 -> 9472: 306 us, 2070 TF/s; 4096 x 9728 -> 2560: 142 us with the rounding (1440 TF/s: 192 tiles of 224 for 74 pairs are three rounds for 2.6).  Bound by
 // the way round from a finished accumulator to an empty one (0.62 us a block where its products alone take 0.3): the wait, two trips to tensor memory, the word back.
 //
 // 12 warps: 0 and 3 TMA, 1 the products (leader) or the news that the own stage is there (peer), 4-11 the sums.  The first four give registers to the others.
@@ -97,12 +97,13 @@ fp8_pairs_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const int unit = blockIdx.x >> 1, units = gridDim.x >> 1;
     const uint32_t base = g_smem_u32(pr_smem);
     constexpr int kBars = kPrStages * kPrStage + kPrSumWarps * kPrOut + kPrMost;
-    const uint32_t full = base + kBars, empty = full + 8 * kPrStages, acc_full = empty + 8 * kPrStages, acc_empty = acc_full + 16;
-    volatile int *dead = reinterpret_cast<volatile int *>(pr_smem + kBars + 16 * kPrStages + 32);
+    const uint32_t full = base + kBars, empty = full + 8 * kPrStages, acc_full = empty + 8 * kPrStages, acc_empty = acc_full + 32;
+    constexpr int BUFFERS = N == 160 ? 3 : 2, APART = N == 160 ? 160 : 256;  // accumulators, of 512 columns
+    volatile int *dead = reinterpret_cast<volatile int *>(pr_smem + kBars + 16 * kPrStages + 64);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(const_cast<int *>(dead)) + 1;
     if (warp == 1 && lane == 0) {
         for (int i = 0; i < kPrStages; ++i) g_mbar_init(full + 8 * i, rank == 0 ? 3 : 2), g_mbar_init(empty + 8 * i, 1);  // both kinds of copies, and on the leader's the peer's word
-        for (int i = 0; i < 2; ++i) g_mbar_init(acc_full + 8 * i, 1), g_mbar_init(acc_empty + 8 * i, 2 * kPrSumWarps);  // both CTAs' warps, on the leader's
+        for (int i = 0; i < BUFFERS; ++i) g_mbar_init(acc_full + 8 * i, 1), g_mbar_init(acc_empty + 8 * i, 2 * kPrSumWarps);  // both CTAs' warps, on the leader's
         *dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
@@ -152,9 +153,9 @@ fp8_pairs_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         if (!(ok = (acc_free || tc_wait_one(acc_empty + 8 * buf, acc_ph, dead)) && (there || tc_wait_one(full + 8 * s, ph, dead)))) break;
                         g_tc_fence_after();
                         const uint64_t q = g_smem_desc_sw128(base + s * kPrStage, 0, 1024), w = g_smem_desc_sw128(base + s * kPrStage + 128 * 128, 0, 1024);
-                        const uint32_t d = tmem + buf * 256, done = acc_full + 8 * buf, used = empty + 8 * s;
+                        const uint32_t d = tmem + buf * APART, done = acc_full + 8 * buf, used = empty + 8 * s;
                         if (++s == kPrStages) s = 0, ph ^= 1u;
-                        if (++buf == 2) buf = 0, acc_ph ^= 1u;
+                        if (++buf == BUFFERS) buf = 0, acc_ph ^= 1u;
                         pr_block<N>(d, q, w, done, used, acc_empty + 8 * buf, acc_ph, full + 8 * s, ph, acc_free, there);
                     }
             }
@@ -214,7 +215,7 @@ fp8_pairs_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 }
                 ok &= tc_wait(acc_full + 8 * buf, acc_ph, dead);
                 g_tc_fence_after();
-                const uint32_t at = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buf * 256;
+                const uint32_t at = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buf * APART;
                 uint32_t v[2][32];  // two reads on their way, and again two as soon as their places are free: the accumulator is empty after half of the additions
                 pr_ld<32>(at + row_a, v[0]);
                 pr_ld<32>(at + row_a + 32, v[1]);
@@ -234,7 +235,7 @@ fp8_pairs_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 }
 #pragma unroll
                 for (int i = 0; i < NB; ++i) acc_b[i] = fmaf(__uint_as_float(i < 32 ? v[0][i] : v[1][i - 32]), fb[i / RUN_B], acc_b[i]);
-                if (++buf == 2) buf = 0, acc_ph ^= 1u;
+                if (++buf == BUFFERS) buf = 0, acc_ph ^= 1u;
             }
             const float bad = tc_verdict(ok, dead);
             if constexpr (GATED) {
@@ -368,10 +369,11 @@ static int pr_launch(const F8Product &p, F8PairArgs &a, cudaStream_t st) {
 }
 
 // The width of the tiles: the one whose tiles the pairs are done with first, by what a block of a tile took where every pair had many (8192 x 4096 -> 9472: widths
-// 256, 224, 192, 160 took 322, 359, 368, 392 us).  2048 x 9728 -> 2560, 80 tiles of 256 for 74 pairs or 128 of 160: 94 us or 81; 512 x 2560 -> 9728: 32 or 25.
+// 256, 224, 192 took 322, 359, 368 us; 2048 x 9728 -> 2560 with 160 74).  2048 x 9728 -> 2560, 80 tiles of 256 for 74 pairs or 128 of 160: 90 us or 74; 512 x 2560 ->
+// 9728: 32 or 24.
 F8PairsWidth f8_pairs_width(int rows, int n) {
     F8PairsWidth best{256, INFINITY};
-    for (const F8PairsWidth &w : {F8PairsWidth{256, 0.62f}, F8PairsWidth{224, 0.60f}, F8PairsWidth{192, 0.54f}, F8PairsWidth{160, 0.49f}}) {
+    for (const F8PairsWidth &w : {F8PairsWidth{256, 0.62f}, F8PairsWidth{224, 0.60f}, F8PairsWidth{192, 0.54f}, F8PairsWidth{160, 0.46f}}) {
         const long long tiles = (long long)ceil_div(n, w.outputs) * ceil_div(rows, 256);
         const float time = (float)((tiles + sm_count() / 2 - 1) / (sm_count() / 2)) * w.block;
         if (time < best.block) best = {w.outputs, time};
