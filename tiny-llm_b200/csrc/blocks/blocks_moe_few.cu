@@ -19,10 +19,10 @@
 // columns of an expert for up to 10 (bf16: 16) of its tokens, over a part of the reduction; its partial sums go to memory, and whoever writes a token's last one adds
 // them all, in order (a counter tells; no CTA waits for another outside its cluster).
 //
-// 64 experts of 1408 x 2048, 6 a token: 1 token 30 us in e4m3 and 38 in bf16, of which some 17 are the weights' and the rest one latency behind another (tokens and
-// router rows, choice, first tile, sums, inner rows, sums, outputs); 32 tokens 136 us in e4m3, 528 MB of weights: 3.9 TB/s over the whole call, about 6 within the
+// 64 experts of 1408 x 2048, 6 a token: 1 token 29 us in e4m3 and 37 in bf16, of which some 8 and 16 are the weights' and the rest one latency behind another (tokens and
+// router rows, choice, first tile, sums, inner rows, sums, outputs); 32 tokens 134 us in e4m3, 528 MB of weights: 3.9 TB/s over the whole call, about 6 within the
 // two launches' tiles, some 17 us of prologue (all CTAs: 128 KB of tokens, their columns, 32 choices).  With tokens in fp16 on mma.sync and weights through a queue of
-// cp.async it took 184.
+// cp.async it took 184.  Asking the second launch's first matrices into L2 behind the first's last cost a microsecond: the two are close enough.
 #include <atomic>
 
 #include "../per_device.h"
@@ -47,8 +47,6 @@ struct FewArgs {
     float limit, slope;
     const bf16 *shared;
     void *out;
-    const uint8_t *w2;
-    int ld_out, row_out /* whole 16 bytes of a row */, prefetch;  // the first launch asks the second's first matrices into L2: bytes of a CTA
     // between the launches
     int32_t *idx;        // [tokens, top]
     float *gate;         // [tokens, top]
@@ -429,14 +427,6 @@ moe_few_first_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
                     tl::g_tma_load_3d(g_smem_u32(few_smem + at.ring) + s * kFewStage + (warp == 3 ? kFewStage / 2 : 0), warp == 3 ? &map1 : &map0, b * 128, f0, e,
                             bars.full + 8 * s);
                     if (++s == at.stages) s = 0, ph ^= 1u;
-                }
-            }
-            if (warp == 0) {  // the last weights of this launch are on their way: the first of the next one's are asked into L2 behind them
-                const int outs = (a.dim + 127) / 128, all = count * outs;
-                for (int i = blockIdx.x, left = a.prefetch; i < all && left > 0; i += gridDim.x) {
-                    const int d0 = i % outs * 128, bytes = (min(128, a.dim - d0) - 1) * a.ld_out + a.row_out;  // not past the last row's last number
-                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a.w2 + ((size_t)lists.active[i / outs] * a.dim + d0) * a.ld_out), "r"(bytes) : "memory");
-                    left -= bytes;
                 }
             }
         }
@@ -893,7 +883,6 @@ moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) 
 // ---- host ------------------------------------------------------------------------------------------------------------
 
 constexpr int kFewSmem = 227 * 1024, kFewMostGrid = 1024;
-constexpr int kFewPrefetch = 40 << 20;  // a third of L2
 
 // CTAs of the first launch: as many clusters as are resident at once, which a device's SMs in groups decide (132 CTAs of a B200).
 template <typename K>
@@ -931,6 +920,7 @@ static int few_blocks(int ff, bool fp8) { return ceil_div(ff, fp8 ? 128 : 64); }
 
 // Parts of the second product's reduction: as many as an item's columns need, or more where they let the SMs end closer together, by the blocks that the busiest
 // takes (and six more an item for what it costs besides), if no two tokens choose the same expert.  The number of experts does not matter: it changes no bits.
+// 1 token, 6 of 64 experts of 1408 x 2048: in one part 29.0 us (bf16 37.2), in three 30.7 (38.6).
 static int few_splits(int tokens, int dim, int top, int ff, bool fp8) {
     const int blocks = few_blocks(ff, fp8), outs = ceil_div(dim, 128);
     const int terms = fp8 ? 3 : 2, cols_block = ceil_div(std::min(tokens, kFewSecondN / terms) * terms, 8) * 1024, fewest = ceil_div(blocks, kFewItemCols / cols_block);
@@ -1024,7 +1014,7 @@ int tlb_moe_few(const tlb_moe_few_layer *l, const void *x, int tokens, const voi
     a.side_w = (const bf16 *)l->side_w, a.tokens = tokens, a.dim = dim, a.outputs = outputs, a.experts = experts, a.top = top, a.scoring = l->scoring, a.group_count = groups;
     a.group_keep = l->group_keep, a.weight_scale = l->weight_scale;
     a.s0 = l->w_gate ? l->s_gate : l->s_up, a.s1 = l->w_gate ? l->s_up : nullptr, a.s2 = l->s_down;
-    a.ff = ff, a.w2 = (const uint8_t *)l->w_down, a.ld_out = l->ld_out, a.row_out = ff * size / 16 * 16, a.prefetch = kFewPrefetch / sm_count();
+    a.ff = ff;
     a.act = l->act, a.limit = l->limit, a.slope = l->slope, a.shared = (const bf16 *)shared, a.out = out;
     uint8_t *at = (uint8_t *)workspace;
     a.idx = (int32_t *)at, at += few_align(pairs * 4);
