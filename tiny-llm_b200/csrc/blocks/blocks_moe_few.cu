@@ -199,7 +199,7 @@ constexpr int kFewBuffers = 4;  // accumulators, of bf16 experts 2 are used
 
 // ---- first launch ----------------------------------------------------------------------------------------------------
 
-constexpr int kFewCluster = 4;
+constexpr int kFewCluster = 4;  // of 2 (all 148 SMs) 1 token took 30.5 us for 29.1, 32 tokens the same
 // Columns of the products, for eight tokens each; e4m3: the first terms of all tokens, then the second.
 __host__ __device__ constexpr int few_columns(int nt, bool fp8) { return fp8 ? 16 * nt : nt <= 2 ? 16 : 32; }
 __host__ __device__ constexpr int few_router_sums(int nt) { return 16 * (nt * 8 + 2); }  // of a warp: 16 rows
