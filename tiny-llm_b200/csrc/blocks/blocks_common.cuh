@@ -56,11 +56,23 @@ __device__ __forceinline__ float act_apply(float z, int act) {
     return 0.5f * z * (1.0f + tanhf(inner));
 }
 
+// Bounds that a NaN passes (fminf and fmaxf would give the bound for it).
+__device__ __forceinline__ float at_most(float v, float limit) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(limit));
+    return r;
+}
+__device__ __forceinline__ float at_least(float v, float limit) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(limit));
+    return r;
+}
+
 // The inside of a gated feed-forward: act(g) * u, or (act 3) the clamped form, the gate bounded from above and the other half on
-// both sides: g sigmoid(slope g) (u + 1).
+// both sides: g sigmoid(slope g) (u + 1).  A NaN in either stays one.
 __device__ __forceinline__ float gated_pair(float g, float u, int act, float limit, float slope) {
     if (act == 3) {
-        g = fminf(g, limit), u = fminf(fmaxf(u, -limit), limit);
+        g = at_most(g, limit), u = at_most(at_least(u, -limit), limit);
         return g / (1.0f + expf(-slope * g)) * (u + 1.0f);
     }
     return act_apply(g, act) * u;
@@ -74,7 +86,7 @@ __device__ __forceinline__ void gated_pairs(const float (&g)[COUNT], const float
     } else if constexpr (ACT == 3) {
         float num[COUNT], factor[COUNT];
 #pragma unroll
-        for (int i = 0; i < COUNT; ++i) num[i] = fminf(g[i], limit), factor[i] = fminf(fmaxf(u[i], -limit), limit) + 1.0f;
+        for (int i = 0; i < COUNT; ++i) num[i] = at_most(g[i], limit), factor[i] = at_most(at_least(u[i], -limit), limit) + 1.0f;
         tl::quotient_times<T>(num, [&](float n) { return 1.0f + expf(-slope * n); }, factor, y, live);
     } else {
 #pragma unroll

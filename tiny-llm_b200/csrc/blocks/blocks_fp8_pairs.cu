@@ -244,7 +244,7 @@ fp8_pairs_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 float largest = 0.f;
 #pragma unroll
                 for (int i = 0; i < 64; ++i) {
-                    acc_a[i] = f0 + i < a.ff ? gated_pair(acc_a[i] * bad, acc_b[i], a.act, a.limit, a.slope) : 0.f;
+                    acc_a[i] = f0 + i < a.ff ? gated_pair(acc_a[i], acc_b[i], a.act, a.limit, a.slope) * bad : 0.f;
                     largest = f8_most(largest, fabsf(acc_a[i]));
                 }
                 most[half * 128 + quarter * 32 + lane] = largest;

@@ -516,12 +516,12 @@ moe_few_first_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
                         const float scale = m < 0x7f800000u ? few_exp2(few_exponent(__uint_as_float(m)) - 8) : __int_as_float(0x7fffffff);
                         return sums[t * 64 + r] * scale;
                     };
-                    const float v = of(in) * bad;
+                    const float v = of(in);
                     float y;
                     if constexpr (GATED) y = gated_pair(v, of(in + 32), a.act, a.limit, a.slope);
                     else y = a.act == 2 ? (v > 0.f ? v * v : v == v ? 0.f : v) : act_apply(v, a.act);
                     float *to = a.inner + ((size_t)t * a.top + (c & 255)) * a.ld_inner + f0;
-                    to[f] = y;
+                    to[f] = y * bad;
                     if (f0 + here == a.ff && f >= here - 16)  // zeros behind the last features
                         for (int z = a.ff + here - 1 - f; z < a.ld_inner; z += min(here, 16)) to[z - f0] = 0.f;
                 }
