@@ -237,4 +237,4 @@ class FewTokenExperts:
             y = self._few(h, shared, wide)
         else:
             y = torch.cat([self._few(h[t : t + self.run], None if shared is None else shared[t : t + self.run], wide) for t in range(0, T, self.run)])
-        return y[:, : self.width] if self._pad else y
+        return y[:, : self.width].contiguous() if self._pad else y  # the norm behind reads whole rows
