@@ -35,7 +35,8 @@ __device__ __forceinline__ void rows_load(const T *p, int left, float (&v)[8]) {
 template <typename T, bool GATED, bool WIDE>
 __global__ void __launch_bounds__(kRowsThreads)
 fp8_rows_kernel(const T *x, long long ldx, int rows, int cols, int act, float limit, float slope, uint8_t *q, int ldq, float *scales, int ld_scales) {
-    const unsigned runs = (cols + kF8Block - 1) / kF8Block, total = rows * runs, lane = threadIdx.x & 15, mine = (blockIdx.x * kRowsThreads + threadIdx.x) >> 4;
+    const unsigned runs = (cols + kF8Block - 1) / kF8Block, total = rows * runs, lane = threadIdx.x & 15;
+    const unsigned mine = blockIdx.x * (kRowsThreads / 16) + (threadIdx.x >> 4);  // a thread's number itself does not fit into 32 bits
     tl::griddep_wait();
     tl::griddep_launch();  // behind the wait: what a dependent reads ahead of its own is older than this launch
     const bool live = mine < total;  // a half warp as one
@@ -77,7 +78,7 @@ template <typename T>
 __global__ void __launch_bounds__(kRowsThreads)
 fp8_many_rows_kernel(const T *x, long long ldx, int rows, int cols, uint8_t *q, int ldq, float *scales, int ld_scales) {
     const unsigned runs = (cols + kF8Block - 1) / kF8Block, total = rows * runs, lane = threadIdx.x & 31;
-    const unsigned first = ((blockIdx.x * kRowsThreads + threadIdx.x) >> 5) * 8;
+    const unsigned first = (blockIdx.x * (kRowsThreads / 32) + (threadIdx.x >> 5)) * 8;
     tl::griddep_wait();
     tl::griddep_launch();
     if (first >= total) return;
