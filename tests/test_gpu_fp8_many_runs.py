@@ -21,3 +21,10 @@ def test_rows_behind_the_threads_of_32_bits():
     for start in range(0, rows, len(piece)):
         here = got[start : start + len(piece)]
         assert torch.equal(here, want[: len(here)]), start
+
+
+def test_more_rows_than_an_int_holds_are_refused():
+    w = Fp8Weights.from_tensor(torch.ones(8, 8, device="cuda"))
+    for rows in (2**31, 2**32 + 1):
+        with pytest.raises(RuntimeError, match="rows"):
+            fp8_linear(torch.zeros(1, 8, dtype=torch.bfloat16, device="cuda").expand(rows, 8), w)  # one row of memory: refused ahead of any copy

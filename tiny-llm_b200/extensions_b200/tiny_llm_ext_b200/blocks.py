@@ -1083,12 +1083,17 @@ def shift_mix(h, mu, *, seq_info, state, max_tokens: int):
     return out
 
 
+_MOST_ROWS = 2**31 - 256  # the C entries count rows in an int, and tiles of them up to a multiple of 256
+
+
 def _rows_of(op: str, x: torch.Tensor, width: int, device: int) -> torch.Tensor:
     """``x`` as a matrix of rows with unit inner stride on the weights' device."""
     if x.shape[-1] != width:
         raise RuntimeError(f"{op}: rows of {x.shape[-1]} for weights of {width} columns")
     if x.get_device() != device or device < 0:
         raise RuntimeError(f"{op}: the blocks extension is GPU-only, and rows and weights must be on one device")
+    if x.numel() > _MOST_ROWS * width:
+        raise RuntimeError(f"{op}: {x.numel() // width} rows, at most {_MOST_ROWS}")
     if x.dim() != 2:
         x = x.reshape(-1, width)
     return x if x.is_contiguous() or (x.stride(1) == 1 and x.stride(0) >= width) else x.contiguous()
