@@ -1110,10 +1110,23 @@ def _on_device(device: int, call):
         return call()
 
 
+def _fp8_matrix(op: str, values: torch.Tensor, scales: torch.Tensor, outputs: int, width: int) -> None:
+    if values.dtype != torch.float8_e4m3fn or values.dim() != 2 or values.shape[0] != outputs or values.shape[1] < width or values.stride(1) != 1:
+        raise RuntimeError(f"{op}: values must be float8_e4m3fn [{outputs}, >= {width}], entries of a row side by side")
+    if scales.dtype != torch.float32 or scales.shape != (-(-outputs // 128), -(-width // 128)) or not scales.is_contiguous() or scales.get_device() != values.get_device():
+        raise RuntimeError(f"{op}: scales must be contiguous float32, one for each block of 128 x 128, on the values' device")
+
+
 def fp8_linear(x: torch.Tensor, values: torch.Tensor, scales: torch.Tensor, width: int, bias=None) -> torch.Tensor:
     """``x [.., width]`` (bf16 or fp32; rows may be apart) times ``values [N, >= width]`` (e4m3, rows of a multiple of 16 bytes,
     zero behind ``width``) with ``scales [ceil(N / 128), ceil(width / 128)]`` fp32, plus ``bias [N]`` -> ``[.., N]`` in ``x``'s dtype.  The rows are
     rounded to e4m3 with a scale for each run of 128, see ``tlb_fp8_linear``."""
+    _fp8_matrix("fp8_linear", values, scales, values.shape[0], width)
+    return fp8_linear_of(x, values, scales, width, bias)
+
+
+def fp8_linear_of(x: torch.Tensor, values: torch.Tensor, scales: torch.Tensor, width: int, bias=None) -> torch.Tensor:
+    """``fp8_linear`` for a matrix that its holder has checked (``Fp8Weights``): of small calls the host sets the pace."""
     device = values.get_device()
     rows = _rows_of("fp8_linear", x, width, device)
     n, ld = values.shape[0], values.stride(0)
@@ -1139,6 +1152,13 @@ def fp8_gated_mlp(x: torch.Tensor, gate_up, down, width: int, inner: int, act: i
     """``down(act(gate x) * (up x))`` over e4m3 matrices, the inner rows rounded as ``x``'s are (from fp32) -> ``x``'s shape and dtype.  ``gate_up`` =
     (values ``[2 * 128 * ceil(inner / 128), ..]``, scales): runs of 128 rows of the gate and of the up projection in turn, zero behind
     ``inner``; ``down`` = (values ``[width, ..]``, scales).  ``limit`` and ``slope`` go with ``ACT_CLAMPED_SWISH``."""
+    _fp8_matrix("fp8_gated_mlp", *gate_up, 256 * -(-inner // 128), width)
+    _fp8_matrix("fp8_gated_mlp", *down, width, inner)
+    return fp8_gated_mlp_of(x, gate_up, down, width, inner, act, limit, slope)
+
+
+def fp8_gated_mlp_of(x: torch.Tensor, gate_up, down, width: int, inner: int, act: int, limit: float = 0.0, slope: float = 1.0) -> torch.Tensor:
+    """``fp8_gated_mlp`` for matrices that their holder has checked (``mlp.Fp8GatedMLP``)."""
     (wg, sg), (wd, sd) = gate_up, down
     device = wg.get_device()
     rows = _rows_of("fp8_gated_mlp", x, width, device)

@@ -76,7 +76,7 @@ def fp8_linear(x: torch.Tensor, w: Fp8Weights, bias: torch.Tensor | None = None)
     """``x [.., K]`` (bf16 or fp32) times the transposed matrix -> ``[.., N]`` in ``x``'s dtype, any number of rows from none up."""
     if len(w.shape) != 2:
         raise ValueError("fp8_linear: one matrix, not a stack")
-    return blocks.fp8_linear(x, w.values, w.scales, w.shape[1], bias)
+    return blocks.fp8_linear_of(x, w.values, w.scales, w.shape[1], bias)
 
 
 def interleaved(gate: Fp8Weights, up: Fp8Weights):

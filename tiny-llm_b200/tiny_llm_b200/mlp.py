@@ -83,7 +83,7 @@ class Fp8GatedMLP:
             raise ValueError("Fp8GatedMLP: the clamped activation needs a positive limit")
 
     def __call__(self, h: torch.Tensor) -> torch.Tensor:
-        return self._blocks.fp8_gated_mlp(h, self.gate_up, self.down, self.width, self.inner_width, self.act, self.limit, self.slope)
+        return self._blocks.fp8_gated_mlp_of(h, self.gate_up, self.down, self.width, self.inner_width, self.act, self.limit, self.slope)
 
 
 class TopKRouter:
