@@ -54,8 +54,16 @@ struct FewArgs {
     uint32_t *finished;  // [blocks of 128 output columns][32 tokens]: partial sums that are written
     float *inner;        // [tokens * top, ld_inner], zero behind ff
     float *part;         // [splits][tokens * top, dim]
-    int ld_inner, splits, room /* bytes of shared memory that a launch may use */;
+    int32_t *lost;       // [first_ctas]: whether a CTA of the first launch gave up a wait
+    int ld_inner, splits, first_ctas, room /* bytes of shared memory that a launch may use */;
 };
+
+#ifdef TLB_FEW_STARVED  // a test's build: for one CTA of the first launch the tokens never come in whole
+static __device__ int g_few_starved = -1;
+__device__ __forceinline__ bool few_starved() { return static_cast<int>(blockIdx.x) == g_few_starved; }
+#else
+__device__ __forceinline__ constexpr bool few_starved() { return false; }
+#endif
 
 // ---- small things ----------------------------------------------------------------------------------------------------
 
@@ -277,10 +285,11 @@ moe_few_first_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     // 16 of the router's rows are shared by all warps, or by eight where there are more than the cluster has at once
     const int parts = rows > 16 * static_cast<int>(ranks) ? 8 : 16, part = warp & (parts - 1), group = parts == 8 ? warp >> 3 : 0, groups = kFewWarps / parts;
     if (warp == 1 && g_elect_one()) {
-        g_mbar_expect_tx(bars.cols_full, pieces * NT * 1024);
+        g_mbar_expect_tx(bars.cols_full, pieces * NT * 1024 + (few_starved() ? 16 : 0));
         for (int i = 0; i < pieces; ++i) tl::g_tma_load_2d(g_smem_u32(few_smem + at.cols) + i * NT * 1024, &map_x, i * 128, 0, bars.cols_full);
     }
     __syncwarp();
+    if (tid == 0) a.lost[blockIdx.x] = 0;
     if (blockIdx.x == 0)
         for (int i = tid; i < (a.dim + 127) / 128 * kFewTokens; i += kFewThreads) a.finished[i] = 0;
     // ---- the router's rows, 16 for eight or all warps, which share the reduction
@@ -300,7 +309,7 @@ moe_few_first_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     };
     const int m_first = rank * groups + group;
     ask(m_first, part);
-    tc_wait(bars.cols_full, 0, bars.dead);
+    tc_wait(bars.cols_full, 0, bars.dead, few_starved() ? 1000 : 1u << 22);  // given up: see the end of this kernel
     const unsigned char *raw = few_smem + at.cols;
     auto entries = [&](int b, int t) {  // four of a token, of 128 that a warp has
         return *reinterpret_cast<const uint2 *>(raw + (b * 2 + (lane >> 4)) * NT * 1024 + few_swizzled(t, (lane & 15) * 8));
@@ -532,6 +541,9 @@ moe_few_first_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     __syncwarp();
     g_tc_fence_before();
     __syncthreads();
+    // A CTA without its tokens has given its cluster logits that are none, and the cluster took other experts than the rest of the grid: rows of `inner` that nobody
+    // writes, or two write.  No mark of the numbers themselves reaches these, so the second launch makes no output of a layer of which a wait was given up.
+    if (tid == 0 && *bars.dead) a.lost[blockIdx.x] = 1;
     if (warp == 2) {
         tc_settle(bars.dead);
         g_tc_fence_after();
@@ -633,12 +645,19 @@ moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) 
     }
     tl::griddep_wait();
     tl::griddep_launch();
-    if (tid < pairs) idx[tid] = tl::ld_cg(a.idx + tid), gate[tid] = tl::ld_cg(a.gate + tid);
+    const int mark = tid < a.first_ctas ? tl::ld_cg(a.lost + tid) : 0;  // asked for ahead of the choices: one behind the other cost a microsecond
+    if (tid < pairs) {
+        const int e = tl::ld_cg(a.idx + tid);
+        const float weight = tl::ld_cg(a.gate + tid);
+        idx[tid] = e, gate[tid] = weight;
+    }
     if (tid < kFewTokens) need[tid] = 0;
     g_tc_fence_before();
-    __syncthreads();
+    const bool lost = __syncthreads_or(mark);
     g_tc_fence_after();
     const uint32_t tmem = *bars.tmem;
+    if (lost)
+        for (int i = blockIdx.x * kFewThreads + tid; i < a.tokens * a.dim; i += gridDim.x * kFewThreads) static_cast<OUT *>(a.out)[i] = from_f<OUT>(__int_as_float(0x7fffffff));
     const bool live = few_lists(a, idx, lists);
     if (live) atomicAdd(&need[tid / a.top], a.splits);
     else if (tid < pairs && idx[tid] < a.experts) idx[tid] = -1;  // named twice
@@ -659,7 +678,7 @@ moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) 
         if (lane == 0) group[pairs] = n;
     }
     __syncthreads();
-    const int groups = group[pairs], outs = (a.dim + 127) / 128, of_group = outs * a.splits, items = groups * of_group, blocks = (a.ff + ENTRIES - 1) / ENTRIES;
+    const int groups = group[pairs], outs = (a.dim + 127) / 128, of_group = outs * a.splits, items = lost ? 0 : groups * of_group, blocks = (a.ff + ENTRIES - 1) / ENTRIES;
     const int scale_cols = (a.ff + 127) / 128, scale_rows = (a.dim + 127) / 128;
     struct Item {
         int pos, first, tokens, n, m, split, b0, b1;  // n: columns of the products; b0, b1: blocks of the reduction
@@ -868,7 +887,7 @@ moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) 
             if (++slot == 2) slot = 0, part_ph ^= 1u;
         }
         for (int j = blockIdx.x * 8 + warp - 8; j < a.tokens * outs; j += gridDim.x * 8)  // tokens without an expert's product
-            if (need[j / outs] == 0) few_output<OUT>(a, j / outs, j % outs * 128 + lane * 4, pairs, idx, gate);
+            if (!lost && need[j / outs] == 0) few_output<OUT>(a, j / outs, j % outs * 128 + lane * 4, pairs, idx, gate);
     }
     __syncwarp();
     g_tc_fence_before();
@@ -882,7 +901,7 @@ moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) 
 
 // ---- host ------------------------------------------------------------------------------------------------------------
 
-constexpr int kFewSmem = 227 * 1024, kFewMostGrid = 1024;
+constexpr int kFewSmem = 227 * 1024, kFewMostGrid = kFewThreads;  // the second launch reads a mark a thread
 
 // CTAs of the first launch: as many clusters as are resident at once, which a device's SMs in groups decide (132 CTAs of a B200).
 template <typename K>
@@ -936,19 +955,21 @@ static int few_splits(int tokens, int dim, int top, int ff, bool fp8) {
 static size_t few_align(size_t n) { return (n + 15) & ~(size_t)15; }
 static size_t few_bytes(int tokens, int dim, int top, int ff, bool fp8) {
     const size_t pairs = (size_t)tokens * top;
-    return few_align(pairs * 4) * 2 + few_align((size_t)tokens * 4) + few_align((size_t)ceil_div(dim, 128) * kFewTokens * 4) + pairs * few_inner_ld(ff) * 4 +
+    return few_align(pairs * 4) * 2 + few_align((size_t)tokens * 4) + few_align((size_t)ceil_div(dim, 128) * kFewTokens * 4) + kFewMostGrid * 4 + pairs * few_inner_ld(ff) * 4 +
            (size_t)few_splits(tokens, dim, top, ff, fp8) * pairs * dim * 4;
 }
 
-template <typename K, typename... A>
-static int few_launch(K kernel, tl::PerDevice &ready, int grid, int cluster, int smem, cudaStream_t st, const A &...args) {
+template <typename K>
+static int few_ready(K kernel, tl::PerDevice &ready) {
     int device = 0;
     cudaGetDevice(&device);
-    if (!ready(device, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem) == cudaSuccess; })) {
-        cudaGetLastError();
-        return tl::fail(TL_ECUDA, "moe_few: no shared memory");
-    }
-    if (grid == 0) grid = few_grid(kernel);
+    if (ready(device, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem) == cudaSuccess; })) return TL_OK;
+    cudaGetLastError();
+    return tl::fail(TL_ECUDA, "moe_few: no shared memory");
+}
+
+template <typename K, typename... A>
+static int few_launch(K kernel, int grid, int cluster, int smem, cudaStream_t st, const A &...args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid), cfg.blockDim = dim3(kFewThreads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -963,15 +984,20 @@ static int few_launch(K kernel, tl::PerDevice &ready, int grid, int cluster, int
 }
 
 template <bool FP8, int NT>
-static int few_run(const CUtensorMap &mx, const CUtensorMap &m0, const CUtensorMap &m1, const CUtensorMap &m2, const FewArgs &a, bool gated, bool wide, cudaStream_t st) {
+static int few_run(const CUtensorMap &mx, const CUtensorMap &m0, const CUtensorMap &m1, const CUtensorMap &m2, FewArgs a, bool gated, bool wide, cudaStream_t st) {
     static tl::PerDevice with, without, second16, second32;
-    const int smem = FewFirstSmem(a.tokens, NT, a.dim, a.outputs, a.experts, a.top, a.group_count, FP8, kFewSmem).total;
-    if (int e = gated ? few_launch(moe_few_first_kernel<FP8, true, NT>, with, 0, kFewCluster, smem, st, mx, m0, m1, a)
-                      : few_launch(moe_few_first_kernel<FP8, false, NT>, without, 0, kFewCluster, smem, st, mx, m0, m1, a))
-        return e;
-    const int smem2 = FewSecondSmem(a.tokens, a.experts, a.top, kFewSmem).total;
-    return wide ? few_launch(moe_few_second_kernel<FP8, float>, second32, sm_count(), 1, smem2, st, m2, a)
-                : few_launch(moe_few_second_kernel<FP8, bf16>, second16, sm_count(), 1, smem2, st, m2, a);
+    auto first = [&](auto kernel, tl::PerDevice &ready) {
+        if (int e = few_ready(kernel, ready)) return e;
+        a.first_ctas = few_grid(kernel);
+        const int smem = FewFirstSmem(a.tokens, NT, a.dim, a.outputs, a.experts, a.top, a.group_count, FP8, kFewSmem).total;
+        return few_launch(kernel, a.first_ctas, kFewCluster, smem, st, mx, m0, m1, a);
+    };
+    auto second = [&](auto kernel, tl::PerDevice &ready) {
+        if (int e = few_ready(kernel, ready)) return e;
+        return few_launch(kernel, sm_count(), 1, FewSecondSmem(a.tokens, a.experts, a.top, kFewSmem).total, st, m2, a);
+    };
+    if (int e = gated ? first(moe_few_first_kernel<FP8, true, NT>, with) : first(moe_few_first_kernel<FP8, false, NT>, without)) return e;
+    return wide ? second(moe_few_second_kernel<FP8, float>, second32) : second(moe_few_second_kernel<FP8, bf16>, second16);
 }
 
 long long few_gave_up() { return tl::read_gave_up(); }
@@ -1021,6 +1047,7 @@ int tlb_moe_few(const tlb_moe_few_layer *l, const void *x, int tokens, const voi
     a.gate = (float *)at, at += few_align(pairs * 4);
     a.side = (float *)at, at += few_align((size_t)tokens * 4);
     a.finished = (uint32_t *)at, at += few_align((size_t)ceil_div(dim, 128) * kFewTokens * 4);
+    a.lost = (int32_t *)at, at += kFewMostGrid * 4;
     a.inner = (float *)at, a.ld_inner = few_inner_ld(ff), at += pairs * a.ld_inner * 4;
     a.part = (float *)at, a.splits = few_splits(tokens, dim, top, ff, fp8 != 0), a.room = kFewSmem;
     // what lies between a row's last number and the next row is read as zeros
@@ -1044,5 +1071,10 @@ int tlb_moe_few(const tlb_moe_few_layer *l, const void *x, int tokens, const voi
         default: return few_run<true, 4>(mx, m0, m1, m2, a, gated, wide, st);
     }
 }
+
+#ifdef TLB_FEW_STARVED
+int tlb_few_starve(int cta) { return cudaMemcpyToSymbol(g_few_starved, &cta, sizeof(cta)) == cudaSuccess ? TL_OK : TL_ECUDA; }
+long long tlb_few_starved_waits(void) { return few_gave_up(); }
+#endif
 
 }  // extern "C"
