@@ -142,7 +142,7 @@ __device__ __forceinline__ void few_ld_wait() { asm volatile("tcgen05.wait::ld.s
 // The chosen experts in ascending order and the tokens that chose each, in ascending order: a token's place is its column.  Both launches make these for
 // themselves.
 struct FewLists {
-    uint32_t *words;   // [32]: a bit for every expert, zero at the start
+    uint32_t *words;   // [32]: a bit for every expert, and behind them whether a token names one again; zero at the start
     uint32_t *tokens;  // [most]: the tokens of an active expert, zero at the start
     int *active;       // [most]
     uint16_t *column;  // [most][32]: token * 256 + choice
@@ -152,7 +152,7 @@ struct FewListsSmem {  // from `at` on, a multiple of 4
     int words, tokens, active, count, column, end;
     __host__ __device__ FewListsSmem(int at, int tokens_, int top, int experts) {
         const int most = tokens_ * top < experts ? tokens_ * top : experts;
-        words = at, tokens = words + 128, active = tokens + most * 4, count = active + most * 4, column = count + 4, end = (column + most * 64 + 15) / 16 * 16;
+        words = at, tokens = words + 132, active = tokens + most * 4, count = active + most * 4, column = count + 4, end = (column + most * 64 + 15) / 16 * 16;
     }
     __device__ FewLists lists(unsigned char *smem) const {
         return {reinterpret_cast<uint32_t *>(smem + words), reinterpret_cast<uint32_t *>(smem + tokens), reinterpret_cast<int *>(smem + active),
@@ -162,16 +162,30 @@ struct FewListsSmem {  // from `at` on, a multiple of 4
         for (int i = threadIdx.x; i < (active - words) / 4; i += kFewThreads) reinterpret_cast<uint32_t *>(smem + words)[i] = 0;
     }
 };
-// All threads of the CTA, a pair each; behind a barrier after clear() and the last write of idx, which is in shared memory.  Whether the pair has an expert's product.
-__device__ __forceinline__ bool few_lists(const FewArgs &a, const int *idx, const FewLists &l) {
+// All threads of the CTA, a pair each; behind a barrier after clear() and the last write of idx and gate, which are in shared memory.  Whether the pair has an
+// expert's product.  A token that names an expert twice (scores of minus infinity are equal, and the first of them comes again) has it once, with the sum of its
+// weights: the first launch, with CHOICES, joins them, and the later ones become -1.
+template <bool CHOICES>
+__device__ __forceinline__ bool few_lists(const FewArgs &a, const FewLists &l, int *idx, float *gate) {
     static_assert(kFewPairs <= kFewThreads, "a pair a thread");
     const int p = threadIdx.x, lane = p & 31, t = p / a.top, k = p % a.top;
     int e = p < a.tokens * a.top ? idx[p] : a.experts;
-    for (int j = 1; j <= k && e < a.experts; ++j)  // a token that names an expert twice (equal logits of minus infinity) has it once, by its first choice
-        if (idx[p - j] == e) e = a.experts;
-    const bool live = e < a.experts;
+    bool again = false;
+    if constexpr (CHOICES) {
+        for (int j = 1; j <= k && e < a.experts; ++j)
+            if (idx[p - j] == e) e = a.experts, again = true;
+        if (again) l.words[32] = 1;
+    }
+    const bool live = static_cast<uint32_t>(e) < static_cast<uint32_t>(a.experts);
     if (live) atomicOr(&l.words[e >> 5], 1u << (e & 31));
     __syncthreads();
+    const bool join = CHOICES && l.words[32] && live;
+    float weight = 0.f;
+    if (join) {
+        weight = gate[p];
+        for (int j = 1; k + j < a.top; ++j)
+            if (idx[p + j] == e) weight += gate[p + j];
+    }
     const uint32_t word = l.words[lane];
     int before = __popc(word);
 #pragma unroll
@@ -185,6 +199,8 @@ __device__ __forceinline__ bool few_lists(const FewArgs &a, const int *idx, cons
     const int pos = first + __popc(__shfl_sync(0xffffffffu, word, at) & ((1u << (e & 31)) - 1));
     if (live) l.active[pos] = e, atomicOr(&l.tokens[pos], 1u << t);
     __syncthreads();
+    if (join) gate[p] = weight;  // read by all before the barrier
+    if (again) idx[p] = -1;
     if (live) l.column[pos * 32 + __popc(l.tokens[pos] & ((1u << t) - 1))] = (uint16_t)(t * 256 + k);
     __syncthreads();
     return live;
@@ -412,12 +428,10 @@ moe_few_first_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
                    gate + t * a.top);
     }
     __syncthreads();
-    if (blockIdx.x == 0) {
-        for (int p = tid; p < a.tokens * a.top; p += kFewThreads) a.idx[p] = idx[p], a.gate[p] = gate[p];
-        if (a.side_w && tid < a.tokens) a.side[tid] = sigmoid(side[tid]);
-    }
+    if (blockIdx.x == 0 && a.side_w && tid < a.tokens) a.side[tid] = sigmoid(side[tid]);
     tl::g_fence_proxy_async();  // the logits have been read, copies may come over them
-    few_lists(a, idx, lists);
+    few_lists<true>(a, lists, idx, gate);
+    if (blockIdx.x == 0 && tid < a.tokens * a.top) a.idx[tid] = idx[tid], a.gate[tid] = gate[tid];
 
     // ---- the first products: tiles of 64 features with their gates, or 128 without
     constexpr int FEATURES = GATED ? 64 : 128;
@@ -658,9 +672,7 @@ moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) 
     const uint32_t tmem = *bars.tmem;
     if (lost)
         for (int i = blockIdx.x * kFewThreads + tid; i < a.tokens * a.dim; i += gridDim.x * kFewThreads) static_cast<OUT *>(a.out)[i] = from_f<OUT>(__int_as_float(0x7fffffff));
-    const bool live = few_lists(a, idx, lists);
-    if (live) atomicAdd(&need[tid / a.top], a.splits);
-    else if (tid < pairs && idx[tid] < a.experts) idx[tid] = -1;  // named twice
+    if (few_lists<false>(a, lists, idx, gate)) atomicAdd(&need[tid / a.top], a.splits);
     const int count = *lists.count;
     if (warp == 0) {  // the experts' groups of up to GROUP tokens, in order
         int n = 0;
