@@ -359,9 +359,9 @@ int tlb_argmax_rows(const float *logits, int32_t *out, int rows, int vocab, void
  *   y[t] = sum over choices  weight * down_e(act(gate_e x) * (up_e x))   (+ sigmoid(side_w . x) * shared[t], shared bf16 [tokens, dim] or NULL)
  * rounded to bf16, or fp32 (out_f32).  Experts w_gate, w_up [experts, ff, ld_in bytes], w_down [experts, dim, ld_out bytes], bf16 (fp8 = 0) or e4m3 with scales
  * [experts, ceil(rows / 128), ceil(columns / 128)]; rows are whole 16-byte pieces, zero behind the last number; w_gate NULL: act(up_e x), act 2 allowed.
- * Ids from `experts` up to `outputs` are identity experts.  dim must be a multiple of 8.  Products are exact, their sums fp32.  Inner rows are kept to 2^-16 of a
- * number (bf16 experts), or to 2^-12, or 2^-25 of the largest of its block of 128 (8-bit experts); of x, 8-bit experts use what lies above 2^-21 of a token's
- * largest magnitude.  Of a token with a NaN no output is a number; an infinity makes it NaN for all 8-bit experts, and gives over bf16 ones what the formula gives.
+ * Ids from `experts` up to `outputs` are identity experts.  dim must be a multiple of 8.  Products are exact, their sums fp32.  Inner rows are fp32 numbers,
+ * of which the second product uses all bits over bf16 experts; over 8-bit ones all but 2^-24 of a number or 2^-37 of the largest of its block of 128 (out_f32), or but 2^-12 or
+ * 2^-25 (bf16 outputs).  Of x, 8-bit experts use what lies above 2^-21 of a token's largest magnitude.  Of a token with a NaN no output is a number; an infinity makes it NaN for all 8-bit experts, and gives over bf16 ones what the formula gives.
  * tlb_moe_few_tokens: the most tokens a call takes at these sizes (0: none; up to 32, 16 at dim 4096, 8 up to 11264).  A token's result does not depend on the other
  * tokens, nor its bits, but for their number: it decides in how many parts the second product is added up.  The workspace need not be initialised; calls that may run
  * at once need one each. */

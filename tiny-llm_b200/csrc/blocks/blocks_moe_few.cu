@@ -8,15 +8,15 @@
 // TMA in boxes of 128 bytes a row, and the tokens as 16 to 64 columns: a matrix costs no thread more than its copies and the sums' additions (mma.sync on
 // fragments that threads unpack took 380 instructions for 2 KB).  What the columns hold:
 //
-//   bf16 experts:  x as it is; an inner row as two bf16 terms (off by 2^-16 of a number)
+//   bf16 experts:  x as it is; an inner row as three bf16 terms
 //   e4m3 experts:  both operands of a product have 8 bits, so a number is several e4m3 terms, a column each, added when the sums are taken out: x, whose 8 bits
-//                  two terms of 4 hold exactly (times a power of two for each token; bits below 2^-21 of the token's largest magnitude are lost), an inner row
-//                  three (off by 2^-12, or by 2^-25 of the largest of its block of 128: a power of two for each block).  A block of 128 is added in the
+//                  two terms of 4 hold exactly (times a power of two for each token; of bits below 2^-21 of the token's largest magnitude, which its sums of fp32 hardly
+//                  hold beside it, the second term has none), an inner row three or six (times a power of two for each block of 128; few_terms).  A block of 128 is added in the
 //                  tensor cores, then times its scales in fp32.
 //
 // First launch: the CTAs of a cluster share the router's rows and exchange the logits through shared memory, and every CTA makes the same choices and the columns
 // for itself, in the place the tokens were copied to.  A tile is 64 features of an expert, gate rows and up rows in one accumulator.  Second launch: an item is 128 output
-// columns of an expert for up to 10 (bf16: 16) of its tokens, over a part of the reduction; its partial sums go to memory, and whoever writes a token's last one adds
+// columns of an expert for up to five of its tokens, over a part of the reduction; its partial sums go to memory, and whoever writes a token's last one adds
 // them all, in order (a counter tells; no CTA waits for another outside its cluster).
 //
 // 64 experts of 1408 x 2048, 6 a token: 1 token 29 us in e4m3 and 37 in bf16, of which some 8 and 16 are the weights' and the rest one latency behind another (tokens and
@@ -569,6 +569,14 @@ moe_few_first_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
 
 constexpr int kFewSecondN = 32;  // the most columns of an item: terms times tokens
 
+// Terms of an inner number, and the tokens of an item.  Three terms of bf16 hold all bits of an fp32 number, and so do six of e4m3, four bits each (off by 2^-24, or by 2^-37
+// of the largest of its block of 128).  Over 8 bits an output that is rounded to bf16, off by 2^-8, hides what three leave out of the numbers it adds up (2^-12, 2^-25) and has
+// these: 1 token 28.7 us for 29.7, 32 tokens 135 for 143.  Five tokens of three terms are 16 columns, which fit beside the ring for a whole reduction and are half as
+// many to take out as 32: with ten tokens an item, 16 tokens over 16 bits took 168 us for 155, 32 took 220 for 199; the few experts with more tokens come out of L2 again.
+__host__ __device__ constexpr int few_terms(bool fp8, bool wide) { return fp8 && wide ? 6 : 3; }
+constexpr int kFewGroup = 5;
+static_assert(kFewGroup * few_terms(true, true) <= kFewSecondN && (kFewTokens + kFewGroup - 1) / kFewGroup <= 8, "an item's columns; groups of an expert, in three bits");
+
 struct FewSecondSmem {
     int cols, factors, sums, idx, gate, need, group, bars, ring, stages, total;
     static constexpr int kCols = kFewItemCols + 4096, kFactors = kFewItemBlocks * kFewSecondN * 4;  // of either place of an item's columns
@@ -635,12 +643,12 @@ template <bool FP8, typename OUT>
 __global__ void __launch_bounds__(kFewThreads, 1)
 moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) {
     extern __shared__ __align__(1024) unsigned char few_smem[];
-    constexpr int TERMS = FP8 ? 3 : 2, GROUP = kFewSecondN / TERMS, BUFFERS = FP8 ? kFewBuffers : 2, TMEM = kFewSecondN * BUFFERS, ENTRIES = FP8 ? 128 : 64;
+    constexpr int TERMS = few_terms(FP8, sizeof(OUT) == 4), GROUP = kFewGroup, BUFFERS = FP8 ? kFewBuffers : 2, TMEM = kFewSecondN * BUFFERS, ENTRIES = FP8 ? 128 : 64;
     const FewSecondSmem at(a.tokens, a.experts, a.top, a.room);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, pairs = a.tokens * a.top;
     float *sums = reinterpret_cast<float *>(few_smem + at.sums), *gate = reinterpret_cast<float *>(few_smem + at.gate), *factors = reinterpret_cast<float *>(few_smem + at.factors);
     int *need = reinterpret_cast<int *>(few_smem + at.need);  // [tokens]: the partial sums of an output
-    int *idx = reinterpret_cast<int *>(few_smem + at.idx), *group = reinterpret_cast<int *>(few_smem + at.group);  // group: [groups] position * 4 + number
+    int *idx = reinterpret_cast<int *>(few_smem + at.idx), *group = reinterpret_cast<int *>(few_smem + at.group);  // group: [groups] position * 8 + number
     const FewLists lists = at.lists.lists(few_smem);
     const FewBars bars(few_smem, at.bars);
     at.lists.clear(few_smem);
@@ -684,7 +692,7 @@ moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) 
                 const int v = __shfl_up_sync(0xffffffffu, before, o);
                 if (lane >= o) before += v;
             }
-            for (int j = 0; j < mine; ++j) group[n + before - mine + j] = (p0 + lane) * 4 + j;
+            for (int j = 0; j < mine; ++j) group[n + before - mine + j] = (p0 + lane) * 8 + j;
             n += __shfl_sync(0xffffffffu, before, 31);
         }
         if (lane == 0) group[pairs] = n;
@@ -698,7 +706,7 @@ moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) 
     auto item_of = [&](int i) {
         Item it;
         const int entry = group[i / of_group], r = i % of_group;
-        it.pos = entry >> 2, it.first = (entry & 3) * GROUP, it.tokens = min(GROUP, __popc(lists.tokens[it.pos]) - it.first), it.n = (it.tokens * TERMS + 15) & ~15;
+        it.pos = entry >> 3, it.first = (entry & 7) * GROUP, it.tokens = min(GROUP, __popc(lists.tokens[it.pos]) - it.first), it.n = (it.tokens * TERMS + 15) & ~15;
         it.m = r / a.splits, it.split = r % a.splits;
         it.b0 = blocks * it.split / a.splits, it.b1 = blocks * (it.split + 1) / a.splits;
         return it;
@@ -792,16 +800,18 @@ moe_few_second_kernel(const __grid_constant__ CUtensorMap map, const FewArgs a) 
                     } else {
                         const int b = r * 2 + (lane >> 4);
                         if (b < here) {
-                            uint32_t hi[2], lo[2];
 #pragma unroll
-                            for (int q = 0; q < 2; ++q) {
-                                hi[q] = tl::pack2<bf16>(v[u][2 * q], v[u][2 * q + 1]);
-                                const float2 f = tl::unpack2<bf16>(hi[q]);
-                                // an infinity has no second term
-                                lo[q] = tl::pack2<bf16>(fabsf(f.x) < INFINITY ? v[u][2 * q] - f.x : 0.f, fabsf(f.y) < INFINITY ? v[u][2 * q + 1] - f.y : 0.f);
+                            for (int term = 0; term < TERMS; ++term) {
+                                uint32_t w[2];
+#pragma unroll
+                                for (int q = 0; q < 2; ++q) {
+                                    w[q] = tl::pack2<bf16>(v[u][2 * q], v[u][2 * q + 1]);
+                                    const float2 f = tl::unpack2<bf16>(w[q]);
+                                    // an infinity has no further terms
+                                    v[u][2 * q] = fabsf(f.x) < INFINITY ? v[u][2 * q] - f.x : 0.f, v[u][2 * q + 1] = fabsf(f.y) < INFINITY ? v[u][2 * q + 1] - f.y : 0.f;
+                                }
+                                *reinterpret_cast<uint2 *>(cols + b * cols_block + few_swizzled(term * it.tokens + c, (lane & 15) * 8)) = make_uint2(w[0], w[1]);
                             }
-                            *reinterpret_cast<uint2 *>(cols + b * cols_block + few_swizzled(c, (lane & 15) * 8)) = make_uint2(hi[0], hi[1]);
-                            *reinterpret_cast<uint2 *>(cols + b * cols_block + few_swizzled(it.tokens + c, (lane & 15) * 8)) = make_uint2(lo[0], lo[1]);
                         }
                     }
                 }
@@ -952,9 +962,9 @@ static int few_blocks(int ff, bool fp8) { return ceil_div(ff, fp8 ? 128 : 64); }
 // Parts of the second product's reduction: as many as an item's columns need, or more where they let the SMs end closer together, by the blocks that the busiest
 // takes (and six more an item for what it costs besides), if no two tokens choose the same expert.  The number of experts does not matter: it changes no bits.
 // 1 token, 6 of 64 experts of 1408 x 2048: in one part 29.0 us (bf16 37.2), in three 30.7 (38.6).
-static int few_splits(int tokens, int dim, int top, int ff, bool fp8) {
+static int few_splits(int tokens, int dim, int top, int ff, bool fp8, bool wide) {
     const int blocks = few_blocks(ff, fp8), outs = ceil_div(dim, 128);
-    const int terms = fp8 ? 3 : 2, cols_block = ceil_div(std::min(tokens, kFewSecondN / terms) * terms, 8) * 1024, fewest = ceil_div(blocks, kFewItemCols / cols_block);
+    const int cols_block = ceil_div(std::min(tokens, kFewGroup) * few_terms(fp8, wide), 8) * 1024, fewest = ceil_div(blocks, kFewItemCols / cols_block);
     int best = fewest;
     long long least = 0;
     for (int s = fewest; s <= std::max(fewest, std::min(blocks, 8)); ++s) {
@@ -968,7 +978,7 @@ static size_t few_align(size_t n) { return (n + 15) & ~(size_t)15; }
 static size_t few_bytes(int tokens, int dim, int top, int ff, bool fp8) {
     const size_t pairs = (size_t)tokens * top;
     return few_align(pairs * 4) * 2 + few_align((size_t)tokens * 4) + few_align((size_t)ceil_div(dim, 128) * kFewTokens * 4) + kFewMostGrid * 4 + pairs * few_inner_ld(ff) * 4 +
-           (size_t)few_splits(tokens, dim, top, ff, fp8) * pairs * dim * 4;
+           (size_t)std::max(few_splits(tokens, dim, top, ff, fp8, false), few_splits(tokens, dim, top, ff, fp8, true)) * pairs * dim * 4;
 }
 
 template <typename K>
@@ -1061,7 +1071,7 @@ int tlb_moe_few(const tlb_moe_few_layer *l, const void *x, int tokens, const voi
     a.finished = (uint32_t *)at, at += few_align((size_t)ceil_div(dim, 128) * kFewTokens * 4);
     a.lost = (int32_t *)at, at += kFewMostGrid * 4;
     a.inner = (float *)at, a.ld_inner = few_inner_ld(ff), at += pairs * a.ld_inner * 4;
-    a.part = (float *)at, a.splits = few_splits(tokens, dim, top, ff, fp8 != 0), a.room = kFewSmem;
+    a.part = (float *)at, a.splits = few_splits(tokens, dim, top, ff, fp8 != 0, out_f32 != 0), a.room = kFewSmem;
     // what lies between a row's last number and the next row is read as zeros
     const uint64_t in = (uint64_t)dim * size, inner = (uint64_t)ff * size;
     CUtensorMap mx, m0, m1, m2;

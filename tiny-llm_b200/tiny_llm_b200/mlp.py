@@ -139,7 +139,7 @@ class MixtureOfExperts:
 
     def use_few_tokens(self) -> "MixtureOfExperts":
         """Steps of at most as many tokens as one call of ``FewTokenExperts`` takes go to it from now on (bf16 experts whose weight is on their output; the
-        same definition, sums in another order and inner rows of more bits than bf16)."""
+        same definition, sums in another order and inner rows of fp32 in place of bf16)."""
         if self.scale_input:
             raise ValueError("mixture of experts: the few-token layer takes the router's weight on the experts' output")
         act = next(name for name, code in ACTIVATIONS.items() if code == self.act)
@@ -184,8 +184,8 @@ class FewTokenExperts:
     """A whole mixture-of-experts layer for the few tokens of a decoding step in two launches: router and first products, second products
     and their sum.  Arguments as ``MixtureOfExperts`` takes them, the experts bf16 ``[E, ff, D]`` / ``[E, D, ff]`` or ``Fp8Weights`` of those shapes; the
     router's weight is on the experts' output.  A step of more tokens than one call takes (``run``: 32, at width 4096 16, 8 up to 11264, wider ones are refused) is
-    several calls, each of which reads its experts anew: prompts are better served by ``MixtureOfExperts``.  Inner rows keep 2^-16 of a number over bf16 experts and 2^-12 over
-    8-bit ones, which use of a token what lies above 2^-21 of its largest magnitude."""
+    several calls, each of which reads its experts anew: prompts are better served by ``MixtureOfExperts``.  Inner rows are fp32;
+    8-bit experts use all but 2^-12 of a number of theirs where the output is bf16 (``wide``: 2^-24), and of a token what lies above 2^-21 of its largest magnitude."""
 
     def __init__(self, router: TopKRouter, w_gate, w_up, w_down, act: str, shared: GatedMLP | None = None, identity: int = 0, limit: float = 0.0, slope: float = 1.0,
                  shared_gate: torch.Tensor | None = None):
