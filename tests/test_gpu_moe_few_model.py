@@ -59,6 +59,15 @@ def test_two_launches_a_layer(D):
     assert counts[1] == 2 < counts[0]
 
 
+def test_steps_of_more_tokens_keep_to_the_chain():
+    most = MixtureOfExperts.FEW_TOKENS
+    h, router, wg, wu, wd = make(most + 1, 64, 64, 8, False)
+    chain = MixtureOfExperts(TopKRouter(router, None, 2), wg, wu, wd, "silu")
+    few = MixtureOfExperts(chain.router, wg, wu, wd, "silu").use_few_tokens()
+    assert torch.equal(few(h), chain(h))
+    assert torch.equal(few(h[:most]), few.few(h[:most], wide=True)) and not torch.equal(few(h[:most]), chain(h[:most]))
+
+
 @pytest.mark.parametrize("eight", [False, True])
 @pytest.mark.parametrize("T", [1, 5, 40])
 def test_outputs_of_odd_widths_are_whole(T, eight):

@@ -113,6 +113,11 @@ class TopKRouter:
 
 
 class MixtureOfExperts:
+    # With use_few_tokens(), the most tokens of a step that goes to the two launches.  They / the chain of launches, us in a replayed graph, bf16: 64 experts of 1408 x 2048, 6 a token,
+    # 1 token 38 / 45, 4 79 / 85, 8 113 / 116, 12 140 / 145, 16 158 / 156, 32 197 / 186; with a shared expert 12 154 / 157, 16 172 / 169; 16 experts of 2048 x 4096, 2 a token,
+    # 8 106 / 126, 12 133 / 133, 16 144 / 136.  (2 tokens of the first 55 / 54, with the shared expert 75 / 71; called eagerly 56 / 62 and 83 / 88.)
+    FEW_TOKENS = 12
+
     def __init__(self, router: TopKRouter, w_gate: torch.Tensor | None, w_up: torch.Tensor, w_down: torch.Tensor, act: str,
                  shared: GatedMLP | None = None, weight_on: str = "output", identity: int = 0, limit: float = 0.0, slope: float = 1.0,
                  shared_gate: torch.Tensor | None = None):
@@ -138,8 +143,9 @@ class MixtureOfExperts:
         self.few = None
 
     def use_few_tokens(self) -> "MixtureOfExperts":
-        """Steps of at most as many tokens as one call of ``FewTokenExperts`` takes go to it from now on (bf16 experts whose weight is on their output; the
-        same definition, sums in another order and inner rows of fp32 in place of bf16)."""
+        """Steps of up to ``FEW_TOKENS`` tokens, or as many as one call of ``FewTokenExperts`` takes if that is less, go to it from now on (bf16 experts whose weight is on
+        their output; the same definition, sums in another order and inner rows of fp32 in place of bf16).  Calls with ``into`` do not: their end is fused with the
+        sublayer's."""
         if self.scale_input:
             raise ValueError("mixture of experts: the few-token layer takes the router's weight on the experts' output")
         act = next(name for name, code in ACTIVATIONS.items() if code == self.act)
@@ -151,7 +157,7 @@ class MixtureOfExperts:
         ``beside``: a model whose second stream runs the shared expert while this one routes (``RaggedDecoderModel._beside``)."""
         from extensions_b200.tiny_llm_ext_b200 import blocks
 
-        if self.few is not None and into is None and h.shape[0] <= self.few.run:
+        if self.few is not None and into is None and h.shape[0] <= min(self.few.run, self.FEW_TOKENS):
             return self.few(h, wide=True)
         shared = side = None
         if beside is not None and self.shared is not None:

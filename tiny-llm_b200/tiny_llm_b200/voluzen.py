@@ -50,8 +50,8 @@ class VoluzenModel(RaggedDecoderModel):
 
     def __init__(self, config: dict, tensors: dict, dtype=torch.bfloat16, device="cuda", page_size: int = 64, max_tokens: int | None = None,
                  max_requests: int | None = None, few_token_experts: bool = False):
-        """``max_requests``: accepted for all designs; no per-request state here.  ``few_token_experts`` (bf16): steps of up to 32 tokens (fewer above
-        width 2048) run their experts' layers in two launches (``mlp.FewTokenExperts``)."""
+        """``max_requests``: accepted for all designs; no per-request state here.  ``few_token_experts`` (bf16): steps of up to 12 tokens run
+        their experts' layers in two launches (``MixtureOfExperts.use_few_tokens``)."""
         if few_token_experts and dtype != torch.bfloat16:
             raise ValueError("few_token_experts: bfloat16 only")
         if dtype not in (torch.bfloat16, torch.float32):
