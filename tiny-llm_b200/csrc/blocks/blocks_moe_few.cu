@@ -34,6 +34,7 @@ namespace tlb {
 
 constexpr int kFewThreads = 512, kFewWarps = 16;
 constexpr int kFewTokens = 32, kFewPairs = 512, kFewOutputs = 1024;
+constexpr int kFewWidth = 1 << 16;     // far wider than what fits: bytes of wider rows would not be ints
 constexpr int kFewStage = 128 * 128;  // a stage of the ring: 128 matrix rows of 128 bytes
 constexpr int kFewMostStages = 8;
 constexpr int kFewItemCols = 48 * 1024, kFewItemBlocks = kFewItemCols / 1024;  // second launch: bytes of an item's columns, the most blocks of its reduction
@@ -1041,7 +1042,9 @@ using namespace tlb;
 extern "C" {
 
 int tlb_moe_few_tokens(int dim, int outputs, int experts, int top, int group_count, int fp8) {
-    if (dim <= 0 || outputs <= 0 || outputs > kFewOutputs || experts <= 0 || experts > outputs || top <= 0 || top > outputs || top > 255 || group_count < 0) return 0;
+    if (dim <= 0 || dim > kFewWidth || outputs <= 0 || outputs > kFewOutputs || experts <= 0 || experts > outputs || top <= 0 || top > outputs || top > 255 || group_count < 0 ||
+        group_count > outputs)
+        return 0;
     int tokens = std::min(kFewTokens, kFewPairs / top);
     while (tokens > 0 && !few_fits(tokens, few_nt(tokens), dim, outputs, experts, top, group_count, fp8 != 0)) --tokens;
     return tokens;
