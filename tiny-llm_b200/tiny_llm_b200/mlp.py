@@ -145,7 +145,7 @@ class MixtureOfExperts:
     def use_few_tokens(self) -> "MixtureOfExperts":
         """Steps of up to ``FEW_TOKENS`` tokens, or as many as one call of ``FewTokenExperts`` takes if that is less, go to it from now on (bf16 experts whose weight is on
         their output; the same definition, sums in another order and inner rows of fp32 in place of bf16).  Calls with ``into`` do not: their end is fused with the
-        sublayer's."""
+        sublayer's.  Experts of odd widths are held twice from then on (``FewTokenExperts``)."""
         if self.scale_input:
             raise ValueError("mixture of experts: the few-token layer takes the router's weight on the experts' output")
         act = next(name for name, code in ACTIVATIONS.items() if code == self.act)
@@ -189,8 +189,10 @@ def _whole_rows(w: torch.Tensor, rows: int) -> torch.Tensor:
 class FewTokenExperts:
     """A whole mixture-of-experts layer for the few tokens of a decoding step in two launches: router and first products, second products
     and their sum.  Arguments as ``MixtureOfExperts`` takes them, the experts bf16 ``[E, ff, D]`` / ``[E, D, ff]`` or ``Fp8Weights`` of those shapes; the
-    router's weight is on the experts' output.  A step of more tokens than one call takes (``run``: 32, at width 4096 16, 8 up to 11264, wider ones are refused) is
-    several calls, each of which reads its experts anew: prompts are better served by ``MixtureOfExperts``.  Inner rows are fp32;
+    router's weight is on the experts' output.  A step of more tokens than one call takes (``run``, see ``blocks.moe_few_tokens``: at most 32, fewer of wide rows, over
+    bf16 experts, with many router outputs or choices; sizes that take none are refused) is several calls, each of which reads its experts anew: prompts are better served
+    by ``MixtureOfExperts``.  Matrices whose rows are no whole 16-byte pieces (or, of ``w_down``, whose number of rows is no multiple of 8) are copied into such rows when the layer is made: a
+    second copy of the experts, which later writes to the first do not reach.  Inner rows are fp32;
     8-bit experts use all but 2^-12 of a number of theirs where the output is bf16 (``wide``: 2^-24), and of a token what lies above 2^-21 of its largest magnitude."""
 
     def __init__(self, router: TopKRouter, w_gate, w_up, w_down, act: str, shared: GatedMLP | None = None, identity: int = 0, limit: float = 0.0, slope: float = 1.0,
