@@ -361,7 +361,8 @@ int tlb_argmax_rows(const float *logits, int32_t *out, int rows, int vocab, void
  * [experts, ceil(rows / 128), ceil(columns / 128)]; rows are whole 16-byte pieces, zero behind the last number; w_gate NULL: act(up_e x), act 2 allowed.
  * Ids from `experts` up to `outputs` are identity experts.  dim must be a multiple of 8.  Products are exact, their sums fp32.  Inner rows are fp32 numbers,
  * of which the second product uses all bits over bf16 experts; over 8-bit ones all but 2^-24 of a number or 2^-37 of the largest of its block of 128 (out_f32), or but 2^-12 or
- * 2^-25 (bf16 outputs).  Of x, 8-bit experts use what lies above 2^-21 of a token's largest magnitude.  Of a token with a NaN no output is a number; an infinity makes it NaN for all 8-bit experts, and gives over bf16 ones what the formula gives.
+ * 2^-25 (bf16 outputs).  Of x, 8-bit experts use what lies above 2^-21 of a token's largest magnitude (a largest magnitude
+ * below 2^-100 counts as that, here and in a block).  Of a token with a NaN no output is a number; an infinity makes it NaN for all 8-bit experts, and gives over bf16 ones what the formula gives.
  * tlb_moe_few_tokens: the most tokens a call takes at these sizes (0: none).  32 up to dim 2048 (8-bit experts 2560) with 64 outputs and 6 choices, 16 at 4096, 8 at 8192, none from
  * 12296 on; more outputs or choices lower it (2048 with 256 outputs and 8 choices: 24; with 1024: 15, or 16 of 8-bit experts), and tokens * choices is 512 at most.
  * After a wait that gives up no output is a number where the first launch's was it, and none of the tokens concerned where the second's was.  A token's result does not depend on the other
