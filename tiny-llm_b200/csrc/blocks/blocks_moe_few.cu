@@ -604,16 +604,7 @@ struct FewSecondSmem {
 template <typename OUT>
 __device__ __forceinline__ void few_output(const FewArgs &a, int t, int d, int pairs, const int *idx, const float *gate) {
     if (d >= a.dim) return;
-    const bool identity = a.experts < a.outputs;
-    float y[4] = {0.f, 0.f, 0.f, 0.f}, x[4], shared[4], side = 1.f;  // the token's own and its shared expert's are on their way with the first of the choices'
-    if (identity)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) x[c] = to_f(tl::ld_cg(a.x + (size_t)t * a.dim + d + c));
-    if (a.shared) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) shared[c] = to_f(tl::ld_cg(a.shared + (size_t)t * a.dim + d + c));
-        if (a.side_w) side = tl::ld_cg(a.side + t);
-    }
+    float y[4] = {0.f, 0.f, 0.f, 0.f};
     constexpr int AT_ONCE = 4;
     for (int k0 = t * a.top; k0 < (t + 1) * a.top; k0 += AT_ONCE) {
         float4 z[AT_ONCE];
@@ -636,14 +627,23 @@ __device__ __forceinline__ void few_output(const FewArgs &a, int t, int d, int p
             y[0] = fmaf(g, z[u].x, y[0]), y[1] = fmaf(g, z[u].y, y[1]), y[2] = fmaf(g, z[u].z, y[2]), y[3] = fmaf(g, z[u].w, y[3]);
         }
     }
-    if (identity)
+    if (a.experts < a.outputs) {
+        float x[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[c] = to_f(tl::ld_cg(a.x + (size_t)t * a.dim + d + c));
         for (int k = t * a.top; k < (t + 1) * a.top; ++k)
             if (idx[k] >= a.experts && idx[k] < a.outputs)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) y[c] = fmaf(gate[k], x[c], y[c]);
-    if (a.shared)
+    }
+    if (a.shared) {  // all four on their way before the first is used
+        float shared[4], side = 1.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) shared[c] = to_f(tl::ld_cg(a.shared + (size_t)t * a.dim + d + c));
+        if (a.side_w) side = tl::ld_cg(a.side + t);
 #pragma unroll
         for (int c = 0; c < 4; ++c) y[c] = fmaf(side, shared[c], y[c]);
+    }
     for (int k = t * a.top; k < (t + 1) * a.top; ++k)  // a choice that is no output at all: the token's logits are no numbers
         if (idx[k] >= a.outputs) y[0] = y[1] = y[2] = y[3] = __int_as_float(0x7fffffff);
 #pragma unroll
