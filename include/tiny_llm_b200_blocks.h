@@ -396,6 +396,31 @@ size_t tlb_fp8_gated_mlp_workspace(int rows, int dim, int ff);
 int tlb_fp8_gated_mlp(const void *x, long long ldx, const void *w_gate_up, int ld_gate_up, const float *s_gate_up, const void *w_down, int ld_down, const float *s_down,
                       void *out, int rows, int dim, int ff, int act, float limit, float slope, void *workspace, size_t workspace_bytes, int dtype, void *stream);
 
+/* A paged key/value cache of 8 bits.  keys, values: e4m3 numbers [num_pages, heads, page_size, dim], 16-byte aligned; key_scales, value_scales: fp32
+ * [num_pages, heads, page_size / 16], one for each block of 16 tokens of a head; a number stands for itself times its block's scale.  dim: a multiple of 16 up to
+ * 256; page_size: a multiple of 16.  A scale is a power of two, 2^-100 at the least, or NaN: then every number of the block is none. */
+typedef struct {
+    uint8_t *keys, *values;
+    float *key_scales, *value_scales;
+    int num_pages, heads, page_size, dim;
+} tlb_fp8_pages;
+/* A step's `tokens` new tokens of each request (q [batch, heads, tokens, dim], k and v [batch, pages->heads, tokens, dim], any strides with unit inner one, given in
+ * entries) at positions lens[b] - tokens .. lens[b] - 1 (lens: after the step; 0: idle, nothing is appended and the queries come out as zeros).  Queries and
+ * keys pass an RMS norm per head (weights `dtype` [dim], NULL: none) and the rotation of their first `rot` entries by position * base^(-2i / rot), pairs
+ * (i, i + rot/2) or (2i, 2i + 1) (interleaved): in 64 bits for the keys and for all angles, in 32 for the queries.  q_out [batch, tokens, heads, dim], which must
+ * not overlap q.  Of a block with m the largest magnitude of its new rows, the scale is the larger of 2^e (the smallest e with m <= 448 * 2^e) and, if the block holds
+ * earlier tokens, the scale before; new rows are rounded to e4m3(x / scale), numbers of earlier tokens to e4m3(number * scale before / scale).  A NaN or infinity
+ * among the new rows makes the scale NaN.  Slots behind the last token stay as they are.  Table entries outside [0, num_pages): nothing is stored there. */
+int tlb_fp8_append(const tlb_fp8_pages *pages, const void *q, long long q_b, long long q_h, long long q_l, void *q_out, const void *k, long long k_b, long long k_h,
+                   long long k_l, const void *v, long long v_b, long long v_h, long long v_l, int batch, int heads, int tokens, const int32_t *table, int max_pages,
+                   const int32_t *lens, const void *q_norm, float q_eps, const void *k_norm, float k_eps, int rot, double base, int interleaved, int dtype, void *stream);
+/* out [batch, tokens, heads, dim] = softmax(q k^T * scale) v over the first lens[b] slots of each request (the `tokens` newest among them); causal: new token i sees
+ * lens[b] - tokens + i + 1 of them.  Rows that see nothing come out as zeros.  Products with the cache's numbers are exact, their sums, the softmax and the scales fp32;
+ * weights are rounded to f16 (relative to the largest so far) for bf16 outputs, and use 22 bits for fp32 ones, whose queries do so too.  longest: the largest of lens as far as the host knows;
+ * it decides how the work is cut and never the result but for the order of sums. */
+int tlb_fp8_attention(const tlb_fp8_pages *pages, const void *q, long long q_b, long long q_h, long long q_l, void *out, int batch, int heads, int tokens,
+                      const int32_t *table, int max_pages, const int32_t *lens, int longest, double scale, int causal, int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -62,6 +62,8 @@ BLOCKS_SOURCES = [
     "blocks/blocks_fp8_rows.cu",
     "blocks/blocks_fp8_product.cu",
     "blocks/blocks_fp8_pairs.cu",
+    "blocks/blocks_fp8_append.cu",
+    "blocks/blocks_fp8_attention.cu",
 ]
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")

@@ -1,0 +1,133 @@
+"""A paged key/value cache of 8 bits: e4m3 numbers with one scale, a power of two, for each 16 tokens of a head.
+
+``Fp8KvPages`` is the storage (the page layout of ``TinyKvPagedPool``, one byte a number), ``rotate_append_fp8`` puts a step's keys and values
+into it, with the norm and the rotation that queries and keys pass on the way, and ``paged_attention_fp8`` is ``paged_attention`` over it.  The block
+table and the context lengths are those of the 16-bit cache: a request's tokens fill its pages in order, ``context_lens`` count the step's own
+tokens, 0 marks an idle slot."""
+
+from __future__ import annotations
+
+import numpy as np
+import torch
+
+from extensions_b200.tiny_llm_ext_b200 import blocks
+
+from .attention import validate_paged_metadata
+
+TOKENS = 16  # that share a scale
+_DTYPES = (torch.float32, torch.bfloat16)
+
+
+class Fp8KvPages:
+    """``keys`` and ``values`` (``torch.float8_e4m3fn``) ``[P, H_kv, page_size, D]``, ``key_scales`` and ``value_scales`` (fp32)
+    ``[P, H_kv, page_size / 16]``; ``page_size`` and ``D`` are multiples of 16, ``D`` at most 256.  A number stands for itself times its block's
+    scale; where that is NaN (an infinity or a NaN was stored), every number of the block is."""
+
+    def __init__(self, keys: torch.Tensor, values: torch.Tensor, key_scales: torch.Tensor, value_scales: torch.Tensor):
+        for name, t in (("keys", keys), ("values", values)):
+            if t.dtype != torch.float8_e4m3fn or t.dim() != 4 or t.shape != keys.shape or min(t.shape) <= 0:
+                raise ValueError(f"Fp8KvPages: {name} must be float8_e4m3fn [P, H_kv, page_size, D], keys and values alike")
+        pages, heads, size, dim = keys.shape
+        if size % TOKENS or dim % 16 or dim > 256:
+            raise ValueError(f"Fp8KvPages: page_size must be a multiple of {TOKENS}, D a multiple of 16 up to 256, got {size} and {dim}")
+        for name, t in (("key_scales", key_scales), ("value_scales", value_scales)):
+            if t.dtype != torch.float32 or t.shape != (pages, heads, size // TOKENS):
+                raise ValueError(f"Fp8KvPages: {name} must be float32 {(pages, heads, size // TOKENS)}, one for each {TOKENS} tokens of a head")
+        if any(t.device != keys.device or not t.is_contiguous() for t in (keys, values, key_scales, value_scales)) or keys.data_ptr() % 16 or values.data_ptr() % 16:
+            raise ValueError("Fp8KvPages: tensors must be contiguous, on one device, the numbers on a boundary of 16 bytes")
+        self.keys, self.values, self.key_scales, self.value_scales = keys, values, key_scales, value_scales
+        self.num_pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, size, dim
+        self.index = keys.get_device()
+        self.native = blocks.Fp8Pages(keys.data_ptr(), values.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), pages, heads, size, dim)
+
+    @staticmethod
+    def zeros(num_pages: int, kv_heads: int, page_size: int, head_dim: int, device="cuda") -> "Fp8KvPages":
+        if min(num_pages, kv_heads, page_size, head_dim) <= 0 or page_size % TOKENS:
+            raise ValueError(f"Fp8KvPages: page_size must be a multiple of {TOKENS} and every size positive")
+        numbers = [torch.zeros((num_pages, kv_heads, page_size, head_dim), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2)]
+        return Fp8KvPages(*numbers, *(torch.zeros((num_pages, kv_heads, page_size // TOKENS), dtype=torch.float32, device=device) for _ in range(2)))
+
+    @property
+    def device(self) -> torch.device:
+        return self.keys.device
+
+    @property
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.keys, self.values, self.key_scales, self.value_scales))
+
+    def dequantize(self, pages=slice(None), dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
+        """(keys, values) that the numbers of ``pages`` (an index into the first dimension) stand for."""
+        wide = lambda numbers, scales: (numbers.view(torch.uint8)[pages].view(torch.float8_e4m3fn).float() * scales[pages].repeat_interleave(TOKENS, -1)[..., None]).to(dtype)  # noqa: E731
+        return wide(self.keys, self.key_scales), wide(self.values, self.value_scales)
+
+
+def _step(op: str, pages: Fp8KvPages, query: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor, block_table_host, context_lens_host):
+    """Checks of a step's shapes and metadata -> (block table, context lengths, the lengths on the host)."""
+    if query.dim() != 4:
+        raise ValueError(f"{op}: query must be 4D [B, H_q, L, D]")
+    B, heads, L, D = query.shape
+    if min(query.shape) <= 0:
+        raise ValueError(f"{op}: dimensions must be positive")
+    if D != pages.head_dim:
+        raise ValueError(f"{op}: query and pages must have the same head dimension")
+    if heads % pages.kv_heads:
+        raise ValueError(f"{op}: query heads must be divisible by K/V heads")
+    if query.dtype not in _DTYPES:
+        raise ValueError(f"{op}: supports float32 or bfloat16 inputs")
+    if block_table.dim() != 2 or context_lens.dim() != 1 or block_table.dtype != torch.int32 or context_lens.dtype != torch.int32:
+        raise ValueError(f"{op}: block_table must be 2D int32 and context_lens 1D int32")
+    if block_table.shape[0] != B or context_lens.shape[0] != B or block_table.shape[1] <= 0:
+        raise ValueError(f"{op}: query, block_table, and context_lens batch sizes must match, with at least one page slot")
+    if context_lens_host is None:
+        context_lens_host = context_lens.detach().cpu().numpy()
+    if block_table_host is None:
+        block_table_host = block_table.detach().cpu().numpy()
+    lens = np.asarray(context_lens_host).reshape(B)
+    table = np.asarray(block_table_host).reshape(B, -1)
+    if table.shape[1] != block_table.shape[1]:
+        raise ValueError(f"{op}: block_table_host must be a copy of block_table")
+    validate_paged_metadata(lens, table, pages.page_size, pages.num_pages, L)
+    return block_table if block_table.is_contiguous() else block_table.contiguous(), context_lens if context_lens.is_contiguous() else context_lens.contiguous(), lens
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    return x if x.stride(3) == 1 else x.contiguous()
+
+
+def rotate_append_fp8(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, pages: Fp8KvPages, block_table: torch.Tensor, context_lens: torch.Tensor, *, rope=None,
+                      query_norm=None, key_norm=None, block_table_host: np.ndarray | None = None, context_lens_host: np.ndarray | None = None) -> torch.Tensor:
+    """Append a step's ``key`` and ``value [B, H_kv, L, D]`` to the pages at positions ``context_lens - L ..``; -> the queries ``[B, H_q, L, D]`` to attend with.
+
+    ``query_norm`` and ``key_norm`` (``FastRMSNorm``) and ``rope`` (``FastRoPE``, turned by a token's position) are applied on the way, the keys' in 64 bits
+    ahead of their one rounding.  Any strides will do; float32 or bfloat16.  A block of 16 tokens of a head has one scale: it grows where the new
+    tokens need it to, and the block's earlier numbers are rounded to it again."""
+    table, lens, _ = _step("rotate_append_fp8", pages, query, block_table, context_lens, block_table_host, context_lens_host)
+    B, _, L, D = query.shape
+    if key.shape != value.shape or tuple(key.shape) != (B, pages.kv_heads, L, D):
+        raise ValueError("rotate_append_fp8: key and value must be [B, H_kv, L, D] beside the query")
+    if key.dtype != query.dtype or value.dtype != query.dtype:
+        raise ValueError("rotate_append_fp8: query, key, and value must have the same dtype")
+    rot = 0
+    if rope is not None:
+        rot = int(rope.dims)
+        if rot % 2 or not 0 < rot <= D or not rope.base > 0:
+            raise ValueError(f"rotate_append_fp8: cannot rotate {rot} of {D} entries")
+    more = {}
+    for name, norm in (("q", query_norm), ("k", key_norm)):
+        if norm is not None:
+            if norm.weight.numel() != D:
+                raise ValueError(f"rotate_append_fp8: a norm of {norm.weight.numel()} entries for heads of {D}")
+            more[name + "_norm"], more[name + "_eps"] = norm._weight_as(query.dtype, query.device), float(norm.eps)
+    return blocks.fp8_append(pages.native, pages.index, _rows(query), _rows(key), _rows(value), table, lens, rot=rot, base=float(rope.base) if rot else 1.0,
+                             interleaved=bool(rot and rope.traditional), **more)
+
+
+def paged_attention_fp8(query: torch.Tensor, pages: Fp8KvPages, block_table: torch.Tensor, context_lens: torch.Tensor, scale: float | None = None,
+                        mask: torch.Tensor | str | None = None, *, block_table_host: np.ndarray | None = None, context_lens_host: np.ndarray | None = None) -> torch.Tensor:
+    """``paged_attention`` over pages of 8 bits: ``query [B, H_q, L, D]`` (float32 or bfloat16, any strides) -> the same shape and dtype, laid out token by token.
+    ``mask``: None or ``"causal"``; ``scale``: ``D ** -0.5`` by default.  Rows of idle slots come out as zeros."""
+    if isinstance(mask, torch.Tensor) or mask not in (None, "causal"):
+        raise NotImplementedError("Paged attention only supports mask=None or causal")
+    table, lens, host = _step("paged_attention_fp8", pages, query, block_table, context_lens, block_table_host, context_lens_host)
+    factor = query.shape[-1] ** -0.5 if scale is None else float(scale)
+    return blocks.fp8_attention(pages.native, pages.index, _rows(query), table, lens, int(host.max()), factor, mask == "causal")
