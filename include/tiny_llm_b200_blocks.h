@@ -411,15 +411,31 @@ typedef struct {
  * not overlap q.  Of a block with m the largest magnitude of its new rows, the scale is the larger of 2^e (the smallest e with m <= 448 * 2^e) and, if the block holds
  * earlier tokens, the scale before; new rows are rounded to e4m3(x / scale), numbers of earlier tokens to e4m3(number * scale before / scale).  A NaN or infinity
  * among the new rows makes the scale NaN.  Slots behind the last token stay as they are.  Table entries outside [0, num_pages): nothing is stored there. */
-int tlb_fp8_append(const tlb_fp8_pages *pages, const void *q, long long q_b, long long q_h, long long q_l, void *q_out, const void *k, long long k_b, long long k_h,
-                   long long k_l, const void *v, long long v_b, long long v_h, long long v_l, int batch, int heads, int tokens, const int32_t *table, int max_pages,
-                   const int32_t *lens, const void *q_norm, float q_eps, const void *k_norm, float k_eps, int rot, double base, int interleaved, int dtype, void *stream);
+typedef struct {
+    const void *q, *k, *v;
+    void *q_out;
+    const int32_t *table, *lens; /* table [batch, max_pages] */
+    const void *q_norm, *k_norm;
+    long long q_b, q_h, q_l, k_b, k_h, k_l, v_b, v_h, v_l;
+    double base;
+    float q_eps, k_eps;
+    int batch, heads, tokens, max_pages, rot, interleaved, dtype;
+} tlb_fp8_append_call;
+int tlb_fp8_append(const tlb_fp8_pages *pages, const tlb_fp8_append_call *call, void *stream);
 /* out [batch, tokens, heads, dim] = softmax(q k^T * scale) v over the first lens[b] slots of each request (the `tokens` newest among them); causal: new token i sees
  * lens[b] - tokens + i + 1 of them.  Rows that see nothing come out as zeros.  Products with the cache's numbers are exact, their sums, the softmax and the scales fp32;
  * weights are rounded to f16 (relative to the largest so far) for bf16 outputs, and use 22 bits for fp32 ones, whose queries do so too.  longest: the largest of lens as far as the host knows;
  * it decides how the work is cut and never the result but for the order of sums. */
-int tlb_fp8_attention(const tlb_fp8_pages *pages, const void *q, long long q_b, long long q_h, long long q_l, void *out, int batch, int heads, int tokens,
-                      const int32_t *table, int max_pages, const int32_t *lens, int longest, double scale, int causal, int dtype, void *stream);
+typedef struct {
+    const void *q;
+    void *out;
+    const int32_t *table, *lens;
+    void *workspace; /* unused: NULL */
+    long long q_b, q_h, q_l;
+    double scale;
+    int batch, heads, tokens, max_pages, longest, causal, dtype;
+} tlb_fp8_attention_call;
+int tlb_fp8_attention(const tlb_fp8_pages *pages, const tlb_fp8_attention_call *call, void *stream);
 
 #ifdef __cplusplus
 }

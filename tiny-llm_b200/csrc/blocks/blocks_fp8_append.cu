@@ -25,15 +25,10 @@ struct F8Turns {
     double of[kApMostDim / 2];  // base^(-2i / dims) / (2 pi): turns a position
 };
 
-struct F8Append {
+struct F8Append : tlb_fp8_append_call {
     tlb_fp8_pages pages;
-    const void *q, *k, *v;
-    long long q_b, q_h, q_l, k_b, k_h, k_l, v_b, v_h, v_l;  // strides, in entries
-    void *q_out;                                             // [batch, tokens, heads, dim]
-    const int32_t *table, *lens;
-    const void *q_norm, *k_norm;
-    float q_eps, k_eps;
-    int batch, heads, group, tokens, max_pages, rot, interleaved;
+    int group;
+    F8Append(const tlb_fp8_pages &p, const tlb_fp8_append_call &c, int g) : tlb_fp8_append_call(c), pages(p), group(g) {}
 };
 
 __device__ __forceinline__ int2 ap_pair(const F8Append &a, int i) { return a.interleaved ? make_int2(2 * i, 2 * i + 1) : make_int2(i, i + a.rot / 2); }
@@ -211,26 +206,22 @@ static int append_launch(const F8Append &a, const F8Turns &turns, cudaStream_t s
 
 using namespace tlb;
 
-extern "C" int tlb_fp8_append(const tlb_fp8_pages *pages, const void *q, long long q_b, long long q_h, long long q_l, void *q_out, const void *k, long long k_b, long long k_h,
-                              long long k_l, const void *v, long long v_b, long long v_h, long long v_l, int batch, int heads, int tokens, const int32_t *table, int max_pages,
-                              const int32_t *lens, const void *q_norm, float q_eps, const void *k_norm, float k_eps, int rot, double base, int interleaved, int dtype,
-                              void *stream) {
+extern "C" int tlb_fp8_append(const tlb_fp8_pages *pages, const tlb_fp8_append_call *c, void *stream) {
     const int rc = f8_check_pages("fp8_append", pages);
     if (rc != TL_OK) return rc;
-    if (batch < 0 || tokens < 0 || heads <= 0 || heads % pages->heads) return tl::fail(TL_EINVAL, "fp8_append: %d query heads over %d key/value heads", heads, pages->heads);
-    if (rot < 0 || rot % 2 || rot > pages->dim || !(base > 0.0)) return tl::fail(TL_EINVAL, "fp8_append: cannot rotate %d of %d entries", rot, pages->dim);
-    if (batch == 0 || tokens == 0) return TL_OK;
-    if (batch > 65535 || pages->heads > 65535 || tokens > (1 << 30) || max_pages <= 0) return tl::fail(TL_EINVAL, "fp8_append: sizes out of range");
-    if (!q || !q_out || !k || !v || !table || !lens) return tl::fail(TL_EINVAL, "fp8_append: missing argument");
-    // the frequencies of the last call of this thread; 64 to 128 powers otherwise
+    if (!c || c->batch < 0 || c->tokens < 0 || c->heads <= 0 || c->heads % pages->heads) return tl::fail(TL_EINVAL, "fp8_append: query heads over %d key/value heads", pages->heads);
+    if (c->rot < 0 || c->rot % 2 || c->rot > pages->dim || !(c->base > 0.0)) return tl::fail(TL_EINVAL, "fp8_append: cannot rotate %d of %d entries", c->rot, pages->dim);
+    if (c->batch == 0 || c->tokens == 0) return TL_OK;
+    if (c->batch > 65535 || pages->heads > 65535 || c->tokens > (1 << 30) || c->max_pages <= 0) return tl::fail(TL_EINVAL, "fp8_append: sizes out of range");
+    if (!c->q || !c->q_out || !c->k || !c->v || !c->table || !c->lens) return tl::fail(TL_EINVAL, "fp8_append: missing argument");
+    // the frequencies of this thread's last call; half as many powers otherwise
     static thread_local F8Turns turns;
     static thread_local int turns_rot = -1;
     static thread_local double turns_base = 0.0;
-    if (rot != turns_rot || base != turns_base) {
-        for (int i = 0; i < rot / 2; ++i) turns.of[i] = pow(base, -2.0 * i / rot) / (2.0 * M_PI);
-        turns_rot = rot, turns_base = base;
+    if (c->rot != turns_rot || c->base != turns_base) {
+        for (int i = 0; i < c->rot / 2; ++i) turns.of[i] = pow(c->base, -2.0 * i / c->rot) / (2.0 * M_PI);
+        turns_rot = c->rot, turns_base = c->base;
     }
-    const F8Append a{*pages, q, k, v, q_b, q_h, q_l, k_b, k_h, k_l, v_b, v_h, v_l, q_out, table, lens, q_norm, k_norm, q_eps, k_eps, batch, heads, heads / pages->heads, tokens,
-                     max_pages, rot, interleaved != 0};
-    TLB_DISPATCH(dtype, "fp8_append", return append_launch<T>(a, turns, as_stream(stream)));
+    const F8Append a{*pages, *c, c->heads / pages->heads};
+    TLB_DISPATCH(c->dtype, "fp8_append", return append_launch<T>(a, turns, as_stream(stream)));
 }

@@ -372,12 +372,12 @@ static int attend_launch(F8Attend a, int ranks, cudaStream_t st) {
 }
 
 template <typename T>
-static int attend_any(const F8Attend &a, int longest, cudaStream_t st) {
+static int attend_any(const F8Attend &a, cudaStream_t st) {
     const int D = a.pages.dim, rows = a.group * a.tokens;
     const int nt = D > 128 || rows <= 8 ? 1 : 2;
     const long long ctas = static_cast<long long>((rows + 8 * nt - 1) / (8 * nt)) * a.pages.heads * a.batch;
     int ranks = 1;  // as many CTAs as fill the GPU, each with two blocks a warp at the least
-    while (ranks < 8 && ctas * ranks < 2 * sm_count() && longest > ranks * 2 * 8 * kF8Tokens) ranks *= 2;
+    while (ranks < 8 && ctas * ranks < 2 * sm_count() && a.longest > ranks * 2 * 8 * kF8Tokens) ranks *= 2;
     if (D <= 64) return nt == 1 ? attend_launch<T, 64, 1, 8>(a, ranks, st) : attend_launch<T, 64, 2, 8>(a, ranks, st);
     if (D <= 128) return nt == 1 ? attend_launch<T, 128, 1, 8>(a, ranks, st) : attend_launch<T, 128, 2, 8>(a, ranks, st);
     return attend_launch<T, 256, 1, 8>(a, ranks, st);
@@ -387,16 +387,13 @@ static int attend_any(const F8Attend &a, int longest, cudaStream_t st) {
 
 using namespace tlb;
 
-extern "C" int tlb_fp8_attention(const tlb_fp8_pages *pages, const void *q, long long q_b, long long q_h, long long q_l, void *out, int batch, int heads, int tokens,
-                                 const int32_t *table, int max_pages, const int32_t *lens, int longest, double scale, int causal, int dtype, void *stream) {
+extern "C" int tlb_fp8_attention(const tlb_fp8_pages *pages, const tlb_fp8_attention_call *c, void *stream) {
     const int rc = f8_check_pages("fp8_attention", pages);
     if (rc != TL_OK) return rc;
-    if (batch < 0 || tokens < 0 || heads <= 0 || heads % pages->heads) return tl::fail(TL_EINVAL, "fp8_attention: %d query heads over %d key/value heads", heads, pages->heads);
-    if (batch == 0 || tokens == 0) return TL_OK;
-    if (max_pages <= 0 || static_cast<long long>(heads / pages->heads) * tokens > (1 << 30)) return tl::fail(TL_EINVAL, "fp8_attention: sizes out of range");
-    if (!q || !out || !table || !lens) return tl::fail(TL_EINVAL, "fp8_attention: missing argument");
-    const double log2 = scale * 1.4426950408889634;
-    F8Attend a{*pages, q, q_b, q_h, q_l, out, table, lens, batch, heads, heads / pages->heads, tokens, max_pages, causal != 0, 0, static_cast<float>(log2), 0.f};
-    a.scale_rest = static_cast<float>(log2 - a.scale_log2);
-    TLB_DISPATCH(dtype, "fp8_attention", return attend_any<T>(a, longest, as_stream(stream)));
+    if (!c || c->batch < 0 || c->tokens < 0 || c->heads <= 0 || c->heads % pages->heads) return tl::fail(TL_EINVAL, "fp8_attention: query heads over %d key/value heads", pages->heads);
+    if (c->batch == 0 || c->tokens == 0) return TL_OK;
+    if (c->max_pages <= 0 || static_cast<long long>(c->heads / pages->heads) * c->tokens > (1 << 30)) return tl::fail(TL_EINVAL, "fp8_attention: sizes out of range");
+    if (!c->q || !c->out || !c->table || !c->lens) return tl::fail(TL_EINVAL, "fp8_attention: missing argument");
+    const F8Attend a(*pages, *c);
+    TLB_DISPATCH(c->dtype, "fp8_attention", return attend_any<T>(a, as_stream(stream)));
 }

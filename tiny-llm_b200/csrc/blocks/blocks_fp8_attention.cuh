@@ -5,14 +5,14 @@
 
 namespace tlb {
 
-struct F8Attend {
+struct F8Attend : tlb_fp8_attention_call {
     tlb_fp8_pages pages;
-    const void *q;  // strides in entries
-    long long q_b, q_h, q_l;
-    void *out;  // [batch, tokens, heads, dim]
-    const int32_t *table, *lens;
-    int batch, heads, group, tokens, max_pages, causal, col_blocks;
+    int group, col_blocks;
     float scale_log2, scale_rest;  // scale * log2(e), and what its rounding to fp32 left
+    F8Attend(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c) : tlb_fp8_attention_call(c), pages(p), group(c.heads / p.heads), col_blocks(0) {
+        const double log2 = c.scale * 1.4426950408889634;
+        scale_log2 = static_cast<float>(log2), scale_rest = static_cast<float>(log2 - scale_log2);
+    }
 };
 
 }  // namespace tlb

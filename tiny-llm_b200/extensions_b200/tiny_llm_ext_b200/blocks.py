@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import importlib.util
 import os
+import struct
 from pathlib import Path
 
 import torch
@@ -98,8 +99,8 @@ _SIGNATURES = {
     "tlb_fp8_linear_workspace": (ctypes.c_size_t, [_I, _I]),
     "tlb_fp8_linear": (_I, [_VP, _LL, _VP, _I, _VP, _VP, _VP, _I, _I, _I, _VP, ctypes.c_size_t, _I, _VP]),
     "tlb_fp8_gated_mlp_workspace": (ctypes.c_size_t, [_I, _I, _I]),
-    "tlb_fp8_append": (_I, [_VP, _VP, _LL, _LL, _LL, _VP, _VP, _LL, _LL, _LL, _VP, _LL, _LL, _LL, _I, _I, _I, _VP, _I, _VP, _VP, _F, _VP, _F, _I, _D, _I, _I, _VP]),
-    "tlb_fp8_attention": (_I, [_VP, _VP, _LL, _LL, _LL, _VP, _I, _I, _I, _VP, _I, _VP, _I, _D, _I, _I, _VP]),
+    "tlb_fp8_append": (_I, [_VP, ctypes.c_char_p, _VP]),
+    "tlb_fp8_attention": (_I, [_VP, ctypes.c_char_p, _VP]),
     "tlb_fp8_gated_mlp": (_I, [_VP, _LL, _VP, _I, _VP, _VP, _I, _VP, _VP, _I, _I, _I, _I, _F, _F, _VP, ctypes.c_size_t, _I, _VP]),
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -1186,61 +1187,78 @@ class Fp8Pages(ctypes.Structure):
     _fields_ = [(name, _VP) for name in ("keys", "values", "key_scales", "value_scales")] + [(name, _I) for name in ("num_pages", "heads", "page_size", "dim")]
 
 
-def _fp8_step(op: str, pages: Fp8Pages, device: int, heads: int, *tensors) -> tuple:
-    """(batch, tokens) of a step's ``[B, heads, L, dim]`` tensors with unit inner stride."""
+# tlb_fp8_append_call and tlb_fp8_attention_call, packed at once: of small calls the host sets the pace, and ctypes converts two dozen arguments one by one
+_FP8_APPEND = struct.Struct("@PPPPPPPPqqqqqqqqqdffiiiiiii")
+_FP8_ATTENTION = struct.Struct("@PPPPPqqqdiiiiiii")
+
+
+def _fp8_step(op: str, pages: Fp8Pages, device: int, table: torch.Tensor, lens: torch.Tensor, *tensors) -> None:
+    """What the C entries cannot see of a step's ``[B, heads, L, dim]`` tensors, block table and lengths."""
     first = tensors[0]
-    for t, n in zip(tensors, (heads, pages.heads, pages.heads)):
-        if t.dim() != 4 or t.shape != (first.shape[0], n, first.shape[2], pages.dim) or t.dtype != first.dtype or t.stride(3) != 1:
-            raise RuntimeError(f"{op}: tensors must be [B, {n}, L, {pages.dim}] of one dtype, entries of a row side by side")
+    for t in tensors:
+        heads = t.shape[1] if t is first and t.dim() == 4 else pages.heads
+        if t.dim() != 4 or t.shape != (first.shape[0], heads, first.shape[2], pages.dim) or t.dtype != first.dtype or t.stride(3) != 1:
+            raise RuntimeError(f"{op}: tensors must be [B, {heads}, L, {pages.dim}] of one dtype, entries of a row side by side")
+    if table.dtype != torch.int32 or lens.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != first.shape[0] or lens.shape != first.shape[:1]:
+        raise RuntimeError(f"{op}: the block table must be int32 [{first.shape[0]}, pages], the lengths int32 [{first.shape[0]}]")
+    if not table.is_contiguous() or not lens.is_contiguous():
+        raise RuntimeError(f"{op}: block table and lengths must be contiguous")
+    fp8_devices(op, device, table, lens, *tensors)
+
+
+def fp8_devices(op: str, device: int, *tensors) -> None:
+    for t in tensors:
         if t.get_device() != device or device < 0:
             raise RuntimeError(f"{op}: the blocks extension is GPU-only, and a step and the pages must be on one device")
-    return first.shape[0], first.shape[2]
-
-
-def _fp8_table(op: str, table: torch.Tensor, lens: torch.Tensor, batch: int, device: int) -> None:
-    if table.dtype != torch.int32 or lens.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != batch or lens.shape != (batch,):
-        raise RuntimeError(f"{op}: the block table must be int32 [{batch}, pages], the lengths int32 [{batch}]")
-    if table.get_device() != device or lens.get_device() != device or not table.is_contiguous() or not lens.is_contiguous():
-        raise RuntimeError(f"{op}: block table and lengths must be contiguous, on the pages' device")
 
 
 def fp8_append(pages: Fp8Pages, device: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, *, q_norm=None, q_eps: float = 0.0, k_norm=None,
                k_eps: float = 0.0, rot: int = 0, base: float = 1.0, interleaved: bool = False) -> torch.Tensor:
     """``tlb_fp8_append``: a step's ``k`` and ``v [B, G, L, dim]`` into the pages, ``q [B, H, L, dim]`` -> the same shape (laid out token by token)."""
-    B, L = _fp8_step("fp8_append", pages, device, q.shape[1], q, k, v)
-    H = q.shape[1]
-    _fp8_table("fp8_append", table, lens, B, device)
+    _fp8_step("fp8_append", pages, device, table, lens, q, k, v)
     for w in (q_norm, k_norm):
         if w is not None and (w.shape != (pages.dim,) or w.dtype != q.dtype or w.get_device() != device or not w.is_contiguous()):
             raise RuntimeError("fp8_append: norm weights must be [dim] of the step's dtype")
-    code = _code(q.dtype)
+    return fp8_append_of(pages, device, q, k, v, table, lens, q_norm, q_eps, k_norm, k_eps, rot, base, interleaved)
 
-    def call():
-        out = q.new_empty((B, L, H, pages.dim))
-        qs, ks, vs = q.stride(), k.stride(), v.stride()
-        _check(library().tlb_fp8_append(ctypes.addressof(pages), q.data_ptr(), qs[0], qs[1], qs[2], out.data_ptr(), k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2],
-                                        B, H, L, table.data_ptr(), table.shape[1], lens.data_ptr(), _ptr(q_norm), q_eps, _ptr(k_norm), k_eps, rot, base, int(interleaved), code,
-                                        _raw_stream(device)))
-        return out
 
-    return _on_device(device, call).transpose(1, 2)
+def fp8_append_of(pages: Fp8Pages, device: int, q, k, v, table, lens, q_norm=None, q_eps=0.0, k_norm=None, k_eps=0.0, rot=0, base=1.0, interleaved=False) -> torch.Tensor:
+    """``fp8_append`` of tensors that the caller has checked (``rotate_append_fp8``)."""
+    if _current_device() != device:
+        with torch.cuda.device(device):
+            return fp8_append_of(pages, device, q, k, v, table, lens, q_norm, q_eps, k_norm, k_eps, rot, base, interleaved)
+    B, H, L, D = q.shape
+    out = q.new_empty((B, L, H, D))
+    qb, qh, ql, _ = q.stride()
+    kb, kh, kl, _ = k.stride()
+    vb, vh, vl, _ = v.stride()
+    call = _FP8_APPEND.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(), 0 if q_norm is None else q_norm.data_ptr(),
+                            0 if k_norm is None else k_norm.data_ptr(), qb, qh, ql, kb, kh, kl, vb, vh, vl, base, q_eps, k_eps, B, H, L, table.shape[1], rot, interleaved, _code(q.dtype))
+    rc = library().tlb_fp8_append(ctypes.addressof(pages), call, _raw_stream(device))
+    if rc:
+        _check(rc)
+    return out.transpose(1, 2)
 
 
 def fp8_attention(pages: Fp8Pages, device: int, q: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, longest: int, scale: float, causal: bool) -> torch.Tensor:
     """``tlb_fp8_attention``: ``q [B, H, L, dim]`` -> the same shape (laid out token by token)."""
-    B, L = _fp8_step("fp8_attention", pages, device, q.shape[1], q)
-    H = q.shape[1]
-    _fp8_table("fp8_attention", table, lens, B, device)
-    code = _code(q.dtype)
+    _fp8_step("fp8_attention", pages, device, table, lens, q)
+    return fp8_attention_of(pages, device, q, table, lens, longest, scale, causal)
 
-    def call():
-        out = q.new_empty((B, L, H, pages.dim))
-        qs = q.stride()
-        _check(library().tlb_fp8_attention(ctypes.addressof(pages), q.data_ptr(), qs[0], qs[1], qs[2], out.data_ptr(), B, H, L, table.data_ptr(), table.shape[1], lens.data_ptr(),
-                                           longest, scale, int(causal), code, _raw_stream(device)))
-        return out
 
-    return _on_device(device, call).transpose(1, 2)
+def fp8_attention_of(pages: Fp8Pages, device: int, q, table, lens, longest, scale, causal) -> torch.Tensor:
+    """``fp8_attention`` of tensors that the caller has checked (``paged_attention_fp8``)."""
+    if _current_device() != device:
+        with torch.cuda.device(device):
+            return fp8_attention_of(pages, device, q, table, lens, longest, scale, causal)
+    B, H, L, D = q.shape
+    out = q.new_empty((B, L, H, D))
+    qb, qh, ql, _ = q.stride()
+    call = _FP8_ATTENTION.pack(q.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(), 0, qb, qh, ql, scale, B, H, L, table.shape[1], longest, causal, _code(q.dtype))
+    rc = library().tlb_fp8_attention(ctypes.addressof(pages), call, _raw_stream(device))
+    if rc:
+        _check(rc)
+    return out.transpose(1, 2)
 
 
 def moe_few_tokens(dim: int, outputs: int, experts: int, top: int, group_count: int = 0, fp8: bool = False) -> int:

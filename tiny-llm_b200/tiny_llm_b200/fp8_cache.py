@@ -63,10 +63,11 @@ class Fp8KvPages:
 
 def _step(op: str, pages: Fp8KvPages, query: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor, block_table_host, context_lens_host):
     """Checks of a step's shapes and metadata -> (block table, context lengths, the lengths on the host)."""
-    if query.dim() != 4:
+    shape, rows = query.shape, block_table.shape
+    if len(shape) != 4:
         raise ValueError(f"{op}: query must be 4D [B, H_q, L, D]")
-    B, heads, L, D = query.shape
-    if min(query.shape) <= 0:
+    B, heads, L, D = shape
+    if min(shape) <= 0:
         raise ValueError(f"{op}: dimensions must be positive")
     if D != pages.head_dim:
         raise ValueError(f"{op}: query and pages must have the same head dimension")
@@ -74,18 +75,17 @@ def _step(op: str, pages: Fp8KvPages, query: torch.Tensor, block_table: torch.Te
         raise ValueError(f"{op}: query heads must be divisible by K/V heads")
     if query.dtype not in _DTYPES:
         raise ValueError(f"{op}: supports float32 or bfloat16 inputs")
-    if block_table.dim() != 2 or context_lens.dim() != 1 or block_table.dtype != torch.int32 or context_lens.dtype != torch.int32:
+    if len(rows) != 2 or context_lens.dim() != 1 or block_table.dtype != torch.int32 or context_lens.dtype != torch.int32:
         raise ValueError(f"{op}: block_table must be 2D int32 and context_lens 1D int32")
-    if block_table.shape[0] != B or context_lens.shape[0] != B or block_table.shape[1] <= 0:
+    if rows[0] != B or len(context_lens) != B or rows[1] <= 0:
         raise ValueError(f"{op}: query, block_table, and context_lens batch sizes must match, with at least one page slot")
     if context_lens_host is None:
         context_lens_host = context_lens.detach().cpu().numpy()
     if block_table_host is None:
         block_table_host = block_table.detach().cpu().numpy()
-    lens = np.asarray(context_lens_host).reshape(B)
-    table = np.asarray(block_table_host).reshape(B, -1)
-    if table.shape[1] != block_table.shape[1]:
-        raise ValueError(f"{op}: block_table_host must be a copy of block_table")
+    lens, table = np.asarray(context_lens_host), np.asarray(block_table_host)
+    if lens.shape != (B,) or table.shape != rows:
+        raise ValueError(f"{op}: context_lens_host and block_table_host must be copies of the tensors")
     validate_paged_metadata(lens, table, pages.page_size, pages.num_pages, L)
     return block_table if block_table.is_contiguous() else block_table.contiguous(), context_lens if context_lens.is_contiguous() else context_lens.contiguous(), lens
 
@@ -103,23 +103,26 @@ def rotate_append_fp8(query: torch.Tensor, key: torch.Tensor, value: torch.Tenso
     tokens need it to, and the block's earlier numbers are rounded to it again."""
     table, lens, _ = _step("rotate_append_fp8", pages, query, block_table, context_lens, block_table_host, context_lens_host)
     B, _, L, D = query.shape
-    if key.shape != value.shape or tuple(key.shape) != (B, pages.kv_heads, L, D):
+    if key.shape != (B, pages.kv_heads, L, D) or key.shape != value.shape:
         raise ValueError("rotate_append_fp8: key and value must be [B, H_kv, L, D] beside the query")
     if key.dtype != query.dtype or value.dtype != query.dtype:
         raise ValueError("rotate_append_fp8: query, key, and value must have the same dtype")
-    rot = 0
+    blocks.fp8_devices("rotate_append_fp8", pages.index, query, key, value, table, lens)
+    rot, base, interleaved = 0, 1.0, False
     if rope is not None:
-        rot = int(rope.dims)
-        if rot % 2 or not 0 < rot <= D or not rope.base > 0:
+        rot, base, interleaved = rope.dims, rope.base, rope.traditional
+        if rot % 2 or not 0 < rot <= D or not base > 0:
             raise ValueError(f"rotate_append_fp8: cannot rotate {rot} of {D} entries")
-    more = {}
-    for name, norm in (("q", query_norm), ("k", key_norm)):
-        if norm is not None:
-            if norm.weight.numel() != D:
-                raise ValueError(f"rotate_append_fp8: a norm of {norm.weight.numel()} entries for heads of {D}")
-            more[name + "_norm"], more[name + "_eps"] = norm._weight_as(query.dtype, query.device), float(norm.eps)
-    return blocks.fp8_append(pages.native, pages.index, _rows(query), _rows(key), _rows(value), table, lens, rot=rot, base=float(rope.base) if rot else 1.0,
-                             interleaved=bool(rot and rope.traditional), **more)
+    weights = []
+    for norm in (query_norm, key_norm):
+        if norm is None:
+            weights += (None, 0.0)
+            continue
+        weight = norm._weight_as(query.dtype, query.device)
+        if weight.shape != (D,):
+            raise ValueError(f"rotate_append_fp8: a norm of {tuple(weight.shape)} for heads of {D}")
+        weights += (weight, norm.eps)
+    return blocks.fp8_append_of(pages.native, pages.index, _rows(query), _rows(key), _rows(value), table, lens, *weights, rot, base, interleaved)
 
 
 def paged_attention_fp8(query: torch.Tensor, pages: Fp8KvPages, block_table: torch.Tensor, context_lens: torch.Tensor, scale: float | None = None,
@@ -130,4 +133,5 @@ def paged_attention_fp8(query: torch.Tensor, pages: Fp8KvPages, block_table: tor
         raise NotImplementedError("Paged attention only supports mask=None or causal")
     table, lens, host = _step("paged_attention_fp8", pages, query, block_table, context_lens, block_table_host, context_lens_host)
     factor = query.shape[-1] ** -0.5 if scale is None else float(scale)
-    return blocks.fp8_attention(pages.native, pages.index, _rows(query), table, lens, int(host.max()), factor, mask == "causal")
+    blocks.fp8_devices("paged_attention_fp8", pages.index, query, table, lens)
+    return blocks.fp8_attention_of(pages.native, pages.index, _rows(query), table, lens, int(host.max()), factor, mask == "causal")
