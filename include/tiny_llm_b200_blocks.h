@@ -424,18 +424,18 @@ typedef struct {
 int tlb_fp8_append(const tlb_fp8_pages *pages, const tlb_fp8_append_call *call, void *stream);
 /* out [batch, tokens, heads, dim] = softmax(q k^T * scale) v over the first lens[b] slots of each request (the `tokens` newest among them); causal: new token i sees
  * lens[b] - tokens + i + 1 of them.  Rows that see nothing come out as zeros.  Products with the cache's numbers are exact, their sums, the softmax and the scales fp32;
- * weights are rounded to f16 (relative to the largest so far) for bf16 outputs, and use 22 bits for fp32 ones, whose queries do so too.  longest: the largest of lens as far as the host knows;
- * it decides how the work is cut and never the result but for the order of sums. */
+ * weights are rounded to f16 (relative to the largest so far) for bf16 outputs, and use 22 bits for fp32 ones, whose queries do so too.  How the keys are divided
+ * follows lens as it is when the launch runs; it decides the order of sums.  The workspace need not be initialised; calls that may run at once need one each. */
 typedef struct {
     const void *q;
     void *out;
     const int32_t *table, *lens;
-    void *workspace; /* unused: NULL */
     long long q_b, q_h, q_l;
     double scale;
-    int batch, heads, tokens, max_pages, longest, causal, dtype;
+    int batch, heads, tokens, max_pages, causal, dtype;
 } tlb_fp8_attention_call;
-int tlb_fp8_attention(const tlb_fp8_pages *pages, const tlb_fp8_attention_call *call, void *stream);
+size_t tlb_fp8_attention_workspace(const tlb_fp8_pages *pages, const tlb_fp8_attention_call *call);
+int tlb_fp8_attention(const tlb_fp8_pages *pages, const tlb_fp8_attention_call *call, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -7,19 +7,18 @@
 // column's running maximum (which may lag behind by 2^8 before the sums are scaled again), rounded to f16 for the second product: 2^-12 of a weight, where an output is
 // rounded to 2^-9 of itself; fp32 outputs take a second term for the rest.  Running sums are fp32.
 //
-// A warp takes blocks of 16 keys straight from the pages into registers in the layouts that the products want, without shared memory between: lane (g, t) loads 16-byte
-// pieces t, t + 4 .. of key rows g and g + 8, and of the value rows 2t, 2t + 1, 2t + 8, 2t + 9 the g-th eighth.  Which entry of a head a product's k-index means
-// is free as long as queries agree; the values' bytes of two keys are interleaved by byte permutation.  Warps of a CTA and CTAs of a cluster share the
-// keys of their columns and are joined at the end, in a fixed order.
-#include <cooperative_groups.h>
-
+// A warp takes blocks of 16 keys through a ring of its own in shared memory, filled by asynchronous copies, two blocks ahead of the one it works on; it waits for nobody
+// else.  Lane (g, t) reads 16-byte pieces t, t + 4 .. of key rows g and g + 8, and of the value rows 2t, 2t + 1, 2t + 8, 2t + 9 the g-th eighth: which entry of a head a product's
+// k-index means is free as long as queries agree, and the values' bytes of two keys are interleaved by byte permutation.  The warps of a CTA share its keys and are
+// joined in a fixed order.
+//
+// An item is 8 (or 16) columns of one request and key/value head.  A CTA takes an item, or, where the requests are few or of unlike length, a piece of one; an item in several
+// pieces leaves a partial result for each, which fp8_attend_join_kernel adds up in order.  The cut follows the lengths on the device, so a captured launch does.
 #include "../per_device.h"
 #include "blocks_fp8_cache.cuh"
 #include "blocks_fp8_attention.cuh"
 
 namespace tlb {
-
-namespace cg = cooperative_groups;
 
 constexpr float kAtLag = 8.f;  // log2: how far a running maximum may lag behind
 
@@ -28,10 +27,8 @@ __device__ __forceinline__ float at_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ uint32_t at_half2(uint32_t two) {  // two e4m3 numbers (the lower 16 bits) as f16
-    uint32_t r;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(two)));
-    return r;
+__device__ __forceinline__ void at_halves(uint32_t four, uint32_t &lo, uint32_t &hi) {  // four e4m3 numbers as f16
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(four));
 }
 __device__ __forceinline__ uint32_t at_turn(uint32_t v) {  // an 8 x 8 matrix of f16, transposed
     uint32_t r;
@@ -49,107 +46,233 @@ __device__ __forceinline__ float2 at_rest(uint32_t two, float lo, float hi) {  /
     return make_float2(lo - f.x, hi - f.y);
 }
 
-// 16 keys of a head, as a lane holds them.
-template <int DP>
-struct AtBlock {
-    uint4 k[2][DP / 64];
-    uint32_t v[4][DP / 32];
-    float ks, vs;
-};
+constexpr int kAtWarps = 8, kAtStages = 3;
+constexpr int kAtLeast = 32;  // blocks of a piece at the least
 
-template <int DP>
-__device__ __forceinline__ void at_load(AtBlock<DP> &x, const F8Attend &a, int b, int h, int key0, int page, int lane) {
-    const tlb_fp8_pages &pg = a.pages;
-    const int g = lane >> 2, t = lane & 3, D = pg.dim;
-    if (page < 0 || page >= pg.num_pages) page = 0;  // its keys are masked; nothing outside the pages is read
-    const int slot = key0 % pg.page_size;
-    const uint8_t *k = pg.keys + f8_row(pg, page, h, slot), *v = pg.values + f8_row(pg, page, h, slot);
-#pragma unroll
-    for (int r = 0; r < DP / 64; ++r) {
-        const int d = (4 * r + t) * 16;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) x.k[i][r] = d < D ? tl::ldg_stream(k + static_cast<size_t>(g + 8 * i) * D + d) : make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint8_t *row = v + static_cast<size_t>(2 * t + (i & 1) + 4 * (i & 2)) * D;
-        if constexpr (DP == 64) {
-            const uint2 w = g * 8 < D ? *reinterpret_cast<const uint2 *>(row + g * 8) : make_uint2(0, 0);
-            x.v[i][0] = w.x, x.v[i][1] = w.y;
-        } else {
-#pragma unroll
-            for (int p = 0; p < DP / 128; ++p) {
-                const int d = g * (DP / 8) + 16 * p;
-                const uint4 w = d < D ? tl::ldg_stream(row + d) : make_uint4(0, 0, 0, 0);
-                x.v[i][4 * p] = w.x, x.v[i][4 * p + 1] = w.y, x.v[i][4 * p + 2] = w.z, x.v[i][4 * p + 3] = w.w;
-            }
-        }
-    }
-    const size_t s = f8_scale_at(pg, page, h, slot);
-    x.ks = __ldg(pg.key_scales + s), x.vs = __ldg(pg.value_scales + s);
+__device__ __forceinline__ void at_copy16(uint32_t to, const void *from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ void at_copy4(uint32_t to, const void *from) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory"); }
+
+// A block in shared memory: 16 rows of keys, 16 of values, the two scales.  Rows of 128 bytes have their pieces moved about so that the eight lanes of a reading phase meet
+// all banks: a key's halves change places in odd rows (lanes read 4 pieces of 2 rows), a value's pairs of pieces go by the pair of rows (2 pieces of 4 rows).
+__host__ __device__ constexpr int at_stage(int dim) { return 2 * kF8Tokens * dim + 16; }
+template <bool MOVED>
+__device__ __forceinline__ int at_key(int row, int D, int byte) {
+    return row * D + (MOVED ? byte ^ ((row & 1) << 6) : byte);
+}
+template <bool MOVED>
+__device__ __forceinline__ int at_value(int row, int D, int byte) {
+    return row * D + (MOVED ? byte ^ (((row >> 1) & 3) << 5) : byte);
 }
 
-template <typename T, int DP, int NT, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) fp8_attend_kernel(const __grid_constant__ F8Attend a) {
+// DIM: entries of a head, 0: as the pages say.
+template <int DIM>
+__device__ __forceinline__ void at_issue(uint32_t stage, const F8Attend &a, int h, int blk, int in_page, int page, int lane) {
+    const tlb_fp8_pages &pg = a.pages;
+    const int D = DIM ? DIM : pg.dim;
+    if (static_cast<unsigned>(page) >= static_cast<unsigned>(pg.num_pages)) page = 0;  // its keys are skipped; nothing outside the pages is read
+    const size_t block = (static_cast<size_t>(page) * pg.heads + h) * a.page_blocks + in_page, byte = block * kF8Tokens * D + 16 * lane;
+    if constexpr (DIM == 128) {
+        const uint32_t k = stage + ((16 * lane) ^ ((lane >> 3 & 1) << 6)), v = stage + 16 * D + ((16 * lane) ^ ((lane >> 4) << 5)), w = stage + 16 * D + ((16 * lane) ^ ((lane >> 4) << 5) ^ 64);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) at_copy16(k + 512 * i, pg.keys + byte + 512 * i), at_copy16((i & 1 ? w : v) + 512 * i, pg.values + byte + 512 * i);
+    } else {
+        for (int i = lane; i < D; i += 32) {  // 16 rows of D / 16 pieces lie one behind the other
+            at_copy16(stage + 16 * i, pg.keys + byte + 16 * (i - lane));
+            at_copy16(stage + 16 * D + 16 * i, pg.values + byte + 16 * (i - lane));
+        }
+    }
+    if (lane < 2) at_copy4(stage + 32 * D + 4 * lane, (lane ? pg.value_scales : pg.key_scales) + block);
+}
+
+// n / d by a product; magic 0: where that might be off.
+__device__ __forceinline__ int at_div(int n, int d, unsigned magic) { return magic ? static_cast<int>(__umulhi(n, magic)) : n / d; }
+
+// 8 entries of a query
+template <typename T>
+__device__ __forceinline__ void at_query(const T *q, bool wide, float (&x)[8]) {
+    if (wide) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float4 v = load4(q + 4 * i);
+            x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = to_f(q[e]);
+    }
+}
+
+__device__ __forceinline__ int at_context(const F8Attend &a, int b) {
+    return static_cast<int>(max(0LL, min(static_cast<long long>(a.lens[b]), static_cast<long long>(a.max_pages) * a.pages.page_size)));
+}
+__device__ __forceinline__ int at_blocks(const F8Attend &a, int b) { return (at_context(a, b) + kF8Tokens - 1) / kF8Tokens; }
+
+// How long a piece of an item may be, in blocks: such that the pieces are about as many as the CTAs that the GPU holds at a time, or the items and half of those.  A piece
+// costs its CTA some microseconds beside its blocks, so it has kAtLeast of them.  Nothing here depends on how many idle slots there are: a step over more of
+// them is cut the same way, to the bit.  Whole warps; 0: nothing is cut.
+typedef int AtCut;
+__device__ __forceinline__ AtCut at_cut(const F8Attend &a) {
+    if (!a.workspace) return 0;
+    int total = 0, live = 0;  // at most 2^27 blocks a request
+    long long all = 0;
+    for (int r = threadIdx.x & 31; r < a.batch; r += 32) {
+        const int n = at_blocks(a, r);
+        all += n, live += n > 0;
+    }
+    total = static_cast<int>(min(all, 0x3ffffffLL));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o), live += __shfl_xor_sync(0xffffffffu, live, o);
+    const int each = a.pages.heads * a.col_blocks, room = max(a.slots - live * each, a.slots / 2);
+    return static_cast<int>(max(min((static_cast<long long>(total) * each + room - 1) / room, 0x3fffffffLL), static_cast<long long>(kAtLeast)));
+}
+__device__ __forceinline__ int at_pieces(const F8Attend &a, AtCut cut, int b) {
+    const int n = at_blocks(a, b);
+    return cut == 0 || n <= cut + cut / 4 ? 1 : (n + cut - 1) / cut;  // a quarter more is no reason to cut
+}
+// pieces of a head's eight (or sixteen) columns, over the requests before `request`
+__device__ __forceinline__ long long at_before(const F8Attend &a, AtCut cut, int request) {
+    int n = 0;
+    for (int r = threadIdx.x & 31; r < request; r += 32) n += at_pieces(a, cut, r);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    return n;
+}
+
+// The index-th piece: a request's items one after another, an item's pieces side by side.
+struct AtPiece {
+    int b, item, piece, pieces, size;  // size: blocks of a piece; b < 0: there are not so many
+};
+__device__ __forceinline__ AtPiece at_piece(const F8Attend &a, int index) {
+    const int each = a.pages.heads * a.col_blocks, lane = threadIdx.x & 31;
+    const AtCut cut = at_cut(a);
+    AtPiece x{-1, 0, 0, 1, 0x3fffffff};
+    if (cut == 0) {
+        x.b = at_div(index, each, a.each_magic), x.item = index - x.b * each;
+        return x;
+    }
+    const int want = at_div(index, each, a.each_magic);  // rounded down: an item's pieces over all items of a request are a multiple of them
+    int run = 0;
+    for (int r0 = 0; r0 < a.batch; r0 += 32) {
+        const int mine = r0 + lane < a.batch ? at_pieces(a, cut, r0 + lane) : 0;
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int below = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += below;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, want < run + upto);
+        if (past) {
+            const int src = __ffs(past) - 1;
+            x.b = r0 + src, x.pieces = __shfl_sync(0xffffffffu, mine, src);
+            const int at = index - (run + __shfl_sync(0xffffffffu, upto - mine, src)) * each;
+            x.item = at / x.pieces, x.piece = at % x.pieces;
+            if (x.pieces > 1) x.size = (at_blocks(a, x.b) + x.pieces - 1) / x.pieces;
+            return x;
+        }
+        run += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return x;
+}
+
+// DP: entries of a head that the lanes' shares make room for; DIM: entries it has, 0: fewer than DP.
+template <typename T, int DP, int DIM, int NT>
+__global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(T) == 2 ? 2 : 1) fp8_attend_kernel(const __grid_constant__ F8Attend a) {
     constexpr bool kTwo = sizeof(T) == 4;  // a second term of queries and weights
-    constexpr int KR = DP / 64, COLS = 8 * NT, J = DP / 16;
+    constexpr bool kMoved = DIM == 128;
+    constexpr int KR = DP / 64, COLS = 8 * NT, J = DP / 16, WARPS = kAtWarps, ROW = DP + 4;
     extern __shared__ __align__(16) unsigned char sm[];
-    float *part = reinterpret_cast<float *>(sm);  // [WARPS][COLS][DP], then maxima and sums [WARPS][COLS]
-    float *part_m = part + WARPS * COLS * DP, *part_l = part_m + WARPS * COLS;
-    tl::griddep_launch();
+    constexpr int QROW = DP + 8;
+    __shared__ __align__(16) __half q_tile[(kTwo ? 2 : 1) * COLS * QROW];
+    __shared__ float q_back[COLS];
+    // first the warps' rings, then, once all are through,
+    float *part = reinterpret_cast<float *>(sm);  // [WARPS][COLS][ROW], then maxima, sums and factors [WARPS][COLS]
+    float *part_m = part + WARPS * COLS * ROW, *part_l = part_m + WARPS * COLS, *part_w = part_l + WARPS * COLS;
     tl::griddep_wait();
-    cg::cluster_group cluster = cg::this_cluster();
-    const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+    tl::griddep_launch();  // behind the wait: the launch that joins the pieces reads the lengths ahead of its own
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const tlb_fp8_pages &pg = a.pages;
-    const int D = pg.dim, G = a.group, L = a.tokens;
-    // this CTA: columns of one request and key/value head; column = new token * group + query head
-    const unsigned item = blockIdx.x / ranks;
-    const int h = static_cast<int>(item % pg.heads), cb = static_cast<int>(item / pg.heads % a.col_blocks), b = static_cast<int>(item / pg.heads / a.col_blocks);
-    const int c0 = cb * COLS;
-    const int ctx = static_cast<int>(max(0LL, min(static_cast<long long>(a.lens[b]), static_cast<long long>(a.max_pages) * pg.page_size)));
+    const int D = DIM ? DIM : pg.dim, G = a.group, L = a.tokens;
+    const AtPiece mine = at_piece(a, blockIdx.x);
+    if (mine.b < 0) return;
+    const int b = mine.b, cb = at_div(mine.item, pg.heads, a.heads_magic), h = mine.item - cb * pg.heads, c0 = cb * COLS, ctx = at_context(a, b);
     // keys [0, limit) are seen; a column behind the last one goes along with it, its query is 0 and nothing of it is stored
-    auto limit_of = [&](int col) { return a.causal ? max(ctx - L + 1 + min(col, G * L - 1) / G, 0) : ctx; };
+    auto limit_of = [&](int col) { return a.causal ? max(ctx - L + 1 + at_div(min(col, G * L - 1), G, a.group_magic), 0) : ctx; };
     const int low = limit_of(c0), end = min(limit_of(c0 + COLS - 1), ctx);
+    const int begin = mine.piece * mine.size, stop = min((end + kF8Tokens - 1) / kF8Tokens, begin + mine.size);
+    const int32_t *table = a.table + static_cast<size_t>(b) * a.max_pages;
+    auto page_at = [&](int blk) { return at_div(blk, a.page_blocks, a.page_magic); };  // the blk-th block's place in the table
+    const int stage_bytes = at_stage(D);
+    unsigned char *ring = sm + warp * kAtStages * stage_bytes;
+    const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+    auto issue = [&](int stage, int blk, int page) {
+        if (blk < stop) at_issue<DIM>(ring_at + stage * stage_bytes, a, h, blk, blk - page_at(blk) * a.page_blocks, page, lane);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto page_of = [&](int blk) {  // by the table's bounds, so that the first ones need not wait for the length
+        const int i = page_at(blk);
+        return i < a.max_pages ? table[i] : -1;
+    };
+    // queries: eight entries a thread, brought to f16 once for all warps
+    static_assert(COLS * DP / 8 <= WARPS * 32, "every entry has a thread");
+    const int qcol = threadIdx.x / (DP / 8), qd = threadIdx.x % (DP / 8) * 8;
+    float x8[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x8[e] = 0.f;
+    if (qcol < COLS && c0 + qcol < G * L && (DIM || qd < D)) {
+        const int l = at_div(c0 + qcol, G, a.group_magic);
+        at_query(static_cast<const T *>(a.q) + b * a.q_b + (static_cast<long long>(h) * G + c0 + qcol - l * G) * a.q_h + l * a.q_l + qd, a.wide_rows, x8);
+    }
+    int at = begin + warp, stage = 0;
+    int pages_of[kAtStages];  // of the blocks in the ring, and of the one that comes next
+#pragma unroll
+    for (int i = 0; i < kAtStages; ++i) pages_of[i] = page_of(at + i * WARPS);
+#pragma unroll
+    for (int i = 0; i < kAtStages - 1; ++i) issue(i, at + i * WARPS, pages_of[i]);
 
-    // queries: column g of n-tile nt, the entries that this lane's key pieces stand for
+    {
+        float m = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = f8_most(m, fabsf(x8[e]));
+#pragma unroll
+        for (int o = 1; o < DP / 8; o <<= 1) m = f8_most(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const int e2 = static_cast<int>(__float_as_uint(m) >> 23);  // 255: no number, whose scores are none either
+        const int up = e2 == 255 ? 0 : min(13 + 127 - e2, 100);      // m * 2^up lies in [2^13, 2^14)
+        const float times = f8_power(up);
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float u = x8[2 * e] * times, w = x8[2 * e + 1] * times;
+            hi[e] = at_pack(u, w);
+            const float2 z = at_rest(hi[e], u, w);
+            lo[e] = at_pack(z.x, z.y);
+        }
+        if (qcol < COLS) {
+            *reinterpret_cast<uint4 *>(q_tile + qcol * QROW + qd) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if constexpr (kTwo) *reinterpret_cast<uint4 *>(q_tile + (COLS + qcol) * QROW + qd) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            if (qd == 0) q_back[qcol] = f8_power(-up);
+        }
+    }
+    __syncthreads();
+    // column g of n-tile nt, the entries that this lane's key pieces stand for
     uint32_t qf[NT][KR][4][2], ql[kTwo ? NT : 1][KR][4][2];
     float factor[NT][2], rest[NT][2];  // of columns 2t and 2t + 1: scores in log2; what its rounding left
     int limit[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int col = c0 + 8 * nt + g;
-        const bool live = col < G * L;
-        const T *q = static_cast<const T *>(a.q) + b * a.q_b + (static_cast<long long>(h) * G + (live ? col % G : 0)) * a.q_h + (live ? col / G : 0) * a.q_l;
-        float x[KR][16], m = 0.f;
-#pragma unroll
-        for (int r = 0; r < KR; ++r) {
-            const int d = (4 * r + t) * 16;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) x[r][e] = live && d < D ? to_f(q[d + e]) : 0.f;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) m = f8_most(m, fabsf(x[r][e]));
-        }
-        m = f8_most(m, __shfl_xor_sync(0xffffffffu, m, 1)), m = f8_most(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const int e2 = static_cast<int>(__float_as_uint(m) >> 23);  // 255: no number, whose scores are none either
-        const int up = e2 == 255 ? 0 : min(13 + 127 - e2, 100);      // m * 2^up lies in [2^13, 2^14)
-        const float times = f8_power(up);
 #pragma unroll
         for (int r = 0; r < KR; ++r)
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float u = x[r][4 * s + 2 * e] * times, w = x[r][4 * s + 2 * e + 1] * times;
-                    qf[nt][r][s][e] = at_pack(u, w);
-                    if constexpr (kTwo) {
-                        const float2 z = at_rest(qf[nt][r][s][e], u, w);
-                        ql[nt][r][s][e] = at_pack(z.x, z.y);
-                    }
+            for (int s = 0; s < 2; ++s) {
+                const uint4 u = *reinterpret_cast<const uint4 *>(q_tile + (8 * nt + g) * QROW + (4 * r + t) * 16 + 8 * s);
+                qf[nt][r][2 * s][0] = u.x, qf[nt][r][2 * s][1] = u.y, qf[nt][r][2 * s + 1][0] = u.z, qf[nt][r][2 * s + 1][1] = u.w;
+                if constexpr (kTwo) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(q_tile + (COLS + 8 * nt + g) * QROW + (4 * r + t) * 16 + 8 * s);
+                    ql[nt][r][2 * s][0] = w.x, ql[nt][r][2 * s][1] = w.y, ql[nt][r][2 * s + 1][0] = w.z, ql[nt][r][2 * s + 1][1] = w.w;
                 }
+            }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const float back = f8_power(-__shfl_sync(0xffffffffu, up, (2 * t + e) * 4));
+            const float back = q_back[8 * nt + 2 * t + e];
             factor[nt][e] = a.scale_log2 * back, rest[nt][e] = a.scale_rest * back;
             limit[nt][e] = limit_of(c0 + 8 * nt + 2 * t + e);
         }
@@ -166,21 +289,18 @@ __global__ void __launch_bounds__(WARPS * 32) fp8_attend_kernel(const __grid_con
         for (int e = 0; e < 2; ++e) m_run[nt][e] = -INFINITY, l_run[nt][e] = 0.f;
     }
 
-    // the cluster's shares of the blocks, then every WARPS-th one
-    const int blocks = (end + kF8Tokens - 1) / kF8Tokens, share = (blocks + ranks - 1) / ranks;
-    const int begin = min(rank * share, blocks), stop = min(begin + share, blocks);
-    const int32_t *table = a.table + static_cast<size_t>(b) * a.max_pages;
-    auto page_of = [&](int blk) { return blk < stop ? table[blk * kF8Tokens / pg.page_size] : -1; };
-    int at = begin + warp;
-    AtBlock<DP> x;
-    int page = page_of(at), page_next = page_of(at + WARPS);
-    if (at < stop) at_load<DP>(x, a, b, h, at * kF8Tokens, page, lane);
     for (; at < stop; at += WARPS) {
-        AtBlock<DP> y = x;
-        const int key0 = at * kF8Tokens, here = page;
-        page = page_next, page_next = page_of(at + 2 * WARPS);
-        if (at + WARPS < stop) at_load<DP>(x, a, b, h, key0 + WARPS * kF8Tokens, page, lane);
-        if (here < 0 || here >= pg.num_pages) continue;
+        const int key0 = at * kF8Tokens, here = pages_of[0], ahead = at + (kAtStages - 1) * WARPS;
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAtStages - 2) : "memory");
+        __syncwarp();  // all lanes' copies of this block are there, and all lanes are through with the block before, whose place is next
+        issue(stage ? stage - 1 : kAtStages - 1, ahead, pages_of[kAtStages - 1]);
+#pragma unroll
+        for (int i = 0; i + 1 < kAtStages; ++i) pages_of[i] = pages_of[i + 1];
+        pages_of[kAtStages - 1] = page_of(ahead + WARPS);
+        const unsigned char *block = ring + stage * stage_bytes;
+        stage = stage + 1 == kAtStages ? 0 : stage + 1;
+        if (static_cast<unsigned>(here) >= static_cast<unsigned>(pg.num_pages)) continue;
+        const float2 scales = *reinterpret_cast<const float2 *>(block + 32 * D);
 
         // scores: rows g and g + 8 (keys), columns 2t and 2t + 1
         float sc[NT][4];
@@ -190,42 +310,82 @@ __global__ void __launch_bounds__(WARPS * 32) fp8_attend_kernel(const __grid_con
             for (int i = 0; i < 4; ++i) sc[nt][i] = 0.f;
 #pragma unroll
         for (int r = 0; r < KR; ++r) {
-            const uint32_t w0[4] = {y.k[0][r].x, y.k[0][r].y, y.k[0][r].z, y.k[0][r].w}, w1[4] = {y.k[1][r].x, y.k[1][r].y, y.k[1][r].z, y.k[1][r].w};
+            const int d = (4 * r + t) * 16;
+            uint4 one = make_uint4(0, 0, 0, 0), two = one;
+            if (DIM || d < D) one = *reinterpret_cast<const uint4 *>(block + at_key<kMoved>(g, D, d)), two = *reinterpret_cast<const uint4 *>(block + at_key<kMoved>(g + 8, D, d));
+            const uint32_t w0[4] = {one.x, one.y, one.z, one.w}, w1[4] = {two.x, two.y, two.z, two.w};
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-                const uint32_t f[4] = {at_half2(w0[s]), at_half2(w1[s]), at_half2(w0[s] >> 16), at_half2(w1[s] >> 16)};
+                uint32_t f[4];
+                at_halves(w0[s], f[0], f[2]), at_halves(w1[s], f[1], f[3]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     if constexpr (kTwo) {  // every product's sum begins anew: the tensor cores cut what they add up, fp32 additions round
-                        float d[4] = {0.f, 0.f, 0.f, 0.f}, c[4] = {0.f, 0.f, 0.f, 0.f};
-                        at_mma(d, f, ql[nt][r][s][0], ql[nt][r][s][1]);
-                        at_mma(c, f, qf[nt][r][s][0], qf[nt][r][s][1]);
+                        float d4[4] = {0.f, 0.f, 0.f, 0.f}, c4[4] = {0.f, 0.f, 0.f, 0.f};
+                        at_mma(d4, f, ql[nt][r][s][0], ql[nt][r][s][1]);
+                        at_mma(c4, f, qf[nt][r][s][0], qf[nt][r][s][1]);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) sc[nt][i] += c[i] + d[i];
+                        for (int i = 0; i < 4; ++i) sc[nt][i] += c4[i] + d4[i];
                     } else {
                         at_mma(sc[nt], f, qf[nt][r][s][0], qf[nt][r][s][1]);
                     }
                 }
             }
         }
-        float most[NT][2];
-        bool grow = false;
-        const bool whole = key0 + kF8Tokens <= low;
+        uint32_t v[4][DP / 32];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = 2 * t + (i & 1) + 4 * (i & 2);
+            if constexpr (DP == 64) {
+                const uint2 w = DIM || g * 8 < D ? *reinterpret_cast<const uint2 *>(block + 16 * D + row * D + g * 8) : make_uint2(0, 0);
+                v[i][0] = w.x, v[i][1] = w.y;
+            } else {
+#pragma unroll
+                for (int c = 0; c < DP / 128; ++c) {
+                    const int d = g * (DP / 8) + 16 * c;
+                    const uint4 w = DIM || d < D ? *reinterpret_cast<const uint4 *>(block + 16 * D + at_value<kMoved>(row, D, d)) : make_uint4(0, 0, 0, 0);
+                    v[i][4 * c] = w.x, v[i][4 * c + 1] = w.y, v[i][4 * c + 2] = w.z, v[i][4 * c + 3] = w.w;
+                }
+            }
+        }
+
+        // scaled to log2, masked scores -inf whatever the factor (which may be no number, 0 or negative)
+        float f[NT][2], x[NT][4], vs[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float f = factor[nt][e] * y.ks;
-                const float u = !whole && key0 + g >= limit[nt][e] ? -INFINITY : sc[nt][e] * f, w = !whole && key0 + g + 8 >= limit[nt][e] ? -INFINITY : sc[nt][2 + e] * f;
-                most[nt][e] = fmaxf(u, w);
-                grow |= most[nt][e] > m_run[nt][e] + kAtLag;
+                f[nt][e] = factor[nt][e] * scales.x, vs[nt][e] = scales.y;
+                x[nt][e] = sc[nt][e] * f[nt][e], x[nt][2 + e] = sc[nt][2 + e] * f[nt][e];
             }
+        if (key0 + kF8Tokens > low) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    if (key0 + g >= limit[nt][e]) x[nt][e] = -INFINITY;
+                    if (key0 + g + 8 >= limit[nt][e]) x[nt][2 + e] = -INFINITY;
+                    if (key0 >= limit[nt][e]) vs[nt][e] = 0.f;  // a column that sees none of the block takes nothing from a scale that is no number
+                }
+            if (key0 + kF8Tokens > ctx) {  // rows behind the last token may hold anything
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (key0 + 2 * t + (i & 1) + 4 * (i & 2) >= ctx)
+#pragma unroll
+                        for (int w = 0; w < DP / 32; ++w) v[i][w] = 0;
+            }
+        }
+        bool grow = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) grow |= fmaxf(x[nt][e], x[nt][2 + e]) > m_run[nt][e] + kAtLag;
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float m = most[nt][e];
+                    float m = fmaxf(x[nt][e], x[nt][2 + e]);
 #pragma unroll
                     for (int w = 4; w < 32; w <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
                     m = fmaxf(m, m_run[nt][e]);
@@ -241,13 +401,12 @@ __global__ void __launch_bounds__(WARPS * 32) fp8_attend_kernel(const __grid_con
             float w[4];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float m = m_run[nt][e] == -INFINITY ? 0.f : m_run[nt][e], f = factor[nt][e] * y.ks;
+                const float m = m_run[nt][e] == -INFINITY ? 0.f : m_run[nt][e];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float s = sc[nt][2 * i + e];
-                    float z = kTwo ? fmaf(s, f, fmaf(s, rest[nt][e] * y.ks, -m)) : fmaf(s, f, -m);
-                    if (!whole && key0 + g + 8 * i >= limit[nt][e]) z = -INFINITY;
-                    w[2 * i + e] = kTwo ? exp2f(z) : at_ex2(z);
+                    const float u = x[nt][2 * i + e], s = sc[nt][2 * i + e];
+                    if constexpr (kTwo) w[2 * i + e] = exp2f(u == -INFINITY ? u : fmaf(s, f[nt][e], fmaf(s, rest[nt][e] * scales.x, -m)));
+                    else w[2 * i + e] = at_ex2(u - m);
                 }
                 l_run[nt][e] += w[e] + w[2 + e];
             }
@@ -261,30 +420,18 @@ __global__ void __launch_bounds__(WARPS * 32) fp8_attend_kernel(const __grid_con
                 p[nt][i] = at_turn(p[nt][i]);
             }
         }
-        if (key0 + kF8Tokens > ctx) {  // rows behind the last token may hold anything
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (key0 + 2 * t + (i & 1) + 4 * (i & 2) >= ctx)
-#pragma unroll
-                    for (int w = 0; w < DP / 32; ++w) y.v[i][w] = 0;
-        }
-        float vs[NT][2];  // a column that sees none of the block takes nothing from a scale that is no number
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) vs[nt][e] = whole || key0 < limit[nt][e] ? y.vs : 0.f;
 #pragma unroll
         for (int j = 0; j < J; ++j) {  // entries 2j (rows g) and 2j + 1 (rows g + 8) of the lanes' eighths
             const uint32_t sel = j & 1 ? 0x7362 : 0x5140;
-            const uint32_t one = __byte_perm(y.v[0][j >> 1], y.v[1][j >> 1], sel), two = __byte_perm(y.v[2][j >> 1], y.v[3][j >> 1], sel);
-            const uint32_t f[4] = {at_half2(one), at_half2(one >> 16), at_half2(two), at_half2(two >> 16)};
+            uint32_t f4[4];
+            at_halves(__byte_perm(v[0][j >> 1], v[1][j >> 1], sel), f4[0], f4[1]), at_halves(__byte_perm(v[2][j >> 1], v[3][j >> 1], sel), f4[2], f4[3]);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float d[4] = {0.f, 0.f, 0.f, 0.f};
-                at_mma(d, f, p[nt][0], p[nt][1]);
+                at_mma(d, f4, p[nt][0], p[nt][1]);
                 if constexpr (kTwo) {
                     float c[4] = {0.f, 0.f, 0.f, 0.f};
-                    at_mma(c, f, pl[nt][0], pl[nt][1]);
+                    at_mma(c, f4, pl[nt][0], pl[nt][1]);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) d[i] = fmaf(c[i], 1.f / 2048.f, d[i]);
                 }
@@ -295,6 +442,9 @@ __global__ void __launch_bounds__(WARPS * 32) fp8_attend_kernel(const __grid_con
     }
 
     // join the warps
+    const int live = min(COLS, G * L - c0);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -304,96 +454,194 @@ __global__ void __launch_bounds__(WARPS * 32) fp8_attend_kernel(const __grid_con
             for (int w = 4; w < 32; w <<= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
             const int col = 8 * nt + 2 * t + e;
             if (g == 0) part_m[warp * COLS + col] = m_run[nt][e], part_l[warp * COLS + col] = l;
-            float *to = part + (static_cast<size_t>(warp) * COLS + col) * DP + g * (DP / 8);
+            if (col < live) {
+                float4 *to = reinterpret_cast<float4 *>(part + (warp * COLS + col) * ROW + g * (DP / 8));
 #pragma unroll
-            for (int j = 0; j < J; ++j) to[2 * j] = o[nt][j][e], to[2 * j + 1] = o[nt][j][2 + e];
+                for (int j = 0; j < J; j += 2) to[j / 2] = make_float4(o[nt][j][e], o[nt][j][2 + e], o[nt][j + 1][e], o[nt][j + 1][2 + e]);
+            }
         }
-    __syncthreads();
-    for (int i = threadIdx.x; i < COLS * DP; i += WARPS * 32) {
-        const int col = i / DP;
-        float m = -INFINITY, v = 0.f;
-        for (int w = 0; w < WARPS; ++w) m = fmaxf(m, part_m[w * COLS + col]);
-        for (int w = 0; w < WARPS; ++w)
-            if (part_l[w * COLS + col] != 0.f) v = fmaf(part[w * COLS * DP + i], m == -INFINITY ? 1.f : at_ex2(part_m[w * COLS + col] - m), v);
-        part[i] = v;
-    }
     __syncthreads();
     if (threadIdx.x < COLS) {
         const int col = threadIdx.x;
         float m = -INFINITY, l = 0.f;
         for (int w = 0; w < WARPS; ++w) m = fmaxf(m, part_m[w * COLS + col]);
-        for (int w = 0; w < WARPS; ++w) l = fmaf(part_l[w * COLS + col], m == -INFINITY ? 1.f : at_ex2(part_m[w * COLS + col] - m), l);
+        for (int w = 0; w < WARPS; ++w) {
+            const float f = part_m[w * COLS + col] == m ? 1.f : at_ex2(part_m[w * COLS + col] - m);
+            part_w[w * COLS + col] = f, l = fmaf(part_l[w * COLS + col], f, l);
+        }
         part_m[col] = m, part_l[col] = l;
     }
-    // join the cluster: each CTA a share of the numbers
-    if (ranks > 1) cluster.sync();
-    else __syncthreads();
-    const int live = min(COLS, G * L - c0), each = (live * D + ranks - 1) / ranks;
-    for (int i = rank * each + threadIdx.x; i < min((rank + 1) * each, live * D); i += WARPS * 32) {
-        const int col = i / D, d = i - col * D;
-        float m = -INFINITY, l = 0.f, v = 0.f;
-        for (int r = 0; r < ranks; ++r) m = fmaxf(m, ranks > 1 ? cluster.map_shared_rank(part_m, r)[col] : part_m[col]);
-        for (int r = 0; r < ranks; ++r) {
-            const float lr = ranks > 1 ? cluster.map_shared_rank(part_l, r)[col] : part_l[col];
-            if (lr == 0.f) continue;
-            const float mr = ranks > 1 ? cluster.map_shared_rank(part_m, r)[col] : part_m[col], w = m == -INFINITY ? 1.f : at_ex2(mr - m);
-            l = fmaf(lr, w, l), v = fmaf((ranks > 1 ? cluster.map_shared_rank(part, r) : part)[col * DP + d], w, v);
+    __syncthreads();
+    for (int i = threadIdx.x; i < live * (DP / 4); i += WARPS * 32) {
+        const int col = i / (DP / 4);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float f = part_w[w * COLS + col];
+            const float4 u = reinterpret_cast<const float4 *>(part + (w * COLS + col) * ROW)[i % (DP / 4)];
+            v.x = fmaf(u.x, f, v.x), v.y = fmaf(u.y, f, v.y), v.z = fmaf(u.z, f, v.z), v.w = fmaf(u.w, f, v.w);
         }
-        const int c = c0 + col;
-        static_cast<T *>(a.out)[((static_cast<size_t>(b) * L + c / G) * a.heads + static_cast<size_t>(h) * G + c % G) * D + d] = from_f<T>(l == 0.f ? 0.f : v / l);
+        reinterpret_cast<float4 *>(part + col * ROW)[i % (DP / 4)] = v;
     }
-    if (ranks > 1) cluster.sync();  // the others may still read this CTA's shared memory
+    __syncthreads();
+    if (mine.pieces > 1) {
+        float *to = static_cast<float *>(a.workspace) + static_cast<size_t>(blockIdx.x) * (COLS * (D + 2));
+        for (int i = threadIdx.x; i < live * (D / 4); i += WARPS * 32)
+            reinterpret_cast<float4 *>(to)[i] = reinterpret_cast<const float4 *>(part + i / (D / 4) * ROW)[i % (D / 4)];
+        if (threadIdx.x < live) to[COLS * D + threadIdx.x] = part_m[threadIdx.x], to[COLS * (D + 1) + threadIdx.x] = part_l[threadIdx.x];
+    } else {
+        for (int i = threadIdx.x; i < live * (D / 4); i += WARPS * 32) {
+            const int col = i / (D / 4), d = i % (D / 4), c = c0 + col;
+            const float4 v = reinterpret_cast<const float4 *>(part + col * ROW)[d];
+            const float inv = part_l[col] == 0.f ? 0.f : 1.f / part_l[col];  // nothing seen: zeros
+            store4(static_cast<T *>(a.out) + ((static_cast<size_t>(b) * L + c / G) * a.heads + static_cast<size_t>(h) * G + c % G) * D + 4 * d,
+                   make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+        }
+    }
 }
 
-template <typename T, int DP, int NT, int WARPS>
-static int attend_launch(F8Attend a, int ranks, cudaStream_t st) {
+// Adds up the pieces of an item that has several.
+constexpr int kAtJoin = 512, kAtJoinColumns = 16;
+template <typename T>
+__global__ void __launch_bounds__(kAtJoin) fp8_attend_join_kernel(const __grid_constant__ F8Attend a, int cols) {
+    extern __shared__ __align__(16) float js[];  // [pieces][cols] maxima, then factors; the threads' sums
+    __shared__ float sums[kAtJoinColumns];
+    const tlb_fp8_pages &pg = a.pages;
+    const int D = pg.dim, G = a.group, L = a.tokens, each = pg.heads * a.col_blocks;
+    const int b = at_div(blockIdx.x, each, a.each_magic), item = static_cast<int>(blockIdx.x) - b * each, cb = at_div(item, pg.heads, a.heads_magic), h = item - cb * pg.heads, c0 = cb * cols;
+    // the lengths are there: this launch begins once the one before it, which makes the pieces, is past its own wait
+    const AtCut cut = at_cut(a);
+    const int pieces = at_pieces(a, cut, b);
+    const long long before = at_before(a, cut, b);
+    tl::griddep_launch();
+    tl::griddep_wait();  // also without work: what follows relies on this launch ending after the one before it
+    if (pieces <= 1) return;
+    const int live = min(cols, G * L - c0), size = cols * (D + 2), quads = live * (D / 4), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const float *ws = static_cast<const float *>(a.workspace) + static_cast<size_t>(before * each + item * pieces) * size;
+    // a column a warp: the maximum over the pieces, their factors
+    for (int col = warp; col < live; col += kAtJoin / 32) {
+        float m = -INFINITY, l = 0.f;
+        for (int k = lane; k < pieces; k += 32) {
+            const float v = ws[static_cast<size_t>(k) * size + cols * D + col];
+            js[k * cols + col] = v, m = fmaxf(m, v);
+        }
+        m = tl::warp_max(m);
+        for (int k = lane; k < pieces; k += 32) {
+            const float v = js[k * cols + col], f = v == m ? 1.f : at_ex2(v - m);
+            js[k * cols + col] = f, l = fmaf(ws[static_cast<size_t>(k) * size + cols * (D + 1) + col], f, l);
+        }
+        l = tl::warp_sum(l);
+        if (lane == 0) sums[col] = l == 0.f ? 0.f : 1.f / l;
+    }
+    __syncthreads();
+    // groups of threads take every groups-th piece
+    const int groups = max(kAtJoin / quads, 1), group = threadIdx.x / quads;
+    float4 *both = reinterpret_cast<float4 *>(js + (pieces * cols + 3) / 4 * 4);
+    for (int q0 = 0; q0 < quads; q0 += kAtJoin) {
+        const int i = groups > 1 ? threadIdx.x % quads : q0 + threadIdx.x, col = i / (D / 4), d = i % (D / 4);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (group < groups && i < quads) {
+#pragma unroll 8
+            for (int k = groups > 1 ? group : 0; k < pieces; k += groups) {
+                const float4 u = reinterpret_cast<const float4 *>(ws + static_cast<size_t>(k) * size)[i];
+                const float f = js[k * cols + col];
+                v.x = fmaf(u.x, f, v.x), v.y = fmaf(u.y, f, v.y), v.z = fmaf(u.z, f, v.z), v.w = fmaf(u.w, f, v.w);
+            }
+        }
+        if (groups > 1) {
+            both[threadIdx.x] = v;
+            __syncthreads();
+            if (group != 0) continue;
+            for (int k = 1; k < groups; ++k) {
+                const float4 u = both[k * quads + i];
+                v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+            }
+        }
+        if (i >= quads) continue;
+        const float inv = sums[col];
+        const int c = c0 + col;
+        store4(static_cast<T *>(a.out) + ((static_cast<size_t>(b) * L + c / G) * a.heads + static_cast<size_t>(h) * G + c % G) * D + 4 * d,
+               make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+    }
+}
+
+// CTAs of the kernels that the GPU holds at a time, as far as the division of the work goes: two an SM, one of the wider forms.
+static int attend_slots(int dtype, int dim, int rows) { return sm_count() * (dtype == TL_BF16 && dim <= 128 && rows <= 8 ? 2 : 1); }
+static int attend_cols(int dim, int rows) { return dim > 128 || rows <= 8 ? 8 : 16; }
+
+// 2^32 / d, rounded up: n / d is the upper half of n times it while n * d < 2^32.
+static unsigned at_magic(unsigned long long most, unsigned d) { return d > 1 && most < (1ull << 32) / d ? static_cast<unsigned>((1ull << 32) / d) + 1 : 0; }
+
+template <typename T, int DP, int DIM, int NT>
+static int attend_launch(F8Attend a, cudaStream_t st) {
     static tl::PerDevice ready;
-    constexpr int cols = 8 * NT, smem = WARPS * cols * (DP + 2) * 4;
-    const auto kernel = fp8_attend_kernel<T, DP, NT, WARPS>;
+    constexpr int cols = 8 * NT, joined = kAtWarps * cols * (DP + 4 + 3) * 4, most = kAtWarps * kAtStages * at_stage(DP);
+    const auto kernel = fp8_attend_kernel<T, DP, DIM, NT>;
+    const int rings = kAtWarps * kAtStages * at_stage(a.pages.dim), smem = rings > joined ? rings : joined;
     int device = 0;
     cudaGetDevice(&device);
-    if (!ready(device, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess; }))
+    if (!ready(device, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most > joined ? most : joined) == cudaSuccess; }))
         return tl::fail(TL_ECUDA, "fp8_attention: %s", cudaGetErrorString(cudaGetLastError()));
     a.col_blocks = (a.group * a.tokens + cols - 1) / cols;
-    const long long ctas = static_cast<long long>(a.col_blocks) * a.pages.heads * a.batch * ranks;
-    if (ctas > 0x7fffffff) return tl::fail(TL_EINVAL, "fp8_attention: sizes out of range");
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(ctas)), cfg.blockDim = dim3(WARPS * 32), cfg.dynamicSmemBytes = smem, cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim = {static_cast<unsigned>(ranks), 1, 1};
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr, cfg.numAttrs = tl::use_pdl() ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+    const long long items = static_cast<long long>(a.col_blocks) * a.pages.heads * a.batch;
+    if (items > 0x3fffffff) return tl::fail(TL_EINVAL, "fp8_attention: sizes out of range");
+    a.each_magic = at_magic(items + a.slots, a.pages.heads * a.col_blocks);
+    cudaError_t e = tl::launch_chained(kernel, dim3(static_cast<unsigned>(items + (a.workspace ? a.slots : 0))), dim3(kAtWarps * 32), smem, st, a);
     if (e != cudaSuccess) return tl::fail(TL_ECUDA, "fp8_attention: %s", cudaGetErrorString(e));
     TL_LAUNCH_CHECK("fp8_attention");
+    if (!a.workspace) return TL_OK;
+    // an item has at most slots + 1 pieces
+    const size_t sums = ((static_cast<size_t>(a.slots) + 1) * cols + 3) / 4 * 16 + kAtJoin * 16;
+    e = tl::launch_chained(fp8_attend_join_kernel<T>, dim3(static_cast<unsigned>(items)), dim3(kAtJoin), sums, st, a, cols);
+    if (e != cudaSuccess) return tl::fail(TL_ECUDA, "fp8_attention: %s", cudaGetErrorString(e));
+    TL_LAUNCH_CHECK("fp8_attention (join)");
     return TL_OK;
 }
 
+template <typename T, int DP, int DIM>
+static int attend_columns(const F8Attend &a, cudaStream_t st) {
+    if constexpr (DP <= 128)
+        if (attend_cols(DP, a.group * a.tokens) == 16) return attend_launch<T, DP, DIM, 2>(a, st);
+    return attend_launch<T, DP, DIM, 1>(a, st);
+}
+
 template <typename T>
-static int attend_any(const F8Attend &a, cudaStream_t st) {
-    const int D = a.pages.dim, rows = a.group * a.tokens;
-    const int nt = D > 128 || rows <= 8 ? 1 : 2;
-    const long long ctas = static_cast<long long>((rows + 8 * nt - 1) / (8 * nt)) * a.pages.heads * a.batch;
-    int ranks = 1;  // as many CTAs as fill the GPU, each with two blocks a warp at the least
-    while (ranks < 8 && ctas * ranks < 2 * sm_count() && a.longest > ranks * 2 * 8 * kF8Tokens) ranks *= 2;
-    if (D <= 64) return nt == 1 ? attend_launch<T, 64, 1, 8>(a, ranks, st) : attend_launch<T, 64, 2, 8>(a, ranks, st);
-    if (D <= 128) return nt == 1 ? attend_launch<T, 128, 1, 8>(a, ranks, st) : attend_launch<T, 128, 2, 8>(a, ranks, st);
-    return attend_launch<T, 256, 1, 8>(a, ranks, st);
+static int attend_any(F8Attend a, cudaStream_t st) {
+    const int D = a.pages.dim;
+    a.wide_rows = tl::aligned16(a.q) && ((a.q_b | a.q_h | a.q_l) * static_cast<long long>(sizeof(T)) & 15) == 0;
+    a.page_blocks = a.pages.page_size / kF8Tokens;
+    a.page_magic = at_magic(static_cast<unsigned long long>(a.max_pages) * a.page_blocks + 64, a.page_blocks);  // the first pages are looked up ahead of the length
+    a.group_magic = at_magic(static_cast<unsigned long long>(a.group) * a.tokens, a.group);
+    a.heads_magic = at_magic(static_cast<unsigned long long>(a.pages.heads) * ((a.group * a.tokens + 7) / 8), a.pages.heads);
+    a.slots = attend_slots(a.dtype, D, a.group * a.tokens);
+    if (D <= 64) return D == 64 ? attend_columns<T, 64, 64>(a, st) : attend_columns<T, 64, 0>(a, st);
+    if (D <= 128) return D == 128 ? attend_columns<T, 128, 128>(a, st) : attend_columns<T, 128, 0>(a, st);
+    return attend_launch<T, 256, 0, 1>(a, st);
 }
 
 }  // namespace tlb
 
 using namespace tlb;
 
-extern "C" int tlb_fp8_attention(const tlb_fp8_pages *pages, const tlb_fp8_attention_call *c, void *stream) {
+extern "C" size_t tlb_fp8_attention_workspace(const tlb_fp8_pages *pages, const tlb_fp8_attention_call *c) {
+    if (f8_check_pages("fp8_attention", pages) != TL_OK || !c || c->heads <= 0 || c->tokens <= 0 || c->batch <= 0) return 0;
+    const long long rows = static_cast<long long>(c->heads / pages->heads) * c->tokens;
+    const int few = rows <= 8 ? 8 : 9, cols = attend_cols(pages->dim, few), slots = attend_slots(c->dtype, pages->dim, few);
+    const long long items = (rows + cols - 1) / cols * pages->heads * c->batch;
+    // requests that can't be long, or more items than any cut would serve
+    if (static_cast<long long>(c->max_pages) * (pages->page_size / kF8Tokens) <= kAtLeast + kAtLeast / 4 || items > 16LL * slots) return 0;
+    return static_cast<size_t>(items + slots) * cols * (pages->dim + 2) * sizeof(float);
+}
+
+extern "C" int tlb_fp8_attention(const tlb_fp8_pages *pages, const tlb_fp8_attention_call *c, void *workspace, size_t workspace_bytes, void *stream) {
     const int rc = f8_check_pages("fp8_attention", pages);
     if (rc != TL_OK) return rc;
     if (!c || c->batch < 0 || c->tokens < 0 || c->heads <= 0 || c->heads % pages->heads) return tl::fail(TL_EINVAL, "fp8_attention: query heads over %d key/value heads", pages->heads);
     if (c->batch == 0 || c->tokens == 0) return TL_OK;
     if (c->max_pages <= 0 || static_cast<long long>(c->heads / pages->heads) * c->tokens > (1 << 30)) return tl::fail(TL_EINVAL, "fp8_attention: sizes out of range");
     if (!c->q || !c->out || !c->table || !c->lens) return tl::fail(TL_EINVAL, "fp8_attention: missing argument");
-    const F8Attend a(*pages, *c);
+    const size_t need = tlb_fp8_attention_workspace(pages, c);
+    if (need && (!workspace || workspace_bytes < need || !tl::aligned16(workspace))) return tl::fail(TL_EWORKSPACE, "fp8_attention: a workspace of %zu bytes is needed", need);
+    const F8Attend a(*pages, *c, need ? workspace : nullptr);
     TLB_DISPATCH(c->dtype, "fp8_attention", return attend_any<T>(a, as_stream(stream)));
 }

@@ -100,7 +100,8 @@ _SIGNATURES = {
     "tlb_fp8_linear": (_I, [_VP, _LL, _VP, _I, _VP, _VP, _VP, _I, _I, _I, _VP, ctypes.c_size_t, _I, _VP]),
     "tlb_fp8_gated_mlp_workspace": (ctypes.c_size_t, [_I, _I, _I]),
     "tlb_fp8_append": (_I, [_VP, ctypes.c_char_p, _VP]),
-    "tlb_fp8_attention": (_I, [_VP, ctypes.c_char_p, _VP]),
+    "tlb_fp8_attention_workspace": (ctypes.c_size_t, [_VP, ctypes.c_char_p]),
+    "tlb_fp8_attention": (_I, [_VP, ctypes.c_char_p, _VP, ctypes.c_size_t, _VP]),
     "tlb_fp8_gated_mlp": (_I, [_VP, _LL, _VP, _I, _VP, _VP, _I, _VP, _VP, _I, _I, _I, _I, _F, _F, _VP, ctypes.c_size_t, _I, _VP]),
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -1189,7 +1190,7 @@ class Fp8Pages(ctypes.Structure):
 
 # tlb_fp8_append_call and tlb_fp8_attention_call, packed at once: of small calls the host sets the pace, and ctypes converts two dozen arguments one by one
 _FP8_APPEND = struct.Struct("@PPPPPPPPqqqqqqqqqdffiiiiiii")
-_FP8_ATTENTION = struct.Struct("@PPPPPqqqdiiiiiii")
+_FP8_ATTENTION = struct.Struct("@PPPPqqqdiiiiii")
 
 
 def _fp8_step(op: str, pages: Fp8Pages, device: int, table: torch.Tensor, lens: torch.Tensor, *tensors) -> None:
@@ -1240,22 +1241,25 @@ def fp8_append_of(pages: Fp8Pages, device: int, q, k, v, table, lens, q_norm=Non
     return out.transpose(1, 2)
 
 
-def fp8_attention(pages: Fp8Pages, device: int, q: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, longest: int, scale: float, causal: bool) -> torch.Tensor:
+def fp8_attention(pages: Fp8Pages, device: int, q: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, scale: float, causal: bool) -> torch.Tensor:
     """``tlb_fp8_attention``: ``q [B, H, L, dim]`` -> the same shape (laid out token by token)."""
     _fp8_step("fp8_attention", pages, device, table, lens, q)
-    return fp8_attention_of(pages, device, q, table, lens, longest, scale, causal)
+    return fp8_attention_of(pages, device, q, table, lens, scale, causal)
 
 
-def fp8_attention_of(pages: Fp8Pages, device: int, q, table, lens, longest, scale, causal) -> torch.Tensor:
+def fp8_attention_of(pages: Fp8Pages, device: int, q, table, lens, scale, causal) -> torch.Tensor:
     """``fp8_attention`` of tensors that the caller has checked (``paged_attention_fp8``)."""
     if _current_device() != device:
         with torch.cuda.device(device):
-            return fp8_attention_of(pages, device, q, table, lens, longest, scale, causal)
+            return fp8_attention_of(pages, device, q, table, lens, scale, causal)
     B, H, L, D = q.shape
     out = q.new_empty((B, L, H, D))
     qb, qh, ql, _ = q.stride()
-    call = _FP8_ATTENTION.pack(q.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(), 0, qb, qh, ql, scale, B, H, L, table.shape[1], longest, causal, _code(q.dtype))
-    rc = library().tlb_fp8_attention(ctypes.addressof(pages), call, _raw_stream(device))
+    call = _FP8_ATTENTION.pack(q.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(), qb, qh, ql, scale, B, H, L, table.shape[1], causal, _code(q.dtype))
+    lib, at = library(), ctypes.addressof(pages)
+    size = lib.tlb_fp8_attention_workspace(at, call)
+    scratch = q.new_empty(size, dtype=torch.uint8) if size else None
+    rc = lib.tlb_fp8_attention(at, call, _ptr(scratch), size, _raw_stream(device))
     if rc:
         _check(rc)
     return out.transpose(1, 2)
