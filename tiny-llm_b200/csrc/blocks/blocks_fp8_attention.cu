@@ -20,16 +20,6 @@
 
 namespace tlb {
 
-constexpr float kAtLag = 8.f;  // log2: how far a running maximum may lag behind
-
-__device__ __forceinline__ float at_ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ void at_halves(uint32_t four, uint32_t &lo, uint32_t &hi) {  // four e4m3 numbers as f16
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(four));
-}
 __device__ __forceinline__ uint32_t at_turn(uint32_t v) {  // an 8 x 8 matrix of f16, transposed
     uint32_t r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -47,7 +37,6 @@ __device__ __forceinline__ float2 at_rest(uint32_t two, float lo, float hi) {  /
 }
 
 constexpr int kAtWarps = 8, kAtStages = 3;
-constexpr int kAtLeast = 32;  // blocks of a piece at the least
 
 __device__ __forceinline__ void at_copy16(uint32_t to, const void *from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
 __device__ __forceinline__ void at_copy4(uint32_t to, const void *from) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory"); }
@@ -82,96 +71,6 @@ __device__ __forceinline__ void at_issue(uint32_t stage, const F8Attend &a, int 
         }
     }
     if (lane < 2) at_copy4(stage + 32 * D + 4 * lane, (lane ? pg.value_scales : pg.key_scales) + block);
-}
-
-// n / d by a product; magic 0: where that might be off.
-__device__ __forceinline__ int at_div(int n, int d, unsigned magic) { return magic ? static_cast<int>(__umulhi(n, magic)) : n / d; }
-
-// 8 entries of a query
-template <typename T>
-__device__ __forceinline__ void at_query(const T *q, bool wide, float (&x)[8]) {
-    if (wide) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const float4 v = load4(q + 4 * i);
-            x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = to_f(q[e]);
-    }
-}
-
-__device__ __forceinline__ int at_context(const F8Attend &a, int b) {
-    return static_cast<int>(max(0LL, min(static_cast<long long>(a.lens[b]), static_cast<long long>(a.max_pages) * a.pages.page_size)));
-}
-__device__ __forceinline__ int at_blocks(const F8Attend &a, int b) { return (at_context(a, b) + kF8Tokens - 1) / kF8Tokens; }
-
-// How long a piece of an item may be, in blocks: such that the pieces are about as many as the CTAs that the GPU holds at a time, or the items and half of those.  A piece
-// costs its CTA some microseconds beside its blocks, so it has kAtLeast of them.  Nothing here depends on how many idle slots there are: a step over more of
-// them is cut the same way, to the bit.  Whole warps; 0: nothing is cut.
-typedef int AtCut;
-__device__ __forceinline__ AtCut at_cut(const F8Attend &a) {
-    if (!a.workspace) return 0;
-    int total = 0, live = 0;  // at most 2^27 blocks a request
-    long long all = 0;
-    for (int r = threadIdx.x & 31; r < a.batch; r += 32) {
-        const int n = at_blocks(a, r);
-        all += n, live += n > 0;
-    }
-    total = static_cast<int>(min(all, 0x3ffffffLL));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o), live += __shfl_xor_sync(0xffffffffu, live, o);
-    const int each = a.pages.heads * a.col_blocks, room = max(a.slots - live * each, a.slots / 2);
-    return static_cast<int>(max(min((static_cast<long long>(total) * each + room - 1) / room, 0x3fffffffLL), static_cast<long long>(kAtLeast)));
-}
-__device__ __forceinline__ int at_pieces(const F8Attend &a, AtCut cut, int b) {
-    const int n = at_blocks(a, b);
-    return cut == 0 || n <= cut + cut / 4 ? 1 : (n + cut - 1) / cut;  // a quarter more is no reason to cut
-}
-// pieces of a head's eight (or sixteen) columns, over the requests before `request`
-__device__ __forceinline__ long long at_before(const F8Attend &a, AtCut cut, int request) {
-    int n = 0;
-    for (int r = threadIdx.x & 31; r < request; r += 32) n += at_pieces(a, cut, r);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    return n;
-}
-
-// The index-th piece: a request's items one after another, an item's pieces side by side.
-struct AtPiece {
-    int b, item, piece, pieces, size;  // size: blocks of a piece; b < 0: there are not so many
-};
-__device__ __forceinline__ AtPiece at_piece(const F8Attend &a, int index) {
-    const int each = a.pages.heads * a.col_blocks, lane = threadIdx.x & 31;
-    const AtCut cut = at_cut(a);
-    AtPiece x{-1, 0, 0, 1, 0x3fffffff};
-    if (cut == 0) {
-        x.b = at_div(index, each, a.each_magic), x.item = index - x.b * each;
-        return x;
-    }
-    const int want = at_div(index, each, a.each_magic);  // rounded down: an item's pieces over all items of a request are a multiple of them
-    int run = 0;
-    for (int r0 = 0; r0 < a.batch; r0 += 32) {
-        const int mine = r0 + lane < a.batch ? at_pieces(a, cut, r0 + lane) : 0;
-        int upto = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int below = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += below;
-        }
-        const unsigned past = __ballot_sync(0xffffffffu, want < run + upto);
-        if (past) {
-            const int src = __ffs(past) - 1;
-            x.b = r0 + src, x.pieces = __shfl_sync(0xffffffffu, mine, src);
-            const int at = index - (run + __shfl_sync(0xffffffffu, upto - mine, src)) * each;
-            x.item = at / x.pieces, x.piece = at % x.pieces;
-            if (x.pieces > 1) x.size = (at_blocks(a, x.b) + x.pieces - 1) / x.pieces;
-            return x;
-        }
-        run += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    return x;
 }
 
 // DP: entries of a head that the lanes' shares make room for; DIM: entries it has, 0: fewer than DP.
@@ -491,44 +390,47 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
         if (threadIdx.x < live) to[COLS * D + threadIdx.x] = part_m[threadIdx.x], to[COLS * (D + 1) + threadIdx.x] = part_l[threadIdx.x];
     } else {
         for (int i = threadIdx.x; i < live * (D / 4); i += WARPS * 32) {
-            const int col = i / (D / 4), d = i % (D / 4), c = c0 + col;
+            const int col = i / (D / 4), d = i % (D / 4), c = c0 + col, l = at_div(c, G, a.group_magic);
             const float4 v = reinterpret_cast<const float4 *>(part + col * ROW)[d];
             const float inv = part_l[col] == 0.f ? 0.f : 1.f / part_l[col];  // nothing seen: zeros
-            store4(static_cast<T *>(a.out) + ((static_cast<size_t>(b) * L + c / G) * a.heads + static_cast<size_t>(h) * G + c % G) * D + 4 * d,
+            store4(static_cast<T *>(a.out) + ((static_cast<size_t>(b) * L + l) * a.heads + static_cast<size_t>(h) * G + c - l * G) * D + 4 * d,
                    make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
         }
     }
 }
 
-// Adds up the pieces of an item that has several.
+// Adds up the pieces of an item that has several, up to 16 of its columns a CTA.
 constexpr int kAtJoin = 512, kAtJoinColumns = 16;
 template <typename T>
 __global__ void __launch_bounds__(kAtJoin) fp8_attend_join_kernel(const __grid_constant__ F8Attend a, int cols) {
-    extern __shared__ __align__(16) float js[];  // [pieces][cols] maxima, then factors; the threads' sums
+    extern __shared__ __align__(16) float js[];  // [pieces][16] maxima, then factors; the threads' sums
     __shared__ float sums[kAtJoinColumns];
     const tlb_fp8_pages &pg = a.pages;
-    const int D = pg.dim, G = a.group, L = a.tokens, each = pg.heads * a.col_blocks;
-    const int b = at_div(blockIdx.x, each, a.each_magic), item = static_cast<int>(blockIdx.x) - b * each, cb = at_div(item, pg.heads, a.heads_magic), h = item - cb * pg.heads, c0 = cb * cols;
+    const int D = pg.dim, G = a.group, L = a.tokens, each = pg.heads * a.col_blocks, skip = blockIdx.y * kAtJoinColumns;
+    const int b = at_div(blockIdx.x, each, a.each_magic), item = static_cast<int>(blockIdx.x) - b * each, cb = at_div(item, pg.heads, a.heads_magic), h = item - cb * pg.heads;
+    const int c0 = cb * cols + skip;
     // the lengths are there: this launch begins once the one before it, which makes the pieces, is past its own wait
     const AtCut cut = at_cut(a);
     const int pieces = at_pieces(a, cut, b);
     const long long before = at_before(a, cut, b);
     tl::griddep_launch();
     tl::griddep_wait();  // also without work: what follows relies on this launch ending after the one before it
-    if (pieces <= 1) return;
-    const int live = min(cols, G * L - c0), size = cols * (D + 2), quads = live * (D / 4), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const float *ws = static_cast<const float *>(a.workspace) + static_cast<size_t>(before * each + item * pieces) * size;
+    const int live = min(min(cols - skip, kAtJoinColumns), G * L - c0);
+    if (pieces <= 1 || live <= 0) return;
+    const int size = cols * (D + 2), quads = live * (D / 4), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const float *ws = static_cast<const float *>(a.workspace) + static_cast<size_t>(before * each + static_cast<long long>(item) * pieces) * size;
+    const float *maxima = ws + static_cast<size_t>(cols) * D + skip, *parts = maxima + cols;
     // a column a warp: the maximum over the pieces, their factors
     for (int col = warp; col < live; col += kAtJoin / 32) {
         float m = -INFINITY, l = 0.f;
         for (int k = lane; k < pieces; k += 32) {
-            const float v = ws[static_cast<size_t>(k) * size + cols * D + col];
-            js[k * cols + col] = v, m = fmaxf(m, v);
+            const float v = maxima[static_cast<size_t>(k) * size + col];
+            js[k * kAtJoinColumns + col] = v, m = fmaxf(m, v);
         }
         m = tl::warp_max(m);
         for (int k = lane; k < pieces; k += 32) {
-            const float v = js[k * cols + col], f = v == m ? 1.f : at_ex2(v - m);
-            js[k * cols + col] = f, l = fmaf(ws[static_cast<size_t>(k) * size + cols * (D + 1) + col], f, l);
+            const float v = js[k * kAtJoinColumns + col], f = v == m ? 1.f : at_ex2(v - m);
+            js[k * kAtJoinColumns + col] = f, l = fmaf(parts[static_cast<size_t>(k) * size + col], f, l);
         }
         l = tl::warp_sum(l);
         if (lane == 0) sums[col] = l == 0.f ? 0.f : 1.f / l;
@@ -536,15 +438,16 @@ __global__ void __launch_bounds__(kAtJoin) fp8_attend_join_kernel(const __grid_c
     __syncthreads();
     // groups of threads take every groups-th piece
     const int groups = max(kAtJoin / quads, 1), group = threadIdx.x / quads;
-    float4 *both = reinterpret_cast<float4 *>(js + (pieces * cols + 3) / 4 * 4);
+    const float *numbers = ws + static_cast<size_t>(skip) * D;
+    float4 *both = reinterpret_cast<float4 *>(js + pieces * kAtJoinColumns);
     for (int q0 = 0; q0 < quads; q0 += kAtJoin) {
         const int i = groups > 1 ? threadIdx.x % quads : q0 + threadIdx.x, col = i / (D / 4), d = i % (D / 4);
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         if (group < groups && i < quads) {
 #pragma unroll 8
             for (int k = groups > 1 ? group : 0; k < pieces; k += groups) {
-                const float4 u = reinterpret_cast<const float4 *>(ws + static_cast<size_t>(k) * size)[i];
-                const float f = js[k * cols + col];
+                const float4 u = reinterpret_cast<const float4 *>(numbers + static_cast<size_t>(k) * size)[i];
+                const float f = js[k * kAtJoinColumns + col];
                 v.x = fmaf(u.x, f, v.x), v.y = fmaf(u.y, f, v.y), v.z = fmaf(u.z, f, v.z), v.w = fmaf(u.w, f, v.w);
             }
         }
@@ -557,20 +460,28 @@ __global__ void __launch_bounds__(kAtJoin) fp8_attend_join_kernel(const __grid_c
                 v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
             }
         }
-        if (i >= quads) continue;
+        if (i >= quads || (groups == 1 && group > 0 && quads <= kAtJoin)) continue;
         const float inv = sums[col];
-        const int c = c0 + col;
-        store4(static_cast<T *>(a.out) + ((static_cast<size_t>(b) * L + c / G) * a.heads + static_cast<size_t>(h) * G + c % G) * D + 4 * d,
+        const int c = c0 + col, l = at_div(c, G, a.group_magic);
+        store4(static_cast<T *>(a.out) + ((static_cast<size_t>(b) * L + l) * a.heads + static_cast<size_t>(h) * G + c - l * G) * D + 4 * d,
                make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
     }
+}
+
+int f8_attend_join(const F8Attend &a, int cols, cudaStream_t st) {
+    const unsigned items = static_cast<unsigned>(a.col_blocks) * a.pages.heads * a.batch;
+    const size_t sums = static_cast<size_t>(a.most_pieces + 1) * kAtJoinColumns * 4 + kAtJoin * 16;
+    const dim3 grid(items, (cols + kAtJoinColumns - 1) / kAtJoinColumns);
+    const cudaError_t e = a.dtype == TL_F32 ? tl::launch_chained(fp8_attend_join_kernel<float>, grid, dim3(kAtJoin), sums, st, a, cols)
+                                            : tl::launch_chained(fp8_attend_join_kernel<bf16>, grid, dim3(kAtJoin), sums, st, a, cols);
+    if (e != cudaSuccess) return tl::fail(TL_ECUDA, "fp8_attention: %s", cudaGetErrorString(e));
+    TL_LAUNCH_CHECK("fp8_attention (join)");
+    return TL_OK;
 }
 
 // CTAs of the kernels that the GPU holds at a time, as far as the division of the work goes: two an SM, one of the wider forms.
 static int attend_slots(int dtype, int dim, int rows) { return sm_count() * (dtype == TL_BF16 && dim <= 128 && rows <= 8 ? 2 : 1); }
 static int attend_cols(int dim, int rows) { return dim > 128 || rows <= 8 ? 8 : 16; }
-
-// 2^32 / d, rounded up: n / d is the upper half of n times it while n * d < 2^32.
-static unsigned at_magic(unsigned long long most, unsigned d) { return d > 1 && most < (1ull << 32) / d ? static_cast<unsigned>((1ull << 32) / d) + 1 : 0; }
 
 template <typename T, int DP, int DIM, int NT>
 static int attend_launch(F8Attend a, cudaStream_t st) {
@@ -590,12 +501,7 @@ static int attend_launch(F8Attend a, cudaStream_t st) {
     if (e != cudaSuccess) return tl::fail(TL_ECUDA, "fp8_attention: %s", cudaGetErrorString(e));
     TL_LAUNCH_CHECK("fp8_attention");
     if (!a.workspace) return TL_OK;
-    // an item has at most slots + 1 pieces
-    const size_t sums = ((static_cast<size_t>(a.slots) + 1) * cols + 3) / 4 * 16 + kAtJoin * 16;
-    e = tl::launch_chained(fp8_attend_join_kernel<T>, dim3(static_cast<unsigned>(items)), dim3(kAtJoin), sums, st, a, cols);
-    if (e != cudaSuccess) return tl::fail(TL_ECUDA, "fp8_attention: %s", cudaGetErrorString(e));
-    TL_LAUNCH_CHECK("fp8_attention (join)");
-    return TL_OK;
+    return f8_attend_join(a, cols, st);
 }
 
 template <typename T, int DP, int DIM>
@@ -613,7 +519,8 @@ static int attend_any(F8Attend a, cudaStream_t st) {
     a.page_magic = at_magic(static_cast<unsigned long long>(a.max_pages) * a.page_blocks + 64, a.page_blocks);  // the first pages are looked up ahead of the length
     a.group_magic = at_magic(static_cast<unsigned long long>(a.group) * a.tokens, a.group);
     a.heads_magic = at_magic(static_cast<unsigned long long>(a.pages.heads) * ((a.group * a.tokens + 7) / 8), a.pages.heads);
-    a.slots = attend_slots(a.dtype, D, a.group * a.tokens);
+    a.slots = attend_slots(a.dtype, D, a.group * a.tokens), a.most_pieces = 128;
+    if (f8_portion_takes(a.pages, a)) return f8_portion(a, st);
     if (D <= 64) return D == 64 ? attend_columns<T, 64, 64>(a, st) : attend_columns<T, 64, 0>(a, st);
     if (D <= 128) return D == 128 ? attend_columns<T, 128, 128>(a, st) : attend_columns<T, 128, 0>(a, st);
     return attend_launch<T, 256, 0, 1>(a, st);
@@ -626,11 +533,12 @@ using namespace tlb;
 extern "C" size_t tlb_fp8_attention_workspace(const tlb_fp8_pages *pages, const tlb_fp8_attention_call *c) {
     if (f8_check_pages("fp8_attention", pages) != TL_OK || !c || c->heads <= 0 || c->tokens <= 0 || c->batch <= 0) return 0;
     const long long rows = static_cast<long long>(c->heads / pages->heads) * c->tokens;
-    const int few = rows <= 8 ? 8 : 9, cols = attend_cols(pages->dim, few), slots = attend_slots(c->dtype, pages->dim, few);
+    const bool portion = f8_portion_takes(*pages, *c);
+    const int few = rows <= 8 ? 8 : 9, cols = portion ? kPoRows : attend_cols(pages->dim, few), slots = portion ? 2 * sm_count() : attend_slots(c->dtype, pages->dim, few);
     const long long items = (rows + cols - 1) / cols * pages->heads * c->batch;
-    // requests that can't be long, or more items than any cut would serve
-    if (static_cast<long long>(c->max_pages) * (pages->page_size / kF8Tokens) <= kAtLeast + kAtLeast / 4 || items > 16LL * slots) return 0;
-    return static_cast<size_t>(items + slots) * cols * (pages->dim + 2) * sizeof(float);
+    // requests that can't be long, or more items than a cut would serve
+    if (static_cast<long long>(c->max_pages) * (pages->page_size / kF8Tokens) <= kAtLeast + kAtLeast / 4 || items > (portion ? 1LL : 16LL) * slots) return 0;
+    return static_cast<size_t>(items + slots) * at_piece_floats(cols, pages->dim) * sizeof(float);
 }
 
 extern "C" int tlb_fp8_attention(const tlb_fp8_pages *pages, const tlb_fp8_attention_call *c, void *workspace, size_t workspace_bytes, void *stream) {

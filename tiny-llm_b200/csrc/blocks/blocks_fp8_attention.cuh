@@ -10,15 +10,132 @@ struct F8Attend : tlb_fp8_attention_call {
     void *workspace;
     int group, col_blocks;  // query heads of a key/value head; items of a head: its columns by eights or sixteens
     int slots;              // CTAs that the GPU holds at a time
+    int most_pieces;        // of an item
+    int granule;            // pieces are a multiple of so many blocks
     int page_blocks;        // blocks of 16 tokens in a page
     unsigned page_magic, group_magic, heads_magic, each_magic;  // for divisions by page_blocks, group, heads and the items of a request (at_div)
     bool wide_rows;         // query rows may be read 16 bytes at a time
     float scale_log2, scale_rest;  // scale * log2(e), and what its rounding to fp32 left
     F8Attend(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c, void *ws)
-        : tlb_fp8_attention_call(c), pages(p), workspace(ws), group(c.heads / p.heads), col_blocks(0), slots(0), page_blocks(1), page_magic(0), group_magic(0), heads_magic(0), each_magic(0), wide_rows(false) {
+        : tlb_fp8_attention_call(c), pages(p), workspace(ws), group(c.heads / p.heads), col_blocks(0), slots(0), most_pieces(1), granule(1), page_blocks(1), page_magic(0), group_magic(0), heads_magic(0), each_magic(0), wide_rows(false) {
         const double log2 = c.scale * 1.4426950408889634;
         scale_log2 = static_cast<float>(log2), scale_rest = static_cast<float>(log2 - scale_log2);
     }
 };
+
+constexpr float kAtLag = 8.f;   // log2: how far a running maximum may lag behind
+constexpr int kAtLeast = 32;    // blocks of a piece at the least
+
+__device__ __forceinline__ float at_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void at_halves(uint32_t four, uint32_t &lo, uint32_t &hi) {  // four e4m3 numbers as f16
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(four));
+}
+// n / d by a product; magic 0: where that might be off.
+__device__ __forceinline__ int at_div(int n, int d, unsigned magic) { return magic ? static_cast<int>(__umulhi(n, magic)) : n / d; }
+
+// 8 entries of a query
+template <typename T>
+__device__ __forceinline__ void at_query(const T *q, bool wide, float (&x)[8]) {
+    if (wide) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float4 v = load4(q + 4 * i);
+            x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = to_f(q[e]);
+    }
+}
+
+__device__ __forceinline__ int at_context(const F8Attend &a, int b) {
+    return static_cast<int>(max(0LL, min(static_cast<long long>(a.lens[b]), static_cast<long long>(a.max_pages) * a.pages.page_size)));
+}
+__device__ __forceinline__ int at_blocks(const F8Attend &a, int b) { return (at_context(a, b) + kF8Tokens - 1) / kF8Tokens; }
+
+// How long a piece of an item may be, in blocks: such that the pieces are about as many as the CTAs that the GPU holds at a time, or the items and half of those.  A piece
+// costs its CTA some microseconds beside its blocks, so it has kAtLeast of them.  Nothing here depends on how many idle slots there are: a step over more of
+// them is cut the same way, to the bit.  Whole warps; 0: nothing is cut.
+typedef int AtCut;
+__device__ __forceinline__ AtCut at_cut(const F8Attend &a) {
+    if (!a.workspace) return 0;
+    int live = 0, longest = 0;  // at most 2^27 blocks a request
+    long long all = 0;
+    for (int r = threadIdx.x & 31; r < a.batch; r += 32) {
+        const int n = at_blocks(a, r);
+        all += n, live += n > 0, longest = max(longest, n);
+    }
+    int total = static_cast<int>(min(all, 0x3ffffffLL));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        total += __shfl_xor_sync(0xffffffffu, total, o), live += __shfl_xor_sync(0xffffffffu, live, o);
+        longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+    }
+    const int each = a.pages.heads * a.col_blocks, room = max(a.slots - live * each, a.slots / 2);
+    const int mean = static_cast<int>(min((static_cast<long long>(total) * each + room - 1) / room, 0x3fffffffLL));
+    return max(max(mean, (longest + a.most_pieces - 1) / a.most_pieces), kAtLeast);
+}
+__device__ __forceinline__ int at_pieces(const F8Attend &a, AtCut cut, int b) {
+    const int n = at_blocks(a, b);
+    return cut == 0 || n <= cut + cut / 4 ? 1 : (n + cut - 1) / cut;  // a quarter more is no reason to cut
+}
+// pieces of a head's eight (or sixteen) columns, over the requests before `request`
+__device__ __forceinline__ long long at_before(const F8Attend &a, AtCut cut, int request) {
+    int n = 0;
+    for (int r = threadIdx.x & 31; r < request; r += 32) n += at_pieces(a, cut, r);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    return n;
+}
+
+// The index-th piece: a request's items one after another, an item's pieces side by side.
+struct AtPiece {
+    int b, item, piece, pieces, size;  // size: blocks of a piece; b < 0: there are not so many
+};
+__device__ __forceinline__ AtPiece at_piece(const F8Attend &a, int index) {
+    const int each = a.pages.heads * a.col_blocks, lane = threadIdx.x & 31;
+    const AtCut cut = at_cut(a);
+    AtPiece x{-1, 0, 0, 1, 0x3fffffff};
+    if (cut == 0) {
+        x.b = at_div(index, each, a.each_magic), x.item = index - x.b * each;
+        return x;
+    }
+    const int want = at_div(index, each, a.each_magic);  // rounded down: an item's pieces over all items of a request are a multiple of them
+    int run = 0;
+    for (int r0 = 0; r0 < a.batch; r0 += 32) {
+        const int mine = r0 + lane < a.batch ? at_pieces(a, cut, r0 + lane) : 0;
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int below = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += below;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, want < run + upto);
+        if (past) {
+            const int src = __ffs(past) - 1;
+            x.b = r0 + src, x.pieces = __shfl_sync(0xffffffffu, mine, src);
+            const int at = index - (run + __shfl_sync(0xffffffffu, upto - mine, src)) * each;
+            x.item = at / x.pieces, x.piece = at % x.pieces;
+            if (x.pieces > 1) x.size = ((at_blocks(a, x.b) + x.pieces - 1) / x.pieces + a.granule - 1) / a.granule * a.granule;  // the last may come out empty
+            return x;
+        }
+        run += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return x;
+}
+
+// blocks_fp8_attention.cu: adds up the pieces of the launch in front, items of `cols` columns each.
+int f8_attend_join(const F8Attend &a, int cols, cudaStream_t st);
+// 2^32 / d, rounded up: n / d is the upper half of n times it while n * d < 2^32; 0 where `most`, the largest n, is too large for that.
+static inline unsigned at_magic(unsigned long long most, unsigned d) { return d > 1 && most < (1ull << 32) / d ? static_cast<unsigned>((1ull << 32) / d) + 1 : 0; }
+__host__ __device__ static inline size_t at_piece_floats(int cols, int dim) { return static_cast<size_t>(cols) * (dim + 2); }
+// blocks_fp8_portion.cu: bf16 queries of many columns
+constexpr int kPoRows = 128;
+bool f8_portion_takes(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c);
+int f8_portion(F8Attend a, cudaStream_t st);
 
 }  // namespace tlb

@@ -1,0 +1,405 @@
+// Attention of many columns (prompt portions) over pages of 8 bits on the 5th-generation tensor cores, bf16 queries, heads of 64 or 128 entries.
+//
+// The arithmetic is that of blocks_fp8_attention.cu; the operands of both products are f16 here too, so that nothing is lost ahead of the weights' rounding (2^-12):
+// a query row is brought to the top of f16's range by a power of two, keys and values are their e4m3 numbers times their block's scale over the largest
+// scale of the CTA's blocks - exact down to 2^-15 of that, and below it off by at most 2^-34 of the largest block's numbers.  A block whose
+// scale is no number counts as zeros in the products, and the rows that see it are made NaN at the end.
+//
+// A CTA takes 128 columns (rows of the products, tensor-memory lanes) of one request and key/value head, or a piece of their keys; two CTAs share an SM, so that one's
+// exponentials run beside the other's products.  Per 64 keys:
+//   warps 5, 6  bring keys and values from the pages into f16 operand tiles (128-byte swizzle) of two stages each, the next tile's bytes on their way in registers meanwhile
+//   warp 4      tcgen05.mma, one elected lane: S = Q K^T into one of two score buffers, O += P V; the next tile's scores are issued ahead of this tile's values
+//   warps 0-3   softmax, thread = row: scores from tensor memory, 2^x of them over a running maximum that may lag behind by 2^8, P as f16 back over its own scores
+#include "../per_device.h"
+#include "blocks_fp8_attention.cuh"
+#include "blocks_tc.cuh"
+
+namespace tlb {
+
+using tl::g_fence_proxy_async;
+using tl::g_tmem_ld32;
+using tl::g_tmem_ld32_nowait;
+using tl::g_tmem_ld_wait;
+using tl::g_tmem_st32;
+using tl::g_tmem_st_wait;
+
+constexpr int kPoKeys = 64;
+constexpr int kPoThreads = 7 * 32;
+constexpr int kPoColumns = 256;  // of tensor memory: two score buffers of 64, the output from 128 on
+constexpr uint32_t kPoOut = 128;
+
+// kind::f16, f16 x f16 -> f32, 128 rows
+__host__ __device__ constexpr uint32_t po_idesc(int n, bool b_mn) { return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24); }
+
+template <int DIM>
+struct PoShape {
+    static constexpr int halves = DIM / 64;                                // 64-column blocks
+    static constexpr int q_block = kPoRows * 128, kv_block = kPoKeys * 128;  // bytes
+    static constexpr int k_off = halves * q_block, v_off = k_off + 2 * halves * kv_block, bar_off = v_off + 2 * halves * kv_block;
+    static constexpr int row_off = bar_off + 256, smem = row_off + kPoRows * 4;
+};
+
+// 16 e4m3 numbers (entries 16 c .. of a row) times `ratio`, as f16, into their places in a tile of 64-column blocks.
+template <int DIM>
+__device__ __forceinline__ void po_store(unsigned char *tile, int row, int c, uint4 raw, __half2 ratio, bool live) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    uint32_t f[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        at_halves(w[i], f[2 * i], f[2 * i + 1]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const __half2 v = __hmul2(*reinterpret_cast<__half2 *>(&f[2 * i + e]), ratio);
+            f[2 * i + e] = live ? *reinterpret_cast<const uint32_t *>(&v) : 0u;  // slots behind the last token may hold anything
+        }
+    }
+    unsigned char *at = tile + (c >> 2) * PoShape<DIM>::kv_block + row * 128;
+    const int j = 2 * (c & 3), odd = (c >> 2) & 1;  // the second block's lanes write their second half first: eight lanes meet all banks
+    const uint4 one = make_uint4(f[0], f[1], f[2], f[3]), two = make_uint4(f[4], f[5], f[6], f[7]);
+    *reinterpret_cast<uint4 *>(at + (((j + odd) ^ (row & 7)) << 4)) = odd ? two : one;
+    *reinterpret_cast<uint4 *>(at + (((j + 1 - odd) ^ (row & 7)) << 4)) = odd ? one : two;
+}
+
+template <int DIM>
+__global__ void __launch_bounds__(kPoThreads, 2) fp8_portion_kernel(const __grid_constant__ F8Attend a) {
+    using Z = PoShape<DIM>;
+    constexpr int CH = DIM / 16, PER = kPoKeys * CH / 64;  // 16-byte pieces of a row; of a tile's side, a converting thread's
+    extern __shared__ __align__(1024) unsigned char psm[];
+    tl::griddep_wait();
+    tl::griddep_launch();  // behind the wait: the launch that joins the pieces reads the lengths ahead of its own
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const tlb_fp8_pages &pg = a.pages;
+    const int G = a.group, L = a.tokens, columns = G * L;
+    const int index = static_cast<int>(gridDim.x - 1 - blockIdx.x);  // late columns, which see most, first
+    const AtPiece mine = at_piece(a, index);
+    if (mine.b < 0) return;
+    const int b = mine.b, cb = at_div(mine.item, pg.heads, a.heads_magic), h = mine.item - cb * pg.heads, c0 = cb * kPoRows, ctx = at_context(a, b);
+    // keys [0, limit) are seen; a row behind the last one goes along with it
+    auto limit_of = [&](int col) { return a.causal ? max(ctx - L + 1 + at_div(min(col, columns - 1), G, a.group_magic), 0) : ctx; };
+    const int end = min(limit_of(c0 + kPoRows - 1), ctx), begin = mine.piece * mine.size, stop = min((end + kF8Tokens - 1) / kF8Tokens, begin + mine.size);
+    const int first = begin * kF8Tokens, past = min(stop * kF8Tokens, end), n_tiles = max((past - first + kPoKeys - 1) / kPoKeys, 0);  // keys [first, past)
+    const int32_t *table = a.table + static_cast<size_t>(b) * a.max_pages;
+    auto page_at = [&](int blk) { return at_div(blk, a.page_blocks, a.page_magic); };
+    // the scale of block blk, NaN where its page is none
+    auto block_at = [&](int blk, int &page) {
+        const int at = page_at(blk);
+        page = table[at];
+        return (static_cast<size_t>(page) * pg.heads + h) * a.page_blocks + (blk - at * a.page_blocks);
+    };
+
+    const uint32_t base = g_smem_u32(psm), k_at = base + Z::k_off, v_at = base + Z::v_off, bar = base + Z::bar_off;
+    const uint32_t s_full = bar, p_full = bar + 16, pv_done = bar + 32, k_full = bar + 48, k_empty = bar + 64, v_full = bar + 80, v_empty = bar + 96;  // two of each
+    volatile int *dead = reinterpret_cast<volatile int *>(psm + Z::bar_off + 112);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(psm + Z::bar_off + 116);
+    int *seen = reinterpret_cast<int *>(psm + Z::bar_off + 120);  // largest scales of the CTA's blocks, keys' and values' (bits of positive numbers); whether a scale or page is none
+    float *row_factor = reinterpret_cast<float *>(psm + Z::row_off);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            g_mbar_init(s_full + 8 * i, 1), g_mbar_init(p_full + 8 * i, 4), g_mbar_init(pv_done + 8 * i, 1);
+            g_mbar_init(k_full + 8 * i, 2), g_mbar_init(k_empty + 8 * i, 1), g_mbar_init(v_full + 8 * i, 2), g_mbar_init(v_empty + 8 * i, 1);
+        }
+        *dead = 0, seen[0] = 0, seen[1] = 0, seen[2] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 4) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(g_smem_u32(tmem_slot)), "n"(kPoColumns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    __syncthreads();
+
+    // the largest scales
+    for (int blk = begin + threadIdx.x; blk < stop; blk += kPoThreads) {
+        int page;
+        const size_t at = block_at(blk, page);
+        const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(pg.num_pages);
+        const float k = there ? __ldg(pg.key_scales + at) : NAN, v = there ? __ldg(pg.value_scales + at) : NAN;
+        if (k < INFINITY) atomicMax(seen, __float_as_int(k));
+        if (v < INFINITY) atomicMax(seen + 1, __float_as_int(v));
+        if (!(k < INFINITY) || !(v < INFINITY)) seen[2] = 1;
+    }
+    // queries: 8 entries a thread, a row to 8 or 16 lanes
+    {
+        constexpr int LANES = DIM / 8, ROWS = 32 / LANES, STEP = 7 * ROWS, N = (kPoRows + STEP - 1) / STEP;
+        const bf16 *q = static_cast<const bf16 *>(a.q) + b * a.q_b + static_cast<long long>(h) * G * a.q_h + lane % LANES * 8;
+        const float sign = a.scale_log2 < 0.f ? -1.f : 1.f;
+        constexpr int HALF = (N + 1) / 2;
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+            float x[HALF][8];
+#pragma unroll
+            for (int i = 0; i < HALF; ++i) {
+                const int row = warp * ROWS + lane / LANES + (part * HALF + i) * STEP, col = c0 + row;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
+                if (row < kPoRows && col < columns) {
+                    const int l = at_div(col, G, a.group_magic);
+                    at_query(q + l * a.q_l + (col - l * G) * a.q_h, a.wide_rows, x[i]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < HALF; ++i) {
+                const int row = warp * ROWS + lane / LANES + (part * HALF + i) * STEP;
+                float m = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) m = f8_most(m, fabsf(x[i][e]));
+#pragma unroll
+                for (int o = 1; o < LANES; o <<= 1) m = f8_most(m, __shfl_xor_sync(0xffffffffu, m, o));
+                const int e2 = static_cast<int>(__float_as_uint(m) >> 23), up = e2 == 255 ? 0 : min(13 + 127 - e2, 100);
+                const float times = f8_power(up) * sign;
+                if (row < kPoRows) {
+                    const int j = lane % LANES;
+                    uint4 f;
+                    f.x = tl::pack2<__half>(x[i][0] * times, x[i][1] * times), f.y = tl::pack2<__half>(x[i][2] * times, x[i][3] * times);
+                    f.z = tl::pack2<__half>(x[i][4] * times, x[i][5] * times), f.w = tl::pack2<__half>(x[i][6] * times, x[i][7] * times);
+                    *reinterpret_cast<uint4 *>(psm + (j >> 3) * Z::q_block + row * 128 + (((j & 7) ^ (row & 7)) << 4)) = f;
+                    if (j == 0) row_factor[row] = f8_power(-up);
+                }
+            }
+        }
+        g_fence_proxy_async();
+    }
+    g_tc_fence_before();
+    __syncthreads();
+    g_tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    // 1 over the largest scales; both are powers of two
+    const float top_k = seen[0] ? __int_as_float(seen[0]) : 1.f, top_v = seen[1] ? __int_as_float(seen[1]) : 1.f, under_k = 1.f / top_k, under_v = 1.f / top_v;
+
+    if (warp >= 5) {  // ---- pages to operands
+        const int tid = threadIdx.x - 5 * 32;
+        uint4 kr[PER], vr[PER];
+        // a thread's pieces lie 64 apart: rows 64 / CH apart, so that a group of 16 rows (a scale) is a fixed part of them
+        auto load = [&](int t, bool values, uint4 (&x)[PER], __half2 (&ratio)[4]) {
+            const int key0 = first + t * kPoKeys;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int key = key0 + kF8Tokens * g;
+                int page = -1;
+                size_t at = 0;
+                if (key < past) at = block_at(key / kF8Tokens, page);
+                const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(pg.num_pages);
+                const float s = there ? __ldg((values ? pg.value_scales : pg.key_scales) + at) : 0.f;
+                ratio[g] = __float2half2_rn(s < INFINITY ? s * (values ? under_v : under_k) : 0.f);
+                const uint8_t *rows = (values ? pg.values : pg.keys) + (there ? at : 0) * (kF8Tokens * DIM);
+#pragma unroll
+                for (int i = 0; i < PER / 4; ++i) x[g * (PER / 4) + i] = there ? tl::ldg_stream(rows + 16 * (tid + 64 * i)) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        auto store = [&](int t, unsigned char *tile, const uint4 (&x)[PER], const __half2 (&ratio)[4]) {
+            const int key0 = first + t * kPoKeys;
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+#pragma unroll
+                for (int i = 0; i < PER / 4; ++i) {
+                    const int piece = tid + 64 * i, row = kF8Tokens * g + piece / CH;
+                    po_store<DIM>(tile, row, piece % CH, x[g * (PER / 4) + i], ratio[g], key0 + row < ctx);
+                }
+        };
+        __half2 rk[4], rv[4];
+        if (n_tiles > 0) load(0, false, kr, rk), load(0, true, vr, rv);
+        for (int t = 0; t < n_tiles; ++t) {
+            const int s = t & 1;
+            const uint32_t ph = (t >> 1 & 1) ^ 1u;  // the first pass through the stages does not wait
+            if (!tc_wait(k_empty + 8 * s, ph, dead)) break;
+            store(t, psm + Z::k_off + s * Z::halves * Z::kv_block, kr, rk);
+            g_fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) g_mbar_arrive(k_full + 8 * s);
+            if (t + 1 < n_tiles) load(t + 1, false, kr, rk);
+            if (!tc_wait(v_empty + 8 * s, ph, dead)) break;
+            store(t, psm + Z::v_off + s * Z::halves * Z::kv_block, vr, rv);
+            g_fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) g_mbar_arrive(v_full + 8 * s);
+            if (t + 1 < n_tiles) load(t + 1, true, vr, rv);
+        }
+    } else if (warp == 4) {  // ---- products: S_0, then per tile S_(t+1), P_t V_t
+        constexpr uint32_t idesc_s = po_idesc(kPoKeys, false), idesc_o = po_idesc(DIM, true);
+        const uint64_t qd = g_smem_desc_sw128(base, 0, 1024), kd0 = g_smem_desc_sw128(k_at, 0, 1024), vd0 = g_smem_desc_sw128(v_at, Z::kv_block, 1024);
+        auto scores = [&](int t) {
+            const int s = t & 1;
+            if (!tc_wait(k_full + 8 * s, t >> 1 & 1, dead)) return false;
+            g_tc_fence_after();
+            if (g_elect_one()) {
+                const uint64_t kd = kd0 + static_cast<uint64_t>(s * Z::halves * (Z::kv_block >> 4));
+#pragma unroll
+                for (int k = 0; k < DIM / 16; ++k)
+                    g_tc_mma(tmem + s * kPoKeys, qd + (k >> 2) * (Z::q_block >> 4) + 2 * (k & 3), kd + (k >> 2) * (Z::kv_block >> 4) + 2 * (k & 3), idesc_s, k > 0);
+                g_tc_commit(k_empty + 8 * s);
+                g_tc_commit(s_full + 8 * s);
+            }
+            __syncwarp();
+            return true;
+        };
+        const bool begun = n_tiles > 0 && scores(0);
+        for (int t = 0; begun && t < n_tiles; ++t) {
+            const int s = t & 1;
+            if (t + 1 < n_tiles && !scores(t + 1)) break;  // its buffer held P_(t-1), read by a product already queued ahead of this one
+            if (!tc_wait(p_full + 8 * s, t >> 1 & 1, dead) || !tc_wait(v_full + 8 * s, t >> 1 & 1, dead)) break;
+            g_tc_fence_after();
+            if (g_elect_one()) {
+                const uint64_t vd = vd0 + static_cast<uint64_t>(s * Z::halves * (Z::kv_block >> 4));
+#pragma unroll
+                for (int k = 0; k < kPoKeys / 16; ++k) g_tc_mma_ts(tmem + kPoOut, tmem + s * kPoKeys + 8 * k, vd + k * (2048 >> 4), idesc_o, t > 0 || k > 0);
+                g_tc_commit(v_empty + 8 * s);
+                g_tc_commit(pv_done + 8 * s);
+            }
+            __syncwarp();
+        }
+    } else {  // ---- softmax: thread = row
+        const int r = threadIdx.x, col = c0 + r;
+        const bool live = col < columns;
+        const int limit = min(limit_of(col), past);
+        const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+        const float mult = fmaxf(fabsf(a.scale_log2) * row_factor[r] * top_k, 0x1p-126f);  // never 0: a masked score stays -inf
+        const bool care = seen[2] != 0;
+        float m = -INFINITY, sum = 0.f;
+        bool ok = true;
+        for (int t = 0; t < n_tiles; ++t) {
+            const int key0 = first + t * kPoKeys, s2 = t & 1;
+            if (!(ok = tc_wait(s_full + 8 * s2, t >> 1 & 1, dead))) break;
+            g_tc_fence_after();
+            uint32_t s[2][32];
+            g_tmem_ld32_nowait(tmem + lanes + s2 * kPoKeys, s[0]);
+            g_tmem_ld32_nowait(tmem + lanes + s2 * kPoKeys + 32, s[1]);
+            g_tmem_ld_wait();
+            if (__any_sync(0xffffffffu, key0 + kPoKeys > limit)) {
+#pragma unroll
+                for (int c = 0; c < kPoKeys; ++c)
+                    if (key0 + c >= limit) s[c >> 5][c & 31] = 0xff800000u;
+            }
+            if (care) {  // a page that is none hides its keys; a scale that is none makes the row NaN
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int key = key0 + kF8Tokens * g;
+                    if (key >= past) continue;
+                    int page;
+                    const size_t at = block_at(key / kF8Tokens, page);
+                    if (static_cast<unsigned>(page) >= static_cast<unsigned>(pg.num_pages)) {
+#pragma unroll
+                        for (int c = 0; c < kF8Tokens; ++c) s[g >> 1][(g & 1) * 16 + c] = 0xff800000u;
+                    } else if (key < limit && !(pg.key_scales[at] < INFINITY && pg.value_scales[at] < INFINITY)) {
+                        sum = NAN;
+                    }
+                }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < kPoKeys; ++c) top = fmaxf(top, __uint_as_float(s[c >> 5][c & 31]));
+            top *= mult;
+            const bool grow = top > m + kAtLag || (m == -INFINITY && top > m);
+            if (__any_sync(0xffffffffu, grow)) {
+                if (t > 0) {
+                    if (!(ok = tc_wait(pv_done + 8 * (s2 ^ 1), ((t - 1) >> 1) & 1, dead))) break;  // O has to be still while it is rescaled
+                    g_tc_fence_after();
+                    const float to = grow ? top : m, alpha = !grow ? 1.f : m == -INFINITY ? 0.f : at_ex2(m - to);
+                    sum *= alpha;
+#pragma unroll
+                    for (int i = 0; i < DIM / 32; ++i) {
+                        uint32_t o[32];
+                        g_tmem_ld32(tmem + lanes + kPoOut + i * 32, o);
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+                        g_tmem_st32(tmem + lanes + kPoOut + i * 32, o);
+                    }
+                    g_tmem_st_wait();
+                }
+                m = grow ? top : m;
+            }
+            const float at = m == -INFINITY ? 0.f : m;
+            uint32_t pk[32];
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int c = 0; c < kPoKeys; c += 2) {
+                const float u = __uint_as_float(s[c >> 5][c & 31]), v = __uint_as_float(s[c >> 5][(c & 31) + 1]);
+                const float x = at_ex2(fmaf(u, mult, -at)), y = at_ex2(fmaf(v, mult, -at));
+                pk[c / 2] = tl::pack2<__half>(x, y);
+                s0 += x, s1 += y;
+            }
+            sum += s0 + s1;
+            g_tmem_st32(tmem + lanes + s2 * kPoKeys, pk);  // column c = keys 2 c and 2 c + 1
+            g_tmem_st_wait();
+            g_tc_fence_before();
+            __syncwarp();
+            if (lane == 0) g_mbar_arrive(p_full + 8 * s2);
+        }
+        if (n_tiles > 0) {
+            ok = ok && tc_wait(pv_done + 8 * ((n_tiles - 1) & 1), ((n_tiles - 1) >> 1) & 1, dead);
+            g_tc_fence_after();
+        }
+        const float verdict = tc_verdict(ok, dead) * top_v;
+        const bool whole = mine.pieces == 1;
+        const float inv = (whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f) * verdict;
+        float *part = whole ? nullptr : static_cast<float *>(a.workspace) + index * at_piece_floats(kPoRows, DIM);
+        const int l = at_div(live ? col : 0, G, a.group_magic);
+        bf16 *out = static_cast<bf16 *>(a.out) + ((static_cast<size_t>(b) * L + l) * a.heads + static_cast<size_t>(h) * G + (live ? col : 0) - l * G) * DIM;
+#pragma unroll
+        for (int i = 0; i < DIM / 32; ++i) {
+            uint32_t o[32];
+            if (n_tiles > 0) {
+                g_tmem_ld32(tmem + lanes + kPoOut + i * 32, o);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 32; ++c) o[c] = 0u;
+            }
+            if (!live) continue;
+            if (whole) {
+#pragma unroll
+                for (int c = 0; c < 32; c += 8) {
+                    uint4 u;
+                    u.x = tl::pack2<bf16>(__uint_as_float(o[c]) * inv, __uint_as_float(o[c + 1]) * inv), u.y = tl::pack2<bf16>(__uint_as_float(o[c + 2]) * inv, __uint_as_float(o[c + 3]) * inv);
+                    u.z = tl::pack2<bf16>(__uint_as_float(o[c + 4]) * inv, __uint_as_float(o[c + 5]) * inv), u.w = tl::pack2<bf16>(__uint_as_float(o[c + 6]) * inv, __uint_as_float(o[c + 7]) * inv);
+                    *reinterpret_cast<uint4 *>(out + i * 32 + c) = u;
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < 32; c += 4)
+                    *reinterpret_cast<float4 *>(part + r * DIM + i * 32 + c) = make_float4(__uint_as_float(o[c]) * inv, __uint_as_float(o[c + 1]) * inv, __uint_as_float(o[c + 2]) * inv,
+                                                                                          __uint_as_float(o[c + 3]) * inv);
+            }
+        }
+        if (live && !whole) part[kPoRows * DIM + r] = m, part[kPoRows * (DIM + 1) + r] = sum;
+    }
+    g_tc_fence_before();
+    __syncthreads();
+    if (warp == 4) {
+        tc_settle(dead);
+        g_tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kPoColumns) : "memory");
+    }
+}
+
+bool f8_portion_takes(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c) {
+    return c.dtype == TL_BF16 && (p.dim == 64 || p.dim == 128) && static_cast<long long>(c.heads / p.heads) * c.tokens > 32;
+}
+
+template <int DIM>
+static int portion_launch(const F8Attend &a, unsigned ctas, cudaStream_t st) {
+    static tl::PerDevice ready;
+    using Z = PoShape<DIM>;
+    int device = 0;
+    cudaGetDevice(&device);
+    if (!ready(device, [&] {
+            return cudaFuncSetAttribute(fp8_portion_kernel<DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, Z::smem) == cudaSuccess &&
+                   cudaFuncSetAttribute(fp8_portion_kernel<DIM>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) == cudaSuccess;
+        }))
+        return tl::fail(TL_ECUDA, "fp8_attention: %s", cudaGetErrorString(cudaGetLastError()));
+    const cudaError_t e = tl::launch_chained(fp8_portion_kernel<DIM>, dim3(ctas), dim3(kPoThreads), Z::smem, st, a);
+    if (e != cudaSuccess) return tl::fail(TL_ECUDA, "fp8_attention: %s", cudaGetErrorString(e));
+    TL_LAUNCH_CHECK("fp8_attention (portion)");
+    return a.workspace ? f8_attend_join(a, kPoRows, st) : TL_OK;
+}
+
+int f8_portion(F8Attend a, cudaStream_t st) {
+    a.slots = 2 * sm_count(), a.most_pieces = 32, a.granule = kPoKeys / kF8Tokens;
+    a.col_blocks = (a.group * a.tokens + kPoRows - 1) / kPoRows;
+    const long long items = static_cast<long long>(a.col_blocks) * a.pages.heads * a.batch;
+    if (items > 0x3fffffff) return tl::fail(TL_EINVAL, "fp8_attention: sizes out of range");
+    const unsigned ctas = static_cast<unsigned>(items + (a.workspace ? a.slots : 0));
+    a.each_magic = at_magic(ctas, a.pages.heads * a.col_blocks);
+    return a.pages.dim == 64 ? portion_launch<64>(a, ctas, st) : portion_launch<128>(a, ctas, st);
+}
+
+long long f8_portion_gave_up() { return tl::read_gave_up(); }
+
+}  // namespace tlb

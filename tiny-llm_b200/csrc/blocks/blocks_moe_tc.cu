@@ -475,8 +475,8 @@ int tlb_moe_sort(const int32_t *idx, int tokens, int top, int experts, int32_t *
 }
 
 long long tlb_tc_gave_up(void) {
-    const long long experts = tl::read_gave_up(), attention = flash_tc_gave_up(), bytes = f8_gave_up(), few = few_gave_up();
-    return experts < 0 || attention < 0 || bytes < 0 || few < 0 ? -1 : experts + attention + bytes + few;
+    const long long experts = tl::read_gave_up(), attention = flash_tc_gave_up(), bytes = f8_gave_up(), few = few_gave_up(), portions = f8_portion_gave_up();
+    return experts < 0 || attention < 0 || bytes < 0 || few < 0 || portions < 0 ? -1 : experts + attention + bytes + few + portions;
 }
 
 }  // extern "C"

@@ -27,6 +27,7 @@ using tl::tc_wait_one;
 long long flash_tc_gave_up();  // of the attention kernels
 long long f8_gave_up();        // of the 8-bit products
 long long few_gave_up();       // of the experts for few tokens
+long long f8_portion_gave_up();  // of attention over pages of 8 bits
 
 // kind::f16 instruction descriptor: bf16 x bf16 -> f32, 128 rows, n columns; A K-major, B K-major or (b_mn) MN-major.
 __host__ __device__ __forceinline__ constexpr uint32_t tc_idesc(int n, bool b_mn = false) {

@@ -64,6 +64,7 @@ BLOCKS_SOURCES = [
     "blocks/blocks_fp8_pairs.cu",
     "blocks/blocks_fp8_append.cu",
     "blocks/blocks_fp8_attention.cu",
+    "blocks/blocks_fp8_portion.cu",
 ]
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
