@@ -534,7 +534,7 @@ extern "C" size_t tlb_fp8_attention_workspace(const tlb_fp8_pages *pages, const 
     if (f8_check_pages("fp8_attention", pages) != TL_OK || !c || c->heads <= 0 || c->tokens <= 0 || c->batch <= 0) return 0;
     const long long rows = static_cast<long long>(c->heads / pages->heads) * c->tokens;
     const bool portion = f8_portion_takes(*pages, *c);
-    const int few = rows <= 8 ? 8 : 9, cols = portion ? kPoRows : attend_cols(pages->dim, few), slots = portion ? 2 * sm_count() : attend_slots(c->dtype, pages->dim, few);
+    const int few = rows <= 8 ? 8 : 9, cols = portion ? kPoRows : attend_cols(pages->dim, few), slots = portion ? sm_count() : attend_slots(c->dtype, pages->dim, few);
     const long long items = (rows + cols - 1) / cols * pages->heads * c->batch;
     // requests that can't be long, or more items than a cut would serve
     if (static_cast<long long>(c->max_pages) * (pages->page_size / kF8Tokens) <= kAtLeast + kAtLeast / 4 || items > (portion ? 1LL : 16LL) * slots) return 0;

@@ -134,7 +134,7 @@ int f8_attend_join(const F8Attend &a, int cols, cudaStream_t st);
 static inline unsigned at_magic(unsigned long long most, unsigned d) { return d > 1 && most < (1ull << 32) / d ? static_cast<unsigned>((1ull << 32) / d) + 1 : 0; }
 __host__ __device__ static inline size_t at_piece_floats(int cols, int dim) { return static_cast<size_t>(cols) * (dim + 2); }
 // blocks_fp8_portion.cu: bf16 queries of many columns
-constexpr int kPoRows = 128;
+constexpr int kPoRows = 256;  // columns of a CTA
 bool f8_portion_takes(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c);
 int f8_portion(F8Attend a, cudaStream_t st);
 

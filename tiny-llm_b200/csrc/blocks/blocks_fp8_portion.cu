@@ -5,11 +5,11 @@
 // scale of the CTA's blocks - exact down to 2^-15 of that, and below it off by at most 2^-34 of the largest block's numbers.  A block whose
 // scale is no number counts as zeros in the products, and the rows that see it are made NaN at the end.
 //
-// A CTA takes 128 columns (rows of the products, tensor-memory lanes) of one request and key/value head, or a piece of their keys; two CTAs share an SM, so that one's
-// exponentials run beside the other's products.  Per 64 keys:
-//   warps 5, 6  bring keys and values from the pages into f16 operand tiles (128-byte swizzle) of two stages each, the next tile's bytes on their way in registers meanwhile
-//   warp 4      tcgen05.mma, one elected lane: S = Q K^T into one of two score buffers, O += P V; the next tile's scores are issued ahead of this tile's values
-//   warps 0-3   softmax, thread = row: scores from tensor memory, 2^x of them over a running maximum that may lag behind by 2^8, P as f16 back over its own scores
+// A CTA takes 256 columns of one request and key/value head, or a piece of their keys, as two sets of 128 rows (tensor-memory lanes) that work on the same keys, so that one's
+// exponentials run beside the other's products and the cache's numbers are turned into operands once for both.  Per 64 keys:
+//   warps 8-11   bring keys and values from the pages into f16 operand tiles (128-byte swizzle) of two stages each, the next tile's bytes on their way in registers meanwhile
+//   warp 12      tcgen05.mma, one elected lane: of either set S = Q K^T into one of two score buffers, O += P V; the next tile's scores are issued ahead of this tile's values
+//   warps 0-7    softmax, thread = row: scores from tensor memory, 2^x of them over a running maximum that may lag behind by 2^8, P as f16 back over its own scores
 #include "../per_device.h"
 #include "blocks_fp8_attention.cuh"
 #include "blocks_tc.cuh"
@@ -24,9 +24,10 @@ using tl::g_tmem_st32;
 using tl::g_tmem_st_wait;
 
 constexpr int kPoKeys = 64;
-constexpr int kPoThreads = 7 * 32;
-constexpr int kPoColumns = 256;  // of tensor memory: two score buffers of 64, the output from 128 on
-constexpr uint32_t kPoOut = 128;
+constexpr int kPoSet = 128;  // rows of a set
+constexpr int kPoThreads = 13 * 32;
+constexpr int kPoColumns = 512;      // of tensor memory; a set's half: two score buffers of 64, the output from 128 on
+constexpr uint32_t kPoHalf = 256, kPoOut = 128;
 
 // kind::f16, f16 x f16 -> f32, 128 rows
 __host__ __device__ constexpr uint32_t po_idesc(int n, bool b_mn) { return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24); }
@@ -34,14 +35,14 @@ __host__ __device__ constexpr uint32_t po_idesc(int n, bool b_mn) { return (1u <
 template <int DIM>
 struct PoShape {
     static constexpr int halves = DIM / 64;                                // 64-column blocks
-    static constexpr int q_block = kPoRows * 128, kv_block = kPoKeys * 128;  // bytes
-    static constexpr int k_off = halves * q_block, v_off = k_off + 2 * halves * kv_block, bar_off = v_off + 2 * halves * kv_block;
+    static constexpr int q_block = kPoSet * 128, kv_block = kPoKeys * 128;  // bytes
+    static constexpr int k_off = 2 * halves * q_block, v_off = k_off + 2 * halves * kv_block, bar_off = v_off + 2 * halves * kv_block;
     static constexpr int row_off = bar_off + 256, smem = row_off + kPoRows * 4;
 };
 
 // 16 e4m3 numbers (entries 16 c .. of a row) times `ratio`, as f16, into their places in a tile of 64-column blocks.
 template <int DIM>
-__device__ __forceinline__ void po_store(unsigned char *tile, int row, int c, uint4 raw, __half2 ratio, bool live) {
+__device__ __forceinline__ void po_store(unsigned char *tile, int row, int c, uint4 raw, __half2 ratio) {
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
     uint32_t f[8];
 #pragma unroll
@@ -50,7 +51,7 @@ __device__ __forceinline__ void po_store(unsigned char *tile, int row, int c, ui
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const __half2 v = __hmul2(*reinterpret_cast<__half2 *>(&f[2 * i + e]), ratio);
-            f[2 * i + e] = live ? *reinterpret_cast<const uint32_t *>(&v) : 0u;  // slots behind the last token may hold anything
+            f[2 * i + e] = *reinterpret_cast<const uint32_t *>(&v);
         }
     }
     unsigned char *at = tile + (c >> 2) * PoShape<DIM>::kv_block + row * 128;
@@ -61,9 +62,9 @@ __device__ __forceinline__ void po_store(unsigned char *tile, int row, int c, ui
 }
 
 template <int DIM>
-__global__ void __launch_bounds__(kPoThreads, 2) fp8_portion_kernel(const __grid_constant__ F8Attend a) {
+__global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid_constant__ F8Attend a) {
     using Z = PoShape<DIM>;
-    constexpr int CH = DIM / 16, PER = kPoKeys * CH / 64;  // 16-byte pieces of a row; of a tile's side, a converting thread's
+    constexpr int CH = DIM / 16, PER = kPoKeys * CH / 128;  // 16-byte pieces of a row; of a tile's side, a converting thread's
     extern __shared__ __align__(1024) unsigned char psm[];
     tl::griddep_wait();
     tl::griddep_launch();  // behind the wait: the launch that joins the pieces reads the lengths ahead of its own
@@ -88,20 +89,18 @@ __global__ void __launch_bounds__(kPoThreads, 2) fp8_portion_kernel(const __grid
     };
 
     const uint32_t base = g_smem_u32(psm), k_at = base + Z::k_off, v_at = base + Z::v_off, bar = base + Z::bar_off;
-    const uint32_t s_full = bar, p_full = bar + 16, pv_done = bar + 32, k_full = bar + 48, k_empty = bar + 64, v_full = bar + 80, v_empty = bar + 96;  // two of each
-    volatile int *dead = reinterpret_cast<volatile int *>(psm + Z::bar_off + 112);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(psm + Z::bar_off + 116);
-    int *seen = reinterpret_cast<int *>(psm + Z::bar_off + 120);  // largest scales of the CTA's blocks, keys' and values' (bits of positive numbers); whether a scale or page is none
+    const uint32_t s_full = bar, p_full = bar + 32, pv_done = bar + 64, k_full = bar + 96, k_empty = bar + 112, v_full = bar + 128, v_empty = bar + 144;  // two of each, of the first three for either set
+    volatile int *dead = reinterpret_cast<volatile int *>(psm + Z::bar_off + 160);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(psm + Z::bar_off + 164);
+    int *seen = reinterpret_cast<int *>(psm + Z::bar_off + 168);  // largest scales of the CTA's blocks, keys' and values' (bits of positive numbers); whether a scale or page is none
     float *row_factor = reinterpret_cast<float *>(psm + Z::row_off);
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2; ++i) {
-            g_mbar_init(s_full + 8 * i, 1), g_mbar_init(p_full + 8 * i, 4), g_mbar_init(pv_done + 8 * i, 1);
-            g_mbar_init(k_full + 8 * i, 2), g_mbar_init(k_empty + 8 * i, 1), g_mbar_init(v_full + 8 * i, 2), g_mbar_init(v_empty + 8 * i, 1);
-        }
+        for (int i = 0; i < 4; ++i) g_mbar_init(s_full + 8 * i, 1), g_mbar_init(p_full + 8 * i, 4), g_mbar_init(pv_done + 8 * i, 1);
+        for (int i = 0; i < 2; ++i) g_mbar_init(k_full + 8 * i, 4), g_mbar_init(k_empty + 8 * i, 1), g_mbar_init(v_full + 8 * i, 4), g_mbar_init(v_empty + 8 * i, 1);
         *dead = 0, seen[0] = 0, seen[1] = 0, seen[2] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 4) {
+    if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(g_smem_u32(tmem_slot)), "n"(kPoColumns) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -118,11 +117,11 @@ __global__ void __launch_bounds__(kPoThreads, 2) fp8_portion_kernel(const __grid
         if (!(k < INFINITY) || !(v < INFINITY)) seen[2] = 1;
     }
     // queries: 8 entries a thread, a row to 8 or 16 lanes
-    {
-        constexpr int LANES = DIM / 8, ROWS = 32 / LANES, STEP = 7 * ROWS, N = (kPoRows + STEP - 1) / STEP;
+    if (warp < 8) {
+        constexpr int LANES = DIM / 8, ROWS = 32 / LANES, STEP = 8 * ROWS, N = kPoRows / STEP;  // the eight softmax warps
         const bf16 *q = static_cast<const bf16 *>(a.q) + b * a.q_b + static_cast<long long>(h) * G * a.q_h + lane % LANES * 8;
         const float sign = a.scale_log2 < 0.f ? -1.f : 1.f;
-        constexpr int HALF = (N + 1) / 2;
+        constexpr int HALF = N / 2;
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
             float x[HALF][8];
@@ -131,7 +130,7 @@ __global__ void __launch_bounds__(kPoThreads, 2) fp8_portion_kernel(const __grid
                 const int row = warp * ROWS + lane / LANES + (part * HALF + i) * STEP, col = c0 + row;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
-                if (row < kPoRows && col < columns) {
+                if (col < columns) {
                     const int l = at_div(col, G, a.group_magic);
                     at_query(q + l * a.q_l + (col - l * G) * a.q_h, a.wide_rows, x[i]);
                 }
@@ -146,14 +145,12 @@ __global__ void __launch_bounds__(kPoThreads, 2) fp8_portion_kernel(const __grid
                 for (int o = 1; o < LANES; o <<= 1) m = f8_most(m, __shfl_xor_sync(0xffffffffu, m, o));
                 const int e2 = static_cast<int>(__float_as_uint(m) >> 23), up = e2 == 255 ? 0 : min(13 + 127 - e2, 100);
                 const float times = f8_power(up) * sign;
-                if (row < kPoRows) {
-                    const int j = lane % LANES;
-                    uint4 f;
-                    f.x = tl::pack2<__half>(x[i][0] * times, x[i][1] * times), f.y = tl::pack2<__half>(x[i][2] * times, x[i][3] * times);
-                    f.z = tl::pack2<__half>(x[i][4] * times, x[i][5] * times), f.w = tl::pack2<__half>(x[i][6] * times, x[i][7] * times);
-                    *reinterpret_cast<uint4 *>(psm + (j >> 3) * Z::q_block + row * 128 + (((j & 7) ^ (row & 7)) << 4)) = f;
-                    if (j == 0) row_factor[row] = f8_power(-up);
-                }
+                const int j = lane % LANES, in_set = row % kPoSet;
+                uint4 f;
+                f.x = tl::pack2<__half>(x[i][0] * times, x[i][1] * times), f.y = tl::pack2<__half>(x[i][2] * times, x[i][3] * times);
+                f.z = tl::pack2<__half>(x[i][4] * times, x[i][5] * times), f.w = tl::pack2<__half>(x[i][6] * times, x[i][7] * times);
+                *reinterpret_cast<uint4 *>(psm + (row / kPoSet * Z::halves + (j >> 3)) * Z::q_block + in_set * 128 + (((j & 7) ^ (in_set & 7)) << 4)) = f;
+                if (j == 0) row_factor[row] = f8_power(-up);
             }
         }
         g_fence_proxy_async();
@@ -165,55 +162,7 @@ __global__ void __launch_bounds__(kPoThreads, 2) fp8_portion_kernel(const __grid
     // 1 over the largest scales; both are powers of two
     const float top_k = seen[0] ? __int_as_float(seen[0]) : 1.f, top_v = seen[1] ? __int_as_float(seen[1]) : 1.f, under_k = 1.f / top_k, under_v = 1.f / top_v;
 
-    if (warp >= 5) {  // ---- pages to operands
-        const int tid = threadIdx.x - 5 * 32;
-        uint4 kr[PER], vr[PER];
-        // a thread's pieces lie 64 apart: rows 64 / CH apart, so that a group of 16 rows (a scale) is a fixed part of them
-        auto load = [&](int t, bool values, uint4 (&x)[PER], __half2 (&ratio)[4]) {
-            const int key0 = first + t * kPoKeys;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int key = key0 + kF8Tokens * g;
-                int page = -1;
-                size_t at = 0;
-                if (key < past) at = block_at(key / kF8Tokens, page);
-                const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(pg.num_pages);
-                const float s = there ? __ldg((values ? pg.value_scales : pg.key_scales) + at) : 0.f;
-                ratio[g] = __float2half2_rn(s < INFINITY ? s * (values ? under_v : under_k) : 0.f);
-                const uint8_t *rows = (values ? pg.values : pg.keys) + (there ? at : 0) * (kF8Tokens * DIM);
-#pragma unroll
-                for (int i = 0; i < PER / 4; ++i) x[g * (PER / 4) + i] = there ? tl::ldg_stream(rows + 16 * (tid + 64 * i)) : make_uint4(0, 0, 0, 0);
-            }
-        };
-        auto store = [&](int t, unsigned char *tile, const uint4 (&x)[PER], const __half2 (&ratio)[4]) {
-            const int key0 = first + t * kPoKeys;
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-#pragma unroll
-                for (int i = 0; i < PER / 4; ++i) {
-                    const int piece = tid + 64 * i, row = kF8Tokens * g + piece / CH;
-                    po_store<DIM>(tile, row, piece % CH, x[g * (PER / 4) + i], ratio[g], key0 + row < ctx);
-                }
-        };
-        __half2 rk[4], rv[4];
-        if (n_tiles > 0) load(0, false, kr, rk), load(0, true, vr, rv);
-        for (int t = 0; t < n_tiles; ++t) {
-            const int s = t & 1;
-            const uint32_t ph = (t >> 1 & 1) ^ 1u;  // the first pass through the stages does not wait
-            if (!tc_wait(k_empty + 8 * s, ph, dead)) break;
-            store(t, psm + Z::k_off + s * Z::halves * Z::kv_block, kr, rk);
-            g_fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) g_mbar_arrive(k_full + 8 * s);
-            if (t + 1 < n_tiles) load(t + 1, false, kr, rk);
-            if (!tc_wait(v_empty + 8 * s, ph, dead)) break;
-            store(t, psm + Z::v_off + s * Z::halves * Z::kv_block, vr, rv);
-            g_fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) g_mbar_arrive(v_full + 8 * s);
-            if (t + 1 < n_tiles) load(t + 1, true, vr, rv);
-        }
-    } else if (warp == 4) {  // ---- products: S_0, then per tile S_(t+1), P_t V_t
+    if (warp >= 12) {  // ---- products: of either set S_0, then per tile S_(t+1), P_t V_t
         constexpr uint32_t idesc_s = po_idesc(kPoKeys, false), idesc_o = po_idesc(DIM, true);
         const uint64_t qd = g_smem_desc_sw128(base, 0, 1024), kd0 = g_smem_desc_sw128(k_at, 0, 1024), vd0 = g_smem_desc_sw128(v_at, Z::kv_block, 1024);
         auto scores = [&](int t) {
@@ -223,41 +172,104 @@ __global__ void __launch_bounds__(kPoThreads, 2) fp8_portion_kernel(const __grid
             if (g_elect_one()) {
                 const uint64_t kd = kd0 + static_cast<uint64_t>(s * Z::halves * (Z::kv_block >> 4));
 #pragma unroll
-                for (int k = 0; k < DIM / 16; ++k)
-                    g_tc_mma(tmem + s * kPoKeys, qd + (k >> 2) * (Z::q_block >> 4) + 2 * (k & 3), kd + (k >> 2) * (Z::kv_block >> 4) + 2 * (k & 3), idesc_s, k > 0);
+                for (int set = 0; set < 2; ++set) {
+#pragma unroll
+                    for (int k = 0; k < DIM / 16; ++k)
+                        g_tc_mma(tmem + set * kPoHalf + s * kPoKeys, qd + (set * Z::halves + (k >> 2)) * (Z::q_block >> 4) + 2 * (k & 3), kd + (k >> 2) * (Z::kv_block >> 4) + 2 * (k & 3),
+                                 idesc_s, k > 0);
+                    g_tc_commit(s_full + 16 * set + 8 * s);
+                }
                 g_tc_commit(k_empty + 8 * s);
-                g_tc_commit(s_full + 8 * s);
             }
             __syncwarp();
             return true;
         };
-        const bool begun = n_tiles > 0 && scores(0);
+        const bool begun = warp == 12 && n_tiles > 0 && scores(0);
         for (int t = 0; begun && t < n_tiles; ++t) {
             const int s = t & 1;
-            if (t + 1 < n_tiles && !scores(t + 1)) break;  // its buffer held P_(t-1), read by a product already queued ahead of this one
-            if (!tc_wait(p_full + 8 * s, t >> 1 & 1, dead) || !tc_wait(v_full + 8 * s, t >> 1 & 1, dead)) break;
-            g_tc_fence_after();
-            if (g_elect_one()) {
-                const uint64_t vd = vd0 + static_cast<uint64_t>(s * Z::halves * (Z::kv_block >> 4));
+            if (t + 1 < n_tiles && !scores(t + 1)) break;  // its buffers held P_(t-1), read by products already queued ahead of this one
+            if (!tc_wait(v_full + 8 * s, t >> 1 & 1, dead)) break;
+            bool ok = true;
 #pragma unroll
-                for (int k = 0; k < kPoKeys / 16; ++k) g_tc_mma_ts(tmem + kPoOut, tmem + s * kPoKeys + 8 * k, vd + k * (2048 >> 4), idesc_o, t > 0 || k > 0);
-                g_tc_commit(v_empty + 8 * s);
-                g_tc_commit(pv_done + 8 * s);
+            for (int set = 0; set < 2; ++set) {
+                if (!(ok = ok && tc_wait(p_full + 16 * set + 8 * s, t >> 1 & 1, dead))) break;
+                g_tc_fence_after();
+                if (g_elect_one()) {
+                    const uint64_t vd = vd0 + static_cast<uint64_t>(s * Z::halves * (Z::kv_block >> 4));
+#pragma unroll
+                    for (int k = 0; k < kPoKeys / 16; ++k)
+                        g_tc_mma_ts(tmem + set * kPoHalf + kPoOut, tmem + set * kPoHalf + s * kPoKeys + 8 * k, vd + k * (2048 >> 4), idesc_o, t > 0 || k > 0);
+                    if (set) g_tc_commit(v_empty + 8 * s);
+                    g_tc_commit(pv_done + 16 * set + 8 * s);
+                }
+                __syncwarp();
             }
+            if (!ok) break;
+        }
+    } else if (warp >= 8) {  // ---- pages to operands
+        // a thread's i-th piece of a tile's side: row (tid + 128 i) / CH, in the block of 16 rows that it is part of
+        const int tid = threadIdx.x - 8 * 32, c = tid % CH;
+        uint4 kr[PER], vr[PER];
+        float ks[PER], vs[PER];
+        int pages[PER];  // of the tile whose bytes are next to be asked for
+        auto block_of = [&](int t, int i) { return begin + t * (kPoKeys / kF8Tokens) + (tid + 128 * i) / (kF8Tokens * CH); };
+        auto look_up = [&](int t) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int blk = block_of(t, i);
+                pages[i] = blk < stop ? table[page_at(blk)] : -1;
+            }
+        };
+        auto load = [&](int t, const uint8_t *numbers, const float *scales, uint4 (&x)[PER], float (&s)[PER]) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int blk = block_of(t, i);
+                x[i] = make_uint4(0, 0, 0, 0), s[i] = 0.f;
+                if (static_cast<unsigned>(pages[i]) < static_cast<unsigned>(pg.num_pages)) {
+                    const size_t at = (static_cast<size_t>(pages[i]) * pg.heads + h) * a.page_blocks + (blk - page_at(blk) * a.page_blocks);
+                    x[i] = tl::ldg_stream(numbers + at * (kF8Tokens * DIM) + 16 * ((tid + 128 * i) % (kF8Tokens * CH)));
+                    s[i] = __ldg(scales + at);
+                }
+            }
+        };
+        auto store = [&](int t, unsigned char *tile, uint4 (&x)[PER], const float (&s)[PER], float under) {
+            const int key0 = first + t * kPoKeys;
+            if (key0 + kPoKeys > ctx) {  // slots behind the last token may hold anything
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+                    if (key0 + (tid + 128 * i) / CH >= ctx) x[i] = make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < PER; ++i) po_store<DIM>(tile, (tid + 128 * i) / CH, c, x[i], __float2half2_rn(s[i] < INFINITY ? s[i] * under : 0.f));
+            g_fence_proxy_async();
             __syncwarp();
+        };
+        if (n_tiles > 0) look_up(0), load(0, pg.keys, pg.key_scales, kr, ks), load(0, pg.values, pg.value_scales, vr, vs), look_up(1);
+        for (int t = 0; t < n_tiles; ++t) {
+            const int s = t & 1;
+            const uint32_t ph = (t >> 1 & 1) ^ 1u;  // the first pass through the stages does not wait
+            if (!tc_wait(k_empty + 8 * s, ph, dead)) break;
+            store(t, psm + Z::k_off + s * Z::halves * Z::kv_block, kr, ks, under_k);
+            if (lane == 0) g_mbar_arrive(k_full + 8 * s);
+            if (t + 1 < n_tiles) load(t + 1, pg.keys, pg.key_scales, kr, ks);
+            if (!tc_wait(v_empty + 8 * s, ph, dead)) break;
+            store(t, psm + Z::v_off + s * Z::halves * Z::kv_block, vr, vs, under_v);
+            if (lane == 0) g_mbar_arrive(v_full + 8 * s);
+            if (t + 1 < n_tiles) load(t + 1, pg.values, pg.value_scales, vr, vs), look_up(t + 2);
         }
     } else {  // ---- softmax: thread = row
-        const int r = threadIdx.x, col = c0 + r;
+        const int r = threadIdx.x, col = c0 + r, set = warp >> 2;
+        const uint32_t s_mine = s_full + 16 * set, p_mine = p_full + 16 * set, pv_mine = pv_done + 16 * set;
         const bool live = col < columns;
         const int limit = min(limit_of(col), past);
-        const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+        const uint32_t lanes = (static_cast<uint32_t>((warp & 3) * 32) << 16) + set * kPoHalf;
         const float mult = fmaxf(fabsf(a.scale_log2) * row_factor[r] * top_k, 0x1p-126f);  // never 0: a masked score stays -inf
         const bool care = seen[2] != 0;
         float m = -INFINITY, sum = 0.f;
         bool ok = true;
         for (int t = 0; t < n_tiles; ++t) {
             const int key0 = first + t * kPoKeys, s2 = t & 1;
-            if (!(ok = tc_wait(s_full + 8 * s2, t >> 1 & 1, dead))) break;
+            if (!(ok = tc_wait(s_mine + 8 * s2, t >> 1 & 1, dead))) break;
             g_tc_fence_after();
             uint32_t s[2][32];
             g_tmem_ld32_nowait(tmem + lanes + s2 * kPoKeys, s[0]);
@@ -290,7 +302,7 @@ __global__ void __launch_bounds__(kPoThreads, 2) fp8_portion_kernel(const __grid
             const bool grow = top > m + kAtLag || (m == -INFINITY && top > m);
             if (__any_sync(0xffffffffu, grow)) {
                 if (t > 0) {
-                    if (!(ok = tc_wait(pv_done + 8 * (s2 ^ 1), ((t - 1) >> 1) & 1, dead))) break;  // O has to be still while it is rescaled
+                    if (!(ok = tc_wait(pv_mine + 8 * (s2 ^ 1), ((t - 1) >> 1) & 1, dead))) break;  // O has to be still while it is rescaled
                     g_tc_fence_after();
                     const float to = grow ? top : m, alpha = !grow ? 1.f : m == -INFINITY ? 0.f : at_ex2(m - to);
                     sum *= alpha;
@@ -321,10 +333,10 @@ __global__ void __launch_bounds__(kPoThreads, 2) fp8_portion_kernel(const __grid
             g_tmem_st_wait();
             g_tc_fence_before();
             __syncwarp();
-            if (lane == 0) g_mbar_arrive(p_full + 8 * s2);
+            if (lane == 0) g_mbar_arrive(p_mine + 8 * s2);
         }
         if (n_tiles > 0) {
-            ok = ok && tc_wait(pv_done + 8 * ((n_tiles - 1) & 1), ((n_tiles - 1) >> 1) & 1, dead);
+            ok = ok && tc_wait(pv_mine + 8 * ((n_tiles - 1) & 1), ((n_tiles - 1) >> 1) & 1, dead);
             g_tc_fence_after();
         }
         const float verdict = tc_verdict(ok, dead) * top_v;
@@ -362,7 +374,7 @@ __global__ void __launch_bounds__(kPoThreads, 2) fp8_portion_kernel(const __grid
     }
     g_tc_fence_before();
     __syncthreads();
-    if (warp == 4) {
+    if (warp == 12) {
         tc_settle(dead);
         g_tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kPoColumns) : "memory");
@@ -391,7 +403,7 @@ static int portion_launch(const F8Attend &a, unsigned ctas, cudaStream_t st) {
 }
 
 int f8_portion(F8Attend a, cudaStream_t st) {
-    a.slots = 2 * sm_count(), a.most_pieces = 32, a.granule = kPoKeys / kF8Tokens;
+    a.slots = sm_count(), a.most_pieces = 32, a.granule = kPoKeys / kF8Tokens;
     a.col_blocks = (a.group * a.tokens + kPoRows - 1) / kPoRows;
     const long long items = static_cast<long long>(a.col_blocks) * a.pages.heads * a.batch;
     if (items > 0x3fffffff) return tl::fail(TL_EINVAL, "fp8_attention: sizes out of range");
