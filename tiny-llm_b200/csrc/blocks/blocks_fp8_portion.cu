@@ -25,7 +25,7 @@ using tl::g_tmem_st_wait;
 
 constexpr int kPoKeys = 64;
 constexpr int kPoSet = 128;  // rows of a set
-constexpr int kPoThreads = 13 * 32;
+constexpr int kPoThreads = 16 * 32;  // the last three warps have nothing to do: registers are moved between groups of four (168, 168, 112 and 64 are the launch's 128 a thread)
 constexpr int kPoColumns = 512;      // of tensor memory; a set's half: two score buffers of 64, the output from 128 on
 constexpr uint32_t kPoHalf = 256, kPoOut = 128;
 
@@ -163,6 +163,7 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
     const float top_k = seen[0] ? __int_as_float(seen[0]) : 1.f, top_v = seen[1] ? __int_as_float(seen[1]) : 1.f, under_k = 1.f / top_k, under_v = 1.f / top_v;
 
     if (warp >= 12) {  // ---- products: of either set S_0, then per tile S_(t+1), P_t V_t
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         constexpr uint32_t idesc_s = po_idesc(kPoKeys, false), idesc_o = po_idesc(DIM, true);
         const uint64_t qd = g_smem_desc_sw128(base, 0, 1024), kd0 = g_smem_desc_sw128(k_at, 0, 1024), vd0 = g_smem_desc_sw128(v_at, Z::kv_block, 1024);
         auto scores = [&](int t) {
@@ -207,6 +208,7 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
             if (!ok) break;
         }
     } else if (warp >= 8) {  // ---- pages to operands
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
         // a thread's i-th piece of a tile's side: row (tid + 128 i) / CH, in the block of 16 rows that it is part of
         const int tid = threadIdx.x - 8 * 32, c = tid % CH;
         uint4 kr[PER], vr[PER];
@@ -258,6 +260,7 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
             if (t + 1 < n_tiles) load(t + 1, pg.values, pg.value_scales, vr, vs), look_up(t + 2);
         }
     } else {  // ---- softmax: thread = row
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
         const int r = threadIdx.x, col = c0 + r, set = warp >> 2;
         const uint32_t s_mine = s_full + 16 * set, p_mine = p_full + 16 * set, pv_mine = pv_done + 16 * set;
         const bool live = col < columns;
