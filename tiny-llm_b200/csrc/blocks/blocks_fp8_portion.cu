@@ -7,8 +7,8 @@
 //
 // A CTA takes 256 columns of one request and key/value head, or a piece of their keys, as two sets of 128 rows (tensor-memory lanes) that work on the same keys, so that one's
 // exponentials run beside the other's products and the cache's numbers are turned into operands once for both.  Per 64 keys:
-//   warps 8-11   bring keys and values from the pages into f16 operand tiles (128-byte swizzle) of two stages each, the next tile's bytes on their way in registers meanwhile
-//   warp 12      tcgen05.mma, one elected lane: of either set S = Q K^T into one of two score buffers, O += P V; the next tile's scores are issued ahead of this tile's values
+//   warps 8-15   turn keys (the first four) and values into f16 operand tiles (128-byte swizzle) of two stages each, the bytes of the next two tiles on their way in registers
+//   warp 16      tcgen05.mma, one elected lane: of either set S = Q K^T into one of two score buffers, O += P V; the next tile's scores are issued ahead of this tile's values
 //   warps 0-7    softmax, thread = row: scores from tensor memory, 2^x of them over a running maximum that may lag behind by 2^8, P as f16 back over its own scores
 #include "../per_device.h"
 #include "blocks_fp8_attention.cuh"
@@ -25,9 +25,37 @@ using tl::g_tmem_st_wait;
 
 constexpr int kPoKeys = 64;
 constexpr int kPoSet = 128;  // rows of a set
-constexpr int kPoThreads = 16 * 32;  // the last three warps have nothing to do: registers are moved between groups of four (168, 168, 112 and 64 are the launch's 128 a thread)
+// The last three warps have nothing to do: registers are moved between groups of four warps (144, 144, 72, 72 and 48 are five times the launch's 96).
+constexpr int kPoThreads = 20 * 32;
 constexpr int kPoColumns = 512;      // of tensor memory; a set's half: two score buffers of 64, the output from 128 on
 constexpr uint32_t kPoHalf = 256, kPoOut = 128;
+
+__device__ __forceinline__ float po_max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// Two fp32 numbers side by side: one instruction for both.
+__device__ __forceinline__ uint64_t po_two(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 po_each(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t po_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t po_add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 
 // kind::f16, f16 x f16 -> f32, 128 rows
 __host__ __device__ constexpr uint32_t po_idesc(int n, bool b_mn) { return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24); }
@@ -100,7 +128,7 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
         *dead = 0, seen[0] = 0, seen[1] = 0, seen[2] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 12) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(g_smem_u32(tmem_slot)), "n"(kPoColumns) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -121,9 +149,9 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
         constexpr int LANES = DIM / 8, ROWS = 32 / LANES, STEP = 8 * ROWS, N = kPoRows / STEP;  // the eight softmax warps
         const bf16 *q = static_cast<const bf16 *>(a.q) + b * a.q_b + static_cast<long long>(h) * G * a.q_h + lane % LANES * 8;
         const float sign = a.scale_log2 < 0.f ? -1.f : 1.f;
-        constexpr int HALF = N / 2;
+        constexpr int HALF = N / 4;
 #pragma unroll
-        for (int part = 0; part < 2; ++part) {
+        for (int part = 0; part < 4; ++part) {
             float x[HALF][8];
 #pragma unroll
             for (int i = 0; i < HALF; ++i) {
@@ -162,8 +190,8 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
     // 1 over the largest scales; both are powers of two
     const float top_k = seen[0] ? __int_as_float(seen[0]) : 1.f, top_v = seen[1] ? __int_as_float(seen[1]) : 1.f, under_k = 1.f / top_k, under_v = 1.f / top_v;
 
-    if (warp >= 12) {  // ---- products: of either set S_0, then per tile S_(t+1), P_t V_t
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp >= 16) {  // ---- products: of either set S_0, then per tile S_(t+1), P_t V_t
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         constexpr uint32_t idesc_s = po_idesc(kPoKeys, false), idesc_o = po_idesc(DIM, true);
         const uint64_t qd = g_smem_desc_sw128(base, 0, 1024), kd0 = g_smem_desc_sw128(k_at, 0, 1024), vd0 = g_smem_desc_sw128(v_at, Z::kv_block, 1024);
         auto scores = [&](int t) {
@@ -185,7 +213,7 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
             __syncwarp();
             return true;
         };
-        const bool begun = warp == 12 && n_tiles > 0 && scores(0);
+        const bool begun = warp == 16 && n_tiles > 0 && scores(0);
         for (int t = 0; begun && t < n_tiles; ++t) {
             const int s = t & 1;
             if (t + 1 < n_tiles && !scores(t + 1)) break;  // its buffers held P_(t-1), read by products already queued ahead of this one
@@ -208,11 +236,17 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
             if (!ok) break;
         }
     } else if (warp >= 8) {  // ---- pages to operands
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
-        // a thread's i-th piece of a tile's side: row (tid + 128 i) / CH, in the block of 16 rows that it is part of
-        const int tid = threadIdx.x - 8 * 32, c = tid % CH;
-        uint4 kr[PER], vr[PER];
-        float ks[PER], vs[PER];
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        const bool values = warp >= 12;
+        const uint8_t *numbers = values ? pg.values : pg.keys;
+        const float *scales = values ? pg.value_scales : pg.key_scales;
+        const float under = values ? under_v : under_k;
+        unsigned char *tiles = psm + (values ? Z::v_off : Z::k_off);
+        const uint32_t full = values ? v_full : k_full, empty = values ? v_empty : k_empty;
+        // a thread's i-th piece of a tile: row (tid + 128 i) / CH, in the block of 16 rows that it is part of
+        const int tid = threadIdx.x & 127, c = tid % CH;
+        uint4 x[2][PER];
+        float scale[2][PER];
         int pages[PER];  // of the tile whose bytes are next to be asked for
         auto block_of = [&](int t, int i) { return begin + t * (kPoKeys / kF8Tokens) + (tid + 128 * i) / (kF8Tokens * CH); };
         auto look_up = [&](int t) {
@@ -222,45 +256,42 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
                 pages[i] = blk < stop ? table[page_at(blk)] : -1;
             }
         };
-        auto load = [&](int t, const uint8_t *numbers, const float *scales, uint4 (&x)[PER], float (&s)[PER]) {
+        auto load = [&](int t, uint4 (&to)[PER], float (&s)[PER]) {
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
                 const int blk = block_of(t, i);
-                x[i] = make_uint4(0, 0, 0, 0), s[i] = 0.f;
+                to[i] = make_uint4(0, 0, 0, 0), s[i] = 0.f;
                 if (static_cast<unsigned>(pages[i]) < static_cast<unsigned>(pg.num_pages)) {
                     const size_t at = (static_cast<size_t>(pages[i]) * pg.heads + h) * a.page_blocks + (blk - page_at(blk) * a.page_blocks);
-                    x[i] = tl::ldg_stream(numbers + at * (kF8Tokens * DIM) + 16 * ((tid + 128 * i) % (kF8Tokens * CH)));
+                    to[i] = tl::ldg_stream(numbers + at * (kF8Tokens * DIM) + 16 * ((tid + 128 * i) % (kF8Tokens * CH)));
                     s[i] = __ldg(scales + at);
                 }
             }
         };
-        auto store = [&](int t, unsigned char *tile, uint4 (&x)[PER], const float (&s)[PER], float under) {
-            const int key0 = first + t * kPoKeys;
-            if (key0 + kPoKeys > ctx) {  // slots behind the last token may hold anything
+        look_up(0), load(0, x[0], scale[0]), look_up(1), load(1, x[1], scale[1]), look_up(2);
+        bool ok = true;
+        for (int t0 = 0; ok && t0 < n_tiles; t0 += 2) {
+            const uint32_t ph = (t0 >> 1 & 1) ^ 1u;  // the first pass through the stages does not wait
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int t = t0 + u, key0 = first + t * kPoKeys;
+                if (t >= n_tiles || !(ok = tc_wait(empty + 8 * u, ph, dead))) break;
+                if (key0 + kPoKeys > ctx) {  // slots behind the last token may hold anything
+#pragma unroll
+                    for (int i = 0; i < PER; ++i)
+                        if (key0 + (tid + 128 * i) / CH >= ctx) x[u][i] = make_uint4(0, 0, 0, 0);
+                }
 #pragma unroll
                 for (int i = 0; i < PER; ++i)
-                    if (key0 + (tid + 128 * i) / CH >= ctx) x[i] = make_uint4(0, 0, 0, 0);
+                    po_store<DIM>(tiles + u * Z::halves * Z::kv_block, (tid + 128 * i) / CH, c, x[u][i], __float2half2_rn(scale[u][i] < INFINITY ? scale[u][i] * under : 0.f));
+                g_fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) g_mbar_arrive(full + 8 * u);
+                load(t + 2, x[u], scale[u]), look_up(t + 3);
             }
-#pragma unroll
-            for (int i = 0; i < PER; ++i) po_store<DIM>(tile, (tid + 128 * i) / CH, c, x[i], __float2half2_rn(s[i] < INFINITY ? s[i] * under : 0.f));
-            g_fence_proxy_async();
-            __syncwarp();
-        };
-        if (n_tiles > 0) look_up(0), load(0, pg.keys, pg.key_scales, kr, ks), load(0, pg.values, pg.value_scales, vr, vs), look_up(1);
-        for (int t = 0; t < n_tiles; ++t) {
-            const int s = t & 1;
-            const uint32_t ph = (t >> 1 & 1) ^ 1u;  // the first pass through the stages does not wait
-            if (!tc_wait(k_empty + 8 * s, ph, dead)) break;
-            store(t, psm + Z::k_off + s * Z::halves * Z::kv_block, kr, ks, under_k);
-            if (lane == 0) g_mbar_arrive(k_full + 8 * s);
-            if (t + 1 < n_tiles) load(t + 1, pg.keys, pg.key_scales, kr, ks);
-            if (!tc_wait(v_empty + 8 * s, ph, dead)) break;
-            store(t, psm + Z::v_off + s * Z::halves * Z::kv_block, vr, vs, under_v);
-            if (lane == 0) g_mbar_arrive(v_full + 8 * s);
-            if (t + 1 < n_tiles) load(t + 1, pg.values, pg.value_scales, vr, vs), look_up(t + 2);
         }
     } else {  // ---- softmax: thread = row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
         const int r = threadIdx.x, col = c0 + r, set = warp >> 2;
         const uint32_t s_mine = s_full + 16 * set, p_mine = p_full + 16 * set, pv_mine = pv_done + 16 * set;
         const bool live = col < columns;
@@ -298,10 +329,12 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
                     }
                 }
             }
-            float top = -INFINITY;
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < kPoKeys; ++c) top = fmaxf(top, __uint_as_float(s[c >> 5][c & 31]));
-            top *= mult;
+            for (int c = 0; c < kPoKeys; c += 8)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tops[i] = po_max3(tops[i], __uint_as_float(s[c >> 5][(c & 31) + 2 * i]), __uint_as_float(s[c >> 5][(c & 31) + 2 * i + 1]));
+            const float top = po_max3(fmaxf(tops[0], tops[1]), tops[2], tops[3]) * mult;
             const bool grow = top > m + kAtLag || (m == -INFINITY && top > m);
             if (__any_sync(0xffffffffu, grow)) {
                 if (t > 0) {
@@ -323,15 +356,17 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
             }
             const float at = m == -INFINITY ? 0.f : m;
             uint32_t pk[32];
-            float s0 = 0.f, s1 = 0.f;
+            const uint64_t mult2 = po_two(mult, mult), minus = po_two(-at, -at);
+            uint64_t sums[2] = {0, 0};  // two pairs of zeros
 #pragma unroll
             for (int c = 0; c < kPoKeys; c += 2) {
-                const float u = __uint_as_float(s[c >> 5][c & 31]), v = __uint_as_float(s[c >> 5][(c & 31) + 1]);
-                const float x = at_ex2(fmaf(u, mult, -at)), y = at_ex2(fmaf(v, mult, -at));
+                const float2 z = po_each(po_fma2(po_two(__uint_as_float(s[c >> 5][c & 31]), __uint_as_float(s[c >> 5][(c & 31) + 1])), mult2, minus));
+                const float x = at_ex2(z.x), y = at_ex2(z.y);
                 pk[c / 2] = tl::pack2<__half>(x, y);
-                s0 += x, s1 += y;
+                sums[(c >> 1) & 1] = po_add2(sums[(c >> 1) & 1], po_two(x, y));
             }
-            sum += s0 + s1;
+            const float2 both = po_each(po_add2(sums[0], sums[1]));
+            sum += both.x + both.y;
             g_tmem_st32(tmem + lanes + s2 * kPoKeys, pk);  // column c = keys 2 c and 2 c + 1
             g_tmem_st_wait();
             g_tc_fence_before();
@@ -377,7 +412,7 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
     }
     g_tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 16) {
         tc_settle(dead);
         g_tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kPoColumns) : "memory");
