@@ -7,8 +7,9 @@
 //
 // A CTA takes 256 columns of one request and key/value head, or a piece of their keys, as two sets of 128 rows (tensor-memory lanes) that work on the same keys, so that one's
 // exponentials run beside the other's products and the cache's numbers are turned into operands once for both.  Per 64 keys:
-//   warps 8-15   turn keys (the first four) and values into f16 operand tiles (128-byte swizzle) of two stages each, the bytes of the next two tiles on their way in registers
-//   warp 16      tcgen05.mma, one elected lane: of either set S = Q K^T into one of two score buffers, O += P V; the next tile's scores are issued ahead of this tile's values
+//   warps 8-15   turn keys (the first four) and values into f16 operand tiles (128-byte swizzle) of two stages each, the next tile's bytes on their way in registers meanwhile
+//   warps 16, 17 tcgen05.mma, one elected lane, a set each: S = Q K^T into one of two score buffers, O += P V; the next tile's scores are issued ahead of this tile's values.
+//                (One warp for both sets took 2000 cycles to issue a tile's 24 products of 32 cycles each.)
 //   warps 0-7    softmax, thread = row: scores from tensor memory, 2^x of them over a running maximum that may lag behind by 2^8, P as f16 back over its own scores
 #include "../per_device.h"
 #include "blocks_fp8_attention.cuh"
@@ -25,7 +26,7 @@ using tl::g_tmem_st_wait;
 
 constexpr int kPoKeys = 64;
 constexpr int kPoSet = 128;  // rows of a set
-// The last three warps have nothing to do: registers are moved between groups of four warps (144, 144, 72, 72 and 48 are five times the launch's 96).
+// The last two warps have nothing to do: registers are moved between groups of four warps (144, 144, 72, 72 and 48 are five times the launch's 96).
 constexpr int kPoThreads = 20 * 32;
 constexpr int kPoColumns = 512;      // of tensor memory; a set's half: two score buffers of 64, the output from 128 on
 constexpr uint32_t kPoHalf = 256, kPoOut = 128;
@@ -124,7 +125,7 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
     float *row_factor = reinterpret_cast<float *>(psm + Z::row_off);
     if (threadIdx.x == 0) {
         for (int i = 0; i < 4; ++i) g_mbar_init(s_full + 8 * i, 1), g_mbar_init(p_full + 8 * i, 4), g_mbar_init(pv_done + 8 * i, 1);
-        for (int i = 0; i < 2; ++i) g_mbar_init(k_full + 8 * i, 4), g_mbar_init(k_empty + 8 * i, 1), g_mbar_init(v_full + 8 * i, 4), g_mbar_init(v_empty + 8 * i, 1);
+        for (int i = 0; i < 2; ++i) g_mbar_init(k_full + 8 * i, 4), g_mbar_init(k_empty + 8 * i, 2), g_mbar_init(v_full + 8 * i, 4), g_mbar_init(v_empty + 8 * i, 2);
         *dead = 0, seen[0] = 0, seen[1] = 0, seen[2] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -134,49 +135,83 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
     }
     __syncthreads();
 
-    // the largest scales
-    for (int blk = begin + threadIdx.x; blk < stop; blk += kPoThreads) {
-        int page;
-        const size_t at = block_at(blk, page);
-        const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(pg.num_pages);
-        const float k = there ? __ldg(pg.key_scales + at) : NAN, v = there ? __ldg(pg.value_scales + at) : NAN;
-        if (k < INFINITY) atomicMax(seen, __float_as_int(k));
-        if (v < INFINITY) atomicMax(seen + 1, __float_as_int(v));
-        if (!(k < INFINITY) || !(v < INFINITY)) seen[2] = 1;
-    }
-    // queries: 8 entries a thread, a row to 8 or 16 lanes
-    if (warp < 8) {
-        constexpr int LANES = DIM / 8, ROWS = 32 / LANES, STEP = 8 * ROWS, N = kPoRows / STEP;  // the eight softmax warps
+    // the converting warps' side of a tile: a thread's i-th piece is in row (tid + 128 i) / CH, part of a block of 16 rows
+    const bool values = warp >= 12;
+    const uint8_t *numbers = values ? pg.values : pg.keys;
+    const float *scales = values ? pg.value_scales : pg.key_scales;
+    const int tid = threadIdx.x & 127, c = tid % CH;
+    uint4 x[PER];
+    float scale[PER];
+    int pages[PER];  // of the tile whose bytes are next to be asked for
+    auto block_of = [&](int t, int i) { return begin + t * (kPoKeys / kF8Tokens) + (tid + 128 * i) / (kF8Tokens * CH); };
+    auto look_up = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int blk = min(block_of(t, i), max(stop - 1, 0));
+            pages[i] = table[page_at(blk)];
+        }
+    };
+    auto load = [&](int t) {  // of a page that is none, the first page's bytes, which count as zeros; no branch, so that the addresses are made side by side
+        size_t at[PER];
+        bool there[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int blk = block_of(t, i);
+            there[i] = blk < stop && static_cast<unsigned>(pages[i]) < static_cast<unsigned>(pg.num_pages);
+            at[i] = (static_cast<size_t>(there[i] ? pages[i] : 0) * pg.heads + h) * a.page_blocks + (there[i] ? blk - page_at(blk) * a.page_blocks : 0);
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) x[i] = tl::ldg_stream(numbers + at[i] * (kF8Tokens * DIM) + 16 * ((tid + 128 * i) % (kF8Tokens * CH)));
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            scale[i] = __ldg(scales + at[i]);
+            if (!there[i]) scale[i] = -1.f;
+        }
+    };
+    if (warp >= 8 && warp < 16 && n_tiles > 0) look_up(0), load(0), look_up(1);
+    if (warp >= 8) {  // the largest scales
+        for (int blk = begin + threadIdx.x - 8 * 32; blk < stop; blk += kPoThreads - 8 * 32) {
+            int page;
+            const size_t at = block_at(blk, page);
+            const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(pg.num_pages);
+            const float k = there ? __ldg(pg.key_scales + at) : NAN, v = there ? __ldg(pg.value_scales + at) : NAN;
+            if (k < INFINITY) atomicMax(seen, __float_as_int(k));
+            if (v < INFINITY) atomicMax(seen + 1, __float_as_int(v));
+            if (!(k < INFINITY) || !(v < INFINITY)) seen[2] = 1;
+        }
+    } else {  // queries: 8 entries a lane, a row to 8 or 16 lanes
+        constexpr int LANES = DIM / 8, ROWS = 32 / LANES, STEP = 8 * ROWS, N = kPoRows / STEP;
         const bf16 *q = static_cast<const bf16 *>(a.q) + b * a.q_b + static_cast<long long>(h) * G * a.q_h + lane % LANES * 8;
         const float sign = a.scale_log2 < 0.f ? -1.f : 1.f;
-        constexpr int HALF = N / 4;
+        for (int i0 = 0; i0 < N; i0 += N / 2) {
+            uint4 raw[N / 2];
 #pragma unroll
-        for (int part = 0; part < 4; ++part) {
-            float x[HALF][8];
-#pragma unroll
-            for (int i = 0; i < HALF; ++i) {
-                const int row = warp * ROWS + lane / LANES + (part * HALF + i) * STEP, col = c0 + row;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
-                if (col < columns) {
-                    const int l = at_div(col, G, a.group_magic);
-                    at_query(q + l * a.q_l + (col - l * G) * a.q_h, a.wide_rows, x[i]);
+            for (int i = 0; i < N / 2; ++i) {
+                const int col = c0 + warp * ROWS + lane / LANES + (i0 + i) * STEP, l = at_div(min(col, columns - 1), G, a.group_magic);
+                const bf16 *from = q + l * a.q_l + (min(col, columns - 1) - l * G) * a.q_h;
+                if (a.wide_rows) {
+                    raw[i] = *reinterpret_cast<const uint4 *>(from);
+                } else {
+                    const uint16_t *e = reinterpret_cast<const uint16_t *>(from);
+                    raw[i] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
                 }
+                if (col >= columns) raw[i] = make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
-            for (int i = 0; i < HALF; ++i) {
-                const int row = warp * ROWS + lane / LANES + (part * HALF + i) * STEP;
+            for (int i = 0; i < N / 2; ++i) {
+                const int row = warp * ROWS + lane / LANES + (i0 + i) * STEP;
+                const float2 y[4] = {tl::unpack2<bf16>(raw[i].x), tl::unpack2<bf16>(raw[i].y), tl::unpack2<bf16>(raw[i].z), tl::unpack2<bf16>(raw[i].w)};
                 float m = 0.f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) m = f8_most(m, fabsf(x[i][e]));
+                for (int e = 0; e < 4; ++e) m = f8_most(m, f8_most(fabsf(y[e].x), fabsf(y[e].y)));
 #pragma unroll
                 for (int o = 1; o < LANES; o <<= 1) m = f8_most(m, __shfl_xor_sync(0xffffffffu, m, o));
                 const int e2 = static_cast<int>(__float_as_uint(m) >> 23), up = e2 == 255 ? 0 : min(13 + 127 - e2, 100);
                 const float times = f8_power(up) * sign;
                 const int j = lane % LANES, in_set = row % kPoSet;
                 uint4 f;
-                f.x = tl::pack2<__half>(x[i][0] * times, x[i][1] * times), f.y = tl::pack2<__half>(x[i][2] * times, x[i][3] * times);
-                f.z = tl::pack2<__half>(x[i][4] * times, x[i][5] * times), f.w = tl::pack2<__half>(x[i][6] * times, x[i][7] * times);
+                f.x = tl::pack2<__half>(y[0].x * times, y[0].y * times), f.y = tl::pack2<__half>(y[1].x * times, y[1].y * times);
+                f.z = tl::pack2<__half>(y[2].x * times, y[2].y * times), f.w = tl::pack2<__half>(y[3].x * times, y[3].y * times);
                 *reinterpret_cast<uint4 *>(psm + (row / kPoSet * Z::halves + (j >> 3)) * Z::q_block + in_set * 128 + (((j & 7) ^ (in_set & 7)) << 4)) = f;
                 if (j == 0) row_factor[row] = f8_power(-up);
             }
@@ -190,10 +225,12 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
     // 1 over the largest scales; both are powers of two
     const float top_k = seen[0] ? __int_as_float(seen[0]) : 1.f, top_v = seen[1] ? __int_as_float(seen[1]) : 1.f, under_k = 1.f / top_k, under_v = 1.f / top_v;
 
-    if (warp >= 16) {  // ---- products: of either set S_0, then per tile S_(t+1), P_t V_t
+    if (warp >= 16) {  // ---- products: S_0, then per tile S_(t+1), P_t V_t
         asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         constexpr uint32_t idesc_s = po_idesc(kPoKeys, false), idesc_o = po_idesc(DIM, true);
-        const uint64_t qd = g_smem_desc_sw128(base, 0, 1024), kd0 = g_smem_desc_sw128(k_at, 0, 1024), vd0 = g_smem_desc_sw128(v_at, Z::kv_block, 1024);
+        const int set = warp & 1;
+        const uint32_t scores_at = tmem + set * kPoHalf, out_at = scores_at + kPoOut;
+        const uint64_t qd = g_smem_desc_sw128(base + set * Z::halves * Z::q_block, 0, 1024), kd0 = g_smem_desc_sw128(k_at, 0, 1024), vd0 = g_smem_desc_sw128(v_at, Z::kv_block, 1024);
         auto scores = [&](int t) {
             const int s = t & 1;
             if (!tc_wait(k_full + 8 * s, t >> 1 & 1, dead)) return false;
@@ -201,94 +238,47 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
             if (g_elect_one()) {
                 const uint64_t kd = kd0 + static_cast<uint64_t>(s * Z::halves * (Z::kv_block >> 4));
 #pragma unroll
-                for (int set = 0; set < 2; ++set) {
-#pragma unroll
-                    for (int k = 0; k < DIM / 16; ++k)
-                        g_tc_mma(tmem + set * kPoHalf + s * kPoKeys, qd + (set * Z::halves + (k >> 2)) * (Z::q_block >> 4) + 2 * (k & 3), kd + (k >> 2) * (Z::kv_block >> 4) + 2 * (k & 3),
-                                 idesc_s, k > 0);
-                    g_tc_commit(s_full + 16 * set + 8 * s);
-                }
+                for (int k = 0; k < DIM / 16; ++k)
+                    g_tc_mma(scores_at + s * kPoKeys, qd + (k >> 2) * (Z::q_block >> 4) + 2 * (k & 3), kd + (k >> 2) * (Z::kv_block >> 4) + 2 * (k & 3), idesc_s, k > 0);
+                g_tc_commit(s_full + 16 * set + 8 * s);
                 g_tc_commit(k_empty + 8 * s);
             }
             __syncwarp();
             return true;
         };
-        const bool begun = warp == 16 && n_tiles > 0 && scores(0);
+        const bool begun = warp < 18 && n_tiles > 0 && scores(0);
         for (int t = 0; begun && t < n_tiles; ++t) {
             const int s = t & 1;
-            if (t + 1 < n_tiles && !scores(t + 1)) break;  // its buffers held P_(t-1), read by products already queued ahead of this one
-            if (!tc_wait(v_full + 8 * s, t >> 1 & 1, dead)) break;
-            bool ok = true;
+            if (t + 1 < n_tiles && !scores(t + 1)) break;  // its buffer held P_(t-1), read by a product already queued ahead of this one
+            if (!tc_wait(v_full + 8 * s, t >> 1 & 1, dead) || !tc_wait(p_full + 16 * set + 8 * s, t >> 1 & 1, dead)) break;
+            g_tc_fence_after();
+            if (g_elect_one()) {
+                const uint64_t vd = vd0 + static_cast<uint64_t>(s * Z::halves * (Z::kv_block >> 4));
 #pragma unroll
-            for (int set = 0; set < 2; ++set) {
-                if (!(ok = ok && tc_wait(p_full + 16 * set + 8 * s, t >> 1 & 1, dead))) break;
-                g_tc_fence_after();
-                if (g_elect_one()) {
-                    const uint64_t vd = vd0 + static_cast<uint64_t>(s * Z::halves * (Z::kv_block >> 4));
-#pragma unroll
-                    for (int k = 0; k < kPoKeys / 16; ++k)
-                        g_tc_mma_ts(tmem + set * kPoHalf + kPoOut, tmem + set * kPoHalf + s * kPoKeys + 8 * k, vd + k * (2048 >> 4), idesc_o, t > 0 || k > 0);
-                    if (set) g_tc_commit(v_empty + 8 * s);
-                    g_tc_commit(pv_done + 16 * set + 8 * s);
-                }
-                __syncwarp();
+                for (int k = 0; k < kPoKeys / 16; ++k) g_tc_mma_ts(out_at, scores_at + s * kPoKeys + 8 * k, vd + k * (2048 >> 4), idesc_o, t > 0 || k > 0);
+                g_tc_commit(v_empty + 8 * s);
+                g_tc_commit(pv_done + 16 * set + 8 * s);
             }
-            if (!ok) break;
+            __syncwarp();
         }
     } else if (warp >= 8) {  // ---- pages to operands
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        const bool values = warp >= 12;
-        const uint8_t *numbers = values ? pg.values : pg.keys;
-        const float *scales = values ? pg.value_scales : pg.key_scales;
         const float under = values ? under_v : under_k;
         unsigned char *tiles = psm + (values ? Z::v_off : Z::k_off);
         const uint32_t full = values ? v_full : k_full, empty = values ? v_empty : k_empty;
-        // a thread's i-th piece of a tile: row (tid + 128 i) / CH, in the block of 16 rows that it is part of
-        const int tid = threadIdx.x & 127, c = tid % CH;
-        uint4 x[2][PER];
-        float scale[2][PER];
-        int pages[PER];  // of the tile whose bytes are next to be asked for
-        auto block_of = [&](int t, int i) { return begin + t * (kPoKeys / kF8Tokens) + (tid + 128 * i) / (kF8Tokens * CH); };
-        auto look_up = [&](int t) {
+        for (int t = 0; t < n_tiles; ++t) {
+            const int s = t & 1, key0 = first + t * kPoKeys;
+            if (!tc_wait(empty + 8 * s, (t >> 1 & 1) ^ 1u, dead)) break;  // the first pass through the stages does not wait
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
-                const int blk = block_of(t, i);
-                pages[i] = blk < stop ? table[page_at(blk)] : -1;
+                // a page that is none, and slots behind the last token, may hold anything
+                if (scale[i] < 0.f || key0 + (tid + 128 * i) / CH >= ctx) x[i] = make_uint4(0, 0, 0, 0);
+                po_store<DIM>(tiles + s * Z::halves * Z::kv_block, (tid + 128 * i) / CH, c, x[i], __float2half2_rn(scale[i] < INFINITY ? fabsf(scale[i]) * under : 0.f));
             }
-        };
-        auto load = [&](int t, uint4 (&to)[PER], float (&s)[PER]) {
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const int blk = block_of(t, i);
-                to[i] = make_uint4(0, 0, 0, 0), s[i] = 0.f;
-                if (static_cast<unsigned>(pages[i]) < static_cast<unsigned>(pg.num_pages)) {
-                    const size_t at = (static_cast<size_t>(pages[i]) * pg.heads + h) * a.page_blocks + (blk - page_at(blk) * a.page_blocks);
-                    to[i] = tl::ldg_stream(numbers + at * (kF8Tokens * DIM) + 16 * ((tid + 128 * i) % (kF8Tokens * CH)));
-                    s[i] = __ldg(scales + at);
-                }
-            }
-        };
-        look_up(0), load(0, x[0], scale[0]), look_up(1), load(1, x[1], scale[1]), look_up(2);
-        bool ok = true;
-        for (int t0 = 0; ok && t0 < n_tiles; t0 += 2) {
-            const uint32_t ph = (t0 >> 1 & 1) ^ 1u;  // the first pass through the stages does not wait
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int t = t0 + u, key0 = first + t * kPoKeys;
-                if (t >= n_tiles || !(ok = tc_wait(empty + 8 * u, ph, dead))) break;
-                if (key0 + kPoKeys > ctx) {  // slots behind the last token may hold anything
-#pragma unroll
-                    for (int i = 0; i < PER; ++i)
-                        if (key0 + (tid + 128 * i) / CH >= ctx) x[u][i] = make_uint4(0, 0, 0, 0);
-                }
-#pragma unroll
-                for (int i = 0; i < PER; ++i)
-                    po_store<DIM>(tiles + u * Z::halves * Z::kv_block, (tid + 128 * i) / CH, c, x[u][i], __float2half2_rn(scale[u][i] < INFINITY ? scale[u][i] * under : 0.f));
-                g_fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) g_mbar_arrive(full + 8 * u);
-                load(t + 2, x[u], scale[u]), look_up(t + 3);
-            }
+            g_fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) g_mbar_arrive(full + 8 * s);
+            if (t + 1 < n_tiles) load(t + 1), look_up(t + 2);
         }
     } else {  // ---- softmax: thread = row
         asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
