@@ -4,7 +4,7 @@
 // column being one (query head of the group, new token).  An e4m3 number is an f16 number, so the cache's side is exact; a column is brought to the top of
 // f16's range by a power of two, where bf16 keeps all its bits, and an fp32 query is two such terms.  The scales never meet f16: a block's
 // key scale multiplies its scores and its value scale the product of its weights and values, both in fp32.  Weights are exp2 of a number up to the
-// column's running maximum (which may lag behind by 2^8 before the sums are scaled again), rounded to f16 for the second product: 2^-12 of a weight, where an output is
+// column's running maximum (which may lag behind by 2^15 before the sums are scaled again), rounded to f16 for the second product: 2^-12 of a weight, where an output is
 // rounded to 2^-9 of itself; fp32 outputs take a second term for the rest.  Running sums are fp32.
 //
 // A warp takes blocks of 16 keys through a ring of its own in shared memory, filled by asynchronous copies, two blocks ahead of the one it works on; it waits for nobody

@@ -23,7 +23,7 @@ struct F8Attend : tlb_fp8_attention_call {
     }
 };
 
-constexpr float kAtLag = 8.f;   // log2: how far a running maximum may lag behind
+constexpr float kAtLag = 15.f;  // log2: how far a running maximum may lag behind: weights up to 2^15 are f16 numbers
 constexpr int kAtLeast = 32;    // blocks of a piece at the least
 
 __device__ __forceinline__ float at_ex2(float x) {

@@ -10,7 +10,7 @@
 //   warps 8-15   turn keys (the first four) and values into f16 operand tiles (128-byte swizzle) of two stages each, the next tile's bytes on their way in registers meanwhile
 //   warps 16, 17 tcgen05.mma, one elected lane, a set each: S = Q K^T into one of two score buffers, O += P V; the next tile's scores are issued ahead of this tile's values.
 //                (One warp for both sets took 2000 cycles to issue a tile's 24 products of 32 cycles each.)
-//   warps 0-7    softmax, thread = row: scores from tensor memory, 2^x of them over a running maximum that may lag behind by 2^8, P as f16 back over its own scores
+//   warps 0-7    softmax, thread = row: scores from tensor memory, 2^x of them over a running maximum that may lag behind by 2^15, P as f16 back over its own scores
 #include "../per_device.h"
 #include "blocks_fp8_attention.cuh"
 #include "blocks_tc.cuh"
