@@ -19,8 +19,6 @@ namespace tlb {
 
 using tl::g_fence_proxy_async;
 using tl::g_tmem_ld32;
-using tl::g_tmem_ld32_nowait;
-using tl::g_tmem_ld_wait;
 using tl::g_tmem_st32;
 using tl::g_tmem_st_wait;
 
@@ -31,6 +29,13 @@ constexpr int kPoThreads = 20 * 32;
 constexpr int kPoColumns = 512;      // of tensor memory; a set's half: two score buffers of 64, the output from 128 on
 constexpr uint32_t kPoHalf = 256, kPoOut = 128;
 
+// Asynchronous copies; zeros where `there` is false.
+__device__ __forceinline__ void po_copy16(uint32_t to, const void *from, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void po_copy4(uint32_t to, const void *from, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
+}
 __device__ __forceinline__ float po_max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -58,6 +63,13 @@ __device__ __forceinline__ uint64_t po_add2(uint64_t a, uint64_t b) {
     return r;
 }
 
+// 16 columns of the warp's 32 lanes.
+__device__ __forceinline__ void po_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+
 // kind::f16, f16 x f16 -> f32, 128 rows
 __host__ __device__ constexpr uint32_t po_idesc(int n, bool b_mn) { return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24); }
 
@@ -66,12 +78,13 @@ struct PoShape {
     static constexpr int halves = DIM / 64;                                // 64-column blocks
     static constexpr int q_block = kPoSet * 128, kv_block = kPoKeys * 128;  // bytes
     static constexpr int k_off = 2 * halves * q_block, v_off = k_off + 2 * halves * kv_block, bar_off = v_off + 2 * halves * kv_block;
-    static constexpr int row_off = bar_off + 256, smem = row_off + kPoRows * 4;
+    // behind the row factors: the bytes of two tiles of either side
+    static constexpr int row_off = bar_off + 256, raw_off = row_off + kPoRows * 4, raw_tile = kPoKeys * DIM, smem = raw_off + 4 * raw_tile;
+    static_assert(4 * halves * kv_block >= kPoRows * DIM * 2, "the queries as they come fit where the operand tiles will be");
 };
 
-// 16 e4m3 numbers (entries 16 c .. of a row) times `ratio`, as f16, into their places in a tile of 64-column blocks.
-template <int DIM>
-__device__ __forceinline__ void po_store(unsigned char *tile, int row, int c, uint4 raw, __half2 ratio) {
+// 16 e4m3 numbers times `ratio` (two alike), as f16, to the two places of a row.
+__device__ __forceinline__ void po_store(unsigned char *one, unsigned char *two, uint4 raw, uint32_t ratio) {
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
     uint32_t f[8];
 #pragma unroll
@@ -79,15 +92,11 @@ __device__ __forceinline__ void po_store(unsigned char *tile, int row, int c, ui
         at_halves(w[i], f[2 * i], f[2 * i + 1]);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const __half2 v = __hmul2(*reinterpret_cast<__half2 *>(&f[2 * i + e]), ratio);
+            const __half2 v = __hmul2(*reinterpret_cast<__half2 *>(&f[2 * i + e]), *reinterpret_cast<const __half2 *>(&ratio));
             f[2 * i + e] = *reinterpret_cast<const uint32_t *>(&v);
         }
     }
-    unsigned char *at = tile + (c >> 2) * PoShape<DIM>::kv_block + row * 128;
-    const int j = 2 * (c & 3), odd = (c >> 2) & 1;  // the second block's lanes write their second half first: eight lanes meet all banks
-    const uint4 one = make_uint4(f[0], f[1], f[2], f[3]), two = make_uint4(f[4], f[5], f[6], f[7]);
-    *reinterpret_cast<uint4 *>(at + (((j + odd) ^ (row & 7)) << 4)) = odd ? two : one;
-    *reinterpret_cast<uint4 *>(at + (((j + 1 - odd) ^ (row & 7)) << 4)) = odd ? one : two;
+    *reinterpret_cast<uint4 *>(one) = make_uint4(f[0], f[1], f[2], f[3]), *reinterpret_cast<uint4 *>(two) = make_uint4(f[4], f[5], f[6], f[7]);
 }
 
 template <int DIM>
@@ -135,40 +144,32 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
     }
     __syncthreads();
 
-    // the converting warps' side of a tile: a thread's i-th piece is in row (tid + 128 i) / CH, part of a block of 16 rows
+    // the converting warps: a thread's i-th piece of a tile is in row (tid + 128 i) / CH, part of the block (tid + 128 i) / (16 CH); it copies, reads and converts
+    // its own pieces, so they wait for nobody.  Lane j knows where block j of the tile that is asked for next lies, and the scales of those that were.
     const bool values = warp >= 12;
-    const uint8_t *numbers = values ? pg.values : pg.keys;
+    const int tid = threadIdx.x & 127;
+    const uint32_t raw_at = base + Z::raw_off + (values ? 2 * Z::raw_tile : 0) + 16 * tid;
+    const uint8_t *numbers = (values ? pg.values : pg.keys) + 16 * tid;
     const float *scales = values ? pg.value_scales : pg.key_scales;
-    const int tid = threadIdx.x & 127, c = tid % CH;
-    uint4 x[PER];
-    float scale[PER];
-    int pages[PER];  // of the tile whose bytes are next to be asked for
-    auto block_of = [&](int t, int i) { return begin + t * (kPoKeys / kF8Tokens) + (tid + 128 * i) / (kF8Tokens * CH); };
+    int place = -1;  // of a block among all pages' (fewer than 2^31: they are 16 rows each); -1: none
+    float scale_next = 0.f, scale_after = 0.f;
     auto look_up = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int blk = min(block_of(t, i), max(stop - 1, 0));
-            pages[i] = table[page_at(blk)];
-        }
+        const int blk = begin + t * (kPoKeys / kF8Tokens) + lane, at = page_at(blk);
+        const int page = lane < kPoKeys / kF8Tokens && blk < stop ? table[at] : -1;
+        place = static_cast<unsigned>(page) < static_cast<unsigned>(pg.num_pages) ? (page * pg.heads + h) * a.page_blocks + blk - at * a.page_blocks : -1;
     };
-    auto load = [&](int t) {  // of a page that is none, the first page's bytes, which count as zeros; no branch, so that the addresses are made side by side
-        size_t at[PER];
-        bool there[PER];
+    auto ask = [&](int t) {  // of a page that is none: zeros
+        scale_next = scale_after, scale_after = place < 0 ? 0.f : __ldg(scales + place);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int blk = block_of(t, i);
-            there[i] = blk < stop && static_cast<unsigned>(pages[i]) < static_cast<unsigned>(pg.num_pages);
-            at[i] = (static_cast<size_t>(there[i] ? pages[i] : 0) * pg.heads + h) * a.page_blocks + (there[i] ? blk - page_at(blk) * a.page_blocks : 0);
+            const int at = __shfl_sync(0xffffffffu, place, (tid + 128 * i) / (kF8Tokens * CH));
+            const size_t byte = static_cast<size_t>(static_cast<unsigned>(max(at, 0))) * (kF8Tokens * DIM);
+            // the pieces before this thread's i-th that are not of its block
+            po_copy16(raw_at + (t & 1) * Z::raw_tile + 2048 * i, numbers + byte + (DIM == 128 ? 0 : -(tid / 64) * 1024), at >= 0);
         }
-#pragma unroll
-        for (int i = 0; i < PER; ++i) x[i] = tl::ldg_stream(numbers + at[i] * (kF8Tokens * DIM) + 16 * ((tid + 128 * i) % (kF8Tokens * CH)));
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            scale[i] = __ldg(scales + at[i]);
-            if (!there[i]) scale[i] = -1.f;
-        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    if (warp >= 8 && warp < 16 && n_tiles > 0) look_up(0), load(0), look_up(1);
+    if (warp >= 8 && warp < 16) look_up(0), ask(0), look_up(1), ask(1), look_up(2);
     if (warp >= 8) {  // the largest scales
         for (int blk = begin + threadIdx.x - 8 * 32; blk < stop; blk += kPoThreads - 8 * 32) {
             int page;
@@ -179,42 +180,41 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
             if (v < INFINITY) atomicMax(seen + 1, __float_as_int(v));
             if (!(k < INFINITY) || !(v < INFINITY)) seen[2] = 1;
         }
-    } else {  // queries: 8 entries a lane, a row to 8 or 16 lanes
-        constexpr int LANES = DIM / 8, ROWS = 32 / LANES, STEP = 8 * ROWS, N = kPoRows / STEP;
+    } else {  // queries: 8 entries a lane, a row to 8 or 16 lanes; first as they are, to where the operand tiles will be
+        constexpr int LANES = DIM / 8, ROWS = 32 / LANES, N = kPoRows / (8 * ROWS);
         const bf16 *q = static_cast<const bf16 *>(a.q) + b * a.q_b + static_cast<long long>(h) * G * a.q_h + lane % LANES * 8;
         const float sign = a.scale_log2 < 0.f ? -1.f : 1.f;
-        for (int i0 = 0; i0 < N; i0 += N / 2) {
-            uint4 raw[N / 2];
-#pragma unroll
-            for (int i = 0; i < N / 2; ++i) {
-                const int col = c0 + warp * ROWS + lane / LANES + (i0 + i) * STEP, l = at_div(min(col, columns - 1), G, a.group_magic);
-                const bf16 *from = q + l * a.q_l + (min(col, columns - 1) - l * G) * a.q_h;
-                if (a.wide_rows) {
-                    raw[i] = *reinterpret_cast<const uint4 *>(from);
-                } else {
-                    const uint16_t *e = reinterpret_cast<const uint16_t *>(from);
-                    raw[i] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-                }
-                if (col >= columns) raw[i] = make_uint4(0, 0, 0, 0);
+        unsigned char *mine_q = psm + Z::k_off + (warp * 32 + lane) * 16;
+#pragma unroll 2
+        for (int i = 0; i < N; ++i) {
+            const int col = c0 + (i * 8 + warp) * ROWS + lane / LANES, l = at_div(min(col, columns - 1), G, a.group_magic);
+            const bf16 *from = q + l * a.q_l + (min(col, columns - 1) - l * G) * a.q_h;
+            if (a.wide_rows) {
+                po_copy16(g_smem_u32(mine_q + i * 4096), from, col < columns);
+            } else {
+#pragma unroll 1
+                for (int e = 0; e < 8; ++e) reinterpret_cast<bf16 *>(mine_q + i * 4096)[e] = col < columns ? from[e] : __float2bfloat16_rn(0.f);
             }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 2
+        for (int i = 0; i < N; ++i) {
+            const int row = (i * 8 + warp) * ROWS + lane / LANES;
+            const uint4 u = *reinterpret_cast<const uint4 *>(mine_q + i * 4096);
+            const float2 y[4] = {tl::unpack2<bf16>(u.x), tl::unpack2<bf16>(u.y), tl::unpack2<bf16>(u.z), tl::unpack2<bf16>(u.w)};
+            float m = 0.f;
 #pragma unroll
-            for (int i = 0; i < N / 2; ++i) {
-                const int row = warp * ROWS + lane / LANES + (i0 + i) * STEP;
-                const float2 y[4] = {tl::unpack2<bf16>(raw[i].x), tl::unpack2<bf16>(raw[i].y), tl::unpack2<bf16>(raw[i].z), tl::unpack2<bf16>(raw[i].w)};
-                float m = 0.f;
+            for (int e = 0; e < 4; ++e) m = f8_most(m, f8_most(fabsf(y[e].x), fabsf(y[e].y)));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) m = f8_most(m, f8_most(fabsf(y[e].x), fabsf(y[e].y)));
-#pragma unroll
-                for (int o = 1; o < LANES; o <<= 1) m = f8_most(m, __shfl_xor_sync(0xffffffffu, m, o));
-                const int e2 = static_cast<int>(__float_as_uint(m) >> 23), up = e2 == 255 ? 0 : min(13 + 127 - e2, 100);
-                const float times = f8_power(up) * sign;
-                const int j = lane % LANES, in_set = row % kPoSet;
-                uint4 f;
-                f.x = tl::pack2<__half>(y[0].x * times, y[0].y * times), f.y = tl::pack2<__half>(y[1].x * times, y[1].y * times);
-                f.z = tl::pack2<__half>(y[2].x * times, y[2].y * times), f.w = tl::pack2<__half>(y[3].x * times, y[3].y * times);
-                *reinterpret_cast<uint4 *>(psm + (row / kPoSet * Z::halves + (j >> 3)) * Z::q_block + in_set * 128 + (((j & 7) ^ (in_set & 7)) << 4)) = f;
-                if (j == 0) row_factor[row] = f8_power(-up);
-            }
+            for (int o = 1; o < LANES; o <<= 1) m = f8_most(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const int e2 = static_cast<int>(__float_as_uint(m) >> 23), up = e2 == 255 ? 0 : min(13 + 127 - e2, 100);
+            const float times = f8_power(up) * sign;
+            const int j = lane % LANES, in_set = row % kPoSet;
+            uint4 f;
+            f.x = tl::pack2<__half>(y[0].x * times, y[0].y * times), f.y = tl::pack2<__half>(y[1].x * times, y[1].y * times);
+            f.z = tl::pack2<__half>(y[2].x * times, y[2].y * times), f.w = tl::pack2<__half>(y[3].x * times, y[3].y * times);
+            *reinterpret_cast<uint4 *>(psm + (row / kPoSet * Z::halves + (j >> 3)) * Z::q_block + in_set * 128 + (((j & 7) ^ (in_set & 7)) << 4)) = f;
+            if (j == 0) row_factor[row] = f8_power(-up);
         }
         g_fence_proxy_async();
     }
@@ -266,20 +266,31 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
         const float under = values ? under_v : under_k;
         unsigned char *tiles = psm + (values ? Z::v_off : Z::k_off);
         const uint32_t full = values ? v_full : k_full, empty = values ? v_empty : k_empty;
+        // a thread's first piece in the operand tile; its others lie 128 / CH rows further each, so in the same places of their groups of eight rows.  The second 64 columns'
+        // lanes write their second half first: eight lanes meet all banks
+        const int row0 = tid / CH, c = tid % CH, odd = (c >> 2) & 1;
+        unsigned char *at = tiles + (c >> 2) * Z::kv_block + row0 * 128;
+        unsigned char *one = at + (((2 * (c & 3) + odd) ^ (row0 & 7)) << 4), *two = at + (((2 * (c & 3) + 1 - odd) ^ (row0 & 7)) << 4);
         for (int t = 0; t < n_tiles; ++t) {
             const int s = t & 1, key0 = first + t * kPoKeys;
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            const __half2 r2 = __float2half2_rn(scale_next < INFINITY ? scale_next * under : 0.f);
+            const uint32_t ratio = *reinterpret_cast<const uint32_t *>(&r2);
             if (!tc_wait(empty + 8 * s, (t >> 1 & 1) ^ 1u, dead)) break;  // the first pass through the stages does not wait
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
-                // a page that is none, and slots behind the last token, may hold anything
-                if (scale[i] < 0.f || key0 + (tid + 128 * i) / CH >= ctx) x[i] = make_uint4(0, 0, 0, 0);
-                po_store<DIM>(tiles + s * Z::halves * Z::kv_block, (tid + 128 * i) / CH, c, x[i], __float2half2_rn(scale[i] < INFINITY ? fabsf(scale[i]) * under : 0.f));
+                uint4 x = *reinterpret_cast<const uint4 *>(psm + (raw_at - base) + s * Z::raw_tile + 2048 * i);
+                if (key0 + kPoKeys > ctx && key0 + row0 + 128 / CH * i >= ctx) x = make_uint4(0, 0, 0, 0);  // slots behind the last token may hold anything
+                if (odd) x = make_uint4(x.z, x.w, x.x, x.y);
+                const int by = s * Z::halves * Z::kv_block + 128 / CH * 128 * i;
+                po_store(one + by, two + by, x, __shfl_sync(0xffffffffu, ratio, (tid + 128 * i) / (kF8Tokens * CH)));
             }
             g_fence_proxy_async();
             __syncwarp();
             if (lane == 0) g_mbar_arrive(full + 8 * s);
-            if (t + 1 < n_tiles) load(t + 1), look_up(t + 2);
+            ask(t + 2), look_up(t + 3);
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else {  // ---- softmax: thread = row
         asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
         const int r = threadIdx.x, col = c0 + r, set = warp >> 2;
@@ -295,36 +306,42 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
             const int key0 = first + t * kPoKeys, s2 = t & 1;
             if (!(ok = tc_wait(s_mine + 8 * s2, t >> 1 & 1, dead))) break;
             g_tc_fence_after();
-            uint32_t s[2][32];
-            g_tmem_ld32_nowait(tmem + lanes + s2 * kPoKeys, s[0]);
-            g_tmem_ld32_nowait(tmem + lanes + s2 * kPoKeys + 32, s[1]);
-            g_tmem_ld_wait();
-            if (__any_sync(0xffffffffu, key0 + kPoKeys > limit)) {
-#pragma unroll
-                for (int c = 0; c < kPoKeys; ++c)
-                    if (key0 + c >= limit) s[c >> 5][c & 31] = 0xff800000u;
-            }
-            if (care) {  // a page that is none hides its keys; a scale that is none makes the row NaN
-#pragma unroll
+            // the two halves of the tile one after the other, read again for the exponentials: half the code and registers
+            const uint32_t mine_s = tmem + lanes + s2 * kPoKeys;
+            const bool cut = __any_sync(0xffffffffu, key0 + kPoKeys > limit);
+            unsigned hidden = 0;  // blocks whose page is none
+            if (care) {           // such a page hides its keys; a scale that is none makes the row NaN
+#pragma unroll 1
                 for (int g = 0; g < 4; ++g) {
                     const int key = key0 + kF8Tokens * g;
                     if (key >= past) continue;
                     int page;
                     const size_t at = block_at(key / kF8Tokens, page);
-                    if (static_cast<unsigned>(page) >= static_cast<unsigned>(pg.num_pages)) {
-#pragma unroll
-                        for (int c = 0; c < kF8Tokens; ++c) s[g >> 1][(g & 1) * 16 + c] = 0xff800000u;
-                    } else if (key < limit && !(pg.key_scales[at] < INFINITY && pg.value_scales[at] < INFINITY)) {
-                        sum = NAN;
-                    }
+                    if (static_cast<unsigned>(page) >= static_cast<unsigned>(pg.num_pages)) hidden |= 1u << g;
+                    else if (key < limit && !(pg.key_scales[at] < INFINITY && pg.value_scales[at] < INFINITY)) sum = NAN;
                 }
             }
-            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            auto half = [&](int i, uint32_t (&s)[32]) {
+                g_tmem_ld32(mine_s + 32 * i, s);
+                if (cut || hidden) {
 #pragma unroll
-            for (int c = 0; c < kPoKeys; c += 8)
+                    for (int c = 0; c < 32; ++c)
+                        if (key0 + 32 * i + c >= limit || (hidden >> (2 * i + c / 16) & 1)) s[c] = 0xff800000u;
+                }
+            };
+            float top = -INFINITY;
+#pragma unroll 1
+            for (int i = 0; i < 2; ++i) {
+                uint32_t s[32];
+                half(i, s);
+                float tops[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) tops[i] = po_max3(tops[i], __uint_as_float(s[c >> 5][(c & 31) + 2 * i]), __uint_as_float(s[c >> 5][(c & 31) + 2 * i + 1]));
-            const float top = po_max3(fmaxf(tops[0], tops[1]), tops[2], tops[3]) * mult;
+                for (int c = 0; c < 32; c += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) tops[e] = po_max3(tops[e], __uint_as_float(s[c + 2 * e]), __uint_as_float(s[c + 2 * e + 1]));
+                top = po_max3(fmaxf(tops[0], tops[1]), tops[2], tops[3]);
+            }
+            top *= mult;
             const bool grow = top > m + kAtLag || (m == -INFINITY && top > m);
             if (__any_sync(0xffffffffu, grow)) {
                 if (t > 0) {
@@ -332,7 +349,7 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
                     g_tc_fence_after();
                     const float to = grow ? top : m, alpha = !grow ? 1.f : m == -INFINITY ? 0.f : at_ex2(m - to);
                     sum *= alpha;
-#pragma unroll
+#pragma unroll 1
                     for (int i = 0; i < DIM / 32; ++i) {
                         uint32_t o[32];
                         g_tmem_ld32(tmem + lanes + kPoOut + i * 32, o);
@@ -345,19 +362,23 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
                 m = grow ? top : m;
             }
             const float at = m == -INFINITY ? 0.f : m;
-            uint32_t pk[32];
             const uint64_t mult2 = po_two(mult, mult), minus = po_two(-at, -at);
             uint64_t sums[2] = {0, 0};  // two pairs of zeros
+#pragma unroll 1
+            for (int i = 0; i < 2; ++i) {
+                uint32_t s[32], pk[16];
+                half(i, s);
 #pragma unroll
-            for (int c = 0; c < kPoKeys; c += 2) {
-                const float2 z = po_each(po_fma2(po_two(__uint_as_float(s[c >> 5][c & 31]), __uint_as_float(s[c >> 5][(c & 31) + 1])), mult2, minus));
-                const float x = at_ex2(z.x), y = at_ex2(z.y);
-                pk[c / 2] = tl::pack2<__half>(x, y);
-                sums[(c >> 1) & 1] = po_add2(sums[(c >> 1) & 1], po_two(x, y));
+                for (int c = 0; c < 32; c += 2) {
+                    const float2 z = po_each(po_fma2(po_two(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), mult2, minus));
+                    const float x = at_ex2(z.x), y = at_ex2(z.y);
+                    pk[c / 2] = tl::pack2<__half>(x, y);
+                    sums[(c >> 1) & 1] = po_add2(sums[(c >> 1) & 1], po_two(x, y));
+                }
+                po_st16(mine_s + 16 * i, pk);  // column c = keys 2 c and 2 c + 1; over scores that have been read
             }
             const float2 both = po_each(po_add2(sums[0], sums[1]));
             sum += both.x + both.y;
-            g_tmem_st32(tmem + lanes + s2 * kPoKeys, pk);  // column c = keys 2 c and 2 c + 1
             g_tmem_st_wait();
             g_tc_fence_before();
             __syncwarp();
@@ -373,7 +394,7 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
         float *part = whole ? nullptr : static_cast<float *>(a.workspace) + index * at_piece_floats(kPoRows, DIM);
         const int l = at_div(live ? col : 0, G, a.group_magic);
         bf16 *out = static_cast<bf16 *>(a.out) + ((static_cast<size_t>(b) * L + l) * a.heads + static_cast<size_t>(h) * G + (live ? col : 0) - l * G) * DIM;
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < DIM / 32; ++i) {
             uint32_t o[32];
             if (n_tiles > 0) {
