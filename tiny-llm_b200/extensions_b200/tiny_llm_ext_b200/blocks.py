@@ -1217,10 +1217,16 @@ def fp8_append(pages: Fp8Pages, device: int, q: torch.Tensor, k: torch.Tensor, v
                k_eps: float = 0.0, rot: int = 0, base: float = 1.0, interleaved: bool = False) -> torch.Tensor:
     """``tlb_fp8_append``: a step's ``k`` and ``v [B, G, L, dim]`` into the pages, ``q [B, H, L, dim]`` -> the same shape (laid out token by token)."""
     _fp8_step("fp8_append", pages, device, table, lens, q, k, v)
+    _code(q.dtype)
     for w in (q_norm, k_norm):
         if w is not None and (w.shape != (pages.dim,) or w.dtype != q.dtype or w.get_device() != device or not w.is_contiguous()):
             raise RuntimeError("fp8_append: norm weights must be [dim] of the step's dtype")
     return fp8_append_of(pages, device, q, k, v, table, lens, q_norm, q_eps, k_norm, k_eps, rot, base, interleaved)
+
+
+def _token_by_token(like: torch.Tensor, B: int, H: int, L: int, D: int) -> torch.Tensor:
+    """Room for ``[B, H, L, D]``, a token's heads side by side."""
+    return torch.empty_strided((B, H, L, D), (L * H * D, D, H * D, 1), dtype=like.dtype, device=like.device)
 
 
 def fp8_append_of(pages: Fp8Pages, device: int, q, k, v, table, lens, q_norm=None, q_eps=0.0, k_norm=None, k_eps=0.0, rot=0, base=1.0, interleaved=False) -> torch.Tensor:
@@ -1229,21 +1235,22 @@ def fp8_append_of(pages: Fp8Pages, device: int, q, k, v, table, lens, q_norm=Non
         with torch.cuda.device(device):
             return fp8_append_of(pages, device, q, k, v, table, lens, q_norm, q_eps, k_norm, k_eps, rot, base, interleaved)
     B, H, L, D = q.shape
-    out = q.new_empty((B, L, H, D))
+    out = _token_by_token(q, B, H, L, D)
     qb, qh, ql, _ = q.stride()
     kb, kh, kl, _ = k.stride()
     vb, vh, vl, _ = v.stride()
     call = _FP8_APPEND.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(), 0 if q_norm is None else q_norm.data_ptr(),
-                            0 if k_norm is None else k_norm.data_ptr(), qb, qh, ql, kb, kh, kl, vb, vh, vl, base, q_eps, k_eps, B, H, L, table.shape[1], rot, interleaved, _code(q.dtype))
+                            0 if k_norm is None else k_norm.data_ptr(), qb, qh, ql, kb, kh, kl, vb, vh, vl, base, q_eps, k_eps, B, H, L, table.shape[1], rot, interleaved, _DTYPE_CODE[q.dtype])
     rc = library().tlb_fp8_append(ctypes.addressof(pages), call, _raw_stream(device))
     if rc:
         _check(rc)
-    return out.transpose(1, 2)
+    return out
 
 
 def fp8_attention(pages: Fp8Pages, device: int, q: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, scale: float, causal: bool) -> torch.Tensor:
     """``tlb_fp8_attention``: ``q [B, H, L, dim]`` -> the same shape (laid out token by token)."""
     _fp8_step("fp8_attention", pages, device, table, lens, q)
+    _code(q.dtype)
     return fp8_attention_of(pages, device, q, table, lens, scale, causal)
 
 
@@ -1253,16 +1260,16 @@ def fp8_attention_of(pages: Fp8Pages, device: int, q, table, lens, scale, causal
         with torch.cuda.device(device):
             return fp8_attention_of(pages, device, q, table, lens, scale, causal)
     B, H, L, D = q.shape
-    out = q.new_empty((B, L, H, D))
+    out = _token_by_token(q, B, H, L, D)
     qb, qh, ql, _ = q.stride()
-    call = _FP8_ATTENTION.pack(q.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(), qb, qh, ql, scale, B, H, L, table.shape[1], causal, _code(q.dtype))
+    call = _FP8_ATTENTION.pack(q.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(), qb, qh, ql, scale, B, H, L, table.shape[1], causal, _DTYPE_CODE[q.dtype])
     lib, at = library(), ctypes.addressof(pages)
     size = lib.tlb_fp8_attention_workspace(at, call)
     scratch = q.new_empty(size, dtype=torch.uint8) if size else None
     rc = lib.tlb_fp8_attention(at, call, _ptr(scratch), size, _raw_stream(device))
     if rc:
         _check(rc)
-    return out.transpose(1, 2)
+    return out
 
 
 def moe_few_tokens(dim: int, outputs: int, experts: int, top: int, group_count: int = 0, fp8: bool = False) -> int:

@@ -67,7 +67,7 @@ def _step(op: str, pages: Fp8KvPages, query: torch.Tensor, block_table: torch.Te
     if len(shape) != 4:
         raise ValueError(f"{op}: query must be 4D [B, H_q, L, D]")
     B, heads, L, D = shape
-    if min(shape) <= 0:
+    if B <= 0 or heads <= 0 or L <= 0 or D <= 0:
         raise ValueError(f"{op}: dimensions must be positive")
     if D != pages.head_dim:
         raise ValueError(f"{op}: query and pages must have the same head dimension")
@@ -75,9 +75,10 @@ def _step(op: str, pages: Fp8KvPages, query: torch.Tensor, block_table: torch.Te
         raise ValueError(f"{op}: query heads must be divisible by K/V heads")
     if query.dtype not in _DTYPES:
         raise ValueError(f"{op}: supports float32 or bfloat16 inputs")
-    if len(rows) != 2 or context_lens.dim() != 1 or block_table.dtype != torch.int32 or context_lens.dtype != torch.int32:
+    counts = context_lens.shape
+    if len(rows) != 2 or len(counts) != 1 or block_table.dtype != torch.int32 or context_lens.dtype != torch.int32:
         raise ValueError(f"{op}: block_table must be 2D int32 and context_lens 1D int32")
-    if rows[0] != B or len(context_lens) != B or rows[1] <= 0:
+    if rows[0] != B or counts[0] != B or rows[1] <= 0:
         raise ValueError(f"{op}: query, block_table, and context_lens batch sizes must match, with at least one page slot")
     if context_lens_host is None:
         context_lens_host = context_lens.detach().cpu().numpy()
