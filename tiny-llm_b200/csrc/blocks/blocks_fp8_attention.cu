@@ -2,8 +2,8 @@
 //
 // The products run on mma.sync (m16n8k16, f16 in, fp32 out) with the cache as the first operand: 16 keys (a block, so one scale of either side) times 8 columns, a
 // column being one (query head of the group, new token).  An e4m3 number is an f16 number, so the cache's side is exact; a column is brought to the top of
-// f16's range by a power of two, where bf16 keeps all its bits, and an fp32 query is two such terms.  The scales never meet f16: a block's
-// key scale multiplies its scores and its value scale the product of its weights and values, both in fp32.  Weights are exp2 of a number up to the
+// f16's range by a power of two, where bf16 keeps all its bits, and an fp32 query is two such terms.  A block's key scale multiplies its scores in fp32; its value
+// scale multiplies its weights, over the largest value scale so far (fp32 outputs: the product of weights and values).  Weights are exp2 of a number up to the
 // column's running maximum (which may lag behind by 2^15 before the sums are scaled again), rounded to f16 for the second product: 2^-12 of a weight, where an output is
 // rounded to 2^-9 of itself; fp32 outputs take a second term for the rest.  Running sums are fp32.
 //
@@ -30,6 +30,11 @@ __device__ __forceinline__ void at_mma(float (&d)[4], const uint32_t (&a)[4], ui
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void at_mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {  // nothing to add to
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t at_pack(float lo, float hi) { return tl::pack2<__half>(lo, hi); }
 __device__ __forceinline__ float2 at_rest(uint32_t two, float lo, float hi) {  // what the rounding to f16 left
     const float2 f = tl::unpack2<__half>(two);
@@ -39,11 +44,10 @@ __device__ __forceinline__ float2 at_rest(uint32_t two, float lo, float hi) {  /
 constexpr int kAtWarps = 8, kAtStages = 3;
 
 __device__ __forceinline__ void at_copy16(uint32_t to, const void *from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
-__device__ __forceinline__ void at_copy4(uint32_t to, const void *from) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory"); }
 
-// A block in shared memory: 16 rows of keys, 16 of values, the two scales.  Rows of 128 bytes have their pieces moved about so that the eight lanes of a reading phase meet
+// A block in shared memory: 16 rows of keys, 16 of values.  Rows of 128 bytes have their pieces moved about so that the eight lanes of a reading phase meet
 // all banks: a key's halves change places in odd rows (lanes read 4 pieces of 2 rows), a value's pairs of pieces go by the pair of rows (2 pieces of 4 rows).
-__host__ __device__ constexpr int at_stage(int dim) { return 2 * kF8Tokens * dim + 16; }
+__host__ __device__ constexpr int at_stage(int dim) { return 2 * kF8Tokens * dim; }
 template <bool MOVED>
 __device__ __forceinline__ int at_key(int row, int D, int byte) {
     return row * D + (MOVED ? byte ^ ((row & 1) << 6) : byte);
@@ -53,13 +57,11 @@ __device__ __forceinline__ int at_value(int row, int D, int byte) {
     return row * D + (MOVED ? byte ^ (((row >> 1) & 3) << 5) : byte);
 }
 
-// DIM: entries of a head, 0: as the pages say.
+// DIM: entries of a head, 0: as the pages say.  place: of the block among all pages'.
 template <int DIM>
-__device__ __forceinline__ void at_issue(uint32_t stage, const F8Attend &a, int h, int blk, int in_page, int page, int lane) {
-    const tlb_fp8_pages &pg = a.pages;
+__device__ __forceinline__ void at_issue(uint32_t stage, const tlb_fp8_pages &pg, int place, int lane) {
     const int D = DIM ? DIM : pg.dim;
-    if (static_cast<unsigned>(page) >= static_cast<unsigned>(pg.num_pages)) page = 0;  // its keys are skipped; nothing outside the pages is read
-    const size_t block = (static_cast<size_t>(page) * pg.heads + h) * a.page_blocks + in_page, byte = block * kF8Tokens * D + 16 * lane;
+    const size_t byte = static_cast<size_t>(static_cast<unsigned>(place)) * (kF8Tokens * D) + 16 * lane;
     if constexpr (DIM == 128) {
         const uint32_t k = stage + ((16 * lane) ^ ((lane >> 3 & 1) << 6)), v = stage + 16 * D + ((16 * lane) ^ ((lane >> 4) << 5)), w = stage + 16 * D + ((16 * lane) ^ ((lane >> 4) << 5) ^ 64);
 #pragma unroll
@@ -70,8 +72,13 @@ __device__ __forceinline__ void at_issue(uint32_t stage, const F8Attend &a, int 
             at_copy16(stage + 16 * D + 16 * i, pg.values + byte + 16 * (i - lane));
         }
     }
-    if (lane < 2) at_copy4(stage + 32 * D + 4 * lane, (lane ? pg.value_scales : pg.key_scales) + block);
 }
+
+// Where 32 of a warp's blocks lie, and their scales: a lane knows one of them.  place -1: the page is none, its keys are skipped.
+struct AtLook {
+    int place;
+    float ks, vs;
+};
 
 // DP: entries of a head that the lanes' shares make room for; DIM: entries it has, 0: fewer than DP.
 template <typename T, int DP, int DIM, int NT>
@@ -103,13 +110,19 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
     const int stage_bytes = at_stage(D);
     unsigned char *ring = sm + warp * kAtStages * stage_bytes;
     const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
-    auto issue = [&](int stage, int blk, int page) {
-        if (blk < stop) at_issue<DIM>(ring_at + stage * stage_bytes, a, h, blk, blk - page_at(blk) * a.page_blocks, page, lane);
-        asm volatile("cp.async.commit_group;" ::: "memory");
+    // blocks are looked up by the table's bounds, so that the first ones need not wait for the length
+    auto look = [&](int i0) {
+        AtLook x{-1, 0.f, 0.f};
+        const int blk = begin + warp + (i0 + lane) * WARPS, at = page_at(blk), page = at < a.max_pages ? table[at] : -1;
+        if (static_cast<unsigned>(page) < static_cast<unsigned>(pg.num_pages)) {
+            x.place = (page * pg.heads + h) * a.page_blocks + blk - at * a.page_blocks;  // fewer than 2^31: they are 16 rows each
+            x.ks = __ldg(pg.key_scales + x.place), x.vs = __ldg(pg.value_scales + x.place);
+        }
+        return x;
     };
-    auto page_of = [&](int blk) {  // by the table's bounds, so that the first ones need not wait for the length
-        const int i = page_at(blk);
-        return i < a.max_pages ? table[i] : -1;
+    auto issue = [&](int stage, bool more, int place) {
+        if (more && place >= 0) at_issue<DIM>(ring_at + stage * stage_bytes, pg, place, lane);
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
     // queries: eight entries a thread, brought to f16 once for all warps
     static_assert(COLS * DP / 8 <= WARPS * 32, "every entry has a thread");
@@ -121,12 +134,10 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
         const int l = at_div(c0 + qcol, G, a.group_magic);
         at_query(static_cast<const T *>(a.q) + b * a.q_b + (static_cast<long long>(h) * G + c0 + qcol - l * G) * a.q_h + l * a.q_l + qd, a.wide_rows, x8);
     }
-    int at = begin + warp, stage = 0;
-    int pages_of[kAtStages];  // of the blocks in the ring, and of the one that comes next
+    const int count = max((stop - begin - warp + WARPS - 1) / WARPS, 0);  // of this warp's blocks
+    AtLook now = look(0), next{-1, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < kAtStages; ++i) pages_of[i] = page_of(at + i * WARPS);
-#pragma unroll
-    for (int i = 0; i < kAtStages - 1; ++i) issue(i, at + i * WARPS, pages_of[i]);
+    for (int i = 0; i < kAtStages - 1; ++i) issue(i, i < count, __shfl_sync(0xffffffffu, now.place, i));
 
     {
         float m = 0.f;
@@ -188,25 +199,28 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
         for (int e = 0; e < 2; ++e) m_run[nt][e] = -INFINITY, l_run[nt][e] = 0.f;
     }
 
-    for (; at < stop; at += WARPS) {
-        const int key0 = at * kF8Tokens, here = pages_of[0], ahead = at + (kAtStages - 1) * WARPS;
+    float vs_most = 0.f, under = 0.f;  // the largest value scale so far, and 1 over it
+    for (int i = 0, stage = 0; i < count; ++i) {
+        const int key0 = (begin + warp + i * WARPS) * kF8Tokens, in_32 = i & 31, ahead = i + kAtStages - 1;
         asm volatile("cp.async.wait_group %0;" ::"n"(kAtStages - 2) : "memory");
         __syncwarp();  // all lanes' copies of this block are there, and all lanes are through with the block before, whose place is next
-        issue(stage ? stage - 1 : kAtStages - 1, ahead, pages_of[kAtStages - 1]);
-#pragma unroll
-        for (int i = 0; i + 1 < kAtStages; ++i) pages_of[i] = pages_of[i + 1];
-        pages_of[kAtStages - 1] = page_of(ahead + WARPS);
+        if (in_32 == 0 && i + 32 < count) next = look(i + 32);
+        issue(stage ? stage - 1 : kAtStages - 1, ahead < count, __shfl_sync(0xffffffffu, (ahead & 31) < in_32 ? next.place : now.place, ahead & 31));
         const unsigned char *block = ring + stage * stage_bytes;
         stage = stage + 1 == kAtStages ? 0 : stage + 1;
-        if (static_cast<unsigned>(here) >= static_cast<unsigned>(pg.num_pages)) continue;
-        const float2 scales = *reinterpret_cast<const float2 *>(block + 32 * D);
+        const int place = __shfl_sync(0xffffffffu, now.place, in_32);
+        const float2 scales = make_float2(__shfl_sync(0xffffffffu, now.ks, in_32), __shfl_sync(0xffffffffu, now.vs, in_32));
+        if (in_32 == 31) now = next;
+        if (place < 0) continue;
 
         // scores: rows g and g + 8 (keys), columns 2t and 2t + 1
         float sc[NT][4];
+        if constexpr (kTwo) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sc[nt][i] = 0.f;
+                for (int i = 0; i < 4; ++i) sc[nt][i] = 0.f;
+        }
 #pragma unroll
         for (int r = 0; r < KR; ++r) {
             const int d = (4 * r + t) * 16;
@@ -220,11 +234,13 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     if constexpr (kTwo) {  // every product's sum begins anew: the tensor cores cut what they add up, fp32 additions round
-                        float d4[4] = {0.f, 0.f, 0.f, 0.f}, c4[4] = {0.f, 0.f, 0.f, 0.f};
-                        at_mma(d4, f, ql[nt][r][s][0], ql[nt][r][s][1]);
-                        at_mma(c4, f, qf[nt][r][s][0], qf[nt][r][s][1]);
+                        float d4[4], c4[4];
+                        at_mma_first(d4, f, ql[nt][r][s][0], ql[nt][r][s][1]);
+                        at_mma_first(c4, f, qf[nt][r][s][0], qf[nt][r][s][1]);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) sc[nt][i] += c4[i] + d4[i];
+                    } else if (r == 0 && s == 0) {
+                        at_mma_first(sc[nt], f, qf[nt][r][s][0], qf[nt][r][s][1]);
                     } else {
                         at_mma(sc[nt], f, qf[nt][r][s][0], qf[nt][r][s][1]);
                     }
@@ -248,13 +264,23 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
             }
         }
 
+        if (!kTwo && scales.y > vs_most) {  // the sums so far are over the smaller scale
+            const float by = vs_most / scales.y;
+            vs_most = scales.y, under = 1.f / scales.y;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[nt][j][e] *= by;
+        }
         // scaled to log2, masked scores -inf whatever the factor (which may be no number, 0 or negative)
         float f[NT][2], x[NT][4], vs[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                f[nt][e] = factor[nt][e] * scales.x, vs[nt][e] = scales.y;
+                f[nt][e] = factor[nt][e] * scales.x, vs[nt][e] = kTwo ? scales.y : scales.y * under;
                 x[nt][e] = sc[nt][e] * f[nt][e], x[nt][2 + e] = sc[nt][2 + e] * f[nt][e];
             }
         if (key0 + kF8Tokens > low) {
@@ -311,7 +337,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                p[nt][i] = at_pack(w[2 * i], w[2 * i + 1]);
+                p[nt][i] = kTwo ? at_pack(w[2 * i], w[2 * i + 1]) : at_pack(w[2 * i] * vs[nt][0], w[2 * i + 1] * vs[nt][1]);
                 if constexpr (kTwo) {
                     const float2 z = at_rest(p[nt][i], w[2 * i], w[2 * i + 1]);
                     pl[nt][i] = at_turn(at_pack(z.x * 2048.f, z.y * 2048.f));  // the rest of a small weight would fall below f16's range
@@ -326,16 +352,15 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
             at_halves(__byte_perm(v[0][j >> 1], v[1][j >> 1], sel), f4[0], f4[1]), at_halves(__byte_perm(v[2][j >> 1], v[3][j >> 1], sel), f4[2], f4[3]);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                float d[4] = {0.f, 0.f, 0.f, 0.f};
-                at_mma(d, f4, p[nt][0], p[nt][1]);
-                if constexpr (kTwo) {
-                    float c[4] = {0.f, 0.f, 0.f, 0.f};
-                    at_mma(c, f4, pl[nt][0], pl[nt][1]);
+                if constexpr (!kTwo) {
+                    at_mma(o[nt][j], f4, p[nt][0], p[nt][1]);
+                } else {
+                    float d[4], c[4];
+                    at_mma_first(d, f4, p[nt][0], p[nt][1]);
+                    at_mma_first(c, f4, pl[nt][0], pl[nt][1]);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) d[i] = fmaf(c[i], 1.f / 2048.f, d[i]);
+                    for (int e = 0; e < 4; ++e) o[nt][j][e] = fmaf(fmaf(c[e], 1.f / 2048.f, d[e]), vs[nt][e & 1], o[nt][j][e]);
                 }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[nt][j][i] = fmaf(d[i], vs[nt][i & 1], o[nt][j][i]);
             }
         }
     }
@@ -356,7 +381,9 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
             if (col < live) {
                 float4 *to = reinterpret_cast<float4 *>(part + (warp * COLS + col) * ROW + g * (DP / 8));
 #pragma unroll
-                for (int j = 0; j < J; j += 2) to[j / 2] = make_float4(o[nt][j][e], o[nt][j][2 + e], o[nt][j + 1][e], o[nt][j + 1][2 + e]);
+                for (int j = 0; j < J; j += 2)
+                    to[j / 2] = kTwo ? make_float4(o[nt][j][e], o[nt][j][2 + e], o[nt][j + 1][e], o[nt][j + 1][2 + e])
+                                     : make_float4(o[nt][j][e] * vs_most, o[nt][j][2 + e] * vs_most, o[nt][j + 1][e] * vs_most, o[nt][j + 1][2 + e] * vs_most);
             }
         }
     __syncthreads();
