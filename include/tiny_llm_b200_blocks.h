@@ -424,8 +424,10 @@ typedef struct {
 int tlb_fp8_append(const tlb_fp8_pages *pages, const tlb_fp8_append_call *call, void *stream);
 /* out [batch, tokens, heads, dim] = softmax(q k^T * scale) v over the first lens[b] slots of each request (the `tokens` newest among them); causal: new token i sees
  * lens[b] - tokens + i + 1 of them.  Rows that see nothing come out as zeros.  Products with the cache's numbers are exact, their sums, the softmax and the scales fp32;
- * weights are rounded to f16 (relative to the largest so far) for bf16 outputs, and use 22 bits for fp32 ones, whose queries do so too.  How the keys are divided
- * follows lens as it is when the launch runs; it decides the order of sums.  The workspace need not be initialised; calls that may run at once need one each. */
+ * weights are rounded to f16 (relative to the largest so far) for bf16 outputs, and use 22 bits for fp32 ones, whose queries do so too.  With a workspace long
+ * requests are cut into pieces, by lens as it is when the launch runs (a captured one follows them): this decides the order of sums.  Without one (NULL) none is.
+ * tlb_fp8_attention_workspace: its bytes, 0 where none would be used; lens_host: the lengths on the host, if the launch is for these alone and no piece of them is worth its
+ * cost the answer is 0 as well; NULL: any lengths.  The workspace need not be initialised; calls that may run at once need one each. */
 typedef struct {
     const void *q;
     void *out;
@@ -434,7 +436,7 @@ typedef struct {
     double scale;
     int batch, heads, tokens, max_pages, causal, dtype;
 } tlb_fp8_attention_call;
-size_t tlb_fp8_attention_workspace(const tlb_fp8_pages *pages, const tlb_fp8_attention_call *call);
+size_t tlb_fp8_attention_workspace(const tlb_fp8_pages *pages, const tlb_fp8_attention_call *call, const int32_t *lens_host);
 int tlb_fp8_attention(const tlb_fp8_pages *pages, const tlb_fp8_attention_call *call, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus

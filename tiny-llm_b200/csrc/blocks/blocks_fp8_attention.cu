@@ -14,6 +14,8 @@
 //
 // An item is 8 (or 16) columns of one request and key/value head.  A CTA takes an item, or, where the requests are few or of unlike length, a piece of one; an item in several
 // pieces leaves a partial result for each, which fp8_attend_join_kernel adds up in order.  The cut follows the lengths on the device, so a captured launch does.
+#include <algorithm>
+
 #include "../per_device.h"
 #include "blocks_fp8_cache.cuh"
 #include "blocks_fp8_attention.cuh"
@@ -205,16 +207,19 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
         asm volatile("cp.async.wait_group %0;" ::"n"(kAtStages - 2) : "memory");
         __syncwarp();  // all lanes' copies of this block are there, and all lanes are through with the block before, whose place is next
         if (in_32 == 0 && i + 32 < count) next = look(i + 32);
-        issue(stage ? stage - 1 : kAtStages - 1, ahead < count, __shfl_sync(0xffffffffu, (ahead & 31) < in_32 ? next.place : now.place, ahead & 31));
+        const int place_ahead = __shfl_sync(0xffffffffu, (ahead & 31) < in_32 ? next.place : now.place, ahead & 31), stage_ahead = stage ? stage - 1 : kAtStages - 1;
         const unsigned char *block = ring + stage * stage_bytes;
         stage = stage + 1 == kAtStages ? 0 : stage + 1;
         const int place = __shfl_sync(0xffffffffu, now.place, in_32);
         const float2 scales = make_float2(__shfl_sync(0xffffffffu, now.ks, in_32), __shfl_sync(0xffffffffu, now.vs, in_32));
         if (in_32 == 31) now = next;
-        if (place < 0) continue;
+        if (place < 0) {
+            issue(stage_ahead, ahead < count, place_ahead);
+            continue;
+        }
 
-        // scores: rows g and g + 8 (keys), columns 2t and 2t + 1
-        float sc[NT][4];
+        // scores: rows g and g + 8 (keys), columns 2t and 2t + 1; of two chains of products
+        float sc[NT][4], sd[NT][4];
         if constexpr (kTwo) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -239,14 +244,15 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
                         at_mma_first(c4, f, qf[nt][r][s][0], qf[nt][r][s][1]);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) sc[nt][i] += c4[i] + d4[i];
-                    } else if (r == 0 && s == 0) {
-                        at_mma_first(sc[nt], f, qf[nt][r][s][0], qf[nt][r][s][1]);
                     } else {
-                        at_mma(sc[nt], f, qf[nt][r][s][0], qf[nt][r][s][1]);
+                        float(&to)[4] = s & 1 ? sd[nt] : sc[nt];
+                        if (r == 0 && s < 2) at_mma_first(to, f, qf[nt][r][s][0], qf[nt][r][s][1]);
+                        else at_mma(to, f, qf[nt][r][s][0], qf[nt][r][s][1]);
                     }
                 }
             }
         }
+        issue(stage_ahead, ahead < count, place_ahead);  // while the products are under way
         uint32_t v[4][DP / 32];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -264,6 +270,12 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
             }
         }
 
+        if constexpr (!kTwo) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[nt][e] += sd[nt][e];
+        }
         if (!kTwo && scales.y > vs_most) {  // the sums so far are over the smaller scale
             const float by = vs_most / scales.y;
             vs_most = scales.y, under = 1.f / scales.y;
@@ -509,6 +521,14 @@ int f8_attend_join(const F8Attend &a, int cols, cudaStream_t st) {
 // CTAs of the kernels that the GPU holds at a time, as far as the division of the work goes: two an SM, one of the wider forms.
 static int attend_slots(int dtype, int dim, int rows) { return sm_count() * (dtype == TL_BF16 && dim <= 128 && rows <= 8 ? 2 : 1); }
 static int attend_cols(int dim, int rows) { return dim > 128 || rows <= 8 ? 8 : 16; }
+constexpr int kAtWhole = 64;  // blocks of a request that is not cut
+// Whether a launch without pieces takes no longer than one with them and the launch that joins them, which is 6.5 us more: an item's CTA takes so long for a block by itself, all of
+// them together so long as their bytes take.  (bf16, 8 columns, heads of 128: 0.075 us a block, 6.2 TB/s.  One request of 1011 tokens 8.9 us whole and 10.7 cut, of 2000 13.4
+// and 10.8; 24 of 70 to 1970 17.9 and 19.2; 16 of 8000 45 and 53; 64 of 8192 157 and 162.)
+static bool attend_whole(int dtype, int dim, int cols, long long longest, double blocks) {
+    const double block = (dtype == TL_BF16 ? 0.075 : 0.18) * (cols == 16 ? 1.3 : 1.0);
+    return longest <= kAtWhole || longest * block <= 6.5 + blocks * (2 * kF8Tokens * dim / 6.2e6);
+}
 
 template <typename T, int DP, int DIM, int NT>
 static int attend_launch(F8Attend a, cudaStream_t st) {
@@ -546,7 +566,7 @@ static int attend_any(F8Attend a, cudaStream_t st) {
     a.page_magic = at_magic(static_cast<unsigned long long>(a.max_pages) * a.page_blocks + 64, a.page_blocks);  // the first pages are looked up ahead of the length
     a.group_magic = at_magic(static_cast<unsigned long long>(a.group) * a.tokens, a.group);
     a.heads_magic = at_magic(static_cast<unsigned long long>(a.pages.heads) * ((a.group * a.tokens + 7) / 8), a.pages.heads);
-    a.slots = attend_slots(a.dtype, D, a.group * a.tokens), a.most_pieces = 128;
+    a.slots = attend_slots(a.dtype, D, a.group * a.tokens), a.most_pieces = 128, a.whole = kAtWhole;
     if (f8_portion_takes(a.pages, a)) return f8_portion(a, st);
     if (D <= 64) return D == 64 ? attend_columns<T, 64, 64>(a, st) : attend_columns<T, 64, 0>(a, st);
     if (D <= 128) return D == 128 ? attend_columns<T, 128, 128>(a, st) : attend_columns<T, 128, 0>(a, st);
@@ -557,14 +577,22 @@ static int attend_any(F8Attend a, cudaStream_t st) {
 
 using namespace tlb;
 
-extern "C" size_t tlb_fp8_attention_workspace(const tlb_fp8_pages *pages, const tlb_fp8_attention_call *c) {
+extern "C" size_t tlb_fp8_attention_workspace(const tlb_fp8_pages *pages, const tlb_fp8_attention_call *c, const int32_t *lens_host) {
     if (f8_check_pages("fp8_attention", pages) != TL_OK || !c || c->heads <= 0 || c->tokens <= 0 || c->batch <= 0) return 0;
     const long long rows = static_cast<long long>(c->heads / pages->heads) * c->tokens;
     const bool portion = f8_portion_takes(*pages, *c);
     const int few = rows <= 8 ? 8 : 9, cols = portion ? kPoRows : attend_cols(pages->dim, few), slots = portion ? sm_count() : attend_slots(c->dtype, pages->dim, few);
-    const long long items = (rows + cols - 1) / cols * pages->heads * c->batch;
-    // requests that can't be long, or more items than a cut would serve
-    if (static_cast<long long>(c->max_pages) * (pages->page_size / kF8Tokens) <= kAtLeast + kAtLeast / 4 || items > (portion ? 1LL : 16LL) * slots) return 0;
+    const long long each = (rows + cols - 1) / cols * pages->heads, items = each * c->batch;
+    if (items > (portion ? 1LL : 16LL) * slots) return 0;  // more items than a cut would serve
+    long long longest = static_cast<long long>(c->max_pages) * (pages->page_size / kF8Tokens), blocks = 0;
+    if (lens_host) {
+        longest = 0;
+        for (int b = 0; b < c->batch; ++b) {
+            const long long n = (std::max(lens_host[b], 0) + kF8Tokens - 1LL) / kF8Tokens;
+            longest = std::max(longest, n), blocks += n;
+        }
+    }
+    if (portion ? longest <= kPoWhole : attend_whole(c->dtype, pages->dim, cols, longest, static_cast<double>(blocks) * each)) return 0;
     return static_cast<size_t>(items + slots) * at_piece_floats(cols, pages->dim) * sizeof(float);
 }
 
@@ -575,8 +603,8 @@ extern "C" int tlb_fp8_attention(const tlb_fp8_pages *pages, const tlb_fp8_atten
     if (c->batch == 0 || c->tokens == 0) return TL_OK;
     if (c->max_pages <= 0 || static_cast<long long>(c->heads / pages->heads) * c->tokens > (1 << 30)) return tl::fail(TL_EINVAL, "fp8_attention: sizes out of range");
     if (!c->q || !c->out || !c->table || !c->lens) return tl::fail(TL_EINVAL, "fp8_attention: missing argument");
-    const size_t need = tlb_fp8_attention_workspace(pages, c);
-    if (need && (!workspace || workspace_bytes < need || !tl::aligned16(workspace))) return tl::fail(TL_EWORKSPACE, "fp8_attention: a workspace of %zu bytes is needed", need);
-    const F8Attend a(*pages, *c, need ? workspace : nullptr);
+    const size_t need = workspace ? tlb_fp8_attention_workspace(pages, c, nullptr) : 0;
+    if (need && (workspace_bytes < need || !tl::aligned16(workspace))) return tl::fail(TL_EWORKSPACE, "fp8_attention: the workspace must have %zu bytes, from a boundary of 16 on", need);
+    const F8Attend a(*pages, *c, need ? workspace : nullptr);  // without one every item is whole
     TLB_DISPATCH(c->dtype, "fp8_attention", return attend_any<T>(a, as_stream(stream)));
 }

@@ -12,12 +12,13 @@ struct F8Attend : tlb_fp8_attention_call {
     int slots;              // CTAs that the GPU holds at a time
     int most_pieces;        // of an item
     int granule;            // pieces are a multiple of so many blocks
+    int whole;              // blocks of a request that is not cut
     int page_blocks;        // blocks of 16 tokens in a page
     unsigned page_magic, group_magic, heads_magic, each_magic;  // for divisions by page_blocks, group, heads and the items of a request (at_div)
     bool wide_rows;         // query rows may be read 16 bytes at a time
     float scale_log2, scale_rest;  // scale * log2(e), and what its rounding to fp32 left
     F8Attend(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c, void *ws)
-        : tlb_fp8_attention_call(c), pages(p), workspace(ws), group(c.heads / p.heads), col_blocks(0), slots(0), most_pieces(1), granule(1), page_blocks(1), page_magic(0), group_magic(0), heads_magic(0), each_magic(0), wide_rows(false) {
+        : tlb_fp8_attention_call(c), pages(p), workspace(ws), group(c.heads / p.heads), col_blocks(0), slots(0), most_pieces(1), granule(1), whole(0), page_blocks(1), page_magic(0), group_magic(0), heads_magic(0), each_magic(0), wide_rows(false) {
         const double log2 = c.scale * 1.4426950408889634;
         scale_log2 = static_cast<float>(log2), scale_rest = static_cast<float>(log2 - scale_log2);
     }
@@ -76,6 +77,7 @@ __device__ __forceinline__ AtCut at_cut(const F8Attend &a) {
         longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
     }
     const int each = a.pages.heads * a.col_blocks, room = max(a.slots - live * each, a.slots / 2);
+    if (longest <= a.whole) return 0;
     const int mean = static_cast<int>(min((static_cast<long long>(total) * each + room - 1) / room, 0x3fffffffLL));
     return max(max(mean, (longest + a.most_pieces - 1) / a.most_pieces), kAtLeast);
 }
@@ -102,6 +104,7 @@ __device__ __forceinline__ AtPiece at_piece(const F8Attend &a, int index) {
     AtPiece x{-1, 0, 0, 1, 0x3fffffff};
     if (cut == 0) {
         x.b = at_div(index, each, a.each_magic), x.item = index - x.b * each;
+        if (x.b >= a.batch) x.b = -1;
         return x;
     }
     const int want = at_div(index, each, a.each_magic);  // rounded down: an item's pieces over all items of a request are a multiple of them
@@ -136,6 +139,7 @@ __host__ __device__ static inline size_t at_piece_floats(int cols, int dim) { re
 // blocks_fp8_portion.cu: bf16 queries of many columns
 constexpr int kPoRows = 256;  // columns of a CTA
 bool f8_portion_takes(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c);
+constexpr int kPoWhole = 40;     // blocks of a request that is not cut
 int f8_portion(F8Attend a, cudaStream_t st);
 
 }  // namespace tlb

@@ -452,7 +452,7 @@ static int portion_launch(const F8Attend &a, unsigned ctas, cudaStream_t st) {
 }
 
 int f8_portion(F8Attend a, cudaStream_t st) {
-    a.slots = sm_count(), a.most_pieces = 32, a.granule = kPoKeys / kF8Tokens;
+    a.slots = sm_count(), a.most_pieces = 32, a.granule = kPoKeys / kF8Tokens, a.whole = kPoWhole;
     a.col_blocks = (a.group * a.tokens + kPoRows - 1) / kPoRows;
     const long long items = static_cast<long long>(a.col_blocks) * a.pages.heads * a.batch;
     if (items > 0x3fffffff) return tl::fail(TL_EINVAL, "fp8_attention: sizes out of range");

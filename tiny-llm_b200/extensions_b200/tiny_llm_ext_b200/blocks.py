@@ -100,7 +100,7 @@ _SIGNATURES = {
     "tlb_fp8_linear": (_I, [_VP, _LL, _VP, _I, _VP, _VP, _VP, _I, _I, _I, _VP, ctypes.c_size_t, _I, _VP]),
     "tlb_fp8_gated_mlp_workspace": (ctypes.c_size_t, [_I, _I, _I]),
     "tlb_fp8_append": (_I, [_VP, ctypes.c_char_p, _VP]),
-    "tlb_fp8_attention_workspace": (ctypes.c_size_t, [_VP, ctypes.c_char_p]),
+    "tlb_fp8_attention_workspace": (ctypes.c_size_t, [_VP, ctypes.c_char_p, ctypes.c_char_p]),
     "tlb_fp8_attention": (_I, [_VP, ctypes.c_char_p, _VP, ctypes.c_size_t, _VP]),
     "tlb_fp8_gated_mlp": (_I, [_VP, _LL, _VP, _I, _VP, _VP, _I, _VP, _VP, _I, _I, _I, _I, _F, _F, _VP, ctypes.c_size_t, _I, _VP]),
 }
@@ -1248,23 +1248,23 @@ def fp8_append_of(pages: Fp8Pages, device: int, q, k, v, table, lens, q_norm=Non
 
 
 def fp8_attention(pages: Fp8Pages, device: int, q: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, scale: float, causal: bool) -> torch.Tensor:
-    """``tlb_fp8_attention``: ``q [B, H, L, dim]`` -> the same shape (laid out token by token)."""
+    """``tlb_fp8_attention``: ``q [B, H, L, dim]`` -> the same shape (laid out token by token), for any lengths."""
     _fp8_step("fp8_attention", pages, device, table, lens, q)
     _code(q.dtype)
     return fp8_attention_of(pages, device, q, table, lens, scale, causal)
 
 
-def fp8_attention_of(pages: Fp8Pages, device: int, q, table, lens, scale, causal) -> torch.Tensor:
-    """``fp8_attention`` of tensors that the caller has checked (``paged_attention_fp8``)."""
+def fp8_attention_of(pages: Fp8Pages, device: int, q, table, lens, scale, causal, lens_host: bytes | None = None) -> torch.Tensor:
+    """``fp8_attention`` of tensors that the caller has checked (``paged_attention_fp8``); ``lens_host``: the lengths as int32, if the call is for these alone."""
     if _current_device() != device:
         with torch.cuda.device(device):
-            return fp8_attention_of(pages, device, q, table, lens, scale, causal)
+            return fp8_attention_of(pages, device, q, table, lens, scale, causal, lens_host)
     B, H, L, D = q.shape
     out = _token_by_token(q, B, H, L, D)
     qb, qh, ql, _ = q.stride()
     call = _FP8_ATTENTION.pack(q.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(), qb, qh, ql, scale, B, H, L, table.shape[1], causal, _DTYPE_CODE[q.dtype])
     lib, at = library(), ctypes.addressof(pages)
-    size = lib.tlb_fp8_attention_workspace(at, call)
+    size = lib.tlb_fp8_attention_workspace(at, call, lens_host)
     scratch = q.new_empty(size, dtype=torch.uint8) if size else None
     rc = lib.tlb_fp8_attention(at, call, _ptr(scratch), size, _raw_stream(device))
     if rc:

@@ -62,7 +62,7 @@ class Fp8KvPages:
 
 
 def _step(op: str, pages: Fp8KvPages, query: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor, block_table_host, context_lens_host):
-    """Checks of a step's shapes and metadata -> (block table, context lengths)."""
+    """Checks of a step's shapes and metadata -> (block table, context lengths, the lengths on the host)."""
     shape, rows = query.shape, block_table.shape
     if len(shape) != 4:
         raise ValueError(f"{op}: query must be 4D [B, H_q, L, D]")
@@ -88,7 +88,7 @@ def _step(op: str, pages: Fp8KvPages, query: torch.Tensor, block_table: torch.Te
     if lens.shape != (B,) or table.shape != rows:
         raise ValueError(f"{op}: context_lens_host and block_table_host must be copies of the tensors")
     validate_paged_metadata(lens, table, pages.page_size, pages.num_pages, L)
-    return block_table if block_table.is_contiguous() else block_table.contiguous(), context_lens if context_lens.is_contiguous() else context_lens.contiguous()
+    return block_table if block_table.is_contiguous() else block_table.contiguous(), context_lens if context_lens.is_contiguous() else context_lens.contiguous(), lens
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -102,7 +102,7 @@ def rotate_append_fp8(query: torch.Tensor, key: torch.Tensor, value: torch.Tenso
     ``query_norm`` and ``key_norm`` (``FastRMSNorm``) and ``rope`` (``FastRoPE``, turned by a token's position) are applied on the way, the keys' in 64 bits
     ahead of their one rounding.  Any strides will do; float32 or bfloat16.  A block of 16 tokens of a head has one scale: it grows where the new
     tokens need it to, and the block's earlier numbers are rounded to it again."""
-    table, lens = _step("rotate_append_fp8", pages, query, block_table, context_lens, block_table_host, context_lens_host)
+    table, lens, _ = _step("rotate_append_fp8", pages, query, block_table, context_lens, block_table_host, context_lens_host)
     B, _, L, D = query.shape
     if key.shape != (B, pages.kv_heads, L, D) or key.shape != value.shape:
         raise ValueError("rotate_append_fp8: key and value must be [B, H_kv, L, D] beside the query")
@@ -132,7 +132,9 @@ def paged_attention_fp8(query: torch.Tensor, pages: Fp8KvPages, block_table: tor
     ``mask``: None or ``"causal"``; ``scale``: ``D ** -0.5`` by default.  Rows of idle slots come out as zeros."""
     if isinstance(mask, torch.Tensor) or mask not in (None, "causal"):
         raise NotImplementedError("Paged attention only supports mask=None or causal")
-    table, lens = _step("paged_attention_fp8", pages, query, block_table, context_lens, block_table_host, context_lens_host)
+    table, lens, host = _step("paged_attention_fp8", pages, query, block_table, context_lens, block_table_host, context_lens_host)
     factor = query.shape[-1] ** -0.5 if scale is None else float(scale)
     blocks.fp8_devices("paged_attention_fp8", pages.index, query, table, lens)
-    return blocks.fp8_attention_of(pages.native, pages.index, _rows(query), table, lens, factor, mask == "causal")
+    # a captured call is replayed for other lengths
+    host = None if torch.cuda.is_current_stream_capturing() else host.astype(np.int32, copy=False).tobytes()
+    return blocks.fp8_attention_of(pages.native, pages.index, _rows(query), table, lens, factor, mask == "causal", host)
