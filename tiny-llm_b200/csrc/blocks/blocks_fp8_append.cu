@@ -34,9 +34,11 @@ struct F8Turns {
 struct F8Append : tlb_fp8_append_call {
     tlb_fp8_pages pages;
     int group;
+    unsigned group_magic, half_magic;  // for divisions by group and rot / 2
     float2 root, k_more;  // sqrt(dim) and dim * k_eps, as sums of two numbers
     F8Append(const tlb_fp8_pages &p, const tlb_fp8_append_call &c, int g) : tlb_fp8_append_call(c), pages(p), group(g) {
         auto two = [](double v) { return make_float2(static_cast<float>(v), static_cast<float>(v - static_cast<float>(v))); };
+        group_magic = f8_magic(kF8Tokens * static_cast<unsigned long long>(g), g), half_magic = f8_magic(kF8Tokens * kApMostDim / 2, c.rot / 2);
         root = two(sqrt(static_cast<double>(p.dim))), k_more = two(static_cast<double>(p.dim) * c.k_eps);
     }
 };
@@ -170,7 +172,10 @@ __device__ __forceinline__ void ap_key(const ApRow<T> &row, const F8Append &a, c
             float g[8];
             w.load(static_cast<const T *>(a.k_norm), at.a0, at.b0), w.get(g);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) u[e] = ap_times(ap_times({x[e], 0.f}, {g[e], 0.f}), r);
+            for (int e = 0; e < 8; ++e) {
+                const float p = x[e] * g[e];  // of two bf16 numbers: all of it
+                u[e] = ap_times({p, sizeof(T) == 2 ? 0.f : fmaf(x[e], g[e], -p)}, r);
+            }
         }
     }
     if (at.pair < 0) {
@@ -230,8 +235,11 @@ __global__ void __launch_bounds__(kApThreads) fp8_append_kernel(const __grid_con
     extern __shared__ __align__(16) unsigned char sm[];
     float4 *angle = reinterpret_cast<float4 *>(sm);  // [tokens][half]
     __shared__ float4 part[kApParts];
+    __shared__ double of[kApMostDim / 2];
     __shared__ float most[2][WARPS];
+    // (parameters read at 32 places at once are read one after another: once, then from shared memory)
     if (threadIdx.x < kApParts) part[threadIdx.x] = turns.part[threadIdx.x];
+    if (threadIdx.x < a.rot / 2) of[threadIdx.x] = turns.of[threadIdx.x];
     tl::griddep_launch();
     tl::griddep_wait();
     const tlb_fp8_pages &pg = a.pages;
@@ -270,7 +278,8 @@ __global__ void __launch_bounds__(kApThreads) fp8_append_kernel(const __grid_con
 #pragma unroll
         for (int s = 0; s < AHEAD; ++s) {
             const int r = r0 + s * ROWS + slot_row;
-            if (at.on && r < n * G) qr[s].load(q + r / G * a.q_l + r % G * a.q_h, at.a0, at.b0);
+            const int l = f8_div(r, G, a.group_magic);
+            if (at.on && r < n * G) qr[s].load(q + l * a.q_l + (r - l * G) * a.q_h, at.a0, at.b0);
             else qr[s].zero();
         }
     };
@@ -278,7 +287,10 @@ __global__ void __launch_bounds__(kApThreads) fp8_append_kernel(const __grid_con
     float before[2] = {0.f, 0.f};
     if (there && kept) before[0] = pg.key_scales[f8_scale_at(pg, page, h, slot)], before[1] = pg.value_scales[f8_scale_at(pg, page, h, slot)];
     __syncthreads();
-    for (int i = threadIdx.x; i < n * half; i += kApThreads) angle[i] = ap_angle(p0 + i / half, turns.of[i % half], part);
+    for (int i = threadIdx.x; i < n * half; i += kApThreads) {
+        const int l = f8_div(i, half, a.half_magic);
+        angle[i] = ap_angle(p0 + l, of[i - l * half], part);
+    }
     __syncthreads();
 
     float x[2][PASSES][8], m[2] = {0.f, 0.f};
@@ -327,12 +339,12 @@ __global__ void __launch_bounds__(kApThreads) fp8_append_kernel(const __grid_con
         if (r0) ask(r0);
 #pragma unroll
         for (int s = 0; s < AHEAD; ++s) {
-            const int r = r0 + s * ROWS + slot_row, row = min(r, n * G - 1);
+            const int r = r0 + s * ROWS + slot_row, row = min(r, n * G - 1), l = f8_div(row, G, a.group_magic);
             if (r0 + s * ROWS + warp * RW >= n * G) continue;  // whole warps
             float y[8];
-            ap_query<T, LP>(qr[s], a, at, angle + row / G * half, y);
+            ap_query<T, LP>(qr[s], a, at, angle + l * half, y);
             if (r < n * G && at.on) {
-                T *to = q_out + (static_cast<size_t>(l0 + row / G) * a.heads + row % G) * D;
+                T *to = q_out + (static_cast<size_t>(l0 + l) * a.heads + row - l * G) * D;
                 store4(to + at.a0, make_float4(y[0], y[1], y[2], y[3])), store4(to + at.b0, make_float4(y[4], y[5], y[6], y[7]));
             }
         }

@@ -102,13 +102,13 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
     const int D = DIM ? DIM : pg.dim, G = a.group, L = a.tokens;
     const AtPiece mine = at_piece(a, blockIdx.x);
     if (mine.b < 0) return;
-    const int b = mine.b, cb = at_div(mine.item, pg.heads, a.heads_magic), h = mine.item - cb * pg.heads, c0 = cb * COLS, ctx = at_context(a, b);
+    const int b = mine.b, cb = f8_div(mine.item, pg.heads, a.heads_magic), h = mine.item - cb * pg.heads, c0 = cb * COLS, ctx = at_context(a, b);
     // keys [0, limit) are seen; a column behind the last one goes along with it, its query is 0 and nothing of it is stored
-    auto limit_of = [&](int col) { return a.causal ? max(ctx - L + 1 + at_div(min(col, G * L - 1), G, a.group_magic), 0) : ctx; };
+    auto limit_of = [&](int col) { return a.causal ? max(ctx - L + 1 + f8_div(min(col, G * L - 1), G, a.group_magic), 0) : ctx; };
     const int low = limit_of(c0), end = min(limit_of(c0 + COLS - 1), ctx);
     const int begin = mine.piece * mine.size, stop = min((end + kF8Tokens - 1) / kF8Tokens, begin + mine.size);
     const int32_t *table = a.table + static_cast<size_t>(b) * a.max_pages;
-    auto page_at = [&](int blk) { return at_div(blk, a.page_blocks, a.page_magic); };  // the blk-th block's place in the table
+    auto page_at = [&](int blk) { return f8_div(blk, a.page_blocks, a.page_magic); };  // the blk-th block's place in the table
     const int stage_bytes = at_stage(D);
     unsigned char *ring = sm + warp * kAtStages * stage_bytes;
     const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
 #pragma unroll
     for (int e = 0; e < 8; ++e) x8[e] = 0.f;
     if (qcol < COLS && c0 + qcol < G * L && (DIM || qd < D)) {
-        const int l = at_div(c0 + qcol, G, a.group_magic);
+        const int l = f8_div(c0 + qcol, G, a.group_magic);
         at_query(static_cast<const T *>(a.q) + b * a.q_b + (static_cast<long long>(h) * G + c0 + qcol - l * G) * a.q_h + l * a.q_l + qd, a.wide_rows, x8);
     }
     const int count = max((stop - begin - warp + WARPS - 1) / WARPS, 0);  // of this warp's blocks
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
         if (threadIdx.x < live) to[COLS * D + threadIdx.x] = part_m[threadIdx.x], to[COLS * (D + 1) + threadIdx.x] = part_l[threadIdx.x];
     } else {
         for (int i = threadIdx.x; i < live * (D / 4); i += WARPS * 32) {
-            const int col = i / (D / 4), d = i % (D / 4), c = c0 + col, l = at_div(c, G, a.group_magic);
+            const int col = i / (D / 4), d = i % (D / 4), c = c0 + col, l = f8_div(c, G, a.group_magic);
             const float4 v = reinterpret_cast<const float4 *>(part + col * ROW)[d];
             const float inv = part_l[col] == 0.f ? 0.f : 1.f / part_l[col];  // nothing seen: zeros
             store4(static_cast<T *>(a.out) + ((static_cast<size_t>(b) * L + l) * a.heads + static_cast<size_t>(h) * G + c - l * G) * D + 4 * d,
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(kAtJoin) fp8_attend_join_kernel(const __grid_c
     __shared__ float sums[kAtJoinColumns];
     const tlb_fp8_pages &pg = a.pages;
     const int D = pg.dim, G = a.group, L = a.tokens, each = pg.heads * a.col_blocks, skip = blockIdx.y * kAtJoinColumns;
-    const int b = at_div(blockIdx.x, each, a.each_magic), item = static_cast<int>(blockIdx.x) - b * each, cb = at_div(item, pg.heads, a.heads_magic), h = item - cb * pg.heads;
+    const int b = f8_div(blockIdx.x, each, a.each_magic), item = static_cast<int>(blockIdx.x) - b * each, cb = f8_div(item, pg.heads, a.heads_magic), h = item - cb * pg.heads;
     const int c0 = cb * cols + skip;
     // the lengths are there: this launch begins once the one before it, which makes the pieces, is past its own wait
     const AtCut cut = at_cut(a);
@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(kAtJoin) fp8_attend_join_kernel(const __grid_c
         }
         if (i >= quads || (groups == 1 && group > 0 && quads <= kAtJoin)) continue;
         const float inv = sums[col];
-        const int c = c0 + col, l = at_div(c, G, a.group_magic);
+        const int c = c0 + col, l = f8_div(c, G, a.group_magic);
         store4(static_cast<T *>(a.out) + ((static_cast<size_t>(b) * L + l) * a.heads + static_cast<size_t>(h) * G + c - l * G) * D + 4 * d,
                make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
     }
@@ -543,7 +543,7 @@ static int attend_launch(F8Attend a, cudaStream_t st) {
     a.col_blocks = (a.group * a.tokens + cols - 1) / cols;
     const long long items = static_cast<long long>(a.col_blocks) * a.pages.heads * a.batch;
     if (items > 0x3fffffff) return tl::fail(TL_EINVAL, "fp8_attention: sizes out of range");
-    a.each_magic = at_magic(items + a.slots, a.pages.heads * a.col_blocks);
+    a.each_magic = f8_magic(items + a.slots, a.pages.heads * a.col_blocks);
     cudaError_t e = tl::launch_chained(kernel, dim3(static_cast<unsigned>(items + (a.workspace ? a.slots : 0))), dim3(kAtWarps * 32), smem, st, a);
     if (e != cudaSuccess) return tl::fail(TL_ECUDA, "fp8_attention: %s", cudaGetErrorString(e));
     TL_LAUNCH_CHECK("fp8_attention");
@@ -563,9 +563,9 @@ static int attend_any(F8Attend a, cudaStream_t st) {
     const int D = a.pages.dim;
     a.wide_rows = tl::aligned16(a.q) && ((a.q_b | a.q_h | a.q_l) * static_cast<long long>(sizeof(T)) & 15) == 0;
     a.page_blocks = a.pages.page_size / kF8Tokens;
-    a.page_magic = at_magic(static_cast<unsigned long long>(a.max_pages) * a.page_blocks + 64, a.page_blocks);  // the first pages are looked up ahead of the length
-    a.group_magic = at_magic(static_cast<unsigned long long>(a.group) * a.tokens, a.group);
-    a.heads_magic = at_magic(static_cast<unsigned long long>(a.pages.heads) * ((a.group * a.tokens + 7) / 8), a.pages.heads);
+    a.page_magic = f8_magic(static_cast<unsigned long long>(a.max_pages) * a.page_blocks + 64, a.page_blocks);  // the first pages are looked up ahead of the length
+    a.group_magic = f8_magic(static_cast<unsigned long long>(a.group) * a.tokens, a.group);
+    a.heads_magic = f8_magic(static_cast<unsigned long long>(a.pages.heads) * ((a.group * a.tokens + 7) / 8), a.pages.heads);
     a.slots = attend_slots(a.dtype, D, a.group * a.tokens), a.most_pieces = 128, a.whole = kAtWhole;
     if (f8_portion_takes(a.pages, a)) return f8_portion(a, st);
     if (D <= 64) return D == 64 ? attend_columns<T, 64, 64>(a, st) : attend_columns<T, 64, 0>(a, st);

@@ -14,7 +14,7 @@ struct F8Attend : tlb_fp8_attention_call {
     int granule;            // pieces are a multiple of so many blocks
     int whole;              // blocks of a request that is not cut
     int page_blocks;        // blocks of 16 tokens in a page
-    unsigned page_magic, group_magic, heads_magic, each_magic;  // for divisions by page_blocks, group, heads and the items of a request (at_div)
+    unsigned page_magic, group_magic, heads_magic, each_magic;  // for divisions by page_blocks, group, heads and the items of a request (f8_div)
     bool wide_rows;         // query rows may be read 16 bytes at a time
     float scale_log2, scale_rest;  // scale * log2(e), and what its rounding to fp32 left
     F8Attend(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c, void *ws)
@@ -35,9 +35,6 @@ __device__ __forceinline__ float at_ex2(float x) {
 __device__ __forceinline__ void at_halves(uint32_t four, uint32_t &lo, uint32_t &hi) {  // four e4m3 numbers as f16
     asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(four));
 }
-// n / d by a product; magic 0: where that might be off.
-__device__ __forceinline__ int at_div(int n, int d, unsigned magic) { return magic ? static_cast<int>(__umulhi(n, magic)) : n / d; }
-
 // 8 entries of a query
 template <typename T>
 __device__ __forceinline__ void at_query(const T *q, bool wide, float (&x)[8]) {
@@ -103,11 +100,11 @@ __device__ __forceinline__ AtPiece at_piece(const F8Attend &a, int index) {
     const AtCut cut = at_cut(a);
     AtPiece x{-1, 0, 0, 1, 0x3fffffff};
     if (cut == 0) {
-        x.b = at_div(index, each, a.each_magic), x.item = index - x.b * each;
+        x.b = f8_div(index, each, a.each_magic), x.item = index - x.b * each;
         if (x.b >= a.batch) x.b = -1;
         return x;
     }
-    const int want = at_div(index, each, a.each_magic);  // rounded down: an item's pieces over all items of a request are a multiple of them
+    const int want = f8_div(index, each, a.each_magic);  // rounded down: an item's pieces over all items of a request are a multiple of them
     int run = 0;
     for (int r0 = 0; r0 < a.batch; r0 += 32) {
         const int mine = r0 + lane < a.batch ? at_pieces(a, cut, r0 + lane) : 0;
@@ -133,8 +130,6 @@ __device__ __forceinline__ AtPiece at_piece(const F8Attend &a, int index) {
 
 // blocks_fp8_attention.cu: adds up the pieces of the launch in front, items of `cols` columns each.
 int f8_attend_join(const F8Attend &a, int cols, cudaStream_t st);
-// 2^32 / d, rounded up: n / d is the upper half of n times it while n * d < 2^32; 0 where `most`, the largest n, is too large for that.
-static inline unsigned at_magic(unsigned long long most, unsigned d) { return d > 1 && most < (1ull << 32) / d ? static_cast<unsigned>((1ull << 32) / d) + 1 : 0; }
 __host__ __device__ static inline size_t at_piece_floats(int cols, int dim) { return static_cast<size_t>(cols) * (dim + 2); }
 // blocks_fp8_portion.cu: bf16 queries of many columns
 constexpr int kPoRows = 256;  // columns of a CTA

@@ -26,6 +26,10 @@ __host__ __device__ __forceinline__ size_t f8_scale_at(const tlb_fp8_pages &p, i
     return (static_cast<size_t>(page) * p.heads + head) * (p.page_size / kF8Tokens) + slot / kF8Tokens;
 }
 
+// 2^32 / d, rounded up: n / d is the upper half of n times it while n * d < 2^32; 0 where `most`, the largest n, is too large for that.
+static inline unsigned f8_magic(unsigned long long most, unsigned d) { return d > 1 && most < (1ull << 32) / d ? static_cast<unsigned>((1ull << 32) / d) + 1 : 0; }
+__device__ __forceinline__ int f8_div(int n, int d, unsigned magic) { return magic ? static_cast<int>(__umulhi(n, magic)) : n / d; }
+
 // What every entry asks of the pages.
 int f8_check_pages(const char *op, const tlb_fp8_pages *p);
 

@@ -112,13 +112,13 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
     const int index = static_cast<int>(gridDim.x - 1 - blockIdx.x);  // late columns, which see most, first
     const AtPiece mine = at_piece(a, index);
     if (mine.b < 0) return;
-    const int b = mine.b, cb = at_div(mine.item, pg.heads, a.heads_magic), h = mine.item - cb * pg.heads, c0 = cb * kPoRows, ctx = at_context(a, b);
+    const int b = mine.b, cb = f8_div(mine.item, pg.heads, a.heads_magic), h = mine.item - cb * pg.heads, c0 = cb * kPoRows, ctx = at_context(a, b);
     // keys [0, limit) are seen; a row behind the last one goes along with it
-    auto limit_of = [&](int col) { return a.causal ? max(ctx - L + 1 + at_div(min(col, columns - 1), G, a.group_magic), 0) : ctx; };
+    auto limit_of = [&](int col) { return a.causal ? max(ctx - L + 1 + f8_div(min(col, columns - 1), G, a.group_magic), 0) : ctx; };
     const int end = min(limit_of(c0 + kPoRows - 1), ctx), begin = mine.piece * mine.size, stop = min((end + kF8Tokens - 1) / kF8Tokens, begin + mine.size);
     const int first = begin * kF8Tokens, past = min(stop * kF8Tokens, end), n_tiles = max((past - first + kPoKeys - 1) / kPoKeys, 0);  // keys [first, past)
     const int32_t *table = a.table + static_cast<size_t>(b) * a.max_pages;
-    auto page_at = [&](int blk) { return at_div(blk, a.page_blocks, a.page_magic); };
+    auto page_at = [&](int blk) { return f8_div(blk, a.page_blocks, a.page_magic); };
     // the scale of block blk, NaN where its page is none
     auto block_at = [&](int blk, int &page) {
         const int at = page_at(blk);
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
         unsigned char *mine_q = psm + Z::k_off + (warp * 32 + lane) * 16;
 #pragma unroll 2
         for (int i = 0; i < N; ++i) {
-            const int col = c0 + (i * 8 + warp) * ROWS + lane / LANES, l = at_div(min(col, columns - 1), G, a.group_magic);
+            const int col = c0 + (i * 8 + warp) * ROWS + lane / LANES, l = f8_div(min(col, columns - 1), G, a.group_magic);
             const bf16 *from = q + l * a.q_l + (min(col, columns - 1) - l * G) * a.q_h;
             if (a.wide_rows) {
                 po_copy16(g_smem_u32(mine_q + i * 4096), from, col < columns);
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
         const bool whole = mine.pieces == 1;
         const float inv = (whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f) * verdict;
         float *part = whole ? nullptr : static_cast<float *>(a.workspace) + index * at_piece_floats(kPoRows, DIM);
-        const int l = at_div(live ? col : 0, G, a.group_magic);
+        const int l = f8_div(live ? col : 0, G, a.group_magic);
         bf16 *out = static_cast<bf16 *>(a.out) + ((static_cast<size_t>(b) * L + l) * a.heads + static_cast<size_t>(h) * G + (live ? col : 0) - l * G) * DIM;
 #pragma unroll 1
         for (int i = 0; i < DIM / 32; ++i) {
@@ -457,7 +457,7 @@ int f8_portion(F8Attend a, cudaStream_t st) {
     const long long items = static_cast<long long>(a.col_blocks) * a.pages.heads * a.batch;
     if (items > 0x3fffffff) return tl::fail(TL_EINVAL, "fp8_attention: sizes out of range");
     const unsigned ctas = static_cast<unsigned>(items + (a.workspace ? a.slots : 0));
-    a.each_magic = at_magic(ctas, a.pages.heads * a.col_blocks);
+    a.each_magic = f8_magic(ctas, a.pages.heads * a.col_blocks);
     return a.pages.dim == 64 ? portion_launch<64>(a, ctas, st) : portion_launch<128>(a, ctas, st);
 }
 
