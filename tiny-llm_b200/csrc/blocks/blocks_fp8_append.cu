@@ -35,10 +35,12 @@ struct F8Append : tlb_fp8_append_call {
     tlb_fp8_pages pages;
     int group;
     unsigned group_magic, half_magic;  // for divisions by group and rot / 2
+    float under_dim;  // 1 / dim
     float2 root, k_more;  // sqrt(dim) and dim * k_eps, as sums of two numbers
     F8Append(const tlb_fp8_pages &p, const tlb_fp8_append_call &c, int g) : tlb_fp8_append_call(c), pages(p), group(g) {
         auto two = [](double v) { return make_float2(static_cast<float>(v), static_cast<float>(v - static_cast<float>(v))); };
         group_magic = f8_magic(kF8Tokens * static_cast<unsigned long long>(g), g), half_magic = f8_magic(kF8Tokens * kApMostDim / 2, c.rot / 2);
+        under_dim = 1.f / p.dim;
         root = two(sqrt(static_cast<double>(p.dim))), k_more = two(static_cast<double>(p.dim) * c.k_eps);
     }
 };
@@ -130,12 +132,14 @@ struct ApRow<float> {
 
 // Where a lane's entries lie, and the pairs that they are: entries e and e + 4 (apart), or 2e and 2e + 1 of the eight.
 struct ApPlace {
-    int a0, b0, pair;  // pair: number of the first one, -1: not rotated
+    int a0, b0, pair;  // pair: a quarter of the number of the first one, -1: not rotated
     bool on, side_by_side;
 };
+// A token's angles: the first of every four pairs, then the second ones and so on, so that lanes side by side read numbers side by side.
+__device__ __forceinline__ int ap_angle_at(int pair, int half) { return (pair & 3) * (half >> 2) + (pair >> 2); }
 __device__ __forceinline__ ApPlace ap_place(const F8Append &a, int l) {
     const bool turned = 8 * l < a.rot, halves = turned && !a.interleaved;
-    return {halves ? 4 * l : 8 * l, halves ? a.rot / 2 + 4 * l : 8 * l + 4, turned ? 4 * l : -1, 8 * l < a.pages.dim, a.interleaved != 0};
+    return {halves ? 4 * l : 8 * l, halves ? a.rot / 2 + 4 * l : 8 * l + 4, turned ? l : -1, 8 * l < a.pages.dim, a.interleaved != 0};
 }
 
 // Norm and rotation in sums of two fp32 numbers.  Whole warps.  1 / sqrt(mean(x^2) + eps) = sqrt(D) / sqrt(sum(x^2) + D eps).
@@ -185,7 +189,7 @@ __device__ __forceinline__ void ap_key(const ApRow<T> &row, const F8Append &a, c
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const float4 t = turn[at.pair + e];
+        const float4 t = turn[e * (a.rot >> 3) + at.pair];
         const ApTwo c{t.x, t.y}, n{t.z, t.w};
         const ApTwo p = at.side_by_side ? u[2 * e] : u[e], q = at.side_by_side ? u[2 * e + 1] : u[e + 4];
         const ApTwo pc = ap_times(p, c), qn = ap_times(q, n), qc = ap_times(q, c), pn = ap_times(p, n);
@@ -198,7 +202,7 @@ __device__ __forceinline__ void ap_key(const ApRow<T> &row, const F8Append &a, c
 
 // The same in 32 bits.
 template <typename T, int LP>
-__device__ __forceinline__ void ap_query(const ApRow<T> &row, const F8Append &a, const ApPlace &at, const float4 *turn, float (&y)[8]) {
+__device__ __forceinline__ void ap_query(const ApRow<T> &row, const F8Append &a, const ApPlace &at, const float (&weight)[8], const float4 *turn, float (&y)[8]) {
     float x[8];
     row.get(x);
     if (a.q_norm) {
@@ -207,22 +211,17 @@ __device__ __forceinline__ void ap_query(const ApRow<T> &row, const F8Append &a,
         for (int e = 0; e < 8; ++e) s = fmaf(x[e], x[e], s);
 #pragma unroll
         for (int o = 1; o < LP; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        const float r = 1.f / sqrtf(s / a.pages.dim + a.q_eps);
-        if (at.on) {
-            ApRow<T> w;
-            float g[8];
-            w.load(static_cast<const T *>(a.q_norm), at.a0, at.b0), w.get(g);
+        const float r = rsqrtf(fmaf(s, a.under_dim, a.q_eps));
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] *= r * g[e];
-        }
+        for (int e = 0; e < 8; ++e) x[e] *= r * weight[e];
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = x[e];
     if (at.pair < 0) return;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const float4 t = turn[at.pair + e];
-        const float c = t.x + t.y, n = t.z + t.w, p = at.side_by_side ? x[2 * e] : x[e], q = at.side_by_side ? x[2 * e + 1] : x[e + 4];
+        const float4 t = turn[e * (a.rot >> 3) + at.pair];
+        const float c = t.x, n = t.z, p = at.side_by_side ? x[2 * e] : x[e], q = at.side_by_side ? x[2 * e + 1] : x[e + 4];
         const float one = p * c - q * n, two = q * c + p * n;
         if (at.side_by_side) y[2 * e] = one, y[2 * e + 1] = two;
         else y[e] = one, y[e + 4] = two;
@@ -289,7 +288,7 @@ __global__ void __launch_bounds__(kApThreads) fp8_append_kernel(const __grid_con
     __syncthreads();
     for (int i = threadIdx.x; i < n * half; i += kApThreads) {
         const int l = f8_div(i, half, a.half_magic);
-        angle[i] = ap_angle(p0 + l, of[i - l * half], part);
+        angle[l * half + ap_angle_at(i - l * half, half)] = ap_angle(p0 + l, of[i - l * half], part);
     }
     __syncthreads();
 
@@ -335,6 +334,13 @@ __global__ void __launch_bounds__(kApThreads) fp8_append_kernel(const __grid_con
             if (threadIdx.x == 0) (side ? pg.value_scales : pg.key_scales)[f8_scale_at(pg, page, h, slot)] = scale;
         }
     }
+    float weight[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) weight[e] = 1.f;
+    if (a.q_norm && at.on) {
+        ApRow<T> w;
+        w.load(static_cast<const T *>(a.q_norm), at.a0, at.b0), w.get(weight);
+    }
     for (int r0 = 0; r0 < n * G; r0 += AHEAD * ROWS) {
         if (r0) ask(r0);
 #pragma unroll
@@ -342,7 +348,7 @@ __global__ void __launch_bounds__(kApThreads) fp8_append_kernel(const __grid_con
             const int r = r0 + s * ROWS + slot_row, row = min(r, n * G - 1), l = f8_div(row, G, a.group_magic);
             if (r0 + s * ROWS + warp * RW >= n * G) continue;  // whole warps
             float y[8];
-            ap_query<T, LP>(qr[s], a, at, angle + l * half, y);
+            ap_query<T, LP>(qr[s], a, at, weight, angle + l * half, y);
             if (r < n * G && at.on) {
                 T *to = q_out + (static_cast<size_t>(l0 + l) * a.heads + row - l * G) * D;
                 store4(to + at.a0, make_float4(y[0], y[1], y[2], y[3])), store4(to + at.b0, make_float4(y[4], y[5], y[6], y[7]));
