@@ -11,7 +11,7 @@ from .batch import ContinuousBatcher, Request, batch_generate
 from .checkpoint import load_checkpoint, load_tokenizer, read_tensors, save_checkpoint
 from .embedding import Embedding, QuantizedEmbedding
 from .fp8 import Fp8Weights, fp8_linear
-from .fp8_cache import Fp8KvPages, paged_attention_fp8, rotate_append_fp8
+from .fp8_cache import Fp8KvPagedCache, Fp8KvPagedPool, Fp8KvPages, paged_attention_fp8, rotate_append_fp8
 from .generate import greedy_generate_ids, simple_generate_with_kv_cache
 from .kv_cache import BatchingKvCache, TinyKvCache, TinyKvFullCache
 from .layer_norm import RMSNorm

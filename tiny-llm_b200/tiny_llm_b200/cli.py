@@ -105,10 +105,14 @@ def _model(args, ns, name):
     from .models import dispatch_model
 
     if name is None:  # already a model object
+        if args.kv_cache != "bf16":
+            raise SystemExit("--kv-cache e4m3 is for Qwen3 checkpoints")
         return ns
     if args.loader == "week2":
+        if args.kv_cache != "bf16":
+            raise SystemExit("--kv-cache e4m3 needs the week3 loader")
         return dispatch_model(name, ns, week=2)
-    return dispatch_model(name, ns, week=3, enable_paged_attention=not args.disable_paged_attention)
+    return dispatch_model(name, ns, week=3, enable_paged_attention=not args.disable_paged_attention, kv_cache=args.kv_cache)
 
 
 def _prompt_ids(args, tokenizer, prompt: str | None):
@@ -187,6 +191,7 @@ def main(argv=None) -> int:
         p.add_argument("--device", default="cuda:0")
         p.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16", help="compute dtype of designs with unquantised weights")
         p.add_argument("--disable-paged-attention", action="store_true")
+        p.add_argument("--kv-cache", choices=["bf16", "e4m3"], default="bf16", help="keys and values of Qwen3 checkpoints in 16 or in 8 bits")
         p.add_argument("--enable-thinking", action="store_true")
         p.add_argument("--max-new-tokens", type=int, default=128)
     sub.choices["generate"].add_argument("--sampler-temp", type=float, default=0.0)

@@ -3,9 +3,14 @@
 ``Fp8KvPages`` is the storage (the page layout of ``TinyKvPagedPool``, one byte a number), ``rotate_append_fp8`` puts a step's keys and values
 into it, with the norm and the rotation that queries and keys pass on the way, and ``paged_attention_fp8`` is ``paged_attention`` over it.  The block
 table and the context lengths are those of the 16-bit cache: a request's tokens fill its pages in order, ``context_lens`` count the step's own
-tokens, 0 marks an idle slot."""
+tokens, 0 marks an idle slot.
+
+``Fp8KvPagedPool`` and ``Fp8KvPagedCache`` are the page allocator and a request's cache over such pages (``Qwen3ModelWeek3(..., kv_cache="e4m3")``); both sides of the
+bookkeeping are those of ``TinyKvPagedPool`` and ``TinyKvPagedCache``."""
 
 from __future__ import annotations
+
+from dataclasses import dataclass
 
 import numpy as np
 import torch
@@ -13,6 +18,7 @@ import torch
 from extensions_b200.tiny_llm_ext_b200 import blocks
 
 from .attention import validate_paged_metadata
+from .paged_kv_cache import _SLAB_VERSIONS, TinyKvPagedCache, TinyKvPagedPool
 
 TOKENS = 16  # that share a scale
 _DTYPES = (torch.float32, torch.bfloat16)
@@ -54,6 +60,14 @@ class Fp8KvPages:
     @property
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.keys, self.values, self.key_scales, self.value_scales))
+
+    def grown(self, num_pages: int, live: int) -> "Fp8KvPages":
+        """Room for ``num_pages``, with the first ``live`` ones as they are here."""
+        new = Fp8KvPages.zeros(num_pages, self.kv_heads, self.page_size, self.head_dim, device=self.device)
+        for to, old in ((new.keys.view(torch.uint8), self.keys.view(torch.uint8)), (new.values.view(torch.uint8), self.values.view(torch.uint8)), (new.key_scales, self.key_scales),
+                        (new.value_scales, self.value_scales)):
+            to[:live] = old[:live]
+        return new
 
     def dequantize(self, pages=slice(None), dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
         """(keys, values) that the numbers of ``pages`` (an index into the first dimension) stand for."""
@@ -138,3 +152,147 @@ def paged_attention_fp8(query: torch.Tensor, pages: Fp8KvPages, block_table: tor
     # a captured call is replayed for other lengths
     host = None if torch.cuda.is_current_stream_capturing() else host.astype(np.int32, copy=False).tobytes()
     return blocks.fp8_attention_of(pages.native, pages.index, _rows(query), table, lens, factor, mask == "causal", host)
+
+
+@dataclass
+class Fp8KvMetadata:
+    """What attention over an 8-bit cache needs for one layer; the ``*_host`` fields are the copies the tensors were made from."""
+
+    pages: Fp8KvPages
+    block_table: torch.Tensor
+    context_lens: torch.Tensor
+    block_table_host: np.ndarray
+    context_lens_host: np.ndarray
+
+
+class Fp8KvPagedPool(TinyKvPagedPool):
+    """A layer's pages of 8 bits: the allocator of ``TinyKvPagedPool`` over ``Fp8KvPages``, which are made with the first tokens (or ``reserve``) and grow
+    geometrically.  ``max_pages``: an append that needs more fails instead."""
+
+    def __init__(self, page_size: int = 128, max_pages: int | None = None):
+        if page_size <= 0 or page_size % TOKENS:
+            raise ValueError(f"an 8-bit page holds a multiple of {TOKENS} tokens, got {page_size}")
+        super().__init__(page_size=page_size)
+        self.pages: Fp8KvPages | None = None
+        self.max_pages = max_pages
+
+    @property
+    def capacity(self) -> int:
+        return 0 if self.pages is None else self.pages.num_pages
+
+    @property
+    def key_pages(self):
+        raise AttributeError("an 8-bit pool has .pages")
+
+    value_pages = key_pages
+
+    @property
+    def storage_nbytes(self) -> int:
+        return 0 if self.pages is None else self.pages.nbytes
+
+    def read_page(self, page_id: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values ``[1, H, page_size, D]`` (fp32) that a page's numbers stand for."""
+        if self.pages is None:
+            raise ValueError(f"Page {page_id} has no storage")
+        if not 0 <= page_id < self.num_pages:
+            raise ValueError(f"Page {page_id} is out of range")
+        return self.pages.dequantize(slice(page_id, page_id + 1))
+
+    def reserve(self, num_pages: int, heads: int, head_dim: int, dtype=None, device="cuda") -> None:
+        """Room for ``num_pages`` (one counted growth; live pages are carried over)."""
+        if self.pages is not None and (self.pages.kv_heads, self.pages.head_dim) != (heads, head_dim):
+            raise ValueError("keys and values must match the existing pages")
+        if self.capacity >= num_pages:
+            return
+        if self.max_pages is not None and num_pages > self.max_pages:
+            raise RuntimeError(f"page pool exhausted: {num_pages} pages wanted, the pool is fixed at {self.max_pages}")
+        if self.pages is None:
+            self.pages = Fp8KvPages.zeros(num_pages, heads, self.page_size, head_dim, device=device)
+        else:
+            live = min(self.num_pages, self.capacity)
+            self.copied_pages_on_growth += live
+            self.copied_bytes_on_growth += self.pages.nbytes // self.pages.num_pages * live
+            self.pages = self.pages.grown(num_pages, live)
+        self.storage_growths += 1
+        self.slab_version = next(_SLAB_VERSIONS)
+
+    def ensure_room(self, fresh_pages: int, heads: int, head_dim: int, device) -> None:
+        """Make sure ``fresh_pages`` allocations will find storage."""
+        wanted = self.num_pages + max(0, fresh_pages - len(self.free_page_ids))
+        if wanted > self.capacity or self.pages is None:
+            self.reserve(max(wanted, min(max(4, wanted, self.capacity * 2), self.max_pages or 1 << 62)), heads, head_dim, device=device)
+        elif (self.pages.kv_heads, self.pages.head_dim) != (heads, head_dim):
+            raise ValueError("keys and values must match the existing pages")
+
+    def reset(self) -> None:
+        super().reset()
+        self.pages = None
+
+    def _snapshot_state(self) -> tuple:
+        return (*super()._snapshot_state(), self.pages)
+
+    def _restore_state(self, state: tuple) -> None:
+        super()._restore_state(state[:-1])
+        if self.pages is not state[-1]:
+            self.pages = state[-1]
+            self.slab_version = next(_SLAB_VERSIONS)
+
+    def _ensure_page_storage(self, key, value) -> None:
+        raise NotImplementedError("an 8-bit pool is filled by rotate_append_paged")
+
+    def can_batch_decode_append(self, keys, slots) -> bool:
+        return False
+
+
+class Fp8KvPagedCache(TinyKvPagedCache):
+    """A request's pages in an ``Fp8KvPagedPool``."""
+
+    def __init__(self, pool: Fp8KvPagedPool):
+        if not isinstance(pool, Fp8KvPagedPool):
+            raise ValueError("an 8-bit cache needs an 8-bit pool")
+        super().__init__(pool)
+
+    def _device(self):
+        return self.pool.pages.device if self.pool.pages is not None else torch.device("cpu")
+
+    def update_and_fetch(self, key, value, mask_length=None, mask=None):
+        raise NotImplementedError("an 8-bit cache is filled by rotate_append_paged")
+
+    update_and_fetch_paged = update_and_fetch
+
+    def rotate_append_paged(self, query, key, value, *, rope=None, query_norm=None, key_norm=None) -> tuple[torch.Tensor, Fp8KvMetadata]:
+        """``rotate_append_fp8`` of the request's next tokens (``[1, H, L, D]``) -> (queries, what ``paged_attention_fp8`` needs)."""
+        return append_step([self], query, key, value, rope=rope, query_norm=query_norm, key_norm=key_norm)
+
+
+def append_step(slots: list, query, key, value, *, rope=None, query_norm=None, key_norm=None) -> tuple[torch.Tensor, Fp8KvMetadata]:
+    """One launch for a step of all ``slots`` (``Fp8KvPagedCache``, or None where idle) of one pool; all or nothing."""
+    live = [s for s in slots if s is not None]
+    if not live:
+        raise ValueError("Cannot build paged metadata without active requests")
+    pool = live[0].pool
+    if any(not isinstance(s, Fp8KvPagedCache) or s.pool is not pool for s in live):
+        raise ValueError("Paged batch caches must share one page pool")
+    if query.dim() != 4 or key.dim() != 4 or key.shape != value.shape or key.shape[0] != len(slots) or min(key.shape) <= 0:
+        raise ValueError("K/V chunks must be 4D [B, H, S, D], a row for every slot")
+    heads, count, dim = key.shape[1:]
+    theirs, mine = pool._snapshot_state(), [s._snapshot_state() for s in live]
+    try:
+        for s in live:
+            room = s.page_size - s.page_lens[-1] if s.page_ids else 0
+            pool.ensure_room(max(0, -(-(count - room) // s.page_size)), heads, dim, key.device)
+            s.append_slots(count)
+        table = np.full((len(slots), max(s.num_pages for s in live)), -1, dtype=np.int32)
+        lens = np.zeros(len(slots), dtype=np.int32)
+        for b, s in enumerate(slots):
+            if s is not None:
+                table[b, : s.num_pages], lens[b] = s.page_ids, s.offset
+        meta = Fp8KvMetadata(pool.pages, torch.from_numpy(table).to(key.device), torch.from_numpy(lens).to(key.device), table, lens)
+        out = rotate_append_fp8(query, key, value, pool.pages, meta.block_table, meta.context_lens, rope=rope, query_norm=query_norm, key_norm=key_norm, block_table_host=table,
+                                context_lens_host=lens)
+    except Exception:
+        pool._restore_state(theirs)
+        for s, state in zip(live, mine):
+            s._restore_state(state)
+        raise
+    return out, meta

@@ -218,6 +218,21 @@ class BatchingKvCache(TinyKvCache):
             context_lens_host=ctx_host,
         )
 
+    def rotate_append_paged(self, query, key, value, *, rope=None, query_norm=None, key_norm=None):
+        """The step of all slots over an 8-bit cache (``fp8_cache.append_step``): one launch, whatever the number of new tokens."""
+        from .fp8_cache import append_step
+
+        if key.dim() != 4 or key.shape[0] != self.max_active_requests:
+            raise ValueError(f"Expected batch size {self.max_active_requests}, got {key.shape[0]}")
+        if self.HD is not None and self.HD != (key.shape[1], key.shape[3]):
+            raise ValueError(f"expect {self.HD} but got {key.shape[1], key.shape[3]}")
+        if self.max_seq_len is not None and any(s is not None and s.offset + key.shape[2] > self.max_seq_len for s in self.kv_caches):
+            raise ValueError("Paged batch append exceeds max_seq_len")
+        answer = append_step(self.kv_caches, query, key, value, rope=rope, query_norm=query_norm, key_norm=key_norm)
+        self.HD = (key.shape[1], key.shape[3])
+        self.last_batch_bytes = 0
+        return answer
+
     def _metadata_host(self, width: int, context: list[int]) -> tuple[np.ndarray, np.ndarray]:
         """Rows of page ids padded with -1 (idle slots are all -1) and the
         post-append context lengths (kv_cache.py:210-221)."""

@@ -17,6 +17,7 @@ import torch
 
 from .attention import paged_attention
 from .embedding import QuantizedEmbedding
+from .fp8_cache import Fp8KvPagedCache, Fp8KvPagedPool, paged_attention_fp8
 from .kv_cache import TinyKvCache
 from .paged_kv_cache import TinyKvPagedCache, TinyKvPagedPool
 from .quantize import QuantizedWeights, quantized_linear, quantized_mlp
@@ -48,6 +49,7 @@ class Qwen3MultiHeadAttention:
         theta: int = 1000000,
         rms_norm_eps: float = 1e-5,
         use_paged_attention: bool = True,
+        kv_cache: str = "bf16",
     ):
         assert num_heads % num_kv_heads == 0, f"num_heads {num_heads} must be divisible by num_kv_heads {num_kv_heads}"
         self.hidden_size = hidden_size
@@ -60,11 +62,22 @@ class Qwen3MultiHeadAttention:
         self.q_norm = FastRMSNorm(head_dim, q_norm, eps=rms_norm_eps)
         self.k_norm = FastRMSNorm(head_dim, k_norm, eps=rms_norm_eps)
         self.use_paged_attention = use_paged_attention
+        self.kv_cache = kv_cache
+
+    def _attend_fp8(self, q, k, v, cache):
+        """Norms, rotation and append in one launch, attention over the pages of 8 bits in another (two where long contexts are cut)."""
+        q, meta = cache.rotate_append_paged(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), rope=self.rope, query_norm=self.q_norm, key_norm=self.k_norm)
+        y = paged_attention_fp8(q, meta.pages, meta.block_table, meta.context_lens, scale=self.scale, mask="causal", block_table_host=meta.block_table_host,
+                                context_lens_host=meta.context_lens_host)
+        return y.transpose(1, 2)
 
     def __call__(self, x, offsets, cache: TinyKvCache, mask=None):
         B, L, _ = x.shape
         q = quantized_linear(x, self.wq).reshape(B, L, self.num_heads, self.head_dim)
         k = quantized_linear(x, self.wk).reshape(B, L, self.num_kv_heads, self.head_dim)
+        if self.kv_cache == "e4m3":
+            v = quantized_linear(x, self.wv).reshape(B, L, self.num_kv_heads, self.head_dim)
+            return quantized_linear(self._attend_fp8(q, k, v, cache).reshape(B, L, self.num_heads * self.head_dim), self.wo)
         q = self.q_norm(q)
         k = self.k_norm(k)
         v = quantized_linear(x, self.wv).reshape(B, L, self.num_kv_heads, self.head_dim)
@@ -131,6 +144,7 @@ class Qwen3TransformerBlock:
         max_seq_len: int = 32768,
         theta: int = 1000000,
         use_paged_attention: bool = True,
+        kv_cache: str = "bf16",
     ):
         self.num_attention_heads = num_attention_heads
         self.hidden_size = hidden_size
@@ -152,6 +166,7 @@ class Qwen3TransformerBlock:
             theta=theta,
             rms_norm_eps=rms_norm_eps,
             use_paged_attention=use_paged_attention,
+            kv_cache=kv_cache,
         )
 
     def __call__(self, x, offset, cache: TinyKvCache, mask=None):
@@ -169,16 +184,22 @@ def is_qwen3_moe_sparse_layer(args: Any, layer_idx: int) -> bool:
 
 
 class Qwen3ModelWeek3:
-    """qwen3_week3.py:218-338."""
+    """qwen3_week3.py:218-338.  ``kv_cache="e4m3"`` (not in the reference) keeps keys and values in 8 bits, half the memory a token: the caches
+    are ``Fp8KvPagedCache`` s, positions are the cache's own, and steps run operator by operator."""
 
-    def __init__(self, mlx_model: Any, page_size: int = 128, enable_paged_attention: bool = True):
+    def __init__(self, mlx_model: Any, page_size: int = 128, enable_paged_attention: bool = True, kv_cache: str = "bf16"):
         args = mlx_model.args
+        if kv_cache not in ("bf16", "e4m3"):
+            raise ValueError(f"kv_cache={kv_cache!r}: bf16 or e4m3")
+        if kv_cache == "e4m3" and (not enable_paged_attention or args.head_dim % 16 or args.head_dim > 256):
+            raise ValueError("an e4m3 cache is paged, for heads of a multiple of 16 entries up to 256")
+        self.kv_cache = kv_cache
         self.num_hidden_layers = args.num_hidden_layers
         self.hidden_size = args.hidden_size
         self.vocab_size = args.vocab_size
         self.page_size = page_size
         # One physical pool per layer; page ids are layer-local (as in the kernels).
-        self.page_pools = [TinyKvPagedPool(page_size=page_size) for _ in range(self.num_hidden_layers)]
+        self.page_pools = [(Fp8KvPagedPool if kv_cache == "e4m3" else TinyKvPagedPool)(page_size=page_size) for _ in range(self.num_hidden_layers)]
         self.precision = torch.bfloat16
 
         def packed(layer: Any) -> QuantizedWeights:
@@ -223,6 +244,7 @@ class Qwen3ModelWeek3:
                     max_seq_len=args.max_position_embeddings,
                     theta=args.rope_theta,
                     use_paged_attention=enable_paged_attention,
+                    kv_cache=kv_cache,
                 )
             )
         self.norm = FastRMSNorm(args.hidden_size, weight=mlx_model.model.norm.weight, eps=args.rms_norm_eps)
@@ -245,13 +267,15 @@ class Qwen3ModelWeek3:
 
     def create_kv_cache(self) -> list[TinyKvCache]:
         """One logical cache per layer, all sharing that layer's pool."""
-        return [TinyKvPagedCache(pool=pool) for pool in self.page_pools]
+        return [(Fp8KvPagedCache if self.kv_cache == "e4m3" else TinyKvPagedCache)(pool=pool) for pool in self.page_pools]
 
     # ---- CUDA-graph decode path ------------------------------------------------
     def decode_engine(self, batch_size: int, max_seq_len: int | None = None, device=None):
         """The (cached) graph engine for ``batch_size`` decode slots."""
         from .engine import DecodeEngine
 
+        if self.kv_cache != "bf16":
+            raise NotImplementedError("graph engines are for a bf16 cache")
         limit = max_seq_len or self.decode_graph_max_seq_len
         key = (batch_size, limit)
         if key not in self._decode_engines:
@@ -262,7 +286,7 @@ class Qwen3ModelWeek3:
         return self._decode_engines[key]
 
     def _graph_decode_applies(self, inputs, cache) -> bool:
-        if self.use_decode_graph is False or not self._paged or inputs.dim() != 2 or inputs.shape[1] != 1 or not inputs.is_cuda:
+        if self.use_decode_graph is False or self.kv_cache != "bf16" or not self._paged or inputs.dim() != 2 or inputs.shape[1] != 1 or not inputs.is_cuda:
             return False
         from .kv_cache import BatchingKvCache
 
@@ -358,7 +382,7 @@ class Qwen3ModelWeek3:
         from .engine import PrefillEngine
 
         chunk = self.prefill_graph_len
-        if chunk == 0 or self.use_decode_graph is False or not self._paged or logits_to_keep != 1:
+        if chunk == 0 or self.use_decode_graph is False or self.kv_cache != "bf16" or not self._paged or logits_to_keep != 1:
             return None
         if inputs.dim() != 2 or inputs.shape[0] != 1 or not inputs.is_cuda:
             return None
@@ -384,7 +408,18 @@ class Qwen3ModelWeek3:
         logits, _ = engine.prefill_chunk(inputs.reshape(-1), off, cache)
         return logits.clone()
 
+    @staticmethod
+    def _check_offsets(offset, cache) -> None:
+        """An 8-bit cache rotates by its own positions: the caller's have to be the same (of idle slots any)."""
+        slots = getattr(cache, "kv_caches", [cache])
+        given = offset.reshape(-1).tolist() if isinstance(offset, torch.Tensor) else [offset] if isinstance(offset, int) else [int(o) for o in offset]
+        given = given * len(slots) if len(given) == 1 else given
+        if len(given) != len(slots) or any(s is not None and s.offset != o for s, o in zip(slots, given)):
+            raise ValueError("offset must be the number of tokens in the cache")
+
     def __call__(self, inputs, offset, cache: list[TinyKvCache], logits_to_keep: int | None = None):
+        if self.kv_cache == "e4m3":
+            self._check_offsets(offset, cache[0])
         if self._graph_decode_applies(inputs, cache):
             return self._graph_decode(inputs, offset, cache, logits_to_keep)
         if inputs.dim() == 2 and inputs.shape[1] > 1 and inputs.is_cuda:
