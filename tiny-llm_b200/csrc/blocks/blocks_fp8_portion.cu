@@ -170,37 +170,39 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     if (warp >= 8 && warp < 16) look_up(0), ask(0), look_up(1), ask(1), look_up(2);
-    if (warp >= 8) {  // the largest scales
-        for (int blk = begin + threadIdx.x - 8 * 32; blk < stop; blk += kPoThreads - 8 * 32) {
-            int page;
-            const size_t at = block_at(blk, page);
-            const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(pg.num_pages);
-            const float k = there ? __ldg(pg.key_scales + at) : NAN, v = there ? __ldg(pg.value_scales + at) : NAN;
-            if (k < INFINITY) atomicMax(seen, __float_as_int(k));
-            if (v < INFINITY) atomicMax(seen + 1, __float_as_int(v));
-            if (!(k < INFINITY) || !(v < INFINITY)) seen[2] = 1;
-        }
-    } else {  // queries: 8 entries a lane, a row to 8 or 16 lanes; first as they are, to where the operand tiles will be
-        constexpr int LANES = DIM / 8, ROWS = 32 / LANES, N = kPoRows / (8 * ROWS);
+    // queries: 8 entries a lane, a row to 8 or 16 lanes of the first sixteen warps; first as they are, to where the operand tiles will be
+    constexpr int LANES = DIM / 8, ROWS = 32 / LANES, N = kPoRows / (16 * ROWS);
+    unsigned char *mine_q = psm + Z::k_off + threadIdx.x * 16;
+    if (warp < 16) {
         const bf16 *q = static_cast<const bf16 *>(a.q) + b * a.q_b + static_cast<long long>(h) * G * a.q_h + lane % LANES * 8;
-        const float sign = a.scale_log2 < 0.f ? -1.f : 1.f;
-        unsigned char *mine_q = psm + Z::k_off + (warp * 32 + lane) * 16;
-#pragma unroll 2
+#pragma unroll 4
         for (int i = 0; i < N; ++i) {
-            const int col = c0 + (i * 8 + warp) * ROWS + lane / LANES, l = f8_div(min(col, columns - 1), G, a.group_magic);
+            const int col = c0 + (i * 16 + warp) * ROWS + lane / LANES, l = f8_div(min(col, columns - 1), G, a.group_magic);
             const bf16 *from = q + l * a.q_l + (min(col, columns - 1) - l * G) * a.q_h;
             if (a.wide_rows) {
-                po_copy16(g_smem_u32(mine_q + i * 4096), from, col < columns);
+                po_copy16(g_smem_u32(mine_q + i * 8192), from, col < columns);
             } else {
 #pragma unroll 1
-                for (int e = 0; e < 8; ++e) reinterpret_cast<bf16 *>(mine_q + i * 4096)[e] = col < columns ? from[e] : __float2bfloat16_rn(0.f);
+                for (int e = 0; e < 8; ++e) reinterpret_cast<bf16 *>(mine_q + i * 8192)[e] = col < columns ? from[e] : __float2bfloat16_rn(0.f);
             }
         }
+    }
+    for (int blk = begin + threadIdx.x; blk < stop; blk += kPoThreads) {  // meanwhile the largest scales
+        int page;
+        const size_t at = block_at(blk, page);
+        const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(pg.num_pages);
+        const float k = there ? __ldg(pg.key_scales + at) : NAN, v = there ? __ldg(pg.value_scales + at) : NAN;
+        if (k < INFINITY) atomicMax(seen, __float_as_int(k));
+        if (v < INFINITY) atomicMax(seen + 1, __float_as_int(v));
+        if (!(k < INFINITY) || !(v < INFINITY)) seen[2] = 1;
+    }
+    if (warp < 16) {
+        const float sign = a.scale_log2 < 0.f ? -1.f : 1.f;
         asm volatile("cp.async.wait_all;" ::: "memory");
-#pragma unroll 2
+#pragma unroll 4
         for (int i = 0; i < N; ++i) {
-            const int row = (i * 8 + warp) * ROWS + lane / LANES;
-            const uint4 u = *reinterpret_cast<const uint4 *>(mine_q + i * 4096);
+            const int row = (i * 16 + warp) * ROWS + lane / LANES;
+            const uint4 u = *reinterpret_cast<const uint4 *>(mine_q + i * 8192);
             const float2 y[4] = {tl::unpack2<bf16>(u.x), tl::unpack2<bf16>(u.y), tl::unpack2<bf16>(u.z), tl::unpack2<bf16>(u.w)};
             float m = 0.f;
 #pragma unroll
