@@ -67,23 +67,28 @@ def pages_of(n=4):
     (dict(lens=LENS.long()), "int32"),
     (dict(lens=LENS[:1]), "batch sizes"),
     (dict(table=TABLE[:1]), "batch sizes"),
-    (dict(table=torch.tensor([[0, 0], [2, -1]], dtype=torch.int32)), "aliased"),
-    (dict(table=torch.tensor([[0, 9], [2, -1]], dtype=torch.int32)), "outside physical"),
-    (dict(table=torch.tensor([[0, 1], [2, 3]], dtype=torch.int32)), "sentinel"),
-    (dict(lens=torch.tensor([40, 5], dtype=torch.int32)), "not covered"),
-    (dict(lens=torch.tensor([20, 2], dtype=torch.int32)), "at least query length"),
-    (dict(lens=torch.tensor([-1, 5], dtype=torch.int32)), "nonnegative"),
+    (dict(table=torch.tensor([[0, 0], [2, -1]], dtype=torch.int32), late=True), "aliased"),
+    (dict(table=torch.tensor([[0, 9], [2, -1]], dtype=torch.int32), late=True), "outside physical"),
+    (dict(table=torch.tensor([[0, 1], [2, 3]], dtype=torch.int32), late=True), "sentinel"),
+    (dict(lens=torch.tensor([40, 5], dtype=torch.int32), late=True), "not covered"),
+    (dict(lens=torch.tensor([20, 2], dtype=torch.int32), late=True), "at least query length"),
+    (dict(lens=torch.tensor([-1, 5], dtype=torch.int32), late=True), "nonnegative"),
     (dict(hosts=dict(context_lens_host=np.array([20, 5, 1], dtype=np.int32))), "copies"),
     (dict(hosts=dict(block_table_host=np.array([[0, 1, -1], [2, -1, -1]], dtype=np.int32))), "copies"),
 ])
-def test_steps_that_do_not_fit_are_refused_by_both(change, text):
+def test_steps_that_do_not_fit_are_refused_by_both(change, text, monkeypatch):
     q, k, v = step()
     table, lens, hosts = change.get("table", TABLE), change.get("lens", LENS), change.get("hosts", {})
     q = change.get("q", q)
-    with pytest.raises(ValueError, match=text):
-        paged_attention_fp8(q, pages_of(), table, lens, **hosts)
-    with pytest.raises(ValueError, match=text):
-        rotate_append_fp8(q, k, v, pages_of(), table, lens, **hosts)
+    for call in (lambda p: paged_attention_fp8(q, p, table, lens, **hosts), lambda p: rotate_append_fp8(q, k, v, p, table, lens, **hosts)):
+        pages = pages_of()
+        if change.get("late"):  # found by the library, behind the check for a GPU: nothing is launched for any of them
+            monkeypatch.setattr(blocks, "fp8_devices", lambda *a: None)
+            monkeypatch.setattr(blocks, "_current_device", lambda: pages.index)
+            monkeypatch.setattr(blocks, "_raw_stream", lambda device: 0)
+            monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+        with pytest.raises(ValueError, match=text):
+            call(pages)
 
 
 def test_what_append_alone_refuses():
@@ -132,16 +137,24 @@ def test_c_entries_refuse_sizes_and_pointers():
     bad_pages = [blocks.Fp8Pages(0, 8192, 4096, 4096, 4, 2, 16, 32), blocks.Fp8Pages(4096, 8192, 4096, 4096, 4, 2, 24, 32), blocks.Fp8Pages(4096, 8192, 4096, 4096, 4, 2, 16, 8),
                  blocks.Fp8Pages(4096, 8192, 4096, 4096, 4, 2, 16, 512), blocks.Fp8Pages(4104, 8192, 4096, 4096, 4, 2, 16, 32), blocks.Fp8Pages(4096, 8192, 4096, 4096, 0, 2, 16, 32)]
     for p in bad_pages:
-        assert lib.tlb_fp8_attention(ctypes.addressof(p), call(), None, 0, None) == -1
+        assert lib.tlb_fp8_attention(ctypes.addressof(p), call(), None, None, None, 0, None) == -1
         assert lib.tlb_fp8_attention_workspace(ctypes.addressof(p), call(), None) == 0
     for bad in (dict(H=3), dict(H=0), dict(B=-1), dict(L=-1), dict(pages=0), dict(q=0), dict(out=0), dict(table=0), dict(lens=0)):
-        assert lib.tlb_fp8_attention(ctypes.addressof(pages), call(**bad), None, 0, None) == -1, bad
-    assert lib.tlb_fp8_attention(ctypes.addressof(pages), call(dtype=1), None, 0, None) == -2
-    assert lib.tlb_fp8_attention(ctypes.addressof(pages), call(B=0, q=0), None, 0, None) == 0  # nothing to do
+        assert lib.tlb_fp8_attention(ctypes.addressof(pages), call(**bad), None, None, None, 0, None) == -1, bad
+    assert lib.tlb_fp8_attention(ctypes.addressof(pages), call(dtype=1), None, None, None, 0, None) == -2
+    assert lib.tlb_fp8_attention(ctypes.addressof(pages), call(B=0, q=0), None, None, None, 0, None) == 0  # nothing to do
     long = blocks.Fp8Pages(4096, 8192, 4096, 4096, 4, 2, 128, 32)
     size = lib.tlb_fp8_attention_workspace(ctypes.addressof(long), call(pages=100), None)
     assert size > 0
-    assert lib.tlb_fp8_attention(ctypes.addressof(long), call(pages=100), 4096, size - 1, None) == -3
+    assert lib.tlb_fp8_attention(ctypes.addressof(long), call(pages=100), None, None, 4096, size - 1, None) == -3
+    ints = lambda *v: np.array(v, dtype=np.int32).tobytes()  # noqa: E731
+    many = blocks.Fp8Pages(4096, 8192, 4096, 4096, 100, 2, 128, 32)
+    assert lib.tlb_fp8_attention(ctypes.addressof(many), call(pages=90), ints(128 * 90), ints(*range(90)), None, 0, None) == -3
+    for lens, table in ((5, (4,)), (5, (-1,)), (20, (0,)), (-1, (0,)), (0, (0,))):  # outside, none, not covered, negative, an idle request's page
+        assert lib.tlb_fp8_attention(ctypes.addressof(pages), call(), ints(lens), ints(*table), None, 0, None) == -1
+    for lens, table in (((5, 5), (1, 1)), ((1, 2), (0, 1))):  # twice the same page, shorter than the step
+        assert lib.tlb_fp8_attention(ctypes.addressof(pages), call(B=2, L=2), ints(*lens), ints(*table), None, 0, None) == -1
+    assert lib.tlb_fp8_attention(ctypes.addressof(pages), call(), ints(5), None, None, 0, None) == -1
     assert lib.tlb_fp8_attention_workspace(ctypes.addressof(long), call(pages=100), np.array([100], dtype=np.int32).tobytes()) == 0  # short for now
 
 

@@ -16,6 +16,8 @@
 // fp8_append_any_kernel takes what that cannot: rows that do not begin on 16 bytes, rotations of dimensions that are no multiple of 8.
 #include <math.h>
 
+#include <vector>
+
 #include "../per_device.h"
 #include "blocks_fp8_cache.cuh"
 
@@ -488,6 +490,32 @@ int f8_check_pages(const char *op, const tlb_fp8_pages *p) {
     return TL_OK;
 }
 
+int f8_check_step(const char *op, const tlb_fp8_pages &p, const int32_t *lens, const int32_t *table, int batch, int max_pages, int tokens) {
+    if (!lens && !table) return TL_OK;
+    if (!lens || !table) return tl::fail(TL_EINVAL, "%s: lengths and block table on the host go together", op);
+    std::vector<uint64_t> seen;  // a bit for every page
+    try {
+        seen.resize((static_cast<size_t>(p.num_pages) + 63) / 64);
+    } catch (...) {  // no exception leaves a C entry
+        return tl::fail(TL_EINVAL, "%s: no memory for the checks", op);
+    }
+    for (int b = 0; b < batch; ++b) {
+        const int32_t *row = table + static_cast<size_t>(b) * max_pages;
+        const long long n = lens[b], live = (n + p.page_size - 1) / p.page_size;
+        bool fine = n >= 0 && (n == 0 || n >= tokens) && live <= max_pages;
+        for (int i = 0; fine && i < max_pages; ++i) {
+            const int32_t id = row[i];
+            if (i >= live) {
+                fine = id == -1;
+            } else if ((fine = id >= 0 && id < p.num_pages && !(seen[id >> 6] >> (id & 63) & 1))) {
+                seen[id >> 6] |= uint64_t{1} << (id & 63);
+            }
+        }
+        if (!fine) return tl::fail(TL_EINVAL, "%s: lengths or block table of request %d", op, b);
+    }
+    return TL_OK;
+}
+
 template <typename T>
 static int append_launch(const F8Append &a, const F8Turns &turns, cudaStream_t st) {
     static tl::PerDevice ready;
@@ -515,7 +543,7 @@ static int append_launch(const F8Append &a, const F8Turns &turns, cudaStream_t s
 
 using namespace tlb;
 
-extern "C" int tlb_fp8_append(const tlb_fp8_pages *pages, const tlb_fp8_append_call *c, void *stream) {
+extern "C" int tlb_fp8_append(const tlb_fp8_pages *pages, const tlb_fp8_append_call *c, const int32_t *lens_host, const int32_t *table_host, void *stream) {
     const int rc = f8_check_pages("fp8_append", pages);
     if (rc != TL_OK) return rc;
     if (!c || c->batch < 0 || c->tokens < 0 || c->heads <= 0 || c->heads % pages->heads) return tl::fail(TL_EINVAL, "fp8_append: query heads over %d key/value heads", pages->heads);
@@ -523,6 +551,7 @@ extern "C" int tlb_fp8_append(const tlb_fp8_pages *pages, const tlb_fp8_append_c
     if (c->batch == 0 || c->tokens == 0) return TL_OK;
     if (c->batch > 65535 || pages->heads > 65535 || c->tokens > (1 << 30) || c->max_pages <= 0) return tl::fail(TL_EINVAL, "fp8_append: sizes out of range");
     if (!c->q || !c->q_out || !c->k || !c->v || !c->table || !c->lens) return tl::fail(TL_EINVAL, "fp8_append: missing argument");
+    if (const int bad = f8_check_step("fp8_append", *pages, lens_host, table_host, c->batch, c->max_pages, c->tokens)) return bad;
     // the frequencies of this thread's last call; half as many powers otherwise
     static thread_local F8Turns turns;
     static thread_local int turns_rot = -1;

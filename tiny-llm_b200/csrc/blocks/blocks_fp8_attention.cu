@@ -596,13 +596,16 @@ extern "C" size_t tlb_fp8_attention_workspace(const tlb_fp8_pages *pages, const 
     return static_cast<size_t>(items + slots) * at_piece_floats(cols, pages->dim) * sizeof(float);
 }
 
-extern "C" int tlb_fp8_attention(const tlb_fp8_pages *pages, const tlb_fp8_attention_call *c, void *workspace, size_t workspace_bytes, void *stream) {
+extern "C" int tlb_fp8_attention(const tlb_fp8_pages *pages, const tlb_fp8_attention_call *c, const int32_t *lens_host, const int32_t *table_host, void *workspace,
+                                 size_t workspace_bytes, void *stream) {
     const int rc = f8_check_pages("fp8_attention", pages);
     if (rc != TL_OK) return rc;
     if (!c || c->batch < 0 || c->tokens < 0 || c->heads <= 0 || c->heads % pages->heads) return tl::fail(TL_EINVAL, "fp8_attention: query heads over %d key/value heads", pages->heads);
     if (c->batch == 0 || c->tokens == 0) return TL_OK;
     if (c->max_pages <= 0 || static_cast<long long>(c->heads / pages->heads) * c->tokens > (1 << 30)) return tl::fail(TL_EINVAL, "fp8_attention: sizes out of range");
     if (!c->q || !c->out || !c->table || !c->lens) return tl::fail(TL_EINVAL, "fp8_attention: missing argument");
+    if (const int bad = f8_check_step("fp8_attention", *pages, lens_host, table_host, c->batch, c->max_pages, c->tokens)) return bad;
+    if (lens_host && !workspace && tlb_fp8_attention_workspace(pages, c, lens_host)) return tl::fail(TL_EWORKSPACE, "fp8_attention: a workspace is needed");
     const size_t need = workspace ? tlb_fp8_attention_workspace(pages, c, nullptr) : 0;
     if (need && (workspace_bytes < need || !tl::aligned16(workspace))) return tl::fail(TL_EWORKSPACE, "fp8_attention: the workspace must have %zu bytes, from a boundary of 16 on", need);
     const F8Attend a(*pages, *c, need ? workspace : nullptr);  // without one every item is whole

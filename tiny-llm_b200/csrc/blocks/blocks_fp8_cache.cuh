@@ -32,5 +32,7 @@ __device__ __forceinline__ int f8_div(int n, int d, unsigned magic) { return mag
 
 // What every entry asks of the pages.
 int f8_check_pages(const char *op, const tlb_fp8_pages *p);
+// The host's copies of a step's lengths and block table, where they are given: see tlb_fp8_append.
+int f8_check_step(const char *op, const tlb_fp8_pages &p, const int32_t *lens, const int32_t *table, int batch, int max_pages, int tokens);
 
 }  // namespace tlb

@@ -99,9 +99,9 @@ _SIGNATURES = {
     "tlb_fp8_linear_workspace": (ctypes.c_size_t, [_I, _I]),
     "tlb_fp8_linear": (_I, [_VP, _LL, _VP, _I, _VP, _VP, _VP, _I, _I, _I, _VP, ctypes.c_size_t, _I, _VP]),
     "tlb_fp8_gated_mlp_workspace": (ctypes.c_size_t, [_I, _I, _I]),
-    "tlb_fp8_append": (_I, [_VP, ctypes.c_char_p, _VP]),
-    "tlb_fp8_attention_workspace": (ctypes.c_size_t, [_VP, ctypes.c_char_p, ctypes.c_char_p]),
-    "tlb_fp8_attention": (_I, [_VP, ctypes.c_char_p, _VP, ctypes.c_size_t, _VP]),
+    "tlb_fp8_append": (_I, [_VP, ctypes.c_char_p, _VP, _VP, _VP]),
+    "tlb_fp8_attention_workspace": (ctypes.c_size_t, [_VP, ctypes.c_char_p, _VP]),
+    "tlb_fp8_attention": (_I, [_VP, ctypes.c_char_p, _VP, _VP, _VP, ctypes.c_size_t, _VP]),
     "tlb_fp8_gated_mlp": (_I, [_VP, _LL, _VP, _I, _VP, _VP, _I, _VP, _VP, _I, _I, _I, _I, _F, _F, _VP, ctypes.c_size_t, _I, _VP]),
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -1188,6 +1188,7 @@ class Fp8Pages(ctypes.Structure):
     _fields_ = [(name, _VP) for name in ("keys", "values", "key_scales", "value_scales")] + [(name, _I) for name in ("num_pages", "heads", "page_size", "dim")]
 
 
+_EINVAL, _EWORKSPACE = -1, -3
 # tlb_fp8_append_call and tlb_fp8_attention_call, packed at once: of small calls the host sets the pace, and ctypes converts two dozen arguments one by one
 _FP8_APPEND = struct.Struct("@PPPPPPPPqqqqqqqqqdffiiiiiii")
 _FP8_ATTENTION = struct.Struct("@PPPPqqqdiiiiii")
@@ -1229,20 +1230,25 @@ def _token_by_token(like: torch.Tensor, B: int, H: int, L: int, D: int) -> torch
     return torch.empty_strided((B, H, L, D), (L * H * D, D, H * D, 1), dtype=like.dtype, device=like.device)
 
 
-def fp8_append_of(pages: Fp8Pages, device: int, q, k, v, table, lens, q_norm=None, q_eps=0.0, k_norm=None, k_eps=0.0, rot=0, base=1.0, interleaved=False) -> torch.Tensor:
-    """``fp8_append`` of tensors that the caller has checked (``rotate_append_fp8``)."""
+def fp8_append_of(pages: Fp8Pages, device: int, q, k, v, table, lens, q_norm=None, q_eps=0.0, k_norm=None, k_eps=0.0, rot=0, base=1.0, interleaved=False, lens_host=None,
+                  table_host=None):
+    """``fp8_append`` of tensors that the caller has checked (``rotate_append_fp8``).  ``lens_host``, ``table_host``: the lengths' and the table's bytes (int32) or addresses; the
+    answer is None where the library refuses them."""
     if _current_device() != device:
         with torch.cuda.device(device):
-            return fp8_append_of(pages, device, q, k, v, table, lens, q_norm, q_eps, k_norm, k_eps, rot, base, interleaved)
+            return fp8_append_of(pages, device, q, k, v, table, lens, q_norm, q_eps, k_norm, k_eps, rot, base, interleaved, lens_host, table_host)
     B, H, L, D = q.shape
     out = _token_by_token(q, B, H, L, D)
     qb, qh, ql, _ = q.stride()
     kb, kh, kl, _ = k.stride()
     vb, vh, vl, _ = v.stride()
     call = _FP8_APPEND.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(), 0 if q_norm is None else q_norm.data_ptr(),
-                            0 if k_norm is None else k_norm.data_ptr(), qb, qh, ql, kb, kh, kl, vb, vh, vl, base, q_eps, k_eps, B, H, L, table.shape[1], rot, interleaved, _DTYPE_CODE[q.dtype])
-    rc = library().tlb_fp8_append(ctypes.addressof(pages), call, _raw_stream(device))
+                            0 if k_norm is None else k_norm.data_ptr(), qb, qh, ql, kb, kh, kl, vb, vh, vl, base, q_eps, k_eps, B, H, L, table.shape[1], rot, interleaved,
+                            _DTYPE_CODE[q.dtype])
+    rc = library().tlb_fp8_append(ctypes.addressof(pages), call, lens_host, table_host, _raw_stream(device))
     if rc:
+        if lens_host is not None and rc == _EINVAL:
+            return None
         _check(rc)
     return out
 
@@ -1254,20 +1260,25 @@ def fp8_attention(pages: Fp8Pages, device: int, q: torch.Tensor, table: torch.Te
     return fp8_attention_of(pages, device, q, table, lens, scale, causal)
 
 
-def fp8_attention_of(pages: Fp8Pages, device: int, q, table, lens, scale, causal, lens_host: bytes | None = None) -> torch.Tensor:
-    """``fp8_attention`` of tensors that the caller has checked (``paged_attention_fp8``); ``lens_host``: the lengths as int32, if the call is for these alone."""
+def fp8_attention_of(pages: Fp8Pages, device: int, q, table, lens, scale, causal, lens_host=None, table_host=None):
+    """``fp8_attention`` of tensors that the caller has checked (``paged_attention_fp8``).  ``lens_host``, ``table_host``: the lengths' and the table's bytes (int32) or addresses,
+    if the call is for these alone; the answer is None where the library refuses them."""
     if _current_device() != device:
         with torch.cuda.device(device):
-            return fp8_attention_of(pages, device, q, table, lens, scale, causal, lens_host)
+            return fp8_attention_of(pages, device, q, table, lens, scale, causal, lens_host, table_host)
     B, H, L, D = q.shape
     out = _token_by_token(q, B, H, L, D)
     qb, qh, ql, _ = q.stride()
     call = _FP8_ATTENTION.pack(q.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(), qb, qh, ql, scale, B, H, L, table.shape[1], causal, _DTYPE_CODE[q.dtype])
-    lib, at = library(), ctypes.addressof(pages)
-    size = lib.tlb_fp8_attention_workspace(at, call, lens_host)
-    scratch = q.new_empty(size, dtype=torch.uint8) if size else None
-    rc = lib.tlb_fp8_attention(at, call, _ptr(scratch), size, _raw_stream(device))
+    lib, at, stream = library(), ctypes.addressof(pages), _raw_stream(device)
+    rc = _EWORKSPACE if lens_host is None else lib.tlb_fp8_attention(at, call, lens_host, table_host, None, 0, stream)
+    if rc == _EWORKSPACE:  # long requests may be cut into pieces
+        size = lib.tlb_fp8_attention_workspace(at, call, lens_host)
+        scratch = q.new_empty(size, dtype=torch.uint8) if size else None
+        rc = lib.tlb_fp8_attention(at, call, None, None, _ptr(scratch), size, stream)
     if rc:
+        if lens_host is not None and rc == _EINVAL:
+            return None
         _check(rc)
     return out
 

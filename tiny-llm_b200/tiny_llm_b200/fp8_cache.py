@@ -22,6 +22,7 @@ from .paged_kv_cache import _SLAB_VERSIONS, TinyKvPagedCache, TinyKvPagedPool
 
 TOKENS = 16  # that share a scale
 _DTYPES = (torch.float32, torch.bfloat16)
+_INT32 = np.dtype(np.int32)
 
 
 class Fp8KvPages:
@@ -76,7 +77,7 @@ class Fp8KvPages:
 
 
 def _step(op: str, pages: Fp8KvPages, query: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor, block_table_host, context_lens_host):
-    """Checks of a step's shapes and metadata -> (block table, context lengths, the lengths on the host)."""
+    """Checks of a step's shapes and metadata -> (block table, context lengths, the host's lengths and table as bytes, and as arrays)."""
     shape, rows = query.shape, block_table.shape
     if len(shape) != 4:
         raise ValueError(f"{op}: query must be 4D [B, H_q, L, D]")
@@ -99,10 +100,21 @@ def _step(op: str, pages: Fp8KvPages, query: torch.Tensor, block_table: torch.Te
     if block_table_host is None:
         block_table_host = block_table.detach().cpu().numpy()
     lens, table = np.asarray(context_lens_host), np.asarray(block_table_host)
-    if lens.shape != (B,) or table.shape != rows:
+    if lens.shape != counts or table.shape != rows:
         raise ValueError(f"{op}: context_lens_host and block_table_host must be copies of the tensors")
-    validate_paged_metadata(lens, table, pages.page_size, pages.num_pages, L)
-    return block_table if block_table.is_contiguous() else block_table.contiguous(), context_lens if context_lens.is_contiguous() else context_lens.contiguous(), lens
+    if lens.dtype != _INT32 or table.dtype != _INT32:  # the library's check is for int32
+        validate_paged_metadata(lens, table, pages.page_size, pages.num_pages, L)
+        lens, table = lens.astype(_INT32), table.astype(_INT32)
+    # a copy of a few kilobytes costs less than numpy's .ctypes
+    bytes_of = table.tobytes() if table.nbytes <= 8192 or not table.flags.c_contiguous else table.ctypes.data
+    return (block_table if block_table.is_contiguous() else block_table.contiguous(), context_lens if context_lens.is_contiguous() else context_lens.contiguous(), lens.tobytes(),
+            bytes_of, (lens, table))
+
+
+def _refused(op: str, pages: Fp8KvPages, hosts: tuple, L: int) -> None:
+    """What the library found in the lengths or the table, as an exception of ``paged_attention``."""
+    validate_paged_metadata(*hosts, pages.page_size, pages.num_pages, L)
+    raise RuntimeError(blocks.library().tlb_last_error().decode() or op)
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -116,7 +128,7 @@ def rotate_append_fp8(query: torch.Tensor, key: torch.Tensor, value: torch.Tenso
     ``query_norm`` and ``key_norm`` (``FastRMSNorm``) and ``rope`` (``FastRoPE``, turned by a token's position) are applied on the way, the keys' in 64 bits
     ahead of their one rounding.  Any strides will do; float32 or bfloat16.  A block of 16 tokens of a head has one scale: it grows where the new
     tokens need it to, and the block's earlier numbers are rounded to it again."""
-    table, lens, _ = _step("rotate_append_fp8", pages, query, block_table, context_lens, block_table_host, context_lens_host)
+    table, lens, lens_host, table_host, hosts = _step("rotate_append_fp8", pages, query, block_table, context_lens, block_table_host, context_lens_host)
     B, _, L, D = query.shape
     if key.shape != (B, pages.kv_heads, L, D) or key.shape != value.shape:
         raise ValueError("rotate_append_fp8: key and value must be [B, H_kv, L, D] beside the query")
@@ -133,11 +145,16 @@ def rotate_append_fp8(query: torch.Tensor, key: torch.Tensor, value: torch.Tenso
         if norm is None:
             weights += (None, 0.0)
             continue
-        weight = norm._weight_as(query.dtype, query.device)
+        weight = norm.weight
+        if weight.dtype != query.dtype or weight.get_device() != pages.index or not weight.is_contiguous():
+            weight = norm._weight_as(query.dtype, query.device)
         if weight.shape != (D,):
             raise ValueError(f"rotate_append_fp8: a norm of {tuple(weight.shape)} for heads of {D}")
         weights += (weight, norm.eps)
-    return blocks.fp8_append_of(pages.native, pages.index, _rows(query), _rows(key), _rows(value), table, lens, *weights, rot, base, interleaved)
+    out = blocks.fp8_append_of(pages.native, pages.index, _rows(query), _rows(key), _rows(value), table, lens, *weights, rot, base, interleaved, lens_host, table_host)
+    if out is None:
+        _refused("rotate_append_fp8", pages, hosts, L)
+    return out
 
 
 def paged_attention_fp8(query: torch.Tensor, pages: Fp8KvPages, block_table: torch.Tensor, context_lens: torch.Tensor, scale: float | None = None,
@@ -146,12 +163,16 @@ def paged_attention_fp8(query: torch.Tensor, pages: Fp8KvPages, block_table: tor
     ``mask``: None or ``"causal"``; ``scale``: ``D ** -0.5`` by default.  Rows of idle slots come out as zeros."""
     if isinstance(mask, torch.Tensor) or mask not in (None, "causal"):
         raise NotImplementedError("Paged attention only supports mask=None or causal")
-    table, lens, host = _step("paged_attention_fp8", pages, query, block_table, context_lens, block_table_host, context_lens_host)
+    table, lens, lens_host, table_host, hosts = _step("paged_attention_fp8", pages, query, block_table, context_lens, block_table_host, context_lens_host)
     factor = query.shape[-1] ** -0.5 if scale is None else float(scale)
     blocks.fp8_devices("paged_attention_fp8", pages.index, query, table, lens)
-    # a captured call is replayed for other lengths
-    host = None if torch.cuda.is_current_stream_capturing() else host.astype(np.int32, copy=False).tobytes()
-    return blocks.fp8_attention_of(pages.native, pages.index, _rows(query), table, lens, factor, mask == "causal", host)
+    if torch.cuda.is_current_stream_capturing():  # a captured call is replayed for other lengths
+        validate_paged_metadata(*hosts, pages.page_size, pages.num_pages, query.shape[2])
+        lens_host = table_host = None
+    out = blocks.fp8_attention_of(pages.native, pages.index, _rows(query), table, lens, factor, mask == "causal", lens_host, table_host)
+    if out is None:
+        _refused("paged_attention_fp8", pages, hosts, query.shape[2])
+    return out
 
 
 @dataclass
