@@ -1,0 +1,179 @@
+"""Calls of the 8-bit cache at the edges of what its documentation allows: rows that begin anywhere, captured launches whose requests grow past the cut into pieces, pages that are
+none, wide groups, far positions, two streams, idle slots.  Helpers and tolerances are those of the operators' own tests."""
+
+import numpy as np
+import pytest
+import torch
+
+from extensions_b200.tiny_llm_ext_b200 import blocks
+from tests.test_gpu_fp8_cache import check_attention, check_side, copy_of, on_host, random_pages, run_append, run_attention, table_of, to_gpu, turned
+from tiny_llm_b200 import FastRoPE, Fp8KvPages, paged_attention_fp8, rotate_append_fp8
+
+DEV = "cuda"
+pytestmark = pytest.mark.gpu
+
+
+def odd_rows(x, pad=3):
+    """The same tensor with rows that begin on any 2 (or 4) bytes."""
+    wide = torch.zeros(*x.shape[:-1], x.shape[-1] + pad, dtype=x.dtype, device=x.device)
+    wide[..., 1 : 1 + x.shape[-1]] = x
+    return wide[..., 1 : 1 + x.shape[-1]]
+
+
+@pytest.mark.parametrize("new", [1, 5, 50])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_that_begin_anywhere(new, dtype):
+    lengths, page, dim = [130, 0, 70], 32, 128
+    table, count = table_of(lengths, page, 2)
+    gen = torch.Generator().manual_seed(new)
+    pages = random_pages(count, 2, page, dim, gen)
+    q, k, v = (torch.randn(3, h, new, dim, generator=gen).to(dtype).to(DEV) for h in (8, 2, 2))
+    args = (torch.from_numpy(table).to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV))
+    even, odd = to_gpu(pages), to_gpu(pages)
+    rope = FastRoPE(dim, 4096, 10000)
+    a, b = rotate_append_fp8(q, k, v, even, *args, rope=rope), rotate_append_fp8(*(odd_rows(x) for x in (q, k, v)), odd, *args, rope=rope)
+    # two kernels: the same definition, so the same numbers but where one lies next to a border
+    assert torch.equal(even.values.view(torch.uint8), odd.values.view(torch.uint8)) and torch.equal(even.value_scales, odd.value_scales) and torch.equal(even.key_scales, odd.key_scales)
+    assert (even.keys.view(torch.uint8) != odd.keys.view(torch.uint8)).float().mean() < 1e-4
+    torch.testing.assert_close(a, b, rtol=2 * torch.finfo(dtype).eps, atol=2.0**-20)
+    whole = paged_attention_fp8(q, even, *args, mask="causal")
+    assert torch.equal(whole, paged_attention_fp8(odd_rows(q), even, *args, mask="causal"))  # the same kernel, read another way
+    assert torch.equal(whole, paged_attention_fp8(q.transpose(1, 2).contiguous().transpose(1, 2), even, *args, mask="causal"))
+    assert torch.equal(whole[:1], paged_attention_fp8(q[:1].expand(3, -1, -1, -1), even, *args, mask="causal")[:1])
+
+
+@pytest.mark.parametrize("new,heads,kv_heads,dim,dtype", [(1, 8, 2, 128, torch.bfloat16), (1, 8, 2, 64, torch.float32), (3, 8, 2, 128, torch.bfloat16), (40, 4, 2, 128, torch.bfloat16), (33, 4, 2, 64, torch.bfloat16)])
+def test_a_captured_call_follows_requests_past_the_cut(new, heads, kv_heads, dim, dtype):
+    page, width = 64, 80
+    gen = torch.Generator().manual_seed(7)
+    pages_host = random_pages(2 * width, kv_heads, page, dim, gen)
+    pages = to_gpu(pages_host)
+    table = np.random.RandomState(1).permutation(2 * width).astype(np.int32).reshape(2, width)
+    q = torch.randn(2, heads, new, dim, generator=gen).to(dtype)
+    gq, gt, lens = q.to(DEV), torch.from_numpy(table).to(DEV), torch.tensor([60, 50], dtype=torch.int32, device=DEV)
+    full = dict(block_table_host=table, context_lens_host=np.asarray([width * page] * 2, dtype=np.int32))  # any lengths are covered
+    paged_attention_fp8(gq, pages, gt, lens, mask="causal", **full)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = paged_attention_fp8(gq, pages, gt, lens, mask="causal", **full)
+    with torch.cuda.graph(side):
+        other = paged_attention_fp8(gq, pages, gt, lens, mask="causal", **full)
+    for lengths in ([60, 50], [5000, 77], [0, 4099], [1100, 1100], [5120, 5120], [new, 0]):
+        lens.copy_(torch.tensor(lengths, dtype=torch.int32))
+        graph.replay(), side.replay()
+        torch.cuda.synchronize()
+        check_attention(out, q, pages_host, table, lengths, True, dim**-0.5, dtype)
+        assert torch.equal(out, other)
+
+
+@pytest.mark.parametrize("lengths,new", [([5000], 1), ([4000, 16, 0, 1030], 1), ([4500, 20], 4), ([3000], 40), ([2500, 100], 70)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_long_requests_in_pieces(lengths, new, dtype):
+    run_attention(lengths, new, 8, 2, 128, 64, dtype, seed=new)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_pages_that_are_none_hide_their_keys(new):
+    """Past the host's checks (a captured launch, another caller of the extension): entries outside the pages are not read."""
+    page, dim, n = 32, 128, 300
+    table, count = table_of([n], page, 3)
+    gen = torch.Generator().manual_seed(4)
+    pages = random_pages(count, 2, page, dim, gen)
+    bad = table.copy()
+    bad[0, 2], bad[0, 5] = -1, count + 7
+    q = torch.randn(1, 8, new, dim, generator=gen).to(torch.bfloat16)
+    gp = to_gpu(pages)
+    out = blocks.fp8_attention(gp.native, gp.index, q.to(DEV), torch.from_numpy(bad).to(DEV), torch.tensor([n], dtype=torch.int32, device=DEV), dim**-0.5, True)
+    # the same with the hidden keys scored far below all others
+    k, v = (torch.cat([x[int(p)] for p in table[0]], dim=1)[:, :n].double() for x in pages.dequantize())
+    hidden = torch.zeros(n, dtype=torch.bool)
+    hidden[2 * page : 3 * page], hidden[5 * page : 6 * page] = True, True
+    keep = ~hidden
+    for h in range(8):
+        x = q[0, h].double()
+        s = (x @ k[h // 4].t() * dim**-0.5).masked_fill(hidden[None] | (torch.arange(n)[None] > torch.arange(n - new, n)[:, None]), -torch.inf)
+        want = torch.softmax(s, -1) @ v[h // 4]
+        # as for attention among the keys that are left: weights off by 2^-12, scores by some 2^-18 of sums of |q k|, outputs by half a step of bf16
+        most = (x.abs() @ k[h // 4].abs().t() * dim**-0.5).amax()
+        tol = (2.0**-11 + 2.0**-18 * most) * (torch.softmax(s, -1) @ v[h // 4].abs() + want.abs()) + 2.0**-8 * want.abs() + 2.0**-16 * v[h // 4][keep].abs().amax(0)
+        assert ((out[0, h].cpu().double() - want).abs() <= tol).all()
+    x = torch.randn(1, 2, 40, dim, generator=gen).to(torch.bfloat16).to(DEV)
+    before = copy_of(gp)
+    turned_q = blocks.fp8_append(gp.native, gp.index, x, x, x, torch.full((1, 10), -1, dtype=torch.int32, device=DEV), torch.tensor([60], dtype=torch.int32, device=DEV))
+    assert torch.equal(turned_q, x) and torch.equal(before.keys.view(torch.uint8), gp.keys.view(torch.uint8)) and torch.equal(before.key_scales, gp.key_scales)
+    for lens in (39, -3, 10 * page + 1):  # shorter than the step, negative, past the table: as an idle slot
+        zeros = blocks.fp8_append(gp.native, gp.index, x, x, x, torch.from_numpy(bad).to(DEV), torch.tensor([lens], dtype=torch.int32, device=DEV))
+        assert not zeros.any() and torch.equal(before.keys.view(torch.uint8), gp.keys.view(torch.uint8))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,new", [(40, 1, 64, 1), (40, 1, 128, 7), (300, 1, 128, 1), (300, 1, 32, 2), (64, 2, 256, 3), (7, 7, 128, 41)])
+def test_wide_groups(heads, kv_heads, dim, new):
+    run_attention([90, 0, 17 + new], new, heads, kv_heads, dim, 16, torch.bfloat16, seed=heads)
+    run_append([90, 0, 17 + new], new, heads, kv_heads, dim, 16, torch.bfloat16, seed=heads)
+
+
+@pytest.mark.parametrize("page", [16, 1024, 4096, 2032])
+def test_page_sizes(page):
+    run_attention([3000, 31], 2, 4, 2, 64, page, torch.bfloat16, seed=page)
+    run_attention([1500, 40], 40, 4, 2, 64, page, torch.bfloat16, seed=page)
+    run_append([3000, 31], 20, 4, 2, 64, page, torch.bfloat16, seed=page)
+
+
+@pytest.mark.parametrize("traditional", [False, True])
+@pytest.mark.parametrize("rot", [128, 120])
+def test_far_positions_turn_exactly(traditional, rot):
+    """Angles of up to a million radians: 24 bits of a turn would be off by a tenth."""
+    n, page, dim, new = 1_000_003, 4096, 128, 19
+    pages = Fp8KvPages.zeros(245, 1, page, dim)
+    table_host = np.arange(245, dtype=np.int32)[None]
+    gen = torch.Generator().manual_seed(8)
+    x = torch.randn(1, 1, new, dim, generator=gen).to(torch.bfloat16)
+    g = x.to(DEV)
+    out = rotate_append_fp8(g, g, g, pages, torch.from_numpy(table_host).to(DEV), torch.tensor([n], dtype=torch.int32, device=DEV), rope=FastRoPE(rot, 4096, 10000, traditional=traditional))
+    want = turned(x[0, 0], None, 0.0, rot, traditional, n - new)
+    size = x[0, 0].double().abs().amax(-1, keepdim=True)
+    assert ((out[0, 0].cpu().double() - want).abs() <= 2.0**-8 * 1.01 * want.abs() + 2.0**-20 * size).all()
+    zero = torch.zeros(245, 1, page, dim, dtype=torch.float64)
+    scales = torch.zeros(245, 1, page // 16, dtype=torch.float64)
+    check_side("keys", on_host(pages.keys), on_host(pages.key_scales), zero, scales, want[None, None], table_host, [n], new, page)
+
+
+def test_idle_slots_and_other_requests_do_not_change_an_answer():
+    gen = torch.Generator().manual_seed(3)
+    pages = to_gpu(random_pages(60, 2, 64, 128, gen))
+    q = torch.randn(1, 8, 1, 128, generator=gen).to(torch.bfloat16).to(DEV)
+    for n in (700, 3000):  # whole, in pieces
+        row = torch.arange(48, dtype=torch.int32, device=DEV)
+        row[-(-n // 64) :] = -1
+        alone = paged_attention_fp8(q, pages, row[None], torch.tensor([n], dtype=torch.int32, device=DEV))
+        idle = torch.full((5, 48), -1, dtype=torch.int32, device=DEV)
+        idle[3] = row
+        beside = paged_attention_fp8(q.expand(5, -1, -1, -1), pages, idle, torch.tensor([0, 0, 0, n, 0], dtype=torch.int32, device=DEV))
+        assert torch.equal(beside[3], alone[0]) and not beside[[0, 1, 2, 4]].any()
+
+
+def test_two_streams_at_once():
+    gen = torch.Generator().manual_seed(6)
+    runs = []
+    for i, (n, new) in enumerate(((4000, 1), (2000, 64))):
+        table, count = table_of([n], 64, i)
+        pages = to_gpu(random_pages(count, 2, 64, 128, gen))
+        q, k, v = (torch.randn(1, h, new, 128, generator=gen).to(torch.bfloat16).to(DEV) for h in (8, 2, 2))
+        runs.append((q, k, v, pages, torch.from_numpy(table).to(DEV), torch.tensor([n], dtype=torch.int32, device=DEV)))
+
+    def once(run):
+        q, k, v, pages, table, lens = run
+        x = rotate_append_fp8(q, k, v, pages, table, lens, rope=FastRoPE(128, 4096, 10000))
+        return paged_attention_fp8(x, pages, table, lens, mask="causal")
+
+    want = [once(r) for r in runs]  # appending the same tokens again leaves the same numbers
+    streams = [torch.cuda.Stream() for _ in runs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(once(runs[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, want[i]) for i in range(2) for a in got[i])
+    assert blocks.library().tlb_tc_gave_up() == 0
