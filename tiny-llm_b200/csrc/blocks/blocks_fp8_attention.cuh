@@ -61,21 +61,20 @@ __device__ __forceinline__ int at_blocks(const F8Attend &a, int b) { return (at_
 typedef int AtCut;
 __device__ __forceinline__ AtCut at_cut(const F8Attend &a) {
     if (!a.workspace) return 0;
-    int live = 0, longest = 0;  // at most 2^27 blocks a request
+    int live = 0, longest = 0;  // at most 2^26 blocks a request
     long long all = 0;
     for (int r = threadIdx.x & 31; r < a.batch; r += 32) {
         const int n = at_blocks(a, r);
         all += n, live += n > 0, longest = max(longest, n);
     }
-    int total = static_cast<int>(min(all, 0x3ffffffLL));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        total += __shfl_xor_sync(0xffffffffu, total, o), live += __shfl_xor_sync(0xffffffffu, live, o);
+        all += __shfl_xor_sync(0xffffffffu, all, o), live += __shfl_xor_sync(0xffffffffu, live, o);
         longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
     }
     const int each = a.pages.heads * a.col_blocks, room = max(a.slots - live * each, a.slots / 2);
     if (longest <= a.whole) return 0;
-    const int mean = static_cast<int>(min((static_cast<long long>(total) * each + room - 1) / room, 0x3fffffffLL));
+    const int mean = static_cast<int>(min((all * each + room - 1) / room, 0x3fffffffLL));
     return max(max(mean, (longest + a.most_pieces - 1) / a.most_pieces), kAtLeast);
 }
 __device__ __forceinline__ int at_pieces(const F8Attend &a, AtCut cut, int b) {
