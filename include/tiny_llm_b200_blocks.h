@@ -398,7 +398,8 @@ int tlb_fp8_gated_mlp(const void *x, long long ldx, const void *w_gate_up, int l
 
 /* A paged key/value cache of 8 bits.  keys, values: e4m3 numbers [num_pages, heads, page_size, dim], 16-byte aligned; key_scales, value_scales: fp32
  * [num_pages, heads, page_size / 16], one for each block of 16 tokens of a head; a number stands for itself times its block's scale.  dim: a multiple of 16 up to
- * 256; page_size: a multiple of 16.  A scale is a power of two, 2^-100 at the least, or NaN: then every number of the block is none. */
+ * 256; page_size: a multiple of 16.  A scale is a power of two, 2^-100 at the least, or NaN: then every number of the block is none.  The numbers
+ * of a request's tokens are finite (other slots may hold anything).  At most 2^31 blocks, and block tables for at most 2^30 tokens a request. */
 typedef struct {
     uint8_t *keys, *values;
     float *key_scales, *value_scales;

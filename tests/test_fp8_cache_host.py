@@ -158,6 +158,18 @@ def test_c_entries_refuse_sizes_and_pointers():
     assert lib.tlb_fp8_attention_workspace(ctypes.addressof(long), call(pages=100), np.array([100], dtype=np.int32).tobytes()) == 0  # short for now
 
 
+def test_sizes_whose_places_an_int_does_not_hold_are_refused():
+    import ctypes
+
+    lib = blocks.library()
+    attend = lambda pages: blocks._FP8_ATTENTION.pack(16, 16, 16, 16, 0, 0, 0, 1.0, 1, 4, 1, pages, 1, 2)  # noqa: E731
+    append = lambda pages: blocks._FP8_APPEND.pack(16, 16, 16, 16, 16, 16, 0, 0, *[0] * 9, 1.0, 0.0, 0.0, 1, 4, 1, pages, 0, 0, 2)  # noqa: E731
+    wide, many = blocks.Fp8Pages(4096, 8192, 4096, 4096, 4, 2, 128, 32), blocks.Fp8Pages(4096, 8192, 4096, 4096, 1 << 28, 2, 128, 32)
+    for pages, width in ((wide, (1 << 23) + 1), (many, 1)):
+        assert lib.tlb_fp8_attention(ctypes.addressof(pages), attend(width), None, None, None, 0, None) == -1
+        assert lib.tlb_fp8_append(ctypes.addressof(pages), append(width), None, None, None) == -1
+
+
 # ---- pool and caches ----------------------------------------------------------------------------------------------------
 
 

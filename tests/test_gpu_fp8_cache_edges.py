@@ -7,7 +7,7 @@ import torch
 
 from extensions_b200.tiny_llm_ext_b200 import blocks
 from tests.test_gpu_fp8_cache import check_attention, check_side, copy_of, on_host, random_pages, run_append, run_attention, table_of, to_gpu, turned
-from tiny_llm_b200 import FastRoPE, Fp8KvPages, paged_attention_fp8, rotate_append_fp8
+from tiny_llm_b200 import FastRMSNorm, FastRoPE, Fp8KvPages, paged_attention_fp8, rotate_append_fp8
 
 DEV = "cuda"
 pytestmark = pytest.mark.gpu
@@ -18,6 +18,30 @@ def odd_rows(x, pad=3):
     wide = torch.zeros(*x.shape[:-1], x.shape[-1] + pad, dtype=x.dtype, device=x.device)
     wide[..., 1 : 1 + x.shape[-1]] = x
     return wide[..., 1 : 1 + x.shape[-1]]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("layout", ["tokens", "columns"])
+def test_norms_of_keys_far_from_one(dtype, layout):
+    def change(q, k, v):
+        k[0, :, 0] *= 1e28
+        k[0, 3, 1] *= 1e13
+        k[1, :, 1] *= 1e-25
+
+    for dim in (64, 144):
+        run_append([40, 35], 20, 4, 2, dim, 16, dtype, change=change, layout=layout, seed=dim)
+
+
+def test_norms_without_an_eps():
+    gen = torch.Generator().manual_seed(2)
+    x = torch.randn(1, 1, 16, 64, generator=gen) * torch.exp2(torch.arange(-75.0, 69.0, 9.0))[:, None]
+    pages = Fp8KvPages.zeros(1, 1, 16, 64)
+    g = x.to(DEV)
+    rotate_append_fp8(g, g, g, pages, torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.full((1,), 16, dtype=torch.int32, device=DEV), key_norm=FastRMSNorm(64, torch.ones(64, device=DEV), eps=0.0))
+    y = x[0].double()
+    want = y / y.square().mean(-1, keepdim=True).sqrt()
+    zero = torch.zeros(1, 1, 16, 64, dtype=torch.float64)
+    check_side("keys", on_host(pages.keys), on_host(pages.key_scales), zero, torch.zeros(1, 1, 1, dtype=torch.float64), want[None], np.zeros((1, 1), dtype=np.int32), [16], 16, 16)
 
 
 @pytest.mark.parametrize("new", [1, 5, 50])

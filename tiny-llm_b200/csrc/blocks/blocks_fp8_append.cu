@@ -153,24 +153,36 @@ __device__ __forceinline__ void ap_key(const ApRow<T> &row, const F8Append &a, c
 #pragma unroll
     for (int e = 0; e < 8; ++e) u[e] = {x[e], 0.f};
     if (a.k_norm) {
-        ApTwo s{0.f, 0.f};
+        ApTwo s;
+        float2 more = a.k_more;
+        // Squares of keys beyond 2^60 or of nothing but numbers (and a root of eps) below 2^-38 would leave fp32's range: such a row is brought nearer to 1 and summed again
+#pragma unroll 1
+        for (int again = 0;; ++again) {
+            s = {0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float q = __fmul_rn(x[e], x[e]);
-            const ApTwo t = ap_sum(s.h, q);
-            s = {t.h, s.l + t.l + fmaf(x[e], x[e], -q)};
-        }
+            for (int e = 0; e < 8; ++e) {
+                const float q = __fmul_rn(x[e], x[e]);
+                const ApTwo t = ap_sum(s.h, q);
+                s = {t.h, s.l + t.l + fmaf(x[e], x[e], -q)};
+            }
 #pragma unroll
-        for (int o = 1; o < LP; o <<= 1) {
-            const float oh = __shfl_xor_sync(0xffffffffu, s.h, o), ol = __shfl_xor_sync(0xffffffffu, s.l, o);
-            const ApTwo t = ap_sum(s.h, oh);
-            s = {t.h, s.l + ol + t.l};
+            for (int o = 1; o < LP; o <<= 1) {
+                const float oh = __shfl_xor_sync(0xffffffffu, s.h, o), ol = __shfl_xor_sync(0xffffffffu, s.l, o);
+                const ApTwo t = ap_sum(s.h, oh);
+                s = {t.h, s.l + ol + t.l};
+            }
+            const ApTwo all = ap_sum(s.h, more.x);
+            s = {all.h, all.l + s.l + more.y};
+            const bool large = !(all.h < 0x1p124f), small = all.h < 0x1p-76f;
+            if (again == 2 || !__any_sync(0xffffffffu, large || small)) break;
+            const float by = large ? 0x1p-70f : small ? 0x1p64f : 1.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= by;
+            more.x = more.x * by * by, more.y = more.y * by * by;
         }
-        const ApTwo all = ap_sum(s.h, a.k_more.x);
-        s = {all.h, all.l + s.l + a.k_more.y};
         // r0 = 1 / sqrt(s) to 2^-22 or so; 1 - s r0^2 makes it better by as many bits again
         const float r0 = rsqrtf(s.h);
-        const ApTwo sq = ap_times({r0, 0.f}, {r0, 0.f}), one = ap_times(sq, s);
+        const ApTwo one = ap_times(ap_times({r0, 0.f}, s), {r0, 0.f});
         const float left = (1.f - one.h) - one.l;
         const ApTwo r = ap_times({r0, 0.5f * r0 * left}, {a.root.x, a.root.y});
         if (at.on) {
@@ -487,10 +499,12 @@ int f8_check_pages(const char *op, const tlb_fp8_pages *p) {
     if (p->num_pages <= 0 || p->heads <= 0 || p->page_size <= 0 || p->page_size % kF8Tokens) return tl::fail(TL_EINVAL, "%s: pages of a multiple of %d slots", op, kF8Tokens);
     if (p->dim <= 0 || p->dim > kApMostDim || p->dim % 16) return tl::fail(TL_EINVAL, "%s: heads of a multiple of 16 entries, at most %d", op, kApMostDim);
     if (!tl::aligned16(p->keys) || !tl::aligned16(p->values)) return tl::fail(TL_EINVAL, "%s: pages must begin on 16 bytes", op);
+    if (static_cast<double>(p->num_pages) * p->heads * (p->page_size / kF8Tokens) > 2147483647.0) return tl::fail(TL_EINVAL, "%s: more than 2^31 blocks", op);  // a block's place is an int
     return TL_OK;
 }
 
 int f8_check_step(const char *op, const tlb_fp8_pages &p, const int32_t *lens, const int32_t *table, int batch, int max_pages, int tokens) {
+    if (static_cast<long long>(max_pages) * p.page_size > 1LL << 30) return tl::fail(TL_EINVAL, "%s: a block table for more than 2^30 tokens", op);  // positions are ints
     if (!lens && !table) return TL_OK;
     if (!lens || !table) return tl::fail(TL_EINVAL, "%s: lengths and block table on the host go together", op);
     std::vector<uint64_t> seen;  // a bit for every page

@@ -28,7 +28,8 @@ _INT32 = np.dtype(np.int32)
 class Fp8KvPages:
     """``keys`` and ``values`` (``torch.float8_e4m3fn``) ``[P, H_kv, page_size, D]``, ``key_scales`` and ``value_scales`` (fp32)
     ``[P, H_kv, page_size / 16]``; ``page_size`` and ``D`` are multiples of 16, ``D`` at most 256.  A number stands for itself times its block's
-    scale; where that is NaN (an infinity or a NaN was stored), every number of the block is."""
+    scale, a power of two; where that is NaN (an infinity or a NaN was stored), every number of the block is.  Numbers by themselves are finite: pages that
+    something else than ``rotate_append_fp8`` fills have to keep to that where a request's tokens are."""
 
     def __init__(self, keys: torch.Tensor, values: torch.Tensor, key_scales: torch.Tensor, value_scales: torch.Tensor):
         for name, t in (("keys", keys), ("values", values)):
