@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
     const int D = DIM ? DIM : pg.dim, G = a.group, L = a.tokens;
     const AtPiece mine = at_piece(a, blockIdx.x);
     if (mine.b < 0) return;
-    const int b = mine.b, cb = f8_div(mine.item, pg.heads, a.heads_magic), h = mine.item - cb * pg.heads, c0 = cb * COLS, ctx = at_context(a, b);
+    const int b = mine.b, cb = f8_div(mine.item, pg.heads, a.heads_magic), h = mine.item - cb * pg.heads, c0 = cb * COLS, ctx = mine.ctx;
     // keys [0, limit) are seen; a column behind the last one goes along with it, its query is 0 and nothing of it is stored
     auto limit_of = [&](int col) { return a.causal ? max(ctx - L + 1 + f8_div(min(col, G * L - 1), G, a.group_magic), 0) : ctx; };
     const int low = limit_of(c0), end = min(limit_of(c0 + COLS - 1), ctx);
@@ -449,15 +449,14 @@ __global__ void __launch_bounds__(kAtJoin) fp8_attend_join_kernel(const __grid_c
     const int b = f8_div(blockIdx.x, each, a.each_magic), item = static_cast<int>(blockIdx.x) - b * each, cb = f8_div(item, pg.heads, a.heads_magic), h = item - cb * pg.heads;
     const int c0 = cb * cols + skip;
     // the lengths are there: this launch begins once the one before it, which makes the pieces, is past its own wait
-    const AtCut cut = at_cut(a);
-    const int pieces = at_pieces(a, cut, b);
-    const long long before = at_before(a, cut, b);
+    int before;
+    const int pieces = at_pieces_of(a, b, before);
     tl::griddep_launch();
     tl::griddep_wait();  // also without work: what follows relies on this launch ending after the one before it
     const int live = min(min(cols - skip, kAtJoinColumns), G * L - c0);
     if (pieces <= 1 || live <= 0) return;
     const int size = cols * (D + 2), quads = live * (D / 4), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const float *ws = static_cast<const float *>(a.workspace) + static_cast<size_t>(before * each + static_cast<long long>(item) * pieces) * size;
+    const float *ws = static_cast<const float *>(a.workspace) + static_cast<size_t>(static_cast<long long>(before) * each + static_cast<long long>(item) * pieces) * size;
     const float *maxima = ws + static_cast<size_t>(cols) * D + skip, *parts = maxima + cols;
     // a column a warp: the maximum over the pieces, their factors
     for (int col = warp; col < live; col += kAtJoin / 32) {

@@ -5,6 +5,8 @@
 
 namespace tlb {
 
+constexpr int kAtLeast = 32;  // blocks of a piece at the least
+
 struct F8Attend : tlb_fp8_attention_call {
     tlb_fp8_pages pages;
     void *workspace;
@@ -12,20 +14,19 @@ struct F8Attend : tlb_fp8_attention_call {
     int slots;              // CTAs that the GPU holds at a time
     int most_pieces;        // of an item
     int granule;            // pieces are a multiple of so many blocks
-    int whole;              // blocks of a request that is not cut
+    int whole, least;       // blocks of a request that is not cut; of a piece at the least
     int page_blocks;        // blocks of 16 tokens in a page
     unsigned page_magic, group_magic, heads_magic, each_magic;  // for divisions by page_blocks, group, heads and the items of a request (f8_div)
     bool wide_rows;         // query rows may be read 16 bytes at a time
     float scale_log2, scale_rest;  // scale * log2(e), and what its rounding to fp32 left
     F8Attend(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c, void *ws)
-        : tlb_fp8_attention_call(c), pages(p), workspace(ws), group(c.heads / p.heads), col_blocks(0), slots(0), most_pieces(1), granule(1), whole(0), page_blocks(1), page_magic(0), group_magic(0), heads_magic(0), each_magic(0), wide_rows(false) {
+        : tlb_fp8_attention_call(c), pages(p), workspace(ws), group(c.heads / p.heads), col_blocks(0), slots(0), most_pieces(1), granule(1), whole(0), least(kAtLeast), page_blocks(1), page_magic(0), group_magic(0), heads_magic(0), each_magic(0), wide_rows(false) {
         const double log2 = c.scale * 1.4426950408889634;
         scale_log2 = static_cast<float>(log2), scale_rest = static_cast<float>(log2 - scale_log2);
     }
 };
 
 constexpr float kAtLag = 15.f;  // log2: how far a running maximum may lag behind: weights up to 2^15 are f16 numbers
-constexpr int kAtLeast = 32;    // blocks of a piece at the least
 
 __device__ __forceinline__ float at_ex2(float x) {
     float y;
@@ -53,18 +54,17 @@ __device__ __forceinline__ void at_query(const T *q, bool wide, float (&x)[8]) {
 __device__ __forceinline__ int at_context(const F8Attend &a, int b) {
     return static_cast<int>(max(0LL, min(static_cast<long long>(a.lens[b]), static_cast<long long>(a.max_pages) * a.pages.page_size)));
 }
-__device__ __forceinline__ int at_blocks(const F8Attend &a, int b) { return (at_context(a, b) + kF8Tokens - 1) / kF8Tokens; }
+__device__ __forceinline__ int at_blocks(int context) { return (context + kF8Tokens - 1) / kF8Tokens; }
 
 // How long a piece of an item may be, in blocks: such that the pieces are about as many as the CTAs that the GPU holds at a time, or the items and half of those.  A piece
-// costs its CTA some microseconds beside its blocks, so it has kAtLeast of them.  Nothing here depends on how many idle slots there are: a step over more of
-// them is cut the same way, to the bit.  Whole warps; 0: nothing is cut.
+// costs its CTA some microseconds beside its blocks, so it has a.least of them.  Nothing here depends on how many idle slots there are: a step over more of
+// them is cut the same way, to the bit.  Whole warps; `mine`: the blocks of request number lane; 0: nothing is cut.
 typedef int AtCut;
-__device__ __forceinline__ AtCut at_cut(const F8Attend &a) {
-    if (!a.workspace) return 0;
-    int live = 0, longest = 0;  // at most 2^26 blocks a request
-    long long all = 0;
-    for (int r = threadIdx.x & 31; r < a.batch; r += 32) {
-        const int n = at_blocks(a, r);
+__device__ __forceinline__ AtCut at_cut(const F8Attend &a, int mine) {
+    int live = mine > 0, longest = mine;  // at most 2^26 blocks a request
+    long long all = mine;
+    for (int r = (threadIdx.x & 31) + 32; r < a.batch; r += 32) {
+        const int n = at_blocks(at_context(a, r));
         all += n, live += n > 0, longest = max(longest, n);
     }
 #pragma unroll
@@ -74,39 +74,30 @@ __device__ __forceinline__ AtCut at_cut(const F8Attend &a) {
     }
     const int each = a.pages.heads * a.col_blocks, room = max(a.slots - live * each, a.slots / 2);
     if (longest <= a.whole) return 0;
-    const int mean = static_cast<int>(min((all * each + room - 1) / room, 0x3fffffffLL));
-    return max(max(mean, (longest + a.most_pieces - 1) / a.most_pieces), kAtLeast);
+    const long long shares = all * each + room - 1;
+    const int mean = shares <= 0x7fffffff ? static_cast<int>(shares) / room : static_cast<int>(min(shares / room, 0x3fffffffLL));  // (a division of 64 bits is long)
+    return max(max(mean, (longest + a.most_pieces - 1) / a.most_pieces), a.least);
 }
-__device__ __forceinline__ int at_pieces(const F8Attend &a, AtCut cut, int b) {
-    const int n = at_blocks(a, b);
-    return cut == 0 || n <= cut + cut / 4 ? 1 : (n + cut - 1) / cut;  // a quarter more is no reason to cut
-}
-// pieces of a head's eight (or sixteen) columns, over the requests before `request`
-__device__ __forceinline__ long long at_before(const F8Attend &a, AtCut cut, int request) {
-    int n = 0;
-    for (int r = threadIdx.x & 31; r < request; r += 32) n += at_pieces(a, cut, r);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    return n;
-}
+__device__ __forceinline__ int at_pieces(AtCut cut, int n) { return cut == 0 || n <= cut + cut / 4 ? 1 : (n + cut - 1) / cut; }  // a quarter more is no reason to cut
 
 // The index-th piece: a request's items one after another, an item's pieces side by side.
 struct AtPiece {
-    int b, item, piece, pieces, size;  // size: blocks of a piece; b < 0: there are not so many
+    int b, ctx, item, piece, pieces, size;  // size: blocks of a piece; b < 0: there are not so many
 };
 __device__ __forceinline__ AtPiece at_piece(const F8Attend &a, int index) {
     const int each = a.pages.heads * a.col_blocks, lane = threadIdx.x & 31;
-    const AtCut cut = at_cut(a);
-    AtPiece x{-1, 0, 0, 1, 0x3fffffff};
-    if (cut == 0) {
-        x.b = f8_div(index, each, a.each_magic), x.item = index - x.b * each;
-        if (x.b >= a.batch) x.b = -1;
+    const int want = f8_div(index, each, a.each_magic);  // rounded down: an item's pieces over all items of a request are a multiple of them
+    AtPiece x{-1, 0, 0, 0, 1, 0x3fffffff};
+    if (!a.workspace) {
+        if (want < a.batch) x.b = want, x.ctx = at_context(a, want);
+        x.item = index - want * each;
         return x;
     }
-    const int want = f8_div(index, each, a.each_magic);  // rounded down: an item's pieces over all items of a request are a multiple of them
-    int run = 0;
+    int ctx = lane < a.batch ? at_context(a, lane) : 0, run = 0;  // lengths are read once where there are no more than lanes
+    const AtCut cut = at_cut(a, at_blocks(ctx));
     for (int r0 = 0; r0 < a.batch; r0 += 32) {
-        const int mine = r0 + lane < a.batch ? at_pieces(a, cut, r0 + lane) : 0;
+        if (r0) ctx = r0 + lane < a.batch ? at_context(a, r0 + lane) : 0;
+        const int mine = r0 + lane < a.batch ? at_pieces(cut, at_blocks(ctx)) : 0;
         int upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -116,15 +107,33 @@ __device__ __forceinline__ AtPiece at_piece(const F8Attend &a, int index) {
         const unsigned past = __ballot_sync(0xffffffffu, want < run + upto);
         if (past) {
             const int src = __ffs(past) - 1;
-            x.b = r0 + src, x.pieces = __shfl_sync(0xffffffffu, mine, src);
-            const int at = index - (run + __shfl_sync(0xffffffffu, upto - mine, src)) * each;
-            x.item = at / x.pieces, x.piece = at % x.pieces;
-            if (x.pieces > 1) x.size = ((at_blocks(a, x.b) + x.pieces - 1) / x.pieces + a.granule - 1) / a.granule * a.granule;  // the last may come out empty
+            x.b = r0 + src, x.ctx = __shfl_sync(0xffffffffu, ctx, src), x.pieces = __shfl_sync(0xffffffffu, mine, src);
+            x.item = index - (run + __shfl_sync(0xffffffffu, upto - mine, src)) * each;
+            if (x.pieces > 1) {
+                x.piece = x.item % x.pieces, x.item /= x.pieces;
+                x.size = ((at_blocks(x.ctx) + x.pieces - 1) / x.pieces + a.granule - 1) / a.granule * a.granule;  // the last may come out empty
+            }
             return x;
         }
         run += __shfl_sync(0xffffffffu, upto, 31);
     }
     return x;
+}
+// The pieces of a request's items, and those of the requests before it, of one item each.
+__device__ __forceinline__ int at_pieces_of(const F8Attend &a, int request, int &before) {
+    const int lane = threadIdx.x & 31;
+    int ctx = lane < a.batch ? at_context(a, lane) : 0, n = 0, of = 0;
+    const AtCut cut = at_cut(a, at_blocks(ctx));
+    for (int r0 = 0; r0 <= request; r0 += 32) {
+        if (r0) ctx = r0 + lane < a.batch ? at_context(a, r0 + lane) : 0;
+        const int mine = at_pieces(cut, at_blocks(ctx));
+        if (r0 + lane < request) n += mine;
+        if (r0 + lane == request) of = mine;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    before = n;
+    return __shfl_sync(0xffffffffu, of, request & 31);
 }
 
 // blocks_fp8_attention.cu: adds up the pieces of the launch in front, items of `cols` columns each.
@@ -133,7 +142,7 @@ __host__ __device__ static inline size_t at_piece_floats(int cols, int dim) { re
 // blocks_fp8_portion.cu: bf16 queries of many columns
 constexpr int kPoRows = 256;  // columns of a CTA
 bool f8_portion_takes(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c);
-constexpr int kPoWhole = 40;     // blocks of a request that is not cut
+constexpr int kPoWhole = 40, kPoLeast = 24;  // blocks of a request that is not cut, of a piece at the least
 int f8_portion(F8Attend a, cudaStream_t st);
 
 }  // namespace tlb
