@@ -67,11 +67,8 @@ __device__ __forceinline__ AtCut at_cut(const F8Attend &a, int mine) {
         const int n = at_blocks(at_context(a, r));
         all += n, live += n > 0, longest = max(longest, n);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        all += __shfl_xor_sync(0xffffffffu, all, o), live += __shfl_xor_sync(0xffffffffu, live, o);
-        longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
-    }
+    live = __reduce_add_sync(0xffffffffu, live), longest = __reduce_max_sync(0xffffffffu, longest);
+    all = (static_cast<long long>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(all >> 16))) << 16) + __reduce_add_sync(0xffffffffu, static_cast<unsigned>(all & 0xffff));
     const int each = a.pages.heads * a.col_blocks, room = max(a.slots - live * each, a.slots / 2);
     if (longest <= a.whole) return 0;
     const long long shares = all * each + room - 1;
@@ -130,9 +127,7 @@ __device__ __forceinline__ int at_pieces_of(const F8Attend &a, int request, int 
         if (r0 + lane < request) n += mine;
         if (r0 + lane == request) of = mine;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    before = n;
+    before = __reduce_add_sync(0xffffffffu, n);
     return __shfl_sync(0xffffffffu, of, request & 31);
 }
 
