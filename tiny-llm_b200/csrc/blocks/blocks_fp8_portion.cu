@@ -24,6 +24,7 @@ using tl::g_tmem_st_wait;
 
 constexpr int kPoKeys = 64;
 constexpr int kPoSet = 128;  // rows of a set
+constexpr int kPoStages = 2;  // of operand tiles, a power of two; four take as long
 // Registers are moved between groups of four warps (128, 128, 72, 72, 32 and 48 are six times the launch's 80); warps 18 and 19 have nothing to do.
 constexpr int kPoThreads = 24 * 32;
 constexpr int kPoColumns = 512;      // of tensor memory; a set's half: two score buffers of 64, the output from 128 on
@@ -32,9 +33,6 @@ constexpr uint32_t kPoHalf = 256, kPoOut = 128;
 // Asynchronous copies; zeros where `there` is false.
 __device__ __forceinline__ void po_copy16(uint32_t to, const void *from, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void po_copy4(uint32_t to, const void *from, bool there) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
 }
 __device__ __forceinline__ float po_max3(float a, float b, float c) {
     float r;
@@ -90,10 +88,10 @@ template <int DIM>
 struct PoShape {
     static constexpr int halves = DIM / 64;                                // 64-column blocks
     static constexpr int q_block = kPoSet * 128, kv_block = kPoKeys * 128;  // bytes
-    static constexpr int k_off = 2 * halves * q_block, v_off = k_off + 2 * halves * kv_block, bar_off = v_off + 2 * halves * kv_block;
-    // behind the row factors and two tiles' factors of the rescaled rows: the bytes of two tiles of either side
-    static constexpr int row_off = bar_off + 512, raw_off = row_off + 3 * kPoRows * 4, raw_tile = kPoKeys * DIM, smem = raw_off + 4 * raw_tile;
-    static_assert(4 * halves * kv_block >= kPoRows * DIM * 2, "the queries as they come fit where the operand tiles will be");
+    static constexpr int k_off = 2 * halves * q_block, v_off = k_off + kPoStages * halves * kv_block, bar_off = v_off + kPoStages * halves * kv_block;
+    // the row factors and two tiles' factors of the rescaled rows
+    static constexpr int row_off = bar_off + 512, smem = row_off + 3 * kPoRows * 4;
+    static_assert(2 * kPoStages * halves * kv_block >= kPoRows * DIM * 2, "the queries as they come fit where the operand tiles will be");
 };
 
 // 16 e4m3 numbers times `ratio` (two alike), as f16, to the two places of a row.
@@ -140,14 +138,14 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
     };
 
     const uint32_t base = g_smem_u32(psm), k_at = base + Z::k_off, v_at = base + Z::v_off, bar = base + Z::bar_off;
-    const uint32_t s_full = bar, p_full = bar + 32, pv_done = bar + 64, k_full = bar + 96, k_empty = bar + 112, v_full = bar + 128, v_empty = bar + 144, told = bar + 256;  // two of each, of the first three for either set, of the last for each softmax warp
-    volatile int *dead = reinterpret_cast<volatile int *>(psm + Z::bar_off + 160);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(psm + Z::bar_off + 164);
-    int *seen = reinterpret_cast<int *>(psm + Z::bar_off + 168);  // largest scales of the CTA's blocks, keys' and values' (bits of positive numbers); whether a scale or page is none
+    const uint32_t s_full = bar, p_full = bar + 32, pv_done = bar + 64, k_full = bar + 96, k_empty = bar + 128, v_full = bar + 160, v_empty = bar + 192, told = bar + 256;  // two of each, of the first three for either set, of the last for each softmax warp
+    volatile int *dead = reinterpret_cast<volatile int *>(psm + Z::bar_off + 224);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(psm + Z::bar_off + 228);
+    int *seen = reinterpret_cast<int *>(psm + Z::bar_off + 232);  // largest scales of the CTA's blocks, keys' and values' (bits of positive numbers); whether a scale or page is none
     float *row_factor = reinterpret_cast<float *>(psm + Z::row_off), *shrink = row_factor + kPoRows;  // [2][kPoRows]
     if (threadIdx.x == 0) {
         for (int i = 0; i < 4; ++i) g_mbar_init(s_full + 8 * i, 1), g_mbar_init(p_full + 8 * i, 8), g_mbar_init(pv_done + 8 * i, 1);
-        for (int i = 0; i < 2; ++i) g_mbar_init(k_full + 8 * i, 4), g_mbar_init(k_empty + 8 * i, 2), g_mbar_init(v_full + 8 * i, 4), g_mbar_init(v_empty + 8 * i, 2);
+        for (int i = 0; i < kPoStages; ++i) g_mbar_init(k_full + 8 * i, 4), g_mbar_init(k_empty + 8 * i, 2), g_mbar_init(v_full + 8 * i, 4), g_mbar_init(v_empty + 8 * i, 2);
         for (int i = 0; i < 16; ++i) g_mbar_init(told + 8 * i, 1);
         *dead = 0, seen[0] = 0, seen[1] = 0, seen[2] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -162,28 +160,27 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
     // its own pieces, so they wait for nobody.  Lane j knows where block j of the tile that is asked for next lies, and the scales of those that were.
     const bool values = warp >= 12;
     const int tid = threadIdx.x & 127;
-    const uint32_t raw_at = base + Z::raw_off + (values ? 2 * Z::raw_tile : 0) + 16 * tid;
     const uint8_t *numbers = (values ? pg.values : pg.keys) + 16 * tid;
     const float *scales = values ? pg.value_scales : pg.key_scales;
     int place = -1;  // of a block among all pages' (fewer than 2^31: they are 16 rows each); -1: none
-    float scale_next = 0.f, scale_after = 0.f;
+    float scale_next = 0.f;
+    uint4 raw[PER];  // the next tile's
     auto look_up = [&](int t) {
         const int blk = begin + t * (kPoKeys / kF8Tokens) + lane, at = page_at(blk);
         const int page = lane < kPoKeys / kF8Tokens && blk < stop ? table[at] : -1;
         place = static_cast<unsigned>(page) < static_cast<unsigned>(pg.num_pages) ? (page * pg.heads + h) * a.page_blocks + blk - at * a.page_blocks : -1;
     };
     auto ask = [&](int t) {  // of a page that is none: zeros
-        scale_next = scale_after, scale_after = place < 0 ? 0.f : __ldg(scales + place);
+        scale_next = place < 0 ? 0.f : __ldg(scales + place);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int at = __shfl_sync(0xffffffffu, place, (tid + 128 * i) / (kF8Tokens * CH));
             const size_t byte = static_cast<size_t>(static_cast<unsigned>(max(at, 0))) * (kF8Tokens * DIM);
             // the pieces before this thread's i-th that are not of its block
-            po_copy16(raw_at + (t & 1) * Z::raw_tile + 2048 * i, numbers + byte + (DIM == 128 ? 0 : -(tid / 64) * 1024), at >= 0);
+            raw[i] = at >= 0 ? __ldg(reinterpret_cast<const uint4 *>(numbers + byte + (DIM == 128 ? 0 : -(tid / 64) * 1024))) : make_uint4(0, 0, 0, 0);
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    if (warp >= 8 && warp < 16) look_up(0), ask(0), look_up(1), ask(1), look_up(2);
+    if (warp >= 8 && warp < 16) look_up(0), ask(0), look_up(1);
     // queries: 8 entries a lane, a row to 8 or 16 lanes of the first sixteen warps; first as they are, to where the operand tiles will be
     constexpr int LANES = DIM / 8, ROWS = 32 / LANES, N = kPoRows / (16 * ROWS);
     unsigned char *mine_q = psm + Z::k_off + threadIdx.x * 16;
@@ -276,31 +273,31 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
         const uint32_t scores_at = tmem + set * kPoHalf, out_at = scores_at + kPoOut;
         const uint64_t qd = g_smem_desc_sw128(base + set * Z::halves * Z::q_block, 0, 1024), kd0 = g_smem_desc_sw128(k_at, 0, 1024), vd0 = g_smem_desc_sw128(v_at, Z::kv_block, 1024);
         auto scores = [&](int t) {
-            const int s = t & 1;
-            if (!tc_wait(k_full + 8 * s, t >> 1 & 1, dead)) return false;
+            const int s = t & 1, k = t & (kPoStages - 1);
+            if (!tc_wait(k_full + 8 * k, t / kPoStages & 1, dead)) return false;
             g_tc_fence_after();
             if (g_elect_one()) {
-                const uint64_t kd = kd0 + static_cast<uint64_t>(s * Z::halves * (Z::kv_block >> 4));
+                const uint64_t kd = kd0 + static_cast<uint64_t>(k * Z::halves * (Z::kv_block >> 4));
 #pragma unroll
-                for (int k = 0; k < DIM / 16; ++k)
-                    g_tc_mma(scores_at + s * kPoKeys, qd + (k >> 2) * (Z::q_block >> 4) + 2 * (k & 3), kd + (k >> 2) * (Z::kv_block >> 4) + 2 * (k & 3), idesc_s, k > 0);
+                for (int i = 0; i < DIM / 16; ++i)
+                    g_tc_mma(scores_at + s * kPoKeys, qd + (i >> 2) * (Z::q_block >> 4) + 2 * (i & 3), kd + (i >> 2) * (Z::kv_block >> 4) + 2 * (i & 3), idesc_s, i > 0);
                 g_tc_commit(s_full + 16 * set + 8 * s);
-                g_tc_commit(k_empty + 8 * s);
+                g_tc_commit(k_empty + 8 * k);
             }
             __syncwarp();
             return true;
         };
         const bool begun = warp < 18 && n_tiles > 0 && scores(0);
         for (int t = 0; begun && t < n_tiles; ++t) {
-            const int s = t & 1;
+            const int s = t & 1, v = t & (kPoStages - 1);
             if (t + 1 < n_tiles && !scores(t + 1)) break;  // its buffer held P_(t-1), read by a product already queued ahead of this one
-            if (!tc_wait(v_full + 8 * s, t >> 1 & 1, dead) || !tc_wait(p_full + 16 * set + 8 * s, t >> 1 & 1, dead)) break;
+            if (!tc_wait(v_full + 8 * v, t / kPoStages & 1, dead) || !tc_wait(p_full + 16 * set + 8 * s, t >> 1 & 1, dead)) break;
             g_tc_fence_after();
             if (g_elect_one()) {
-                const uint64_t vd = vd0 + static_cast<uint64_t>(s * Z::halves * (Z::kv_block >> 4));
+                const uint64_t vd = vd0 + static_cast<uint64_t>(v * Z::halves * (Z::kv_block >> 4));
 #pragma unroll
                 for (int k = 0; k < kPoKeys / 16; ++k) g_tc_mma_ts(out_at, scores_at + s * kPoKeys + 8 * k, vd + k * (2048 >> 4), idesc_o, t > 0 || k > 0);
-                g_tc_commit(v_empty + 8 * s);
+                g_tc_commit(v_empty + 8 * v);
                 g_tc_commit(pv_done + 16 * set + 8 * s);
             }
             __syncwarp();
@@ -316,14 +313,13 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
         unsigned char *at = tiles + (c >> 2) * Z::kv_block + row0 * 128;
         unsigned char *one = at + (((2 * (c & 3) + odd) ^ (row0 & 7)) << 4), *two = at + (((2 * (c & 3) + 1 - odd) ^ (row0 & 7)) << 4);
         for (int t = 0; t < n_tiles; ++t) {
-            const int s = t & 1, key0 = first + t * kPoKeys;
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            const int s = t & (kPoStages - 1), key0 = first + t * kPoKeys;
             const __half2 r2 = __float2half2_rn(scale_next < INFINITY ? scale_next * under : 0.f);
             const uint32_t ratio = *reinterpret_cast<const uint32_t *>(&r2);
-            if (!tc_wait(empty + 8 * s, (t >> 1 & 1) ^ 1u, dead)) break;  // the first pass through the stages does not wait
+            if (!tc_wait(empty + 8 * s, (t / kPoStages & 1) ^ 1u, dead)) break;  // the first pass through the stages does not wait
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
-                uint4 x = *reinterpret_cast<const uint4 *>(psm + (raw_at - base) + s * Z::raw_tile + 2048 * i);
+                uint4 x = raw[i];
                 if (key0 + kPoKeys > ctx && key0 + row0 + 128 / CH * i >= ctx) x = make_uint4(0, 0, 0, 0);  // slots behind the last token may hold anything
                 if (odd) x = make_uint4(x.z, x.w, x.x, x.y);
                 const int by = s * Z::halves * Z::kv_block + 128 / CH * 128 * i;
@@ -332,9 +328,8 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
             g_fence_proxy_async();
             __syncwarp();
             if (lane == 0) g_mbar_arrive(full + 8 * s);
-            ask(t + 2), look_up(t + 3);
+            ask(t + 1), look_up(t + 2);
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
     } else {  // ---- softmax: thread = row
         asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
         const int r = threadIdx.x, col = c0 + r, set = warp >> 2;
