@@ -1210,7 +1210,7 @@ def _fp8_step(op: str, pages: Fp8Pages, device: int, table: torch.Tensor, lens: 
 
 def fp8_devices(op: str, device: int, *tensors) -> None:
     for t in tensors:
-        if t.get_device() != device or device < 0:
+        if t.get_device() != device or device < 0:  # (-1: the host)
             raise RuntimeError(f"{op}: the blocks extension is GPU-only, and a step and the pages must be on one device")
 
 
@@ -1225,23 +1225,30 @@ def fp8_append(pages: Fp8Pages, device: int, q: torch.Tensor, k: torch.Tensor, v
     return fp8_append_of(pages, device, q, k, v, table, lens, q_norm, q_eps, k_norm, k_eps, rot, base, interleaved)
 
 
-def _token_by_token(like: torch.Tensor, B: int, H: int, L: int, D: int) -> torch.Tensor:
-    """Room for ``[B, H, L, D]``, a token's heads side by side."""
-    return torch.empty_strided((B, H, L, D), (L * H * D, D, H * D, 1), dtype=like.dtype, device=like.device)
+def _token_by_token(x: torch.Tensor) -> tuple:
+    """``x`` [B, H, L, D] with its entries side by side -> it, its shape and strides, and room for the same shape with a token's heads side by side."""
+    strides = x.stride()
+    if strides[3] != 1:
+        x = x.contiguous()
+        strides = x.stride()
+    B, H, L, D = shape = x.shape
+    laid = (L * H * D, D, H * D, 1)
+    return x, shape, strides, torch.empty_like(x) if strides == laid else torch.empty_strided(shape, laid, dtype=x.dtype, device=x.device)
 
 
 def fp8_append_of(pages: Fp8Pages, device: int, q, k, v, table, lens, q_norm=None, q_eps=0.0, k_norm=None, k_eps=0.0, rot=0, base=1.0, interleaved=False, lens_host=None,
                   table_host=None):
-    """``fp8_append`` of tensors that the caller has checked (``rotate_append_fp8``).  ``lens_host``, ``table_host``: the lengths' and the table's bytes (int32) or addresses; the
+    """``fp8_append`` of tensors that the caller has checked (``rotate_append_fp8``), any strides.  ``lens_host``, ``table_host``: the lengths' and the table's bytes (int32) or addresses; the
     answer is None where the library refuses them."""
     if _current_device() != device:
         with torch.cuda.device(device):
             return fp8_append_of(pages, device, q, k, v, table, lens, q_norm, q_eps, k_norm, k_eps, rot, base, interleaved, lens_host, table_host)
-    B, H, L, D = q.shape
-    out = _token_by_token(q, B, H, L, D)
-    qb, qh, ql, _ = q.stride()
-    kb, kh, kl, _ = k.stride()
-    vb, vh, vl, _ = v.stride()
+    q, (B, H, L, _), (qb, qh, ql, _), out = _token_by_token(q)
+    kb, kh, kl, ke = k.stride()
+    vb, vh, vl, ve = v.stride()
+    if ke != 1 or ve != 1:
+        k, v = k.contiguous(), v.contiguous()
+        (kb, kh, kl, _), (vb, vh, vl, _) = k.stride(), v.stride()
     call = _FP8_APPEND.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(), 0 if q_norm is None else q_norm.data_ptr(),
                             0 if k_norm is None else k_norm.data_ptr(), qb, qh, ql, kb, kh, kl, vb, vh, vl, base, q_eps, k_eps, B, H, L, table.shape[1], rot, interleaved,
                             _DTYPE_CODE[q.dtype])
@@ -1261,14 +1268,12 @@ def fp8_attention(pages: Fp8Pages, device: int, q: torch.Tensor, table: torch.Te
 
 
 def fp8_attention_of(pages: Fp8Pages, device: int, q, table, lens, scale, causal, lens_host=None, table_host=None):
-    """``fp8_attention`` of tensors that the caller has checked (``paged_attention_fp8``).  ``lens_host``, ``table_host``: the lengths' and the table's bytes (int32) or addresses,
+    """``fp8_attention`` of tensors that the caller has checked (``paged_attention_fp8``), any strides.  ``lens_host``, ``table_host``: the lengths' and the table's bytes (int32) or addresses,
     if the call is for these alone; the answer is None where the library refuses them."""
     if _current_device() != device:
         with torch.cuda.device(device):
             return fp8_attention_of(pages, device, q, table, lens, scale, causal, lens_host, table_host)
-    B, H, L, D = q.shape
-    out = _token_by_token(q, B, H, L, D)
-    qb, qh, ql, _ = q.stride()
+    q, (B, H, L, _), (qb, qh, ql, _), out = _token_by_token(q)
     call = _FP8_ATTENTION.pack(q.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(), qb, qh, ql, scale, B, H, L, table.shape[1], causal, _DTYPE_CODE[q.dtype])
     lib, at, stream = library(), ctypes.addressof(pages), _raw_stream(device)
     rc = _EWORKSPACE if lens_host is None else lib.tlb_fp8_attention(at, call, lens_host, table_host, None, 0, stream)

@@ -78,7 +78,7 @@ class Fp8KvPages:
 
 
 def _step(op: str, pages: Fp8KvPages, query: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor, block_table_host, context_lens_host):
-    """Checks of a step's shapes and metadata -> (block table, context lengths, the host's lengths and table as bytes, and as arrays)."""
+    """Checks of a step's shapes and metadata -> (the query's shape, block table, context lengths, the host's lengths and table as bytes, and as arrays)."""
     shape, rows = query.shape, block_table.shape
     if len(shape) != 4:
         raise ValueError(f"{op}: query must be 4D [B, H_q, L, D]")
@@ -108,7 +108,7 @@ def _step(op: str, pages: Fp8KvPages, query: torch.Tensor, block_table: torch.Te
         lens, table = lens.astype(_INT32), table.astype(_INT32)
     # a copy of a few kilobytes costs less than numpy's .ctypes
     bytes_of = table.tobytes() if table.nbytes <= 8192 or not table.flags.c_contiguous else table.ctypes.data
-    return (block_table if block_table.is_contiguous() else block_table.contiguous(), context_lens if context_lens.is_contiguous() else context_lens.contiguous(), lens.tobytes(),
+    return (shape, block_table if block_table.is_contiguous() else block_table.contiguous(), context_lens if context_lens.is_contiguous() else context_lens.contiguous(), lens.tobytes(),
             bytes_of, (lens, table))
 
 
@@ -118,10 +118,6 @@ def _refused(op: str, pages: Fp8KvPages, hosts: tuple, L: int) -> None:
     raise RuntimeError(blocks.library().tlb_last_error().decode() or op)
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    return x if x.stride(3) == 1 else x.contiguous()
-
-
 def rotate_append_fp8(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, pages: Fp8KvPages, block_table: torch.Tensor, context_lens: torch.Tensor, *, rope=None,
                       query_norm=None, key_norm=None, block_table_host: np.ndarray | None = None, context_lens_host: np.ndarray | None = None) -> torch.Tensor:
     """Append a step's ``key`` and ``value [B, H_kv, L, D]`` to the pages at positions ``context_lens - L ..``; -> the queries ``[B, H_q, L, D]`` to attend with.
@@ -129,11 +125,13 @@ def rotate_append_fp8(query: torch.Tensor, key: torch.Tensor, value: torch.Tenso
     ``query_norm`` and ``key_norm`` (``FastRMSNorm``) and ``rope`` (``FastRoPE``, turned by a token's position) are applied on the way, the keys' in 64 bits
     ahead of their one rounding.  Any strides will do; float32 or bfloat16.  A block of 16 tokens of a head has one scale: it grows where the new
     tokens need it to, and the block's earlier numbers are rounded to it again."""
-    table, lens, lens_host, table_host, hosts = _step("rotate_append_fp8", pages, query, block_table, context_lens, block_table_host, context_lens_host)
-    B, _, L, D = query.shape
-    if key.shape != (B, pages.kv_heads, L, D) or key.shape != value.shape:
+    shape, table, lens, lens_host, table_host, hosts = _step("rotate_append_fp8", pages, query, block_table, context_lens, block_table_host, context_lens_host)
+    B, _, L, D = shape
+    theirs = key.shape
+    if theirs != (B, pages.kv_heads, L, D) or theirs != value.shape:
         raise ValueError("rotate_append_fp8: key and value must be [B, H_kv, L, D] beside the query")
-    if key.dtype != query.dtype or value.dtype != query.dtype:
+    dtype = query.dtype
+    if key.dtype != dtype or value.dtype != dtype:
         raise ValueError("rotate_append_fp8: query, key, and value must have the same dtype")
     blocks.fp8_devices("rotate_append_fp8", pages.index, query, key, value, table, lens)
     rot, base, interleaved = 0, 1.0, False
@@ -147,12 +145,12 @@ def rotate_append_fp8(query: torch.Tensor, key: torch.Tensor, value: torch.Tenso
             weights += (None, 0.0)
             continue
         weight = norm.weight
-        if weight.dtype != query.dtype or weight.get_device() != pages.index or not weight.is_contiguous():
-            weight = norm._weight_as(query.dtype, query.device)
+        if weight.dtype != dtype or weight.get_device() != pages.index or not weight.is_contiguous():
+            weight = norm._weight_as(dtype, query.device)
         if weight.shape != (D,):
             raise ValueError(f"rotate_append_fp8: a norm of {tuple(weight.shape)} for heads of {D}")
         weights += (weight, norm.eps)
-    out = blocks.fp8_append_of(pages.native, pages.index, _rows(query), _rows(key), _rows(value), table, lens, *weights, rot, base, interleaved, lens_host, table_host)
+    out = blocks.fp8_append_of(pages.native, pages.index, query, key, value, table, lens, *weights, rot, base, interleaved, lens_host, table_host)
     if out is None:
         _refused("rotate_append_fp8", pages, hosts, L)
     return out
@@ -164,15 +162,15 @@ def paged_attention_fp8(query: torch.Tensor, pages: Fp8KvPages, block_table: tor
     ``mask``: None or ``"causal"``; ``scale``: ``D ** -0.5`` by default.  Rows of idle slots come out as zeros."""
     if isinstance(mask, torch.Tensor) or mask not in (None, "causal"):
         raise NotImplementedError("Paged attention only supports mask=None or causal")
-    table, lens, lens_host, table_host, hosts = _step("paged_attention_fp8", pages, query, block_table, context_lens, block_table_host, context_lens_host)
-    factor = query.shape[-1] ** -0.5 if scale is None else float(scale)
+    shape, table, lens, lens_host, table_host, hosts = _step("paged_attention_fp8", pages, query, block_table, context_lens, block_table_host, context_lens_host)
+    factor = shape[3] ** -0.5 if scale is None else float(scale)
     blocks.fp8_devices("paged_attention_fp8", pages.index, query, table, lens)
     if torch.cuda.is_current_stream_capturing():  # a captured call is replayed for other lengths
-        validate_paged_metadata(*hosts, pages.page_size, pages.num_pages, query.shape[2])
+        validate_paged_metadata(*hosts, pages.page_size, pages.num_pages, shape[2])
         lens_host = table_host = None
-    out = blocks.fp8_attention_of(pages.native, pages.index, _rows(query), table, lens, factor, mask == "causal", lens_host, table_host)
+    out = blocks.fp8_attention_of(pages.native, pages.index, query, table, lens, factor, mask == "causal", lens_host, table_host)
     if out is None:
-        _refused("paged_attention_fp8", pages, hosts, query.shape[2])
+        _refused("paged_attention_fp8", pages, hosts, shape[2])
     return out
 
 
