@@ -201,3 +201,11 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     assert all(torch.equal(a, want[i]) for i in range(2) for a in got[i])
     assert blocks.library().tlb_tc_gave_up() == 0
+
+
+@pytest.mark.parametrize("batch,kv_heads", [(1, 1), (1, 8), (2, 8), (3, 8), (5, 8), (9, 8), (20, 8)])
+@pytest.mark.parametrize("group,dim,dtype", [(4, 128, torch.bfloat16), (12, 64, torch.bfloat16), (2, 256, torch.bfloat16), (10, 80, torch.float32), (1, 256, torch.float32)])
+def test_few_and_more_items(batch, kv_heads, group, dim, dtype):
+    """Items that clusters of 8, 7 .. 2 CTAs share, and too many for that; lengths of less than a block a CTA, idle slots, and long ones beside them."""
+    lengths = [(700, 0, 33, 16, 210, 5, 129, 1, 64, 300)[i % 10] for i in range(batch)]
+    run_attention(lengths, 1, kv_heads * group, kv_heads, dim, 32, dtype, seed=batch + dim)

@@ -12,9 +12,11 @@
 // k-index means is free as long as queries agree, and the values' bytes of two keys are interleaved by byte permutation.  The warps of a CTA share its keys and are
 // joined in a fixed order.
 //
-// An item is 8 (or 16) columns of one request and key/value head.  A CTA takes an item, or, where the requests are few or of unlike length, a piece of one; an item in several
-// pieces leaves a partial result for each, which fp8_attend_join_kernel adds up in order.  The cut follows the lengths on the device, so a captured launch does.
+// An item is 8 (or 16) columns of one request and key/value head.  A CTA takes an item; or, where items are few, a cluster does, whose CTAs read each other's sums; or, where
+// requests are of unlike length or very long, a CTA takes a piece of one, which leaves a partial result for fp8_attend_join_kernel to add up in order.  Both follow the lengths
+// on the device, so a captured launch does.  attend_plan chooses.
 #include <algorithm>
+#include <atomic>
 
 #include "../per_device.h"
 #include "blocks_fp8_cache.cuh"
@@ -59,6 +61,22 @@ __device__ __forceinline__ int at_value(int row, int D, int byte) {
     return row * D + (MOVED ? byte ^ (((row >> 1) & 3) << 5) : byte);
 }
 
+// Of a cluster's CTAs: a barrier, and numbers in the shared memory of the r-th.
+__device__ __forceinline__ void at_cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float at_theirs(uint32_t at, int r) {
+    float v;
+    asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %1, %2;\n\tld.shared::cluster.f32 %0, [ra];\n\t}" : "=f"(v) : "r"(at), "r"(r) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 at_theirs4(uint32_t at, int r) {
+    float4 v;
+    asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [ra];\n\t}"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(at), "r"(r)
+                 : "memory");
+    return v;
+}
+
 // DIM: entries of a head, 0: as the pages say.  place: of the block among all pages'.
 template <int DIM>
 __device__ __forceinline__ void at_issue(uint32_t stage, const tlb_fp8_pages &pg, int place, int lane) {
@@ -100,8 +118,12 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const tlb_fp8_pages &pg = a.pages;
     const int D = DIM ? DIM : pg.dim, G = a.group, L = a.tokens;
-    const AtPiece mine = at_piece(a, blockIdx.x);
-    if (mine.b < 0) return;
+    int item, rank;  // of a launch without clusters: the CTA's number and 0
+    asm("mov.u32 %0, %%clusterid.x;" : "=r"(item));
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    AtPiece mine = at_piece(a, item);
+    if (mine.b < 0) return;  // a whole cluster
+    if (a.ranks > 1) mine.piece = rank, mine.size = (at_blocks(mine.ctx) + a.ranks - 1) / a.ranks;
     const int b = mine.b, cb = f8_div(mine.item, pg.heads, a.heads_magic), h = mine.item - cb * pg.heads, c0 = cb * COLS, ctx = mine.ctx;
     // keys [0, limit) are seen; a column behind the last one goes along with it, its query is 0 and nothing of it is stored
     auto limit_of = [&](int col) { return a.causal ? max(ctx - L + 1 + f8_div(min(col, G * L - 1), G, a.group_magic), 0) : ctx; };
@@ -422,7 +444,30 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
         reinterpret_cast<float4 *>(part + col * ROW)[i % (DP / 4)] = v;
     }
     __syncthreads();
-    if (mine.pieces > 1) {
+    if (a.ranks > 1) {
+        // the CTAs of a cluster have a share of the item's blocks each; each adds up a share of its numbers, in the order of the ranks
+        at_cluster_sync();
+        const uint32_t all = static_cast<uint32_t>(__cvta_generic_to_shared(part)), all_m = all + WARPS * COLS * ROW * 4, all_l = all_m + WARPS * COLS * 4;
+        for (int i = threadIdx.x * a.ranks + rank; i < live * (D / 4); i += WARPS * 32 * a.ranks) {
+            const int col = i / (D / 4), d = i % (D / 4);
+            float m = -INFINITY, l = 0.f;
+#pragma unroll 8
+            for (int r = 0; r < a.ranks; ++r) m = fmaxf(m, at_theirs(all_m + 4 * col, r));
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+            for (int r = 0; r < a.ranks; ++r) {
+                const float most = at_theirs(all_m + 4 * col, r), f = most == m ? 1.f : at_ex2(most - m);
+                const float4 u = at_theirs4(all + (col * ROW + 4 * d) * 4, r);
+                l = fmaf(at_theirs(all_l + 4 * col, r), f, l);
+                v.x = fmaf(u.x, f, v.x), v.y = fmaf(u.y, f, v.y), v.z = fmaf(u.z, f, v.z), v.w = fmaf(u.w, f, v.w);
+            }
+            const int c = c0 + col, at = f8_div(c, G, a.group_magic);
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            store4(static_cast<T *>(a.out) + ((static_cast<size_t>(b) * L + at) * a.heads + static_cast<size_t>(h) * G + c - at * G) * D + 4 * d,
+                   make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+        }
+        at_cluster_sync();  // nobody's memory is read any more
+    } else if (mine.pieces > 1) {
         float *to = static_cast<float *>(a.workspace) + static_cast<size_t>(blockIdx.x) * (COLS * (D + 2));
         for (int i = threadIdx.x; i < live * (D / 4); i += WARPS * 32)
             reinterpret_cast<float4 *>(to)[i] = reinterpret_cast<const float4 *>(part + i / (D / 4) * ROW)[i % (D / 4)];
@@ -520,13 +565,68 @@ int f8_attend_join(const F8Attend &a, int cols, cudaStream_t st) {
 // CTAs of the kernels that the GPU holds at a time, as far as the division of the work goes: two an SM, one of the wider forms.
 static int attend_slots(int dtype, int dim, int rows) { return sm_count() * (dtype == TL_BF16 && dim <= 128 && rows <= 8 ? 2 : 1); }
 static int attend_cols(int dim, int rows) { return dim > 128 || rows <= 8 ? 8 : 16; }
-constexpr int kAtWhole = 64;  // blocks of a request that is not cut
-// Whether a launch without pieces takes no longer than one with them and the launch that joins them, which is 6.5 us more: an item's CTA takes so long for a block by itself, all of
-// them together so long as their bytes take.  (bf16, 8 columns, heads of 128: 0.075 us a block, 6.2 TB/s.  One request of 1011 tokens 8.9 us whole and 10.7 cut, of 2000 13.4
-// and 10.8; 24 of 70 to 1970 17.9 and 19.2; 16 of 8000 45 and 53; 64 of 8192 157 and 162.)
-static bool attend_whole(int dtype, int dim, int cols, long long longest, double blocks) {
-    const double block = (dtype == TL_BF16 ? 0.075 : 0.18) * (cols == 16 ? 1.3 : 1.0);
-    return longest <= kAtWhole || longest * block <= 6.5 + blocks * (2 * kF8Tokens * dim / 6.2e6);
+constexpr int kAtWhole = 64;  // blocks of a request that is not cut into pieces
+constexpr int kAtAlone = 120 * 1024;  // of shared memory: a CTA has its SM to itself
+static cudaLaunchConfig_t at_clusters(unsigned ctas, int ranks, int smem, cudaStream_t st, cudaLaunchAttribute (&attr)[2]) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(kAtWarps * 32), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ranks, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr, cfg.numAttrs = tl::use_pdl() ? 2 : 1;
+    return cfg;
+}
+// CTAs of a cluster for so few items that all of them are on the GPU at once, an SM each; 1: no clusters.
+static int attend_ranks(long long items) {
+    constexpr int kMost = 8;  // of 13 one request of 1011 tokens takes 6.5 us for 6.0, of 8000 10.9 for 11.1
+    static std::atomic<int> held[64][kMost + 1];  // clusters of so many CTAs that a device holds, and 1 (the division of its SMs into groups decides: 15 of 8, 33 of 4)
+    int device = 0;
+    if (items <= 0 || items > sm_count() / 2 || cudaGetDevice(&device) != cudaSuccess || device >= 64) return 1;
+    for (int ranks = kMost; ranks > 1; --ranks) {
+        int known = held[device][ranks].load(std::memory_order_relaxed);
+        if (known == 0) {
+            const auto kernel = fp8_attend_kernel<bf16, 128, 128, 1>;
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kAtAlone);
+            cudaLaunchAttribute attr[2];
+            const cudaLaunchConfig_t cfg = at_clusters(ranks, ranks, kAtAlone, nullptr, attr);
+            int clusters = 0;
+            if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) clusters = 0, cudaGetLastError();
+            held[device][ranks].store(known = clusters + 1, std::memory_order_relaxed);
+        }
+        if (items < known) return ranks;
+    }
+    return 1;
+}
+
+// How a call's work is divided: an item a CTA, an item a cluster (`ranks` CTAs), or pieces, which a second launch joins.  `lens`: the lengths on the host, NULL: any.
+struct AtPlan {
+    int ranks;
+    size_t workspace;  // for pieces; 0: none
+};
+// What decides, in microseconds beside what all have in common (bf16, 8 columns, heads of 128): a CTA takes 0.075 a block; a cluster's joining takes 1.8 and the
+// launch that joins pieces 6.5, which stream at 6.2 TB/s whatever the lengths.  Measured, whole / clusters / pieces: one request of 100 tokens 4.0 / 5.8 / -, of 500 6.4 / 5.6 / -,
+// of 1011 8.7 / 6.0 / 10.7, of 8000 - / 11.1 / 13.6, of 32000 - / 25.0 / 19.8; 8 of 8000 - / 26.1 / 30.7; 24 of 70 to 1970 17.9 / - / 19.2; 16 of 8000 45 / - / 53.  Without lengths
+// clusters are for one or two requests: of more, one may be far longer than the others, which pieces make up for.
+static AtPlan attend_plan(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c, const int32_t *lens) {
+    const long long rows = static_cast<long long>(c.heads / p.heads) * c.tokens;
+    const int cols = attend_cols(p.dim, rows <= 8 ? 8 : 9), slots = attend_slots(c.dtype, p.dim, rows <= 8 ? 8 : 9);
+    const long long each = (rows + cols - 1) / cols * p.heads, items = each * c.batch;
+    long long longest = static_cast<long long>(c.max_pages) * (p.page_size / kF8Tokens), blocks = 0, live = c.batch;
+    if (lens) {
+        longest = live = 0;
+        for (int b = 0; b < c.batch; ++b) {
+            const long long n = (std::max(lens[b], 0) + kF8Tokens - 1LL) / kF8Tokens;
+            longest = std::max(longest, n), blocks += n, live += n > 0;
+        }
+    }
+    const int ranks = items <= 2 * sm_count() ? attend_ranks(each * live) : 1;  // idle slots are clusters too, which leave at once
+    const bool pieces = longest > kAtWhole && items <= 16LL * slots;            // more items than that have no use for pieces
+    const size_t workspace = static_cast<size_t>(items + slots) * at_piece_floats(cols, p.dim) * sizeof(float);
+    const double whole = longest * (c.dtype == TL_BF16 ? 0.075 : 0.18) * (cols == 16 ? 1.3 : 1.0), clusters = ranks > 1 ? 1.8 + whole / ranks : whole,
+                 cut = pieces ? 6.5 + static_cast<double>(blocks * each) * (2 * kF8Tokens * p.dim / 6.2e6) : whole;
+    if (lens ? clusters < whole && clusters <= cut : clusters < whole && ranks == 8) return {ranks, 0};
+    return {1, (lens ? cut < whole : pieces) ? workspace : 0};
 }
 
 template <typename T, int DP, int DIM, int NT>
@@ -537,13 +637,20 @@ static int attend_launch(F8Attend a, cudaStream_t st) {
     const int rings = kAtWarps * kAtStages * at_stage(a.pages.dim), smem = rings > joined ? rings : joined;
     int device = 0;
     cudaGetDevice(&device);
-    if (!ready(device, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most > joined ? most : joined) == cudaSuccess; }))
+    if (!ready(device, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, std::max(most > joined ? most : joined, kAtAlone)) == cudaSuccess; }))
         return tl::fail(TL_ECUDA, "fp8_attention: %s", cudaGetErrorString(cudaGetLastError()));
     a.col_blocks = (a.group * a.tokens + cols - 1) / cols;
     const long long items = static_cast<long long>(a.col_blocks) * a.pages.heads * a.batch;
     if (items > 0x3fffffff) return tl::fail(TL_EINVAL, "fp8_attention: sizes out of range");
     a.each_magic = f8_magic(items + a.slots, a.pages.heads * a.col_blocks);
-    cudaError_t e = tl::launch_chained(kernel, dim3(static_cast<unsigned>(items + (a.workspace ? a.slots : 0))), dim3(kAtWarps * 32), smem, st, a);
+    cudaError_t e;
+    if (a.ranks > 1) {
+        cudaLaunchAttribute attr[2];
+        const cudaLaunchConfig_t cfg = at_clusters(static_cast<unsigned>(items * a.ranks), a.ranks, std::max(smem, kAtAlone), st, attr);
+        e = cudaLaunchKernelEx(&cfg, kernel, a);
+    } else {
+        e = tl::launch_chained(kernel, dim3(static_cast<unsigned>(items + (a.workspace ? a.slots : 0))), dim3(kAtWarps * 32), smem, st, a);
+    }
     if (e != cudaSuccess) return tl::fail(TL_ECUDA, "fp8_attention: %s", cudaGetErrorString(e));
     TL_LAUNCH_CHECK("fp8_attention");
     if (!a.workspace) return TL_OK;
@@ -578,21 +685,7 @@ using namespace tlb;
 
 extern "C" size_t tlb_fp8_attention_workspace(const tlb_fp8_pages *pages, const tlb_fp8_attention_call *c, const int32_t *lens_host) {
     if (f8_check_pages("fp8_attention", pages) != TL_OK || !c || c->heads <= 0 || c->tokens <= 0 || c->batch <= 0) return 0;
-    const long long rows = static_cast<long long>(c->heads / pages->heads) * c->tokens;
-    const bool portion = f8_portion_takes(*pages, *c);
-    const int few = rows <= 8 ? 8 : 9, cols = portion ? kPoRows : attend_cols(pages->dim, few), slots = portion ? sm_count() : attend_slots(c->dtype, pages->dim, few);
-    const long long each = (rows + cols - 1) / cols * pages->heads, items = each * c->batch;
-    if (items > (portion ? 1LL : 16LL) * slots) return 0;  // more items than a cut would serve
-    long long longest = static_cast<long long>(c->max_pages) * (pages->page_size / kF8Tokens), blocks = 0;
-    if (lens_host) {
-        longest = 0;
-        for (int b = 0; b < c->batch; ++b) {
-            const long long n = (std::max(lens_host[b], 0) + kF8Tokens - 1LL) / kF8Tokens;
-            longest = std::max(longest, n), blocks += n;
-        }
-    }
-    if (portion ? longest <= kPoWhole : attend_whole(c->dtype, pages->dim, cols, longest, static_cast<double>(blocks) * each)) return 0;
-    return static_cast<size_t>(items + slots) * at_piece_floats(cols, pages->dim) * sizeof(float);
+    return f8_portion_takes(*pages, *c) ? f8_portion_workspace(*pages, *c, lens_host) : attend_plan(*pages, *c, lens_host).workspace;
 }
 
 extern "C" int tlb_fp8_attention(const tlb_fp8_pages *pages, const tlb_fp8_attention_call *c, const int32_t *lens_host, const int32_t *table_host, void *workspace,
@@ -604,9 +697,12 @@ extern "C" int tlb_fp8_attention(const tlb_fp8_pages *pages, const tlb_fp8_atten
     if (c->max_pages <= 0 || static_cast<long long>(c->heads / pages->heads) * c->tokens > (1 << 30)) return tl::fail(TL_EINVAL, "fp8_attention: sizes out of range");
     if (!c->q || !c->out || !c->table || !c->lens) return tl::fail(TL_EINVAL, "fp8_attention: missing argument");
     if (const int bad = f8_check_step("fp8_attention", *pages, lens_host, table_host, c->batch, c->max_pages, c->tokens)) return bad;
-    if (lens_host && !workspace && tlb_fp8_attention_workspace(pages, c, lens_host)) return tl::fail(TL_EWORKSPACE, "fp8_attention: a workspace is needed");
-    const size_t need = workspace ? tlb_fp8_attention_workspace(pages, c, nullptr) : 0;
-    if (need && (workspace_bytes < need || !tl::aligned16(workspace))) return tl::fail(TL_EWORKSPACE, "fp8_attention: the workspace must have %zu bytes, from a boundary of 16 on", need);
-    const F8Attend a(*pages, *c, need ? workspace : nullptr);  // without one every item is whole
+    const bool portion = f8_portion_takes(*pages, *c);
+    const AtPlan plan = portion ? AtPlan{1, f8_portion_workspace(*pages, *c, lens_host)} : attend_plan(*pages, *c, lens_host);
+    if (lens_host && !workspace && plan.workspace) return tl::fail(TL_EWORKSPACE, "fp8_attention: a workspace is needed");
+    if (workspace && plan.workspace && (workspace_bytes < plan.workspace || !tl::aligned16(workspace)))
+        return tl::fail(TL_EWORKSPACE, "fp8_attention: the workspace must have %zu bytes, from a boundary of 16 on", plan.workspace);
+    F8Attend a(*pages, *c, plan.workspace ? workspace : nullptr);  // without one no item is in pieces
+    a.ranks = plan.ranks;
     TLB_DISPATCH(c->dtype, "fp8_attention", return attend_any<T>(a, as_stream(stream)));
 }

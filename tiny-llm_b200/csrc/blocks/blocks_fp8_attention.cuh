@@ -13,6 +13,7 @@ struct F8Attend : tlb_fp8_attention_call {
     int group, col_blocks;  // query heads of a key/value head; items of a head: its columns by eights or sixteens
     int slots;              // CTAs that the GPU holds at a time
     int most_pieces;        // of an item
+    int ranks;              // CTAs of an item, a cluster; 1: no clusters
     int granule;            // pieces are a multiple of so many blocks
     int whole, least;       // blocks of a request that is not cut; of a piece at the least
     int page_blocks;        // blocks of 16 tokens in a page
@@ -20,7 +21,7 @@ struct F8Attend : tlb_fp8_attention_call {
     bool wide_rows;         // query rows may be read 16 bytes at a time
     float scale_log2, scale_rest;  // scale * log2(e), and what its rounding to fp32 left
     F8Attend(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c, void *ws)
-        : tlb_fp8_attention_call(c), pages(p), workspace(ws), group(c.heads / p.heads), col_blocks(0), slots(0), most_pieces(1), granule(1), whole(0), least(kAtLeast), page_blocks(1), page_magic(0), group_magic(0), heads_magic(0), each_magic(0), wide_rows(false) {
+        : tlb_fp8_attention_call(c), pages(p), workspace(ws), group(c.heads / p.heads), col_blocks(0), slots(0), most_pieces(1), ranks(1), granule(1), whole(0), least(kAtLeast), page_blocks(1), page_magic(0), group_magic(0), heads_magic(0), each_magic(0), wide_rows(false) {
         const double log2 = c.scale * 1.4426950408889634;
         scale_log2 = static_cast<float>(log2), scale_rest = static_cast<float>(log2 - scale_log2);
     }
@@ -139,5 +140,6 @@ constexpr int kPoRows = 256;  // columns of a CTA
 bool f8_portion_takes(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c);
 constexpr int kPoWhole = 40, kPoLeast = 24;  // blocks of a request that is not cut, of a piece at the least
 int f8_portion(F8Attend a, cudaStream_t st);
+size_t f8_portion_workspace(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c, const int32_t *lens);
 
 }  // namespace tlb

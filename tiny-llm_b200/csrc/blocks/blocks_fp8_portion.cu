@@ -11,6 +11,8 @@
 //   warps 16, 17 tcgen05.mma, one elected lane, a set each: S = Q K^T into one of two score buffers, O += P V; the next tile's scores are issued ahead of this tile's values.
 //                (One warp for both sets took 2000 cycles to issue a tile's 24 products of 32 cycles each.)
 //   warps 0-7    softmax, thread = row: scores from tensor memory, 2^x of them over a running maximum that may lag behind by 2^15, P as f16 back over its own scores
+#include <algorithm>
+
 #include "../per_device.h"
 #include "blocks_fp8_attention.cuh"
 #include "blocks_tc.cuh"
@@ -489,6 +491,17 @@ static int portion_launch(const F8Attend &a, unsigned ctas, cudaStream_t st) {
     if (e != cudaSuccess) return tl::fail(TL_ECUDA, "fp8_attention: %s", cudaGetErrorString(e));
     TL_LAUNCH_CHECK("fp8_attention (portion)");
     return a.workspace ? f8_attend_join(a, kPoRows, st) : TL_OK;
+}
+
+size_t f8_portion_workspace(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c, const int32_t *lens) {
+    const long long each = (static_cast<long long>(c.heads / p.heads) * c.tokens + kPoRows - 1) / kPoRows * p.heads, items = each * c.batch;
+    long long longest = static_cast<long long>(c.max_pages) * (p.page_size / kF8Tokens);
+    if (lens) {
+        longest = 0;
+        for (int b = 0; b < c.batch; ++b) longest = std::max(longest, (std::max(lens[b], 0) + kF8Tokens - 1LL) / kF8Tokens);
+    }
+    if (items > sm_count() || longest <= kPoWhole) return 0;  // more items than a cut would serve
+    return static_cast<size_t>(items + sm_count()) * at_piece_floats(kPoRows, p.dim) * sizeof(float);
 }
 
 int f8_portion(F8Attend a, cudaStream_t st) {

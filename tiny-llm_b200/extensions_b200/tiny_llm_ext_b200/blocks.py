@@ -1280,7 +1280,7 @@ def fp8_attention_of(pages: Fp8Pages, device: int, q, table, lens, scale, causal
     if rc == _EWORKSPACE:  # long requests may be cut into pieces
         size = lib.tlb_fp8_attention_workspace(at, call, lens_host)
         scratch = q.new_empty(size, dtype=torch.uint8) if size else None
-        rc = lib.tlb_fp8_attention(at, call, None, None, _ptr(scratch), size, stream)
+        rc = lib.tlb_fp8_attention(at, call, lens_host, table_host, _ptr(scratch), size, stream)
     if rc:
         if lens_host is not None and rc == _EINVAL:
             return None
