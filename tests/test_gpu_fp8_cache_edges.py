@@ -1,12 +1,14 @@
 """Calls of the 8-bit cache at the edges of what its documentation allows: rows that begin anywhere, captured launches whose requests grow past the cut into pieces, pages that are
 none, wide groups, far positions, two streams, idle slots.  Helpers and tolerances are those of the operators' own tests."""
 
+import math
+
 import numpy as np
 import pytest
 import torch
 
 from extensions_b200.tiny_llm_ext_b200 import blocks
-from tests.test_gpu_fp8_cache import check_attention, check_side, copy_of, on_host, random_pages, run_append, run_attention, table_of, to_gpu, turned
+from tests.test_gpu_fp8_cache import attention_tolerance, check_attention, check_side, copy_of, dense, on_host, random_pages, run_append, run_attention, table_of, to_gpu, turned
 from tiny_llm_b200 import FastRMSNorm, FastRoPE, Fp8KvPages, paged_attention_fp8, rotate_append_fp8
 
 DEV = "cuda"
@@ -209,3 +211,132 @@ def test_few_and_more_items(batch, kv_heads, group, dim, dtype):
     """Items that clusters of 8, 7 .. 2 CTAs share, and too many for that; lengths of less than a block a CTA, idle slots, and long ones beside them."""
     lengths = [(700, 0, 33, 16, 210, 5, 129, 1, 64, 300)[i % 10] for i in range(batch)]
     run_attention(lengths, 1, kv_heads * group, kv_heads, dim, 32, dtype, seed=batch + dim)
+
+
+# ---- portions of so many columns that the 5th-generation tensor cores take them ------------------------------------------
+
+
+def check_portion(out, q, pages, table, lengths, causal, scale):
+    """A weight rounded to f16 (11 significant bits) is off by at most half a step, 2^-11 of itself, and the sum that divides is of the weights before: 2^-11 of sum(p |v|).  The
+    shared bound counts 2^-12 of that and 2^-12 of the output, which is less where values cancel: 2^-12 of sum(p |v|) are added here.  Everything else is as there."""
+    page, new = pages.page_size, q.shape[2]
+    group = q.shape[1] // pages.kv_heads
+    for b, n in enumerate(lengths):
+        if n == 0:
+            assert (out[b] == 0).all()
+            continue
+        k, v = dense(pages, table[b], n, page)
+        for h in range(q.shape[1]):
+            x, keys, values = q[b, h].double(), k[h // group], v[h // group]
+            s = x @ keys.t() * scale
+            if causal:
+                s = s.masked_fill(torch.arange(n)[None] > torch.arange(n - new, n)[:, None], -math.inf)
+            p = torch.softmax(s, dim=-1)
+            want = p @ values
+            tol = attention_tolerance(x, keys, values, p, scale, want, torch.bfloat16, q.shape[3]) + 2.0**-12 * (p @ values.abs())
+            far = (out[b, h].cpu().double() - want).abs() - tol
+            assert (far <= 0).all(), (b, h, float(far.max()), float(tol.mean()))
+
+
+def run_portion(lengths, new, heads, kv_heads, dim, page, *, causal=True, seed=0, wide=1.0, strength=1.0):
+    gen = torch.Generator().manual_seed(seed + 5)
+    table, count = table_of(lengths, page, seed)
+    pages = random_pages(count, kv_heads, page, dim, gen, wide)
+    q = (strength * torch.randn(len(lengths), new, heads, dim, generator=gen)).to(torch.bfloat16).transpose(1, 2)
+    out = paged_attention_fp8(q.to(DEV), to_gpu(pages), torch.from_numpy(table).to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV), mask="causal" if causal else None)
+    check_portion(out, q, pages, table, lengths, causal, dim**-0.5)
+
+
+@pytest.mark.parametrize("lengths", [(1300, 0, 700), (600, 0, 401), (400, 400, 400)])
+@pytest.mark.parametrize("dim,page", [(128, 128), (64, 48), (128, 16)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_portions_of_many_columns(lengths, dim, page, causal):
+    run_portion(list(lengths), 400, 16, 2, dim, page, causal=causal, seed=dim + page, wide=3.0)
+
+
+@pytest.mark.parametrize("group,new,n", [(1, 2500, 2600), (5, 517, 2000), (64, 70, 900), (3, 1001, 1001)])
+def test_large_portions_of_other_groups(group, new, n):
+    run_portion([n], new, 2 * group, 2, 128, 64, seed=group, strength=2.0)
+
+
+@pytest.mark.parametrize("lengths", [(1300, 700), (600, 401)])
+@pytest.mark.parametrize("strided", [False, True])
+def test_a_large_portion_over_numbers_that_are_none(lengths, strided):
+    """A scale that is none reaches the rows that see its block, a query that is none its own row; what lies behind the last token reaches nobody."""
+    new, page, dim = 400, 64, 128
+    gen = torch.Generator().manual_seed(11)
+    table, count = table_of(lengths, page, 6)
+    pages = random_pages(count, 2, page, dim, gen)
+    q = torch.randn(2, 16, new, dim, generator=gen).to(torch.bfloat16)
+    first_bad = [lengths[0] - 150, lengths[1] - 33]  # tokens in whose blocks a scale is none
+    for b, (n, token) in enumerate(zip(lengths, first_bad)):
+        home, at = int(table[b, token // page]), token % page // 16
+        (pages.key_scales if b else pages.value_scales)[home, 1, at] = math.nan
+        home, slot = int(table[b, n // page]) if n % page else -1, n % page
+        if home >= 0:
+            pages.keys.view(torch.uint8)[home, :, slot:] = 0x7F
+            pages.values.view(torch.uint8)[home, :, slot:] = 0xFF
+            pages.key_scales[home, :, (slot + 15) // 16 :] = math.nan
+            pages.value_scales[home, :, (slot + 15) // 16 :] = math.nan
+    q[0, 3, 17, 5], q[1, 9, 399, 100] = math.inf, math.nan
+    gq = odd_rows(q.to(DEV)) if strided else q.to(DEV)
+    out = paged_attention_fp8(gq, to_gpu(pages), torch.from_numpy(table).to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV), mask="causal").cpu()
+    none = torch.zeros(2, 16, new, dtype=torch.bool)
+    none[0, 3, 17] = none[1, 9, 399] = True
+    for b, (n, token) in enumerate(zip(lengths, first_bad)):
+        sees = torch.arange(n - new, n) >= token // 16 * 16
+        none[b, 8:, sees] = True
+    assert torch.equal(out.isnan().any(-1), none) and torch.equal(out.isnan().all(-1), none)
+    # the others as if there were nothing of it
+    fine = Fp8KvPages(pages.keys, pages.values, torch.nan_to_num(pages.key_scales, nan=0.0), torch.nan_to_num(pages.value_scales, nan=0.0))
+    fine.keys.view(torch.uint8)[(pages.keys.view(torch.uint8) & 0x7F) == 0x7F] = 0
+    fine.values.view(torch.uint8)[(pages.values.view(torch.uint8) & 0x7F) == 0x7F] = 0
+    calm = q.clone()
+    calm[0, 3, 17, 5] = calm[1, 9, 399, 100] = 0.0
+    again = paged_attention_fp8(calm.to(DEV), to_gpu(fine), torch.from_numpy(table).to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV), mask="causal").cpu()
+    assert torch.equal(out[~none], again[~none])
+
+
+def test_a_large_portion_hides_pages_that_are_none():
+    new, page, dim, n = 600, 32, 128, 1500
+    table, count = table_of([n], page, 3)
+    gen = torch.Generator().manual_seed(4)
+    pages = random_pages(count, 2, page, dim, gen)
+    bad = table.copy()
+    bad[0, 2], bad[0, 40] = -1, count + 7
+    q = torch.randn(1, 16, new, dim, generator=gen).to(torch.bfloat16)
+    gp = to_gpu(pages)
+    # any lengths are covered by so wide a table: the kernel is chosen for them
+    out = blocks.fp8_attention(gp.native, gp.index, q.to(DEV), torch.from_numpy(bad).to(DEV), torch.tensor([n], dtype=torch.int32, device=DEV), dim**-0.5, True).cpu().double()
+    k, v = (torch.cat([x[int(p)] for p in table[0]], dim=1)[:, :n].double() for x in pages.dequantize())
+    hidden = torch.zeros(n, dtype=torch.bool)
+    hidden[2 * page : 3 * page], hidden[40 * page : 41 * page] = True, True
+    for h in range(0, 16, 5):
+        x = q[0, h].double()
+        s = (x @ k[h // 8].t() * dim**-0.5).masked_fill(hidden[None] | (torch.arange(n)[None] > torch.arange(n - new, n)[:, None]), -torch.inf)
+        p = torch.softmax(s, -1)
+        want = p @ v[h // 8]
+        most = (x.abs() @ k[h // 8].abs().t() * dim**-0.5).amax()
+        tol = (2.0**-11 + 2.0**-18 * most) * (p @ v[h // 8].abs() + want.abs()) + 2.0**-8 * want.abs() + 2.0**-16 * v[h // 8][~hidden].abs().amax(0)
+        assert ((out[0, h] - want).abs() <= tol).all()
+
+
+def test_a_captured_large_portion_follows_its_lengths():
+    new, page, dim, width = 512, 64, 64, 40
+    gen = torch.Generator().manual_seed(7)
+    pages_host = random_pages(2 * width, 2, page, dim, gen)
+    pages = to_gpu(pages_host)
+    table = np.random.RandomState(1).permutation(2 * width).astype(np.int32).reshape(2, width)
+    q = torch.randn(2, 16, new, dim, generator=gen).to(torch.bfloat16)
+    gq, gt, lens = q.to(DEV), torch.from_numpy(table).to(DEV), torch.tensor([600, 512], dtype=torch.int32, device=DEV)
+    full = dict(block_table_host=table, context_lens_host=np.asarray([width * page] * 2, dtype=np.int32))
+    graph = torch.cuda.CUDAGraph()
+    paged_attention_fp8(gq, pages, gt, lens, mask="causal", **full)
+    with torch.cuda.graph(graph):
+        out = paged_attention_fp8(gq, pages, gt, lens, mask="causal", **full)
+    for lengths in ([600, 512], [2560, 0], [513, 2500]):
+        lens.copy_(torch.tensor(lengths, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        check_portion(out, q, pages_host, table, lengths, True, dim**-0.5)
+    assert blocks.library().tlb_tc_gave_up() == 0

@@ -4,7 +4,7 @@
 // column being one (query head of the group, new token).  An e4m3 number is an f16 number, so the cache's side is exact; a column is brought to the top of
 // f16's range by a power of two, where bf16 keeps all its bits, and an fp32 query is two such terms.  A block's key scale multiplies its scores in fp32; its value
 // scale multiplies its weights, over the largest value scale so far (fp32 outputs: the product of weights and values).  Weights are exp2 of a number up to the
-// column's running maximum (which may lag behind by 2^15 before the sums are scaled again), rounded to f16 for the second product: 2^-12 of a weight, where an output is
+// column's running maximum (which may lag behind by 2^15 before the sums are scaled again), rounded to f16 for the second product: 2^-11 of a weight, where an output is
 // rounded to 2^-9 of itself; fp32 outputs take a second term for the rest.  Running sums are fp32.
 //
 // A warp takes blocks of 16 keys through a ring of its own in shared memory, filled by asynchronous copies, two blocks ahead of the one it works on; it waits for nobody
@@ -599,34 +599,39 @@ static int attend_ranks(long long items) {
     return 1;
 }
 
-// How a call's work is divided: an item a CTA, an item a cluster (`ranks` CTAs), or pieces, which a second launch joins.  `lens`: the lengths on the host, NULL: any.
-struct AtPlan {
-    int ranks;
-    size_t workspace;  // for pieces; 0: none
-};
 // What decides, in microseconds beside what all have in common (bf16, 8 columns, heads of 128): a CTA takes 0.075 a block; a cluster's joining takes 1.8 and the
 // launch that joins pieces 6.5, which stream at 6.2 TB/s whatever the lengths.  Measured, whole / clusters / pieces: one request of 100 tokens 4.0 / 5.8 / -, of 500 6.4 / 5.6 / -,
 // of 1011 8.7 / 6.0 / 10.7, of 8000 - / 11.1 / 13.6, of 32000 - / 25.0 / 19.8; 8 of 8000 - / 26.1 / 30.7; 24 of 70 to 1970 17.9 / - / 19.2; 16 of 8000 45 / - / 53.  Without lengths
 // clusters are for one or two requests: of more, one may be far longer than the others, which pieces make up for.
-static AtPlan attend_plan(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c, const int32_t *lens) {
+static AtPlan attend_plan(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c, const AtLengths &n, bool lens) {
     const long long rows = static_cast<long long>(c.heads / p.heads) * c.tokens;
     const int cols = attend_cols(p.dim, rows <= 8 ? 8 : 9), slots = attend_slots(c.dtype, p.dim, rows <= 8 ? 8 : 9);
     const long long each = (rows + cols - 1) / cols * p.heads, items = each * c.batch;
-    long long longest = static_cast<long long>(c.max_pages) * (p.page_size / kF8Tokens), blocks = 0, live = c.batch;
+    const int ranks = items <= 2 * sm_count() ? attend_ranks(each * n.live) : 1;  // idle slots are clusters too, which leave at once
+    const bool pieces = n.longest > kAtWhole && items <= 16LL * slots;            // more items than that have no use for pieces
+    const size_t workspace = static_cast<size_t>(items + slots) * at_piece_floats(cols, p.dim) * sizeof(float);
+    const double whole = n.longest * (c.dtype == TL_BF16 ? 0.075 : 0.18) * (cols == 16 ? 1.3 : 1.0), clusters = ranks > 1 ? 1.8 + whole / ranks : whole,
+                 cut = pieces ? 6.5 + static_cast<double>(n.blocks * each) * (2 * kF8Tokens * p.dim / 6.2e6) : whole;
+    if (lens ? clusters < whole && clusters <= cut : clusters < whole && ranks == 8) return {ranks, 0, 4 + clusters, false};
+    if (lens ? cut < whole : pieces) return {1, workspace, 4 + cut, false};
+    return {1, 0, ((each * n.live + slots - 1) / slots) * (4 + whole), false};
+}
+// Portions of many columns go to the kernel of blocks_fp8_portion.cu unless this one is sooner through, as it is with few items, which clusters divide (16 tokens over 1000 with
+// groups of 4: 9.9 us here, 22.6 there; 64 over 1000 12.4 and 24.5, over 3500 26.9 and 25.9; 8 requests of 16 over 1000 23.5 and 30.7, 32 of them 79 and 58).
+static AtPlan any_plan(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c, const int32_t *lens) {
+    AtLengths n{static_cast<long long>(c.max_pages) * (p.page_size / kF8Tokens), 0, c.batch};
+    n.blocks = n.longest * c.batch;
     if (lens) {
-        longest = live = 0;
+        n = {0, 0, 0};
         for (int b = 0; b < c.batch; ++b) {
-            const long long n = (std::max(lens[b], 0) + kF8Tokens - 1LL) / kF8Tokens;
-            longest = std::max(longest, n), blocks += n, live += n > 0;
+            const long long one = (std::max(lens[b], 0) + kF8Tokens - 1LL) / kF8Tokens;
+            n.longest = std::max(n.longest, one), n.blocks += one, n.live += one > 0;
         }
     }
-    const int ranks = items <= 2 * sm_count() ? attend_ranks(each * live) : 1;  // idle slots are clusters too, which leave at once
-    const bool pieces = longest > kAtWhole && items <= 16LL * slots;            // more items than that have no use for pieces
-    const size_t workspace = static_cast<size_t>(items + slots) * at_piece_floats(cols, p.dim) * sizeof(float);
-    const double whole = longest * (c.dtype == TL_BF16 ? 0.075 : 0.18) * (cols == 16 ? 1.3 : 1.0), clusters = ranks > 1 ? 1.8 + whole / ranks : whole,
-                 cut = pieces ? 6.5 + static_cast<double>(blocks * each) * (2 * kF8Tokens * p.dim / 6.2e6) : whole;
-    if (lens ? clusters < whole && clusters <= cut : clusters < whole && ranks == 8) return {ranks, 0};
-    return {1, (lens ? cut < whole : pieces) ? workspace : 0};
+    const AtPlan rows = attend_plan(p, c, n, lens != nullptr);
+    if (!f8_portion_takes(p, c)) return rows;
+    const AtPlan portion = f8_portion_plan(p, c, n);
+    return rows.time < portion.time ? rows : portion;
 }
 
 template <typename T, int DP, int DIM, int NT>
@@ -665,7 +670,7 @@ static int attend_columns(const F8Attend &a, cudaStream_t st) {
 }
 
 template <typename T>
-static int attend_any(F8Attend a, cudaStream_t st) {
+static int attend_any(F8Attend a, bool portion, cudaStream_t st) {
     const int D = a.pages.dim;
     a.wide_rows = tl::aligned16(a.q) && ((a.q_b | a.q_h | a.q_l) * static_cast<long long>(sizeof(T)) & 15) == 0;
     a.page_blocks = a.pages.page_size / kF8Tokens;
@@ -673,7 +678,7 @@ static int attend_any(F8Attend a, cudaStream_t st) {
     a.group_magic = f8_magic(static_cast<unsigned long long>(a.group) * a.tokens, a.group);
     a.heads_magic = f8_magic(static_cast<unsigned long long>(a.pages.heads) * ((a.group * a.tokens + 7) / 8), a.pages.heads);
     a.slots = attend_slots(a.dtype, D, a.group * a.tokens), a.most_pieces = 128, a.whole = kAtWhole;
-    if (f8_portion_takes(a.pages, a)) return f8_portion(a, st);
+    if (portion) return f8_portion(a, st);
     if (D <= 64) return D == 64 ? attend_columns<T, 64, 64>(a, st) : attend_columns<T, 64, 0>(a, st);
     if (D <= 128) return D == 128 ? attend_columns<T, 128, 128>(a, st) : attend_columns<T, 128, 0>(a, st);
     return attend_launch<T, 256, 0, 1>(a, st);
@@ -685,7 +690,7 @@ using namespace tlb;
 
 extern "C" size_t tlb_fp8_attention_workspace(const tlb_fp8_pages *pages, const tlb_fp8_attention_call *c, const int32_t *lens_host) {
     if (f8_check_pages("fp8_attention", pages) != TL_OK || !c || c->heads <= 0 || c->tokens <= 0 || c->batch <= 0) return 0;
-    return f8_portion_takes(*pages, *c) ? f8_portion_workspace(*pages, *c, lens_host) : attend_plan(*pages, *c, lens_host).workspace;
+    return any_plan(*pages, *c, lens_host).workspace;
 }
 
 extern "C" int tlb_fp8_attention(const tlb_fp8_pages *pages, const tlb_fp8_attention_call *c, const int32_t *lens_host, const int32_t *table_host, void *workspace,
@@ -697,12 +702,11 @@ extern "C" int tlb_fp8_attention(const tlb_fp8_pages *pages, const tlb_fp8_atten
     if (c->max_pages <= 0 || static_cast<long long>(c->heads / pages->heads) * c->tokens > (1 << 30)) return tl::fail(TL_EINVAL, "fp8_attention: sizes out of range");
     if (!c->q || !c->out || !c->table || !c->lens) return tl::fail(TL_EINVAL, "fp8_attention: missing argument");
     if (const int bad = f8_check_step("fp8_attention", *pages, lens_host, table_host, c->batch, c->max_pages, c->tokens)) return bad;
-    const bool portion = f8_portion_takes(*pages, *c);
-    const AtPlan plan = portion ? AtPlan{1, f8_portion_workspace(*pages, *c, lens_host)} : attend_plan(*pages, *c, lens_host);
+    const AtPlan plan = any_plan(*pages, *c, lens_host);
     if (lens_host && !workspace && plan.workspace) return tl::fail(TL_EWORKSPACE, "fp8_attention: a workspace is needed");
     if (workspace && plan.workspace && (workspace_bytes < plan.workspace || !tl::aligned16(workspace)))
         return tl::fail(TL_EWORKSPACE, "fp8_attention: the workspace must have %zu bytes, from a boundary of 16 on", plan.workspace);
     F8Attend a(*pages, *c, plan.workspace ? workspace : nullptr);  // without one no item is in pieces
     a.ranks = plan.ranks;
-    TLB_DISPATCH(c->dtype, "fp8_attention", return attend_any<T>(a, as_stream(stream)));
+    TLB_DISPATCH(c->dtype, "fp8_attention", return attend_any<T>(a, plan.portion, as_stream(stream)));
 }

@@ -132,14 +132,24 @@ __device__ __forceinline__ int at_pieces_of(const F8Attend &a, int request, int 
     return __shfl_sync(0xffffffffu, of, request & 31);
 }
 
+// How a call's work is divided: an item a CTA, an item a cluster (`ranks` CTAs), or pieces, which a second launch joins.
+struct AtPlan {
+    int ranks;
+    size_t workspace;  // for pieces; 0: none
+    double time;       // about how many microseconds it takes
+    bool portion;      // by the kernel of blocks_fp8_portion.cu
+};
+struct AtLengths {
+    long long longest, blocks, live;  // blocks of the longest request, of all; requests that are not idle
+};
 // blocks_fp8_attention.cu: adds up the pieces of the launch in front, items of `cols` columns each.
 int f8_attend_join(const F8Attend &a, int cols, cudaStream_t st);
 __host__ __device__ static inline size_t at_piece_floats(int cols, int dim) { return static_cast<size_t>(cols) * (dim + 2); }
 // blocks_fp8_portion.cu: bf16 queries of many columns
 constexpr int kPoRows = 256;  // columns of a CTA
-bool f8_portion_takes(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c);
+bool f8_portion_takes(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c);  // more than 32 columns: fewer are never sooner through there
 constexpr int kPoWhole = 40, kPoLeast = 24;  // blocks of a request that is not cut, of a piece at the least
 int f8_portion(F8Attend a, cudaStream_t st);
-size_t f8_portion_workspace(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c, const int32_t *lens);
+AtPlan f8_portion_plan(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c, const AtLengths &n);
 
 }  // namespace tlb

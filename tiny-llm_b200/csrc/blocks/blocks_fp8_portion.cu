@@ -1,6 +1,6 @@
 // Attention of many columns (prompt portions) over pages of 8 bits on the 5th-generation tensor cores, bf16 queries, heads of 64 or 128 entries.
 //
-// The arithmetic is that of blocks_fp8_attention.cu; the operands of both products are f16 here too, so that nothing is lost ahead of the weights' rounding (2^-12):
+// The arithmetic is that of blocks_fp8_attention.cu; the operands of both products are f16 here too, so that nothing is lost ahead of the weights' rounding (2^-11):
 // a query row is brought to the top of f16's range by a power of two, keys and values are their e4m3 numbers times their block's scale over the largest
 // scale of the CTA's blocks - exact down to 2^-15 of that, and below it off by at most 2^-34 of the largest block's numbers.  A block whose
 // scale is no number counts as zeros in the products, and the rows that see it are made NaN at the end.
@@ -11,8 +11,6 @@
 //   warps 16, 17 tcgen05.mma, one elected lane, a set each: S = Q K^T into one of two score buffers, O += P V; the next tile's scores are issued ahead of this tile's values.
 //                (One warp for both sets took 2000 cycles to issue a tile's 24 products of 32 cycles each.)
 //   warps 0-7    softmax, thread = row: scores from tensor memory, 2^x of them over a running maximum that may lag behind by 2^15, P as f16 back over its own scores
-#include <algorithm>
-
 #include "../per_device.h"
 #include "blocks_fp8_attention.cuh"
 #include "blocks_tc.cuh"
@@ -493,15 +491,13 @@ static int portion_launch(const F8Attend &a, unsigned ctas, cudaStream_t st) {
     return a.workspace ? f8_attend_join(a, kPoRows, st) : TL_OK;
 }
 
-size_t f8_portion_workspace(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c, const int32_t *lens) {
-    const long long each = (static_cast<long long>(c.heads / p.heads) * c.tokens + kPoRows - 1) / kPoRows * p.heads, items = each * c.batch;
-    long long longest = static_cast<long long>(c.max_pages) * (p.page_size / kF8Tokens);
-    if (lens) {
-        longest = 0;
-        for (int b = 0; b < c.batch; ++b) longest = std::max(longest, (std::max(lens[b], 0) + kF8Tokens - 1LL) / kF8Tokens);
-    }
-    if (items > sm_count() || longest <= kPoWhole) return 0;  // more items than a cut would serve
-    return static_cast<size_t>(items + sm_count()) * at_piece_floats(kPoRows, p.dim) * sizeof(float);
+// A CTA takes 9 us and 1.3 for every 64 keys; with pieces, which are about as many as SMs, and the launch that joins them it is 20 beside the keys.
+AtPlan f8_portion_plan(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c, const AtLengths &n) {
+    const long long each = (static_cast<long long>(c.heads / p.heads) * c.tokens + kPoRows - 1) / kPoRows * p.heads, items = each * c.batch, slots = sm_count();
+    const double block = 1.3 * kF8Tokens / kPoKeys;
+    if (items > slots || n.longest <= kPoWhole)  // more items than a cut would serve
+        return {1, 0, ((each * n.live + slots - 1) / slots) * (9 + n.longest * block), true};
+    return {1, static_cast<size_t>(items + slots) * at_piece_floats(kPoRows, p.dim) * sizeof(float), 20 + static_cast<double>(n.blocks * each) / slots * block, true};
 }
 
 int f8_portion(F8Attend a, cudaStream_t st) {
