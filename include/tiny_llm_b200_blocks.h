@@ -2,7 +2,7 @@
  * tiny_llm_b200_blocks.h - C ABI of libtiny_llm_b200_blocks.so: building blocks for decoder layers with
  * unquantised (bf16 or fp32) weights on B200 (sm_100a): row-wise norms with a residual stream kept in fp32,
  * rotary positions in both pair layouts, paged latent (low-rank) key/value storage, latent attention with an
- * optional sliding window over ragged batches, gated activations and a top-k mixture-of-experts feed-forward.
+ * optional sliding window over ragged batches, gated activations and a top-k mixture-of-experts feed-forward; products over 8-bit weights, a paged key/value cache of 8 bits.
  *
  * Conventions are those of tiny_llm_b200.h: plain device pointers and sizes, the caller owns every buffer, a
  * launcher never allocates, frees or synchronises and enqueues on `stream` (a cudaStream_t passed as void*);

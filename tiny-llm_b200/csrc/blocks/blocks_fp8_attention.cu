@@ -15,6 +15,9 @@
 // An item is 8 (or 16) columns of one request and key/value head.  A CTA takes an item; or, where items are few, a cluster does, whose CTAs read each other's sums; or, where
 // requests are of unlike length or very long, a CTA takes a piece of one, which leaves a partial result for fp8_attend_join_kernel to add up in order.  Both follow the lengths
 // on the device, so a captured launch does.  attend_plan chooses.
+//
+// 64 requests of 8192 (1.08 GB) take 159 us, 6.8 TB/s: HBM.  With fewer, a block is a chain of latencies (1100 cycles of a warp: copies, eight products, exponentials, eight products), so an item of 1970 tokens
+// takes 10 us of the 18 of a step of 24 requests.  Not faster: 16 warps a CTA (24 requests 14.8 us, but 30 of 1000 tokens 18.7 for 14.2), rings of six blocks.
 #include <algorithm>
 #include <atomic>
 
