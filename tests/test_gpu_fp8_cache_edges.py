@@ -340,3 +340,10 @@ def test_a_captured_large_portion_follows_its_lengths():
         torch.cuda.synchronize()
         check_portion(out, q, pages_host, table, lengths, True, dim**-0.5)
     assert blocks.library().tlb_tc_gave_up() == 0
+
+
+@pytest.mark.parametrize("batch", [20, 32, 33])
+def test_unlike_requests_in_any_order(batch):
+    """More items than SMs: requests are taken by their length, equal ones and idle slots among them."""
+    lengths = [(5, 300, 0, 17, 300, 1, 64, 900)[(3 * i) % 8] for i in range(batch)]
+    run_attention(lengths, 1, 32, 8, 64, 32, torch.bfloat16, seed=batch)

@@ -17,7 +17,7 @@
 // on the device, so a captured launch does.  attend_plan chooses.
 //
 // 64 requests of 8192 (1.08 GB) take 159 us, 6.8 TB/s: HBM.  With fewer, a block is a chain of latencies (1100 cycles of a warp: copies, eight products, exponentials, eight products), so an item of 1970 tokens
-// takes 10 us of the 18 of a step of 24 requests.  Not faster: 16 warps a CTA (24 requests 14.8 us, but 30 of 1000 tokens 18.7 for 14.2), rings of six blocks.
+// takes 10 us of the 17 of a step of 24 requests.  Not faster: 16 warps a CTA (24 requests 14.8 us, but 30 of 1000 tokens 18.7 for 14.2), rings of six blocks.
 #include <algorithm>
 #include <atomic>
 
@@ -604,7 +604,7 @@ static int attend_ranks(long long items) {
 
 // What decides, in microseconds beside what all have in common (bf16, 8 columns, heads of 128): a CTA takes 0.075 a block; a cluster's joining takes 1.8 and the
 // launch that joins pieces 6.5, which stream at 6.2 TB/s whatever the lengths.  Measured, whole / clusters / pieces: one request of 100 tokens 4.0 / 5.8 / -, of 500 6.4 / 5.6 / -,
-// of 1011 8.7 / 6.0 / 10.7, of 8000 - / 11.1 / 13.6, of 32000 - / 25.0 / 19.8; 8 of 8000 - / 26.1 / 30.7; 24 of 70 to 1970 17.9 / - / 19.2; 16 of 8000 45 / - / 53.  Without lengths
+// of 1011 8.7 / 6.0 / 10.7, of 8000 - / 11.1 / 13.6, of 32000 - / 25.0 / 19.8; 8 of 8000 - / 26.1 / 30.7; 24 of 70 to 1970 16.8 / - / 19.2; 16 of 8000 45 / - / 53.  Without lengths
 // clusters are for one or two requests: of more, one may be far longer than the others, which pieces make up for.
 static AtPlan attend_plan(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c, const AtLengths &n, bool lens) {
     const long long rows = static_cast<long long>(c.heads / p.heads) * c.tokens;
@@ -617,7 +617,9 @@ static AtPlan attend_plan(const tlb_fp8_pages &p, const tlb_fp8_attention_call &
                  cut = pieces ? 6.5 + static_cast<double>(n.blocks * each) * (2 * kF8Tokens * p.dim / 6.2e6) : whole;
     if (lens ? clusters < whole && clusters <= cut : clusters < whole && ranks == 8) return {ranks, 0, 4 + clusters, false};
     if (lens ? cut < whole : pieces) return {1, workspace, 4 + cut, false};
-    return {1, 0, ((each * n.live + slots - 1) / slots) * (4 + whole), false};
+    // The last items come to an SM beside others, and then both are slower: let these be the short ones (24 requests of 70 to 1970 17.8 -> 16.8 us; 0.3 us where all are alike)
+    const bool long_first = lens && c.batch <= 32 && items > sm_count() && n.longest * n.live > n.blocks + n.blocks / 4;
+    return {1, 0, ((each * n.live + slots - 1) / slots) * (4 + whole), false, long_first};
 }
 // Portions of many columns go to the kernel of blocks_fp8_portion.cu unless this one is sooner through, as it is with few items, which clusters divide (16 tokens over 1000 with
 // groups of 4: 9.9 us here, 22.6 there; 64 over 1000 12.4 and 24.5, over 3500 26.9 and 25.9; 8 requests of 16 over 1000 23.5 and 30.7, 32 of them 79 and 58).
@@ -710,6 +712,6 @@ extern "C" int tlb_fp8_attention(const tlb_fp8_pages *pages, const tlb_fp8_atten
     if (workspace && plan.workspace && (workspace_bytes < plan.workspace || !tl::aligned16(workspace)))
         return tl::fail(TL_EWORKSPACE, "fp8_attention: the workspace must have %zu bytes, from a boundary of 16 on", plan.workspace);
     F8Attend a(*pages, *c, plan.workspace ? workspace : nullptr);  // without one no item is in pieces
-    a.ranks = plan.ranks;
+    a.ranks = plan.ranks, a.long_first = plan.long_first;
     TLB_DISPATCH(c->dtype, "fp8_attention", return attend_any<T>(a, plan.portion, as_stream(stream)));
 }

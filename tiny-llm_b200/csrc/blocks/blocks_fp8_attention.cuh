@@ -19,9 +19,10 @@ struct F8Attend : tlb_fp8_attention_call {
     int page_blocks;        // blocks of 16 tokens in a page
     unsigned page_magic, group_magic, heads_magic, each_magic;  // for divisions by page_blocks, group, heads and the items of a request (f8_div)
     bool wide_rows;         // query rows may be read 16 bytes at a time
+    bool long_first;        // requests (at most 32) are taken by their length, where no item is divided
     float scale_log2, scale_rest;  // scale * log2(e), and what its rounding to fp32 left
     F8Attend(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c, void *ws)
-        : tlb_fp8_attention_call(c), pages(p), workspace(ws), group(c.heads / p.heads), col_blocks(0), slots(0), most_pieces(1), ranks(1), granule(1), whole(0), least(kAtLeast), page_blocks(1), page_magic(0), group_magic(0), heads_magic(0), each_magic(0), wide_rows(false) {
+        : tlb_fp8_attention_call(c), pages(p), workspace(ws), group(c.heads / p.heads), col_blocks(0), slots(0), most_pieces(1), ranks(1), granule(1), whole(0), least(kAtLeast), page_blocks(1), page_magic(0), group_magic(0), heads_magic(0), each_magic(0), wide_rows(false), long_first(false) {
         const double log2 = c.scale * 1.4426950408889634;
         scale_log2 = static_cast<float>(log2), scale_rest = static_cast<float>(log2 - scale_log2);
     }
@@ -86,6 +87,19 @@ __device__ __forceinline__ AtPiece at_piece(const F8Attend &a, int index) {
     const int each = a.pages.heads * a.col_blocks, lane = threadIdx.x & 31;
     const int want = f8_div(index, each, a.each_magic);  // rounded down: an item's pieces over all items of a request are a multiple of them
     AtPiece x{-1, 0, 0, 0, 1, 0x3fffffff};
+    if (a.long_first && !a.workspace) {
+        const int ctx = lane < a.batch ? at_context(a, lane) : -1;
+        int rank = 0;
+#pragma unroll
+        for (int r = 0; r < 32; ++r) {
+            const int other = __shfl_sync(0xffffffffu, ctx, r);
+            rank += other > ctx || (other == ctx && r < lane);
+        }
+        const unsigned mine = __ballot_sync(0xffffffffu, lane < a.batch && rank == want);
+        if (mine) x.b = __ffs(mine) - 1, x.ctx = __shfl_sync(0xffffffffu, ctx, x.b);
+        x.item = index - want * each;
+        return x;
+    }
     if (!a.workspace) {
         if (want < a.batch) x.b = want, x.ctx = at_context(a, want);
         x.item = index - want * each;
@@ -138,6 +152,7 @@ struct AtPlan {
     size_t workspace;  // for pieces; 0: none
     double time;       // about how many microseconds it takes
     bool portion;      // by the kernel of blocks_fp8_portion.cu
+    bool long_first = false;
 };
 struct AtLengths {
     long long longest, blocks, live;  // blocks of the longest request, of all; requests that are not idle
