@@ -347,3 +347,31 @@ def test_unlike_requests_in_any_order(batch):
     """More items than SMs: requests are taken by their length, equal ones and idle slots among them."""
     lengths = [(5, 300, 0, 17, 300, 1, 64, 900)[(3 * i) % 8] for i in range(batch)]
     run_attention(lengths, 1, 32, 8, 64, 32, torch.bfloat16, seed=batch)
+
+
+@pytest.mark.parametrize("bad", [None, 12_900, 13_400])
+def test_a_large_portion_far_into_a_long_request(bad):
+    """More blocks than a CTA has threads, so that scales are looked over in several rounds; one that is none among the last."""
+    new, page, dim, n = 2500, 128, 64, 13_500
+    gen = torch.Generator().manual_seed(9)
+    table, count = table_of([n, 70], page, 1)
+    pages = random_pages(count, 4, page, dim, gen, wide=2.0)
+    if bad is not None:
+        pages.value_scales[int(table[0, bad // page]), :, bad % page // 16] = math.nan
+    q = torch.randn(1, 40, new, dim, generator=gen).to(torch.bfloat16)
+    out = paged_attention_fp8(q.to(DEV), to_gpu(pages), torch.from_numpy(table[:1]).to(DEV), torch.tensor([n], dtype=torch.int32, device=DEV), mask="causal").cpu()
+    sees = torch.arange(n - new, n) >= (n if bad is None else bad // 16 * 16)
+    assert out[0, :, sees].isnan().all() and not out[0, :, ~sees].isnan().any()
+    k, v = dense(pages, table[0], n, page)
+    v = torch.nan_to_num(v, nan=0.0)
+    for h in (0, 13, 39):
+        for rows in (slice(0, 40), slice(1200, 1240), slice(2300, 2340)):
+            rows = torch.arange(new)[rows][~sees[rows]]
+            if not len(rows):
+                continue
+            x = q[0, h, rows].double()
+            s = (x @ k[h // 10].t() * dim**-0.5).masked_fill(torch.arange(n)[None] > (rows + n - new)[:, None], -math.inf)
+            p = torch.softmax(s, -1)
+            want = p @ v[h // 10]
+            tol = attention_tolerance(x, k[h // 10], v[h // 10], p, dim**-0.5, want, torch.bfloat16, dim) + 2.0**-12 * (p @ v[h // 10].abs())
+            assert ((out[0, h, rows].double() - want).abs() <= tol).all()

@@ -186,51 +186,70 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
         }
     };
     if (warp >= 8 && warp < 16) look_up(0), ask(0), look_up(1);
-    // queries: 8 entries a lane, a row to 8 or 16 lanes of the first sixteen warps; first as they are, to where the operand tiles will be
-    constexpr int LANES = DIM / 8, ROWS = 32 / LANES, N = kPoRows / (16 * ROWS);
-    unsigned char *mine_q = psm + Z::k_off + threadIdx.x * 16;
-    if (warp < 16) {
-        const bf16 *q = static_cast<const bf16 *>(a.q) + b * a.q_b + static_cast<long long>(h) * G * a.q_h + lane % LANES * 8;
-#pragma unroll 4
-        for (int i = 0; i < N; ++i) {
-            const int col = c0 + (i * 16 + warp) * ROWS + lane / LANES, l = f8_div(min(col, columns - 1), G, a.group_magic);
-            const bf16 *from = q + l * a.q_l + (min(col, columns - 1) - l * G) * a.q_h;
-            if (a.wide_rows) {
-                po_copy16(g_smem_u32(mine_q + i * 8192), from, col < columns);
-            } else {
-#pragma unroll 1
-                for (int e = 0; e < 8; ++e) reinterpret_cast<bf16 *>(mine_q + i * 8192)[e] = col < columns ? from[e] : __float2bfloat16_rn(0.f);
-            }
-        }
-    }
-    for (int blk = begin + threadIdx.x; blk < stop; blk += kPoThreads) {  // meanwhile the largest scales
+    // scales of the CTA's blocks, for the largest ones: asked for ahead of the queries, looked at behind them
+    auto scales_of = [&](int blk) {
         int page;
         const size_t at = block_at(blk, page);
         const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(pg.num_pages);
-        const float k = there ? __ldg(pg.key_scales + at) : NAN, v = there ? __ldg(pg.value_scales + at) : NAN;
-        if (k < INFINITY) atomicMax(seen, __float_as_int(k));
-        if (v < INFINITY) atomicMax(seen + 1, __float_as_int(v));
-        if (!(k < INFINITY) || !(v < INFINITY)) seen[2] = 1;
+        return make_float2(there ? __ldg(pg.key_scales + at) : NAN, there ? __ldg(pg.value_scales + at) : NAN);
+    };
+    auto look_over = [&](float2 s) {  // whole warps
+        const int k = __reduce_max_sync(0xffffffffu, s.x < INFINITY ? __float_as_int(s.x) : 0), v = __reduce_max_sync(0xffffffffu, s.y < INFINITY ? __float_as_int(s.y) : 0);
+        if (lane == 0 && k > 0) atomicMax(seen, k);
+        if (lane == 0 && v > 0) atomicMax(seen + 1, v);
+        if (!(s.x < INFINITY) || !(s.y < INFINITY)) seen[2] = 1;
+    };
+    float2 of_mine = make_float2(0.f, 0.f);
+    if (begin + static_cast<int>(threadIdx.x) < stop) of_mine = scales_of(begin + threadIdx.x);
+    // queries: 8 entries of either 64 a lane, a row to 8 lanes of the first sixteen warps; first as they are, to where the operand tiles will be
+    constexpr int PARTS = DIM / 64, N = kPoRows / (16 * 4);
+    unsigned char *mine_q = psm + Z::k_off + threadIdx.x * 16;
+    if (warp < 16) {
+        const bf16 *q = static_cast<const bf16 *>(a.q) + b * a.q_b + static_cast<long long>(h) * G * a.q_h + lane % 8 * 8;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int col = c0 + (i * 16 + warp) * 4 + lane / 8, l = f8_div(min(col, columns - 1), G, a.group_magic);
+            const bf16 *from = q + l * a.q_l + (min(col, columns - 1) - l * G) * a.q_h;
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) {
+                unsigned char *to = mine_q + (i * PARTS + p) * 8192;
+                if (a.wide_rows) {
+                    po_copy16(g_smem_u32(to), from + 64 * p, col < columns);
+                } else {
+#pragma unroll 1
+                    for (int e = 0; e < 8; ++e) reinterpret_cast<bf16 *>(to)[e] = col < columns ? from[64 * p + e] : __float2bfloat16_rn(0.f);
+                }
+            }
+        }
     }
+    look_over(of_mine);
+    for (int blk = begin + threadIdx.x + kPoThreads; blk - lane < stop; blk += kPoThreads) look_over(blk < stop ? scales_of(blk) : make_float2(0.f, 0.f));
     if (warp < 16) {
         const float sign = a.scale_log2 < 0.f ? -1.f : 1.f;
         asm volatile("cp.async.wait_all;" ::: "memory");
-#pragma unroll 4
+#pragma unroll 2
         for (int i = 0; i < N; ++i) {
-            const int row = (i * 16 + warp) * ROWS + lane / LANES;
-            const uint4 u = *reinterpret_cast<const uint4 *>(mine_q + i * 8192);
-            // magnitudes are in the order of their bits, numbers that are none on top
-            uint32_t m = __vmaxu2(__vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu), __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu));
+            const int row = (i * 16 + warp) * 4 + lane / 8, j = lane % 8, in_set = row % kPoSet;
+            uint4 u[PARTS];
+            uint32_t m = 0;  // magnitudes are in the order of their bits, numbers that are none on top
 #pragma unroll
-            for (int o = 1; o < LANES; o <<= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+            for (int p = 0; p < PARTS; ++p) {
+                u[p] = *reinterpret_cast<const uint4 *>(mine_q + (i * PARTS + p) * 8192);
+                m = __vmaxu2(m, __vmaxu2(__vmaxu2(u[p].x & 0x7fff7fffu, u[p].y & 0x7fff7fffu), __vmaxu2(u[p].z & 0x7fff7fffu, u[p].w & 0x7fff7fffu)));
+            }
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
             const int e2 = static_cast<int>(max(m >> 16, m & 0xffffu) >> 7), up = e2 == 255 ? 0 : min(13 + 127 - e2, 100);
-            const float2 y[4] = {tl::unpack2<bf16>(u.x), tl::unpack2<bf16>(u.y), tl::unpack2<bf16>(u.z), tl::unpack2<bf16>(u.w)};
             const float times = f8_power(up) * sign;
-            const int j = lane % LANES, in_set = row % kPoSet;
-            uint4 f;
-            f.x = tl::pack2<__half>(y[0].x * times, y[0].y * times), f.y = tl::pack2<__half>(y[1].x * times, y[1].y * times);
-            f.z = tl::pack2<__half>(y[2].x * times, y[2].y * times), f.w = tl::pack2<__half>(y[3].x * times, y[3].y * times);
-            *reinterpret_cast<uint4 *>(psm + (row / kPoSet * Z::halves + (j >> 3)) * Z::q_block + in_set * 128 + (((j & 7) ^ (in_set & 7)) << 4)) = f;
+            unsigned char *to = psm + row / kPoSet * Z::halves * Z::q_block + in_set * 128 + ((j ^ (in_set & 7)) << 4);
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) {
+                const float2 y[4] = {tl::unpack2<bf16>(u[p].x), tl::unpack2<bf16>(u[p].y), tl::unpack2<bf16>(u[p].z), tl::unpack2<bf16>(u[p].w)};
+                uint4 f;
+                f.x = tl::pack2<__half>(y[0].x * times, y[0].y * times), f.y = tl::pack2<__half>(y[1].x * times, y[1].y * times);
+                f.z = tl::pack2<__half>(y[2].x * times, y[2].y * times), f.w = tl::pack2<__half>(y[3].x * times, y[3].y * times);
+                *reinterpret_cast<uint4 *>(to + p * Z::q_block) = f;
+            }
             if (j == 0) row_factor[row] = f8_power(-up);
         }
         g_fence_proxy_async();
