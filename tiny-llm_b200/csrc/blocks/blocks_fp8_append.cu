@@ -60,7 +60,7 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
 // Numbers of earlier tokens rounded to the block's larger scale.
 __device__ __forceinline__ void ap_again(uint8_t *rows, int pieces, float ratio) {
     for (int i = threadIdx.x; i < pieces; i += kApThreads) {
-        uint4 x = reinterpret_cast<uint4 *>(rows)[i];
+        uint4 x = tl::ld_cg(reinterpret_cast<const uint4 *>(rows) + i);
         uint32_t *w = reinterpret_cast<uint32_t *>(&x);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -109,13 +109,14 @@ __device__ __forceinline__ float4 ap_angle(int position, double of, const float4
     return make_float4(co.h, co.l, si.h, si.l);
 }
 
-// A lane's 8 entries of a row: four from a0 on, four from b0 on.
+// A lane's 8 entries of a row: four from a0 on, four from b0 on.  ask: of numbers that the launch in front may have written, through L2.
 template <typename T>
 struct ApRow;
 template <>
 struct ApRow<bf16> {
     uint2 a, b;
     __device__ __forceinline__ void load(const bf16 *p, int a0, int b0) { a = *reinterpret_cast<const uint2 *>(p + a0), b = *reinterpret_cast<const uint2 *>(p + b0); }
+    __device__ __forceinline__ void ask(const bf16 *p, int a0, int b0) { a = tl::ld_cg(reinterpret_cast<const uint2 *>(p + a0)), b = tl::ld_cg(reinterpret_cast<const uint2 *>(p + b0)); }
     __device__ __forceinline__ void zero() { a = b = make_uint2(0, 0); }
     __device__ __forceinline__ void get(float (&x)[8]) const {
         const uint32_t w[4] = {a.x, a.y, b.x, b.y};
@@ -128,10 +129,15 @@ struct ApRow<bf16> {
 };
 template <>
 struct ApRow<float> {
-    float4 a, b;
-    __device__ __forceinline__ void load(const float *p, int a0, int b0) { a = *reinterpret_cast<const float4 *>(p + a0), b = *reinterpret_cast<const float4 *>(p + b0); }
-    __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
-    __device__ __forceinline__ void get(float (&x)[8]) const { x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w; }
+    uint4 a, b;
+    __device__ __forceinline__ void load(const float *p, int a0, int b0) { a = *reinterpret_cast<const uint4 *>(p + a0), b = *reinterpret_cast<const uint4 *>(p + b0); }
+    __device__ __forceinline__ void ask(const float *p, int a0, int b0) { a = tl::ld_cg(reinterpret_cast<const uint4 *>(p + a0)), b = tl::ld_cg(reinterpret_cast<const uint4 *>(p + b0)); }
+    __device__ __forceinline__ void zero() { a = b = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
+    }
 };
 
 // Where a lane's entries lie, and the pairs that they are: entries e and e + 4 (apart), or 2e and 2e + 1 of the eight.
@@ -261,7 +267,7 @@ __global__ void __launch_bounds__(kApThreads) fp8_append_kernel(const __grid_con
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = pg.dim, half = a.rot / 2, slot_row = warp * RW + lane / LP;
     const int b = blockIdx.z, h = blockIdx.y, G = a.group;
     const ApPlace at = ap_place(a, lane % LP);
-    const int ctx = a.lens[b];
+    const int ctx = tl::ld_cg(a.lens + b);
     T *q_out = static_cast<T *>(a.q_out) + (static_cast<size_t>(b) * a.tokens * a.heads + static_cast<size_t>(h) * G) * D;
     // an idle slot (or one whose length does not cover the step) appends nothing; its queries come out as zeros
     if (ctx < a.tokens || static_cast<long long>(ctx) > static_cast<long long>(a.max_pages) * pg.page_size) {
@@ -276,7 +282,7 @@ __global__ void __launch_bounds__(kApThreads) fp8_append_kernel(const __grid_con
     const int first = ctx - a.tokens, start = (first / kF8Tokens + blockIdx.x) * kF8Tokens;  // of the step, of this block
     const int p0 = max(start, first), n = min(start + kF8Tokens, ctx) - p0, l0 = p0 - first;
     if (n <= 0) return;
-    const int page = a.table[static_cast<size_t>(b) * a.max_pages + start / pg.page_size], slot = start % pg.page_size, kept = p0 - start;
+    const int page = tl::ld_cg(a.table + static_cast<size_t>(b) * a.max_pages + start / pg.page_size), slot = start % pg.page_size, kept = p0 - start;
     const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(pg.num_pages);
 
     // everything is asked for: keys, values, the first rows of queries (row r: token r / G, head r % G)
@@ -286,7 +292,7 @@ __global__ void __launch_bounds__(kApThreads) fp8_append_kernel(const __grid_con
 #pragma unroll
     for (int s = 0; s < PASSES; ++s) {
         const int i = s * ROWS + slot_row;
-        if (at.on && i < n) kr[s].load(k + i * a.k_l, at.a0, at.b0), vr[s].load(v + i * a.v_l, at.a0, at.b0);
+        if (at.on && i < n) kr[s].ask(k + i * a.k_l, at.a0, at.b0), vr[s].ask(v + i * a.v_l, at.a0, at.b0);
         else kr[s].zero(), vr[s].zero();
     }
     auto ask = [&](int r0) {
@@ -294,13 +300,13 @@ __global__ void __launch_bounds__(kApThreads) fp8_append_kernel(const __grid_con
         for (int s = 0; s < AHEAD; ++s) {
             const int r = r0 + s * ROWS + slot_row;
             const int l = f8_div(r, G, a.group_magic);
-            if (at.on && r < n * G) qr[s].load(q + l * a.q_l + (r - l * G) * a.q_h, at.a0, at.b0);
+            if (at.on && r < n * G) qr[s].ask(q + l * a.q_l + (r - l * G) * a.q_h, at.a0, at.b0);
             else qr[s].zero();
         }
     };
     ask(0);
     float before[2] = {0.f, 0.f};
-    if (there && kept) before[0] = pg.key_scales[f8_scale_at(pg, page, h, slot)], before[1] = pg.value_scales[f8_scale_at(pg, page, h, slot)];
+    if (there && kept) before[0] = tl::ld_cg(pg.key_scales + f8_scale_at(pg, page, h, slot)), before[1] = tl::ld_cg(pg.value_scales + f8_scale_at(pg, page, h, slot));
     __syncthreads();
     for (int i = threadIdx.x; i < n * half; i += kApThreads) {
         const int l = f8_div(i, half, a.half_magic);
@@ -382,7 +388,7 @@ __global__ void __launch_bounds__(kApThreads) fp8_append_any_kernel(const __grid
     const tlb_fp8_pages &pg = a.pages;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = pg.dim, half = a.rot / 2;
     const int b = blockIdx.z, h = blockIdx.y, G = a.group;
-    const int ctx = a.lens[b];
+    const int ctx = tl::ld_cg(a.lens + b);
     T *q_out = static_cast<T *>(a.q_out) + (static_cast<size_t>(b) * a.tokens * a.heads + static_cast<size_t>(h) * G) * D;
     // an idle slot (or one whose length does not cover the step) appends nothing; its queries come out as zeros
     if (ctx < a.tokens || static_cast<long long>(ctx) > static_cast<long long>(a.max_pages) * pg.page_size) {
@@ -415,10 +421,16 @@ __global__ void __launch_bounds__(kApThreads) fp8_append_any_kernel(const __grid
             float r = 1.f;
             if (w) {
                 float s = 0.f;
-                for (int d = lane; d < D; d += 32) s += to_f(x[d]) * to_f(x[d]);
+                for (int d = lane; d < D; d += 32) {
+                    const float u = to_f(tl::ld_cg(x + d));
+                    s += u * u;
+                }
                 r = 1.f / sqrtf(warp_sum(s) / D + a.q_eps);
             }
-            auto at = [&](int d) { return w ? to_f(x[d]) * r * to_f(w[d]) : to_f(x[d]); };
+            auto at = [&](int d) {
+                const float u = to_f(tl::ld_cg(x + d));
+                return w ? u * r * to_f(w[d]) : u;
+            };
             for (int j = lane; j < half; j += 32) {
                 const int2 e = ap_pair(a, j);
                 const float c = static_cast<float>(turn[j].x), s = static_cast<float>(turn[j].y), u = at(e.x), v = at(e.y);
@@ -436,10 +448,16 @@ __global__ void __launch_bounds__(kApThreads) fp8_append_any_kernel(const __grid
             double r = 1.0;
             if (w) {
                 double s = 0.0;
-                for (int d = lane; d < D; d += 32) s += static_cast<double>(to_f(x[d])) * to_f(x[d]);
+                for (int d = lane; d < D; d += 32) {
+                    const double u = to_f(tl::ld_cg(x + d));
+                    s += u * u;
+                }
                 r = 1.0 / sqrt(warp_sum_f64(s) / D + a.k_eps);
             }
-            auto at = [&](int d) { return w ? to_f(x[d]) * r * to_f(w[d]) : static_cast<double>(to_f(x[d])); };
+            auto at = [&](int d) {
+                const double u = to_f(tl::ld_cg(x + d));
+                return w ? u * r * to_f(w[d]) : u;
+            };
             for (int j = lane; j < half; j += 32) {
                 const int2 e = ap_pair(a, j);
                 const double u = at(e.x), v = at(e.y);
@@ -453,7 +471,7 @@ __global__ void __launch_bounds__(kApThreads) fp8_append_any_kernel(const __grid
         } else {
             const T *x = static_cast<const T *>(a.v) + b * a.v_b + h * a.v_h + (l0 + i) * a.v_l;
             for (int d = lane; d < D; d += 32) {
-                const float f = to_f(x[d]);
+                const float f = to_f(tl::ld_cg(x + d));
                 y[d] = f, m = f8_most(m, fabsf(f));
             }
         }
@@ -463,7 +481,7 @@ __global__ void __launch_bounds__(kApThreads) fp8_append_any_kernel(const __grid
     }
     __syncthreads();
 
-    const int page = a.table[static_cast<size_t>(b) * a.max_pages + start / pg.page_size], slot = start % pg.page_size;
+    const int page = tl::ld_cg(a.table + static_cast<size_t>(b) * a.max_pages + start / pg.page_size), slot = start % pg.page_size;
     if (page < 0 || page >= pg.num_pages) return;
     const int kept = p0 - start, pieces = D / 16;  // rows of earlier tokens, 16-byte pieces of a row
 #pragma unroll
@@ -472,7 +490,7 @@ __global__ void __launch_bounds__(kApThreads) fp8_append_any_kernel(const __grid
         for (int i = 0; i < n; ++i) m = f8_most(m, most[side][i]);
         float *scale_at = (side ? pg.value_scales : pg.key_scales) + f8_scale_at(pg, page, h, slot);
         uint8_t *rows = (side ? pg.values : pg.keys) + f8_row(pg, page, h, slot);
-        const float before = kept ? *scale_at : 0.f;
+        const float before = kept ? tl::ld_cg(scale_at) : 0.f;
         const bool fine = m < INFINITY;
         const float need = fine ? f8_power(f8_exponent(m)) : __int_as_float(0x7fffffff);
         const float scale = f8_most(need, before);  // NaN if either is

@@ -38,23 +38,30 @@ __device__ __forceinline__ float at_ex2(float x) {
 __device__ __forceinline__ void at_halves(uint32_t four, uint32_t &lo, uint32_t &hi) {  // four e4m3 numbers as f16
     asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(four));
 }
+// Everything that the launches in front may have written - queries, pages and their scales, table, lengths, pieces - is read through L2 (tl::ld_cg, asynchronous copies): this
+// launch becomes resident while they still run, and a line that its SM read meanwhile may be older than they are (eight blocks' scales share 32 bytes).
 // 8 entries of a query
 template <typename T>
 __device__ __forceinline__ void at_query(const T *q, bool wide, float (&x)[8]) {
-    if (wide) {
+    if (!wide) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const float4 v = load4(q + 4 * i);
-            x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
-        }
+        for (int e = 0; e < 8; ++e) x[e] = to_f(tl::ld_cg(q + e));
+    } else if constexpr (sizeof(T) == 2) {
+        const uint4 v = tl::ld_cg(reinterpret_cast<const uint4 *>(q));
+        const float2 y[4] = {tl::unpack2<bf16>(v.x), tl::unpack2<bf16>(v.y), tl::unpack2<bf16>(v.z), tl::unpack2<bf16>(v.w)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[2 * e] = y[e].x, x[2 * e + 1] = y[e].y;
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = to_f(q[e]);
+        for (int i = 0; i < 2; ++i) {
+            const uint4 v = tl::ld_cg(reinterpret_cast<const uint4 *>(q + 4 * i));
+            x[4 * i] = __uint_as_float(v.x), x[4 * i + 1] = __uint_as_float(v.y), x[4 * i + 2] = __uint_as_float(v.z), x[4 * i + 3] = __uint_as_float(v.w);
+        }
     }
 }
 
 __device__ __forceinline__ int at_context(const F8Attend &a, int b) {
-    return static_cast<int>(max(0LL, min(static_cast<long long>(a.lens[b]), static_cast<long long>(a.max_pages) * a.pages.page_size)));
+    return static_cast<int>(max(0LL, min(static_cast<long long>(tl::ld_cg(a.lens + b)), static_cast<long long>(a.max_pages) * a.pages.page_size)));
 }
 __device__ __forceinline__ int at_blocks(int context) { return (context + kF8Tokens - 1) / kF8Tokens; }
 

@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
     // the scale of block blk, NaN where its page is none
     auto block_at = [&](int blk, int &page) {
         const int at = page_at(blk);
-        page = table[at];
+        page = tl::ld_cg(table + at);
         return (static_cast<size_t>(page) * pg.heads + h) * a.page_blocks + (blk - at * a.page_blocks);
     };
 
@@ -172,17 +172,17 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
     uint4 raw[PER];  // the next tile's
     auto look_up = [&](int t) {
         const int blk = begin + t * (kPoKeys / kF8Tokens) + lane, at = page_at(blk);
-        const int page = lane < kPoKeys / kF8Tokens && blk < stop ? table[at] : -1;
+        const int page = lane < kPoKeys / kF8Tokens && blk < stop ? tl::ld_cg(table + at) : -1;
         place = static_cast<unsigned>(page) < static_cast<unsigned>(pg.num_pages) ? (page * pg.heads + h) * a.page_blocks + blk - at * a.page_blocks : -1;
     };
     auto ask = [&](int t) {  // of a page that is none: zeros
-        scale_next = place < 0 ? 0.f : __ldg(scales + place);
+        scale_next = place < 0 ? 0.f : tl::ld_cg(scales + place);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int at = __shfl_sync(0xffffffffu, place, (tid + 128 * i) / (kF8Tokens * CH));
             const size_t byte = static_cast<size_t>(static_cast<unsigned>(max(at, 0))) * (kF8Tokens * DIM);
             // the pieces before this thread's i-th that are not of its block
-            raw[i] = at >= 0 ? __ldg(reinterpret_cast<const uint4 *>(numbers + byte + (DIM == 128 ? 0 : -(tid / 64) * 1024))) : make_uint4(0, 0, 0, 0);
+            raw[i] = at >= 0 ? tl::ld_cg(reinterpret_cast<const uint4 *>(numbers + byte + (DIM == 128 ? 0 : -(tid / 64) * 1024))) : make_uint4(0, 0, 0, 0);
         }
     };
     if (warp >= 8 && warp < 16) look_up(0), ask(0), look_up(1);
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
         int page;
         const size_t at = block_at(blk, page);
         const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(pg.num_pages);
-        return make_float2(there ? __ldg(pg.key_scales + at) : NAN, there ? __ldg(pg.value_scales + at) : NAN);
+        return make_float2(there ? tl::ld_cg(pg.key_scales + at) : NAN, there ? tl::ld_cg(pg.value_scales + at) : NAN);
     };
     auto look_over = [&](float2 s) {  // whole warps
         const int k = __reduce_max_sync(0xffffffffu, s.x < INFINITY ? __float_as_int(s.x) : 0), v = __reduce_max_sync(0xffffffffu, s.y < INFINITY ? __float_as_int(s.y) : 0);
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
                     po_copy16(g_smem_u32(to), from + 64 * p, col < columns);
                 } else {
 #pragma unroll 1
-                    for (int e = 0; e < 8; ++e) reinterpret_cast<bf16 *>(to)[e] = col < columns ? from[64 * p + e] : __float2bfloat16_rn(0.f);
+                    for (int e = 0; e < 8; ++e) reinterpret_cast<bf16 *>(to)[e] = col < columns ? tl::ld_cg(from + 64 * p + e) : __float2bfloat16_rn(0.f);
                 }
             }
         }
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
                     int page;
                     const size_t at = block_at(key / kF8Tokens, page);
                     if (static_cast<unsigned>(page) >= static_cast<unsigned>(pg.num_pages)) hidden |= 1u << g;
-                    else if (key < limit && !(pg.key_scales[at] < INFINITY && pg.value_scales[at] < INFINITY)) sum = NAN;
+                    else if (key < limit && !(tl::ld_cg(pg.key_scales + at) < INFINITY && tl::ld_cg(pg.value_scales + at) < INFINITY)) sum = NAN;
                 }
             }
             uint32_t s[64];

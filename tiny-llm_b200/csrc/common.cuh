@@ -141,6 +141,11 @@ __device__ __forceinline__ uint4 ld_cg(const uint4 *p) {
     asm volatile("ld.global.cg.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p) : "memory");
     return r;
 }
+__device__ __forceinline__ uint2 ld_cg(const uint2 *p) {
+    uint2 r;
+    asm volatile("ld.global.cg.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p) : "memory");
+    return r;
+}
 __device__ __forceinline__ float ld_cg(const float *p) {
     float r;
     asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(r) : "l"(p) : "memory");
