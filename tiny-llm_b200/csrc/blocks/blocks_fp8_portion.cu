@@ -2,7 +2,8 @@
 //
 // The arithmetic is that of blocks_fp8_attention.cu; the operands of both products are f16 here too, so that nothing is lost ahead of the weights' rounding (2^-11):
 // a query row is brought to the top of f16's range by a power of two, keys and values are their e4m3 numbers times their block's scale over the largest
-// scale of the CTA's blocks - exact down to 2^-15 of that, and below it off by at most 2^-34 of the largest block's numbers.  A block whose
+// scale of the CTA's blocks, which is exact down to 2^-15 of that.  Where the CTA's scales lie further apart (keys' or values'), f16 would lose the small ones, also for rows that
+// see nothing of the large ones: then the operands are the numbers as they are, a tile is one block of 16 keys, and a row's own fp32 scores and weights take the scales.  A block whose
 // scale is no number counts as zeros in the products, and the rows that see it are made NaN at the end.
 //
 // A CTA takes 256 columns of one request and key/value head, or a piece of their keys, as two sets of 128 rows (tensor-memory lanes) that work on the same keys, so that one's
@@ -86,6 +87,9 @@ __device__ __forceinline__ void po_ld_wait(uint32_t *v) {  // what is read behin
     for (int i = 0; i < 64; ++i) asm volatile("" : "+r"(v[i]));
 }
 
+constexpr float kPoDeep = 90.f;  // log2: how far a row's unit may fall below the largest it has had: the outputs of 2^28 keys stay below 448 * 2^118
+constexpr int kPoApart = 15 << 23;  // the bits of a power of two are this much more than those of one 2^-15 of it: so far f16 holds both sides' numbers
+
 // kind::f16, f16 x f16 -> f32, 128 rows
 __host__ __device__ constexpr uint32_t po_idesc(int n, bool b_mn) { return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24); }
 
@@ -132,7 +136,7 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
     // keys [0, limit) are seen; a row behind the last one goes along with it
     auto limit_of = [&](int col) { return a.causal ? max(ctx - L + 1 + f8_div(min(col, columns - 1), G, a.group_magic), 0) : ctx; };
     const int end = min(limit_of(c0 + kPoRows - 1), ctx), begin = mine.piece * mine.size, stop = min((end + kF8Tokens - 1) / kF8Tokens, begin + mine.size);
-    const int first = begin * kF8Tokens, past = min(stop * kF8Tokens, end), n_tiles = max((past - first + kPoKeys - 1) / kPoKeys, 0);  // keys [first, past)
+    const int first = begin * kF8Tokens, past = min(stop * kF8Tokens, end);  // keys [first, past)
     const int32_t *table = a.table + static_cast<size_t>(b) * a.max_pages;
     auto page_at = [&](int blk) { return f8_div(blk, a.page_blocks, a.page_magic); };
     // the scale of block blk, NaN where its page is none
@@ -146,13 +150,14 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
     const uint32_t s_full = bar, p_full = bar + 32, pv_done = bar + 64, k_full = bar + 96, k_empty = bar + 128, v_full = bar + 160, v_empty = bar + 192, told = bar + 256;  // two of each, of the first three for either set, of the last for each softmax warp
     volatile int *dead = reinterpret_cast<volatile int *>(psm + Z::bar_off + 224);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(psm + Z::bar_off + 228);
-    int *seen = reinterpret_cast<int *>(psm + Z::bar_off + 232);  // largest scales of the CTA's blocks, keys' and values' (bits of positive numbers); whether a scale or page is none
+    // largest scales of the CTA's blocks, keys' and values' (bits of positive numbers); whether a scale or page is none; smallest scales
+    int *seen = reinterpret_cast<int *>(psm + Z::bar_off + 232);
     float *row_factor = reinterpret_cast<float *>(psm + Z::row_off), *shrink = row_factor + kPoRows;  // [2][kPoRows]
     if (threadIdx.x == 0) {
         for (int i = 0; i < 4; ++i) g_mbar_init(s_full + 8 * i, 1), g_mbar_init(p_full + 8 * i, 8), g_mbar_init(pv_done + 8 * i, 1);
         for (int i = 0; i < kPoStages; ++i) g_mbar_init(k_full + 8 * i, 4), g_mbar_init(k_empty + 8 * i, 2), g_mbar_init(v_full + 8 * i, 4), g_mbar_init(v_empty + 8 * i, 2);
         for (int i = 0; i < 16; ++i) g_mbar_init(told + 8 * i, 1);
-        *dead = 0, seen[0] = 0, seen[1] = 0, seen[2] = 0;
+        *dead = 0, seen[0] = 0, seen[1] = 0, seen[2] = 0, seen[3] = 0x7f7fffff, seen[4] = 0x7f7fffff;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 16) {
@@ -170,9 +175,10 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
     int place = -1;  // of a block among all pages' (fewer than 2^31: they are 16 rows each); -1: none
     float scale_next = 0.f;
     uint4 raw[PER];  // the next tile's
+    int step = kPoKeys / kF8Tokens;  // blocks of a tile
     auto look_up = [&](int t) {
-        const int blk = begin + t * (kPoKeys / kF8Tokens) + lane, at = page_at(blk);
-        const int page = lane < kPoKeys / kF8Tokens && blk < stop ? tl::ld_cg(table + at) : -1;
+        const int blk = begin + t * step + lane, at = page_at(blk);
+        const int page = lane < step && blk < stop ? tl::ld_cg(table + at) : -1;
         place = static_cast<unsigned>(page) < static_cast<unsigned>(pg.num_pages) ? (page * pg.heads + h) * a.page_blocks + blk - at * a.page_blocks : -1;
     };
     auto ask = [&](int t) {  // of a page that is none: zeros
@@ -194,9 +200,11 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
         return make_float2(there ? tl::ld_cg(pg.key_scales + at) : NAN, there ? tl::ld_cg(pg.value_scales + at) : NAN);
     };
     auto look_over = [&](float2 s) {  // whole warps
-        const int k = __reduce_max_sync(0xffffffffu, s.x < INFINITY ? __float_as_int(s.x) : 0), v = __reduce_max_sync(0xffffffffu, s.y < INFINITY ? __float_as_int(s.y) : 0);
-        if (lane == 0 && k > 0) atomicMax(seen, k);
-        if (lane == 0 && v > 0) atomicMax(seen + 1, v);
+        const int k = s.x < INFINITY ? __float_as_int(s.x) : 0, v = s.y < INFINITY ? __float_as_int(s.y) : 0;
+        const int k1 = __reduce_max_sync(0xffffffffu, k), v1 = __reduce_max_sync(0xffffffffu, v);
+        const int k0 = __reduce_min_sync(0xffffffffu, k > 0 ? k : 0x7f7fffff), v0 = __reduce_min_sync(0xffffffffu, v > 0 ? v : 0x7f7fffff);
+        if (lane == 0 && k1 > 0) atomicMax(seen, k1), atomicMin(seen + 3, k0);
+        if (lane == 0 && v1 > 0) atomicMax(seen + 1, v1), atomicMin(seen + 4, v0);
         if (!(s.x < INFINITY) || !(s.y < INFINITY)) seen[2] = 1;
     };
     float2 of_mine = make_float2(0.f, 0.f);
@@ -258,8 +266,11 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
     __syncthreads();
     g_tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    const bool apart = seen[0] - seen[3] > kPoApart || seen[1] - seen[4] > kPoApart;  // (without any scale: negative)
+    if (apart) step = 1;
+    const int n_tiles = max((past - first + step * kF8Tokens - 1) / (step * kF8Tokens), 0);
     // 1 over the largest scales; both are powers of two
-    const float top_k = seen[0] ? __int_as_float(seen[0]) : 1.f, top_v = seen[1] ? __int_as_float(seen[1]) : 1.f, under_k = 1.f / top_k, under_v = 1.f / top_v;
+    const float top_k = seen[0] && !apart ? __int_as_float(seen[0]) : 1.f, top_v = seen[1] && !apart ? __int_as_float(seen[1]) : 1.f, under_k = 1.f / top_k, under_v = 1.f / top_v;
 
     if (warp >= 20) {  // ---- rescaling: a quarter of the rows of both sets
         asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
@@ -328,6 +339,7 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
         }
     } else if (warp >= 8) {  // ---- pages to operands
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (apart) look_up(0), ask(0), look_up(1);  // of tiles of one block
         const float under = values ? under_v : under_k;
         unsigned char *tiles = psm + (values ? Z::v_off : Z::k_off);
         const uint32_t full = values ? v_full : k_full, empty = values ? v_empty : k_empty;
@@ -337,8 +349,8 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
         unsigned char *at = tiles + (c >> 2) * Z::kv_block + row0 * 128;
         unsigned char *one = at + (((2 * (c & 3) + odd) ^ (row0 & 7)) << 4), *two = at + (((2 * (c & 3) + 1 - odd) ^ (row0 & 7)) << 4);
         for (int t = 0; t < n_tiles; ++t) {
-            const int s = t & (kPoStages - 1), key0 = first + t * kPoKeys;
-            const __half2 r2 = __float2half2_rn(scale_next < INFINITY ? scale_next * under : 0.f);
+            const int s = t & (kPoStages - 1), key0 = first + t * step * kF8Tokens;
+            const __half2 r2 = __float2half2_rn(scale_next < INFINITY ? (apart ? 1.f : scale_next * under) : 0.f);
             const uint32_t ratio = *reinterpret_cast<const uint32_t *>(&r2);
             if (!tc_wait(empty + 8 * s, (t / kPoStages & 1) ^ 1u, dead)) break;  // the first pass through the stages does not wait
 #pragma unroll
@@ -363,9 +375,64 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
         const uint32_t lanes = (static_cast<uint32_t>((warp & 3) * 32) << 16) + set * kPoHalf;
         const float mult = fmaxf(fabsf(a.scale_log2) * row_factor[r] * top_k, 0x1p-126f);  // never 0: a masked score stays -inf
         const bool care = seen[2] != 0;
-        float m = -INFINITY, sum = 0.f;
+        float m = -INFINITY, sum = 0.f, back = 1.f;  // back: of the row's output, beside what it is divided by
         bool ok = true;
-        for (int t = 0; t < n_tiles; ++t) {
+        // Scales far apart.  A tile is a block: its key scale goes into the scores, its value scale into the weights, which are rounded over a unit of the row's own, 2^mo.  The unit follows the block's
+        // largest weight times scale, up and down, so no block takes anything from another one, nor from a row that does not see it (or gives it no weight).
+        if (apart) {
+            float mo = -INFINITY, highest = -INFINITY;
+            const float unit = fabsf(a.scale_log2) * row_factor[r];
+            for (int t = 0; t < n_tiles; ++t) {
+                const int key0 = first + t * kF8Tokens, s2 = t & 1;
+                if (!(ok = tc_wait(s_mine + 8 * s2, t >> 1 & 1, dead))) break;
+                g_tc_fence_after();
+                const uint32_t mine_s = tmem + lanes + s2 * kPoKeys;
+                int page;
+                const size_t at_block = block_at(key0 / kF8Tokens, page);
+                const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(pg.num_pages);
+                const float ks = there ? tl::ld_cg(pg.key_scales + at_block) : 0.f, vs = there ? tl::ld_cg(pg.value_scales + at_block) : 0.f;
+                const bool fine = ks < INFINITY && vs < INFINITY;
+                const int sees = there ? min(max(limit - key0, 0), kF8Tokens) : 0;  // keys of the block
+                if (sees > 0 && !fine) sum = NAN;
+                const float mult = fmaxf(unit * (fine ? ks : 0.f), 0x1p-126f), lift = fine ? log2f(vs) : -INFINITY;
+                uint32_t s[32], pk[16];
+                g_tmem_ld32(mine_s, s);
+                // scores are rounded ahead of the subtraction, as the maximum is: one of 2^28 would be 2^4 above its own maximum otherwise
+                float top = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < kF8Tokens; ++c) {
+                    const float x = __fmul_rn(__uint_as_float(s[c]), mult);
+                    s[c] = __float_as_uint(c < sees ? x : -INFINITY), top = c < sees ? fmaxf(top, x) : top;
+                }
+                if (top > m + kAtLag || (m == -INFINITY && top > m)) sum *= m == -INFINITY ? 1.f : at_ex2(m - top), m = top;
+                const float at = m == -INFINITY ? 0.f : m;
+                // weights below 2^-126 of the largest are none
+                const float most = ceilf(top - at < -126.f ? -INFINITY : top + lift), next = most == -INFINITY ? mo : fmaxf(most, highest - kPoDeep);
+                shrink[s2 * kPoRows + r] = mo == -INFINITY || next == mo ? 1.f : at_ex2(mo - next);  // without anything so far the output is 0
+                mo = next, highest = fmaxf(highest, mo);
+                __syncwarp();
+                if (lane == 0) g_mbar_arrive(told + 8 * (8 * s2 + warp));
+                const float by = most == -INFINITY ? -INFINITY : lift + (at - mo);
+#pragma unroll
+                for (int c = 0; c < 16; ++c) pk[c] = 0;
+#pragma unroll
+                for (int c = 0; c < kF8Tokens; c += 2) {
+                    const float x = __fsub_rn(__uint_as_float(s[c]), at), y = __fsub_rn(__uint_as_float(s[c + 1]), at);
+                    sum += at_ex2(x) + at_ex2(y);
+                    pk[c / 2] = tl::pack2<__half>(at_ex2(x + by), at_ex2(y + by));
+                }
+                po_st16(mine_s, pk);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) pk[c] = 0;
+                po_st16(mine_s + 16, pk);  // the tile's other keys
+                g_tmem_st_wait();
+                g_tc_fence_before();
+                __syncwarp();
+                if (lane == 0) g_mbar_arrive(p_mine + 8 * s2);
+            }
+            back = mo == -INFINITY ? 0.f : exp2f(0.5f * (mo - m));  // twice: the whole may be beyond fp32's range
+        }
+        for (int t = apart ? n_tiles : 0; t < n_tiles; ++t) {
             const int key0 = first + t * kPoKeys, s2 = t & 1;
             if (!(ok = tc_wait(s_mine + 8 * s2, t >> 1 & 1, dead))) break;
             g_tc_fence_after();
@@ -431,7 +498,7 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
         }
         const float verdict = tc_verdict(ok, dead) * top_v;
         const bool whole = mine.pieces == 1;
-        const float inv = (whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f) * verdict;
+        const float inv = (whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f) * verdict * back;
         float *part = whole ? nullptr : static_cast<float *>(a.workspace) + index * at_piece_floats(kPoRows, DIM);
         // Rows leave by way of the set's queries, whose products are through, a warp's 32 rows side by side: a warp stores whole rows that way, not 32 pieces of 16 bytes
         // (2048 tokens over 3500: 115 and 106 us, 128 tokens 34 and 28).  16-byte piece u of row i lies at u ^ (i & 7).
@@ -442,7 +509,7 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
                 uint32_t u[32];
                 g_tmem_ld32(tmem + lanes + kPoOut + i * 32, u);
 #pragma unroll
-                for (int c = 0; c < 32; ++c) o[c] = __uint_as_float(u[c]) * inv;
+                for (int c = 0; c < 32; ++c) o[c] = __uint_as_float(u[c]) * inv * back;
             } else {
 #pragma unroll
                 for (int c = 0; c < 32; ++c) o[c] = 0.f;
