@@ -427,7 +427,8 @@ typedef struct {
 int tlb_fp8_append(const tlb_fp8_pages *pages, const tlb_fp8_append_call *call, const int32_t *lens_host, const int32_t *table_host, void *stream);
 /* out [batch, tokens, heads, dim] = softmax(q k^T * scale) v over the first lens[b] slots of each request (the `tokens` newest among them); causal: new token i sees
  * lens[b] - tokens + i + 1 of them.  Rows that see nothing come out as zeros.  Products with the cache's numbers are exact, their sums, the softmax and the scales fp32;
- * weights are rounded to f16 (relative to the largest so far) for bf16 outputs, and use 22 bits for fp32 ones, whose queries do so too.  Few requests are divided
+ * weights are rounded to f16 for bf16 outputs (2^-11 of a weight or 2^-21 of the largest, whatever the scales of blocks that a row does not see or gives no weight, as long as scales are within 2^80
+ * of one another), and use 22 bits for fp32 ones, whose queries do so too.  Few requests are divided
  * among clusters of CTAs, and with a workspace long requests are cut into pieces, both by lens as it is when the launch runs (a captured one follows them): this decides the
  * order of sums.  Without a workspace (NULL) there are no pieces.  tlb_fp8_attention_workspace: its bytes, 0 where none would be used; lens_host: the lengths on the host, if
  * the launch is for these alone, by which the division is chosen; NULL: any lengths.  The workspace need not be initialised; calls that may run at once need one each.  lens_host, table_host: as for

@@ -134,5 +134,56 @@ def test_a_portions_visible_key_without_weight(lengths, new, heads, kv_heads, di
     check(attend(q, pages, table, lengths), q, pages, table, lengths, rows=list(range(0, new, 1 + new // 40)) + [new - 1])
 
 
+ROWS = [  # lengths, new, heads, kv_heads, dim: one item, clusters, whole items, pieces; 8 and 16 columns; every form of a head
+    ([100], 1, 8, 2, 128), ([1011], 1, 32, 8, 128), ([700] * 30, 1, 8, 8, 128), ([9000], 1, 8, 2, 128), ([5000, 16, 0, 40], 1, 8, 8, 64), ([300, 90], 4, 8, 2, 128), ([3000], 4, 8, 4, 64), ([260, 77], 3, 6, 2, 96),
+    ([400], 2, 4, 2, 256), ([120], 5, 10, 2, 80),
+]
+
+
+@pytest.mark.parametrize("lengths,new,heads,kv_heads,dim", ROWS)
+@pytest.mark.parametrize("apart", [3, 4, 5, 14, 20, 25, 40, 100])
+def test_a_decoded_tokens_visible_key_without_weight(lengths, new, heads, kv_heads, dim, apart):
+    gen = torch.Generator().manual_seed(apart + dim)
+    table, count = table_of(lengths, 32, 4)
+    pages = random_pages(count, kv_heads, 32, dim, gen, wide=0.0)
+    low = -9 if apart < 90 else -60
+    pages.value_scales.fill_(2.0**low)
+    q = (0.5 * torch.randn(len(lengths), heads, new, dim, generator=gen)).to(BF16)
+    q[..., 0] = 16.0
+    for b, n in enumerate(lengths):
+        for token in (0, n // 3, n - 20) if n > 40 else (n - 1,) if n else ():  # the first, one in the middle, one near the end
+            weightless(pages, table[b], token, low + apart)
+    check(attend(q, pages, table, lengths), q, pages, table, lengths)
+
+
+@pytest.mark.parametrize("lengths,new,heads,kv_heads,dim", [r for r in ROWS if r[1] > 1])
+@pytest.mark.parametrize("side", ["key_scales", "value_scales"])
+@pytest.mark.parametrize("apart", [4, 5, 16, 26, 40, 100])
+def test_few_tokens_that_do_not_see_a_large_block(lengths, new, heads, kv_heads, dim, side, apart):
+    """The last new token begins a block, whose scale is 2^apart times the others'."""
+    lengths = [n - n % 16 + 1 if n else 0 for n in lengths]
+    gen = torch.Generator().manual_seed(apart + dim)
+    table, count = table_of(lengths, 32, 5)
+    pages = random_pages(count, kv_heads, 32, dim, gen, wide=0.0)
+    low = -6 if apart < 90 else -60
+    getattr(pages, side).fill_(2.0**low)
+    for b, n in enumerate(lengths):
+        if n:
+            scale_block(pages, table[b], n - 1, low + apart, side)
+    q = (0.5 * torch.randn(len(lengths), heads, new, dim, generator=gen)).to(BF16)
+    check(attend(q, pages, table, lengths), q, pages, table, lengths)
+
+
+@pytest.mark.parametrize("lengths,new,heads,kv_heads,dim", ROWS)
+@pytest.mark.parametrize("wide", [2.0, 10.0, 30.0])
+def test_few_tokens_over_scales_of_every_size(lengths, new, heads, kv_heads, dim, wide):
+    gen = torch.Generator().manual_seed(int(wide) + dim)
+    table, count = table_of(lengths, 32, 6)
+    pages = random_pages(count, kv_heads, 32, dim, gen, wide=0.0)
+    pages.value_scales.copy_(torch.exp2(torch.round(wide * torch.randn(pages.value_scales.shape, generator=gen)).clamp(-99, 99)))
+    q = (0.5 * torch.randn(len(lengths), heads, new, dim, generator=gen)).to(BF16)
+    check(attend(q, pages, table, lengths), q, pages, table, lengths)
+
+
 def test_nobody_gave_up():
     assert blocks.library().tlb_tc_gave_up() == 0

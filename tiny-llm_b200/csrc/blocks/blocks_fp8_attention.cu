@@ -3,9 +3,9 @@
 // The products run on mma.sync (m16n8k16, f16 in, fp32 out) with the cache as the first operand: 16 keys (a block, so one scale of either side) times 8 columns, a
 // column being one (query head of the group, new token).  An e4m3 number is an f16 number, so the cache's side is exact; a column is brought to the top of
 // f16's range by a power of two, where bf16 keeps all its bits, and an fp32 query is two such terms.  A block's key scale multiplies its scores in fp32; its value
-// scale multiplies its weights, over the largest value scale so far (fp32 outputs: the product of weights and values).  Weights are exp2 of a number up to the
-// column's running maximum (which may lag behind by 2^15 before the sums are scaled again), rounded to f16 for the second product: 2^-11 of a weight, where an output is
-// rounded to 2^-9 of itself; fp32 outputs take a second term for the rest.  Running sums are fp32.
+// scale multiplies its weights, over a unit of the column's own (kAtNear; fp32 outputs: the product of weights and values).  Weights are exp2 of a number up to the
+// column's running maximum (which may lag behind by 2^15 before the sums are scaled again), rounded to f16 for the second product: 2^-11 of a weight or 2^-21 of the largest, where an
+// output is rounded to 2^-8 of itself; fp32 outputs take a second term for the rest.  Running sums are fp32.
 //
 // A warp takes blocks of 16 keys through a ring of its own in shared memory, filled by asynchronous copies, two blocks ahead of the one it works on; it waits for nobody
 // else.  Lane (g, t) reads 16-byte pieces t, t + 4 .. of key rows g and g + 8, and of the value rows 2t, 2t + 1, 2t + 8, 2t + 9 the g-th eighth: which entry of a head a product's
@@ -48,7 +48,15 @@ __device__ __forceinline__ float2 at_rest(uint32_t two, float lo, float hi) {  /
     return make_float2(lo - f.x, hi - f.y);
 }
 
+// 1 over a power of two of 2^-126 to 2^126; one over the next one above what is none.  (A division would be a call: 0.7 us of 6 for one request of 1011 tokens.)
+__device__ __forceinline__ float at_under(float v) { return __int_as_float(0x7f000000 - ((__float_as_int(v) + 0x7fffff) & 0x7f800000)); }
+
 constexpr int kAtWarps = 8, kAtStages = 3;
+// bf16 outputs.  A column's weights take the block's value scale, over a unit of the column's own, ahead of their rounding to f16, whose smallest step is 2^-24.  The unit is the scale of one of the
+// column's blocks; it goes up to a larger one, and down to one of less than 1 / 16 of it, so a weight's error is 2^-11 of itself or 2^-21 of the largest weight.  Blocks that a column does not see, or
+// gives no weight, leave its unit alone.  It falls to 2^-80 of the highest it has had, so that the sums stay within fp32's range.
+constexpr float kAtNear = 0.0625f, kAtDeep = 0x1p-80f;
+constexpr float kAtUnder = 0x1p-20f;  // sums leave a warp times this: scales of 2^-100 to 2^119 stay within fp32's range
 
 __device__ __forceinline__ void at_copy16(uint32_t to, const void *from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
 
@@ -226,7 +234,9 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
         for (int e = 0; e < 2; ++e) m_run[nt][e] = -INFINITY, l_run[nt][e] = 0.f;
     }
 
-    float vs_most = 0.f, under = 0.f;  // the largest value scale so far, and 1 over it
+    float over[NT][2], highest = 0.f;  // 1 over the columns' units (nothing so far: a power of two above all); the largest unit of this lane's columns
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) over[nt][0] = over[nt][1] = 0x1p126f;
     for (int i = 0, stage = 0; i < count; ++i) {
         const int key0 = (begin_warp + i) * kF8Tokens, in_32 = i & 31, ahead = i + kAtStages - 1;
         asm volatile("cp.async.wait_group %0;" ::"n"(kAtStages - 2) : "memory");
@@ -301,23 +311,13 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sc[nt][e] += sd[nt][e];
         }
-        if (!kTwo && scales.y > vs_most) {  // the sums so far are over the smaller scale
-            const float by = vs_most / scales.y;
-            vs_most = scales.y, under = 1.f / scales.y;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int j = 0; j < J; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[nt][j][e] *= by;
-        }
         // scaled to log2, masked scores -inf whatever the factor (which may be no number, 0 or negative)
         float f[NT][2], x[NT][4], vs[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                f[nt][e] = factor[nt][e] * scales.x, vs[nt][e] = kTwo ? scales.y : scales.y * under;
+                f[nt][e] = factor[nt][e] * scales.x, vs[nt][e] = kTwo ? scales.y : scales.y * over[nt][e];
                 x[nt][e] = sc[nt][e] * f[nt][e], x[nt][2 + e] = sc[nt][2 + e] * f[nt][e];
             }
         if (key0 + kF8Tokens > low) {
@@ -341,7 +341,10 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) grow |= fmaxf(x[nt][e], x[nt][2 + e]) > m_run[nt][e] + kAtLag;
+            for (int e = 0; e < 2; ++e) {
+                grow |= fmaxf(x[nt][e], x[nt][2 + e]) > m_run[nt][e] + kAtLag;
+                if constexpr (!kTwo) grow |= static_cast<unsigned>(__float_as_int(vs[nt][e]) - __float_as_int(kAtNear)) > static_cast<unsigned>(__float_as_int(1.f) - __float_as_int(kAtNear));  // not of 1 / 16 to 1
+            }
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -350,11 +353,23 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
                     float m = fmaxf(x[nt][e], x[nt][2 + e]);
 #pragma unroll
                     for (int w = 4; w < 32; w <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+                    const float top = m;  // of this block
                     m = fmaxf(m, m_run[nt][e]);
                     const float alpha = m == m_run[nt][e] ? 1.f : at_ex2(m_run[nt][e] - m);
                     m_run[nt][e] = m, l_run[nt][e] *= alpha;
+                    float by = alpha;
+                    if constexpr (!kTwo) {
+                        if (vs[nt][e] > 1.f || (vs[nt][e] < kAtNear && vs[nt][e] > 0.f)) {
+                            if (top - m < -126.f) {
+                                vs[nt][e] = 0.f;  // none of its weights is a number of fp32
+                            } else {
+                                const float unit = fminf(fmaxf(scales.y, highest * kAtDeep), 0x1p126f), next = at_under(unit);
+                                by *= next * at_under(over[nt][e]), over[nt][e] = next, vs[nt][e] = scales.y * next, highest = fmaxf(highest, unit);
+                            }
+                        }
+                    }
 #pragma unroll
-                    for (int j = 0; j < J; ++j) o[nt][j][e] *= alpha, o[nt][j][2 + e] *= alpha;
+                    for (int j = 0; j < J; ++j) o[nt][j][e] *= by, o[nt][j][2 + e] *= by;
                 }
         }
         uint32_t p[NT][2], pl[kTwo ? NT : 1][2];
@@ -414,13 +429,14 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
             const int col = 8 * nt + 2 * t + e;
-            if (g == 0) part_m[warp * COLS + col] = m_run[nt][e], part_l[warp * COLS + col] = l;
+            if (g == 0) part_m[warp * COLS + col] = m_run[nt][e], part_l[warp * COLS + col] = kTwo ? l : l * kAtUnder;
+            const float unit = kAtUnder * at_under(over[nt][e]);
             if (col < live) {
                 float4 *to = reinterpret_cast<float4 *>(part + (warp * COLS + col) * ROW + g * (DP / 8));
 #pragma unroll
                 for (int j = 0; j < J; j += 2)
                     to[j / 2] = kTwo ? make_float4(o[nt][j][e], o[nt][j][2 + e], o[nt][j + 1][e], o[nt][j + 1][2 + e])
-                                     : make_float4(o[nt][j][e] * vs_most, o[nt][j][2 + e] * vs_most, o[nt][j + 1][e] * vs_most, o[nt][j + 1][2 + e] * vs_most);
+                                     : make_float4(o[nt][j][e] * unit, o[nt][j][2 + e] * unit, o[nt][j + 1][e] * unit, o[nt][j + 1][2 + e] * unit);
             }
         }
     __syncthreads();
