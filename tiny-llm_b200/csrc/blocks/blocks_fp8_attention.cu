@@ -237,6 +237,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
     float over[NT][2], highest = 0.f;  // 1 over the columns' units (nothing so far: a power of two above all); the largest unit of this lane's columns
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) over[nt][0] = over[nt][1] = 0x1p126f;
+    bool strong = false;  // fp32: scores beyond 2^24 were met, which are rounded as their maxima are from then on: what that rounding left would put them above these
     for (int i = 0, stage = 0; i < count; ++i) {
         const int key0 = (begin_warp + i) * kF8Tokens, in_32 = i & 31, ahead = i + kAtStages - 1;
         asm volatile("cp.async.wait_group %0;" ::"n"(kAtStages - 2) : "memory");
@@ -318,7 +319,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 f[nt][e] = factor[nt][e] * scales.x, vs[nt][e] = kTwo ? scales.y : scales.y * over[nt][e];
-                x[nt][e] = sc[nt][e] * f[nt][e], x[nt][2 + e] = sc[nt][2 + e] * f[nt][e];
+                x[nt][e] = __fmul_rn(sc[nt][e], f[nt][e]), x[nt][2 + e] = __fmul_rn(sc[nt][2 + e], f[nt][e]);
             }
         if (key0 + kF8Tokens > low) {
 #pragma unroll
@@ -354,6 +355,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
 #pragma unroll
                     for (int w = 4; w < 32; w <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
                     const float top = m;  // of this block
+                    if constexpr (kTwo) strong |= fabsf(m) > 0x1p24f && m > -INFINITY;
                     m = fmaxf(m, m_run[nt][e]);
                     const float alpha = m == m_run[nt][e] ? 1.f : at_ex2(m_run[nt][e] - m);
                     m_run[nt][e] = m, l_run[nt][e] *= alpha;
@@ -371,6 +373,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
 #pragma unroll
                     for (int j = 0; j < J; ++j) o[nt][j][e] *= by, o[nt][j][2 + e] *= by;
                 }
+            if constexpr (kTwo) strong = __any_sync(0xffffffffu, strong);
         }
         uint32_t p[NT][2], pl[kTwo ? NT : 1][2];
 #pragma unroll
@@ -382,7 +385,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float u = x[nt][2 * i + e], s = sc[nt][2 * i + e];
-                    if constexpr (kTwo) w[2 * i + e] = exp2f(u == -INFINITY ? u : fmaf(s, f[nt][e], fmaf(s, rest[nt][e] * scales.x, -m)));
+                    if constexpr (kTwo) w[2 * i + e] = exp2f(u == -INFINITY ? u : strong ? u - m : fmaf(s, f[nt][e], fmaf(s, rest[nt][e] * scales.x, -m)));
                     else w[2 * i + e] = at_ex2(u - m);
                 }
                 l_run[nt][e] += w[e] + w[2 + e];

@@ -3,7 +3,7 @@
 // The arithmetic is that of blocks_fp8_attention.cu; the operands of both products are f16 here too, so that nothing is lost ahead of the weights' rounding (2^-11):
 // a query row is brought to the top of f16's range by a power of two, keys and values are their e4m3 numbers times their block's scale over the largest
 // scale of the CTA's blocks, which is exact down to 2^-15 of that.  Where the CTA's scales lie further apart (keys' or values'), f16 would lose the small ones, also for rows that
-// see nothing of the large ones: then the operands are the numbers as they are, a tile is one block of 16 keys, and a row's own fp32 scores and weights take the scales.  A block whose
+// see nothing of the large ones; where scores may pass 2^23, weights would be above f16's largest number.  Then the operands are the numbers as they are, a tile is one block of 16 keys, and a row's own fp32 scores and weights take the scales.  A block whose
 // scale is no number counts as zeros in the products, and the rows that see it are made NaN at the end.
 //
 // A CTA takes 256 columns of one request and key/value head, or a piece of their keys, as two sets of 128 rows (tensor-memory lanes) that work on the same keys, so that one's
@@ -150,14 +150,14 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
     const uint32_t s_full = bar, p_full = bar + 32, pv_done = bar + 64, k_full = bar + 96, k_empty = bar + 128, v_full = bar + 160, v_empty = bar + 192, told = bar + 256;  // two of each, of the first three for either set, of the last for each softmax warp
     volatile int *dead = reinterpret_cast<volatile int *>(psm + Z::bar_off + 224);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(psm + Z::bar_off + 228);
-    // largest scales of the CTA's blocks, keys' and values' (bits of positive numbers); whether a scale or page is none; smallest scales
+    // largest scales of the CTA's blocks, keys' and values' (bits of positive numbers); whether a scale or page is none; smallest scales; the largest factor of a row
     int *seen = reinterpret_cast<int *>(psm + Z::bar_off + 232);
     float *row_factor = reinterpret_cast<float *>(psm + Z::row_off), *shrink = row_factor + kPoRows;  // [2][kPoRows]
     if (threadIdx.x == 0) {
         for (int i = 0; i < 4; ++i) g_mbar_init(s_full + 8 * i, 1), g_mbar_init(p_full + 8 * i, 8), g_mbar_init(pv_done + 8 * i, 1);
         for (int i = 0; i < kPoStages; ++i) g_mbar_init(k_full + 8 * i, 4), g_mbar_init(k_empty + 8 * i, 2), g_mbar_init(v_full + 8 * i, 4), g_mbar_init(v_empty + 8 * i, 2);
         for (int i = 0; i < 16; ++i) g_mbar_init(told + 8 * i, 1);
-        *dead = 0, seen[0] = 0, seen[1] = 0, seen[2] = 0, seen[3] = 0x7f7fffff, seen[4] = 0x7f7fffff;
+        *dead = 0, seen[0] = 0, seen[1] = 0, seen[2] = 0, seen[3] = 0x7f7fffff, seen[4] = 0x7f7fffff, seen[5] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 16) {
@@ -258,7 +258,10 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
                 f.z = tl::pack2<__half>(y[2].x * times, y[2].y * times), f.w = tl::pack2<__half>(y[3].x * times, y[3].y * times);
                 *reinterpret_cast<uint4 *>(to + p * Z::q_block) = f;
             }
-            if (j == 0) row_factor[row] = f8_power(-up);
+            if (j == 0) {
+                row_factor[row] = f8_power(-up);
+                if (e2 != 255) atomicMax(seen + 5, __float_as_int(f8_power(-up)));
+            }
         }
         g_fence_proxy_async();
     }
@@ -266,7 +269,9 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
     __syncthreads();
     g_tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const bool apart = seen[0] - seen[3] > kPoApart || seen[1] - seen[4] > kPoApart;  // (without any scale: negative)
+    // (without any scale: negative); or scores may reach 2^23, where they could come to be half above their own rounded maxima (2^15.5 as a weight): a product is at most 2^14 * 448 for each entry
+    const bool apart = seen[0] - seen[3] > kPoApart || seen[1] - seen[4] > kPoApart ||
+                       fabsf(a.scale_log2) * __int_as_float(seen[5]) * __int_as_float(seen[0]) > 0x1p23f / (0x1p14f * 448.f * DIM);
     if (apart) step = 1;
     const int n_tiles = max((past - first + step * kF8Tokens - 1) / (step * kF8Tokens), 0);
     // 1 over the largest scales; both are powers of two
@@ -397,7 +402,7 @@ __global__ void __launch_bounds__(kPoThreads, 1) fp8_portion_kernel(const __grid
                 const float mult = fmaxf(unit * (fine ? ks : 0.f), 0x1p-126f), lift = fine ? log2f(vs) : -INFINITY;
                 uint32_t s[32], pk[16];
                 g_tmem_ld32(mine_s, s);
-                // scores are rounded ahead of the subtraction, as the maximum is: one of 2^28 would be 2^4 above its own maximum otherwise
+                // scores are rounded ahead of the subtraction, as the maximum is: one of 2^28 could be 2^4 above it otherwise
                 float top = -INFINITY;
 #pragma unroll
                 for (int c = 0; c < kF8Tokens; ++c) {
