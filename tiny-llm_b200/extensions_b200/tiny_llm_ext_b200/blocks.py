@@ -1189,8 +1189,9 @@ class Fp8Pages(ctypes.Structure):
 
 
 _EINVAL, _EWORKSPACE = -1, -3
-# tlb_fp8_append_call and tlb_fp8_attention_call, packed at once: of small calls the host sets the pace, and ctypes converts two dozen arguments one by one
-_FP8_APPEND = struct.Struct("@PPPPPPPPqqqqqqqqqdffiiiiiii")
+# tlb_fp8_append_call and tlb_fp8_attention_call, packed at once (to the structure's last byte, 0P: the library copies it whole): of small calls the host sets the pace, and ctypes converts
+# two dozen arguments one by one
+_FP8_APPEND = struct.Struct("@PPPPPPPPqqqqqqqqqdffiiiiiii0P")
 _FP8_ATTENTION = struct.Struct("@PPPPqqqdiiiiii")
 
 
