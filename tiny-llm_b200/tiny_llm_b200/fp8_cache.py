@@ -302,12 +302,16 @@ def append_step(slots: list, query, key, value, *, rope=None, query_norm=None, k
             room = s.page_size - s.page_lens[-1] if s.page_ids else 0
             pool.ensure_room(max(0, -(-(count - room) // s.page_size)), heads, dim, key.device)
             s.append_slots(count)
-        table = np.full((len(slots), max(s.num_pages for s in live)), -1, dtype=np.int32)
-        lens = np.zeros(len(slots), dtype=np.int32)
+        # table and lengths side by side: one copy, which nobody waits for (the host would else wait for the device in every layer)
+        width = max(s.num_pages for s in live)
+        both = np.full((width + 1) * len(slots), -1, dtype=np.int32)
+        table, lens = both[: width * len(slots)].reshape(len(slots), width), both[width * len(slots) :]
+        lens[:] = 0
         for b, s in enumerate(slots):
             if s is not None:
                 table[b, : s.num_pages], lens[b] = s.page_ids, s.offset
-        meta = Fp8KvMetadata(pool.pages, torch.from_numpy(table).to(key.device), torch.from_numpy(lens).to(key.device), table, lens)
+        there = torch.from_numpy(both).to(key.device, non_blocking=True)
+        meta = Fp8KvMetadata(pool.pages, there[: width * len(slots)].view(len(slots), width), there[width * len(slots) :], table, lens)
         out = rotate_append_fp8(query, key, value, pool.pages, meta.block_table, meta.context_lens, rope=rope, query_norm=query_norm, key_norm=key_norm, block_table_host=table,
                                 context_lens_host=lens)
     except Exception:
