@@ -265,7 +265,12 @@ class Fp8KvPagedPool(TinyKvPagedPool):
 
 
 class Fp8KvPagedCache(TinyKvPagedCache):
-    """A request's pages in an ``Fp8KvPagedPool``."""
+    """A request's pages in an ``Fp8KvPagedPool``.
+
+    ``rewind`` to the beginning of a block of 16 tokens, or of the request, leaves nothing of the dropped tokens.  Inside a block it is bookkeeping alone, and a rewind of
+    16 bits' caches is more than that: the block keeps the scale that the dropped tokens made it take, and the numbers of the tokens that stay are rounded to it, as if all had come
+    together.  So a dropped token far larger than these costs them their small bits (or all of them), and a dropped infinity or NaN makes the block's numbers none for good:
+    ``rewind`` further then, to the block's beginning, and append what it held again."""
 
     def __init__(self, pool: Fp8KvPagedPool):
         if not isinstance(pool, Fp8KvPagedPool):
