@@ -3,8 +3,8 @@
 // The products run on mma.sync (m16n8k16, f16 in, fp32 out) with the cache as the first operand: 16 keys (a block, so one scale of either side) times 8 columns, a
 // column being one (query head of the group, new token).  An e4m3 number is an f16 number, so the cache's side is exact; a column is brought to the top of
 // f16's range by a power of two, where bf16 keeps all its bits, and an fp32 query is two such terms.  A block's key scale multiplies its scores in fp32; its value
-// scale multiplies its weights, over a unit of the column's own (kAtNear; fp32 outputs: the product of weights and values).  Weights are exp2 of a number up to the
-// column's running maximum (which may lag behind by 2^15 before the sums are scaled again), rounded to f16 for the second product: 2^-11 of a weight or 2^-21 of the largest, where an
+// scale multiplies its weights, over a unit of the column's own (kAtLow; fp32 outputs: the product of weights and values).  Weights are exp2 of a number up to the
+// column's running maximum (which may lag behind by 2^12 before the sums are scaled again), rounded to f16 for the second product: 2^-11 of a weight or 2^-21 of the largest, where an
 // output is rounded to 2^-8 of itself; fp32 outputs take a second term for the rest.  Running sums are fp32.
 //
 // A warp takes blocks of 16 keys through a ring of its own in shared memory, filled by asynchronous copies, two blocks ahead of the one it works on; it waits for nobody
@@ -53,9 +53,10 @@ __device__ __forceinline__ float at_under(float v) { return __int_as_float(0x7f0
 
 constexpr int kAtWarps = 8, kAtStages = 3;
 // bf16 outputs.  A column's weights take the block's value scale, over a unit of the column's own, ahead of their rounding to f16, whose smallest step is 2^-24.  The unit is the scale of one of the
-// column's blocks; it goes up to a larger one, and down to one of less than 1 / 16 of it, so a weight's error is 2^-11 of itself or 2^-21 of the largest weight.  Blocks that a column does not see, or
-// gives no weight, leave its unit alone.  It falls to 2^-80 of the highest it has had, so that the sums stay within fp32's range.
-constexpr float kAtNear = 0.0625f, kAtDeep = 0x1p-80f;
+// column's blocks; it moves to one of more than 8 times as much (a weight of up to 2^12 is an f16 number then) or of less than 1 / 16 of it, so a weight's error is 2^-11 of itself or 2^-21 of the
+// largest weight.  Blocks that a column does not see, or gives no weight, leave its unit alone.  It falls to 2^-80 of the highest it has had, so that the sums stay within fp32's range.
+constexpr float kAtLow = 0.0625f, kAtHigh = 8.f, kAtDeep = 0x1p-80f;
+constexpr float kAtRowLag = 12.f;  // log2: how far a running maximum may lag behind here
 constexpr float kAtUnder = 0x1p-20f;  // sums leave a warp times this: scales of 2^-100 to 2^119 stay within fp32's range
 
 __device__ __forceinline__ void at_copy16(uint32_t to, const void *from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
@@ -338,15 +339,16 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
                         for (int w = 0; w < DP / 32; ++w) v[i][w] = 0;
             }
         }
-        bool grow = false;
+        bool grow = false, move = false;  // of maxima; of units
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                grow |= fmaxf(x[nt][e], x[nt][2 + e]) > m_run[nt][e] + kAtLag;
-                if constexpr (!kTwo) grow |= static_cast<unsigned>(__float_as_int(vs[nt][e]) - __float_as_int(kAtNear)) > static_cast<unsigned>(__float_as_int(1.f) - __float_as_int(kAtNear));  // not of 1 / 16 to 1
+                grow |= fmaxf(x[nt][e], x[nt][2 + e]) > m_run[nt][e] + kAtRowLag;
+                if constexpr (!kTwo) move |= static_cast<unsigned>(__float_as_int(vs[nt][e]) - __float_as_int(kAtLow)) > static_cast<unsigned>(__float_as_int(kAtHigh) - __float_as_int(kAtLow));
             }
-        if (__any_sync(0xffffffffu, grow)) {
+        if (__any_sync(0xffffffffu, grow | move)) {
+            float by[NT][2], top[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -354,26 +356,45 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
                     float m = fmaxf(x[nt][e], x[nt][2 + e]);
 #pragma unroll
                     for (int w = 4; w < 32; w <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
-                    const float top = m;  // of this block
+                    top[nt][e] = m, m = fmaxf(m, m_run[nt][e]);
+                    by[nt][e] = m == m_run[nt][e] ? 1.f : at_ex2(m_run[nt][e] - m);
+                    m_run[nt][e] = m, l_run[nt][e] *= by[nt][e];
                     if constexpr (kTwo) strong |= fabsf(m) > 0x1p24f && m > -INFINITY;
-                    m = fmaxf(m, m_run[nt][e]);
-                    const float alpha = m == m_run[nt][e] ? 1.f : at_ex2(m_run[nt][e] - m);
-                    m_run[nt][e] = m, l_run[nt][e] *= alpha;
-                    float by = alpha;
-                    if constexpr (!kTwo) {
-                        if (vs[nt][e] > 1.f || (vs[nt][e] < kAtNear && vs[nt][e] > 0.f)) {
-                            if (top - m < -126.f) {
+                }
+            if (!kTwo && __any_sync(0xffffffffu, move)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        if (vs[nt][e] > kAtHigh || (vs[nt][e] < kAtLow && vs[nt][e] > 0.f)) {
+                            if (top[nt][e] - m_run[nt][e] < -126.f) {
                                 vs[nt][e] = 0.f;  // none of its weights is a number of fp32
                             } else {
                                 const float unit = fminf(fmaxf(scales.y, highest * kAtDeep), 0x1p126f), next = at_under(unit);
-                                by *= next * at_under(over[nt][e]), over[nt][e] = next, vs[nt][e] = scales.y * next, highest = fmaxf(highest, unit);
+                                by[nt][e] *= next * at_under(over[nt][e]), over[nt][e] = next, vs[nt][e] = scales.y * next, highest = fmaxf(highest, unit);
                             }
                         }
-                    }
+            }
 #pragma unroll
-                    for (int j = 0; j < J; ++j) o[nt][j][e] *= by, o[nt][j][2 + e] *= by;
-                }
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[nt][j][e] *= by[nt][e & 1];
             if constexpr (kTwo) strong = __any_sync(0xffffffffu, strong);
+        }
+        float left[NT][2];
+        if constexpr (kTwo) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) left[nt][e] = rest[nt][e] * scales.x;
+            if (strong) {  // the rounded scores themselves
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sc[nt][e] = x[nt][e], f[nt][e & 1] = 1.f, left[nt][e & 1] = 0.f;
+            }
         }
         uint32_t p[NT][2], pl[kTwo ? NT : 1][2];
 #pragma unroll
@@ -385,7 +406,7 @@ __global__ void __launch_bounds__(kAtWarps * 32, DP <= 128 && NT == 1 && sizeof(
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float u = x[nt][2 * i + e], s = sc[nt][2 * i + e];
-                    if constexpr (kTwo) w[2 * i + e] = exp2f(u == -INFINITY ? u : strong ? u - m : fmaf(s, f[nt][e], fmaf(s, rest[nt][e] * scales.x, -m)));
+                    if constexpr (kTwo) w[2 * i + e] = exp2f(u == -INFINITY ? u : fmaf(s, f[nt][e], fmaf(s, left[nt][e], -m)));
                     else w[2 * i + e] = at_ex2(u - m);
                 }
                 l_run[nt][e] += w[e] + w[2 + e];
