@@ -12,9 +12,9 @@
 // A CTA takes one block of one request and key/value head, with the group's query heads: the angles of its at most 16 tokens are made once, in
 // shared memory.  A row goes to 8, 16 or 32 lanes; a lane holds four entries of either half of the rotated part, which are each other's partners, or eight of the
 // rest.  Everything is asked for at the start; keys and values stay in registers until the block's largest magnitude is known.
-// fp8_append_any_kernel takes what that cannot: rows that do not begin on 16 bytes, rotations of dimensions that are no multiple of 8 (2048 tokens of 32 + 8 heads 59 us for 22).
+// fp8_append_any_kernel takes what that cannot: rows that do not begin on 16 bytes, rotations of dimensions that are no multiple of 8 (2048 tokens of 32 + 8 heads 59 us for 23).
 //
-// 1 token of 32 + 8 heads of 128 takes 4.3 us: a launch, length, table, rows and angles, one latency behind another.  128 tokens 6.9, 64 requests of one 5.7.  2048 tokens take 22.4 us (46 MB, 2.1 TB/s):
+// 1 token of 32 + 8 heads of 128 takes 4.3 us: a launch, length, table, rows and angles, one latency behind another.  128 tokens 6.9, 64 requests of one 6.2.  2048 tokens take 22.9 us (46 MB, 2.0 TB/s):
 // instructions, 72 % of the issue slots, of which angles for every key/value head are a fourth.  One set of angles for two or four heads took 115 registers for 64 and 24 us at the best.
 #include <math.h>
 

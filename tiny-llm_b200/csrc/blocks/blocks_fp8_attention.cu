@@ -16,8 +16,9 @@
 // requests are of unlike length or very long, a CTA takes a piece of one, which leaves a partial result for fp8_attend_join_kernel to add up in order.  Both follow the lengths
 // on the device, so a captured launch does.  attend_plan chooses.
 //
-// 64 requests of 8192 (1.08 GB) take 159 us, 6.8 TB/s: HBM.  With fewer, a block is a chain of latencies (1100 cycles of a warp: copies, eight products, exponentials, eight products), so an item of 1970 tokens
-// takes 10 us of the 17 of a step of 24 requests.  Not faster: 16 warps a CTA (24 requests 14.8 us, but 30 of 1000 tokens 18.7 for 14.2), rings of six blocks.
+// 64 requests of 8192 (1.08 GB) take 160 us in replays over the same pages (some of which stay in L2), 175 over others, 6.2 TB/s: HBM.  With fewer, a block is a chain of latencies (1100 cycles of a warp: copies, eight products, exponentials, eight products), so an item of 1970 tokens
+// takes 10 us of the 17 of a step of 24 requests.  Not faster: 16 warps a CTA (24 requests 14.8 us, but 30 of 1000 tokens 18.7 for 14.2), rings of six blocks.  Scales of values anywhere within 2^16
+// of one another, whose units move again and again, make it 24 requests 19.5, 64 x 8192 168 us.
 #include <algorithm>
 #include <atomic>
 
@@ -642,9 +643,9 @@ static int attend_ranks(long long items) {
     return 1;
 }
 
-// What decides, in microseconds beside what all have in common (bf16, 8 columns, heads of 128): a CTA takes 0.075 a block; a cluster's joining takes 1.8 and the
-// launch that joins pieces 6.5, which stream at 6.2 TB/s whatever the lengths.  Measured, whole / clusters / pieces: one request of 100 tokens 4.0 / 5.8 / -, of 500 6.4 / 5.6 / -,
-// of 1011 8.7 / 6.0 / 10.7, of 8000 - / 11.1 / 13.6, of 32000 - / 25.0 / 19.8; 8 of 8000 - / 26.1 / 30.7; 24 of 70 to 1970 16.8 / - / 19.2; 16 of 8000 45 / - / 53.  Without lengths
+// What decides, in microseconds beside what all have in common (bf16, 8 columns, heads of 128; other heads and columns go by the same, which nobody has fitted to them): a CTA takes 0.075 a block; a cluster's joining takes 1.8 and the
+// launch that joins pieces 6.5, which stream at 6.2 TB/s whatever the lengths.  Measured, whole / clusters / pieces: one request of 100 tokens 4.3 / 5.8 / -, of 500 6.4 / 5.7 / -,
+// of 1011 8.7 / 6.0 / 10.7, of 8000 - / 10.9 / 13.6, of 32000 - / 25.0 / 20.6; 8 of 8000 - / 26.4 / 30.7; 24 of 70 to 1970 17.2 / - / 19.2; 16 of 8000 45 / - / 53.  Without lengths
 // clusters are for one or two requests: of more, one may be far longer than the others, which pieces make up for.
 static AtPlan attend_plan(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c, const AtLengths &n, bool lens) {
     const long long rows = static_cast<long long>(c.heads / p.heads) * c.tokens;
@@ -662,7 +663,7 @@ static AtPlan attend_plan(const tlb_fp8_pages &p, const tlb_fp8_attention_call &
     return {1, 0, ((each * n.live + slots - 1) / slots) * (4 + whole), false, long_first};
 }
 // Portions of many columns go to the kernel of blocks_fp8_portion.cu unless this one is sooner through, as it is with few items, which clusters divide (16 tokens over 1000 with
-// groups of 4: 9.9 us here, 22.6 there; 64 over 1000 12.4 and 24.5, over 3500 26.9 and 25.9; 8 requests of 16 over 1000 23.5 and 30.7, 32 of them 79 and 58).
+// groups of 4: 9.9 us here, 22.6 there; 64 over 1000 12.7 and 24.5, over 3500 26.9 and 26.2; 8 requests of 16 over 1000 24.2 and 30.7, 32 of them 79 and 57).
 static AtPlan any_plan(const tlb_fp8_pages &p, const tlb_fp8_attention_call &c, const int32_t *lens) {
     AtLengths n{static_cast<long long>(c.max_pages) * (p.page_size / kF8Tokens), 0, c.batch};
     n.blocks = n.longest * c.batch;

@@ -14,7 +14,8 @@
 //   warps 0-7    softmax, thread = row: scores from tensor memory, 2^x of them over a running maximum that may lag behind by 2^15, P as f16 back over its own scores
 //   warps 20-23  rescale the output's rows whose maximum grew, while the softmax goes on (with queries of heavy tails one warp in eight has such a row: 127 us -> 115 for 2048 tokens over 3500)
 //
-// 2048 tokens over 3500 (32 over 8 heads of 128) take 103 us, 800 TF/s; 128 tokens 27, of which 6 are the prologue and 5 the launch that joins the pieces.  A tile of 256 columns and 64 keys takes 2400 cycles, 2120 if nothing is
+// 2048 tokens over 3500 (32 over 8 heads of 128) take 106 us, 785 TF/s; 128 tokens 28, of which 6 are the prologue and 5 the launch that joins the pieces.  Block by block (one block with a scale 2^20 times the others') they take
+// 433 and 58.  A tile of 256 columns and 64 keys takes 2400 cycles, 2120 if nothing is
 // rescaled, where its exponentials and its products take 1024 each: the softmax's own chain is 1600, the products' 1750 (a step of 64 keys reads the queries from shared memory again, which
 // is 4 KB for 32 cycles of work).  Leaving out half of the products or all exponentials brings 2120 to 2050 and 1950 only.
 #include "../per_device.h"
