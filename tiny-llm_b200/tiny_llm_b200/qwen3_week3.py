@@ -410,7 +410,8 @@ class Qwen3ModelWeek3:
 
     @staticmethod
     def _check_offsets(offset, cache) -> None:
-        """An 8-bit cache rotates by its own positions: the caller's have to be the same (of idle slots any)."""
+        """An 8-bit cache rotates by its own positions: the caller's have to be the same (of idle slots any).  Offsets on the device are waited for: lists and numbers
+        are not."""
         slots = getattr(cache, "kv_caches", [cache])
         given = offset.reshape(-1).tolist() if isinstance(offset, torch.Tensor) else [offset] if isinstance(offset, int) else [int(o) for o in offset]
         given = given * len(slots) if len(given) == 1 else given
