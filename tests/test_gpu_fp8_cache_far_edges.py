@@ -137,3 +137,29 @@ def test_other_scales_of_the_scores(new, scale):
         assert torch.equal(out, same)
     else:  # every weight alike
         check(out, torch.zeros_like(q), pages, table, [n], rows=list(range(0, new, 1 + new // 40)))
+
+
+@pytest.mark.parametrize("lengths,new,heads,kv_heads,dim", [([1011], 1, 32, 8, 128), ([5000, 16, 0, 40], 1, 8, 8, 64), ([300, 90], 40, 8, 2, 128), ([260, 77], 3, 6, 2, 96), ([400], 2, 4, 2, 256)])
+@pytest.mark.parametrize("wide", [10.0, 30.0])
+def test_fp32_over_scales_of_every_size(lengths, new, heads, kv_heads, dim, wide):
+    """Weights are two f16 terms, the second one 2^11 times what the first left: 2^-21 of a weight, 2^-36 of the largest; queries two such terms, 2^-21 of the row's largest entry with the rest.  Value scales
+    are fp32 factors behind the products."""
+    gen = torch.Generator().manual_seed(int(wide) + dim)
+    table, count = table_of(lengths, 32, 6)
+    pages = far_pages(gen, count, kv_heads, 32, dim, wide)
+    q = 0.5 * torch.randn(len(lengths), heads, new, dim, generator=gen)
+    out = attend(q, pages, table, lengths).cpu().double()
+    for b, n in enumerate(lengths):
+        if n == 0:
+            assert not out[b].any()
+            continue
+        homes = [int(p) for p in table[b, : -(-n // 32)]]
+        k, v = ((x.float().double()[homes] * s.double()[homes].repeat_interleave(16, -1)[..., None]).transpose(0, 1).flatten(1, 2)[:, :n] for x, s in ((pages.keys, pages.key_scales), (pages.values, pages.value_scales)))
+        hidden = torch.arange(n)[None] > torch.arange(n - new, n)[:, None]
+        for h in range(heads):
+            g, x = h // (heads // kv_heads), q[b, h].double()
+            p = torch.softmax((x @ k[g].t() * dim**-0.5).masked_fill(hidden, -math.inf), -1)
+            want = p @ v[g]
+            d = (dim / 16 + 6) * 2.0**-22 * (x.abs() @ k[g].abs().t() * dim**-0.5) + 2.0**-20
+            tol = (p * (d + 2.0**-21)) @ v[g].abs() + (p * d).sum(-1, keepdim=True) * want.abs() + torch.minimum(2.0**-36 * p.amax(-1, keepdim=True), p) @ v[g].abs() + 2.0**-23 * want.abs()
+            assert ((out[b, h] - want).abs() <= tol).all(), (b, h, float(((out[b, h] - want).abs() / tol).max()))
